@@ -511,6 +511,94 @@ int xb_augru_shared(const void* x, const void* att, void* y_final, int32_t reque
                     const void* Wg, const void* bg, const void* Wc, const void* bc, int32_t engine, xb_stream_t stream);
 
 /* ------------------------------------------------------------------------- */
+/* Selective state-space layer over behaviour lists: the short causal convolution and the scan of a block
+ *   u = in-projection, v = ssm_conv(u), (delta, B, C) = projections of v, y = ssm_scan(v, delta, A, B, C, gate z), out-projection.
+ * No operator of Blaze; it stands where xb_gru stands (an extractor over a user's behaviours, blaze/blaze/operator/op/
+ * gru_op.h:41-158), with a state that a server may keep per user and move on by one behaviour at a time.
+ * Lists lie one after the other in the rows of the inputs:
+ *   - `offsets` [batch + 1] (device): list i is the rows [offsets[i], offsets[i + 1]), ascending. Rows from offsets[batch] to
+ *     `rows` belong to no list: nothing of them is read into a result, and their outputs are left as they were. Offsets are cut
+ *     to [0, rows]; an end before its beginning is an empty list.
+ *   - offsets NULL: every list has rows / batch rows (batch divides rows). One row a list is the form for single tokens.
+ * Kept states: list i begins with state slots[i] of the first array and leaves its state in slots[i] of the second (slots NULL:
+ * i). The two may be the same array: the states are then moved on in place. Two lists of a call never share a slot. A slot
+ * outside [0, n_slots) begins with zeros and is not kept. First array NULL: every list begins with zeros; second NULL: nothing
+ * is kept. An empty list leaves the state that it began with.
+ * x, y, z, delta, B, C share `dtype` (XB_F32, XB_F16, XB_BF16); every sum and the scan's states are fp32. Outputs overlap no
+ * input. */
+
+/* y[t, c] = act(bias[c] + sum_{j < K} w[c, j] x[t - K + 1 + j, c]), x before the list's first row from its state
+ * (zeros without one); act is SiLU (x * sigmoid(x)) or none. 2 <= K <= 8. */
+typedef struct xb_ssm_conv_args {
+  const void* x; int64_t ldx;           /* [rows, D] */
+  void* y; int64_t ldy;                 /* [rows, D] */
+  const void* w;                        /* [D, K] */
+  const void* bias;                     /* [D], NULL: none */
+  const int32_t* offsets;
+  const int32_t* slots;                 /* [batch] */
+  const void* state_in;                 /* [n_slots, K - 1, D], oldest row first */
+  void* state_out;
+  int64_t rows;
+  int32_t batch, n_slots, D, K;
+  int32_t silu;
+  int32_t dtype;
+} xb_ssm_conv_args;
+int xb_ssm_conv(const xb_ssm_conv_args* args, xb_stream_t stream);
+
+/* For row t and channel c, with g = c / (D / groups):
+ *   d    = softplus ? log(1 + exp(delta[t, c] + delta_bias[c])) : delta[t, c] + delta_bias[c]
+ *   h[n] = exp(d A[c, n]) h[n] + d x[t, c] B[t, g, n]                     n < N <= 64
+ *   y    = (sum_n C[t, g, n] h[n] + skip[c] x[t, c]) * (z ? z[t, c] * sigmoid(z[t, c]) : 1)
+ * A, skip, delta_bias and the states are fp32. */
+typedef struct xb_ssm_scan_args {
+  const void* x; int64_t ldx;           /* [rows, D] */
+  const void* delta; int64_t lddelta;   /* [rows, D] */
+  const void* z; int64_t ldz;           /* [rows, D], NULL: no gate */
+  const void* B; int64_t ldb;           /* [rows, groups * N] */
+  const void* C; int64_t ldc;           /* [rows, groups * N] */
+  void* y; int64_t ldy;                 /* [rows, D] */
+  const float* A;                       /* [D, N] */
+  const float* skip;                    /* [D], NULL: none */
+  const float* delta_bias;              /* [D], NULL: none */
+  const int32_t* offsets;
+  const int32_t* slots;                 /* [batch] */
+  const float* h_in;                    /* [n_slots, D, N] */
+  float* h_out;
+  int64_t rows;
+  int64_t longest;                      /* no list has more rows than this, or 0: not known. Only the plan goes by it. */
+  int32_t batch, n_slots, D, N, groups;
+  int32_t softplus;
+  int32_t dtype;
+} xb_ssm_scan_args;
+/* Scratch of a call with these arguments (0 for many): one call uses it at a time. */
+size_t xb_ssm_scan_workspace_bytes(const xb_ssm_scan_args* args);
+int xb_ssm_scan(const xb_ssm_scan_args* args, void* workspace, size_t workspace_bytes, xb_stream_t stream);
+
+/* ------------------------------------------------------------------------- */
+/* A projection shared by all rows beside a low-rank adapter of each row's own: scenes (pages, markets, tenants) whose requests
+ * are stacked into one call share the weight of a layer and differ by a product of rank r.
+ *   Y[m] = X[m] W + bias + scale[a] (X[m] A[a]^T) B[a]^T,  a = adapter[m];  without the last term where a is outside [0, n_adapters)
+ * Stands beside xb_gemm (GemmOp, blaze/blaze/operator/op/gemm_op.h:33-107): W as its B operand, [K, N] or with trans_w [N, K].
+ * The rank-r intermediate is held in fp32. r <= 128. Y overlaps no input. */
+typedef struct xb_lora_args {
+  int32_t M, N, K, r, n_adapters;
+  int32_t trans_w;
+  const void* X; int64_t ldx;                        /* [M, K] */
+  const void* W; int64_t ldw;                        /* [K, N], or [N, K] with trans_w */
+  const void* A; int64_t lda; int64_t stride_a;      /* [n_adapters][r, K] */
+  const void* B; int64_t ldb; int64_t stride_b;      /* [n_adapters][N, r] */
+  const float* scale;                                /* [n_adapters], NULL: 1 */
+  const float* bias;                                 /* [N], NULL: none */
+  const int32_t* adapter;                            /* [M] */
+  void* Y; int64_t ldy;                              /* [M, N] */
+  int32_t dtype;                                     /* X, W, A, B: XB_F32, XB_F16 or XB_BF16 */
+  int32_t y_dtype;                                   /* dtype or XB_F32 */
+} xb_lora_args;
+/* Scratch of a call with these arguments: one call uses it at a time. */
+size_t xb_lora_workspace_bytes(const xb_lora_args* args);
+int xb_lora_gemm(const xb_lora_args* args, void* workspace, size_t workspace_bytes, xb_stream_t stream);
+
+/* ------------------------------------------------------------------------- */
 /* Stand-alone operators for graphs that were not fused. x/y share `dtype`;
  * per-column parameters share it too (Blaze keeps them in the model dtype). */
 /* DiceOp, blaze/blaze/operator/op/dice_op.h:41-98 */

@@ -75,6 +75,25 @@ class DinTowerArgs(C.Structure):
                 ("softmax", i32), ("packed", vp), ("act", i32)]
 
 
+class SsmConvArgs(C.Structure):
+    _fields_ = [("x", vp), ("ldx", i64), ("y", vp), ("ldy", i64), ("w", vp), ("bias", vp), ("offsets", vp), ("slots", vp),
+                ("state_in", vp), ("state_out", vp), ("rows", i64), ("batch", i32), ("n_slots", i32), ("D", i32), ("K", i32),
+                ("silu", i32), ("dtype", i32)]
+
+
+class SsmScanArgs(C.Structure):
+    _fields_ = [("x", vp), ("ldx", i64), ("delta", vp), ("lddelta", i64), ("z", vp), ("ldz", i64), ("B", vp), ("ldb", i64),
+                ("C", vp), ("ldc", i64), ("y", vp), ("ldy", i64), ("A", vp), ("skip", vp), ("delta_bias", vp), ("offsets", vp),
+                ("slots", vp), ("h_in", vp), ("h_out", vp), ("rows", i64), ("longest", i64), ("batch", i32), ("n_slots", i32),
+                ("D", i32), ("N", i32), ("groups", i32), ("softplus", i32), ("dtype", i32)]
+
+
+class LoraArgs(C.Structure):
+    _fields_ = [("M", i32), ("N", i32), ("K", i32), ("r", i32), ("n_adapters", i32), ("trans_w", i32), ("X", vp), ("ldx", i64),
+                ("W", vp), ("ldw", i64), ("A", vp), ("lda", i64), ("stride_a", i64), ("B", vp), ("ldb", i64), ("stride_b", i64),
+                ("scale", vp), ("bias", vp), ("adapter", vp), ("Y", vp), ("ldy", i64), ("dtype", i32), ("y_dtype", i32)]
+
+
 # every symbol include/xdlb200.h declares: (restype, argtypes)
 SYMBOLS = {
     "xb_last_error": (C.c_char_p, []),
@@ -139,6 +158,11 @@ SYMBOLS = {
     "xb_gru": (i32, [vp, vp, i64, i32, i32, vp, vp, vp, vp, i32, vp]),
     "xb_augru": (i32, [vp, vp, vp, i64, i32, i32, vp, vp, vp, vp, i32, vp]),
     "xb_augru_shared": (i32, [vp, vp, vp, i32, i32, i32, i32, vp, vp, vp, vp, i32, vp]),
+    "xb_ssm_conv": (i32, [C.POINTER(SsmConvArgs), vp]),
+    "xb_ssm_scan_workspace_bytes": (C.c_size_t, [C.POINTER(SsmScanArgs)]),
+    "xb_ssm_scan": (i32, [C.POINTER(SsmScanArgs), vp, C.c_size_t, vp]),
+    "xb_lora_workspace_bytes": (C.c_size_t, [C.POINTER(LoraArgs)]),
+    "xb_lora_gemm": (i32, [C.POINTER(LoraArgs), vp, C.c_size_t, vp]),
     "xb_dice": (i32, [vp, vp, i64, i32, vp, vp, vp, i32, i32, vp]),
     "xb_prelu": (i32, [vp, vp, i64, vp, i64, i32, i32, vp]),
     "xb_sigmoid": (i32, [vp, vp, i64, i32, vp]),
