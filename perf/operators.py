@@ -162,12 +162,12 @@ def run(s):
         if s["kind"] == "lora":
             return ops.lora_gemm(s["X"], s["W"], s["A"], s["B"], s["adapter"], bias=s["bias"], scale=s["scale"], trans_b=s["packed"],
                                  out_dtype=_T[s["out"]])
-        lists = dict(T=s["equal"]) if s["equal"] else dict(offsets=s["offsets"], longest=s["longest"])
+        lists = dict(T=s["equal"]) if s["equal"] else dict(offsets=s["offsets"])
         if s["kind"] == "conv":
             y = ops.ssm_conv(s["x"], s["w"], s["b"], state_in=s["state"], state_out=s["state_out"], slots=s["slots"], **lists)
             return y, s["state_out"]
         y = ops.ssm_scan(s["x"], s["delta"], s["A"], s["B"], s["C"], D=s["Dskip"], z=s["z"], delta_bias=s["delta_bias"], groups=s["groups"],
-                         h_in=s["h"], h_out=s["h_out"], slots=s["slots"], **lists)
+                         h_in=s["h"], h_out=s["h_out"], slots=s["slots"], longest=s["longest"], **lists)
         return y, s["h_out"]
     return {"lora": _plain_lora, "conv": _plain_conv, "scan": _plain_scan}[s["kind"]](s)
 
