@@ -518,7 +518,7 @@ int xb_augru_shared(const void* x, const void* att, void* y_final, int32_t reque
  * Lists lie one after the other in the rows of the inputs:
  *   - `offsets` [batch + 1] (device): list i is the rows [offsets[i], offsets[i + 1]), ascending. Rows from offsets[batch] to
  *     `rows` belong to no list: nothing of them is read into a result, and their outputs are left as they were. Offsets are cut
- *     to [0, rows]; an end before its beginning is an empty list.
+ *     to [0, rows]; what falls back leaves the results of its lists open, and nothing outside the arrays is touched.
  *   - offsets NULL: every list has rows / batch rows (batch divides rows). One row a list is the form for single tokens.
  * Kept states: list i begins with state slots[i] of the first array and leaves its state in slots[i] of the second (slots NULL:
  * i). The two may be the same array: the states are then moved on in place. Two lists of a call never share a slot. A slot

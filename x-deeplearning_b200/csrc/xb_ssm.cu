@@ -2,134 +2,137 @@
 #include <algorithm>
 
 #include "xb_common.cuh"
+#include "xb_ssm_scan.cuh"
 
 namespace xb {
 namespace {
 
-// The lists of a call and their kept states (see xdlb200.h). Every offset and slot that a kernel takes from memory goes through
-// here and is cut to what exists.
-struct Lists {
-  const int32_t* offsets;
-  const int32_t* slots;
-  int64_t rows, per;                      // per: rows a list where there are no offsets
-  int batch, n_slots;
-  __device__ __forceinline__ int64_t begin(int i) const {
-    if (!offsets) return (int64_t)i * per;
-    const int64_t o = offsets[i];
-    return o < 0 ? 0 : (o > rows ? rows : o);
-  }
-  __device__ __forceinline__ int slot(int i) const {
-    const int s = slots ? slots[i] : i;
-    return s >= 0 && s < n_slots ? s : -1;
-  }
-};
-
-template <typename T>
 struct ConvParams {
-  const T* x; int64_t ldx;
-  T* y; int64_t ldy;
-  const T* w; const T* bias;
-  const T* state_in; T* state_out;
+  const void* x; int64_t ldx;
+  void* y; int64_t ldy;
+  const void* w; const void* bias;
+  const void* state_in; void* state_out;
   Lists lists;
-  int D, K, silu;
+  int D, silu, bf16, vec, vec_w, vec_state;
+  int pieces, n_chunks, rows_a_chunk;     // threads of a row; what a thread walks
 };
 
-__device__ __forceinline__ float silu(float v) { return v / (1.f + expf(-v)); }
-
-// A thread walks one channel of one list.
-template <typename T>
-__global__ void __launch_bounds__(128) ssm_conv_kernel(const ConvParams<T> p) {
+// A thread walks `rows_a_chunk` rows of V channels with the last K - 1 inputs in registers; the threads of a chunk lie side by side, and
+// chunks follow one another without a gap, so no lane idles whatever D is. Bound by memory: x is read 1 + (K - 1) / rows_a_chunk times.
+// The thread that has a list's first row makes its first K - 1 rows (they read the state) and its last state, so that states moved
+// on in place are read and written by one thread.
+constexpr int CONV_THREADS = 128, CONV_AHEAD = 4;
+template <int SIZE, int V, int K>
+__global__ void __launch_bounds__(CONV_THREADS) ssm_conv_kernel(const ConvParams p) {
   pdl_begin();
-  const int c = blockIdx.y * 128 + threadIdx.x;
-  if (c >= p.D) return;
-  const int K = p.K;
-  float w[8], past[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) w[j] = j < K ? to_f32<T>(p.w[(int64_t)c * K + j]) : 0.f;
-  const float b = p.bias ? to_f32<T>(p.bias[c]) : 0.f;
-  for (int i = blockIdx.x; i < p.lists.batch; i += gridDim.x) {
-    const int64_t r0 = p.lists.begin(i), r1 = p.lists.begin(i + 1);
-    const int slot = p.lists.slot(i);
-#pragma unroll
-    for (int j = 0; j < 7; ++j)
-      past[j] = j < K - 1 && p.state_in && slot >= 0 ? to_f32<T>(p.state_in[((int64_t)slot * (K - 1) + j) * p.D + c]) : 0.f;
-    for (int64_t r = r0; r < r1; ++r) {
-      const float x = to_f32<T>(p.x[r * p.ldx + c]);
-      float v = b;
-#pragma unroll
-      for (int j = 0; j < 7; ++j)
-        if (j < K - 1) v = fmaf(w[j], past[j], v);
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (j == K - 1) v = fmaf(w[j], x, v);
-#pragma unroll
-      for (int j = 0; j < 7; ++j) past[j] = j == K - 2 ? x : past[j + 1];
-      p.y[r * p.ldy + c] = from_f32<T>(p.silu ? silu(v) : v);
-    }
-    if (p.state_out && slot >= 0)
-      for (int j = 0; j < K - 1; ++j) p.state_out[((int64_t)slot * (K - 1) + j) * p.D + c] = from_f32<T>(past[j]);
+  __shared__ int s_first[CONV_THREADS];                // the first list that begins in or behind each of the block's chunks
+  const int lane = threadIdx.x & 31;
+  const int64_t at = (int64_t)blockIdx.x * CONV_THREADS, at_me = at + threadIdx.x;
+  const int64_t c_first = at / p.pieces;
+  const int chunks = (int)((at + CONV_THREADS - 1) / p.pieces - c_first) + 1;
+  for (int i = threadIdx.x / 32; i < chunks; i += CONV_THREADS / 32) {
+    const int f = p.lists.first_from((c_first + i) * p.rows_a_chunk, lane);
+    if (lane == 0) s_first[i] = f;
   }
-}
-
-template <typename T>
-struct ScanParams {
-  const T* x; int64_t ldx;
-  const T* delta; int64_t lddelta;
-  const T* z; int64_t ldz;
-  const T* B; int64_t ldb;
-  const T* C; int64_t ldc;
-  T* y; int64_t ldy;
-  const float* A; const float* skip; const float* delta_bias;
-  const float* h_in; float* h_out;
-  Lists lists;
-  int D, N, per_group, softplus;
-};
-
-constexpr int SPL = 4;                    // states of a lane
-
-// LPC lanes walk one channel of one list, four states a lane.
-template <typename T, int LPC>
-__global__ void __launch_bounds__(128) ssm_scan_kernel(const ScanParams<T> p, int channel_blocks) {
-  pdl_begin();
-  const int i = blockIdx.x / channel_blocks;
-  const int n0 = threadIdx.x % LPC * SPL;
-  const int at = (blockIdx.x % channel_blocks) * (128 / LPC) + threadIdx.x / LPC;
-  const bool mine = at < p.D;
-  const int c = mine ? at : p.D - 1, g = c / p.per_group;
-  const int64_t r0 = p.lists.begin(i), r1 = p.lists.begin(i + 1);
-  const int slot = p.lists.slot(i);
-  float A[SPL], h[SPL];
+  __syncthreads();
+  const int64_t chunk = at_me / p.pieces;
+  if (chunk >= p.n_chunks) return;
+  const int c = (int)(at_me - chunk * p.pieces) * V, in = min(V, p.D - c);
+  const bool bf16 = p.bf16 != 0, last_chunk = chunk == p.n_chunks - 1;
+  const int64_t r0 = chunk * p.rows_a_chunk, r1 = r0 + p.rows_a_chunk;
+  float w[V][K], bias[V], past[K - 1][V];
+  {
+    Raw<SIZE, V> t[K];
 #pragma unroll
-  for (int s = 0; s < SPL; ++s) {
-    const bool in = n0 + s < p.N;
-    A[s] = in ? p.A[(int64_t)c * p.N + n0 + s] : 0.f;
-    h[s] = in && p.h_in && slot >= 0 ? p.h_in[((int64_t)slot * p.D + c) * p.N + n0 + s] : 0.f;
+    for (int j = 0; j < K; ++j) t[j].load(p.w, (int64_t)c * K + j * V, in * K - j * V, p.vec_w);
+#pragma unroll
+    for (int e = 0; e < V * K; ++e) w[e / K][e % K] = t[e / V].get(e % V, bf16);
+    if (p.bias) t[0].load(p.bias, c, in, p.vec_w);
+#pragma unroll
+    for (int v = 0; v < V; ++v) bias[v] = p.bias ? t[0].get(v, bf16) : 0.f;
   }
-  const float bias = p.delta_bias ? p.delta_bias[c] : 0.f, skip = p.skip ? p.skip[c] : 0.f;
-  for (int64_t r = r0; r < r1; ++r) {
-    const float x = to_f32<T>(p.x[r * p.ldx + c]);
-    const float v = to_f32<T>(p.delta[r * p.lddelta + c]) + bias;
-    const float d = p.softplus ? (v > 0.f ? v + log1pf(expf(-v)) : log1pf(expf(v))) : v;
-    float y = 0.f;
+  auto row_of = [&](const Raw<SIZE, V>& t, int64_t r) {
+    Raw<SIZE, V> out;
 #pragma unroll
-    for (int s = 0; s < SPL; ++s) {
-      if (n0 + s >= p.N) continue;
-      const float Bn = to_f32<T>(p.B[r * p.ldb + g * p.N + n0 + s]), Cn = to_f32<T>(p.C[r * p.ldc + g * p.N + n0 + s]);
-      h[s] = fmaf(expf(d * A[s]), h[s], d * x * Bn);
-      y = fmaf(Cn, h[s], y);
+    for (int v = 0; v < V; ++v) {
+      const float x = t.get(v, bf16);
+      float s = bias[v];
+#pragma unroll
+      for (int j = 0; j < K - 1; ++j) s = fmaf(w[v][j], past[j][v], s);
+      s = fmaf(w[v][K - 1], x, s);
+#pragma unroll
+      for (int j = 0; j + 1 < K - 1; ++j) past[j][v] = past[j + 1][v];
+      past[K - 2][v] = x;
+      out.put(v, p.silu ? silu(s) : s, bf16);
     }
+    out.store(p.y, r * p.ldy + c, in, p.vec);
+  };
+  int nxt = s_first[(int)(chunk - c_first)];
+  int64_t r = r0, stop = r0;
+  if (nxt > 0 && p.lists.begin(nxt) > r0) {            // a list from before: its rows from the K-th on
+    const int64_t b = p.lists.begin(nxt - 1);
+    r = max(r0, b + K - 1);
+    stop = min(r1, p.lists.begin(nxt));
+    if (r < stop) {
 #pragma unroll
-    for (int m = LPC / 2; m > 0; m >>= 1) y += __shfl_xor_sync(0xffffffffu, y, m);
-    if (mine && n0 == 0) {
-      y = fmaf(skip, x, y);
-      if (p.z) y *= silu(to_f32<T>(p.z[r * p.ldz + c]));
-      p.y[r * p.ldy + c] = from_f32<T>(y);
+      for (int j = 0; j < K - 1; ++j) {
+        Raw<SIZE, V> t;
+        t.load(p.x, (r - (K - 1) + j) * p.ldx + c, in, p.vec);
+#pragma unroll
+        for (int v = 0; v < V; ++v) past[j][v] = t.get(v, bf16);
+      }
     }
   }
-  if (p.h_out && slot >= 0 && mine)
+  for (;;) {
+    for (; r + CONV_AHEAD <= stop; r += CONV_AHEAD) {
+      Raw<SIZE, V> t[CONV_AHEAD];
 #pragma unroll
-    for (int s = 0; s < SPL; ++s)
-      if (n0 + s < p.N) p.h_out[((int64_t)slot * p.D + c) * p.N + n0 + s] = h[s];
+      for (int i = 0; i < CONV_AHEAD; ++i) t[i].load(p.x, (r + i) * p.ldx + c, in, p.vec);
+#pragma unroll
+      for (int i = 0; i < CONV_AHEAD; ++i) row_of(t[i], r + i);
+    }
+    for (; r < stop; ++r) {
+      Raw<SIZE, V> t;
+      t.load(p.x, r * p.ldx + c, in, p.vec);
+      row_of(t, r);
+    }
+    if (nxt >= p.lists.batch) return;
+    const int64_t b = p.lists.begin(nxt), e = max(b, p.lists.begin(nxt + 1));
+    if (b >= r1 && !last_chunk) return;
+    const int slot = p.lists.slot(nxt);
+    const int64_t state = ((int64_t)slot * (K - 1)) * p.D + c;
+#pragma unroll
+    for (int j = 0; j < K - 1; ++j) {
+      Raw<SIZE, V> t;
+#pragma unroll
+      for (int i = 0; i < Raw<SIZE, V>::W; ++i) t.w[i] = 0u;
+      if (p.state_in && slot >= 0) t.load(p.state_in, state + (int64_t)j * p.D, in, p.vec_state);
+#pragma unroll
+      for (int v = 0; v < V; ++v) past[j][v] = t.get(v, bf16);
+    }
+    if (p.state_out && slot >= 0) {
+#pragma unroll
+      for (int j = 0; j < K - 1; ++j) {                // place len - (K - 1) + j of the list, before its first row in the state
+        const int64_t place = e - b - (K - 1) + j;
+        Raw<SIZE, V> t;
+        if (place >= 0) {
+          t.load(p.x, (b + place) * p.ldx + c, in, p.vec);
+        } else {
+#pragma unroll
+          for (int v = 0; v < V; ++v) {
+            float was = 0.f;
+#pragma unroll
+            for (int k = 0; k < K - 1; ++k) was = k == (int)place + K - 1 ? past[k][v] : was;
+            t.put(v, was, bf16);
+          }
+        }
+        t.store(p.state_out, state + (int64_t)j * p.D, in, p.vec_state);
+      }
+    }
+    ++nxt;
+    r = b;
+    stop = min(e, max(r1, b + K - 1));
+  }
 }
 
 int check_lists(const char* what, const int32_t* offsets, const int32_t* slots, bool states, int64_t rows, int32_t batch, int32_t n_slots) {
@@ -145,32 +148,145 @@ Lists lists_of(const int32_t* offsets, const int32_t* slots, int64_t rows, int32
 }
 bool ssm_dtype(int dtype) { return dtype == XB_F32 || dtype == XB_F16 || dtype == XB_BF16; }
 
-template <typename T>
-int launch_conv(const xb_ssm_conv_args& a, cudaStream_t s) {
-  ConvParams<T> p = {(const T*)a.x, a.ldx, (T*)a.y, a.ldy, (const T*)a.w, (const T*)a.bias, (const T*)a.state_in, (T*)a.state_out,
-                     lists_of(a.offsets, a.slots, a.rows, a.batch, a.n_slots), a.D, a.K, a.silu};
-  const dim3 grid((unsigned)a.batch, (unsigned)((a.D + 127) / 128));
-  launch_dependent(ssm_conv_kernel<T>, grid, 128, 0, s, p);
+template <int SIZE, int V, int K>
+int launch_conv_taps(const ConvParams& p, cudaStream_t s) {
+  const int64_t blocks = ((int64_t)p.n_chunks * p.pieces + CONV_THREADS - 1) / CONV_THREADS;
+  XB_REQUIRE(blocks < ((int64_t)1 << 31), XB_ERR_LIMIT, "xb_ssm_conv: too many rows and channels");
+  launch_dependent(ssm_conv_kernel<SIZE, V, K>, (unsigned)blocks, CONV_THREADS, 0, s, p);
   return check_launch("ssm_conv_kernel");
 }
+template <int SIZE, int V>
+int launch_conv_pieces(ConvParams p, int K, cudaStream_t s) {
+  p.pieces = (p.D + V - 1) / V;
+  // Longer walks read less twice, shorter ones keep more threads in flight. Single rows: nothing is read twice.
+  const int64_t threads = p.lists.rows * p.pieces, fill = (int64_t)sm_count() * 1024;
+  p.rows_a_chunk = (int)std::min<int64_t>(std::max<int64_t>(threads / fill, 1), !p.lists.offsets && p.lists.per <= 1 ? 1 : 32);
+  p.n_chunks = (int)std::max<int64_t>((p.lists.rows + p.rows_a_chunk - 1) / p.rows_a_chunk, 1);
+  switch (K) {
+    case 2: return launch_conv_taps<SIZE, V, 2>(p, s);
+    case 3: return launch_conv_taps<SIZE, V, 3>(p, s);
+    case 4: return launch_conv_taps<SIZE, V, 4>(p, s);
+    case 5: return launch_conv_taps<SIZE, V, 5>(p, s);
+    case 6: return launch_conv_taps<SIZE, V, 6>(p, s);
+    case 7: return launch_conv_taps<SIZE, V, 7>(p, s);
+    default: return launch_conv_taps<SIZE, V, 8>(p, s);
+  }
+}
+bool whole(const void* q, int64_t ld_bytes, int64_t unit) { return reinterpret_cast<uintptr_t>(q) % unit == 0 && ld_bytes % unit == 0; }
+template <int SIZE>
+int launch_conv(const xb_ssm_conv_args& a, cudaStream_t s) {
+  ConvParams p = {};
+  p.x = a.x; p.ldx = a.ldx; p.y = a.y; p.ldy = a.ldy; p.w = a.w; p.bias = a.bias; p.state_in = a.state_in; p.state_out = a.state_out;
+  p.lists = lists_of(a.offsets, a.slots, a.rows, a.batch, a.n_slots);
+  p.D = a.D; p.silu = a.silu; p.bf16 = a.dtype == XB_BF16;
+  p.vec = whole(a.x, a.ldx * SIZE, 16) && whole(a.y, a.ldy * SIZE, 16);
+  p.vec_w = whole(a.w, 0, 16) && whole(a.bias, 0, 16);
+  p.vec_state = whole(a.state_in, (int64_t)a.D * SIZE, 16) && whole(a.state_out, 0, 16);
+  // rows that do not start on 16 bytes: a channel a thread, adjacent lanes adjacent channels
+  return p.vec ? launch_conv_pieces<SIZE, 16 / SIZE>(p, a.K, s) : launch_conv_pieces<SIZE, 1>(p, a.K, s);
+}
 
-template <typename T, int LPC>
-int launch_scan_lanes(const ScanParams<T>& p, cudaStream_t s) {
-  const int blocks = (p.D + 128 / LPC - 1) / (128 / LPC);
-  XB_REQUIRE((int64_t)blocks * p.lists.batch < ((int64_t)1 << 31), XB_ERR_LIMIT, "xb_ssm_scan: too many lists and channels");
-  launch_dependent(ssm_scan_kernel<T, LPC>, (unsigned)((int64_t)blocks * p.lists.batch), 128, 0, s, p, blocks);
+// What a scan runs as.
+struct ScanPlan {
+  enum { STEP, LISTS, CHUNKS } how;
+  int lanes, K;                           // lanes of a channel; channels of a lane
+  int64_t chunk;
+  int n_chunks;
+};
+int scan_blocks(const xb_ssm_scan_args& a, int lanes, int K) {
+  const int per = a.D / a.groups, ch = SCAN_THREADS / lanes * K;
+  return a.groups * ((per + ch - 1) / ch);
+}
+ScanPlan scan_plan(const xb_ssm_scan_args& a) {
+  ScanPlan p = {};
+  p.lanes = a.N <= 4 ? 1 : a.N <= 8 ? 2 : a.N <= 16 ? 4 : a.N <= 32 ? 8 : 16;
+  if (!a.offsets && a.rows == a.batch) { p.how = ScanPlan::STEP; return p; }
+  const double sms = std::max(sm_count(), 1);
+  const double longest = !a.offsets ? (double)(a.rows / a.batch) : (double)(a.longest > 0 ? std::min(a.longest, a.rows) : a.rows);
+  double best = 0;
+  for (int K : {1, 4}) {
+    // cycles of a row of a block: of an SM with four blocks, and of one alone
+    const double work = K == 4 ? 160 : 50, alone = K == 4 ? 260 : 100;
+    const int blocks = scan_blocks(a, p.lanes, K);
+    const double full = (double)a.rows * blocks * work / sms, lists = std::max(full, longest * alone);
+    if (best == 0 || lists < best) { best = lists; p.how = ScanPlan::LISTS; p.K = K; }
+    int64_t n = std::min<int64_t>((int64_t)(8 * sms) / blocks, a.rows / 64);
+    if (n < 2) continue;
+    const int64_t chunk = (a.rows + n - 1) / n;
+    n = (a.rows + chunk - 1) / chunk;
+    const double chunks = 1.8 * std::max(full, chunk * alone) + 20000;
+    if (chunks < best) { best = chunks; p.how = ScanPlan::CHUNKS; p.K = K; p.chunk = chunk; p.n_chunks = (int)n; }
+  }
+  return p;
+}
+constexpr size_t align256(size_t n) { return (n + 255) / 256 * 256; }
+struct ScanScratch { size_t end, first, steps, kind, bytes; };
+ScanScratch scan_scratch(const xb_ssm_scan_args& a, const ScanPlan& p) {
+  ScanScratch w = {};
+  if (p.how != ScanPlan::CHUNKS) return w;
+  const size_t states = align256((size_t)p.n_chunks * a.D * a.N * 4);
+  w.first = w.end + states;
+  w.steps = w.first + (a.h_in ? states : 0);
+  w.kind = w.steps + align256((size_t)p.n_chunks * a.D * 4);
+  w.bytes = w.kind + align256((size_t)p.n_chunks * 4);
+  return w;
+}
+
+template <int SIZE, int LPC, int K>
+int launch_tiles(const ScanParams& p, const ScanPlan& plan, cudaStream_t s) {
+  const int ch = ScanShape<LPC, K>::CH, a_group = (p.per_group + ch - 1) / ch, blocks = a_group * p.groups;
+  const int64_t units = plan.how == ScanPlan::LISTS ? p.lists.batch : plan.n_chunks;
+  XB_REQUIRE(units * blocks < ((int64_t)1 << 31), XB_ERR_LIMIT, "xb_ssm_scan: too many lists and channels");
+  if (plan.how == ScanPlan::LISTS) {
+    launch_dependent(ssm_scan_kernel<SIZE, LPC, K, SCAN_LISTS>, (unsigned)(units * blocks), SCAN_THREADS, 0, s, p, a_group);
+    return check_launch("ssm_scan_kernel");
+  }
+  launch_dependent(ssm_scan_kernel<SIZE, LPC, K, SCAN_TAILS>, (unsigned)((units - 1) * blocks), SCAN_THREADS, 0, s, p, a_group);
+  if (int rc = check_launch("ssm_scan_kernel")) return rc;
+  launch_dependent(ssm_carry_kernel, (unsigned)(((int64_t)p.D * p.N + 31) / 32), 32 * CARRY_PARTS, 0, s, p);
+  if (int rc = check_launch("ssm_carry_kernel")) return rc;
+  launch_dependent(ssm_scan_kernel<SIZE, LPC, K, SCAN_CHUNKS>, (unsigned)(units * blocks), SCAN_THREADS, 0, s, p, a_group);
   return check_launch("ssm_scan_kernel");
 }
-template <typename T>
-int launch_scan(const xb_ssm_scan_args& a, cudaStream_t s) {
-  ScanParams<T> p = {(const T*)a.x, a.ldx, (const T*)a.delta, a.lddelta, (const T*)a.z, a.ldz, (const T*)a.B, a.ldb, (const T*)a.C, a.ldc,
-                     (T*)a.y, a.ldy, a.A, a.skip, a.delta_bias, a.h_in, a.h_out,
-                     lists_of(a.offsets, a.slots, a.rows, a.batch, a.n_slots), a.D, a.N, a.D / a.groups, a.softplus};
-  if (a.N <= 4) return launch_scan_lanes<T, 1>(p, s);
-  if (a.N <= 8) return launch_scan_lanes<T, 2>(p, s);
-  if (a.N <= 16) return launch_scan_lanes<T, 4>(p, s);
-  if (a.N <= 32) return launch_scan_lanes<T, 8>(p, s);
-  return launch_scan_lanes<T, 16>(p, s);
+template <int SIZE, int LPC>
+int launch_lanes(const ScanParams& p, const ScanPlan& plan, cudaStream_t s) {
+  if (plan.how == ScanPlan::STEP) {
+    const int ch = SCAN_THREADS / LPC * STEP_U, blocks = (p.D + ch - 1) / ch;
+    XB_REQUIRE((int64_t)blocks * p.lists.batch < ((int64_t)1 << 31), XB_ERR_LIMIT, "xb_ssm_scan: too many lists and channels");
+    launch_dependent(ssm_step_kernel<SIZE, LPC>, (unsigned)((int64_t)blocks * p.lists.batch), SCAN_THREADS, 0, s, p, blocks);
+    return check_launch("ssm_step_kernel");
+  }
+  return plan.K == 4 ? launch_tiles<SIZE, LPC, 4>(p, plan, s) : launch_tiles<SIZE, LPC, 1>(p, plan, s);
+}
+template <int SIZE>
+int launch_scan(const ScanParams& p, const ScanPlan& plan, cudaStream_t s) {
+  switch (plan.lanes) {
+    case 1: return launch_lanes<SIZE, 1>(p, plan, s);
+    case 2: return launch_lanes<SIZE, 2>(p, plan, s);
+    case 4: return launch_lanes<SIZE, 4>(p, plan, s);
+    case 8: return launch_lanes<SIZE, 8>(p, plan, s);
+    default: return launch_lanes<SIZE, 16>(p, plan, s);
+  }
+}
+ScanParams scan_params(const xb_ssm_scan_args& a, const ScanPlan& plan, uint8_t* ws) {
+  ScanParams p = {};
+  p.x = a.x; p.ldx = a.ldx; p.delta = a.delta; p.lddelta = a.lddelta; p.z = a.z; p.ldz = a.ldz;
+  p.B = a.B; p.ldb = a.ldb; p.C = a.C; p.ldc = a.ldc; p.y = a.y; p.ldy = a.ldy;
+  p.A = a.A; p.skip = a.skip; p.delta_bias = a.delta_bias; p.h_in = a.h_in; p.h_out = a.h_out;
+  p.lists = lists_of(a.offsets, a.slots, a.rows, a.batch, a.n_slots);
+  p.D = a.D; p.N = a.N; p.per_group = a.D / a.groups; p.groups = a.groups; p.softplus = a.softplus; p.bf16 = a.dtype == XB_BF16;
+  const int64_t size = (int64_t)dtype_size(a.dtype);
+  p.vec = whole(a.x, a.ldx * size, 16) && whole(a.delta, a.lddelta * size, 16) && whole(a.y, a.ldy * size, 16) &&
+          (!a.z || whole(a.z, a.ldz * size, 16)) && (a.groups == 1 || p.per_group * size % 16 == 0);
+  p.vec_bc = a.N % 4 == 0 && whole(a.B, a.ldb * size, 4 * size) && whole(a.C, a.ldc * size, 4 * size);
+  p.vec_h = a.N % 4 == 0 && whole(a.A, 0, 16) && whole(a.h_in, 0, 16) && whole(a.h_out, 0, 16);
+  const ScanScratch w = scan_scratch(a, plan);
+  if (w.bytes) {
+    p.chunk = plan.chunk; p.n_chunks = plan.n_chunks;
+    p.end = reinterpret_cast<float*>(ws + w.end); p.first = reinterpret_cast<float*>(ws + w.first);
+    p.steps = reinterpret_cast<float*>(ws + w.steps); p.kind = reinterpret_cast<int*>(ws + w.kind);
+  }
+  return p;
 }
 
 }  // namespace
@@ -188,17 +304,11 @@ extern "C" int xb_ssm_conv(const xb_ssm_conv_args* a, xb_stream_t s) {
   XB_REQUIRE(a->w && (a->rows == 0 || (a->x && a->y)), XB_ERR_ARG, "xb_ssm_conv: null tensor");
   XB_REQUIRE(a->rows == 0 || (a->ldx >= a->D && a->ldy >= a->D), XB_ERR_ARG, "xb_ssm_conv: row strides %lld, %lld of %d channels",
              (long long)a->ldx, (long long)a->ldy, a->D);
-  if (a->dtype == XB_F32) return launch_conv<float>(*a, (cudaStream_t)s);
-  if (a->dtype == XB_F16) return launch_conv<__half>(*a, (cudaStream_t)s);
-  return launch_conv<__nv_bfloat16>(*a, (cudaStream_t)s);
+  return a->dtype == XB_F32 ? launch_conv<4>(*a, (cudaStream_t)s) : launch_conv<2>(*a, (cudaStream_t)s);
 }
 
-extern "C" size_t xb_ssm_scan_workspace_bytes(const xb_ssm_scan_args* a) {
-  (void)a;
-  return 0;
-}
-
-extern "C" int xb_ssm_scan(const xb_ssm_scan_args* a, void* workspace, size_t workspace_bytes, xb_stream_t s) {
+namespace {
+int check_scan(const xb_ssm_scan_args* a) {
   XB_REQUIRE(a, XB_ERR_ARG, "xb_ssm_scan: null arguments");
   XB_REQUIRE(ssm_dtype(a->dtype), XB_ERR_UNSUPPORTED, "xb_ssm_scan: dtype %d", a->dtype);
   XB_REQUIRE(a->D >= 1 && a->N >= 1 && a->groups >= 1 && a->D % a->groups == 0, XB_ERR_ARG, "xb_ssm_scan: %d channels in %d groups, %d states",
@@ -212,10 +322,23 @@ extern "C" int xb_ssm_scan(const xb_ssm_scan_args* a, void* workspace, size_t wo
              "xb_ssm_scan: a row stride below %d channels", a->D);
   XB_REQUIRE(a->rows == 0 || (a->ldb >= (int64_t)a->groups * a->N && a->ldc >= (int64_t)a->groups * a->N), XB_ERR_ARG,
              "xb_ssm_scan: a row stride of B or C below %d x %d", a->groups, a->N);
-  const size_t need = xb_ssm_scan_workspace_bytes(a);
+  return 0;
+}
+}  // namespace
+
+extern "C" size_t xb_ssm_scan_workspace_bytes(const xb_ssm_scan_args* a) {
+  if (check_scan(a) != 0 || a->batch == 0) return 0;
+  return scan_scratch(*a, scan_plan(*a)).bytes;
+}
+
+extern "C" int xb_ssm_scan(const xb_ssm_scan_args* a, void* workspace, size_t workspace_bytes, xb_stream_t s) {
+  if (int rc = check_scan(a)) return rc;
+  if (a->batch == 0) return 0;
+  const ScanPlan plan = scan_plan(*a);
+  const size_t need = scan_scratch(*a, plan).bytes;
   XB_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), XB_ERR_SCRATCH, "xb_ssm_scan: workspace of %zu bytes, %zu needed",
              workspace_bytes, need);
-  if (a->dtype == XB_F32) return launch_scan<float>(*a, (cudaStream_t)s);
-  if (a->dtype == XB_F16) return launch_scan<__half>(*a, (cudaStream_t)s);
-  return launch_scan<__nv_bfloat16>(*a, (cudaStream_t)s);
+  XB_REQUIRE(need == 0 || (reinterpret_cast<uintptr_t>(workspace) & 15) == 0, XB_ERR_ARG, "xb_ssm_scan: the workspace is not on 16 bytes");
+  const ScanParams p = scan_params(*a, plan, static_cast<uint8_t*>(workspace));
+  return a->dtype == XB_F32 ? launch_scan<4>(p, plan, (cudaStream_t)s) : launch_scan<2>(p, plan, (cudaStream_t)s);
 }
