@@ -218,7 +218,8 @@ def binding():
         spec = importlib.util.spec_from_file_location("xb_binding", path, loader=loader)
         m = importlib.util.module_from_spec(spec)
         loader.exec_module(m)
-        for name in ("xb_gemm", "xb_embedding_pool"):
+        for name in ("xb_gemm", "xb_embedding_pool", "xb_ssm_conv", "xb_ssm_scan_workspace_bytes", "xb_ssm_scan", "xb_lora_workspace_bytes",
+                     "xb_lora_gemm"):
             m.bind(name, C.cast(getattr(L, name), C.c_void_p).value)
         _binding = m
     return _binding

@@ -1,8 +1,10 @@
-// Selective state-space layer over behaviour lists: the short causal convolution and the scan (formulas in xdlb200.h).
+// Selective state-space layer over behaviour lists: the short causal convolution, and what a scan runs as (formulas in xdlb200.h; the scan's
+// kernels are in xb_ssm_scan.cuh, compiled for one type each in xb_ssm_scan_*.cu).
 #include <algorithm>
+#include <cmath>
 
 #include "xb_common.cuh"
-#include "xb_ssm_scan.cuh"
+#include "xb_ssm.cuh"
 
 namespace xb {
 namespace {
@@ -13,7 +15,7 @@ struct ConvParams {
   const void* w; const void* bias;
   const void* state_in; void* state_out;
   Lists lists;
-  int D, silu, bf16, vec, vec_w, vec_state;
+  int D, silu, vec, vec_w, vec_state;
   int pieces, n_chunks, rows_a_chunk;     // threads of a row; what a thread walks
 };
 
@@ -22,7 +24,7 @@ struct ConvParams {
 // The thread that has a list's first row makes its first K - 1 rows (they read the state) and its last state, so that states moved
 // on in place are read and written by one thread.
 constexpr int CONV_THREADS = 128, CONV_AHEAD = 4;
-template <int SIZE, int V, int K>
+template <typename T, int V, int K>
 __global__ void __launch_bounds__(CONV_THREADS) ssm_conv_kernel(const ConvParams p) {
   pdl_begin();
   __shared__ int s_first[CONV_THREADS];                // the first list that begins in or behind each of the block's chunks
@@ -38,24 +40,26 @@ __global__ void __launch_bounds__(CONV_THREADS) ssm_conv_kernel(const ConvParams
   const int64_t chunk = at_me / p.pieces;
   if (chunk >= p.n_chunks) return;
   const int c = (int)(at_me - chunk * p.pieces) * V, in = min(V, p.D - c);
-  const bool bf16 = p.bf16 != 0, last_chunk = chunk == p.n_chunks - 1;
+  const bool last_chunk = chunk == p.n_chunks - 1;
   const int64_t r0 = chunk * p.rows_a_chunk, r1 = r0 + p.rows_a_chunk;
+  const T *px = static_cast<const T*>(p.x) + c, *pw = static_cast<const T*>(p.w) + (int64_t)c * K, *pb = static_cast<const T*>(p.bias) + c;
+  T* py = static_cast<T*>(p.y) + c;
   float w[V][K], bias[V], past[K - 1][V];
   {
-    Raw<SIZE, V> t[K];
+    Raw<T, V> t[K];
 #pragma unroll
-    for (int j = 0; j < K; ++j) t[j].load(p.w, (int64_t)c * K + j * V, in * K - j * V, p.vec_w);
+    for (int j = 0; j < K; ++j) t[j].load(pw + j * V, in * K - j * V, p.vec_w);
 #pragma unroll
-    for (int e = 0; e < V * K; ++e) w[e / K][e % K] = t[e / V].get(e % V, bf16);
-    if (p.bias) t[0].load(p.bias, c, in, p.vec_w);
+    for (int e = 0; e < V * K; ++e) w[e / K][e % K] = t[e / V].get(e % V);
+    if (p.bias) t[0].load(pb, in, p.vec_w);
 #pragma unroll
-    for (int v = 0; v < V; ++v) bias[v] = p.bias ? t[0].get(v, bf16) : 0.f;
+    for (int v = 0; v < V; ++v) bias[v] = p.bias ? t[0].get(v) : 0.f;
   }
-  auto row_of = [&](const Raw<SIZE, V>& t, int64_t r) {
-    Raw<SIZE, V> out;
+  auto row_of = [&](const Raw<T, V>& t, int64_t r) {
+    float o[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      const float x = t.get(v, bf16);
+      const float x = t.get(v);
       float s = bias[v];
 #pragma unroll
       for (int j = 0; j < K - 1; ++j) s = fmaf(w[v][j], past[j][v], s);
@@ -63,9 +67,15 @@ __global__ void __launch_bounds__(CONV_THREADS) ssm_conv_kernel(const ConvParams
 #pragma unroll
       for (int j = 0; j + 1 < K - 1; ++j) past[j][v] = past[j + 1][v];
       past[K - 2][v] = x;
-      out.put(v, p.silu ? silu(s) : s, bf16);
+      o[v] = s;
     }
-    out.store(p.y, r * p.ldy + c, in, p.vec);
+    if (p.silu) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) o[v] = silu(o[v]);
+    }
+    Raw<T, V> out;
+    out.put_all(o);
+    out.store(py + r * p.ldy, in, p.vec);
   };
   int nxt = s_first[(int)(chunk - c_first)];
   int64_t r = r0, stop = r0;
@@ -76,24 +86,24 @@ __global__ void __launch_bounds__(CONV_THREADS) ssm_conv_kernel(const ConvParams
     if (r < stop) {
 #pragma unroll
       for (int j = 0; j < K - 1; ++j) {
-        Raw<SIZE, V> t;
-        t.load(p.x, (r - (K - 1) + j) * p.ldx + c, in, p.vec);
+        Raw<T, V> t;
+        t.load(px + (r - (K - 1) + j) * p.ldx, in, p.vec);
 #pragma unroll
-        for (int v = 0; v < V; ++v) past[j][v] = t.get(v, bf16);
+        for (int v = 0; v < V; ++v) past[j][v] = t.get(v);
       }
     }
   }
   for (;;) {
     for (; r + CONV_AHEAD <= stop; r += CONV_AHEAD) {
-      Raw<SIZE, V> t[CONV_AHEAD];
+      Raw<T, V> t[CONV_AHEAD];
 #pragma unroll
-      for (int i = 0; i < CONV_AHEAD; ++i) t[i].load(p.x, (r + i) * p.ldx + c, in, p.vec);
+      for (int i = 0; i < CONV_AHEAD; ++i) t[i].load(px + (r + i) * p.ldx, in, p.vec);
 #pragma unroll
       for (int i = 0; i < CONV_AHEAD; ++i) row_of(t[i], r + i);
     }
     for (; r < stop; ++r) {
-      Raw<SIZE, V> t;
-      t.load(p.x, r * p.ldx + c, in, p.vec);
+      Raw<T, V> t;
+      t.load(px + r * p.ldx, in, p.vec);
       row_of(t, r);
     }
     if (nxt >= p.lists.batch) return;
@@ -103,30 +113,29 @@ __global__ void __launch_bounds__(CONV_THREADS) ssm_conv_kernel(const ConvParams
     const int64_t state = ((int64_t)slot * (K - 1)) * p.D + c;
 #pragma unroll
     for (int j = 0; j < K - 1; ++j) {
-      Raw<SIZE, V> t;
+      Raw<T, V> t;
+      t.zero();
+      if (p.state_in && slot >= 0) t.load(static_cast<const T*>(p.state_in) + state + (int64_t)j * p.D, in, p.vec_state);
 #pragma unroll
-      for (int i = 0; i < Raw<SIZE, V>::W; ++i) t.w[i] = 0u;
-      if (p.state_in && slot >= 0) t.load(p.state_in, state + (int64_t)j * p.D, in, p.vec_state);
-#pragma unroll
-      for (int v = 0; v < V; ++v) past[j][v] = t.get(v, bf16);
+      for (int v = 0; v < V; ++v) past[j][v] = t.get(v);
     }
     if (p.state_out && slot >= 0) {
 #pragma unroll
       for (int j = 0; j < K - 1; ++j) {                // place len - (K - 1) + j of the list, before its first row in the state
         const int64_t place = e - b - (K - 1) + j;
-        Raw<SIZE, V> t;
+        Raw<T, V> t;
         if (place >= 0) {
-          t.load(p.x, (b + place) * p.ldx + c, in, p.vec);
+          t.load(px + (b + place) * p.ldx, in, p.vec);
         } else {
 #pragma unroll
           for (int v = 0; v < V; ++v) {
             float was = 0.f;
 #pragma unroll
             for (int k = 0; k < K - 1; ++k) was = k == (int)place + K - 1 ? past[k][v] : was;
-            t.put(v, was, bf16);
+            t.put(v, was);
           }
         }
-        t.store(p.state_out, state + (int64_t)j * p.D, in, p.vec_state);
+        t.store(static_cast<T*>(p.state_out) + state + (int64_t)j * p.D, in, p.vec_state);
       }
     }
     ++nxt;
@@ -148,14 +157,14 @@ Lists lists_of(const int32_t* offsets, const int32_t* slots, int64_t rows, int32
 }
 bool ssm_dtype(int dtype) { return dtype == XB_F32 || dtype == XB_F16 || dtype == XB_BF16; }
 
-template <int SIZE, int V, int K>
+template <typename T, int V, int K>
 int launch_conv_taps(const ConvParams& p, cudaStream_t s) {
   const int64_t blocks = ((int64_t)p.n_chunks * p.pieces + CONV_THREADS - 1) / CONV_THREADS;
   XB_REQUIRE(blocks < ((int64_t)1 << 31), XB_ERR_LIMIT, "xb_ssm_conv: too many rows and channels");
-  launch_dependent(ssm_conv_kernel<SIZE, V, K>, (unsigned)blocks, CONV_THREADS, 0, s, p);
+  launch_dependent(ssm_conv_kernel<T, V, K>, (unsigned)blocks, CONV_THREADS, 0, s, p);
   return check_launch("ssm_conv_kernel");
 }
-template <int SIZE, int V>
+template <typename T, int V>
 int launch_conv_pieces(ConvParams p, int K, cudaStream_t s) {
   p.pieces = (p.D + V - 1) / V;
   // Longer walks read less twice, shorter ones keep more threads in flight. Single rows: nothing is read twice.
@@ -163,36 +172,30 @@ int launch_conv_pieces(ConvParams p, int K, cudaStream_t s) {
   p.rows_a_chunk = (int)std::min<int64_t>(std::max<int64_t>(threads / fill, 1), !p.lists.offsets && p.lists.per <= 1 ? 1 : 32);
   p.n_chunks = (int)std::max<int64_t>((p.lists.rows + p.rows_a_chunk - 1) / p.rows_a_chunk, 1);
   switch (K) {
-    case 2: return launch_conv_taps<SIZE, V, 2>(p, s);
-    case 3: return launch_conv_taps<SIZE, V, 3>(p, s);
-    case 4: return launch_conv_taps<SIZE, V, 4>(p, s);
-    case 5: return launch_conv_taps<SIZE, V, 5>(p, s);
-    case 6: return launch_conv_taps<SIZE, V, 6>(p, s);
-    case 7: return launch_conv_taps<SIZE, V, 7>(p, s);
-    default: return launch_conv_taps<SIZE, V, 8>(p, s);
+    case 2: return launch_conv_taps<T, V, 2>(p, s);
+    case 3: return launch_conv_taps<T, V, 3>(p, s);
+    case 4: return launch_conv_taps<T, V, 4>(p, s);
+    case 5: return launch_conv_taps<T, V, 5>(p, s);
+    case 6: return launch_conv_taps<T, V, 6>(p, s);
+    case 7: return launch_conv_taps<T, V, 7>(p, s);
+    default: return launch_conv_taps<T, V, 8>(p, s);
   }
 }
 bool whole(const void* q, int64_t ld_bytes, int64_t unit) { return reinterpret_cast<uintptr_t>(q) % unit == 0 && ld_bytes % unit == 0; }
-template <int SIZE>
+template <typename T>
 int launch_conv(const xb_ssm_conv_args& a, cudaStream_t s) {
+  constexpr int SIZE = sizeof(T);
   ConvParams p = {};
   p.x = a.x; p.ldx = a.ldx; p.y = a.y; p.ldy = a.ldy; p.w = a.w; p.bias = a.bias; p.state_in = a.state_in; p.state_out = a.state_out;
   p.lists = lists_of(a.offsets, a.slots, a.rows, a.batch, a.n_slots);
-  p.D = a.D; p.silu = a.silu; p.bf16 = a.dtype == XB_BF16;
+  p.D = a.D; p.silu = a.silu;
   p.vec = whole(a.x, a.ldx * SIZE, 16) && whole(a.y, a.ldy * SIZE, 16);
   p.vec_w = whole(a.w, 0, 16) && whole(a.bias, 0, 16);
   p.vec_state = whole(a.state_in, (int64_t)a.D * SIZE, 16) && whole(a.state_out, 0, 16);
   // rows that do not start on 16 bytes: a channel a thread, adjacent lanes adjacent channels
-  return p.vec ? launch_conv_pieces<SIZE, 16 / SIZE>(p, a.K, s) : launch_conv_pieces<SIZE, 1>(p, a.K, s);
+  return p.vec ? launch_conv_pieces<T, 16 / SIZE>(p, a.K, s) : launch_conv_pieces<T, 1>(p, a.K, s);
 }
 
-// What a scan runs as.
-struct ScanPlan {
-  enum { STEP, LISTS, CHUNKS } how;
-  int lanes, K;                           // lanes of a channel; channels of a lane
-  int64_t chunk;
-  int n_chunks;
-};
 int scan_blocks(const xb_ssm_scan_args& a, int lanes, int K) {
   const int per = a.D / a.groups, ch = SCAN_THREADS / lanes * K;
   return a.groups * ((per + ch - 1) / ch);
@@ -200,22 +203,25 @@ int scan_blocks(const xb_ssm_scan_args& a, int lanes, int K) {
 ScanPlan scan_plan(const xb_ssm_scan_args& a) {
   ScanPlan p = {};
   p.lanes = a.N <= 4 ? 1 : a.N <= 8 ? 2 : a.N <= 16 ? 4 : a.N <= 32 ? 8 : 16;
-  if (!a.offsets && a.rows == a.batch) { p.how = ScanPlan::STEP; return p; }
-  const double sms = std::max(sm_count(), 1);
-  const double longest = !a.offsets ? (double)(a.rows / a.batch) : (double)(a.longest > 0 ? std::min(a.longest, a.rows) : a.rows);
+  p.step = !a.offsets && a.rows == a.batch;
+  if (p.step) return p;
+  const double sms = std::max(sm_count(), 1), mean = (double)a.rows / a.batch;
+  const double longest = !a.offsets ? mean : (double)(a.longest > 0 ? std::min(a.longest, a.rows) : a.rows);
+  // Cycles: a row of a block takes `work` of a full SM and `alone` where its SM has little else, which is what the longest list (or
+  // chunk) ends with. Lists that are split are walked nearly twice; of lists of all lengths the share in ones above `chunk` rows is
+  // that of an exponential distribution. us, whole lists and the best split: 256 lists of up to 1860 rows in 70000, D = 256 241,
+  // 230; 16 of up to 3640 in 16384, D = 512 246, 128; one of 4096, D = 1024 302, 70; 300 of 100, D = 256 67, 124.
   double best = 0;
-  for (int K : {1, 4}) {
-    // cycles of a row of a block: of an SM with four blocks, and of one alone
-    const double work = K == 4 ? 160 : 50, alone = K == 4 ? 260 : 100;
-    const int blocks = scan_blocks(a, p.lanes, K);
-    const double full = (double)a.rows * blocks * work / sms, lists = std::max(full, longest * alone);
-    if (best == 0 || lists < best) { best = lists; p.how = ScanPlan::LISTS; p.K = K; }
-    int64_t n = std::min<int64_t>((int64_t)(8 * sms) / blocks, a.rows / 64);
-    if (n < 2) continue;
-    const int64_t chunk = (a.rows + n - 1) / n;
-    n = (a.rows + chunk - 1) / chunk;
-    const double chunks = 1.8 * std::max(full, chunk * alone) + 20000;
-    if (chunks < best) { best = chunks; p.how = ScanPlan::CHUNKS; p.K = K; p.chunk = chunk; p.n_chunks = (int)n; }
+  for (int K : {1, 2}) {
+    if (K == 1 && p.lanes > 4) continue;  // (a block would have 16 channels or fewer)
+    const double work = K == 2 ? 155 : 80, alone = K == 2 ? 260 : 130;
+    const double full = (double)a.rows * scan_blocks(a, p.lanes, K) * work / sms, whole = full + 0.6 * alone * longest;
+    if (best == 0 || whole < best) { best = whole; p.K = K; p.chunk = 0; }
+    for (int64_t chunk = 64; chunk < longest; chunk *= 2) {
+      const double twice = longest > 1.5 * mean ? (1 + chunk / mean) * std::exp(-chunk / mean) : 1;
+      const double split = full * (1 + 0.8 * twice) + 1.2 * alone * chunk + 20000;
+      if (split < best) { best = split; p.K = K; p.chunk = chunk; }
+    }
   }
   return p;
 }
@@ -223,58 +229,22 @@ constexpr size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 struct ScanScratch { size_t end, first, steps, kind, bytes; };
 ScanScratch scan_scratch(const xb_ssm_scan_args& a, const ScanPlan& p) {
   ScanScratch w = {};
-  if (p.how != ScanPlan::CHUNKS) return w;
-  const size_t states = align256((size_t)p.n_chunks * a.D * a.N * 4);
+  if (p.chunk == 0 || a.rows / p.chunk == 0) return w;
+  const size_t n = (size_t)(a.rows / p.chunk), states = align256(n * a.D * a.N * 4);
   w.first = w.end + states;
   w.steps = w.first + (a.h_in ? states : 0);
-  w.kind = w.steps + align256((size_t)p.n_chunks * a.D * 4);
-  w.bytes = w.kind + align256((size_t)p.n_chunks * 4);
+  w.kind = w.steps + align256(n * a.D * 4);
+  w.bytes = w.kind + align256(n * 4);
   return w;
 }
 
-template <int SIZE, int LPC, int K>
-int launch_tiles(const ScanParams& p, const ScanPlan& plan, cudaStream_t s) {
-  const int ch = ScanShape<LPC, K>::CH, a_group = (p.per_group + ch - 1) / ch, blocks = a_group * p.groups;
-  const int64_t units = plan.how == ScanPlan::LISTS ? p.lists.batch : plan.n_chunks;
-  XB_REQUIRE(units * blocks < ((int64_t)1 << 31), XB_ERR_LIMIT, "xb_ssm_scan: too many lists and channels");
-  if (plan.how == ScanPlan::LISTS) {
-    launch_dependent(ssm_scan_kernel<SIZE, LPC, K, SCAN_LISTS>, (unsigned)(units * blocks), SCAN_THREADS, 0, s, p, a_group);
-    return check_launch("ssm_scan_kernel");
-  }
-  launch_dependent(ssm_scan_kernel<SIZE, LPC, K, SCAN_TAILS>, (unsigned)((units - 1) * blocks), SCAN_THREADS, 0, s, p, a_group);
-  if (int rc = check_launch("ssm_scan_kernel")) return rc;
-  launch_dependent(ssm_carry_kernel, (unsigned)(((int64_t)p.D * p.N + 31) / 32), 32 * CARRY_PARTS, 0, s, p);
-  if (int rc = check_launch("ssm_carry_kernel")) return rc;
-  launch_dependent(ssm_scan_kernel<SIZE, LPC, K, SCAN_CHUNKS>, (unsigned)(units * blocks), SCAN_THREADS, 0, s, p, a_group);
-  return check_launch("ssm_scan_kernel");
-}
-template <int SIZE, int LPC>
-int launch_lanes(const ScanParams& p, const ScanPlan& plan, cudaStream_t s) {
-  if (plan.how == ScanPlan::STEP) {
-    const int ch = SCAN_THREADS / LPC * STEP_U, blocks = (p.D + ch - 1) / ch;
-    XB_REQUIRE((int64_t)blocks * p.lists.batch < ((int64_t)1 << 31), XB_ERR_LIMIT, "xb_ssm_scan: too many lists and channels");
-    launch_dependent(ssm_step_kernel<SIZE, LPC>, (unsigned)((int64_t)blocks * p.lists.batch), SCAN_THREADS, 0, s, p, blocks);
-    return check_launch("ssm_step_kernel");
-  }
-  return plan.K == 4 ? launch_tiles<SIZE, LPC, 4>(p, plan, s) : launch_tiles<SIZE, LPC, 1>(p, plan, s);
-}
-template <int SIZE>
-int launch_scan(const ScanParams& p, const ScanPlan& plan, cudaStream_t s) {
-  switch (plan.lanes) {
-    case 1: return launch_lanes<SIZE, 1>(p, plan, s);
-    case 2: return launch_lanes<SIZE, 2>(p, plan, s);
-    case 4: return launch_lanes<SIZE, 4>(p, plan, s);
-    case 8: return launch_lanes<SIZE, 8>(p, plan, s);
-    default: return launch_lanes<SIZE, 16>(p, plan, s);
-  }
-}
 ScanParams scan_params(const xb_ssm_scan_args& a, const ScanPlan& plan, uint8_t* ws) {
   ScanParams p = {};
   p.x = a.x; p.ldx = a.ldx; p.delta = a.delta; p.lddelta = a.lddelta; p.z = a.z; p.ldz = a.ldz;
   p.B = a.B; p.ldb = a.ldb; p.C = a.C; p.ldc = a.ldc; p.y = a.y; p.ldy = a.ldy;
   p.A = a.A; p.skip = a.skip; p.delta_bias = a.delta_bias; p.h_in = a.h_in; p.h_out = a.h_out;
   p.lists = lists_of(a.offsets, a.slots, a.rows, a.batch, a.n_slots);
-  p.D = a.D; p.N = a.N; p.per_group = a.D / a.groups; p.groups = a.groups; p.softplus = a.softplus; p.bf16 = a.dtype == XB_BF16;
+  p.D = a.D; p.N = a.N; p.per_group = a.D / a.groups; p.groups = a.groups; p.softplus = a.softplus;
   const int64_t size = (int64_t)dtype_size(a.dtype);
   p.vec = whole(a.x, a.ldx * size, 16) && whole(a.delta, a.lddelta * size, 16) && whole(a.y, a.ldy * size, 16) &&
           (!a.z || whole(a.z, a.ldz * size, 16)) && (a.groups == 1 || p.per_group * size % 16 == 0);
@@ -282,7 +252,7 @@ ScanParams scan_params(const xb_ssm_scan_args& a, const ScanPlan& plan, uint8_t*
   p.vec_h = a.N % 4 == 0 && whole(a.A, 0, 16) && whole(a.h_in, 0, 16) && whole(a.h_out, 0, 16);
   const ScanScratch w = scan_scratch(a, plan);
   if (w.bytes) {
-    p.chunk = plan.chunk; p.n_chunks = plan.n_chunks;
+    p.chunk = plan.chunk; p.n_ends = (int)(a.rows / plan.chunk);
     p.end = reinterpret_cast<float*>(ws + w.end); p.first = reinterpret_cast<float*>(ws + w.first);
     p.steps = reinterpret_cast<float*>(ws + w.steps); p.kind = reinterpret_cast<int*>(ws + w.kind);
   }
@@ -304,7 +274,9 @@ extern "C" int xb_ssm_conv(const xb_ssm_conv_args* a, xb_stream_t s) {
   XB_REQUIRE(a->w && (a->rows == 0 || (a->x && a->y)), XB_ERR_ARG, "xb_ssm_conv: null tensor");
   XB_REQUIRE(a->rows == 0 || (a->ldx >= a->D && a->ldy >= a->D), XB_ERR_ARG, "xb_ssm_conv: row strides %lld, %lld of %d channels",
              (long long)a->ldx, (long long)a->ldy, a->D);
-  return a->dtype == XB_F32 ? launch_conv<4>(*a, (cudaStream_t)s) : launch_conv<2>(*a, (cudaStream_t)s);
+  if (a->dtype == XB_F32) return launch_conv<float>(*a, (cudaStream_t)s);
+  if (a->dtype == XB_F16) return launch_conv<__half>(*a, (cudaStream_t)s);
+  return launch_conv<__nv_bfloat16>(*a, (cudaStream_t)s);
 }
 
 namespace {
@@ -340,5 +312,7 @@ extern "C" int xb_ssm_scan(const xb_ssm_scan_args* a, void* workspace, size_t wo
              workspace_bytes, need);
   XB_REQUIRE(need == 0 || (reinterpret_cast<uintptr_t>(workspace) & 15) == 0, XB_ERR_ARG, "xb_ssm_scan: the workspace is not on 16 bytes");
   const ScanParams p = scan_params(*a, plan, static_cast<uint8_t*>(workspace));
-  return a->dtype == XB_F32 ? launch_scan<4>(p, plan, (cudaStream_t)s) : launch_scan<2>(p, plan, (cudaStream_t)s);
+  if (a->dtype == XB_F32) return ssm_scan_f32(p, plan, (cudaStream_t)s);
+  if (a->dtype == XB_F16) return ssm_scan_f16(p, plan, (cudaStream_t)s);
+  return ssm_scan_bf16(p, plan, (cudaStream_t)s);
 }

@@ -270,46 +270,25 @@ class DinTower:
         return out
 
 
-def _same(what, device, **tensors):
-    """The tensors that are given lie on the device the call runs on."""
-    for n, t in tensors.items():
-        if t is not None and t.device != device:
-            raise capi.XbError("%s: %s is on %s, the call on %s" % (what, n, t.device, device))
+_checked = None
 
 
-def _rows(what, name, t, rows, width, dtype):
-    if t.dim() != 2 or t.dtype != dtype or t.size(0) != rows or t.size(1) != width or (width > 1 and t.stride(1) != 1):
-        raise capi.XbError("%s: %s is [%d, %d] of %s with adjacent columns" % (what, name, rows, width, dtype))
+def _calls():
+    """The extension module's calls that check their tensors themselves."""
+    global _checked
+    if _checked is None:
+        m = binding()
+        m.dtypes(_DT)
+        m.scratch(lambda like, n: like.new_empty((n,), dtype=torch.uint8))
+        _checked = m
+    return _checked
 
 
-def _dense(what, name, t, shape, dtype):
-    if tuple(t.shape) != tuple(shape) or t.dtype != dtype or not t.is_contiguous():
-        raise capi.XbError("%s: %s is a contiguous %s of %s" % (what, name, list(shape), dtype))
-
-
-def _lists(what, a, rows, offsets, T, slots, first, last, inner, dtype):
-    """rows, offsets, slots and kept states of the lists of a call into its arguments."""
-    if offsets is not None:
-        if offsets.dim() != 1 or offsets.dtype != torch.int32 or offsets.numel() < 1 or not offsets.is_contiguous():
-            raise capi.XbError("%s: offsets are a contiguous int32 [lists + 1]" % what)
-        a.batch = offsets.numel() - 1
-    else:
-        T = rows if T is None else T
-        if T < 0 or (rows and (T < 1 or rows % T)):
-            raise capi.XbError("%s: lists of %d rows in %d rows" % (what, T, rows))
-        a.batch = rows // T if T else 0
-    a.rows, a.offsets = rows, ptr(offsets)
-    if slots is not None:
-        _dense(what, "slots", slots, (a.batch,), torch.int32)
-        a.slots = slots.data_ptr()
-    n = None
-    for name, t in (("the first states", first), ("the last states", last)):
-        if t is None:
-            continue
-        if t.dim() != 3 or tuple(t.shape[1:]) != inner or t.dtype != dtype or not t.is_contiguous() or (n is not None and t.size(0) != n):
-            raise capi.XbError("%s: %s are a contiguous [slots, %d, %d] of %s" % ((what, name) + inner + (dtype,)))
-        n = t.size(0)
-    a.n_slots = n or 0
+def _done(rc):
+    """0, the C function's refusal, or the text of a tensor's"""
+    if rc.__class__ is str:
+        raise capi.XbError(rc)
+    check(rc)
 
 
 def ssm_conv(x, w, bias=None, offsets=None, T=None, state_in=None, state_out=None, slots=None, silu=True, out=None):
@@ -318,58 +297,25 @@ def ssm_conv(x, w, bias=None, offsets=None, T=None, state_in=None, state_out=Non
     w [D, K], bias [D]. Lists: `offsets` int32 [lists + 1], or of T rows each (T = 1: one new row a list; None: one list).
     state_in / state_out [slots, K - 1, D]: the inputs before each list and the last ones of it, in row slots[i] for list i (its own
     number without `slots`); they may be one array. Returns [rows, D]; rows behind the last list are not written."""
-    rows, D = x.shape
-    K = w.size(-1)
-    dev = torch.device("cuda", torch.cuda.current_device())
-    _same("ssm_conv", dev, x=x, w=w, bias=bias, offsets=offsets, state_in=state_in, state_out=state_out, slots=slots, out=out)
+    m = _checked or _calls()
     if out is None:
-        out = torch.empty((rows, D), dtype=x.dtype, device=x.device)
-    _rows("ssm_conv", "x", x, rows, D, x.dtype)
-    _rows("ssm_conv", "out", out, rows, D, x.dtype)
-    _dense("ssm_conv", "w", w, (D, K), x.dtype)
-    if bias is not None:
-        _dense("ssm_conv", "bias", bias, (D,), x.dtype)
-    a = capi.SsmConvArgs()
-    _lists("ssm_conv", a, rows, offsets, T, slots, state_in, state_out, (K - 1, D), x.dtype)
-    a.x, a.ldx, a.y, a.ldy, a.w, a.bias = x.data_ptr(), x.stride(0), out.data_ptr(), out.stride(0), w.data_ptr(), ptr(bias)
-    a.state_in, a.state_out, a.D, a.K, a.silu, a.dtype = ptr(state_in), ptr(state_out), D, K, int(silu), dt(x)
-    check(lib().xb_ssm_conv(C.byref(a), stream()))
+        out = x.new_empty(x.shape)
+    _done(m.ssm_conv(x, w, bias, offsets, T, state_in, state_out, slots, silu, out, torch.cuda.current_device(), raw_stream()))
     return out
 
 
-def ssm_scan(x, delta, A, B, C_, D=None, z=None, delta_bias=None, groups=1, softplus=True, offsets=None, T=None, longest=0, h_in=None,
+def ssm_scan(x, delta, A, B, C, D=None, z=None, delta_bias=None, groups=1, softplus=True, offsets=None, T=None, longest=0, h_in=None,
              h_out=None, slots=None, out=None, workspace=None):
     """The selective state-space scan over lists that lie one after the other in the rows of x [rows, channels].
 
-    delta, z as x; B, C_ [rows, groups * N]; A [channels, N], D and delta_bias [channels], h_in / h_out [slots, channels, N] fp32.
+    delta, z as x; B, C [rows, groups * N]; A [channels, N], D and delta_bias [channels], h_in / h_out [slots, channels, N] fp32.
     Lists and slots as in ssm_conv; `longest`: rows of the longest list where the caller knows it (the plan goes by it, no result).
     `workspace`: uint8 scratch for callers that keep one; by default the call takes its own."""
-    rows, ch = x.shape
-    N = A.size(-1)
-    dev = torch.device("cuda", torch.cuda.current_device())
-    _same("ssm_scan", dev, x=x, delta=delta, A=A, B=B, C=C_, D=D, z=z, delta_bias=delta_bias, offsets=offsets, h_in=h_in, h_out=h_out,
-          slots=slots, out=out, workspace=workspace)
+    m = _checked or _calls()
     if out is None:
-        out = torch.empty((rows, ch), dtype=x.dtype, device=x.device)
-    for n, t, width in (("x", x, ch), ("delta", delta, ch), ("z", z, ch), ("B", B, groups * N), ("C", C_, groups * N), ("out", out, ch)):
-        if t is not None:
-            _rows("ssm_scan", n, t, rows, width, x.dtype)
-    _dense("ssm_scan", "A", A, (ch, N), torch.float32)
-    for n, t in (("D", D), ("delta_bias", delta_bias)):
-        if t is not None:
-            _dense("ssm_scan", n, t, (ch,), torch.float32)
-    a = capi.SsmScanArgs()
-    _lists("ssm_scan", a, rows, offsets, T, slots, h_in, h_out, (ch, N), torch.float32)
-    a.x, a.ldx, a.delta, a.lddelta, a.y, a.ldy = x.data_ptr(), x.stride(0), delta.data_ptr(), delta.stride(0), out.data_ptr(), out.stride(0)
-    if z is not None:
-        a.z, a.ldz = z.data_ptr(), z.stride(0)
-    a.B, a.ldb, a.C, a.ldc = B.data_ptr(), B.stride(0), C_.data_ptr(), C_.stride(0)
-    a.A, a.skip, a.delta_bias, a.h_in, a.h_out = A.data_ptr(), ptr(D), ptr(delta_bias), ptr(h_in), ptr(h_out)
-    a.D, a.N, a.groups, a.softplus, a.dtype, a.longest = ch, N, groups, int(softplus), dt(x), longest
-    need = int(lib().xb_ssm_scan_workspace_bytes(C.byref(a)))
-    if need and workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
-    check(lib().xb_ssm_scan(C.byref(a), ptr(workspace), workspace.numel() if workspace is not None else 0, stream()))
+        out = x.new_empty(x.shape)
+    _done(m.ssm_scan(x, delta, A, B, C, D, z, delta_bias, groups, softplus, offsets, T, longest, h_in, h_out, slots, out, workspace,
+                     torch.cuda.current_device(), raw_stream()))
     return out
 
 
@@ -378,30 +324,8 @@ def lora_gemm(X, W, A, B, adapter, bias=None, scale=None, trans_b=False, out_dty
 
     X [M, K]; W [K, N], or [N, K] with trans_b; A [adapters, r, K]; B [adapters, N, r]; adapter int32 [M], outside [0, adapters) for a
     row without one; bias [N] and scale [adapters] fp32. Results in X's type or fp32."""
-    M, K = X.shape
-    N = W.size(0 if trans_b else 1)
-    dev = torch.device("cuda", torch.cuda.current_device())
-    _same("lora_gemm", dev, X=X, W=W, A=A, B=B, adapter=adapter, bias=bias, scale=scale, Y=Y, workspace=workspace)
+    m = _checked or _calls()
     if Y is None:
-        Y = torch.empty((M, N), dtype=out_dtype or X.dtype, device=X.device)
-    n, r, _ = A.shape
-    _rows("lora_gemm", "X", X, M, K, X.dtype)
-    _rows("lora_gemm", "W", W, N if trans_b else K, K if trans_b else N, X.dtype)
-    _rows("lora_gemm", "Y", Y, M, N, Y.dtype if out_dtype is None else out_dtype)
-    _dense("lora_gemm", "adapter", adapter, (M,), torch.int32)
-    for name, t, rows, cols in (("A", A, r, K), ("B", B, N, r)):
-        if t.dim() != 3 or t.dtype != X.dtype or tuple(t.shape) != (n, rows, cols) or (cols > 1 and t.stride(2) != 1):
-            raise capi.XbError("lora_gemm: %s is [%d, %d, %d] of %s with adjacent columns" % (name, n, rows, cols, X.dtype))
-    for name, t, size in (("bias", bias, N), ("scale", scale, n)):
-        if t is not None:
-            _dense("lora_gemm", name, t, (size,), torch.float32)
-    a = capi.LoraArgs()
-    a.M, a.N, a.K, a.r, a.n_adapters, a.trans_w = M, N, K, r, n, int(trans_b)
-    a.X, a.ldx, a.W, a.ldw, a.Y, a.ldy = X.data_ptr(), X.stride(0), W.data_ptr(), W.stride(0), Y.data_ptr(), Y.stride(0)
-    a.A, a.lda, a.stride_a, a.B, a.ldb, a.stride_b = A.data_ptr(), A.stride(1), A.stride(0), B.data_ptr(), B.stride(1), B.stride(0)
-    a.scale, a.bias, a.adapter, a.dtype, a.y_dtype = ptr(scale), ptr(bias), adapter.data_ptr(), dt(X), dt(Y)
-    need = int(lib().xb_lora_workspace_bytes(C.byref(a)))
-    if need and workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=X.device)
-    check(lib().xb_lora_gemm(C.byref(a), ptr(workspace), workspace.numel() if workspace is not None else 0, stream()))
+        Y = X.new_empty((X.shape[0], W.shape[0 if trans_b else 1]), dtype=out_dtype)
+    _done(m.lora_gemm(X, W, A, B, adapter, bias, scale, trans_b, Y, workspace, torch.cuda.current_device(), raw_stream()))
     return Y
