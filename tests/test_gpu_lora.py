@@ -58,7 +58,9 @@ def _check(s, dtype, out, trans, **more):
 @pytest.mark.parametrize("M,K,N,n,r,trans,pad", [
     (1, 16, 8, 1, 1, True, 0), (7, 40, 24, 3, 4, False, 0), (64, 72, 80, 64, 16, True, 8), (129, 250, 131, 5, 12, False, 0),
     (300, 324, 200, 4, 8, True, 4), (1000, 64, 256, 7, 16, True, 0), (513, 128, 48, 2, 64, False, 0), (260, 88, 176, 3, 32, True, 8),
-    (130, 16, 8, 200, 3, True, 0), (256, 200, 80, 1, 100, True, 0), (700, 512, 304, 6, 24, True, 0)])
+    (130, 16, 8, 200, 3, True, 0), (256, 200, 80, 1, 100, True, 0), (700, 512, 304, 6, 24, True, 0), (600, 72, 40, 3, 100, False, 0),
+    (1111, 324, 200, 12, 8, True, 4), (2000, 640, 520, 40, 16, True, 0), (513, 1280, 1024, 3, 128, True, 0), (900, 24, 1000, 5, 33, False, 0),
+    (640, 136, 17, 9, 20, True, 0)])
 def test_lora(dtype, out, how, M, K, N, n, r, trans, pad):
     rng = np.random.default_rng(M + K + N)
     _check(_case(rng, M, K, N, n, r, dtype, trans, pad, how), dtype, out, trans)
@@ -71,12 +73,13 @@ def test_more_rows_than_a_turn():
     _check(s, "f32", "f32", True)
 
 
-def test_wide_range_of_the_intermediate():
+@pytest.mark.parametrize("M", [200, 700])
+def test_wide_range_of_the_intermediate(M):
     """U = X A^T far above what fp16 holds, and far below its normal numbers, with results that fit."""
     ops, capi = _ops()
     rng = np.random.default_rng(10)
     for up, down in ((2.0 ** 9, 2.0 ** -14), (2.0 ** -11, 2.0 ** 9)):
-        s = _case(rng, 200, 256, 64, 2, 8, "f16", True, 0, "runs")
+        s = _case(rng, M, 256, 64, 2, 8, "f16", True, 0, "runs")
         s["X"] = (s["X"] * (up if up > 1 else 0.1)).contiguous()
         s["A"] = (s["A"] * up).contiguous()
         s["B"] = (s["B"] * down).contiguous()
@@ -84,17 +87,18 @@ def test_wide_range_of_the_intermediate():
         _check(s, "f16", "f16", True)
 
 
-def test_bad_values_stay_in_their_rows():
+@pytest.mark.parametrize("M", [400, 1300])
+def test_bad_values_stay_in_their_rows(M):
     """A row's NaN or infinity, and an adapter that no row names, reach no other row."""
     ops, capi = _ops()
     rng = np.random.default_rng(11)
-    s = _case(rng, 400, 128, 96, 4, 16, "f16", True, 0, "mixed")
+    s = _case(rng, M, 128, 96, 4, 16, "f16", True, 0, "mixed")
     s["adapter"].clamp_(max=2)
     call = lambda: ops.lora_gemm(s["X"], s["W"], s["A"], s["B"], s["adapter"], bias=s["bias"], scale=s["scale"], trans_b=True)
     y = call()
     s["X"][17], s["X"][250], s["A"][3], s["B"][3] = float("nan"), float("inf"), float("nan"), float("inf")
     again = call()
-    others = [m for m in range(400) if m not in (17, 250)]
+    others = [m for m in range(M) if m not in (17, 250)]
     assert torch.equal(again[others], y[others]) and not torch.isfinite(again[17]).any() and not torch.isfinite(again[250]).all()
 
 

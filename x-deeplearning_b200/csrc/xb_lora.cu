@@ -3,6 +3,7 @@
 #include <cstring>
 
 #include "xb_common.cuh"
+#include "xb_lora_umma.cuh"
 
 namespace xb {
 namespace {
@@ -29,7 +30,7 @@ __device__ __forceinline__ int adapter_of(const LoraParams& p, int m) {
 
 // A warp a row: its products with the r rows of its adapter, the lanes along K.
 template <typename T>
-__global__ void __launch_bounds__(256) lora_shrink_kernel(const LoraParams p) {
+__global__ void __launch_bounds__(256) lora_rows_shrink_kernel(const LoraParams p) {
   pdl_begin();
   const int m = blockIdx.x * 8 + threadIdx.x / 32, lane = threadIdx.x % 32;
   if (m >= p.M) return;
@@ -49,7 +50,7 @@ __global__ void __launch_bounds__(256) lora_shrink_kernel(const LoraParams p) {
 
 // A block a row, a thread an output at a time.
 template <typename T>
-__global__ void __launch_bounds__(128) lora_expand_kernel(const LoraParams p) {
+__global__ void __launch_bounds__(128) lora_rows_expand_kernel(const LoraParams p) {
   pdl_begin();
   const int m = blockIdx.x;
   const int a = adapter_of(p, m);
@@ -65,6 +66,9 @@ __global__ void __launch_bounds__(128) lora_expand_kernel(const LoraParams p) {
     p.part[(int64_t)m * p.N + n] = s;
   }
 }
+
+// Few rows: the tiles would leave most SMs idle, and a tile of many adapters walks through all of them.
+bool takes_tiles(const xb_lora_args& a) { return a.M >= 512 && lora_umma_takes(a); }
 
 constexpr size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
@@ -110,11 +114,11 @@ int run_rows(const xb_lora_args& a, uint8_t* ws, cudaStream_t s) {
     p.X = reinterpret_cast<const T*>(a.X) + m0 * a.ldx;
     p.adapter = p.n_adapters ? a.adapter + m0 : nullptr;
     if (p.n_adapters) {
-      launch_dependent(lora_shrink_kernel<T>, (unsigned)((p.M + 7) / 8), 256, 0, s, p);
-      if (int rc = check_launch("lora_shrink_kernel")) return rc;
+      launch_dependent(lora_rows_shrink_kernel<T>, (unsigned)((p.M + 7) / 8), 256, 0, s, p);
+      if (int rc = check_launch("lora_rows_shrink_kernel")) return rc;
     }
-    launch_dependent(lora_expand_kernel<T>, (unsigned)p.M, 128, 0, s, p);
-    if (int rc = check_launch("lora_expand_kernel")) return rc;
+    launch_dependent(lora_rows_expand_kernel<T>, (unsigned)p.M, 128, 0, s, p);
+    if (int rc = check_launch("lora_rows_expand_kernel")) return rc;
     g.M = p.M;
     g.A = p.X;
     g.Y = reinterpret_cast<uint8_t*>(a.Y) + m0 * a.ldy * (int64_t)dtype_size(a.y_dtype);
@@ -124,12 +128,17 @@ int run_rows(const xb_lora_args& a, uint8_t* ws, cudaStream_t s) {
 }
 
 }  // namespace
+
+int lora_status(int* out) { return umma::read_status_word(out); }
+int lora_clear_status() { return umma::clear_status_word(); }
+int lora_set_status_mirror(int* p) { return umma::set_status_mirror(p); }
 }  // namespace xb
 
 using namespace xb;
 
 extern "C" size_t xb_lora_workspace_bytes(const xb_lora_args* a) {
   if (check_args(a) != 0 || a->M == 0 || a->N == 0) return 0;
+  if (takes_tiles(*a)) return lora_scratch(*a).bytes;
   const size_t turn = (size_t)turn_rows(*a);
   return align256(turn * a->r * 4) + turn * a->N * 4;
 }
@@ -140,6 +149,7 @@ extern "C" int xb_lora_gemm(const xb_lora_args* a, void* workspace, size_t works
   const size_t need = xb_lora_workspace_bytes(a);
   XB_REQUIRE(workspace && workspace_bytes >= need, XB_ERR_SCRATCH, "xb_lora_gemm: workspace of %zu bytes, %zu needed", workspace_bytes, need);
   XB_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, XB_ERR_ARG, "xb_lora_gemm: the workspace is not on 16 bytes");
+  if (takes_tiles(*a)) return run_umma(*a, static_cast<uint8_t*>(workspace), (cudaStream_t)s);
   if (a->dtype == XB_F32) return run_rows<float>(*a, static_cast<uint8_t*>(workspace), (cudaStream_t)s);
   if (a->dtype == XB_F16) return run_rows<__half>(*a, static_cast<uint8_t*>(workspace), (cudaStream_t)s);
   return run_rows<__nv_bfloat16>(*a, static_cast<uint8_t*>(workspace), (cudaStream_t)s);

@@ -1,0 +1,535 @@
+// The tensor-core path of xb_lora_gemm, two kernels:
+//   lora_shrink_kernel   U = scale (X A_a^T), every row with its own adapter's A, in fp32; and B as fp32 beside it
+//   lora_gemm_kernel     Y = X W + bias + U B_a^T: the tiles of the projection, whose depth goes on through the adapters' products
+//
+// Rows of a tile belong to any adapters. For each one that occurs in it (ascending) the MMAs run over all 128 rows, and the lanes of
+// the other rows are disabled, so neither sorting nor padding is asked of the caller; a tile of one request has one adapter.
+// U is held as two TF32 terms, hi + lo, each rounded to nearest (|U - hi - lo| <= 2^-22 |U|), side by side along the depth, and B, whose
+// 16-bit values TF32 holds exactly, is read for both: fp16 would overflow or lose U's range, one term of bf16 would show in the result.
+// The products of adapters cost ceil(r / 16) depth blocks of 32 fp32 for each adapter of a tile beside the ceil(K / 64) of the projection.
+#pragma once
+
+#include "xb_gemm_tile.cuh"
+
+namespace xb {
+namespace {
+
+constexpr uint32_t NO_ADAPTER = 0xffffffffu;
+
+// The adapters of a tile's rows, 32 WORDS of them: lane l has those of rows l, 32 + l, ...
+template <int WORDS>
+struct TileAdapters {
+  uint32_t id[WORDS];
+  __device__ __forceinline__ void load(const int32_t* adapter, int n_adapters, int m0, int M, int lane) {
+#pragma unroll
+    for (int w = 0; w < WORDS; ++w) {
+      const int m = m0 + 32 * w + lane;
+      const int a = m < M ? adapter[m] : -1;
+      id[w] = a >= 0 && a < n_adapters ? (uint32_t)a : NO_ADAPTER;
+    }
+  }
+  // the least that is `from` or above; NO_ADAPTER: none is left. The same for all lanes.
+  __device__ __forceinline__ uint32_t next(uint32_t from) const {
+    uint32_t least = NO_ADAPTER;
+#pragma unroll
+    for (int w = 0; w < WORDS; ++w) least = id[w] >= from ? min(least, id[w]) : least;
+    return __reduce_min_sync(0xffffffffu, least);
+  }
+  // lanes of 32-row word w that an MMA for adapter a leaves as they are
+  __device__ __forceinline__ uint32_t others(int w, uint32_t a) const { return ~__ballot_sync(0xffffffffu, id[w] == a); }
+};
+
+// 128 x N MMAs that leave the rows set in m0..m3 as they are (one bit a row), issued by an elected lane of a warp in uniform control flow
+__device__ __forceinline__ void mma_f16_ss_rows_elect(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, const uint32_t (&m)[4], uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}"
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(m[0]), "r"(m[1]), "r"(m[2]), "r"(m[3])
+      : "memory");
+}
+__device__ __forceinline__ void mma_tf32_ss_rows_elect(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, const uint32_t (&m)[4], uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::tf32 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}"
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(m[0]), "r"(m[1]), "r"(m[2]), "r"(m[3])
+      : "memory");
+}
+constexpr int FMT_TF32 = 2;
+
+__device__ __forceinline__ float round_tf32(float v) {
+  uint32_t r;
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(v));
+  return __uint_as_float(r);
+}
+
+struct LoraTiles {
+  int M, N, K, r, n_adapters;
+  int rb;                                 // rank, rounded up to 16, 32, 64 or 128
+  int u_cols, b_cols;                     // floats of a row of U (2 rb: hi, lo) and of B (rb, at least 32: with rb = 16 it stands there twice)
+  const int32_t* adapter;
+  const float* scale;
+  float* U;                               // [M, u_cols]
+  float* B32;                             // [n_adapters, N, b_cols]
+  const void* B; int64_t ldb, stride_b; int dtype;
+  int group;                              // adapters of a pass of the shrink kernel
+  int stages, tiles_m;
+  uint32_t idesc_a, idesc_ext;
+};
+
+constexpr int SHRINK_THREADS = 320;       // producer, MMA, four warps for the results, four for B
+constexpr int SHRINK_GROUP_ROWS = 64;     // rows of A (adapters x rb) in a stage, or rb where that is more
+
+// Persistent, 128 rows a tile. Bound by reading X once; the adapters' A come from L2. A pass over the depth takes the A of up to 64 / rb
+// adapters with it; tiles of more adapters take more passes.
+__global__ void __launch_bounds__(SHRINK_THREADS, 1)
+lora_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ LoraTiles p) {
+  using namespace umma;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int STAGES = p.stages, box = p.rb * BLOCK_K * 2, stage_bytes = A_STAGE_BYTES + p.group * box;
+  __shared__ __align__(8) uint64_t full_bar[MAX_STAGES];
+  __shared__ __align__(8) uint64_t empty_bar[MAX_STAGES];
+  __shared__ __align__(8) uint64_t acc_full[2];
+  __shared__ __align__(8) uint64_t acc_empty[2];
+  __shared__ uint32_t tmem_base_s;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int num_kb = (p.K + BLOCK_K - 1) / BLOCK_K;
+  const uint32_t tmem_cols = (uint32_t)max(32, 2 * p.rb);
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) { mbar_init(smem_u32(&full_bar[s]), 1); mbar_init(smem_u32(&empty_bar[s]), 1); }
+    for (int s = 0; s < 2; ++s) { mbar_init(smem_u32(&acc_full[s]), 1); mbar_init(smem_u32(&acc_empty[s]), 4); }
+    fence_barrier_init();
+    prefetch_tensormap(&map_x);
+    prefetch_tensormap(&map_a);
+  }
+  if (warp == 1) tmem_alloc(smem_u32(&tmem_base_s), tmem_cols);
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = tmem_base_s;
+  pdl_wait();
+
+  if (warp < 2) {
+    // both walk the same passes: the adapters of a tile, `group` at a time
+    int s = 0, it = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    for (int tile = blockIdx.x; tile < p.tiles_m && ok; tile += gridDim.x) {
+      const int m0 = tile * BLOCK_M;
+      TileAdapters<4> t;
+      t.load(p.adapter, p.n_adapters, m0, p.M, lane);
+      uint32_t first = t.next(0);
+      if (first == NO_ADAPTER) continue;
+      const int as = it & 1;
+      if (warp == 1) {
+        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&acc_empty[as]), ((uint32_t)(it >> 1) & 1u) ^ 1u, 54));
+        tc_fence_after_sync();
+      }
+      while (first != NO_ADAPTER && ok) {
+        uint32_t after = first;                            // the adapters of this pass are in [first, after)
+        int n = 0;
+        for (uint32_t a = first; n < p.group && a != NO_ADAPTER; ++n) { after = a + 1; a = t.next(after); }
+        for (int kb = 0; kb < num_kb; ++kb, s = (s + 1 == STAGES ? 0 : s + 1), ph ^= (s == 0 ? 1u : 0u)) {
+          uint8_t* x = smem + s * stage_bytes;
+          if (warp == 0) {
+            ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&empty_bar[s]), ph ^ 1u, 51));
+            if (!ok) break;
+            if (lane == 0) {
+              mbar_arrive_expect_tx(smem_u32(&full_bar[s]), (uint32_t)(A_STAGE_BYTES + n * box));
+              tma_load_3d(smem_u32(x), &map_x, smem_u32(&full_bar[s]), kb * BLOCK_K, m0, 0);
+            }
+            uint32_t a = first;
+            for (int i = 0; i < n; ++i, a = t.next(a + 1))
+              if (lane == 0) tma_load_3d(smem_u32(x + A_STAGE_BYTES + i * box), &map_a, smem_u32(&full_bar[s]), kb * BLOCK_K, 0, (int)a);
+          } else {
+            ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&full_bar[s]), ph, 52));
+            if (!ok) break;
+            tc_fence_after_sync();
+            uint32_t a = first;
+            for (int i = 0; i < n; ++i, a = t.next(a + 1)) {
+              const uint32_t rows[4] = {t.others(0, a), t.others(1, a), t.others(2, a), t.others(3, a)};
+              const uint32_t x_addr = smem_u32(x), a_addr = smem_u32(x + A_STAGE_BYTES + i * box);
+#pragma unroll
+              for (int k = 0; k < BLOCK_K / 16; ++k)
+                mma_f16_ss_rows_elect(tmem_base + as * p.rb, make_desc_sw128(x_addr + k * 32, 1024), make_desc_sw128(a_addr + k * 32, 1024), p.idesc_a,
+                                      rows, (kb > 0 || k > 0) ? 1u : 0u);
+            }
+            mma_commit_elect(smem_u32(&empty_bar[s]));
+          }
+        }
+        first = t.next(after);
+      }
+      if (warp == 1 && ok) mma_commit_elect(smem_u32(&acc_full[as]));
+      ++it;
+    }
+  } else if (warp < 6) {
+    const int q = warp & 3, row = q * 32 + lane;
+    int it = 0;
+    for (int tile = blockIdx.x; tile < p.tiles_m; tile += gridDim.x) {
+      const int m0 = tile * BLOCK_M, gm = m0 + row;
+      TileAdapters<4> t;
+      t.load(p.adapter, p.n_adapters, m0, p.M, lane);
+      if (t.next(0) == NO_ADAPTER) continue;
+      uint32_t mine = NO_ADAPTER;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) mine = w == q ? t.id[w] : mine;
+      const int as = it & 1;
+      const float scale = mine != NO_ADAPTER && p.scale ? p.scale[mine] : 1.f;
+      if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&acc_full[as]), (uint32_t)(it >> 1) & 1u, 53))) break;
+      tc_fence_after_sync();
+      float* u = p.U + (int64_t)gm * p.u_cols;
+      for (int c = 0; c < p.rb; c += 16) {
+        uint32_t raw[16];
+        tmem_ld16_nowait(tmem_base + as * p.rb + c + ((uint32_t)(q * 32) << 16), raw);
+        tmem_wait_ld(raw);
+        if (mine != NO_ADAPTER) {
+#pragma unroll
+          for (int j = 0; j < 16; j += 4) {
+            float hi[4], lo[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float v = scale * __uint_as_float(raw[j + i]);
+              hi[i] = round_tf32(v);
+              // (an infinity or NaN, or what rounds up to one, stays whole in hi)
+              lo[i] = fabsf(hi[i]) <= 3.4028235e38f ? round_tf32(v - hi[i]) : 0.f;
+            }
+            *reinterpret_cast<float4*>(u + c + j) = make_float4(hi[0], hi[1], hi[2], hi[3]);
+            *reinterpret_cast<float4*>(u + p.rb + c + j) = make_float4(lo[0], lo[1], lo[2], lo[3]);
+          }
+        }
+      }
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&acc_empty[as]));
+      ++it;
+    }
+  } else {
+    // B as fp32, zeros behind its r columns
+    const int64_t quads = (int64_t)p.n_adapters * p.N * (p.b_cols / 4);
+    for (int64_t e = (int64_t)blockIdx.x * 128 + (threadIdx.x - 192); e < quads; e += (int64_t)gridDim.x * 128) {
+      const int64_t an = e / (p.b_cols / 4);
+      const int c = (int)(e - an * (p.b_cols / 4)) * 4, a = (int)(an / p.N), n = (int)(an - (int64_t)a * p.N);
+      float v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int j = (c + i) % p.rb;
+        v[i] = j < p.r ? load_as_f32(p.B, (int64_t)a * p.stride_b + (int64_t)n * p.ldb + j, p.dtype) : 0.f;
+      }
+      reinterpret_cast<float4*>(p.B32)[e] = make_float4(v[0], v[1], v[2], v[3]);
+    }
+  }
+
+  pdl_release();
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem_base, tmem_cols);
+  }
+}
+
+// The one-CTA GEMM kernel of xb_gemm_umma.cu without batches and resident weights, whose tiles go on through the adapters' products: the
+// stages have the same size (128 rows of 128 bytes of X or U, block_n of W or B), only the maps and the MMAs differ.
+enum { LORA_Y_TMA, LORA_Y_ANY };
+template <typename TOut, bool B_MN, int Y>
+__global__ void __launch_bounds__(GEMM_THREADS, 1)
+lora_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_u,
+                 const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_y, const __grid_constant__ UmmaGemmParams p,
+                 const __grid_constant__ LoraTiles l) {
+  using namespace umma;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int w_bytes = (B_MN ? (p.block_n + 63) / 64 * 64 : p.block_n) * BLOCK_K * 2, b_bytes = p.block_n * BLOCK_K * 2;
+  const int STAGES = p.stages;
+  uint8_t* smem_a = smem;
+  uint8_t* smem_b = smem + STAGES * A_STAGE_BYTES;
+  __shared__ __align__(8) uint64_t full_bar[MAX_STAGES];
+  __shared__ __align__(8) uint64_t empty_bar[MAX_STAGES];
+  __shared__ __align__(8) uint64_t acc_full[2];
+  __shared__ __align__(8) uint64_t acc_empty[2];
+  __shared__ uint32_t tmem_base_s;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int num_kb = (p.K + BLOCK_K - 1) / BLOCK_K, u_blocks = l.u_cols / 32, b_blocks = l.b_cols / 32;
+  const uint32_t total_tiles = (uint32_t)p.tiles_m * (uint32_t)p.tiles_n;
+  const uint32_t acc_stride = (uint32_t)p.tmem_cols / 2;
+  auto place = [&](uint32_t tile, int& m0, int& n0) {
+    const uint32_t inner = (uint32_t)(p.n_fast ? p.tiles_n : p.tiles_m), o = tile / inner, i = tile - o * inner;
+    m0 = (int)(p.n_fast ? o : i) * BLOCK_M;
+    n0 = (int)(p.n_fast ? i : o) * p.block_n;
+  };
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) { mbar_init(smem_u32(&full_bar[s]), 1); mbar_init(smem_u32(&empty_bar[s]), 1); }
+    for (int s = 0; s < 2; ++s) { mbar_init(smem_u32(&acc_full[s]), 1); mbar_init(smem_u32(&acc_empty[s]), EPI_WARPS); }
+    fence_barrier_init();
+    prefetch_tensormap(&map_x);
+    prefetch_tensormap(&map_w);
+    prefetch_tensormap(&map_u);
+    prefetch_tensormap(&map_b);
+    if (Y == LORA_Y_TMA) prefetch_tensormap(&map_y);
+  }
+  if (warp == 1) tmem_alloc(smem_u32(&tmem_base_s), (uint32_t)p.tmem_cols);
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = tmem_base_s;
+  pdl_wait();
+
+  if (warp == 0) {
+    int s = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    auto advance = [&]() {
+      s = s + 1 == STAGES ? 0 : s + 1;
+      ph ^= s == 0 ? 1u : 0u;
+    };
+    for (uint32_t tile = blockIdx.x; tile < total_tiles && ok; tile += gridDim.x) {
+      int m0, n0;
+      place(tile, m0, n0);
+      TileAdapters<4> t;
+      t.load(l.adapter, l.n_adapters, m0, p.M, lane);      // (used when the projection's loads are under way)
+      for (int kb = 0; kb < num_kb && ok; ++kb, advance()) {
+        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&empty_bar[s]), ph ^ 1u, 61));
+        if (ok && lane == 0) {
+          const uint32_t bar = smem_u32(&full_bar[s]), w = smem_u32(smem_b + s * w_bytes);
+          mbar_arrive_expect_tx(bar, (uint32_t)(A_STAGE_BYTES + w_bytes));
+          tma_load_3d(smem_u32(smem_a + s * A_STAGE_BYTES), &map_x, bar, kb * BLOCK_K, m0, 0);
+          if (!B_MN) {
+            tma_load_3d(w, &map_w, bar, kb * BLOCK_K, n0, 0);
+          } else {
+            for (int j = 0; j * 64 < p.block_n; ++j) tma_load_3d(w + j * MN_BOX_BYTES, &map_w, bar, n0 + j * 64, kb * BLOCK_K, 0);
+          }
+        }
+      }
+      for (uint32_t a = t.next(0); a != NO_ADAPTER && ok; a = t.next(a + 1)) {
+        for (int e = 0; e < u_blocks && ok; ++e, advance()) {
+          ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&empty_bar[s]), ph ^ 1u, 61));
+          if (ok && lane == 0) {
+            const uint32_t bar = smem_u32(&full_bar[s]);
+            mbar_arrive_expect_tx(bar, (uint32_t)(A_STAGE_BYTES + b_bytes));
+            tma_load_3d(smem_u32(smem_a + s * A_STAGE_BYTES), &map_u, bar, e * 32, m0, 0);
+            tma_load_3d(smem_u32(smem_b + s * w_bytes), &map_b, bar, e % b_blocks * 32, n0, (int)a);
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    int s = 0, it = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    auto advance = [&]() {
+      s = s + 1 == STAGES ? 0 : s + 1;
+      ph ^= s == 0 ? 1u : 0u;
+    };
+    for (uint32_t tile = blockIdx.x; tile < total_tiles && ok; tile += gridDim.x, ++it) {
+      int m0, n0;
+      place(tile, m0, n0);
+      TileAdapters<4> t;
+      t.load(l.adapter, l.n_adapters, m0, p.M, lane);
+      const int as = it & 1;
+      ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&acc_empty[as]), ((uint32_t)(it >> 1) & 1u) ^ 1u, 64));
+      if (!ok) break;
+      tc_fence_after_sync();
+      const uint32_t tmem_acc = tmem_base + as * acc_stride;
+      for (int kb = 0; kb < num_kb; ++kb, advance()) {
+        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&full_bar[s]), ph, 62));
+        if (!ok) break;
+        tc_fence_after_sync();
+        const uint32_t a_addr = smem_u32(smem_a + s * A_STAGE_BYTES), b_addr = smem_u32(smem_b + s * w_bytes);
+#pragma unroll
+        for (int k = 0; k < BLOCK_K / 16; ++k)
+          mma_f16_ss_elect(tmem_acc, make_desc_sw128(a_addr + k * 32, 1024),
+                           B_MN ? make_desc_sw128_mn(b_addr + k * 2048, MN_BOX_BYTES) : make_desc_sw128(b_addr + k * 32, 1024), p.idesc,
+                           (kb > 0 || k > 0) ? 1u : 0u);
+        mma_commit_elect(smem_u32(&empty_bar[s]));
+      }
+      for (uint32_t a = t.next(0); a != NO_ADAPTER && ok; a = t.next(a + 1)) {
+        const uint32_t rows[4] = {t.others(0, a), t.others(1, a), t.others(2, a), t.others(3, a)};
+        for (int e = 0; e < u_blocks; ++e, advance()) {
+          ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&full_bar[s]), ph, 62));
+          if (!ok) break;
+          tc_fence_after_sync();
+          const uint32_t a_addr = smem_u32(smem_a + s * A_STAGE_BYTES), b_addr = smem_u32(smem_b + s * w_bytes);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)                        // 32 fp32 are four steps of 8
+            mma_tf32_ss_rows_elect(tmem_acc, make_desc_sw128(a_addr + k * 32, 1024), make_desc_sw128(b_addr + k * 32, 1024), l.idesc_ext, rows, 1u);
+          mma_commit_elect(smem_u32(&empty_bar[s]));
+        }
+      }
+      if (ok) mma_commit_elect(smem_u32(&acc_full[as]));
+    }
+  } else {
+    // (the epilogue of gemm_umma_kernel; the reasons for the order of its barriers stand there)
+    const int ew = warp - 2, q = warp & 3, part = ew >> 2, row = q * 32 + lane;
+    const int chunks = p.block_n / 16, c_begin = chunks * part / 4, c_end = chunks * (part + 1) / 4;
+    const bool vec_base = ((reinterpret_cast<uintptr_t>(p.Y) & 15) == 0) && ((p.ldy * sizeof(TOut)) % 16 == 0);
+    float* s_bias = reinterpret_cast<float*>(smem_b + STAGES * w_bytes);                           // [4][256]
+    uint4* stage = reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(s_bias + 4 * 256) + ew * EPI_STAGE_BYTES);
+    float *s_a = s_bias + 256, *s_b = s_a + 256, *s_c = s_b + 256;
+    uint8_t* area = reinterpret_cast<uint8_t*>(s_bias + 4 * 256) + ew * p.y_bufs * p.y_unit * 64;
+    uint32_t turn = 0;
+    int it = 0, cur_n0 = -1;
+    bool ok = true;
+    for (uint32_t tile = blockIdx.x; tile < total_tiles; tile += gridDim.x, ++it) {
+      int m0, n0;
+      place(tile, m0, n0);
+      const int as = it & 1, gm = m0 + row;
+      if (n0 != cur_n0) {
+        cur_n0 = n0;
+        asm volatile("bar.sync 2, 512;" ::: "memory");
+        const int e = ew * 32 + lane;
+        if (e < p.block_n) stage_columns(p, 0, n0 + e, e, s_bias, s_a, s_b, s_c);
+        asm volatile("bar.sync 2, 512;" ::: "memory");
+      }
+      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&acc_full[as]), (uint32_t)(it >> 1) & 1u, 63));
+      if (!ok) continue;
+      tc_fence_after_sync();
+      const uint32_t tmem_acc = tmem_base + as * acc_stride + ((uint32_t)(q * 32) << 16);
+      TOut* yrow = reinterpret_cast<TOut*>(p.Y) + (int64_t)gm * p.ldy;
+      if constexpr (Y == LORA_Y_TMA) {
+        const int y = m0 + q * 32, cols = min(p.block_n, p.N - n0);
+        if (p.y_unit == 32)
+          epi_tile_tma<TOut, XB_EPI_NONE, 32>(map_y, tmem_acc, part, cols, 1.f, s_bias, s_a, s_b, s_c, area, p.y_bufs, turn, n0, y, 0, y < p.M, lane);
+        else
+          epi_tile_tma<TOut, XB_EPI_NONE, 16>(map_y, tmem_acc, part, cols, 1.f, s_bias, s_a, s_b, s_c, area, p.y_bufs, turn, n0, y, 0, y < p.M, lane);
+      } else if (sizeof(TOut) == 4 && vec_base && m0 + BLOCK_M <= p.M && n0 + p.block_n <= p.N) {
+        epi_tile_fast<TOut, XB_EPI_NONE, true>(tmem_acc, c_begin, c_end, 1.f, s_bias, s_a, s_b, s_c, yrow + n0, p.ldy, 32, p.block_n, stage, lane);
+      } else {
+        epi_tile_edge<TOut>(p, tmem_acc, c_begin, c_end, s_bias, s_a, s_b, s_c, yrow, 0, gm, gm, n0, vec_base, reinterpret_cast<uint16_t*>(stage), lane);
+      }
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&acc_empty[as]));
+    }
+    if (Y == LORA_Y_TMA && lane == 0) tma_store_wait_read<0>();
+  }
+
+  pdl_release();
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem_base, (uint32_t)p.tmem_cols);
+  }
+}
+
+int make_map_f32(CUtensorMap* map, const void* base, int64_t cols, int64_t rows, int64_t batch, int box_rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return fail(XB_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)batch};
+  cuuint64_t strides[2] = {(cuuint64_t)cols * 4, (cuuint64_t)cols * rows * 4};
+  cuuint32_t box[3] = {32, (cuuint32_t)box_rows, 1}, estr[3] = {1, 1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(XB_ERR_CUDA, "cuTensorMapEncodeTiled failed with %d", (int)r);
+  return 0;
+}
+
+template <typename TOut, bool B_MN, int Y>
+int launch_lora_gemm(const CUtensorMap (&m)[5], const UmmaGemmParams& p, const LoraTiles& l, unsigned grid, size_t smem, cudaStream_t s) {
+  static PerDeviceOnce attr_set;          // per instantiation
+  XB_SET_MAX_SMEM_ONCE(attr_set, 226 * 1024, (const void*)lora_gemm_kernel<TOut, B_MN, Y>);
+  launch_dependent(lora_gemm_kernel<TOut, B_MN, Y>, grid, GEMM_THREADS, smem, s, m[0], m[1], m[2], m[3], m[4], p, l);
+  return check_launch("lora_gemm_kernel");
+}
+
+// What the tensor-core path takes: 16-bit operands that TMA can address, results as xb_gemm has them on that engine.
+bool lora_umma_takes(const xb_lora_args& a) {
+  if (a.dtype != XB_F16 && a.dtype != XB_BF16) return false;
+  if (a.n_adapters < 1 || a.r < 1) return false;
+  if (!a.trans_w && a.y_dtype == XB_F32) return false;     // (its sums are not rounded at every step: see xb_gemm)
+  if (a.ldx % 8 || a.ldw % 8 || a.lda % 8 || (a.n_adapters > 1 && (a.stride_a % 8 || a.stride_a == 0))) return false;
+  return ((reinterpret_cast<uintptr_t>(a.X) | reinterpret_cast<uintptr_t>(a.W) | reinterpret_cast<uintptr_t>(a.A)) & 15) == 0;
+}
+struct LoraScratch { int rb, u_cols, b_cols; size_t u, b, bytes; };
+LoraScratch lora_scratch(const xb_lora_args& a) {
+  LoraScratch w;
+  w.rb = a.r <= 16 ? 16 : a.r <= 32 ? 32 : a.r <= 64 ? 64 : 128;
+  w.u_cols = 2 * w.rb;
+  w.b_cols = std::max(w.rb, 32);
+  w.u = 0;
+  w.b = ((size_t)a.M * w.u_cols * 4 + 255) / 256 * 256;
+  w.bytes = w.b + (size_t)a.n_adapters * a.N * w.b_cols * 4;
+  return w;
+}
+
+int run_umma(const xb_lora_args& a, uint8_t* ws, cudaStream_t stream) {
+  const LoraScratch w = lora_scratch(a);
+  const int bf16 = a.dtype == XB_BF16;
+  LoraTiles l;
+  memset(&l, 0, sizeof(l));
+  l.M = a.M; l.N = a.N; l.K = a.K; l.r = a.r; l.n_adapters = a.n_adapters; l.rb = w.rb; l.u_cols = w.u_cols; l.b_cols = w.b_cols;
+  l.adapter = a.adapter; l.scale = a.scale; l.U = reinterpret_cast<float*>(ws + w.u); l.B32 = reinterpret_cast<float*>(ws + w.b);
+  l.B = a.B; l.ldb = a.ldb; l.stride_b = a.stride_b; l.dtype = a.dtype;
+  l.group = std::max(1, SHRINK_GROUP_ROWS / l.rb);
+  l.tiles_m = (a.M + BLOCK_M - 1) / BLOCK_M;
+  l.idesc_a = umma::make_idesc(BLOCK_M, l.rb, bf16);
+  CUtensorMap mx, ma;
+  if (int rc = make_map(&mx, a.X, bf16, a.K, a.M, a.ldx, 1, 0, BLOCK_M)) return rc;
+  if (int rc = make_map(&ma, a.A, bf16, a.K, a.r, a.lda, a.n_adapters, a.stride_a, l.rb)) return rc;
+  {
+    const int stage = A_STAGE_BYTES + l.group * l.rb * BLOCK_K * 2;
+    l.stages = std::min(MAX_STAGES, 220 * 1024 / stage);
+    static PerDeviceOnce attr_set;
+    XB_SET_MAX_SMEM_ONCE(attr_set, 226 * 1024, (const void*)lora_shrink_kernel);
+    launch_dependent(lora_shrink_kernel, (unsigned)std::min(l.tiles_m, sm_count()), SHRINK_THREADS, (size_t)l.stages * stage + 1024, stream, mx, ma, l);
+    if (int rc = check_launch("lora_shrink_kernel")) return rc;
+  }
+  UmmaGemmParams p;
+  memset(&p, 0, sizeof(p));
+  p.M = a.M; p.N = a.N; p.K = a.K; p.batch = 1; p.alpha = p.beta = 1.f;
+  p.bias = a.bias; p.bias_kind = a.bias ? XB_BIAS_ROW : XB_BIAS_NONE; p.bias_dtype = XB_F32; p.bias_group = 1;
+  p.Y = a.Y; p.ldy = a.ldy; p.y_dtype = a.y_dtype;
+  p.b_mn = !a.trans_w;
+  p.tiles_m = l.tiles_m;
+  // all of a product of up to 256 columns, equal shares of a wider one; narrower where the tiles would leave SMs idle
+  const int wide = (a.N + 255) / 256, least = a.trans_w ? 32 : 64;
+  const int64_t split = std::max<int64_t>(wide, std::min<int64_t>(sm_count() / std::max(p.tiles_m, 1), (a.N + least - 1) / least));
+  p.block_n = (int)((a.N + split - 1) / split + 15) / 16 * 16;
+  p.tiles_n = (a.N + p.block_n - 1) / p.block_n;
+  p.tmem_cols = 64;
+  while (p.tmem_cols < 2 * p.block_n) p.tmem_cols <<= 1;
+  p.idesc = umma::make_idesc(BLOCK_M, p.block_n, bf16) | (p.b_mn ? umma::IDESC_B_MN : 0u);
+  l.idesc_ext = umma::make_idesc(BLOCK_M, p.block_n, FMT_TF32);
+  const int64_t total = (int64_t)p.tiles_m * p.tiles_n;
+  XB_REQUIRE(total < ((int64_t)1 << 31), XB_ERR_LIMIT, "xb_lora_gemm: %lld output tiles are too many for one call", (long long)total);
+  p.n_fast = p.tiles_n > 1;               // the n tiles of a row of tiles run together and share its X
+  CUtensorMap m[5];
+  m[0] = mx;
+  if (int rc = p.b_mn ? make_map(&m[1], a.W, bf16, a.N, a.K, a.ldw, 1, 0, BLOCK_K) : make_map(&m[1], a.W, bf16, a.K, a.N, a.ldw, 1, 0, p.block_n)) return rc;
+  if (int rc = make_map_f32(&m[2], l.U, l.u_cols, a.M, 1, BLOCK_M)) return rc;
+  if (int rc = make_map_f32(&m[3], l.B32, l.b_cols, a.N, a.n_adapters, p.block_n)) return rc;
+  m[4] = m[0];
+  const int64_t es = a.y_dtype == XB_F32 ? 4 : 2;
+  int y = LORA_Y_ANY, tail = 4 * 256 * (int)sizeof(float) + EPI_WARPS * EPI_STAGE_BYTES;
+  p.y_unit = 16; p.y_bufs = 1;
+  if (es == 2 && (reinterpret_cast<uintptr_t>(a.Y) & 15) == 0 && a.ldy % 8 == 0 && a.N % 8 == 0) {
+    // copies of 32 columns, 16 where the tile has few or where 32 would reach into the next tile
+    p.y_unit = p.block_n >= 128 && (p.block_n % 32 == 0 || p.tiles_n == 1) ? 32 : 16;
+    p.y_bufs = p.block_n > 4 * p.y_unit ? 2 : 1;
+    if (make_map(&m[4], a.Y, a.y_dtype == XB_BF16, a.N, a.M, a.ldy, 1, 0, 32, p.y_unit,
+                 p.y_unit == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B) == 0) {
+      y = LORA_Y_TMA;
+      tail = 4 * 256 * (int)sizeof(float) + EPI_WARPS * p.y_bufs * p.y_unit * 64;
+    }
+  }
+  const int stage = A_STAGE_BYTES + (p.b_mn ? (p.block_n + 63) / 64 * 64 : p.block_n) * BLOCK_K * 2;
+  p.stages = std::max(2, std::min(MAX_STAGES, (SMEM_BUDGET - tail) / stage));
+  const size_t smem = (size_t)p.stages * stage + tail + 1024;
+  const unsigned grid = (unsigned)std::min<int64_t>(total, sm_count());
+  if (a.y_dtype == XB_F32) return launch_lora_gemm<float, false, LORA_Y_ANY>(m, p, l, grid, smem, stream);
+  auto half = [&](auto type) {
+    using T = decltype(type);
+    if (p.b_mn) return y == LORA_Y_TMA ? launch_lora_gemm<T, true, LORA_Y_TMA>(m, p, l, grid, smem, stream) : launch_lora_gemm<T, true, LORA_Y_ANY>(m, p, l, grid, smem, stream);
+    return y == LORA_Y_TMA ? launch_lora_gemm<T, false, LORA_Y_TMA>(m, p, l, grid, smem, stream) : launch_lora_gemm<T, false, LORA_Y_ANY>(m, p, l, grid, smem, stream);
+  };
+  return bf16 ? half(__nv_bfloat16()) : half(__half());
+}
+
+}  // namespace
+}  // namespace xb
