@@ -271,7 +271,7 @@ static int gemm_half(SimtGemmParams& p, const xb_gemm_args& a, cudaStream_t s) {
     return (int)((reinterpret_cast<uintptr_t>(ptr) & 3) == 0 && ld % 2 == 0 && stride % 2 == 0);
   };
   const int a_even = even(a.A, a.lda, a.stride_a), b_even = even(a.B, a.ldb, a.stride_b);
-  p.y_pairs = even(a.Y, a.ldy, a.stride_y);
+  p.y_pairs = a.y_dtype != XB_F32 && even(a.Y, a.ldy, a.stride_y);
   p.tiles_n = (a.N + HALF_BN - 1) / HALF_BN;
   const int64_t large = ((int64_t)a.M + 127) / 128 * p.tiles_n;
   const int bm = large * a.batch >= sm_count() ? 128 : 64;

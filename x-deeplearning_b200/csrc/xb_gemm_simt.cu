@@ -537,7 +537,7 @@ static void pick_simt_tile(int64_t M, int64_t N, int64_t batch, bool f32, int* t
   }
 }
 
-int gemm_simt(const xb_gemm_args& a, cudaStream_t stream) {
+static SimtGemmParams simt_params(const xb_gemm_args& a) {
   SimtGemmParams p;
   p.M = a.M; p.N = a.N; p.K = a.K; p.trans_a = a.trans_a; p.trans_b = a.trans_b;
   p.in_dtype = a.ab_dtype; p.y_dtype = a.y_dtype;
@@ -557,6 +557,18 @@ int gemm_simt(const xb_gemm_args& a, cudaStream_t stream) {
   p.a_vec = vec(a.A, a.lda, a.stride_a, a.trans_a ? a.M : a.K);
   p.b_vec = vec(a.B, a.ldb, a.stride_b, a.trans_b ? a.K : a.N);
   p.y_pairs = a.y_dtype == XB_F32 && (reinterpret_cast<uintptr_t>(a.Y) & 7) == 0 && a.ldy % 2 == 0 && a.stride_y % 2 == 0;
+  return p;
+}
+
+// 16-bit operands of any alignment through gemm_half_kernel, results of any type (for callers inside the library: what xb_gemm gives for
+// fp32 results keeps the order of its sums)
+int gemm_half_sums(const xb_gemm_args& a, cudaStream_t stream) {
+  SimtGemmParams p = simt_params(a);
+  return gemm_half(p, a, stream);
+}
+
+int gemm_simt(const xb_gemm_args& a, cudaStream_t stream) {
+  SimtGemmParams p = simt_params(a);
   int tm = 8, tn = 8;
   const bool f32 = a.ab_dtype == XB_F32 && !a.trans_a && !a.trans_b;
   pick_simt_tile(a.M, a.N, a.batch, f32, &tm, &tn);

@@ -6,6 +6,9 @@
 #include "xb_lora_umma.cuh"
 
 namespace xb {
+
+int gemm_half_sums(const xb_gemm_args& a, cudaStream_t stream);
+
 namespace {
 
 constexpr int LORA_MAX_RANK = 128;
@@ -28,43 +31,112 @@ __device__ __forceinline__ int adapter_of(const LoraParams& p, int m) {
   return a >= 0 && a < p.n_adapters ? a : -1;
 }
 
-// A warp a row: its products with the r rows of its adapter, the lanes along K.
-template <typename T>
-__global__ void __launch_bounds__(256) lora_rows_shrink_kernel(const LoraParams p) {
+// V adjacent elements as fp32: one load where they lie aligned, which V > 1 says
+template <typename T, int V>
+__device__ __forceinline__ void load_piece(const T* p, float (&v)[V]) {
+  if constexpr (V == 1) {
+    v[0] = to_f32<T>(p[0]);
+  } else {
+    static_assert(V * sizeof(T) == 16, "");
+    const uint4 t = __ldg(reinterpret_cast<const uint4*>(p));
+    const T* e = reinterpret_cast<const T*>(&t);
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = to_f32<T>(e[i]);
+  }
+}
+
+// A warp takes four products of one row with the rows of its adapter's A, the lanes along K. Bound by the latency of the few rounds over K
+// where there are few rows, by A from L2 otherwise. 64 rows of 1280, rank 16: 79 us with a warp for all of a row's products, 4 now;
+// 5003 of 250, rank 12, rows that start anywhere: 20, 5.
+constexpr int SHRINK_J = 4;
+template <typename T, int V>
+__global__ void __launch_bounds__(128) lora_rows_shrink_kernel(const LoraParams p) {
   pdl_begin();
-  const int m = blockIdx.x * 8 + threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int parts = (p.r + SHRINK_J - 1) / SHRINK_J, lane = threadIdx.x % 32;
+  const int64_t w = (int64_t)blockIdx.x * 4 + threadIdx.x / 32;
+  const int m = (int)(w / parts), j0 = (int)(w - (int64_t)m * parts) * SHRINK_J;
   if (m >= p.M) return;
   const int a = adapter_of(p, m);
   if (a < 0) return;
   const T* x = reinterpret_cast<const T*>(p.X) + (int64_t)m * p.ldx;
-  const float scale = p.scale ? p.scale[a] : 1.f;
-  for (int j = 0; j < p.r; ++j) {
-    const T* w = reinterpret_cast<const T*>(p.A) + (int64_t)a * p.stride_a + (int64_t)j * p.lda;
-    float s = 0.f;
-    for (int k = lane; k < p.K; k += 32) s = fmaf(to_f32<T>(x[k]), to_f32<T>(w[k]), s);
+  const T* at = reinterpret_cast<const T*>(p.A) + (int64_t)a * p.stride_a + (int64_t)j0 * p.lda;
+  float s[SHRINK_J] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int k = lane * V; k < p.K; k += 32 * V) {         // (V > 1: whole pieces, K is a multiple of V)
+    float xv[V];
+    load_piece<T, V>(x + k, xv);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (lane == 0) p.U[(int64_t)m * p.r + j] = s * scale;
+    for (int j = 0; j < SHRINK_J; ++j) {
+      if (j0 + j >= p.r) break;
+      float av[V];
+      load_piece<T, V>(at + (int64_t)j * p.lda + k, av);
+#pragma unroll
+      for (int v = 0; v < V; ++v) s[j] = fmaf(xv[v], av[v], s[j]);
+    }
+  }
+  const float scale = p.scale ? p.scale[a] : 1.f;
+#pragma unroll
+  for (int j = 0; j < SHRINK_J; ++j) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s[j] += __shfl_xor_sync(0xffffffffu, s[j], o);
+    if (lane == 0 && j0 + j < p.r) p.U[(int64_t)m * p.r + j0 + j] = s[j] * scale;
   }
 }
 
-// A block a row, a thread an output at a time.
-template <typename T>
+// A thread has one column of ROWS adjacent rows, whose B it keeps while they have the same adapter; 16 of the rank at a time.
+constexpr int EXPAND_J = 16;
+template <typename T, bool VEC, int ROWS>
 __global__ void __launch_bounds__(128) lora_rows_expand_kernel(const LoraParams p) {
   pdl_begin();
-  const int m = blockIdx.x;
-  const int a = adapter_of(p, m);
-  const bool with = a >= 0;
-  for (int n = threadIdx.x; n < p.N; n += 128) {
-    float s = p.bias ? p.bias[n] : 0.f;
-    if (with) {
-      const T* w = reinterpret_cast<const T*>(p.B) + (int64_t)a * p.stride_b + (int64_t)n * p.ldb;
-      float d = 0.f;
-      for (int j = 0; j < p.r; ++j) d = fmaf(p.U[(int64_t)m * p.r + j], to_f32<T>(w[j]), d);
-      s += d;
-    }
-    p.part[(int64_t)m * p.N + n] = s;
+  __shared__ float s_u[ROWS][LORA_MAX_RANK];
+  __shared__ int s_a[ROWS];
+  const int m0 = blockIdx.x * ROWS, n = blockIdx.y * 128 + threadIdx.x;
+  if (threadIdx.x < ROWS) s_a[threadIdx.x] = m0 + (int)threadIdx.x < p.M ? adapter_of(p, m0 + threadIdx.x) : -1;
+  __syncthreads();
+  for (int i = threadIdx.x; i < ROWS * p.r; i += 128) {
+    const int m = i / p.r, j = i - m * p.r;
+    s_u[m][j] = s_a[m] >= 0 ? p.U[(int64_t)(m0 + m) * p.r + j] : 0.f;
   }
+  __syncthreads();
+  if (n >= p.N) return;
+  float sum[ROWS];
+#pragma unroll
+  for (int m = 0; m < ROWS; ++m) sum[m] = 0.f;
+  for (int j0 = 0; j0 < p.r; j0 += EXPAND_J) {
+    float b[EXPAND_J];
+    int held = -1;
+#pragma unroll
+    for (int m = 0; m < ROWS; ++m) {
+      const int a = s_a[m];
+      if (a < 0) continue;
+      if (a != held) {
+        held = a;
+        const T* at = reinterpret_cast<const T*>(p.B) + (int64_t)a * p.stride_b + (int64_t)n * p.ldb + j0;
+        if constexpr (VEC) {
+          constexpr int V = 16 / sizeof(T);
+#pragma unroll
+          for (int i = 0; i < EXPAND_J / V; ++i) {
+            float t[V];
+#pragma unroll
+            for (int v = 0; v < V; ++v) t[v] = 0.f;
+            if (j0 + i * V < p.r) load_piece<T, V>(at + i * V, t);
+#pragma unroll
+            for (int v = 0; v < V; ++v) b[i * V + v] = t[v];
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < EXPAND_J; ++j) b[j] = j0 + j < p.r ? to_f32<T>(at[j]) : 0.f;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < EXPAND_J; ++j)
+        if (j0 + j < p.r) sum[m] = fmaf(s_u[m][j0 + j], b[j], sum[m]);
+    }
+  }
+  const float bias = p.bias ? p.bias[n] : 0.f;
+#pragma unroll
+  for (int m = 0; m < ROWS; ++m)
+    if (m0 + m < p.M) p.part[(int64_t)(m0 + m) * p.N + n] = bias + sum[m];
 }
 
 // Few rows: the tiles would leave most SMs idle, and a tile of many adapters walks through all of them.
@@ -96,6 +168,23 @@ int check_args(const xb_lora_args* a) {
 }
 
 template <typename T>
+int launch_expand(const LoraParams& p, bool vec, cudaStream_t s) {
+  // eight rows a block share what they read of B; two where that would leave SMs idle
+  const unsigned cols = (unsigned)((p.N + 127) / 128);
+  XB_REQUIRE(cols <= 65535, XB_ERR_LIMIT, "xb_lora_gemm: %d columns are too many for this path", p.N);
+  const bool few = (int64_t)((p.M + 7) / 8) * cols < 4 * sm_count();
+  const dim3 grid((unsigned)(few ? (p.M + 1) / 2 : (p.M + 7) / 8), cols);
+  if (few) {
+    if (vec) launch_dependent(lora_rows_expand_kernel<T, true, 2>, grid, 128, 0, s, p);
+    else launch_dependent(lora_rows_expand_kernel<T, false, 2>, grid, 128, 0, s, p);
+  } else {
+    if (vec) launch_dependent(lora_rows_expand_kernel<T, true, 8>, grid, 128, 0, s, p);
+    else launch_dependent(lora_rows_expand_kernel<T, false, 8>, grid, 128, 0, s, p);
+  }
+  return check_launch("lora_rows_expand_kernel");
+}
+
+template <typename T>
 int run_rows(const xb_lora_args& a, uint8_t* ws, cudaStream_t s) {
   const int turn = turn_rows(a);
   LoraParams p;
@@ -104,6 +193,11 @@ int run_rows(const xb_lora_args& a, uint8_t* ws, cudaStream_t s) {
   p.scale = a.scale; p.bias = a.bias; p.ldx = a.ldx;
   p.U = reinterpret_cast<float*>(ws);
   p.part = reinterpret_cast<float*>(ws + align256((size_t)turn * a.r * 4));
+  // 16-byte pieces of X and A along K, and of B along the rank
+  constexpr int V = 16 / (int)sizeof(T);
+  const bool vec_k = a.K % V == 0 && a.ldx % V == 0 && a.lda % V == 0 && a.stride_a % V == 0 &&
+                     ((reinterpret_cast<uintptr_t>(a.X) | reinterpret_cast<uintptr_t>(a.A)) & 15) == 0;
+  const bool vec_r = a.r % V == 0 && a.ldb % V == 0 && a.stride_b % V == 0 && (reinterpret_cast<uintptr_t>(a.B) & 15) == 0;
   xb_gemm_args g;
   memset(&g, 0, sizeof(g));
   g.N = a.N; g.K = a.K; g.trans_b = a.trans_w; g.alpha = g.beta = 1.f; g.batch = 1;
@@ -114,15 +208,20 @@ int run_rows(const xb_lora_args& a, uint8_t* ws, cudaStream_t s) {
     p.X = reinterpret_cast<const T*>(a.X) + m0 * a.ldx;
     p.adapter = p.n_adapters ? a.adapter + m0 : nullptr;
     if (p.n_adapters) {
-      launch_dependent(lora_rows_shrink_kernel<T>, (unsigned)((p.M + 7) / 8), 256, 0, s, p);
+      const int64_t warps = (int64_t)p.M * ((p.r + SHRINK_J - 1) / SHRINK_J);
+      XB_REQUIRE(warps < ((int64_t)1 << 32), XB_ERR_LIMIT, "xb_lora_gemm: %d rows of rank %d are too many for one call", p.M, p.r);
+      if (vec_k) launch_dependent(lora_rows_shrink_kernel<T, 16 / (int)sizeof(T)>, (unsigned)((warps + 3) / 4), 128, 0, s, p);
+      else launch_dependent(lora_rows_shrink_kernel<T, 1>, (unsigned)((warps + 3) / 4), 128, 0, s, p);
       if (int rc = check_launch("lora_rows_shrink_kernel")) return rc;
     }
-    launch_dependent(lora_rows_expand_kernel<T>, (unsigned)p.M, 128, 0, s, p);
-    if (int rc = check_launch("lora_rows_expand_kernel")) return rc;
+    if (int rc = launch_expand<T>(p, vec_r, s)) return rc;
     g.M = p.M;
     g.A = p.X;
     g.Y = reinterpret_cast<uint8_t*>(a.Y) + m0 * a.ldy * (int64_t)dtype_size(a.y_dtype);
-    if (int rc = xb_gemm(&g, s)) return rc;
+    // (fp32 results of rows that TMA cannot address: matrix instructions here, where xb_gemm stays with the CUDA cores for the sake of its bits.
+    // [5003, 250] x [250, 131] bf16: 127 us there)
+    const bool half = a.dtype != XB_F32 && a.y_dtype == XB_F32 && !xb_gemm_uses_tcgen05(&g);
+    if (int rc = half ? gemm_half_sums(g, s) : xb_gemm(&g, s)) return rc;
   }
   return 0;
 }
