@@ -12,7 +12,7 @@ import pkg
 def bound(monkeypatch):
     pkg.load()
     from x_deeplearning_b200 import capi, ops
-    m, seen, need, result = capi.binding(), [], [0], [0]
+    m, seen, need, result = capi.tensors(), [], [0], [0]
 
     def taken(kind):
         def f(a, *rest):
@@ -27,8 +27,7 @@ def bound(monkeypatch):
     real = {n: C.cast(getattr(capi.lib(), n), C.c_void_p).value for n in fs}
     for n, f in fs.items():
         m.bind(n, C.cast(f, C.c_void_p).value)
-    monkeypatch.setattr(ops, "raw_stream", lambda: 77)
-    monkeypatch.setattr(torch.cuda, "current_device", lambda: -1)          # what get_device() says of a CPU tensor
+    monkeypatch.setattr(ops, "_where", lambda: (-1, 77))                    # a CPU tensor's device is -1
     yield ops, capi, seen, need, result
     for n, a in real.items():
         m.bind(n, a)
@@ -125,7 +124,7 @@ def test_lora(bound):
 
 def test_tensors_of_another_device(bound, monkeypatch):
     ops, capi, seen, _, _ = bound
-    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(ops, "_where", lambda: (0, 77))
     with pytest.raises(capi.XbError, match="on device -1"):
         ops.ssm_conv(torch.zeros(4, 8), torch.zeros(8, 4))
     assert not seen

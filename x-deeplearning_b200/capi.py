@@ -203,6 +203,21 @@ def lib():
     return _lib
 
 
+def _extension(name, functions):
+    """The extension module `name` (host/binding/), its calls bound to this process's kernel library."""
+    L = lib()
+    path = os.path.join(HERE, "lib", name + ".so")
+    if not os.path.exists(path):
+        raise RuntimeError("%s is missing: build it first (there is no fallback)" % path)
+    loader = importlib.machinery.ExtensionFileLoader(name, path)
+    spec = importlib.util.spec_from_file_location(name, path, loader=loader)
+    m = importlib.util.module_from_spec(spec)
+    loader.exec_module(m)
+    for f in functions:
+        m.bind(f, C.cast(getattr(L, f), C.c_void_p).value)
+    return m
+
+
 _binding = None
 
 
@@ -210,19 +225,20 @@ def binding():
     """The extension module with the hot calls (host/binding/xb_binding.cc), bound to this process's kernel library."""
     global _binding
     if _binding is None:
-        L = lib()
-        path = os.path.join(HERE, "lib", "xb_binding.so")
-        if not os.path.exists(path):
-            raise RuntimeError("%s is missing: build it first (there is no fallback)" % path)
-        loader = importlib.machinery.ExtensionFileLoader("xb_binding", path)
-        spec = importlib.util.spec_from_file_location("xb_binding", path, loader=loader)
-        m = importlib.util.module_from_spec(spec)
-        loader.exec_module(m)
-        for name in ("xb_gemm", "xb_embedding_pool", "xb_ssm_conv", "xb_ssm_scan_workspace_bytes", "xb_ssm_scan", "xb_lora_workspace_bytes",
-                     "xb_lora_gemm"):
-            m.bind(name, C.cast(getattr(L, name), C.c_void_p).value)
-        _binding = m
+        _binding = _extension("xb_binding", ("xb_gemm", "xb_embedding_pool"))
     return _binding
+
+
+_tensors = None
+
+
+def tensors():
+    """The extension module whose calls check torch's tensors themselves (host/binding/xb_tensors.cc)."""
+    global _tensors
+    if _tensors is None:
+        import torch  # noqa: F401  (its libraries come first)
+        _tensors = _extension("xb_tensors", ("xb_ssm_conv", "xb_ssm_scan_workspace_bytes", "xb_ssm_scan", "xb_lora_workspace_bytes", "xb_lora_gemm"))
+    return _tensors
 
 
 class XbError(RuntimeError):

@@ -274,21 +274,26 @@ _checked = None
 
 
 def _calls():
-    """The extension module's calls that check their tensors themselves."""
     global _checked
-    if _checked is None:
-        m = binding()
-        m.dtypes(_DT)
-        m.scratch(lambda like, n: like.new_empty((n,), dtype=torch.uint8))
-        _checked = m
+    _checked = capi.tensors()
     return _checked
 
 
-def _done(rc):
-    """0, the C function's refusal, or the text of a tensor's"""
-    if rc.__class__ is str:
-        raise capi.XbError(rc)
-    check(rc)
+def _done(r):
+    """The call's tensor; the C function's refusal or the text of a tensor's becomes an XbError."""
+    if r.__class__ is str:
+        raise capi.XbError(r)
+    if r.__class__ is int:
+        check(r)
+    return r
+
+
+def _where():
+    """The current device and its current stream"""
+    if _raw_device is None or not torch.cuda.is_initialized():
+        return torch.cuda.current_device(), raw_stream()
+    d = _raw_device()
+    return d, _raw_stream(d)
 
 
 def ssm_conv(x, w, bias=None, offsets=None, T=None, state_in=None, state_out=None, slots=None, silu=True, out=None):
@@ -297,11 +302,7 @@ def ssm_conv(x, w, bias=None, offsets=None, T=None, state_in=None, state_out=Non
     w [D, K], bias [D]. Lists: `offsets` int32 [lists + 1], or of T rows each (T = 1: one new row a list; None: one list).
     state_in / state_out [slots, K - 1, D]: the inputs before each list and the last ones of it, in row slots[i] for list i (its own
     number without `slots`); they may be one array. Returns [rows, D]; rows behind the last list are not written."""
-    m = _checked or _calls()
-    if out is None:
-        out = x.new_empty(x.shape)
-    _done(m.ssm_conv(x, w, bias, offsets, T, state_in, state_out, slots, silu, out, torch.cuda.current_device(), raw_stream()))
-    return out
+    return _done((_checked or _calls()).ssm_conv(x, w, bias, offsets, T, state_in, state_out, slots, silu, out, *_where()))
 
 
 def ssm_scan(x, delta, A, B, C, D=None, z=None, delta_bias=None, groups=1, softplus=True, offsets=None, T=None, longest=0, h_in=None,
@@ -311,12 +312,8 @@ def ssm_scan(x, delta, A, B, C, D=None, z=None, delta_bias=None, groups=1, softp
     delta, z as x; B, C [rows, groups * N]; A [channels, N], D and delta_bias [channels], h_in / h_out [slots, channels, N] fp32.
     Lists and slots as in ssm_conv; `longest`: rows of the longest list where the caller knows it (the plan goes by it, no result).
     `workspace`: uint8 scratch for callers that keep one; by default the call takes its own."""
-    m = _checked or _calls()
-    if out is None:
-        out = x.new_empty(x.shape)
-    _done(m.ssm_scan(x, delta, A, B, C, D, z, delta_bias, groups, softplus, offsets, T, longest, h_in, h_out, slots, out, workspace,
-                     torch.cuda.current_device(), raw_stream()))
-    return out
+    return _done((_checked or _calls()).ssm_scan(x, delta, A, B, C, D, z, delta_bias, groups, softplus, offsets, T, longest, h_in, h_out, slots,
+                                                 out, workspace, *_where()))
 
 
 def lora_gemm(X, W, A, B, adapter, bias=None, scale=None, trans_b=False, out_dtype=None, Y=None, workspace=None):
@@ -324,8 +321,4 @@ def lora_gemm(X, W, A, B, adapter, bias=None, scale=None, trans_b=False, out_dty
 
     X [M, K]; W [K, N], or [N, K] with trans_b; A [adapters, r, K]; B [adapters, N, r]; adapter int32 [M], outside [0, adapters) for a
     row without one; bias [N] and scale [adapters] fp32. Results in X's type or fp32."""
-    m = _checked or _calls()
-    if Y is None:
-        Y = X.new_empty((X.shape[0], W.shape[0 if trans_b else 1]), dtype=out_dtype)
-    _done(m.lora_gemm(X, W, A, B, adapter, bias, scale, trans_b, Y, workspace, torch.cuda.current_device(), raw_stream()))
-    return Y
+    return _done((_checked or _calls()).lora_gemm(X, W, A, B, adapter, bias, scale, trans_b, Y, out_dtype, workspace, *_where()))
