@@ -9,6 +9,7 @@
 namespace xb {
 namespace {
 
+constexpr int CONV_THREADS = 128, CONV_AHEAD = 8;
 struct ConvParams {
   const void* x; int64_t ldx;
   void* y; int64_t ldy;
@@ -20,12 +21,13 @@ struct ConvParams {
 };
 
 // A thread walks `rows_a_chunk` rows of V channels with the last K - 1 inputs in registers; the threads of a chunk lie side by side, and
-// chunks follow one another without a gap, so no lane idles whatever D is. Bound by memory: x is read 1 + (K - 1) / rows_a_chunk times.
+// chunks follow one another without a gap, so no lane idles whatever D is. x is read 1 + (K - 1) / rows_a_chunk times.
 // The thread that has a list's first row makes its first K - 1 rows (they read the state) and its last state, so that states moved
 // on in place are read and written by one thread.
-constexpr int CONV_THREADS = 128, CONV_AHEAD = 4;
+// Pieces of 8 bytes and eight rows ahead: with 16-byte pieces and four rows the registers let half as many warps in, which is what
+// the loads in flight are. SiLU is the rest: two exponentials and a quotient for two values.
 template <typename T, int V, int K>
-__global__ void __launch_bounds__(CONV_THREADS) ssm_conv_kernel(const ConvParams p) {
+__global__ void __launch_bounds__(CONV_THREADS, K <= 4 && V * sizeof(T) <= 8 ? 6 : 4) ssm_conv_kernel(const ConvParams p) {
   pdl_begin();
   __shared__ int s_first[CONV_THREADS];                // the first list that begins in or behind each of the block's chunks
   const int lane = threadIdx.x & 31;
@@ -44,39 +46,51 @@ __global__ void __launch_bounds__(CONV_THREADS) ssm_conv_kernel(const ConvParams
   const int64_t r0 = chunk * p.rows_a_chunk, r1 = r0 + p.rows_a_chunk;
   const T *px = static_cast<const T*>(p.x) + c, *pw = static_cast<const T*>(p.w) + (int64_t)c * K, *pb = static_cast<const T*>(p.bias) + c;
   T* py = static_cast<T*>(p.y) + c;
-  float w[V][K], bias[V], past[K - 1][V];
+  constexpr int P = (V + 1) / 2;                       // pairs of channels
+  constexpr int CONV_FEW = V == 1 ? CONV_AHEAD : 4;
+  f32x2 w[K][P], bias[P], past[K - 1][P];
+  auto pairs = [](const Raw<T, V>& t, f32x2 (&to)[P]) {
+#pragma unroll
+    for (int q = 0; q < P; ++q) to[q] = pack2(t.get(2 * q), 2 * q + 1 < V ? t.get((2 * q + 1) % V) : 0.f);
+  };
   {
     Raw<T, V> t[K];
 #pragma unroll
     for (int j = 0; j < K; ++j) t[j].load(pw + j * V, in * K - j * V, p.vec_w);
+    auto weight = [&](int e) { return e < V * K ? t[e / V % K].get(e % V) : 0.f; };      // element e of the V channels' K taps
 #pragma unroll
-    for (int e = 0; e < V * K; ++e) w[e / K][e % K] = t[e / V].get(e % V);
+    for (int j = 0; j < K; ++j)
+#pragma unroll
+      for (int q = 0; q < P; ++q) w[j][q] = pack2(weight(2 * q * K + j), weight((2 * q + 1) * K + j));
+    t[0].zero();
     if (p.bias) t[0].load(pb, in, p.vec_w);
-#pragma unroll
-    for (int v = 0; v < V; ++v) bias[v] = p.bias ? t[0].get(v) : 0.f;
+    pairs(t[0], bias);
   }
-  auto row_of = [&](const Raw<T, V>& t, int64_t r) {
-    float o[V];
+  auto row_of = [&](const Raw<T, V>& t, Raw<T, V>& out) {
+    f32x2 x[P], o[P];
+    pairs(t, x);
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const float x = t.get(v);
-      float s = bias[v];
+    for (int q = 0; q < P; ++q) {
+      f32x2 s = bias[q];
 #pragma unroll
-      for (int j = 0; j < K - 1; ++j) s = fmaf(w[v][j], past[j][v], s);
-      s = fmaf(w[v][K - 1], x, s);
+      for (int j = 0; j < K - 1; ++j) s = fma2(w[j][q], past[j][q], s);
+      o[q] = fma2(w[K - 1][q], x[q], s);
 #pragma unroll
-      for (int j = 0; j + 1 < K - 1; ++j) past[j][v] = past[j + 1][v];
-      past[K - 2][v] = x;
-      o[v] = s;
+      for (int j = 0; j + 1 < K - 1; ++j) past[j][q] = past[j + 1][q];
+      past[K - 2][q] = x[q];
     }
     if (p.silu) {
 #pragma unroll
-      for (int v = 0; v < V; ++v) o[v] = silu(o[v]);
+      for (int q = 0; q < P; ++q) o[q] = silu2(o[q]);
     }
-    Raw<T, V> out;
-    out.put_all(o);
-    out.store(py + r * p.ldy, in, p.vec);
+    float v[2 * P], first[V];
+#pragma unroll
+    for (int q = 0; q < P; ++q) unpack2(o[q], v[2 * q], v[2 * q + 1]);
+#pragma unroll
+    for (int i = 0; i < V; ++i) first[i] = v[i];
+    out.put_all(first);
   };
+  const bool whole_piece = Raw<T, V>::PIECE && p.vec && in == V;
   int nxt = s_first[(int)(chunk - c_first)];
   int64_t r = r0, stop = r0;
   if (nxt > 0 && p.lists.begin(nxt) > r0) {            // a list from before: its rows from the K-th on
@@ -88,24 +102,38 @@ __global__ void __launch_bounds__(CONV_THREADS) ssm_conv_kernel(const ConvParams
       for (int j = 0; j < K - 1; ++j) {
         Raw<T, V> t;
         t.load(px + (r - (K - 1) + j) * p.ldx, in, p.vec);
-#pragma unroll
-        for (int v = 0; v < V; ++v) past[j][v] = t.get(v);
+        pairs(t, past[j]);
       }
     }
   }
   for (;;) {
-    for (; r + CONV_AHEAD <= stop; r += CONV_AHEAD) {
-      Raw<T, V> t[CONV_AHEAD];
+    const T* from = px + r * p.ldx;
+    T* to = py + r * p.ldy;
+    if (whole_piece) {
+      for (; r + CONV_AHEAD <= stop; r += CONV_AHEAD, from += CONV_AHEAD * p.ldx, to += CONV_AHEAD * p.ldy) {
+        Raw<T, V> t[CONV_AHEAD];
 #pragma unroll
-      for (int i = 0; i < CONV_AHEAD; ++i) t[i].load(px + (r + i) * p.ldx, in, p.vec);
+        for (int i = 0; i < CONV_AHEAD; ++i) t[i].load_piece(from + i * p.ldx);
 #pragma unroll
-      for (int i = 0; i < CONV_AHEAD; ++i) row_of(t[i], r + i);
+        for (int i = 0; i < CONV_AHEAD; ++i) {
+          Raw<T, V> out;
+          row_of(t[i], out);
+          out.store_piece(to + i * p.ldy);
+        }
+      }
     }
-    for (; r < stop; ++r) {
-      Raw<T, V> t;
-      t.load(px + r * p.ldx, in, p.vec);
-      row_of(t, r);
+    for (; r < stop; r += CONV_FEW, from += CONV_FEW * p.ldx, to += CONV_FEW * p.ldy) {
+      Raw<T, V> t[CONV_FEW], out;
+#pragma unroll
+      for (int i = 0; i < CONV_FEW; ++i) t[i].load(from + i * p.ldx, r + i < stop ? in : 0, p.vec);
+#pragma unroll
+      for (int i = 0; i < CONV_FEW; ++i) {
+        if (r + i >= stop) break;
+        row_of(t[i], out);
+        out.store(to + i * p.ldy, in, p.vec);
+      }
     }
+    r = stop;
     if (nxt >= p.lists.batch) return;
     const int64_t b = p.lists.begin(nxt), e = max(b, p.lists.begin(nxt + 1));
     if (b >= r1 && !last_chunk) return;
@@ -116,8 +144,7 @@ __global__ void __launch_bounds__(CONV_THREADS) ssm_conv_kernel(const ConvParams
       Raw<T, V> t;
       t.zero();
       if (p.state_in && slot >= 0) t.load(static_cast<const T*>(p.state_in) + state + (int64_t)j * p.D, in, p.vec_state);
-#pragma unroll
-      for (int v = 0; v < V; ++v) past[j][v] = t.get(v);
+      pairs(t, past[j]);
     }
     if (p.state_out && slot >= 0) {
 #pragma unroll
@@ -128,11 +155,14 @@ __global__ void __launch_bounds__(CONV_THREADS) ssm_conv_kernel(const ConvParams
           t.load(px + (b + place) * p.ldx, in, p.vec);
         } else {
 #pragma unroll
-          for (int v = 0; v < V; ++v) {
-            float was = 0.f;
+          for (int q = 0; q < P; ++q) {
+            f32x2 was = 0;
 #pragma unroll
-            for (int k = 0; k < K - 1; ++k) was = k == (int)place + K - 1 ? past[k][v] : was;
-            t.put(v, was);
+            for (int k = 0; k < K - 1; ++k) was = k == (int)place + K - 1 ? past[k][q] : was;
+            float lo, hi;
+            unpack2(was, lo, hi);
+            t.put(2 * q, lo);
+            if (2 * q + 1 < V) t.put((2 * q + 1) % V, hi);
           }
         }
         t.store(static_cast<T*>(p.state_out) + state + (int64_t)j * p.D, in, p.vec_state);
@@ -167,6 +197,7 @@ int launch_conv_taps(const ConvParams& p, cudaStream_t s) {
 template <typename T, int V>
 int launch_conv_pieces(ConvParams p, int K, cudaStream_t s) {
   p.pieces = (p.D + V - 1) / V;
+  if (V == 1) p.vec = p.vec_w = p.vec_state = 1;       // (pieces of one element lie aligned)
   // Longer walks read less twice, shorter ones keep more threads in flight. Single rows: nothing is read twice.
   const int64_t threads = p.lists.rows * p.pieces, fill = (int64_t)sm_count() * 1024;
   p.rows_a_chunk = (int)std::min<int64_t>(std::max<int64_t>(threads / fill, 1), !p.lists.offsets && p.lists.per <= 1 ? 1 : 32);
@@ -189,11 +220,12 @@ int launch_conv(const xb_ssm_conv_args& a, cudaStream_t s) {
   p.x = a.x; p.ldx = a.ldx; p.y = a.y; p.ldy = a.ldy; p.w = a.w; p.bias = a.bias; p.state_in = a.state_in; p.state_out = a.state_out;
   p.lists = lists_of(a.offsets, a.slots, a.rows, a.batch, a.n_slots);
   p.D = a.D; p.silu = a.silu;
-  p.vec = whole(a.x, a.ldx * SIZE, 16) && whole(a.y, a.ldy * SIZE, 16);
-  p.vec_w = whole(a.w, 0, 16) && whole(a.bias, 0, 16);
-  p.vec_state = whole(a.state_in, (int64_t)a.D * SIZE, 16) && whole(a.state_out, 0, 16);
-  // rows that do not start on 16 bytes: a channel a thread, adjacent lanes adjacent channels
-  return p.vec ? launch_conv_pieces<T, 16 / SIZE>(p, a.K, s) : launch_conv_pieces<T, 1>(p, a.K, s);
+  constexpr int unit = 4 * SIZE;
+  p.vec = whole(a.x, a.ldx * SIZE, unit) && whole(a.y, a.ldy * SIZE, unit);
+  p.vec_w = whole(a.w, 0, unit) && whole(a.bias, 0, unit);
+  p.vec_state = whole(a.state_in, (int64_t)a.D * SIZE, unit) && whole(a.state_out, 0, unit);
+  // rows that do not start on whole pieces: a channel a thread, adjacent lanes adjacent channels
+  return p.vec ? launch_conv_pieces<T, 4>(p, a.K, s) : launch_conv_pieces<T, 1>(p, a.K, s);
 }
 
 int scan_blocks(const xb_ssm_scan_args& a, int lanes, int K) {

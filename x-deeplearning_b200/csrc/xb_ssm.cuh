@@ -91,6 +91,12 @@ __device__ __forceinline__ float ex2(float v) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
 }
+// 1 / v, right to 1 unit in the last place; 0 for numbers of 2^126 and more
+__device__ __forceinline__ float rcp(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
 // two fp32 operations an instruction
 typedef unsigned long long f32x2;
 __device__ __forceinline__ f32x2 pack2(float lo, float hi) {
@@ -109,13 +115,28 @@ __device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 constexpr float LOG2E = 1.4426950408889634f;
-__device__ __forceinline__ float silu(float v) { return __fdividef(v, 1.f + ex2(-LOG2E * v)); }
+__device__ __forceinline__ float silu(float v) { return v * rcp(1.f + ex2(-LOG2E * v)); }
+// two of them with one reciprocal: 1 / a = b / (a b). exp is cut at 2^60, so that the product of two is finite: below -41.6 the result is
+// v 2^-60 instead of v exp(v), both less than 1e-16 of what the sums before it are rounded by.
+__device__ __forceinline__ f32x2 silu2(f32x2 v) {
+  float e0, e1;
+  unpack2(mul2(v, pack2(-LOG2E, -LOG2E)), e0, e1);
+  e0 = 1.f + ex2(fminf(e0, 60.f));
+  e1 = 1.f + ex2(fminf(e1, 60.f));
+  const float both = rcp(e0 * e1);
+  return mul2(v, mul2(pack2(e1, e0), pack2(both, both)));
+}
 // log(1 + exp(v)) = max(v, 0) + log1p(u), u = exp(-|v|), and log1p(u) = 2 atanh(s) with s = u / (2 + u) <= 1/3 by the series of atanh, cut
 // after s^13 (the next term is 1.4e-8 of the sum at most): right in relative terms where u is small too, which log(1 + u) is not.
 __device__ __forceinline__ float softplus(float v) {
   const float u = ex2(-LOG2E * fabsf(v));
-  const float s = __fdividef(u, 2.f + u), t = s * s;
+  const float s = u * rcp(2.f + u), t = s * s;
   float p = fmaf(t, 1.f / 13, 1.f / 11);
   p = fmaf(t, p, 1.f / 9);
   p = fmaf(t, p, 1.f / 7);
