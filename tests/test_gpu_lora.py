@@ -60,7 +60,8 @@ def _check(s, dtype, out, trans, **more):
     (300, 324, 200, 4, 8, True, 4), (1000, 64, 256, 7, 16, True, 0), (513, 128, 48, 2, 64, False, 0), (260, 88, 176, 3, 32, True, 8),
     (130, 16, 8, 200, 3, True, 0), (256, 200, 80, 1, 100, True, 0), (700, 512, 304, 6, 24, True, 0), (600, 72, 40, 3, 100, False, 0),
     (1111, 324, 200, 12, 8, True, 4), (2000, 640, 520, 40, 16, True, 0), (513, 1280, 1024, 3, 128, True, 0), (900, 24, 1000, 5, 33, False, 0),
-    (640, 136, 17, 9, 20, True, 0)])
+    (640, 136, 17, 9, 20, True, 0), (9600, 72, 200, 12, 8, True, 0), (10001, 136, 24, 40, 16, False, 0), (9473, 24, 190, 3, 64, True, 0),
+    (12000, 200, 240, 2, 5, True, 0), (9999, 72, 81, 6, 30, True, 0), (20000, 16, 232, 1, 16, False, 0)])
 def test_lora(dtype, out, how, M, K, N, n, r, trans, pad):
     rng = np.random.default_rng(M + K + N)
     _check(_case(rng, M, K, N, n, r, dtype, trans, pad, how), dtype, out, trans)

@@ -378,7 +378,8 @@ EncodeTiledFn encode_fn() {
 // [batch, rows, K] tensor of 2-byte elements, box {box_cols, box_rows, box_batch}, swizzled over the box's row (an N-major B is the same with
 // its k rows as rows and its columns as the inner extent; so is Y)
 int make_map(CUtensorMap* map, const void* base, int is_bf16, int64_t K, int64_t rows, int64_t ld, int64_t batch,
-             int64_t batch_stride, int box_rows, int box_cols = BLOCK_K, CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B, int box_batch = 1) {
+             int64_t batch_stride, int box_rows, int box_cols = BLOCK_K, CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B, int box_batch = 1,
+             CUtensorMapL2promotion promotion = CU_TENSOR_MAP_L2_PROMOTION_L2_128B) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return fail(XB_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
   cuuint64_t dims[3] = {(cuuint64_t)K, (cuuint64_t)rows, (cuuint64_t)batch};
@@ -388,7 +389,7 @@ int make_map(CUtensorMap* map, const void* base, int is_bf16, int64_t K, int64_t
   cuuint32_t estr[3] = {1, 1, 1};
   CUresult r = fn(map, is_bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
                   const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                  swizzle, promotion, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(XB_ERR_CUDA, "cuTensorMapEncodeTiled failed with %d", (int)r);
   return 0;
 }

@@ -2,8 +2,9 @@
 //   lora_shrink_kernel   U = scale (X A_a^T), every row with its own adapter's A, in fp32; and B as fp32 beside it
 //   lora_gemm_kernel     Y = X W + bias + U B_a^T: the tiles of the projection, whose depth goes on through the adapters' products
 //
-// Rows of a tile belong to any adapters. For each one that occurs in it (ascending) the MMAs run over all 128 rows, and the lanes of
-// the other rows are disabled, so neither sorting nor padding is asked of the caller; a tile of one request has one adapter.
+// Rows of a tile belong to any adapters, so neither sorting nor padding is asked of the caller; a tile of one request has one. U is made
+// for all 128 rows and up to 64 / rb adapters at once, side by side in tensor memory, and a row takes its own; the product with B
+// runs once for each adapter of the tile (ascending), with the lanes of the other rows disabled.
 // U is held as two TF32 terms, hi + lo, each rounded to nearest (|U - hi - lo| <= 2^-22 |U|), side by side along the depth, and B, whose
 // 16-bit values TF32 holds exactly, is read for both: fp16 would overflow or lose U's range, one term of bf16 would show in the result.
 // The products of adapters cost ceil(r / 16) depth blocks of 32 fp32 for each adapter of a tile beside the ceil(K / 64) of the projection.
@@ -20,13 +21,21 @@ constexpr uint32_t NO_ADAPTER = 0xffffffffu;
 template <int WORDS>
 struct TileAdapters {
   uint32_t id[WORDS];
-  __device__ __forceinline__ void load(const int32_t* adapter, int n_adapters, int m0, int M, int lane) {
+  // as they stand in memory; settle() makes them adapters, so that one tile's may be on their way while another's are used
+  __device__ __forceinline__ void fetch(const int32_t* adapter, int m0, int M, int lane) {
 #pragma unroll
     for (int w = 0; w < WORDS; ++w) {
       const int m = m0 + 32 * w + lane;
-      const int a = m < M ? adapter[m] : -1;
-      id[w] = a >= 0 && a < n_adapters ? (uint32_t)a : NO_ADAPTER;
+      id[w] = m < M ? (uint32_t)adapter[m] : NO_ADAPTER;
     }
+  }
+  __device__ __forceinline__ void settle(int n_adapters) {
+#pragma unroll
+    for (int w = 0; w < WORDS; ++w) id[w] = id[w] < (uint32_t)n_adapters ? id[w] : NO_ADAPTER;
+  }
+  __device__ __forceinline__ void load(const int32_t* adapter, int n_adapters, int m0, int M, int lane) {
+    fetch(adapter, m0, M, lane);
+    settle(n_adapters);
   }
   // the least that is `from` or above; NO_ADAPTER: none is left. The same for all lanes.
   __device__ __forceinline__ uint32_t next(uint32_t from) const {
@@ -39,16 +48,7 @@ struct TileAdapters {
   __device__ __forceinline__ uint32_t others(int w, uint32_t a) const { return ~__ballot_sync(0xffffffffu, id[w] == a); }
 };
 
-// 128 x N MMAs that leave the rows set in m0..m3 as they are (one bit a row), issued by an elected lane of a warp in uniform control flow
-__device__ __forceinline__ void mma_f16_ss_rows_elect(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, const uint32_t (&m)[4], uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "elect.sync _|q, 0xffffffff;\n\t"
-      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}"
-      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(m[0]), "r"(m[1]), "r"(m[2]), "r"(m[3])
-      : "memory");
-}
+// 128 x N TF32 MMA that leaves the rows set in m as they are (one bit a row), issued by an elected lane of a warp in uniform control flow
 __device__ __forceinline__ void mma_tf32_ss_rows_elect(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, const uint32_t (&m)[4], uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .pred p, q;\n\t"
@@ -58,7 +58,33 @@ __device__ __forceinline__ void mma_tf32_ss_rows_elect(uint32_t d, uint64_t a, u
       ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(m[0]), "r"(m[1]), "r"(m[2]), "r"(m[3])
       : "memory");
 }
+// and one for all rows: the masks of the other cost its issue several times as much
+__device__ __forceinline__ void mma_tf32_ss_elect(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.eq.b32 p, 0, 0;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::tf32 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc)
+      : "memory");
+}
 constexpr int FMT_TF32 = 2;
+// A stage's bytes announced and its copies issued the same way
+__device__ __forceinline__ void expect_tx_elect(uint32_t bar, uint32_t bytes) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "@q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}" ::"r"(bar), "r"(bytes)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_3d_elect(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "@q cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];\n\t}"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
 
 __device__ __forceinline__ float round_tf32(float v) {
   uint32_t r;
@@ -80,11 +106,59 @@ struct LoraTiles {
   uint32_t idesc_a, idesc_ext;
 };
 
+// B as fp32, zeros behind its r columns: pieces of four from `first` on, every `step`-th
+__device__ __forceinline__ void widen_b(const LoraTiles& p, int64_t first, int64_t step) {
+  const int64_t quads = (int64_t)p.n_adapters * p.N * (p.b_cols / 4);
+  for (int64_t e = first; e < quads; e += step) {
+    const int64_t an = e / (p.b_cols / 4);
+    const int c = (int)(e - an * (p.b_cols / 4)) * 4, a = (int)(an / p.N), n = (int)(an - (int64_t)a * p.N);
+    float v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int j = (c + i) % p.rb;
+      v[i] = j < p.r ? load_as_f32(p.B, (int64_t)a * p.stride_b + (int64_t)n * p.ldb + j, p.dtype) : 0.f;
+    }
+    reinterpret_cast<float4*>(p.B32)[e] = make_float4(v[0], v[1], v[2], v[3]);
+  }
+}
+__global__ void __launch_bounds__(128) lora_widen_kernel(const __grid_constant__ LoraTiles p) {
+  pdl_begin();
+  widen_b(p, (int64_t)blockIdx.x * 128 + threadIdx.x, (int64_t)gridDim.x * 128);
+}
+
+// v as two TF32 terms (an infinity or NaN, or what rounds up to one, stays whole in hi)
+__device__ __forceinline__ void split_tf32(float v, float& hi, float& lo) {
+  hi = round_tf32(v);
+  lo = fabsf(hi) <= 3.4028235e38f ? round_tf32(v - hi) : 0.f;
+}
+
+// The adapters of a tile, `group` at a time.
+constexpr int SHRINK_GROUP = 4;           // adapters of a pass, at most
+    struct Pass {
+    uint32_t id[SHRINK_GROUP];
+    int n;
+    uint32_t next;                                         // the first that this pass does not take
+    __device__ __forceinline__ void take(const TileAdapters<4>& t, uint32_t first, int group) {
+      n = 0;
+      next = first;
+#pragma unroll
+      for (int i = 0; i < SHRINK_GROUP; ++i) {
+        id[i] = i < group ? next : NO_ADAPTER;
+        if (id[i] != NO_ADAPTER) {
+          ++n;
+          next = t.next(next + 1);
+        }
+      }
+    }
+  };
+
 constexpr int SHRINK_THREADS = 320;       // producer, MMA, four warps for the results, four for B
 constexpr int SHRINK_GROUP_ROWS = 64;     // rows of A (adapters x rb) in a stage, or rb where that is more
 
 // Persistent, 128 rows a tile. Bound by reading X once; the adapters' A come from L2. A pass over the depth takes the A of up to 64 / rb
-// adapters with it; tiles of more adapters take more passes.
+// adapters with it, one MMA for all of them; tiles of more adapters take more passes, each with an accumulator of its own. (With
+// an MMA for each adapter that masks the others' rows out the warp that issues them bounded the kernel: a masked MMA takes it about
+// 150 cycles. [65536, 1280], rank 16: 54 us.)
 __global__ void __launch_bounds__(SHRINK_THREADS, 1)
 lora_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ LoraTiles p) {
   using namespace umma;
@@ -98,7 +172,7 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
   __shared__ uint32_t tmem_base_s;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int num_kb = (p.K + BLOCK_K - 1) / BLOCK_K;
-  const uint32_t tmem_cols = (uint32_t)max(32, 2 * p.rb);
+  const uint32_t acc_cols = (uint32_t)(p.group * p.rb), tmem_cols = max(32u, 2 * acc_cols);
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) { mbar_init(smem_u32(&full_bar[s]), 1); mbar_init(smem_u32(&empty_bar[s]), 1); }
     for (int s = 0; s < 2; ++s) { mbar_init(smem_u32(&acc_full[s]), 1); mbar_init(smem_u32(&acc_empty[s]), 4); }
@@ -113,114 +187,88 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
   const uint32_t tmem_base = tmem_base_s;
   pdl_wait();
 
-  if (warp < 2) {
-    // both walk the same passes: the adapters of a tile, `group` at a time
+  // every role but the last walks the same passes
+  if (warp < 6) {
+    const int q = warp & 3, row = q * 32 + lane;           // (the result warps' rows)
     int s = 0, it = 0;
     uint32_t ph = 0;
     bool ok = true;
+    TileAdapters<4> t, ahead;                              // (the next tile's are read while this one's operands are)
+    ahead.fetch(p.adapter, blockIdx.x * BLOCK_M, p.M, lane);
     for (int tile = blockIdx.x; tile < p.tiles_m && ok; tile += gridDim.x) {
       const int m0 = tile * BLOCK_M;
-      TileAdapters<4> t;
-      t.load(p.adapter, p.n_adapters, m0, p.M, lane);
-      uint32_t first = t.next(0);
-      if (first == NO_ADAPTER) continue;
-      const int as = it & 1;
-      if (warp == 1) {
-        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&acc_empty[as]), ((uint32_t)(it >> 1) & 1u) ^ 1u, 54));
-        tc_fence_after_sync();
-      }
-      while (first != NO_ADAPTER && ok) {
-        uint32_t after = first;                            // the adapters of this pass are in [first, after)
-        int n = 0;
-        for (uint32_t a = first; n < p.group && a != NO_ADAPTER; ++n) { after = a + 1; a = t.next(after); }
-        for (int kb = 0; kb < num_kb; ++kb, s = (s + 1 == STAGES ? 0 : s + 1), ph ^= (s == 0 ? 1u : 0u)) {
-          uint8_t* x = smem + s * stage_bytes;
-          if (warp == 0) {
-            ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&empty_bar[s]), ph ^ 1u, 51));
-            if (!ok) break;
-            if (lane == 0) {
-              mbar_arrive_expect_tx(smem_u32(&full_bar[s]), (uint32_t)(A_STAGE_BYTES + n * box));
-              tma_load_3d(smem_u32(x), &map_x, smem_u32(&full_bar[s]), kb * BLOCK_K, m0, 0);
-            }
-            uint32_t a = first;
-            for (int i = 0; i < n; ++i, a = t.next(a + 1))
-              if (lane == 0) tma_load_3d(smem_u32(x + A_STAGE_BYTES + i * box), &map_a, smem_u32(&full_bar[s]), kb * BLOCK_K, 0, (int)a);
-          } else {
-            ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&full_bar[s]), ph, 52));
-            if (!ok) break;
-            tc_fence_after_sync();
-            uint32_t a = first;
-            for (int i = 0; i < n; ++i, a = t.next(a + 1)) {
-              const uint32_t rows[4] = {t.others(0, a), t.others(1, a), t.others(2, a), t.others(3, a)};
-              const uint32_t x_addr = smem_u32(x), a_addr = smem_u32(x + A_STAGE_BYTES + i * box);
-#pragma unroll
-              for (int k = 0; k < BLOCK_K / 16; ++k)
-                mma_f16_ss_rows_elect(tmem_base + as * p.rb, make_desc_sw128(x_addr + k * 32, 1024), make_desc_sw128(a_addr + k * 32, 1024), p.idesc_a,
-                                      rows, (kb > 0 || k > 0) ? 1u : 0u);
-            }
-            mma_commit_elect(smem_u32(&empty_bar[s]));
-          }
-        }
-        first = t.next(after);
-      }
-      if (warp == 1 && ok) mma_commit_elect(smem_u32(&acc_full[as]));
-      ++it;
-    }
-  } else if (warp < 6) {
-    const int q = warp & 3, row = q * 32 + lane;
-    int it = 0;
-    for (int tile = blockIdx.x; tile < p.tiles_m; tile += gridDim.x) {
-      const int m0 = tile * BLOCK_M, gm = m0 + row;
-      TileAdapters<4> t;
-      t.load(p.adapter, p.n_adapters, m0, p.M, lane);
-      if (t.next(0) == NO_ADAPTER) continue;
+      t = ahead;
+      t.settle(p.n_adapters);
+      if (tile + (int)gridDim.x < p.tiles_m) ahead.fetch(p.adapter, (tile + (int)gridDim.x) * BLOCK_M, p.M, lane);
       uint32_t mine = NO_ADAPTER;
 #pragma unroll
       for (int w = 0; w < 4; ++w) mine = w == q ? t.id[w] : mine;
-      const int as = it & 1;
-      const float scale = mine != NO_ADAPTER && p.scale ? p.scale[mine] : 1.f;
-      if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&acc_full[as]), (uint32_t)(it >> 1) & 1u, 53))) break;
-      tc_fence_after_sync();
-      float* u = p.U + (int64_t)gm * p.u_cols;
-      for (int c = 0; c < p.rb; c += 16) {
-        uint32_t raw[16];
-        tmem_ld16_nowait(tmem_base + as * p.rb + c + ((uint32_t)(q * 32) << 16), raw);
-        tmem_wait_ld(raw);
-        if (mine != NO_ADAPTER) {
+      const float scale = warp >= 2 && mine != NO_ADAPTER && p.scale ? p.scale[mine] : 1.f;
+      Pass pass;
+      for (uint32_t first = t.next(0); first != NO_ADAPTER && ok; first = pass.next, ++it) {
+        pass.take(t, first, p.group);
+        const int as = it & 1;
+        const uint32_t acc = tmem_base + as * acc_cols, acc_ph = (uint32_t)(it >> 1) & 1u;
+        if (warp == 0) {
+          for (int kb = 0; kb < num_kb; ++kb, s = (s + 1 == STAGES ? 0 : s + 1), ph ^= (s == 0 ? 1u : 0u)) {
+            ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&empty_bar[s]), ph ^ 1u, 51));
+            if (!ok) break;
+            const uint32_t x = smem_u32(smem + s * stage_bytes), bar = smem_u32(&full_bar[s]);
+            expect_tx_elect(bar, (uint32_t)(A_STAGE_BYTES + pass.n * box));
+            tma_load_3d_elect(x, &map_x, bar, kb * BLOCK_K, m0, 0);
 #pragma unroll
-          for (int j = 0; j < 16; j += 4) {
-            float hi[4], lo[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float v = scale * __uint_as_float(raw[j + i]);
-              hi[i] = round_tf32(v);
-              // (an infinity or NaN, or what rounds up to one, stays whole in hi)
-              lo[i] = fabsf(hi[i]) <= 3.4028235e38f ? round_tf32(v - hi[i]) : 0.f;
-            }
-            *reinterpret_cast<float4*>(u + c + j) = make_float4(hi[0], hi[1], hi[2], hi[3]);
-            *reinterpret_cast<float4*>(u + p.rb + c + j) = make_float4(lo[0], lo[1], lo[2], lo[3]);
+            for (int i = 0; i < SHRINK_GROUP; ++i)
+              if (i < pass.n) tma_load_3d_elect(x + A_STAGE_BYTES + i * box, &map_a, bar, kb * BLOCK_K, 0, (int)pass.id[i]);
           }
+        } else if (warp == 1) {
+          ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&acc_empty[as]), acc_ph ^ 1u, 54));
+          if (!ok) break;
+          tc_fence_after_sync();
+          const uint32_t idesc = p.idesc_a | (uint32_t)(pass.n * p.rb >> 3) << 17;          // (columns: rb of every adapter of the pass)
+          for (int kb = 0; kb < num_kb; ++kb, s = (s + 1 == STAGES ? 0 : s + 1), ph ^= (s == 0 ? 1u : 0u)) {
+            ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&full_bar[s]), ph, 52));
+            if (!ok) break;
+            tc_fence_after_sync();
+            const uint32_t x = smem_u32(smem + s * stage_bytes);
+#pragma unroll
+            for (int k = 0; k < BLOCK_K / 16; ++k)
+              mma_f16_ss_elect(acc, make_desc_sw128(x + k * 32, 1024), make_desc_sw128(x + A_STAGE_BYTES + k * 32, 1024), idesc, (kb > 0 || k > 0) ? 1u : 0u);
+            mma_commit_elect(smem_u32(&empty_bar[s]));
+          }
+          if (ok) mma_commit_elect(smem_u32(&acc_full[as]));
+        } else {
+          ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&acc_full[as]), acc_ph, 53));
+          if (!ok) break;
+          tc_fence_after_sync();
+          float* u = p.U + (int64_t)(m0 + row) * p.u_cols;
+#pragma unroll
+          for (int i = 0; i < SHRINK_GROUP; ++i) {
+            if (i >= pass.n) break;
+            if (!__any_sync(0xffffffffu, mine == pass.id[i])) continue;
+            for (int c = 0; c < p.rb; c += 16) {
+              uint32_t raw[16];
+              tmem_ld16_nowait(acc + i * p.rb + c + ((uint32_t)(q * 32) << 16), raw);
+              tmem_wait_ld(raw);
+              if (mine != pass.id[i]) continue;
+#pragma unroll
+              for (int j = 0; j < 16; j += 4) {
+                float hi[4], lo[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) split_tf32(scale * __uint_as_float(raw[j + e]), hi[e], lo[e]);
+                *reinterpret_cast<float4*>(u + c + j) = make_float4(hi[0], hi[1], hi[2], hi[3]);
+                *reinterpret_cast<float4*>(u + p.rb + c + j) = make_float4(lo[0], lo[1], lo[2], lo[3]);
+              }
+            }
+            __syncwarp();
+          }
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&acc_empty[as]));
         }
       }
-      tc_fence_before_sync();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&acc_empty[as]));
-      ++it;
     }
   } else {
-    // B as fp32, zeros behind its r columns
-    const int64_t quads = (int64_t)p.n_adapters * p.N * (p.b_cols / 4);
-    for (int64_t e = (int64_t)blockIdx.x * 128 + (threadIdx.x - 192); e < quads; e += (int64_t)gridDim.x * 128) {
-      const int64_t an = e / (p.b_cols / 4);
-      const int c = (int)(e - an * (p.b_cols / 4)) * 4, a = (int)(an / p.N), n = (int)(an - (int64_t)a * p.N);
-      float v[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int j = (c + i) % p.rb;
-        v[i] = j < p.r ? load_as_f32(p.B, (int64_t)a * p.stride_b + (int64_t)n * p.ldb + j, p.dtype) : 0.f;
-      }
-      reinterpret_cast<float4*>(p.B32)[e] = make_float4(v[0], v[1], v[2], v[3]);
-    }
+    widen_b(p, (int64_t)blockIdx.x * 128 + (threadIdx.x - 192), (int64_t)gridDim.x * 128);
   }
 
   pdl_release();
@@ -295,25 +343,25 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
       t.load(l.adapter, l.n_adapters, m0, p.M, lane);      // (used when the projection's loads are under way)
       for (int kb = 0; kb < num_kb && ok; ++kb, advance()) {
         ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&empty_bar[s]), ph ^ 1u, 61));
-        if (ok && lane == 0) {
+        if (ok) {
           const uint32_t bar = smem_u32(&full_bar[s]), w = smem_u32(smem_b + s * w_bytes);
-          mbar_arrive_expect_tx(bar, (uint32_t)(A_STAGE_BYTES + w_bytes));
-          tma_load_3d(smem_u32(smem_a + s * A_STAGE_BYTES), &map_x, bar, kb * BLOCK_K, m0, 0);
+          expect_tx_elect(bar, (uint32_t)(A_STAGE_BYTES + w_bytes));
+          tma_load_3d_elect(smem_u32(smem_a + s * A_STAGE_BYTES), &map_x, bar, kb * BLOCK_K, m0, 0);
           if (!B_MN) {
-            tma_load_3d(w, &map_w, bar, kb * BLOCK_K, n0, 0);
+            tma_load_3d_elect(w, &map_w, bar, kb * BLOCK_K, n0, 0);
           } else {
-            for (int j = 0; j * 64 < p.block_n; ++j) tma_load_3d(w + j * MN_BOX_BYTES, &map_w, bar, n0 + j * 64, kb * BLOCK_K, 0);
+            for (int j = 0; j * 64 < p.block_n; ++j) tma_load_3d_elect(w + j * MN_BOX_BYTES, &map_w, bar, n0 + j * 64, kb * BLOCK_K, 0);
           }
         }
       }
       for (uint32_t a = t.next(0); a != NO_ADAPTER && ok; a = t.next(a + 1)) {
         for (int e = 0; e < u_blocks && ok; ++e, advance()) {
           ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&empty_bar[s]), ph ^ 1u, 61));
-          if (ok && lane == 0) {
+          if (ok) {
             const uint32_t bar = smem_u32(&full_bar[s]);
-            mbar_arrive_expect_tx(bar, (uint32_t)(A_STAGE_BYTES + b_bytes));
-            tma_load_3d(smem_u32(smem_a + s * A_STAGE_BYTES), &map_u, bar, e * 32, m0, 0);
-            tma_load_3d(smem_u32(smem_b + s * w_bytes), &map_b, bar, e % b_blocks * 32, n0, (int)a);
+            expect_tx_elect(bar, (uint32_t)(A_STAGE_BYTES + b_bytes));
+            tma_load_3d_elect(smem_u32(smem_a + s * A_STAGE_BYTES), &map_u, bar, e * 32, m0, 0);
+            tma_load_3d_elect(smem_u32(smem_b + s * w_bytes), &map_b, bar, e % b_blocks * 32, n0, (int)a);
           }
         }
       }
@@ -350,14 +398,22 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
       }
       for (uint32_t a = t.next(0); a != NO_ADAPTER && ok; a = t.next(a + 1)) {
         const uint32_t rows[4] = {t.others(0, a), t.others(1, a), t.others(2, a), t.others(3, a)};
+        const bool all = (rows[0] | rows[1] | rows[2] | rows[3]) == 0u;
         for (int e = 0; e < u_blocks; ++e, advance()) {
           ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&full_bar[s]), ph, 62));
           if (!ok) break;
           tc_fence_after_sync();
           const uint32_t a_addr = smem_u32(smem_a + s * A_STAGE_BYTES), b_addr = smem_u32(smem_b + s * w_bytes);
+          // (32 fp32 are four steps of 8)
+          if (all) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k)                        // 32 fp32 are four steps of 8
-            mma_tf32_ss_rows_elect(tmem_acc, make_desc_sw128(a_addr + k * 32, 1024), make_desc_sw128(b_addr + k * 32, 1024), l.idesc_ext, rows, 1u);
+            for (int k = 0; k < 4; ++k)
+              mma_tf32_ss_elect(tmem_acc, make_desc_sw128(a_addr + k * 32, 1024), make_desc_sw128(b_addr + k * 32, 1024), l.idesc_ext);
+          } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              mma_tf32_ss_rows_elect(tmem_acc, make_desc_sw128(a_addr + k * 32, 1024), make_desc_sw128(b_addr + k * 32, 1024), l.idesc_ext, rows, 1u);
+          }
           mma_commit_elect(smem_u32(&empty_bar[s]));
         }
       }
@@ -418,6 +474,287 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
   }
 }
 
+// Products of one column of tiles: both steps in one kernel, X read once. A tile's walk over the depth makes its projection and the U of up
+// to `group` adapters beside it in tensor memory (further adapters: U alone, over the depth once more). Four warps take U out,
+// scale and split it and leave it in shared memory as the operand of the product with B, which is issued after the next walk, so
+// that nobody waits for them. [74000, 324] x [324, 200], rank 8: 40 us as two kernels.
+constexpr int FUSED_THREADS = GEMM_THREADS + 128;
+struct LoraItem {                                          // one walk
+  uint32_t id[SHRINK_GROUP];
+  uint32_t row[4];                                         // the tile's adapters (TileAdapters)
+  int n, m0, it;                                           // adapters of the walk; first row; which of this CTA's tiles
+  bool first, last;                                        // of the tile
+};
+template <typename TOut, bool B_MN, int Y>
+__global__ void __launch_bounds__(FUSED_THREADS, 1)
+lora_fused_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a,
+                  const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_y, const __grid_constant__ UmmaGemmParams p,
+                  const __grid_constant__ LoraTiles l) {
+  using namespace umma;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int w_bytes = (B_MN ? (p.block_n + 63) / 64 * 64 : p.block_n) * BLOCK_K * 2, b_bytes = p.block_n * BLOCK_K * 2, box = l.rb * BLOCK_K * 2;
+  const int STAGES = p.stages, stage_bytes = A_STAGE_BYTES + w_bytes + l.group * box;         // X, W or B, the adapters' A
+  uint8_t* smem_u = smem + STAGES * stage_bytes;                                              // U: blocks of 128 rows x 32 floats
+  __shared__ __align__(8) uint64_t full_bar[MAX_STAGES];
+  __shared__ __align__(8) uint64_t empty_bar[MAX_STAGES];
+  __shared__ __align__(8) uint64_t acc_full[2];
+  __shared__ __align__(8) uint64_t acc_empty[2];
+  __shared__ __align__(8) uint64_t u_full[2], u_ready, u_free;
+  __shared__ uint32_t tmem_base_s;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int num_kb = (p.K + BLOCK_K - 1) / BLOCK_K, u_blocks = l.u_cols / 32, b_blocks = l.b_cols / 32;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) { mbar_init(smem_u32(&full_bar[s]), 1); mbar_init(smem_u32(&empty_bar[s]), 1); }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(smem_u32(&acc_full[s]), 1);
+      mbar_init(smem_u32(&acc_empty[s]), EPI_WARPS);
+      mbar_init(smem_u32(&u_full[s]), 1);
+    }
+    mbar_init(smem_u32(&u_ready), 4);
+    mbar_init(smem_u32(&u_free), 1);
+    fence_barrier_init();
+    prefetch_tensormap(&map_x);
+    prefetch_tensormap(&map_w);
+    prefetch_tensormap(&map_a);
+    prefetch_tensormap(&map_b);
+    if (Y == LORA_Y_TMA) prefetch_tensormap(&map_y);
+  }
+  if (warp == 1) tmem_alloc(smem_u32(&tmem_base_s), (uint32_t)p.tmem_cols);
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = tmem_base_s, tmem_u = tmem_base + 2 * p.block_n, u_stride = (uint32_t)(l.group * l.rb);
+  pdl_wait();
+
+  // The walks of this CTA's tiles in order; `visit` is false where a wait ran out. The same for every role.
+  auto each_item = [&](auto visit) {
+    TileAdapters<4> t, ahead;                              // (the next tile's are read while this one's operands are)
+    ahead.fetch(l.adapter, blockIdx.x * BLOCK_M, p.M, lane);
+    int it = 0;
+    for (int tile = blockIdx.x; tile < p.tiles_m; tile += gridDim.x, ++it) {
+      t = ahead;
+      t.settle(l.n_adapters);
+      if (tile + (int)gridDim.x < p.tiles_m) ahead.fetch(l.adapter, (tile + (int)gridDim.x) * BLOCK_M, p.M, lane);
+      LoraItem item;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) item.row[w] = t.id[w];
+      item.m0 = tile * BLOCK_M;
+      item.it = it;
+      item.first = true;
+      Pass pass;
+      uint32_t next = t.next(0);
+      do {
+        pass.take(t, next, l.group);
+        next = pass.next;
+#pragma unroll
+        for (int i = 0; i < SHRINK_GROUP; ++i) item.id[i] = pass.id[i];
+        item.n = pass.n;
+        item.last = next == NO_ADAPTER;
+        if (!visit(item)) return false;
+        item.first = false;
+      } while (!item.last);
+    }
+    return true;
+  };
+
+  if (warp < 2) {
+    // both go through the ring in the same order: a walk, then the products with B of the walk before
+    int s = 0, uw = 0;                                     // uw: walks whose U has been used
+    uint32_t ph = 0;
+    auto advance = [&]() {
+      s = s + 1 == STAGES ? 0 : s + 1;
+      ph ^= s == 0 ? 1u : 0u;
+    };
+    LoraItem before;
+    before.n = 0;
+    int walks = 0;                                         // with adapters
+    auto products = [&](const LoraItem& item) {            // U B^T of a walk's adapters
+      if (warp == 1) {
+        if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&u_ready), (uint32_t)uw & 1u, 75))) return false;
+        tc_fence_after_sync();
+      }
+      ++uw;
+#pragma unroll
+      for (int i = 0; i < SHRINK_GROUP; ++i) {
+        if (i >= item.n) break;
+        uint32_t rows[4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) rows[w] = ~__ballot_sync(0xffffffffu, item.row[w] == item.id[i]);
+        const bool all = (rows[0] | rows[1] | rows[2] | rows[3]) == 0u;
+        for (int e = 0; e < u_blocks; ++e, advance()) {
+          const uint32_t b = smem_u32(smem + s * stage_bytes + A_STAGE_BYTES), bar = smem_u32(&full_bar[s]);
+          if (warp == 0) {
+            if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&empty_bar[s]), ph ^ 1u, 71))) return false;
+            expect_tx_elect(bar, (uint32_t)b_bytes);
+            tma_load_3d_elect(b, &map_b, bar, e % b_blocks * 32, 0, (int)item.id[i]);
+          } else {
+            if (!__all_sync(0xffffffffu, mbar_wait(bar, ph, 72))) return false;
+            tc_fence_after_sync();
+            const uint32_t u = smem_u32(smem_u + e * A_STAGE_BYTES), acc = tmem_base + (item.it & 1) * p.block_n;
+            // (32 fp32 are four steps of 8)
+            if (all) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) mma_tf32_ss_elect(acc, make_desc_sw128(u + k * 32, 1024), make_desc_sw128(b + k * 32, 1024), l.idesc_ext);
+            } else {
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                mma_tf32_ss_rows_elect(acc, make_desc_sw128(u + k * 32, 1024), make_desc_sw128(b + k * 32, 1024), l.idesc_ext, rows, 1u);
+            }
+            mma_commit_elect(smem_u32(&empty_bar[s]));
+          }
+        }
+      }
+      if (warp == 1) {
+        mma_commit_elect(smem_u32(&u_free));
+        if (item.last) mma_commit_elect(smem_u32(&acc_full[item.it & 1]));
+      }
+      return true;
+    };
+    const bool ok = each_item([&](const LoraItem& item) {
+      const uint32_t acc = tmem_base + (item.it & 1) * p.block_n, u = tmem_u + (walks & 1) * u_stride;
+      if (warp == 1 && item.first) {
+        if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&acc_empty[item.it & 1]), ((uint32_t)(item.it >> 1) & 1u) ^ 1u, 74))) return false;
+        tc_fence_after_sync();
+      }
+      const uint32_t idesc_u = l.idesc_a | (uint32_t)(item.n * l.rb >> 3) << 17;            // (columns: rb of every adapter of the walk)
+      for (int kb = 0; kb < num_kb; ++kb, advance()) {
+        const uint32_t x = smem_u32(smem + s * stage_bytes), w = x + A_STAGE_BYTES, a = w + w_bytes, bar = smem_u32(&full_bar[s]);
+        if (warp == 0) {
+          if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&empty_bar[s]), ph ^ 1u, 71))) return false;
+          expect_tx_elect(bar, (uint32_t)(A_STAGE_BYTES + (item.first ? w_bytes : 0) + item.n * box));
+          tma_load_3d_elect(x, &map_x, bar, kb * BLOCK_K, item.m0, 0);
+          if (item.first) {
+            if (!B_MN) {
+              tma_load_3d_elect(w, &map_w, bar, kb * BLOCK_K, 0, 0);
+            } else {
+              for (int j = 0; j * 64 < p.block_n; ++j) tma_load_3d_elect(w + j * MN_BOX_BYTES, &map_w, bar, j * 64, kb * BLOCK_K, 0);
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < SHRINK_GROUP; ++i)
+            if (i < item.n) tma_load_3d_elect(a + i * box, &map_a, bar, kb * BLOCK_K, 0, (int)item.id[i]);
+        } else {
+          if (!__all_sync(0xffffffffu, mbar_wait(bar, ph, 72))) return false;
+          tc_fence_after_sync();
+          if (item.first) {
+#pragma unroll
+            for (int k = 0; k < BLOCK_K / 16; ++k)
+              mma_f16_ss_elect(acc, make_desc_sw128(x + k * 32, 1024),
+                               B_MN ? make_desc_sw128_mn(w + k * 2048, MN_BOX_BYTES) : make_desc_sw128(w + k * 32, 1024), p.idesc, (kb > 0 || k > 0) ? 1u : 0u);
+          }
+          if (item.n > 0) {
+#pragma unroll
+            for (int k = 0; k < BLOCK_K / 16; ++k)
+              mma_f16_ss_elect(u, make_desc_sw128(x + k * 32, 1024), make_desc_sw128(a + k * 32, 1024), idesc_u, (kb > 0 || k > 0) ? 1u : 0u);
+          }
+          mma_commit_elect(smem_u32(&empty_bar[s]));
+        }
+      }
+      if (warp == 1) {
+        if (item.n > 0) mma_commit_elect(smem_u32(&u_full[walks & 1]));
+        else mma_commit_elect(smem_u32(&acc_full[item.it & 1]));
+      }
+      if (item.n > 0) ++walks;
+      if (before.n > 0 && !products(before)) return false;
+      before = item;
+      return true;
+    });
+    if (ok && before.n > 0) products(before);
+  } else if (warp >= 2 + EPI_WARPS) {
+    // U: out of tensor memory, times the row's scale, as hi and lo into the operand's layout (rows of 128 bytes, pieces of 16 swapped by the row)
+    const int q = warp & 3, row = q * 32 + lane;
+    int uw = 0;
+    each_item([&](const LoraItem& item) {
+      if (item.n == 0) return true;
+      uint32_t mine = NO_ADAPTER;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) mine = w == q ? item.row[w] : mine;
+      const float scale = mine != NO_ADAPTER && l.scale ? l.scale[mine] : 1.f;
+      if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&u_full[uw & 1]), (uint32_t)(uw >> 1) & 1u, 73))) return false;
+      // the products that read the walk before have been made
+      if (!__all_sync(0xffffffffu, uw == 0 || mbar_wait(smem_u32(&u_free), (uint32_t)(uw - 1) & 1u, 76))) return false;
+      tc_fence_after_sync();
+#pragma unroll
+      for (int i = 0; i < SHRINK_GROUP; ++i) {
+        if (i >= item.n) break;
+        if (!__any_sync(0xffffffffu, mine == item.id[i])) continue;
+        for (int c = 0; c < l.rb; c += 16) {
+          uint32_t raw[16];
+          tmem_ld16_nowait(tmem_u + (uw & 1) * u_stride + i * l.rb + c + ((uint32_t)(q * 32) << 16), raw);
+          tmem_wait_ld(raw);
+          if (mine != item.id[i]) continue;
+#pragma unroll
+          for (int j = 0; j < 16; j += 4) {
+            float hi[4], lo[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) split_tf32(scale * __uint_as_float(raw[j + e]), hi[e], lo[e]);
+            auto put = [&](int at, const float (&v)[4]) {  // column `at` of the row
+              uint8_t* to = smem_u + (at >> 5) * A_STAGE_BYTES + row * 128 + ((((at & 31) >> 2) ^ (row & 7)) << 4);
+              *reinterpret_cast<float4*>(to) = make_float4(v[0], v[1], v[2], v[3]);
+            };
+            put(c + j, hi);
+            put(l.rb + c + j, lo);
+          }
+        }
+        __syncwarp();
+      }
+      fence_proxy_async_smem();
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&u_ready));
+      ++uw;
+      return true;
+    });
+  } else {
+    // (the epilogue of gemm_umma_kernel; the reasons for the order of its barriers stand there)
+    const int ew = warp - 2, q = warp & 3, part = ew >> 2, row = q * 32 + lane;
+    const int chunks = p.block_n / 16, c_begin = chunks * part / 4, c_end = chunks * (part + 1) / 4;
+    const bool vec_base = ((reinterpret_cast<uintptr_t>(p.Y) & 15) == 0) && ((p.ldy * sizeof(TOut)) % 16 == 0);
+    float* s_bias = reinterpret_cast<float*>(smem_u + u_blocks * A_STAGE_BYTES);                   // [4][256]
+    uint4* stage = reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(s_bias + 4 * 256) + ew * EPI_STAGE_BYTES);
+    float *s_a = s_bias + 256, *s_b = s_a + 256, *s_c = s_b + 256;
+    uint8_t* area = reinterpret_cast<uint8_t*>(s_bias + 4 * 256) + ew * p.y_bufs * p.y_unit * 64;
+    uint32_t turn = 0;
+    const int e = ew * 32 + lane;
+    if (e < p.block_n) stage_columns(p, 0, e, e, s_bias, s_a, s_b, s_c);
+    asm volatile("bar.sync 2, 512;" ::: "memory");
+    int it = 0;
+    for (int tile = blockIdx.x; tile < p.tiles_m; tile += gridDim.x, ++it) {
+      const int m0 = tile * BLOCK_M, as = it & 1, gm = m0 + row;
+      if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&acc_full[as]), (uint32_t)(it >> 1) & 1u, 77))) break;
+      tc_fence_after_sync();
+      const uint32_t tmem_acc = tmem_base + as * p.block_n + ((uint32_t)(q * 32) << 16);
+      TOut* yrow = reinterpret_cast<TOut*>(p.Y) + (int64_t)gm * p.ldy;
+      if constexpr (Y == LORA_Y_TMA) {
+        const int y = m0 + q * 32;
+        if (p.y_unit == 32)
+          epi_tile_tma<TOut, XB_EPI_NONE, 32>(map_y, tmem_acc, part, p.N, 1.f, s_bias, s_a, s_b, s_c, area, p.y_bufs, turn, 0, y, 0, y < p.M, lane);
+        else
+          epi_tile_tma<TOut, XB_EPI_NONE, 16>(map_y, tmem_acc, part, p.N, 1.f, s_bias, s_a, s_b, s_c, area, p.y_bufs, turn, 0, y, 0, y < p.M, lane);
+      } else if (sizeof(TOut) == 4 && vec_base && m0 + BLOCK_M <= p.M && p.block_n <= p.N) {
+        epi_tile_fast<TOut, XB_EPI_NONE, true>(tmem_acc, c_begin, c_end, 1.f, s_bias, s_a, s_b, s_c, yrow, p.ldy, 32, p.block_n, stage, lane);
+      } else {
+        epi_tile_edge<TOut>(p, tmem_acc, c_begin, c_end, s_bias, s_a, s_b, s_c, yrow, 0, gm, gm, 0, vec_base, reinterpret_cast<uint16_t*>(stage), lane);
+      }
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&acc_empty[as]));
+    }
+    if (Y == LORA_Y_TMA && lane == 0) tma_store_wait_read<0>();
+  }
+
+  pdl_release();
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem_base, (uint32_t)p.tmem_cols);
+  }
+}
+
 int make_map_f32(CUtensorMap* map, const void* base, int64_t cols, int64_t rows, int64_t batch, int box_rows) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return fail(XB_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
@@ -436,6 +773,14 @@ int launch_lora_gemm(const CUtensorMap (&m)[5], const UmmaGemmParams& p, const L
   XB_SET_MAX_SMEM_ONCE(attr_set, 226 * 1024, (const void*)lora_gemm_kernel<TOut, B_MN, Y>);
   launch_dependent(lora_gemm_kernel<TOut, B_MN, Y>, grid, GEMM_THREADS, smem, s, m[0], m[1], m[2], m[3], m[4], p, l);
   return check_launch("lora_gemm_kernel");
+}
+
+template <typename TOut, bool B_MN, int Y>
+int launch_lora_fused(const CUtensorMap (&m)[5], const UmmaGemmParams& p, const LoraTiles& l, unsigned grid, size_t smem, cudaStream_t s) {
+  static PerDeviceOnce attr_set;          // per instantiation
+  XB_SET_MAX_SMEM_ONCE(attr_set, 226 * 1024, (const void*)lora_fused_kernel<TOut, B_MN, Y>);
+  launch_dependent(lora_fused_kernel<TOut, B_MN, Y>, grid, FUSED_THREADS, smem, s, m[0], m[1], m[2], m[3], m[4], p, l);
+  return check_launch("lora_fused_kernel");
 }
 
 // What the tensor-core path takes: 16-bit operands that TMA can address, results as xb_gemm has them on that engine.
@@ -468,11 +813,19 @@ int run_umma(const xb_lora_args& a, uint8_t* ws, cudaStream_t stream) {
   l.B = a.B; l.ldb = a.ldb; l.stride_b = a.stride_b; l.dtype = a.dtype;
   l.group = std::max(1, SHRINK_GROUP_ROWS / l.rb);
   l.tiles_m = (a.M + BLOCK_M - 1) / BLOCK_M;
-  l.idesc_a = umma::make_idesc(BLOCK_M, l.rb, bf16);
+  l.idesc_a = umma::make_idesc(BLOCK_M, 0, bf16);          // (the columns are the pass's)
   CUtensorMap mx, ma;
-  if (int rc = make_map(&mx, a.X, bf16, a.K, a.M, a.ldx, 1, 0, BLOCK_M)) return rc;
+  if (int rc = make_map(&mx, a.X, bf16, a.K, a.M, a.ldx, 1, 0, BLOCK_M, BLOCK_K, CU_TENSOR_MAP_SWIZZLE_128B, 1, CU_TENSOR_MAP_L2_PROMOTION_L2_256B)) return rc;
   if (int rc = make_map(&ma, a.A, bf16, a.K, a.r, a.lda, a.n_adapters, a.stride_a, l.rb)) return rc;
-  {
+  // One column of tiles, and tensor memory for it and the U of an adapter twice: both steps in one kernel.
+  const int whole_n = (a.N + 15) / 16 * 16, fused_group = whole_n <= 256 ? std::min(SHRINK_GROUP, (256 - whole_n) / l.rb) : 0;
+  const bool fused = fused_group >= 1 && l.rb <= 64 && l.tiles_m >= sm_count() / 2;
+  if (fused) {
+    l.group = fused_group;
+    const int64_t quads = (int64_t)l.n_adapters * l.N * (l.b_cols / 4);
+    launch_dependent(lora_widen_kernel, (unsigned)std::min<int64_t>((quads + 127) / 128, 8 * sm_count()), 128, 0, stream, l);
+    if (int rc = check_launch("lora_widen_kernel")) return rc;
+  } else {
     const int stage = A_STAGE_BYTES + l.group * l.rb * BLOCK_K * 2;
     l.stages = std::min(MAX_STAGES, 220 * 1024 / stage);
     static PerDeviceOnce attr_set;
@@ -489,11 +842,11 @@ int run_umma(const xb_lora_args& a, uint8_t* ws, cudaStream_t stream) {
   p.tiles_m = l.tiles_m;
   // all of a product of up to 256 columns, equal shares of a wider one; narrower where the tiles would leave SMs idle
   const int wide = (a.N + 255) / 256, least = a.trans_w ? 32 : 64;
-  const int64_t split = std::max<int64_t>(wide, std::min<int64_t>(sm_count() / std::max(p.tiles_m, 1), (a.N + least - 1) / least));
+  const int64_t split = fused ? 1 : std::max<int64_t>(wide, std::min<int64_t>(sm_count() / std::max(p.tiles_m, 1), (a.N + least - 1) / least));
   p.block_n = (int)((a.N + split - 1) / split + 15) / 16 * 16;
   p.tiles_n = (a.N + p.block_n - 1) / p.block_n;
   p.tmem_cols = 64;
-  while (p.tmem_cols < 2 * p.block_n) p.tmem_cols <<= 1;
+  while (p.tmem_cols < 2 * (p.block_n + (fused ? l.group * l.rb : 0))) p.tmem_cols <<= 1;
   p.idesc = umma::make_idesc(BLOCK_M, p.block_n, bf16) | (p.b_mn ? umma::IDESC_B_MN : 0u);
   l.idesc_ext = umma::make_idesc(BLOCK_M, p.block_n, FMT_TF32);
   const int64_t total = (int64_t)p.tiles_m * p.tiles_n;
@@ -502,7 +855,8 @@ int run_umma(const xb_lora_args& a, uint8_t* ws, cudaStream_t stream) {
   CUtensorMap m[5];
   m[0] = mx;
   if (int rc = p.b_mn ? make_map(&m[1], a.W, bf16, a.N, a.K, a.ldw, 1, 0, BLOCK_K) : make_map(&m[1], a.W, bf16, a.K, a.N, a.ldw, 1, 0, p.block_n)) return rc;
-  if (int rc = make_map_f32(&m[2], l.U, l.u_cols, a.M, 1, BLOCK_M)) return rc;
+  if (fused) m[2] = ma;
+  else if (int rc = make_map_f32(&m[2], l.U, l.u_cols, a.M, 1, BLOCK_M)) return rc;
   if (int rc = make_map_f32(&m[3], l.B32, l.b_cols, a.N, a.n_adapters, p.block_n)) return rc;
   m[4] = m[0];
   const int64_t es = a.y_dtype == XB_F32 ? 4 : 2;
@@ -511,20 +865,24 @@ int run_umma(const xb_lora_args& a, uint8_t* ws, cudaStream_t stream) {
   if (es == 2 && (reinterpret_cast<uintptr_t>(a.Y) & 15) == 0 && a.ldy % 8 == 0 && a.N % 8 == 0) {
     // copies of 32 columns, 16 where the tile has few or where 32 would reach into the next tile
     p.y_unit = p.block_n >= 128 && (p.block_n % 32 == 0 || p.tiles_n == 1) ? 32 : 16;
-    p.y_bufs = p.block_n > 4 * p.y_unit ? 2 : 1;
+    p.y_bufs = 1;                         // (a second would cost a stage of the ring)
     if (make_map(&m[4], a.Y, a.y_dtype == XB_BF16, a.N, a.M, a.ldy, 1, 0, 32, p.y_unit,
                  p.y_unit == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B) == 0) {
       y = LORA_Y_TMA;
       tail = 4 * 256 * (int)sizeof(float) + EPI_WARPS * p.y_bufs * p.y_unit * 64;
     }
   }
-  const int stage = A_STAGE_BYTES + (p.b_mn ? (p.block_n + 63) / 64 * 64 : p.block_n) * BLOCK_K * 2;
+  const int stage = A_STAGE_BYTES + (p.b_mn ? (p.block_n + 63) / 64 * 64 : p.block_n) * BLOCK_K * 2 + (fused ? l.group * l.rb * BLOCK_K * 2 : 0);
+  if (fused) tail += l.u_cols / 32 * A_STAGE_BYTES;
   p.stages = std::max(2, std::min(MAX_STAGES, (SMEM_BUDGET - tail) / stage));
   const size_t smem = (size_t)p.stages * stage + tail + 1024;
   const unsigned grid = (unsigned)std::min<int64_t>(total, sm_count());
-  if (a.y_dtype == XB_F32) return launch_lora_gemm<float, false, LORA_Y_ANY>(m, p, l, grid, smem, stream);
+  if (a.y_dtype == XB_F32)
+    return fused ? launch_lora_fused<float, false, LORA_Y_ANY>(m, p, l, grid, smem, stream) : launch_lora_gemm<float, false, LORA_Y_ANY>(m, p, l, grid, smem, stream);
   auto half = [&](auto type) {
     using T = decltype(type);
+    if (fused && p.b_mn) return y == LORA_Y_TMA ? launch_lora_fused<T, true, LORA_Y_TMA>(m, p, l, grid, smem, stream) : launch_lora_fused<T, true, LORA_Y_ANY>(m, p, l, grid, smem, stream);
+    if (fused) return y == LORA_Y_TMA ? launch_lora_fused<T, false, LORA_Y_TMA>(m, p, l, grid, smem, stream) : launch_lora_fused<T, false, LORA_Y_ANY>(m, p, l, grid, smem, stream);
     if (p.b_mn) return y == LORA_Y_TMA ? launch_lora_gemm<T, true, LORA_Y_TMA>(m, p, l, grid, smem, stream) : launch_lora_gemm<T, true, LORA_Y_ANY>(m, p, l, grid, smem, stream);
     return y == LORA_Y_TMA ? launch_lora_gemm<T, false, LORA_Y_TMA>(m, p, l, grid, smem, stream) : launch_lora_gemm<T, false, LORA_Y_ANY>(m, p, l, grid, smem, stream);
   };

@@ -27,7 +27,9 @@ struct ConvParams {
 // Pieces of 8 bytes and eight rows ahead: with 16-byte pieces and four rows the registers let half as many warps in, which is what
 // the loads in flight are. SiLU is the rest: two exponentials and a quotient for two values.
 template <typename T, int V, int K>
-__global__ void __launch_bounds__(CONV_THREADS, K <= 4 && V * sizeof(T) <= 8 ? 6 : 4) ssm_conv_kernel(const ConvParams p) {
+constexpr int CONV_BLOCKS = K <= 4 && V * sizeof(T) <= 8 ? 6 : 4;         // of an SM: the registers are shared among so many
+template <typename T, int V, int K>
+__global__ void __launch_bounds__(CONV_THREADS, CONV_BLOCKS<T, V, K>) ssm_conv_kernel(const ConvParams p) {
   pdl_begin();
   __shared__ int s_first[CONV_THREADS];                // the first list that begins in or behind each of the block's chunks
   const int lane = threadIdx.x & 31;
