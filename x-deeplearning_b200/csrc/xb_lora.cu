@@ -246,8 +246,8 @@ extern "C" int xb_lora_gemm(const xb_lora_args* a, void* workspace, size_t works
   if (int rc = check_args(a)) return rc;
   if (a->M == 0 || a->N == 0) return 0;
   const size_t need = xb_lora_workspace_bytes(a);
-  XB_REQUIRE(workspace && workspace_bytes >= need, XB_ERR_SCRATCH, "xb_lora_gemm: workspace of %zu bytes, %zu needed", workspace_bytes, need);
-  XB_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, XB_ERR_ARG, "xb_lora_gemm: the workspace is not on 16 bytes");
+  XB_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), XB_ERR_SCRATCH, "xb_lora_gemm: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+  XB_REQUIRE(need == 0 || (reinterpret_cast<uintptr_t>(workspace) & 15) == 0, XB_ERR_ARG, "xb_lora_gemm: the workspace is not on 16 bytes");
   if (takes_tiles(*a)) return run_umma(*a, static_cast<uint8_t*>(workspace), (cudaStream_t)s);
   if (a->dtype == XB_F32) return run_rows<float>(*a, static_cast<uint8_t*>(workspace), (cudaStream_t)s);
   if (a->dtype == XB_F16) return run_rows<__half>(*a, static_cast<uint8_t*>(workspace), (cudaStream_t)s);

@@ -101,6 +101,7 @@ struct LoraTiles {
   float* U;                               // [M, u_cols]
   float* B32;                             // [n_adapters, N, b_cols]
   const void* B; int64_t ldb, stride_b; int dtype;
+  int vec_b;                              // rows of B in whole 16-byte pieces
   int group;                              // adapters of a pass of the shrink kernel
   int stages, tiles_m;
   uint32_t idesc_a, idesc_ext;
@@ -121,11 +122,6 @@ __device__ __forceinline__ void widen_b(const LoraTiles& p, int64_t first, int64
     reinterpret_cast<float4*>(p.B32)[e] = make_float4(v[0], v[1], v[2], v[3]);
   }
 }
-__global__ void __launch_bounds__(128) lora_widen_kernel(const __grid_constant__ LoraTiles p) {
-  pdl_begin();
-  widen_b(p, (int64_t)blockIdx.x * 128 + threadIdx.x, (int64_t)gridDim.x * 128);
-}
-
 // v as two TF32 terms (an infinity or NaN, or what rounds up to one, stays whole in hi)
 __device__ __forceinline__ void split_tf32(float v, float& hi, float& lo) {
   hi = round_tf32(v);
@@ -474,11 +470,13 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
   }
 }
 
-// Products of one column of tiles: both steps in one kernel, X read once. A tile's walk over the depth makes its projection and the U of up
-// to `group` adapters beside it in tensor memory (further adapters: U alone, over the depth once more). Four warps take U out,
-// scale and split it and leave it in shared memory as the operand of the product with B, which is issued after the next walk, so
-// that nobody waits for them. [74000, 324] x [324, 200], rank 8: 40 us as two kernels.
+// Products of one column of tiles: both steps in one kernel, X read once. A tile's walk over the depth makes its projection and, in the same
+// MMAs, the U of up to `group` adapters beside it in tensor memory (further adapters: U alone, over the depth once more). Four warps
+// take U out, scale and split it, widen B to fp32 beside it, and leave both in shared memory as the operands of U B^T, which is issued
+// after the next walk, so that nobody waits for them. [74000, 324] x [324, 200], rank 8: 40 us as two kernels. What bounds it is the
+// way from L2: 42 KB of X and W for each 64 of the depth.
 constexpr int FUSED_THREADS = GEMM_THREADS + 128;
+constexpr int FUSED_MAX_RB = 32;                           // (the operands of a larger rank would take the ring's space)
 struct LoraItem {                                          // one walk
   uint32_t id[SHRINK_GROUP];
   uint32_t row[4];                                         // the tile's adapters (TileAdapters)
@@ -488,23 +486,23 @@ struct LoraItem {                                          // one walk
 template <typename TOut, bool B_MN, int Y>
 __global__ void __launch_bounds__(FUSED_THREADS, 1)
 lora_fused_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a,
-                  const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_y, const __grid_constant__ UmmaGemmParams p,
-                  const __grid_constant__ LoraTiles l) {
+                  const __grid_constant__ CUtensorMap map_y, const __grid_constant__ UmmaGemmParams p, const __grid_constant__ LoraTiles l) {
   using namespace umma;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  const int w_bytes = (B_MN ? (p.block_n + 63) / 64 * 64 : p.block_n) * BLOCK_K * 2, b_bytes = p.block_n * BLOCK_K * 2, box = l.rb * BLOCK_K * 2;
-  const int STAGES = p.stages, stage_bytes = A_STAGE_BYTES + w_bytes + l.group * box;         // X, W or B, the adapters' A
+  const int w_bytes = (B_MN ? (p.block_n + 63) / 64 * 64 : p.block_n) * BLOCK_K * 2, box = l.rb * BLOCK_K * 2;
+  const int STAGES = p.stages, stage_bytes = A_STAGE_BYTES + w_bytes + l.group * box;         // X, W, the adapters' A behind it
   uint8_t* smem_u = smem + STAGES * stage_bytes;                                              // U: blocks of 128 rows x 32 floats
+  uint8_t* smem_b = smem_u + l.u_cols / 32 * A_STAGE_BYTES;                                   // B: block_n rows x 32 floats
   __shared__ __align__(8) uint64_t full_bar[MAX_STAGES];
   __shared__ __align__(8) uint64_t empty_bar[MAX_STAGES];
   __shared__ __align__(8) uint64_t acc_full[2];
   __shared__ __align__(8) uint64_t acc_empty[2];
-  __shared__ __align__(8) uint64_t u_full[2], u_ready, u_free;
+  __shared__ __align__(8) uint64_t u_full[2], ready, used;
   __shared__ uint32_t tmem_base_s;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int num_kb = (p.K + BLOCK_K - 1) / BLOCK_K, u_blocks = l.u_cols / 32, b_blocks = l.b_cols / 32;
+  const int num_kb = (p.K + BLOCK_K - 1) / BLOCK_K, u_blocks = l.u_cols / 32;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) { mbar_init(smem_u32(&full_bar[s]), 1); mbar_init(smem_u32(&empty_bar[s]), 1); }
@@ -513,20 +511,19 @@ lora_fused_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
       mbar_init(smem_u32(&acc_empty[s]), EPI_WARPS);
       mbar_init(smem_u32(&u_full[s]), 1);
     }
-    mbar_init(smem_u32(&u_ready), 4);
-    mbar_init(smem_u32(&u_free), 1);
+    mbar_init(smem_u32(&ready), 4);
+    mbar_init(smem_u32(&used), 1);
     fence_barrier_init();
     prefetch_tensormap(&map_x);
     prefetch_tensormap(&map_w);
     prefetch_tensormap(&map_a);
-    prefetch_tensormap(&map_b);
     if (Y == LORA_Y_TMA) prefetch_tensormap(&map_y);
   }
   if (warp == 1) tmem_alloc(smem_u32(&tmem_base_s), (uint32_t)p.tmem_cols);
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
-  const uint32_t tmem_base = tmem_base_s, tmem_u = tmem_base + 2 * p.block_n, u_stride = (uint32_t)(l.group * l.rb);
+  const uint32_t tmem_base = tmem_base_s, acc_stride = (uint32_t)(p.block_n + l.group * l.rb);        // an accumulator, its U behind it
   pdl_wait();
 
   // The walks of this CTA's tiles in order; `visit` is false where a wait ran out. The same for every role.
@@ -560,23 +557,35 @@ lora_fused_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
     return true;
   };
 
-  if (warp < 2) {
-    // both go through the ring in the same order: a walk, then the products with B of the walk before
-    int s = 0, uw = 0;                                     // uw: walks whose U has been used
+  if (warp == 0) {
+    int s = 0;
     uint32_t ph = 0;
-    auto advance = [&]() {
-      s = s + 1 == STAGES ? 0 : s + 1;
-      ph ^= s == 0 ? 1u : 0u;
-    };
+    each_item([&](const LoraItem& item) {
+      const uint32_t bytes = (uint32_t)(A_STAGE_BYTES + (item.first ? w_bytes : 0) + item.n * box);
+      for (int kb = 0; kb < num_kb; ++kb, s = (s + 1 == STAGES ? 0 : s + 1), ph ^= (s == 0 ? 1u : 0u)) {
+        const uint32_t x = smem_u32(smem + s * stage_bytes), w = x + A_STAGE_BYTES, a = w + w_bytes, bar = smem_u32(&full_bar[s]);
+        if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&empty_bar[s]), ph ^ 1u, 71))) return false;
+        expect_tx_elect(bar, bytes);
+        tma_load_3d_elect(x, &map_x, bar, kb * BLOCK_K, item.m0, 0);
+        if (item.first) {
+          if (!B_MN) {
+            tma_load_3d_elect(w, &map_w, bar, kb * BLOCK_K, 0, 0);
+          } else {
+            for (int j = 0; j * 64 < p.block_n; ++j) tma_load_3d_elect(w + j * MN_BOX_BYTES, &map_w, bar, j * 64, kb * BLOCK_K, 0);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < SHRINK_GROUP; ++i)
+          if (i < item.n) tma_load_3d_elect(a + i * box, &map_a, bar, kb * BLOCK_K, 0, (int)item.id[i]);
+      }
+      return true;
+    });
+  } else if (warp == 1) {
+    int s = 0, walks = 0, product = 0;                     // walks with adapters; products with B
+    uint32_t ph = 0;
     LoraItem before;
     before.n = 0;
-    int walks = 0;                                         // with adapters
     auto products = [&](const LoraItem& item) {            // U B^T of a walk's adapters
-      if (warp == 1) {
-        if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&u_ready), (uint32_t)uw & 1u, 75))) return false;
-        tc_fence_after_sync();
-      }
-      ++uw;
 #pragma unroll
       for (int i = 0; i < SHRINK_GROUP; ++i) {
         if (i >= item.n) break;
@@ -584,79 +593,58 @@ lora_fused_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
 #pragma unroll
         for (int w = 0; w < 4; ++w) rows[w] = ~__ballot_sync(0xffffffffu, item.row[w] == item.id[i]);
         const bool all = (rows[0] | rows[1] | rows[2] | rows[3]) == 0u;
-        for (int e = 0; e < u_blocks; ++e, advance()) {
-          const uint32_t b = smem_u32(smem + s * stage_bytes + A_STAGE_BYTES), bar = smem_u32(&full_bar[s]);
-          if (warp == 0) {
-            if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&empty_bar[s]), ph ^ 1u, 71))) return false;
-            expect_tx_elect(bar, (uint32_t)b_bytes);
-            tma_load_3d_elect(b, &map_b, bar, e % b_blocks * 32, 0, (int)item.id[i]);
+        if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&ready), (uint32_t)product & 1u, 75))) return false;
+        tc_fence_after_sync();
+        ++product;
+        const uint32_t b = smem_u32(smem_b), acc = tmem_base + (item.it & 1) * acc_stride;
+        for (int e = 0; e < u_blocks; ++e) {
+          const uint32_t u = smem_u32(smem_u + e * A_STAGE_BYTES);
+          // (32 fp32 are four steps of 8)
+          if (all) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) mma_tf32_ss_elect(acc, make_desc_sw128(u + k * 32, 1024), make_desc_sw128(b + k * 32, 1024), l.idesc_ext);
           } else {
-            if (!__all_sync(0xffffffffu, mbar_wait(bar, ph, 72))) return false;
-            tc_fence_after_sync();
-            const uint32_t u = smem_u32(smem_u + e * A_STAGE_BYTES), acc = tmem_base + (item.it & 1) * p.block_n;
-            // (32 fp32 are four steps of 8)
-            if (all) {
 #pragma unroll
-              for (int k = 0; k < 4; ++k) mma_tf32_ss_elect(acc, make_desc_sw128(u + k * 32, 1024), make_desc_sw128(b + k * 32, 1024), l.idesc_ext);
-            } else {
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                mma_tf32_ss_rows_elect(acc, make_desc_sw128(u + k * 32, 1024), make_desc_sw128(b + k * 32, 1024), l.idesc_ext, rows, 1u);
-            }
-            mma_commit_elect(smem_u32(&empty_bar[s]));
+            for (int k = 0; k < 4; ++k)
+              mma_tf32_ss_rows_elect(acc, make_desc_sw128(u + k * 32, 1024), make_desc_sw128(b + k * 32, 1024), l.idesc_ext, rows, 1u);
           }
         }
+        mma_commit_elect(smem_u32(&used));
       }
-      if (warp == 1) {
-        mma_commit_elect(smem_u32(&u_free));
-        if (item.last) mma_commit_elect(smem_u32(&acc_full[item.it & 1]));
-      }
+      if (item.last) mma_commit_elect(smem_u32(&acc_full[item.it & 1]));
       return true;
     };
     const bool ok = each_item([&](const LoraItem& item) {
-      const uint32_t acc = tmem_base + (item.it & 1) * p.block_n, u = tmem_u + (walks & 1) * u_stride;
-      if (warp == 1 && item.first) {
+      const uint32_t acc = tmem_base + (item.it & 1) * acc_stride, u = acc + p.block_n;
+      if (!item.first) {                                   // the U before this one, in the same columns, has been taken out
+        if (!products(before)) return false;
+        before.n = 0;
+      } else {
         if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&acc_empty[item.it & 1]), ((uint32_t)(item.it >> 1) & 1u) ^ 1u, 74))) return false;
         tc_fence_after_sync();
       }
-      const uint32_t idesc_u = l.idesc_a | (uint32_t)(item.n * l.rb >> 3) << 17;            // (columns: rb of every adapter of the walk)
-      for (int kb = 0; kb < num_kb; ++kb, advance()) {
-        const uint32_t x = smem_u32(smem + s * stage_bytes), w = x + A_STAGE_BYTES, a = w + w_bytes, bar = smem_u32(&full_bar[s]);
-        if (warp == 0) {
-          if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&empty_bar[s]), ph ^ 1u, 71))) return false;
-          expect_tx_elect(bar, (uint32_t)(A_STAGE_BYTES + (item.first ? w_bytes : 0) + item.n * box));
-          tma_load_3d_elect(x, &map_x, bar, kb * BLOCK_K, item.m0, 0);
-          if (item.first) {
-            if (!B_MN) {
-              tma_load_3d_elect(w, &map_w, bar, kb * BLOCK_K, 0, 0);
-            } else {
-              for (int j = 0; j * 64 < p.block_n; ++j) tma_load_3d_elect(w + j * MN_BOX_BYTES, &map_w, bar, j * 64, kb * BLOCK_K, 0);
-            }
-          }
+      // the descriptors' columns: those of W, rb of every adapter of the walk, or both where they lie one behind the other
+      const uint32_t cols_u = (uint32_t)(item.n * l.rb >> 3) << 17;
+      const uint32_t idesc_u = l.idesc_a | cols_u, idesc = p.idesc + (B_MN ? 0u : cols_u);
+      for (int kb = 0; kb < num_kb; ++kb, s = (s + 1 == STAGES ? 0 : s + 1), ph ^= (s == 0 ? 1u : 0u)) {
+        const uint32_t x = smem_u32(smem + s * stage_bytes), w = x + A_STAGE_BYTES, a = w + w_bytes;
+        if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&full_bar[s]), ph, 72))) return false;
+        tc_fence_after_sync();
+        if (item.first) {
 #pragma unroll
-          for (int i = 0; i < SHRINK_GROUP; ++i)
-            if (i < item.n) tma_load_3d_elect(a + i * box, &map_a, bar, kb * BLOCK_K, 0, (int)item.id[i]);
-        } else {
-          if (!__all_sync(0xffffffffu, mbar_wait(bar, ph, 72))) return false;
-          tc_fence_after_sync();
-          if (item.first) {
-#pragma unroll
-            for (int k = 0; k < BLOCK_K / 16; ++k)
-              mma_f16_ss_elect(acc, make_desc_sw128(x + k * 32, 1024),
-                               B_MN ? make_desc_sw128_mn(w + k * 2048, MN_BOX_BYTES) : make_desc_sw128(w + k * 32, 1024), p.idesc, (kb > 0 || k > 0) ? 1u : 0u);
-          }
-          if (item.n > 0) {
-#pragma unroll
-            for (int k = 0; k < BLOCK_K / 16; ++k)
-              mma_f16_ss_elect(u, make_desc_sw128(x + k * 32, 1024), make_desc_sw128(a + k * 32, 1024), idesc_u, (kb > 0 || k > 0) ? 1u : 0u);
-          }
-          mma_commit_elect(smem_u32(&empty_bar[s]));
+          for (int k = 0; k < BLOCK_K / 16; ++k)
+            mma_f16_ss_elect(acc, make_desc_sw128(x + k * 32, 1024),
+                             B_MN ? make_desc_sw128_mn(w + k * 2048, MN_BOX_BYTES) : make_desc_sw128(w + k * 32, 1024), idesc, (kb > 0 || k > 0) ? 1u : 0u);
         }
+        if (item.n > 0 && (B_MN || !item.first)) {
+#pragma unroll
+          for (int k = 0; k < BLOCK_K / 16; ++k)
+            mma_f16_ss_elect(u, make_desc_sw128(x + k * 32, 1024), make_desc_sw128(a + k * 32, 1024), idesc_u, (kb > 0 || k > 0) ? 1u : 0u);
+        }
+        mma_commit_elect(smem_u32(&empty_bar[s]));
       }
-      if (warp == 1) {
-        if (item.n > 0) mma_commit_elect(smem_u32(&u_full[walks & 1]));
-        else mma_commit_elect(smem_u32(&acc_full[item.it & 1]));
-      }
+      if (item.n > 0) mma_commit_elect(smem_u32(&u_full[walks & 1]));
+      else mma_commit_elect(smem_u32(&acc_full[item.it & 1]));
       if (item.n > 0) ++walks;
       if (before.n > 0 && !products(before)) return false;
       before = item;
@@ -664,48 +652,92 @@ lora_fused_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
     });
     if (ok && before.n > 0) products(before);
   } else if (warp >= 2 + EPI_WARPS) {
-    // U: out of tensor memory, times the row's scale, as hi and lo into the operand's layout (rows of 128 bytes, pieces of 16 swapped by the row)
-    const int q = warp & 3, row = q * 32 + lane;
-    int uw = 0;
+    // The operands of U B^T, in rows of 128 bytes whose pieces of 16 are swapped by the row: B as fp32, zeros behind its r columns, and (with
+    // the first adapter of a walk) U out of tensor memory, times the row's scale, as hi and lo.
+    const int q = warp & 3, row = q * 32 + lane, thread = threadIdx.x - (2 + EPI_WARPS) * 32;
+    auto put = [](uint8_t* block, int r, int c, const float (&v)[4]) {
+      *reinterpret_cast<float4*>(block + r * 128 + (((c >> 2) ^ (r & 7)) << 4)) = make_float4(v[0], v[1], v[2], v[3]);
+    };
+    int walks = 0, product = 0;
     each_item([&](const LoraItem& item) {
-      if (item.n == 0) return true;
       uint32_t mine = NO_ADAPTER;
 #pragma unroll
       for (int w = 0; w < 4; ++w) mine = w == q ? item.row[w] : mine;
       const float scale = mine != NO_ADAPTER && l.scale ? l.scale[mine] : 1.f;
-      if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&u_full[uw & 1]), (uint32_t)(uw >> 1) & 1u, 73))) return false;
-      // the products that read the walk before have been made
-      if (!__all_sync(0xffffffffu, uw == 0 || mbar_wait(smem_u32(&u_free), (uint32_t)(uw - 1) & 1u, 76))) return false;
-      tc_fence_after_sync();
+#pragma unroll 1
+      for (int i = 0; i < item.n; ++i) {
+        uint32_t id = item.id[0];
 #pragma unroll
-      for (int i = 0; i < SHRINK_GROUP; ++i) {
-        if (i >= item.n) break;
-        if (!__any_sync(0xffffffffu, mine == item.id[i])) continue;
-        for (int c = 0; c < l.rb; c += 16) {
-          uint32_t raw[16];
-          tmem_ld16_nowait(tmem_u + (uw & 1) * u_stride + i * l.rb + c + ((uint32_t)(q * 32) << 16), raw);
-          tmem_wait_ld(raw);
-          if (mine != item.id[i]) continue;
+        for (int k = 1; k < SHRINK_GROUP; ++k) id = i == k ? item.id[k] : id;
+        // the product before has read what is overwritten now
+        if (!__all_sync(0xffffffffu, product == 0 || mbar_wait(smem_u32(&used), (uint32_t)(product - 1) & 1u, 76))) return false;
 #pragma unroll
-          for (int j = 0; j < 16; j += 4) {
-            float hi[4], lo[4];
+        for (int h = 0; h < 2; ++h) {
+          const int n = thread + 128 * h;
+          if (n >= p.block_n) break;
+          const int64_t at = (int64_t)id * l.stride_b + (int64_t)n * l.ldb;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) split_tf32(scale * __uint_as_float(raw[j + e]), hi[e], lo[e]);
-            auto put = [&](int at, const float (&v)[4]) {  // column `at` of the row
-              uint8_t* to = smem_u + (at >> 5) * A_STAGE_BYTES + row * 128 + ((((at & 31) >> 2) ^ (row & 7)) << 4);
-              *reinterpret_cast<float4*>(to) = make_float4(v[0], v[1], v[2], v[3]);
-            };
-            put(c + j, hi);
-            put(l.rb + c + j, lo);
+          for (int j = 0; j < FUSED_MAX_RB; j += 8) {
+            if (j >= l.rb) break;
+            float v[8];
+            if (l.vec_b && n < p.N && j < l.r) {
+              const uint4 t = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(l.B) + at + j));
+              const uint32_t x[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                if (l.dtype == XB_BF16) {
+                  v[2 * k] = __uint_as_float(x[k] << 16);
+                  v[2 * k + 1] = __uint_as_float(x[k] & 0xffff0000u);
+                } else {
+                  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&x[k]));
+                  v[2 * k] = f.x;
+                  v[2 * k + 1] = f.y;
+                }
+              }
+            } else {
+#pragma unroll
+              for (int k = 0; k < 8; ++k) v[k] = n < p.N && j + k < l.r ? load_as_f32(l.B, at + j + k, l.dtype) : 0.f;
+            }
+            const float lo[4] = {v[0], v[1], v[2], v[3]}, hi[4] = {v[4], v[5], v[6], v[7]};
+            put(smem_b, n, j, lo);
+            put(smem_b, n, j + 4, hi);
+            if (l.rb == 16) {                              // 16 columns stand there twice, for U's hi and lo in one block
+              put(smem_b, n, 16 + j, lo);
+              put(smem_b, n, 20 + j, hi);
+            }
           }
         }
+        if (i == 0) {
+          if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&u_full[walks & 1]), (uint32_t)(walks >> 1) & 1u, 73))) return false;
+          tc_fence_after_sync();
+#pragma unroll
+          for (int k = 0; k < SHRINK_GROUP; ++k) {
+            if (k >= item.n) break;
+            if (!__any_sync(0xffffffffu, mine == item.id[k])) continue;
+            for (int c = 0; c < l.rb; c += 16) {
+              uint32_t raw[16];
+              tmem_ld16_nowait(tmem_base + (item.it & 1) * acc_stride + p.block_n + k * l.rb + c + ((uint32_t)(q * 32) << 16), raw);
+              tmem_wait_ld(raw);
+              if (mine != item.id[k]) continue;
+#pragma unroll
+              for (int j = 0; j < 16; j += 4) {
+                float hi[4], lo[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) split_tf32(scale * __uint_as_float(raw[j + e]), hi[e], lo[e]);
+                put(smem_u, row, c + j, hi);               // (hi and lo of 16 columns share the one block there is, of 32 they have one each)
+                put(smem_u + (l.rb >> 5) * A_STAGE_BYTES, row, (l.rb == 16 ? 16 : 0) + c + j, lo);
+              }
+            }
+            __syncwarp();
+          }
+          tc_fence_before_sync();
+          ++walks;
+        }
+        fence_proxy_async_smem();
         __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&ready));
+        ++product;
       }
-      fence_proxy_async_smem();
-      tc_fence_before_sync();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&u_ready));
-      ++uw;
       return true;
     });
   } else {
@@ -713,7 +745,7 @@ lora_fused_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
     const int ew = warp - 2, q = warp & 3, part = ew >> 2, row = q * 32 + lane;
     const int chunks = p.block_n / 16, c_begin = chunks * part / 4, c_end = chunks * (part + 1) / 4;
     const bool vec_base = ((reinterpret_cast<uintptr_t>(p.Y) & 15) == 0) && ((p.ldy * sizeof(TOut)) % 16 == 0);
-    float* s_bias = reinterpret_cast<float*>(smem_u + u_blocks * A_STAGE_BYTES);                   // [4][256]
+    float* s_bias = reinterpret_cast<float*>(smem_b + p.block_n * 128);                            // [4][256]
     uint4* stage = reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(s_bias + 4 * 256) + ew * EPI_STAGE_BYTES);
     float *s_a = s_bias + 256, *s_b = s_a + 256, *s_c = s_b + 256;
     uint8_t* area = reinterpret_cast<uint8_t*>(s_bias + 4 * 256) + ew * p.y_bufs * p.y_unit * 64;
@@ -726,7 +758,7 @@ lora_fused_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
       const int m0 = tile * BLOCK_M, as = it & 1, gm = m0 + row;
       if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&acc_full[as]), (uint32_t)(it >> 1) & 1u, 77))) break;
       tc_fence_after_sync();
-      const uint32_t tmem_acc = tmem_base + as * p.block_n + ((uint32_t)(q * 32) << 16);
+      const uint32_t tmem_acc = tmem_base + as * acc_stride + ((uint32_t)(q * 32) << 16);
       TOut* yrow = reinterpret_cast<TOut*>(p.Y) + (int64_t)gm * p.ldy;
       if constexpr (Y == LORA_Y_TMA) {
         const int y = m0 + q * 32;
@@ -779,19 +811,53 @@ template <typename TOut, bool B_MN, int Y>
 int launch_lora_fused(const CUtensorMap (&m)[5], const UmmaGemmParams& p, const LoraTiles& l, unsigned grid, size_t smem, cudaStream_t s) {
   static PerDeviceOnce attr_set;          // per instantiation
   XB_SET_MAX_SMEM_ONCE(attr_set, 226 * 1024, (const void*)lora_fused_kernel<TOut, B_MN, Y>);
-  launch_dependent(lora_fused_kernel<TOut, B_MN, Y>, grid, FUSED_THREADS, smem, s, m[0], m[1], m[2], m[3], m[4], p, l);
+  launch_dependent(lora_fused_kernel<TOut, B_MN, Y>, grid, FUSED_THREADS, smem, s, m[0], m[1], m[2], m[4], p, l);
   return check_launch("lora_fused_kernel");
 }
 
-// What the tensor-core path takes: 16-bit operands that TMA can address, results as xb_gemm has them on that engine.
-bool lora_umma_takes(const xb_lora_args& a) {
-  if (a.dtype != XB_F16 && a.dtype != XB_BF16) return false;
-  if (a.n_adapters < 1 || a.r < 1) return false;
-  if (!a.trans_w && a.y_dtype == XB_F32) return false;     // (its sums are not rounded at every step: see xb_gemm)
-  if (a.ldx % 8 || a.ldw % 8 || a.lda % 8 || (a.n_adapters > 1 && (a.stride_a % 8 || a.stride_a == 0))) return false;
-  return ((reinterpret_cast<uintptr_t>(a.X) | reinterpret_cast<uintptr_t>(a.W) | reinterpret_cast<uintptr_t>(a.A)) & 15) == 0;
+// Rows that TMA cannot address (they do not start on 16 bytes) are laid out again in the workspace, as K-major rows of `ld` elements; the same
+// for weights in [K, N] whose results are fp32, and for adapters that share one A.
+struct LoraCopies { bool x, w, a; int64_t ld; };
+LoraCopies lora_copies(const xb_lora_args& a) {
+  auto odd = [](const void* p, int64_t ld) { return ld % 8 != 0 || (reinterpret_cast<uintptr_t>(p) & 15) != 0; };
+  LoraCopies c;
+  c.ld = ((int64_t)a.K + 7) / 8 * 8;
+  c.x = odd(a.X, a.ldx);
+  c.w = odd(a.W, a.ldw) || (!a.trans_w && a.y_dtype == XB_F32);
+  c.a = odd(a.A, a.lda) || (a.n_adapters > 1 && (a.stride_a % 8 != 0 || a.stride_a == 0));
+  return c;
 }
-struct LoraScratch { int rb, u_cols, b_cols; size_t u, b, bytes; };
+// `rows` rows of K elements, element (row, k) at from + row * step_row + k * step_k of block row / rows_a_block, into rows of ld
+struct LoraCopy { const uint16_t* from; uint16_t* to; int64_t rows, rows_a_block, step_block, step_row, step_k; };
+struct LoraCopyJobs { LoraCopy job[3]; int n, K, ld; int64_t first_block[4]; };
+// A thread takes eight elements of a row; the rows of a block lie side by side where those are what is adjacent in memory ([K, N] weights).
+constexpr int COPY_THREADS = 256;
+__global__ void __launch_bounds__(COPY_THREADS) lora_copy_kernel(const __grid_constant__ LoraCopyJobs p) {
+  pdl_begin();
+  int j = 0;
+  while (j + 1 < p.n && (int64_t)blockIdx.x >= p.first_block[j + 1]) ++j;
+  const LoraCopy c = p.job[j];
+  const int64_t at = ((int64_t)blockIdx.x - p.first_block[j]) * COPY_THREADS + threadIdx.x;
+  const int pieces = p.ld / 8;
+  const int64_t row = c.step_k == 1 ? at / pieces : at % c.rows;
+  const int k0 = (int)(c.step_k == 1 ? at - row * pieces : at / c.rows) * 8;
+  if (row >= c.rows || k0 >= p.ld) return;
+  const int64_t block = row / c.rows_a_block;
+  const uint16_t* from = c.from + block * c.step_block + (row - block * c.rows_a_block) * c.step_row;
+  uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (k0 + i < p.K) w[i / 2] |= (uint32_t)__ldg(from + (k0 + i) * c.step_k) << (16 * (i & 1));
+  *reinterpret_cast<uint4*>(c.to + row * p.ld + k0) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// What the tensor-core path takes
+bool lora_umma_takes(const xb_lora_args& a) { return (a.dtype == XB_F16 || a.dtype == XB_BF16) && a.n_adapters >= 1 && a.r >= 1; }
+struct LoraScratch {
+  int rb, u_cols, b_cols;
+  int fused_group;                        // adapters of a walk where both steps are one kernel, 0 where they are two
+  size_t u, b, x, w, a, bytes;
+};
 LoraScratch lora_scratch(const xb_lora_args& a) {
   LoraScratch w;
   w.rb = a.r <= 16 ? 16 : a.r <= 32 ? 32 : a.r <= 64 ? 64 : 128;
@@ -799,32 +865,57 @@ LoraScratch lora_scratch(const xb_lora_args& a) {
   w.b_cols = std::max(w.rb, 32);
   w.u = 0;
   w.b = ((size_t)a.M * w.u_cols * 4 + 255) / 256 * 256;
-  w.bytes = w.b + (size_t)a.n_adapters * a.N * w.b_cols * 4;
+  // One column of tiles, and tensor memory for it and the U of an adapter twice: both steps in one kernel. (Two adapters a walk: a third would
+  // be a longer stage for every tile. Fewer tiles than half of the SMs become narrower ones, in two steps.)
+  const int whole_n = (a.N + 15) / 16 * 16;
+  w.fused_group = whole_n <= 256 && w.rb <= FUSED_MAX_RB && ((int64_t)a.M + BLOCK_M - 1) / BLOCK_M >= sm_count() / 2 ? std::min(2, (256 - whole_n) / w.rb) : 0;
+  const LoraCopies c = lora_copies(a);
+  auto rows = [&](bool copy, int64_t n) { return copy ? ((size_t)n * c.ld * 2 + 255) / 256 * 256 : 0; };
+  w.x = w.fused_group > 0 ? 0 : w.b + ((size_t)a.n_adapters * a.N * w.b_cols * 4 + 255) / 256 * 256;
+  w.w = w.x + rows(c.x, a.M);
+  w.a = w.w + rows(c.w, a.N);
+  w.bytes = w.a + rows(c.a, (int64_t)a.n_adapters * a.r);
   return w;
 }
 
-int run_umma(const xb_lora_args& a, uint8_t* ws, cudaStream_t stream) {
-  const LoraScratch w = lora_scratch(a);
+int run_umma(const xb_lora_args& given, uint8_t* ws, cudaStream_t stream) {
+  const LoraScratch w = lora_scratch(given);
+  xb_lora_args a = given;
+  if (const LoraCopies c = lora_copies(given); c.x || c.w || c.a) {
+    LoraCopyJobs jobs;
+    memset(&jobs, 0, sizeof(jobs));
+    jobs.K = a.K;
+    jobs.ld = (int)c.ld;
+    auto add = [&](const void* from, size_t to, int64_t rows, int64_t rows_a_block, int64_t step_block, int64_t step_row, int64_t step_k) {
+      jobs.job[jobs.n] = {static_cast<const uint16_t*>(from), reinterpret_cast<uint16_t*>(ws + to), rows, rows_a_block, step_block, step_row, step_k};
+      jobs.first_block[jobs.n + 1] = jobs.first_block[jobs.n] + (rows * (c.ld / 8) + COPY_THREADS - 1) / COPY_THREADS;
+      ++jobs.n;
+      return ws + to;
+    };
+    if (c.x) { a.X = add(a.X, w.x, a.M, a.M, 0, a.ldx, 1); a.ldx = c.ld; }
+    if (c.w) { a.W = add(a.W, w.w, a.N, a.N, 0, a.trans_w ? a.ldw : 1, a.trans_w ? 1 : a.ldw); a.ldw = c.ld; a.trans_w = 1; }
+    if (c.a) { a.A = add(a.A, w.a, (int64_t)a.n_adapters * a.r, a.r, a.stride_a, a.lda, 1); a.lda = c.ld; a.stride_a = c.ld * a.r; }
+    const int64_t blocks = jobs.first_block[jobs.n];
+    XB_REQUIRE(blocks < ((int64_t)1 << 31), XB_ERR_LIMIT, "xb_lora_gemm: %d rows of %d are too many for one call", a.M, a.K);
+    launch_dependent(lora_copy_kernel, (unsigned)blocks, COPY_THREADS, 0, stream, jobs);
+    if (int rc = check_launch("lora_copy_kernel")) return rc;
+  }
   const int bf16 = a.dtype == XB_BF16;
   LoraTiles l;
   memset(&l, 0, sizeof(l));
   l.M = a.M; l.N = a.N; l.K = a.K; l.r = a.r; l.n_adapters = a.n_adapters; l.rb = w.rb; l.u_cols = w.u_cols; l.b_cols = w.b_cols;
   l.adapter = a.adapter; l.scale = a.scale; l.U = reinterpret_cast<float*>(ws + w.u); l.B32 = reinterpret_cast<float*>(ws + w.b);
   l.B = a.B; l.ldb = a.ldb; l.stride_b = a.stride_b; l.dtype = a.dtype;
+  l.vec_b = a.r % 8 == 0 && a.ldb % 8 == 0 && a.stride_b % 8 == 0 && (reinterpret_cast<uintptr_t>(a.B) & 15) == 0;
   l.group = std::max(1, SHRINK_GROUP_ROWS / l.rb);
   l.tiles_m = (a.M + BLOCK_M - 1) / BLOCK_M;
   l.idesc_a = umma::make_idesc(BLOCK_M, 0, bf16);          // (the columns are the pass's)
   CUtensorMap mx, ma;
   if (int rc = make_map(&mx, a.X, bf16, a.K, a.M, a.ldx, 1, 0, BLOCK_M, BLOCK_K, CU_TENSOR_MAP_SWIZZLE_128B, 1, CU_TENSOR_MAP_L2_PROMOTION_L2_256B)) return rc;
   if (int rc = make_map(&ma, a.A, bf16, a.K, a.r, a.lda, a.n_adapters, a.stride_a, l.rb)) return rc;
-  // One column of tiles, and tensor memory for it and the U of an adapter twice: both steps in one kernel.
-  const int whole_n = (a.N + 15) / 16 * 16, fused_group = whole_n <= 256 ? std::min(SHRINK_GROUP, (256 - whole_n) / l.rb) : 0;
-  const bool fused = fused_group >= 1 && l.rb <= 64 && l.tiles_m >= sm_count() / 2;
+  const bool fused = w.fused_group > 0;
   if (fused) {
-    l.group = fused_group;
-    const int64_t quads = (int64_t)l.n_adapters * l.N * (l.b_cols / 4);
-    launch_dependent(lora_widen_kernel, (unsigned)std::min<int64_t>((quads + 127) / 128, 8 * sm_count()), 128, 0, stream, l);
-    if (int rc = check_launch("lora_widen_kernel")) return rc;
+    l.group = w.fused_group;
   } else {
     const int stage = A_STAGE_BYTES + l.group * l.rb * BLOCK_K * 2;
     l.stages = std::min(MAX_STAGES, 220 * 1024 / stage);
@@ -855,16 +946,23 @@ int run_umma(const xb_lora_args& a, uint8_t* ws, cudaStream_t stream) {
   CUtensorMap m[5];
   m[0] = mx;
   if (int rc = p.b_mn ? make_map(&m[1], a.W, bf16, a.N, a.K, a.ldw, 1, 0, BLOCK_K) : make_map(&m[1], a.W, bf16, a.K, a.N, a.ldw, 1, 0, p.block_n)) return rc;
-  if (fused) m[2] = ma;
-  else if (int rc = make_map_f32(&m[2], l.U, l.u_cols, a.M, 1, BLOCK_M)) return rc;
-  if (int rc = make_map_f32(&m[3], l.B32, l.b_cols, a.N, a.n_adapters, p.block_n)) return rc;
+  if (fused) {
+    m[2] = m[3] = ma;
+  } else {
+    if (int rc = make_map_f32(&m[2], l.U, l.u_cols, a.M, 1, BLOCK_M)) return rc;
+    if (int rc = make_map_f32(&m[3], l.B32, l.b_cols, a.N, a.n_adapters, p.block_n)) return rc;
+  }
   m[4] = m[0];
   const int64_t es = a.y_dtype == XB_F32 ? 4 : 2;
   int y = LORA_Y_ANY, tail = 4 * 256 * (int)sizeof(float) + EPI_WARPS * EPI_STAGE_BYTES;
   p.y_unit = 16; p.y_bufs = 1;
+  const int stage = A_STAGE_BYTES + (p.b_mn ? (p.block_n + 63) / 64 * 64 : p.block_n) * BLOCK_K * 2 + (fused ? l.group * l.rb * BLOCK_K * 2 : 0);
+  const int operands = fused ? l.u_cols / 32 * A_STAGE_BYTES + p.block_n * 128 : 0;          // of U B^T
   if (es == 2 && (reinterpret_cast<uintptr_t>(a.Y) & 15) == 0 && a.ldy % 8 == 0 && a.N % 8 == 0) {
     // copies of 32 columns, 16 where the tile has few or where 32 would reach into the next tile
     p.y_unit = p.block_n >= 128 && (p.block_n % 32 == 0 || p.tiles_n == 1) ? 32 : 16;
+    if (fused && (SMEM_BUDGET - 4096 - operands - EPI_WARPS * 32 * 64) / stage < std::min(MAX_STAGES, (SMEM_BUDGET - 4096 - operands - EPI_WARPS * 16 * 64) / stage))
+      p.y_unit = 16;                      // (a stage more)
     p.y_bufs = 1;                         // (a second would cost a stage of the ring)
     if (make_map(&m[4], a.Y, a.y_dtype == XB_BF16, a.N, a.M, a.ldy, 1, 0, 32, p.y_unit,
                  p.y_unit == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B) == 0) {
@@ -872,8 +970,7 @@ int run_umma(const xb_lora_args& a, uint8_t* ws, cudaStream_t stream) {
       tail = 4 * 256 * (int)sizeof(float) + EPI_WARPS * p.y_bufs * p.y_unit * 64;
     }
   }
-  const int stage = A_STAGE_BYTES + (p.b_mn ? (p.block_n + 63) / 64 * 64 : p.block_n) * BLOCK_K * 2 + (fused ? l.group * l.rb * BLOCK_K * 2 : 0);
-  if (fused) tail += l.u_cols / 32 * A_STAGE_BYTES;
+  tail += operands;
   p.stages = std::max(2, std::min(MAX_STAGES, (SMEM_BUDGET - tail) / stage));
   const size_t smem = (size_t)p.stages * stage + tail + 1024;
   const unsigned grid = (unsigned)std::min<int64_t>(total, sm_count());
