@@ -3,6 +3,7 @@
 #include <cstring>
 
 #include "xb_common.cuh"
+#include "xb_lora_rows.cuh"
 #include "xb_lora_umma.cuh"
 
 namespace xb {
@@ -11,25 +12,6 @@ int gemm_half_sums(const xb_gemm_args& a, cudaStream_t stream);
 
 namespace {
 
-constexpr int LORA_MAX_RANK = 128;
-
-struct LoraParams {
-  int M, N, K, r, n_adapters;
-  const void* X; int64_t ldx;
-  const void* A; int64_t lda, stride_a;
-  const void* B; int64_t ldb, stride_b;
-  const float* scale;
-  const float* bias;
-  const int32_t* adapter;
-  float* U;                               // [M, r]: scale[a] X[m] A[a]^T
-  float* part;                            // [M, N]: bias + U[m] B[a]^T
-};
-
-// the adapter of row m, -1 where it has none (n_adapters is 0 where the call has none: then `adapter` may be null)
-__device__ __forceinline__ int adapter_of(const LoraParams& p, int m) {
-  const int a = p.n_adapters > 0 ? p.adapter[m] : -1;
-  return a >= 0 && a < p.n_adapters ? a : -1;
-}
 
 // V adjacent elements as fp32: one load where they lie aligned, which V > 1 says
 template <typename T, int V>
@@ -59,7 +41,10 @@ __global__ void __launch_bounds__(128) lora_rows_shrink_kernel(const LoraParams 
   const int a = adapter_of(p, m);
   if (a < 0) return;
   const T* x = reinterpret_cast<const T*>(p.X) + (int64_t)m * p.ldx;
-  const T* at = reinterpret_cast<const T*>(p.A) + (int64_t)a * p.stride_a + (int64_t)j0 * p.lda;
+  // (rows of A past the last are the last again, and what they give is dropped: a branch would keep the loads of a round from the next's)
+  const T* at[SHRINK_J];
+#pragma unroll
+  for (int j = 0; j < SHRINK_J; ++j) at[j] = reinterpret_cast<const T*>(p.A) + (int64_t)a * p.stride_a + (int64_t)min(j0 + j, p.r - 1) * p.lda;
   float s[SHRINK_J] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
   for (int k = lane * V; k < p.K; k += 32 * V) {         // (V > 1: whole pieces, K is a multiple of V)
@@ -67,9 +52,8 @@ __global__ void __launch_bounds__(128) lora_rows_shrink_kernel(const LoraParams 
     load_piece<T, V>(x + k, xv);
 #pragma unroll
     for (int j = 0; j < SHRINK_J; ++j) {
-      if (j0 + j >= p.r) break;
       float av[V];
-      load_piece<T, V>(at + (int64_t)j * p.lda + k, av);
+      load_piece<T, V>(at[j] + k, av);
 #pragma unroll
       for (int v = 0; v < V; ++v) s[j] = fmaf(xv[v], av[v], s[j]);
     }
@@ -140,7 +124,8 @@ __global__ void __launch_bounds__(128) lora_rows_expand_kernel(const LoraParams 
 }
 
 // Few rows: the tiles would leave most SMs idle, and a tile of many adapters walks through all of them.
-bool takes_tiles(const xb_lora_args& a) { return a.M >= 512 && lora_umma_takes(a); }
+constexpr int ROWS_MOST = 511;
+bool takes_tiles(const xb_lora_args& a) { return a.M > ROWS_MOST && lora_umma_takes(a); }
 
 constexpr size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
@@ -165,6 +150,16 @@ int check_args(const xb_lora_args* a) {
   XB_REQUIRE(!adapters || (a->lda >= a->K && a->ldb >= a->r && a->stride_a >= 0 && a->stride_b >= 0), XB_ERR_ARG,
              "xb_lora_gemm: a stride of the adapters is too small");
   return 0;
+}
+
+template <typename T>
+int launch_shrink(const LoraParams& p, bool vec, cudaStream_t s) {
+  if (p.n_adapters == 0) return 0;
+  const int64_t warps = (int64_t)p.M * ((p.r + SHRINK_J - 1) / SHRINK_J);
+  XB_REQUIRE(warps < ((int64_t)1 << 32), XB_ERR_LIMIT, "xb_lora_gemm: %d rows of rank %d are too many for one call", p.M, p.r);
+  if (vec) launch_dependent(lora_rows_shrink_kernel<T, 16 / (int)sizeof(T)>, (unsigned)((warps + 3) / 4), 128, 0, s, p);
+  else launch_dependent(lora_rows_shrink_kernel<T, 1>, (unsigned)((warps + 3) / 4), 128, 0, s, p);
+  return check_launch("lora_rows_shrink_kernel");
 }
 
 template <typename T>
@@ -203,17 +198,30 @@ int run_rows(const xb_lora_args& a, uint8_t* ws, cudaStream_t s) {
   g.N = a.N; g.K = a.K; g.trans_b = a.trans_w; g.alpha = g.beta = 1.f; g.batch = 1;
   g.lda = a.ldx; g.B = a.W; g.ldb = a.ldw; g.ldy = a.ldy; g.ab_dtype = a.dtype; g.y_dtype = a.y_dtype;
   g.bias = p.part; g.ldbias = a.N; g.bias_kind = XB_BIAS_FULL; g.bias_dtype = XB_F32;
+  if constexpr (sizeof(T) == 2) {
+    // one turn of rows whose operands lie on 16 bytes: the projection and the products with B in one kernel
+    auto lies = [](const void* q, int64_t ld) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0 && ld % 8 == 0; };
+    if (a.M <= ROWS_MOST && lies(a.X, a.ldx) && lies(a.W, a.ldw)) {
+      p.M = a.M;
+      p.X = a.X;
+      p.adapter = p.n_adapters ? a.adapter : nullptr;
+      if (int rc = launch_shrink<T>(p, vec_k, s)) return rc;
+      LoraRowsParams r;
+      r.l = p;
+      r.W = a.W; r.ldw = a.ldw; r.Y = a.Y; r.ldy = a.ldy;
+      r.y_f32 = a.y_dtype == XB_F32; r.vec_r = vec_r;
+      const int64_t tiles = ((int64_t)a.N + ROWS_BN - 1) / ROWS_BN * ((a.M + ROWS_BM - 1) / ROWS_BM);
+      const int slices = (a.K + ROWS_BK - 1) / ROWS_BK;
+      r.split = 1;
+      while (r.split < 8 && 2 * r.split <= slices && tiles * 2 * r.split <= 2 * sm_count()) r.split *= 2;
+      return a.trans_w ? launch_rows_gemm<T, true>(r, s) : launch_rows_gemm<T, false>(r, s);
+    }
+  }
   for (int64_t m0 = 0; m0 < a.M; m0 += turn) {
     p.M = (int)std::min<int64_t>(turn, a.M - m0);
     p.X = reinterpret_cast<const T*>(a.X) + m0 * a.ldx;
     p.adapter = p.n_adapters ? a.adapter + m0 : nullptr;
-    if (p.n_adapters) {
-      const int64_t warps = (int64_t)p.M * ((p.r + SHRINK_J - 1) / SHRINK_J);
-      XB_REQUIRE(warps < ((int64_t)1 << 32), XB_ERR_LIMIT, "xb_lora_gemm: %d rows of rank %d are too many for one call", p.M, p.r);
-      if (vec_k) launch_dependent(lora_rows_shrink_kernel<T, 16 / (int)sizeof(T)>, (unsigned)((warps + 3) / 4), 128, 0, s, p);
-      else launch_dependent(lora_rows_shrink_kernel<T, 1>, (unsigned)((warps + 3) / 4), 128, 0, s, p);
-      if (int rc = check_launch("lora_rows_shrink_kernel")) return rc;
-    }
+    if (int rc = launch_shrink<T>(p, vec_k, s)) return rc;
     if (int rc = launch_expand<T>(p, vec_r, s)) return rc;
     g.M = p.M;
     g.A = p.X;

@@ -1,0 +1,197 @@
+// The projection and U B^T for few rows: one kernel of warp-level matrix instructions (included by xb_lora.cu).
+#pragma once
+
+#include "xb_common.cuh"
+#include "xb_mma_half.cuh"
+#include "xb_umma.cuh"
+
+namespace xb {
+namespace {
+
+constexpr int LORA_MAX_RANK = 128;
+
+struct LoraParams {
+  int M, N, K, r, n_adapters;
+  const void* X; int64_t ldx;
+  const void* A; int64_t lda, stride_a;
+  const void* B; int64_t ldb, stride_b;
+  const float* scale;
+  const float* bias;
+  const int32_t* adapter;
+  float* U;                               // [M, r]: scale[a] X[m] A[a]^T
+  float* part;                            // [M, N]: bias + U[m] B[a]^T
+};
+
+// the adapter of row m, -1 where it has none (n_adapters is 0 where the call has none: then `adapter` may be null)
+__device__ __forceinline__ int adapter_of(const LoraParams& p, int m) {
+  const int a = p.n_adapters > 0 ? p.adapter[m] : -1;
+  return a >= 0 && a < p.n_adapters ? a : -1;
+}
+
+// Y = X W + bias + U B_a^T for tiles of 64 rows x 32 columns. With few tiles a cluster of `split` CTAs shares one, each with its part of the
+// depth: all of what it reads is on its way at once, it makes its own products with B meanwhile, and the partial sums are added out
+// of one another's shared memory, every CTA for its share of the rows. Sums as in gemm_half_kernel: 16 products by a matrix
+// instruction, added in fp32. What bounds it is the latency of one round to memory, the exchange and the launch.
+// [64, 1280] x [1280, 1024], 64 adapters of rank 16: 12 us less than xb_gemm with a bias matrix, and the kernel that made that.
+constexpr int ROWS_BM = 64, ROWS_BN = 32, ROWS_BK = 320, ROWS_THREADS = 256;
+constexpr int ROWS_XPITCH = ROWS_BK + 8, ROWS_WPITCH = ROWS_BN + 8;          // halves: no bank conflicts of the eight rows that are read together
+constexpr int ROWS_X_BYTES = ROWS_BM * ROWS_XPITCH * 2;
+constexpr int ROWS_W_BYTES = ROWS_BK * ROWS_WPITCH * 2;                      // (as [K, N]; the other form is smaller)
+constexpr int ROWS_SMEM = ROWS_X_BYTES + ROWS_W_BYTES + ROWS_BM * ROWS_BN * 4;
+static_assert(ROWS_BN * ROWS_XPITCH * 2 <= ROWS_W_BYTES, "both forms of W fit the same space");
+
+struct LoraRowsParams {
+  LoraParams l;
+  const void* W; int64_t ldw;
+  void* Y; int64_t ldy;
+  int split;                              // CTAs of a tile
+  int y_f32, vec_r;
+};
+
+// 16 bytes of which the first `bytes` exist (the rest becomes zeros)
+__device__ __forceinline__ void cp_async16_part(void* dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(umma::smem_u32(dst)), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr, uint32_t rank) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(umma::cluster_addr(addr, rank)) : "memory");
+  return v;
+}
+
+template <typename T, bool TRANS_W>
+__global__ void __launch_bounds__(ROWS_THREADS) lora_rows_gemm_kernel(const __grid_constant__ LoraRowsParams p) {
+  pdl_begin();
+  constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+  extern __shared__ __align__(16) uint8_t rows_smem[];
+  uint16_t* xs = reinterpret_cast<uint16_t*>(rows_smem);
+  uint16_t* ws = reinterpret_cast<uint16_t*>(rows_smem + ROWS_X_BYTES);
+  float* part = reinterpret_cast<float*>(rows_smem + ROWS_X_BYTES + ROWS_W_BYTES);       // [64][32]
+  const int rank = blockIdx.x % p.split, m0 = blockIdx.y * ROWS_BM, n0 = (int)(blockIdx.x / p.split) * ROWS_BN;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const LoraParams& l = p.l;
+  // this CTA's part of the depth, whole slices of ROWS_BK
+  const int slices = (l.K + ROWS_BK - 1) / ROWS_BK, per = (slices + p.split - 1) / p.split, s0 = rank * per, s1 = min(slices, s0 + per);
+
+  auto bring = [&](int slice) {
+    const int k0 = slice * ROWS_BK, depth = min(ROWS_BK, l.K - k0), wide = (depth + 15) / 16 * 2;     // pieces of 8, up to whole steps of 16
+    const T* X = reinterpret_cast<const T*>(l.X);
+    const T* W = reinterpret_cast<const T*>(p.W);
+    for (int e = tid; e < ROWS_BM * wide; e += ROWS_THREADS) {
+      const int r = e / wide, c = (e - r * wide) * 8, in = m0 + r < l.M ? max(0, min(8, depth - c)) * 2 : 0;
+      cp_async16_part(xs + r * ROWS_XPITCH + c, X + (in ? (int64_t)(m0 + r) * l.ldx + k0 + c : 0), in);
+    }
+    if (TRANS_W) {
+      for (int e = tid; e < ROWS_BN * wide; e += ROWS_THREADS) {
+        const int r = e / wide, c = (e - r * wide) * 8, in = n0 + r < l.N ? max(0, min(8, depth - c)) * 2 : 0;
+        cp_async16_part(ws + r * ROWS_XPITCH + c, W + (in ? (int64_t)(n0 + r) * p.ldw + k0 + c : 0), in);
+      }
+    } else {
+      for (int e = tid; e < wide * 8 * (ROWS_BN / 8); e += ROWS_THREADS) {
+        const int r = e / (ROWS_BN / 8), c = e % (ROWS_BN / 8) * 8, in = r < depth ? max(0, min(8, l.N - n0 - c)) * 2 : 0;
+        cp_async16_part(ws + r * ROWS_WPITCH + c, W + (in ? (int64_t)(k0 + r) * p.ldw + n0 + c : 0), in);
+      }
+    }
+    umma::cp_async_commit();
+  };
+  if (s0 < s1) bring(s0);
+
+  // the outputs that this thread ends with: OUT rows of one column; bias and U B^T for them
+  const int share = ROWS_BM / p.split, first = rank * share, col = n0 + lane, step = ROWS_THREADS / 32;
+  constexpr int OUT = ROWS_BM / (ROWS_THREADS / 32);
+  float out[OUT];
+#pragma unroll
+  for (int i = 0; i < OUT; ++i) out[i] = 0.f;
+  if (col < l.N) {
+    const float bias = l.bias ? l.bias[col] : 0.f;
+#pragma unroll
+    for (int i = 0; i < OUT; ++i) {
+      const int m = m0 + first + warp + i * step;
+      if (warp + i * step >= share || m >= l.M) continue;
+      const int a = adapter_of(l, m);
+      float sum = 0.f;
+      if (a >= 0) {
+        const T* b = reinterpret_cast<const T*>(l.B) + (int64_t)a * l.stride_b + (int64_t)col * l.ldb;
+        const float* u = l.U + (int64_t)m * l.r;
+        if (p.vec_r) {
+#pragma unroll 2
+          for (int j = 0; j < l.r; j += 8) {
+            const uint4 t = __ldg(reinterpret_cast<const uint4*>(b + j));
+            const T* e = reinterpret_cast<const T*>(&t);
+            const float4 u0 = *reinterpret_cast<const float4*>(u + j), u1 = *reinterpret_cast<const float4*>(u + j + 4);
+            const float uv[8] = {u0.x, u0.y, u0.z, u0.w, u1.x, u1.y, u1.z, u1.w};
+#pragma unroll
+            for (int k = 0; k < 8; ++k) sum = fmaf(uv[k], to_f32<T>(e[k]), sum);
+          }
+        } else {
+          for (int j = 0; j < l.r; ++j) sum = fmaf(u[j], to_f32<T>(b[j]), sum);
+        }
+      }
+      out[i] = bias + sum;
+    }
+  }
+
+  // 4 x 2 warps of 16 x 16 outputs
+  const int wm = (warp >> 1) * 16, wn = (warp & 1) * 16, l8 = lane & 7, g1 = (lane >> 3) & 1, g2 = lane >> 4;
+  const uint32_t x_at = umma::smem_u32(xs) + 2 * ((wm + g1 * 8 + l8) * ROWS_XPITCH + g2 * 8);
+  const uint32_t w_at = umma::smem_u32(ws) + 2 * (TRANS_W ? (wn + g2 * 8 + l8) * ROWS_XPITCH + g1 * 8 : (g1 * 8 + l8) * ROWS_WPITCH + wn + g2 * 8);
+  float acc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+  for (int s = s0; s < s1; ++s) {
+    umma::cp_async_wait_all();
+    __syncthreads();
+    const int depth = min(ROWS_BK, l.K - s * ROWS_BK);
+#pragma unroll 4
+    for (int k = 0; k < depth; k += 16) {
+      uint32_t af[4], bf[4];
+      ldmatrix4<0>(af, x_at + 2 * k);
+      ldmatrix4<TRANS_W ? 0 : 1>(bf, w_at + 2 * (TRANS_W ? k : k * ROWS_WPITCH));
+      mma_half<BF16>(acc[0], af, bf[0], bf[1]);
+      mma_half<BF16>(acc[1], af, bf[2], bf[3]);
+    }
+    __syncthreads();
+    if (s + 1 < s1) bring(s + 1);
+  }
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      *reinterpret_cast<float2*>(part + (wm + 8 * h + (lane >> 2)) * ROWS_BN + wn + 8 * j + 2 * (lane & 3)) = make_float2(acc[j][2 * h], acc[j][2 * h + 1]);
+  if (p.split > 1) umma::cluster_sync();
+  else __syncthreads();
+  if (col < l.N) {
+#pragma unroll
+    for (int i = 0; i < OUT; ++i) {
+      const int r = warp + i * step, m = m0 + first + r;
+      if (r >= share || m >= l.M) continue;
+      const uint32_t at = umma::smem_u32(part + (first + r) * ROWS_BN + lane);
+      float v = 0.f;
+      if (p.split > 1) {
+        for (int c = 0; c < p.split; ++c) v += ld_cluster_f32(at, (uint32_t)c);
+      } else {
+        v = part[(first + r) * ROWS_BN + lane];
+      }
+      v += out[i];
+      if (p.y_f32) reinterpret_cast<float*>(p.Y)[(int64_t)m * p.ldy + col] = v;
+      else reinterpret_cast<T*>(p.Y)[(int64_t)m * p.ldy + col] = from_f32<T>(v);
+    }
+  }
+  if (p.split > 1) umma::cluster_sync();               // nobody leaves while its sums may be read
+}
+
+template <typename T, bool TRANS_W>
+int launch_rows_gemm(const LoraRowsParams& p, cudaStream_t s) {
+  static PerDeviceOnce attr_set;          // per instantiation
+  XB_SET_MAX_SMEM_ONCE(attr_set, ROWS_SMEM, (const void*)lora_rows_gemm_kernel<T, TRANS_W>);
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = (unsigned)p.split; at[1].val.clusterDim.y = 1; at[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((p.l.N + ROWS_BN - 1) / ROWS_BN * p.split), (unsigned)((p.l.M + ROWS_BM - 1) / ROWS_BM));
+  cfg.blockDim = ROWS_THREADS; cfg.dynamicSmemBytes = ROWS_SMEM; cfg.stream = s; cfg.attrs = at; cfg.numAttrs = p.split > 1 ? 2 : 1;
+  cudaLaunchKernelEx(&cfg, lora_rows_gemm_kernel<T, TRANS_W>, p);
+  return check_launch("lora_rows_gemm_kernel");
+}
+
+}  // namespace
+}  // namespace xb
