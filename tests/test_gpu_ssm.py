@@ -148,7 +148,8 @@ def test_scan(dtype, lists, D, N, groups, pad, skew):
 @pytest.mark.parametrize("dtype,lists,D,N,groups", [
     ("f32", (1, 9000), 8, 16, 1), ("f32", (2, 3001), 40, 16, 1), ("bf16", [5000, 1, 0, 700, 3, 2500, 0], 72, 16, 1),
     ("f16", [1] * 300 + [2000] + [0, 7] * 40, 36, 8, 1), ("f32", [0, 0, 2049, 4096, 31], 18, 64, 2), ("f32", [4000], 130, 4, 1),
-    ("bf16", (40, 200), 136, 16, 1), ("f16", (700, 20), 72, 16, 1), ("f32", [900, 10] * 20, 33, 13, 1)], ids=str)
+    ("f32", [int(n) for n in np.random.default_rng(8).integers(0, 41, 900)] + [301], 24, 16, 1),
+    ("bf16", (40, 200), 136, 16, 1), ("f16", (700, 20), 72, 16, 1), ("f32", [900, 10] * 20, 33, 13, 1)], ids=lambda v: str(v)[:40])
 @pytest.mark.parametrize("longest", [True, False])
 def test_scan_of_long_and_many_lists(dtype, lists, D, N, groups, longest):
     _check_scan(dtype, lists, D, N, groups, 0, 0, longest)

@@ -242,27 +242,33 @@ ScanPlan scan_plan(const xb_ssm_scan_args& a) {
   const double sms = std::max(sm_count(), 1), mean = (double)a.rows / a.batch;
   const double longest = !a.offsets ? mean : (double)(a.longest > 0 ? std::min(a.longest, a.rows) : a.rows);
   // Cycles: a row of a block takes `work` of a full SM and `alone` where its SM has little else, which is what the longest list (or
-  // chunk) ends with. Lists that are split are walked nearly twice; of lists of all lengths the share in ones above `chunk` rows is
-  // that of an exponential distribution. us, whole lists and the best split: 256 lists of up to 1860 rows in 70000, D = 256 241,
-  // 230; 16 of up to 3640 in 16384, D = 512 246, 128; one of 4096, D = 1024 302, 70; 300 of 100, D = 256 67, 124.
+  // chunk) ends with; a block begins with 600 of them, one of the two walks of a chunk with 2000. Lists that are split are walked nearly twice; of lists of all lengths the share in ones above
+  // `chunk` rows is that of an exponential distribution. us, whole lists as they come, long ones first, the best split: 256 lists of
+  // up to 1860 rows in 70000, D = 256 229, 193, 226; 1000 in 20000, D = 256 68, 54; 16 of up to 3640 in 16384, D = 512 246 and 125 split;
+  // one of 4096, D = 1024 302 and 68; 300 of 100, D = 256 65 and 124.
   double best = 0;
   for (int K : {1, 2}) {
     if (K == 1 && p.lanes > 4) continue;  // (a block would have 16 channels or fewer)
-    const double work = K == 2 ? 155 : 80, alone = K == 2 ? 260 : 130;
-    const double full = (double)a.rows * scan_blocks(a, p.lanes, K) * work / sms, whole = full + 0.6 * alone * longest;
-    if (best == 0 || whole < best) { best = whole; p.K = K; p.chunk = 0; }
-    for (int64_t chunk = 64; chunk < longest; chunk *= 2) {
+    const double work = K == 2 ? 155 : 80, alone = K == 1 ? 130 : p.lanes <= 4 ? 260 : 32 * p.lanes;
+    const int blocks = scan_blocks(a, p.lanes, K);
+    const double full = (double)a.rows * blocks * work / sms;
+    // lists of unlike lengths in more than a wave of blocks: long ones first
+    const bool order = a.offsets && longest > 1.5 * mean && (double)a.batch * blocks > 5 * sms;
+    const double whole = (order ? std::max(full + 6000, alone * longest) : full + 0.6 * alone * longest) + 600.0 * a.batch * blocks / sms;
+    if (best == 0 || whole < best) { best = whole; p.K = K; p.chunk = 0; p.order = order; }
+    for (int64_t chunk = 64; chunk < longest; chunk += chunk & (chunk - 1) ? chunk / 3 : chunk / 2) {      // 64, 96, 128, 192, ...
       const double twice = longest > 1.5 * mean ? (1 + chunk / mean) * std::exp(-chunk / mean) : 1;
-      const double split = full * (1 + 0.8 * twice) + 1.2 * alone * chunk + 20000;
-      if (split < best) { best = split; p.K = K; p.chunk = chunk; }
+      const double split = full * (1 + 0.8 * twice) + 1.2 * alone * chunk + 4000 * (a.rows / (double)chunk + a.batch) * blocks / sms + 15000;
+      if (split < best) { best = split; p.K = K; p.chunk = chunk; p.order = false; }
     }
   }
   return p;
 }
 constexpr size_t align256(size_t n) { return (n + 255) / 256 * 256; }
-struct ScanScratch { size_t end, first, steps, kind, bytes; };
+struct ScanScratch { size_t end, first, steps, kind, bytes; };      // (a plan has chunks or an order, whose place is the first)
 ScanScratch scan_scratch(const xb_ssm_scan_args& a, const ScanPlan& p) {
   ScanScratch w = {};
+  if (p.order) w.bytes = align256((size_t)a.batch * 4);
   if (p.chunk == 0 || a.rows / p.chunk == 0) return w;
   const size_t n = (size_t)(a.rows / p.chunk), states = align256(n * a.D * a.N * 4);
   w.first = w.end + states;
@@ -280,12 +286,13 @@ ScanParams scan_params(const xb_ssm_scan_args& a, const ScanPlan& plan, uint8_t*
   p.lists = lists_of(a.offsets, a.slots, a.rows, a.batch, a.n_slots);
   p.D = a.D; p.N = a.N; p.per_group = a.D / a.groups; p.groups = a.groups; p.softplus = a.softplus;
   const int64_t size = (int64_t)dtype_size(a.dtype);
-  p.vec = whole(a.x, a.ldx * size, 16) && whole(a.delta, a.lddelta * size, 16) && whole(a.y, a.ldy * size, 16) &&
-          (!a.z || whole(a.z, a.ldz * size, 16)) && (a.groups == 1 || p.per_group * size % 16 == 0);
+  p.vec = whole(a.x, a.ldx * size, 4 * size) && whole(a.delta, a.lddelta * size, 4 * size) && whole(a.y, a.ldy * size, 4 * size) &&
+          (!a.z || whole(a.z, a.ldz * size, 4 * size)) && (a.groups == 1 || p.per_group % 4 == 0);
   p.vec_bc = a.N % 4 == 0 && whole(a.B, a.ldb * size, 4 * size) && whole(a.C, a.ldc * size, 4 * size);
   p.vec_h = a.N % 4 == 0 && whole(a.A, 0, 16) && whole(a.h_in, 0, 16) && whole(a.h_out, 0, 16);
   const ScanScratch w = scan_scratch(a, plan);
-  if (w.bytes) {
+  if (plan.order) p.order = reinterpret_cast<int*>(ws);
+  if (plan.chunk > 0 && w.bytes) {
     p.chunk = plan.chunk; p.n_ends = (int)(a.rows / plan.chunk);
     p.end = reinterpret_cast<float*>(ws + w.end); p.first = reinterpret_cast<float*>(ws + w.first);
     p.steps = reinterpret_cast<float*>(ws + w.steps); p.kind = reinterpret_cast<int*>(ws + w.kind);

@@ -63,7 +63,7 @@ struct ScanParams {
   const float* h_in; float* h_out;
   Lists lists;
   int D, N, per_group, groups, softplus;
-  int vec, vec_bc, vec_h;                 // rows of x, delta, z, y in whole 16-byte pieces; B and C in pieces of four; states and A in float4
+  int vec, vec_bc, vec_h;                 // rows of x, delta, z, y in whole pieces of four; B and C in pieces of four; states and A in float4
   // lists walked in chunks (0: whole): see xb_ssm_scan.cuh
   int64_t chunk;
   int n_ends;                             // rows / chunk
@@ -71,6 +71,7 @@ struct ScanParams {
   float* first;                           // [n_ends][D][N]: copies of the states that lists of several chunks begin with
   float* steps;                           // [n_ends][D]: sum of the chunk's steps
   int* kind;                              // [n_ends]: 0 no such chunk, 1 its list's first, 2 another
+  int* order;                             // [batch]: the lists, long ones first; null: as they come
 };
 
 // What a scan runs as.
@@ -78,6 +79,7 @@ struct ScanPlan {
   bool step;                              // one row a list
   int lanes, K;                           // lanes of a channel; channels of a lane
   int64_t chunk;                          // lists of more rows are split (0: none)
+  bool order;                             // whole lists, long ones first
 };
 // the scan of one type (xb_ssm_scan_*.cu)
 int ssm_scan_f32(const ScanParams& p, const ScanPlan& plan, cudaStream_t s);

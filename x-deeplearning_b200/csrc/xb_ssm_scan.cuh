@@ -146,16 +146,17 @@ struct ScanShape {
   static constexpr int R = 4 / K;                       // rows that a lane walks at a time
 };
 
-// Tiles of ROWS rows x CH channels: the threads bring x and delta (16-byte pieces, those of the next tile while this one is walked), leave
+// Tiles of ROWS rows x CH channels: the threads bring x and delta (pieces of four, those of the next tile while this one is walked), leave
 // the steps d and x in shared memory as fp32 and B and C beside them, walk the rows, leave the sums there too, and write y. Every
 // exponential, softplus and sigmoid is an SFU instruction: N + 4 for a row and channel, 16 a clock and SM.
-constexpr int SCAN_BLOCKS = 6;            // of an SM: the registers are shared among so many
+template <int K>
+constexpr int SCAN_BLOCKS = K == 1 ? 5 : 6;            // of an SM: the registers are shared among so many
 template <typename T, int LPC, int K, int MODE>
-__global__ void __launch_bounds__(SCAN_THREADS, SCAN_BLOCKS) ssm_scan_kernel(const ScanParams p, int blocks_a_group) {
+__global__ void __launch_bounds__(SCAN_THREADS, SCAN_BLOCKS<K>) ssm_scan_kernel(const ScanParams p, int blocks_a_group) {
   pdl_begin();
   using S = ScanShape<LPC, K>;
   constexpr int CH = S::CH, ROWS = S::ROWS, E = S::E, R = S::R, NP = SPL * LPC;
-  constexpr int V = min_c(E, 16 / (int)sizeof(T)), VPR = CH / V, RPI = SCAN_THREADS / VPR, IT = E / V;
+  constexpr int V = min_c(E, 4), VPR = CH / V, RPI = SCAN_THREADS / VPR, IT = E / V;
   static_assert(VPR <= SCAN_THREADS && IT * RPI == ROWS && VPR * V == CH, "");
   constexpr int BC = 2 * ROWS * LPC, IT_BC = (BC + SCAN_THREADS - 1) / SCAN_THREADS;      // pieces of four of B and of C
   __shared__ struct { __align__(16) float d[ROWS][CH], x[ROWS][CH], y[ROWS][CH], b[2][ROWS][NP], bias[CH], skip[CH]; } sm;
@@ -164,7 +165,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, SCAN_BLOCKS) ssm_scan_kernel(con
   const int g = cb / blocks_a_group, c_lo = g * p.per_group + (cb - g * blocks_a_group) * CH, c_hi = min((g + 1) * p.per_group, c_lo + CH);
 
   // the list and the rows of it
-  int list = unit, part = 0;
+  int list = p.order ? p.order[unit] : unit, part = 0;
   if (p.chunk > 0) {
     if (MODE == SCAN_WALK) {
       list = p.lists.of_chunk(unit, p.chunk, lane);
@@ -425,6 +426,36 @@ __global__ void __launch_bounds__(SCAN_THREADS, SCAN_BLOCKS) ssm_scan_kernel(con
   }
 }
 
+// The lists with long ones first, by classes of length (a quarter of a power of two each): the blocks of a launch start in this order, and a
+// long list that starts last keeps a few SMs busy while the others have nothing left. Within a class the order is any; results do
+// not depend on it.
+__global__ void __launch_bounds__(1024) ssm_order_kernel(const ScanParams p) {
+  pdl_begin();
+  constexpr int CLASSES = 33 * 4;
+  __shared__ int s_at[CLASSES];
+  const int tid = threadIdx.x;
+  auto class_of = [&](int i) {
+    const int64_t n = p.lists.begin(i + 1) - p.lists.begin(i);
+    const unsigned len = n > 0 ? (unsigned)n : 0u;
+    const int zeros = __clz(len);
+    return len ? zeros * 4 + 3 - (int)(((len << zeros) >> 29) & 3u) : CLASSES - 1;
+  };
+  for (int c = tid; c < CLASSES; c += 1024) s_at[c] = 0;
+  __syncthreads();
+  for (int i = tid; i < p.lists.batch; i += 1024) atomicAdd(&s_at[class_of(i)], 1);
+  __syncthreads();
+  if (tid == 0) {
+    int sum = 0;
+    for (int c = 0; c < CLASSES; ++c) {
+      const int n = s_at[c];
+      s_at[c] = sum;
+      sum += n;
+    }
+  }
+  __syncthreads();
+  for (int i = tid; i < p.lists.batch; i += 1024) p.order[atomicAdd(&s_at[class_of(i)], 1)] = i;
+}
+
 // What the ends are with the states that come into their chunks: end[j] += exp(A steps[j]) end[j - 1] where chunk j is not its list's first. A
 // block has 32 (channel, state) pairs and splits the chunks among its 8 warps: each makes its own part's product and sum, takes what
 // comes in from the parts before it, and walks its part again.
@@ -471,6 +502,10 @@ int launch_tiles(const ScanParams& p, const ScanPlan& plan, cudaStream_t s) {
   const int a_group = (p.per_group + ch - 1) / ch, blocks = a_group * p.groups;
   const int64_t units = p.lists.batch + (int64_t)p.n_ends;
   XB_REQUIRE(units * blocks < ((int64_t)1 << 31), XB_ERR_LIMIT, "xb_ssm_scan: too many lists and channels");
+  if (p.order) {
+    launch_dependent(ssm_order_kernel, 1, 1024, 0, s, p);
+    if (int rc = check_launch("ssm_order_kernel")) return rc;
+  }
   if (p.chunk > 0) {
     launch_dependent(ssm_scan_kernel<T, LPC, K, SCAN_ENDS>, (unsigned)((int64_t)p.n_ends * blocks), SCAN_THREADS, 0, s, p, a_group);
     if (int rc = check_launch("ssm_scan_kernel")) return rc;
