@@ -213,6 +213,34 @@ def test_slots_outside_and_lists_alone():
     assert torch.equal(again[75:], y[75:]) or torch.isfinite(again[75:]).all()
 
 
+@pytest.mark.parametrize("rows", [0, 1, 70])
+def test_many_lists_without_rows(rows):
+    """Thousands of empty lists ahead of, between and behind the others: their states go from one array to the other."""
+    ops, capi = _ops()
+    rng = np.random.default_rng(rows)
+    lens = [0] * 3000 + ([rows // 2] + [0] * 5000 + [rows - rows // 2] + [0] * 700 if rows else [])
+    lists, rows, off = _lists(lens, rng)
+    n, off = len(lens), torch.from_numpy(off).cuda()
+    x, w, b, st = torch.randn(rows, 20, device="cuda"), torch.randn(20, 4, device="cuda"), torch.randn(20, device="cuda"), torch.randn(n, 3, 20, device="cuda")
+    want, bound, after = ssm_oracle.conv(_np(x), _np(w), _np(b), lists, _np(st), True, "f32")
+    kept, moved = torch.full_like(st, 7.0), st.clone()
+    ssm_oracle.close(_np(ops.ssm_conv(x, w, b, offsets=off, state_in=st, state_out=kept)), want, bound, "y")
+    np.testing.assert_array_equal(_np(kept), np.stack(after))
+    ops.ssm_conv(x, w, b, offsets=off, state_in=moved, state_out=moved)
+    assert torch.equal(moved, kept)
+    ops.ssm_conv(x, w, b, offsets=off, state_out=kept)
+    assert (kept[torch.tensor(lens) == 0] == 0.0).all()
+    s = _scan_inputs(rng, rows, 0, 20, 12, 1, "f32", 0, 0)
+    h = torch.randn(n, 20, 12, device="cuda")
+    want, bound, last, elast = _scan_want(s, lists, 1, _np(h), "f32")
+    kept, moved = torch.full_like(h, 7.0), h.clone()
+    call = lambda **k: ops.ssm_scan(s["x"], s["delta"], s["A"], s["B"], s["C"], D=s["skip"], z=s["z"], delta_bias=s["bias"], offsets=off, **k)
+    ssm_oracle.close(_np(call(h_in=h, h_out=kept)), want, bound, "y")
+    ssm_oracle.close(_np(kept), np.stack(last), np.stack(elast), "states")
+    call(h_in=moved, h_out=moved)
+    assert torch.equal(moved, kept)
+
+
 def test_offsets_that_are_none():
     """Offsets that fall back or lie outside are cut to the rows: nothing outside is read or written."""
     ops, capi = _ops()

@@ -18,6 +18,7 @@ struct ConvParams {
   Lists lists;
   int D, silu, vec, vec_w, vec_state;
   int pieces, n_chunks, rows_a_chunk;     // threads of a row; what a thread walks
+  int walk_blocks;                        // the blocks behind these keep the states of lists without rows
 };
 
 // A thread walks `rows_a_chunk` rows of V channels with the last K - 1 inputs in registers; the threads of a chunk lie side by side, and
@@ -31,6 +32,21 @@ constexpr int CONV_BLOCKS = K <= 4 && V * sizeof(T) <= 8 ? 6 : 4;         // of 
 template <typename T, int V, int K>
 __global__ void __launch_bounds__(CONV_THREADS, CONV_BLOCKS<T, V, K>) ssm_conv_kernel(const ConvParams p) {
   pdl_begin();
+  if ((int)blockIdx.x >= p.walk_blocks) {              // lists without rows: their states go from one array to the other
+    const int64_t e = (int64_t)((int)blockIdx.x - p.walk_blocks) * CONV_THREADS + threadIdx.x, i = e / p.pieces;
+    if (i >= p.lists.batch || p.lists.begin((int)i + 1) > p.lists.begin((int)i)) return;
+    const int slot = p.lists.slot((int)i), c = (int)(e - i * p.pieces) * V, in = min(V, p.D - c);
+    if (slot < 0) return;
+#pragma unroll
+    for (int j = 0; j < K - 1; ++j) {
+      const int64_t at = ((int64_t)slot * (K - 1) + j) * p.D + c;
+      Raw<T, V> t;
+      t.zero();
+      if (p.state_in) t.load_kept(static_cast<const T*>(p.state_in) + at, in, p.vec_state);
+      t.store(static_cast<T*>(p.state_out) + at, in, p.vec_state);
+    }
+    return;
+  }
   __shared__ int s_first[CONV_THREADS];                // the first list that begins in or behind each of the block's chunks
   const int lane = threadIdx.x & 31;
   const int64_t at = (int64_t)blockIdx.x * CONV_THREADS, at_me = at + threadIdx.x;
@@ -44,7 +60,6 @@ __global__ void __launch_bounds__(CONV_THREADS, CONV_BLOCKS<T, V, K>) ssm_conv_k
   const int64_t chunk = at_me / p.pieces;
   if (chunk >= p.n_chunks) return;
   const int c = (int)(at_me - chunk * p.pieces) * V, in = min(V, p.D - c);
-  const bool last_chunk = chunk == p.n_chunks - 1;
   const int64_t r0 = chunk * p.rows_a_chunk, r1 = r0 + p.rows_a_chunk;
   const T *px = static_cast<const T*>(p.x) + c, *pw = static_cast<const T*>(p.w) + (int64_t)c * K, *pb = static_cast<const T*>(p.bias) + c;
   T* py = static_cast<T*>(p.y) + c;
@@ -137,15 +152,27 @@ __global__ void __launch_bounds__(CONV_THREADS, CONV_BLOCKS<T, V, K>) ssm_conv_k
     }
     r = stop;
     if (nxt >= p.lists.batch) return;
-    const int64_t b = p.lists.begin(nxt), e = max(b, p.lists.begin(nxt + 1));
-    if (b >= r1 && !last_chunk) return;
+    const int64_t b = p.lists.begin(nxt);
+    if (b >= r1) return;
+    int64_t e = p.lists.begin(nxt + 1);
+    if (e <= b) {                                      // past all lists without rows: up to the last that begins at b
+      int lo = nxt + 1, hi = p.lists.batch;            // the first that begins behind b is in [lo, hi], or there is none
+      while (lo < hi) {
+        const int mid = lo + (hi - lo) / 2;
+        if (p.lists.begin(mid) > b) hi = mid;
+        else lo = mid + 1;
+      }
+      e = p.lists.begin(hi);
+      if (e <= b) return;
+      nxt = hi - 1;
+    }
     const int slot = p.lists.slot(nxt);
     const int64_t state = ((int64_t)slot * (K - 1)) * p.D + c;
 #pragma unroll
     for (int j = 0; j < K - 1; ++j) {
       Raw<T, V> t;
       t.zero();
-      if (p.state_in && slot >= 0) t.load(static_cast<const T*>(p.state_in) + state + (int64_t)j * p.D, in, p.vec_state);
+      if (p.state_in && slot >= 0) t.load_kept(static_cast<const T*>(p.state_in) + state + (int64_t)j * p.D, in, p.vec_state);
       pairs(t, past[j]);
     }
     if (p.state_out && slot >= 0) {
@@ -190,8 +217,12 @@ Lists lists_of(const int32_t* offsets, const int32_t* slots, int64_t rows, int32
 bool ssm_dtype(int dtype) { return dtype == XB_F32 || dtype == XB_F16 || dtype == XB_BF16; }
 
 template <typename T, int V, int K>
-int launch_conv_taps(const ConvParams& p, cudaStream_t s) {
-  const int64_t blocks = ((int64_t)p.n_chunks * p.pieces + CONV_THREADS - 1) / CONV_THREADS;
+int launch_conv_taps(ConvParams p, cudaStream_t s) {
+  auto blocks_of = [&](int64_t n) { return (n * p.pieces + CONV_THREADS - 1) / CONV_THREADS; };
+  int64_t blocks = blocks_of(p.n_chunks);
+  p.walk_blocks = (int)std::min<int64_t>(blocks, INT32_MAX);
+  // states moved on in place stay as they are
+  if (p.state_out && p.state_out != p.state_in && (p.lists.offsets || p.lists.rows == 0)) blocks += blocks_of(p.lists.batch);
   XB_REQUIRE(blocks < ((int64_t)1 << 31), XB_ERR_LIMIT, "xb_ssm_conv: too many rows and channels");
   launch_dependent(ssm_conv_kernel<T, V, K>, (unsigned)blocks, CONV_THREADS, 0, s, p);
   return check_launch("ssm_conv_kernel");
@@ -242,10 +273,11 @@ ScanPlan scan_plan(const xb_ssm_scan_args& a) {
   const double sms = std::max(sm_count(), 1), mean = (double)a.rows / a.batch;
   const double longest = !a.offsets ? mean : (double)(a.longest > 0 ? std::min(a.longest, a.rows) : a.rows);
   // Cycles: a row of a block takes `work` of a full SM and `alone` where its SM has little else, which is what the longest list (or
-  // chunk) ends with; a block begins with 600 of them, one of the two walks of a chunk with 2000. Lists that are split are walked nearly twice; of lists of all lengths the share in ones above
-  // `chunk` rows is that of an exponential distribution. us, whole lists as they come, long ones first, the best split: 256 lists of
-  // up to 1860 rows in 70000, D = 256 229, 193, 226; 1000 in 20000, D = 256 68, 54; 16 of up to 3640 in 16384, D = 512 246 and 125 split;
-  // one of 4096, D = 1024 302 and 68; 300 of 100, D = 256 65 and 124.
+  // chunk) ends with; a block begins with 600 of them, one of the two walks of a chunk with 2000. Lists that are split are walked nearly
+  // twice; of lists of all lengths the share in ones above `chunk` rows is that of an exponential distribution.
+  // us, whole lists as they come, long ones first, the best split: 256 lists of up to 1860 rows in 70000, D = 256 229, 193, 226; 1000 in
+  // 20000, D = 256 68, 54; 16 of up to 3640 in 16384, D = 512 246 and 125 split; one of 4096, D = 1024 302 and 68; 300 of 100, D = 256
+  // 65 and 124.
   double best = 0;
   for (int K : {1, 2}) {
     if (K == 1 && p.lanes > 4) continue;  // (a block would have 16 channels or fewer)
@@ -253,7 +285,7 @@ ScanPlan scan_plan(const xb_ssm_scan_args& a) {
     const int blocks = scan_blocks(a, p.lanes, K);
     const double full = (double)a.rows * blocks * work / sms;
     // lists of unlike lengths in more than a wave of blocks: long ones first
-    const bool order = a.offsets && longest > 1.5 * mean && (double)a.batch * blocks > 5 * sms;
+    const bool order = a.offsets && longest > 1.5 * mean && a.batch <= 65536 && (double)a.batch * blocks > 5 * sms;
     const double whole = (order ? std::max(full + 6000, alone * longest) : full + 0.6 * alone * longest) + 600.0 * a.batch * blocks / sms;
     if (best == 0 || whole < best) { best = whole; p.K = K; p.chunk = 0; p.order = order; }
     for (int64_t chunk = 64; chunk < longest; chunk += chunk & (chunk - 1) ? chunk / 3 : chunk / 2) {      // 64, 96, 128, 192, ...

@@ -163,6 +163,22 @@ struct Raw {
     else if constexpr (W == 2) { const uint2 t = __ldg(reinterpret_cast<const uint2*>(p)); w[0] = t.x; w[1] = t.y; }
     else w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
   }
+  // the same of memory that this kernel may also write (kept states moved on in place)
+  __device__ __forceinline__ void load_kept(const T* p, int in, bool vec) {
+    if (PIECE && vec && in >= V) {
+      if constexpr (W == 4) { const uint4 t = *reinterpret_cast<const uint4*>(p); w[0] = t.x; w[1] = t.y; w[2] = t.z; w[3] = t.w; }
+      else if constexpr (W == 2) { const uint2 t = *reinterpret_cast<const uint2*>(p); w[0] = t.x; w[1] = t.y; }
+      else w[0] = *reinterpret_cast<const uint32_t*>(p);
+    } else {
+      zero();
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (i < in) {
+          if constexpr (SIZE == 4) w[i] = reinterpret_cast<const uint32_t*>(p)[i];
+          else w[i / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(p)[i] << (16 * (i & 1));
+        }
+    }
+  }
   // `in` of them exist (others are 0); in whole where they do and `vec` says that they lie aligned
   __device__ __forceinline__ void load(const T* p, int in, bool vec) {
     if (PIECE && vec && in >= V) {
