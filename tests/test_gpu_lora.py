@@ -103,6 +103,36 @@ def test_bad_values_stay_in_their_rows(M):
     assert torch.equal(again[others], y[others]) and not torch.isfinite(again[17]).any() and not torch.isfinite(again[250]).all()
 
 
+@pytest.mark.parametrize("dtype,out", [("f16", "f16"), ("bf16", "f32"), ("f32", "f32")])
+@pytest.mark.parametrize("M,K,N,n,r,trans", [
+    (600, 1, 24, 3, 2, True), (520, 5, 40, 2, 3, False), (511, 3, 8, 2, 1, True), (600, 72, 304, 300, 12, True), (9500, 72, 200, 300, 8, True),
+    (9500, 40, 304, 2, 128, False), (700, 2000, 1, 5, 40, True)])
+def test_shallow_products_and_tiles_of_many_adapters(dtype, out, M, K, N, n, r, trans):
+    s = _case(np.random.default_rng(K + n), M, K, N, n, r, dtype, trans, 0, "mixed")
+    _check(s, dtype, out, trans)
+
+
+@pytest.mark.parametrize("M,N", [(60, 72), (700, 300), (9600, 72)])
+def test_adapters_that_share_their_matrices(M, N):
+    """One A or one B for all adapters (a stride of 0), each with its own scale."""
+    for shared in ("A", "B"):
+        s = _case(np.random.default_rng(M), M, 96, N, 4, 8, "bf16", True, 0, "mixed")
+        s[shared] = s[shared][:1].expand(4, -1, -1)
+        assert s[shared].stride(0) == 0
+        _check(s, "bf16", "bf16", True)
+
+
+@pytest.mark.parametrize("M", [60, 700, 9600])
+def test_infinities_of_one_sign_are_infinities(M):
+    ops, capi = _ops()
+    for r in (3, 16, 20):
+        s = _case(np.random.default_rng(M + r), M, 64, 72, 2, r, "bf16", True, 0, "one")
+        W, A, B = s["W"].abs() + 0.01, s["A"].abs() + 0.01, s["B"].abs() + 0.01
+        s["X"][M // 2, 5] = float("inf")
+        y = ops.lora_gemm(s["X"], W, A, B, s["adapter"], trans_b=True)
+        assert (y[M // 2] == float("inf")).all() and torch.isfinite(y[:M // 2]).all() and torch.isfinite(y[M // 2 + 1:]).all()
+
+
 def test_the_same_bits_each_time_and_on_other_streams():
     ops, capi = _ops()
     rng = np.random.default_rng(12)

@@ -74,7 +74,8 @@ def test_lora():
     c, L = m.capi, m.lib()
     assert L.xb_lora_gemm(None, None, 0, None) == ARG and L.xb_lora_workspace_bytes(None) == 0
     for rc, k in ((UNSUPPORTED, dict(dtype=c.XB_I32)), (UNSUPPORTED, dict(y_dtype=c.XB_BF16)), (ARG, dict(M=-1)), (ARG, dict(K=0)), (ARG, dict(r=-1)),
-                  (LIMIT, dict(r=129, ldb=129)), (ARG, dict(X=None)), (ARG, dict(W=None)), (ARG, dict(Y=None)), (ARG, dict(A=None)), (ARG, dict(B=None)),
+                  (LIMIT, dict(r=129, ldb=129)), (LIMIT, dict(M=(1 << 31) - 1000)), (LIMIT, dict(N=(1 << 31) - 1, ldy=1 << 31)),
+                  (LIMIT, dict(K=(1 << 31) - 1, ldx=1 << 31, ldw=1 << 31, lda=1 << 31)), (ARG, dict(X=None)), (ARG, dict(W=None)), (ARG, dict(Y=None)), (ARG, dict(A=None)), (ARG, dict(B=None)),
                   (ARG, dict(adapter=None)), (ARG, dict(ldx=31)), (ARG, dict(ldw=31)), (ARG, dict(trans_w=0, ldw=15)), (ARG, dict(ldy=15)),
                   (ARG, dict(lda=31)), (ARG, dict(ldb=7)), (ARG, dict(stride_a=-1)), (ARG, dict(stride_b=-8))):
         assert L.xb_lora_gemm(C.byref(_lora(c, **k)), AT, 1 << 40, None) == rc, k

@@ -12,7 +12,6 @@ int gemm_half_sums(const xb_gemm_args& a, cudaStream_t stream);
 
 namespace {
 
-
 // V adjacent elements as fp32: one load where they lie aligned, which V > 1 says
 template <typename T, int V>
 __device__ __forceinline__ void load_piece(const T* p, float (&v)[V]) {
@@ -141,6 +140,8 @@ int check_args(const xb_lora_args* a) {
   XB_REQUIRE(a->y_dtype == a->dtype || a->y_dtype == XB_F32, XB_ERR_UNSUPPORTED, "xb_lora_gemm: results of dtype %d from dtype %d", a->y_dtype,
              a->dtype);
   XB_REQUIRE(a->M >= 0 && a->N >= 0 && a->K >= 1 && a->r >= 0 && a->n_adapters >= 0, XB_ERR_ARG, "xb_lora_gemm: bad sizes");
+  // (sizes rounded up to whole tiles are counted in 32 bits)
+  XB_REQUIRE(std::max({a->M, a->N, a->K}) <= INT32_MAX - 1023, XB_ERR_LIMIT, "xb_lora_gemm: %d x %d x %d, at most 2^31 - 1024 each", a->M, a->N, a->K);
   XB_REQUIRE(a->r <= LORA_MAX_RANK, XB_ERR_LIMIT, "xb_lora_gemm: rank %d, at most %d", a->r, LORA_MAX_RANK);
   if (a->M == 0 || a->N == 0) return 0;
   const bool adapters = a->n_adapters > 0 && a->r > 0;

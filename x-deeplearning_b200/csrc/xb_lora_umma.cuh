@@ -122,7 +122,8 @@ __device__ __forceinline__ void widen_b(const LoraTiles& p, int64_t first, int64
     reinterpret_cast<float4*>(p.B32)[e] = make_float4(v[0], v[1], v[2], v[3]);
   }
 }
-// v as two TF32 terms (an infinity or NaN, or what rounds up to one, stays whole in hi)
+// v as two TF32 terms (an infinity or NaN, or what rounds up to one, stays whole in hi). Columns behind the rank are zeros whatever X
+// holds: an infinity times the zeros of A would be a NaN there.
 __device__ __forceinline__ void split_tf32(float v, float& hi, float& lo) {
   hi = round_tf32(v);
   lo = fabsf(hi) <= 3.4028235e38f ? round_tf32(v - hi) : 0.f;
@@ -130,23 +131,23 @@ __device__ __forceinline__ void split_tf32(float v, float& hi, float& lo) {
 
 // The adapters of a tile, `group` at a time.
 constexpr int SHRINK_GROUP = 4;           // adapters of a pass, at most
-    struct Pass {
-    uint32_t id[SHRINK_GROUP];
-    int n;
-    uint32_t next;                                         // the first that this pass does not take
-    __device__ __forceinline__ void take(const TileAdapters<4>& t, uint32_t first, int group) {
-      n = 0;
-      next = first;
+struct Pass {
+  uint32_t id[SHRINK_GROUP];
+  int n;
+  uint32_t next;                          // the first that this pass does not take
+  __device__ __forceinline__ void take(const TileAdapters<4>& t, uint32_t first, int group) {
+    n = 0;
+    next = first;
 #pragma unroll
-      for (int i = 0; i < SHRINK_GROUP; ++i) {
-        id[i] = i < group ? next : NO_ADAPTER;
-        if (id[i] != NO_ADAPTER) {
-          ++n;
-          next = t.next(next + 1);
-        }
+    for (int i = 0; i < SHRINK_GROUP; ++i) {
+      id[i] = i < group ? next : NO_ADAPTER;
+      if (id[i] != NO_ADAPTER) {
+        ++n;
+        next = t.next(next + 1);
       }
     }
-  };
+  }
+};
 
 constexpr int SHRINK_THREADS = 320;       // producer, MMA, four warps for the results, four for B
 constexpr int SHRINK_GROUP_ROWS = 64;     // rows of A (adapters x rb) in a stage, or rb where that is more
@@ -250,7 +251,7 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
               for (int j = 0; j < 16; j += 4) {
                 float hi[4], lo[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) split_tf32(scale * __uint_as_float(raw[j + e]), hi[e], lo[e]);
+                for (int e = 0; e < 4; ++e) split_tf32(c + j + e < p.r ? scale * __uint_as_float(raw[j + e]) : 0.f, hi[e], lo[e]);
                 *reinterpret_cast<float4*>(u + c + j) = make_float4(hi[0], hi[1], hi[2], hi[3]);
                 *reinterpret_cast<float4*>(u + p.rb + c + j) = make_float4(lo[0], lo[1], lo[2], lo[3]);
               }
@@ -723,7 +724,7 @@ lora_fused_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
               for (int j = 0; j < 16; j += 4) {
                 float hi[4], lo[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) split_tf32(scale * __uint_as_float(raw[j + e]), hi[e], lo[e]);
+                for (int e = 0; e < 4; ++e) split_tf32(c + j + e < l.r ? scale * __uint_as_float(raw[j + e]) : 0.f, hi[e], lo[e]);
                 put(smem_u, row, c + j, hi);               // (hi and lo of 16 columns share the one block there is, of 32 they have one each)
                 put(smem_u + (l.rb >> 5) * A_STAGE_BYTES, row, (l.rb == 16 ? 16 : 0) + c + j, lo);
               }
