@@ -21,6 +21,87 @@ struct ConvParams {
   int walk_blocks;                        // the blocks behind these keep the states of lists without rows
 };
 
+// The taps and the last K - 1 inputs of V adjacent channels, as pairs of fp32
+template <typename T, int V, int K>
+struct ConvTaps {
+  static constexpr int P = (V + 1) / 2;
+  f32x2 w[K][P], bias[P], past[K - 1][P];
+  static __device__ __forceinline__ void pairs(const Raw<T, V>& t, f32x2 (&to)[P]) {
+#pragma unroll
+    for (int q = 0; q < P; ++q) to[q] = pack2(t.get(2 * q), 2 * q + 1 < V ? t.get((2 * q + 1) % V) : 0.f);
+  }
+  __device__ __forceinline__ void load(const ConvParams& p, int c, int in) {
+    const T *pw = static_cast<const T*>(p.w) + (int64_t)c * K, *pb = static_cast<const T*>(p.bias) + c;
+    Raw<T, V> t[K];
+#pragma unroll
+    for (int j = 0; j < K; ++j) t[j].load(pw + j * V, in * K - j * V, p.vec_w);
+    auto weight = [&](int e) { return e < V * K ? t[e / V % K].get(e % V) : 0.f; };      // element e of the V channels' K taps
+#pragma unroll
+    for (int j = 0; j < K; ++j)
+#pragma unroll
+      for (int q = 0; q < P; ++q) w[j][q] = pack2(weight(2 * q * K + j), weight((2 * q + 1) * K + j));
+    t[0].zero();
+    if (p.bias) t[0].load(pb, in, p.vec_w);
+    pairs(t[0], bias);
+  }
+  // the outputs of the row `t`, which becomes the last input
+  __device__ __forceinline__ void row(int silu, const Raw<T, V>& t, Raw<T, V>& out) {
+    f32x2 x[P], o[P];
+    pairs(t, x);
+#pragma unroll
+    for (int q = 0; q < P; ++q) {
+      f32x2 s = bias[q];
+#pragma unroll
+      for (int j = 0; j < K - 1; ++j) s = fma2(w[j][q], past[j][q], s);
+      o[q] = fma2(w[K - 1][q], x[q], s);
+#pragma unroll
+      for (int j = 0; j + 1 < K - 1; ++j) past[j][q] = past[j + 1][q];
+      past[K - 2][q] = x[q];
+    }
+    if (silu) {
+#pragma unroll
+      for (int q = 0; q < P; ++q) o[q] = silu2(o[q]);
+    }
+    float v[2 * P], first[V];
+#pragma unroll
+    for (int q = 0; q < P; ++q) unpack2(o[q], v[2 * q], v[2 * q + 1]);
+#pragma unroll
+    for (int i = 0; i < V; ++i) first[i] = v[i];
+    out.put_all(first);
+  }
+};
+
+// One row a list: a thread has V channels of it. All that it reads, states, row and weights, is on its way at once; what the walk reads
+// one after the other is the time of a call of few rows.
+template <typename T, int V, int K>
+__global__ void __launch_bounds__(CONV_THREADS) ssm_conv_step_kernel(const ConvParams p) {
+  pdl_begin();
+  const uint64_t e = (uint64_t)blockIdx.x * CONV_THREADS + threadIdx.x;
+  const int64_t i = e >> 32 ? (int64_t)(e / (uint32_t)p.pieces) : (int64_t)((uint32_t)e / (uint32_t)p.pieces);
+  if (i >= p.lists.rows) return;
+  const int c = (int)((int64_t)e - i * p.pieces) * V, in = min(V, p.D - c), slot = p.lists.slot((int)i);
+  const int64_t state = (int64_t)slot * (K - 1) * p.D + c;
+  Raw<T, V> x, kept[K - 1], out;
+  x.load(static_cast<const T*>(p.x) + i * p.ldx + c, in, p.vec);
+#pragma unroll
+  for (int j = 0; j < K - 1; ++j) {
+    kept[j].zero();
+    if (p.state_in && slot >= 0) kept[j].load_kept(static_cast<const T*>(p.state_in) + state + (int64_t)j * p.D, in, p.vec_state);
+  }
+  ConvTaps<T, V, K> taps;
+  taps.load(p, c, in);
+#pragma unroll
+  for (int j = 0; j < K - 1; ++j) taps.pairs(kept[j], taps.past[j]);
+  taps.row(p.silu, x, out);
+  out.store(static_cast<T*>(p.y) + i * p.ldy + c, in, p.vec);
+  if (p.state_out && slot >= 0) {
+    T* to = static_cast<T*>(p.state_out) + state;
+#pragma unroll
+    for (int j = 0; j + 1 < K - 1; ++j) kept[j + 1].store(to + (int64_t)j * p.D, in, p.vec_state);
+    x.store(to + (int64_t)(K - 2) * p.D, in, p.vec_state);
+  }
+}
+
 // A thread walks `rows_a_chunk` rows of V channels with the last K - 1 inputs in registers; the threads of a chunk lie side by side, and
 // chunks follow one another without a gap, so no lane idles whatever D is. x is read 1 + (K - 1) / rows_a_chunk times.
 // The thread that has a list's first row makes its first K - 1 rows (they read the state) and its last state, so that states moved
@@ -61,52 +142,13 @@ __global__ void __launch_bounds__(CONV_THREADS, CONV_BLOCKS<T, V, K>) ssm_conv_k
   if (chunk >= p.n_chunks) return;
   const int c = (int)(at_me - chunk * p.pieces) * V, in = min(V, p.D - c);
   const int64_t r0 = chunk * p.rows_a_chunk, r1 = r0 + p.rows_a_chunk;
-  const T *px = static_cast<const T*>(p.x) + c, *pw = static_cast<const T*>(p.w) + (int64_t)c * K, *pb = static_cast<const T*>(p.bias) + c;
+  const T* px = static_cast<const T*>(p.x) + c;
   T* py = static_cast<T*>(p.y) + c;
-  constexpr int P = (V + 1) / 2;                       // pairs of channels
   constexpr int CONV_FEW = V == 1 ? CONV_AHEAD : 4;
-  f32x2 w[K][P], bias[P], past[K - 1][P];
-  auto pairs = [](const Raw<T, V>& t, f32x2 (&to)[P]) {
-#pragma unroll
-    for (int q = 0; q < P; ++q) to[q] = pack2(t.get(2 * q), 2 * q + 1 < V ? t.get((2 * q + 1) % V) : 0.f);
-  };
-  {
-    Raw<T, V> t[K];
-#pragma unroll
-    for (int j = 0; j < K; ++j) t[j].load(pw + j * V, in * K - j * V, p.vec_w);
-    auto weight = [&](int e) { return e < V * K ? t[e / V % K].get(e % V) : 0.f; };      // element e of the V channels' K taps
-#pragma unroll
-    for (int j = 0; j < K; ++j)
-#pragma unroll
-      for (int q = 0; q < P; ++q) w[j][q] = pack2(weight(2 * q * K + j), weight((2 * q + 1) * K + j));
-    t[0].zero();
-    if (p.bias) t[0].load(pb, in, p.vec_w);
-    pairs(t[0], bias);
-  }
-  auto row_of = [&](const Raw<T, V>& t, Raw<T, V>& out) {
-    f32x2 x[P], o[P];
-    pairs(t, x);
-#pragma unroll
-    for (int q = 0; q < P; ++q) {
-      f32x2 s = bias[q];
-#pragma unroll
-      for (int j = 0; j < K - 1; ++j) s = fma2(w[j][q], past[j][q], s);
-      o[q] = fma2(w[K - 1][q], x[q], s);
-#pragma unroll
-      for (int j = 0; j + 1 < K - 1; ++j) past[j][q] = past[j + 1][q];
-      past[K - 2][q] = x[q];
-    }
-    if (p.silu) {
-#pragma unroll
-      for (int q = 0; q < P; ++q) o[q] = silu2(o[q]);
-    }
-    float v[2 * P], first[V];
-#pragma unroll
-    for (int q = 0; q < P; ++q) unpack2(o[q], v[2 * q], v[2 * q + 1]);
-#pragma unroll
-    for (int i = 0; i < V; ++i) first[i] = v[i];
-    out.put_all(first);
-  };
+  ConvTaps<T, V, K> taps;
+  taps.load(p, c, in);
+  auto& past = taps.past;
+  auto row_of = [&](const Raw<T, V>& t, Raw<T, V>& out) { taps.row(p.silu, t, out); };
   const bool whole_piece = Raw<T, V>::PIECE && p.vec && in == V;
   int nxt = s_first[(int)(chunk - c_first)];
   int64_t r = r0, stop = r0;
@@ -119,7 +161,7 @@ __global__ void __launch_bounds__(CONV_THREADS, CONV_BLOCKS<T, V, K>) ssm_conv_k
       for (int j = 0; j < K - 1; ++j) {
         Raw<T, V> t;
         t.load(px + (r - (K - 1) + j) * p.ldx, in, p.vec);
-        pairs(t, past[j]);
+        taps.pairs(t, past[j]);
       }
     }
   }
@@ -173,7 +215,7 @@ __global__ void __launch_bounds__(CONV_THREADS, CONV_BLOCKS<T, V, K>) ssm_conv_k
       Raw<T, V> t;
       t.zero();
       if (p.state_in && slot >= 0) t.load_kept(static_cast<const T*>(p.state_in) + state + (int64_t)j * p.D, in, p.vec_state);
-      pairs(t, past[j]);
+      taps.pairs(t, past[j]);
     }
     if (p.state_out && slot >= 0) {
 #pragma unroll
@@ -184,7 +226,7 @@ __global__ void __launch_bounds__(CONV_THREADS, CONV_BLOCKS<T, V, K>) ssm_conv_k
           t.load(px + (b + place) * p.ldx, in, p.vec);
         } else {
 #pragma unroll
-          for (int q = 0; q < P; ++q) {
+          for (int q = 0; q < taps.P; ++q) {
             f32x2 was = 0;
 #pragma unroll
             for (int k = 0; k < K - 1; ++k) was = k == (int)place + K - 1 ? past[k][q] : was;
@@ -219,6 +261,12 @@ bool ssm_dtype(int dtype) { return dtype == XB_F32 || dtype == XB_F16 || dtype =
 template <typename T, int V, int K>
 int launch_conv_taps(ConvParams p, cudaStream_t s) {
   auto blocks_of = [&](int64_t n) { return (n * p.pieces + CONV_THREADS - 1) / CONV_THREADS; };
+  if (!p.lists.offsets && p.lists.per == 1) {
+    const int64_t blocks = blocks_of(p.lists.rows);
+    XB_REQUIRE(blocks < ((int64_t)1 << 31), XB_ERR_LIMIT, "xb_ssm_conv: too many rows and channels");
+    launch_dependent(ssm_conv_step_kernel<T, V, K>, (unsigned)blocks, CONV_THREADS, 0, s, p);
+    return check_launch("ssm_conv_step_kernel");
+  }
   int64_t blocks = blocks_of(p.n_chunks);
   p.walk_blocks = (int)std::min<int64_t>(blocks, INT32_MAX);
   // states moved on in place stay as they are
@@ -231,9 +279,9 @@ template <typename T, int V>
 int launch_conv_pieces(ConvParams p, int K, cudaStream_t s) {
   p.pieces = (p.D + V - 1) / V;
   if (V == 1) p.vec = p.vec_w = p.vec_state = 1;       // (pieces of one element lie aligned)
-  // Longer walks read less twice, shorter ones keep more threads in flight. Single rows: nothing is read twice.
+  // Longer walks read less twice, shorter ones keep more threads in flight.
   const int64_t threads = p.lists.rows * p.pieces, fill = (int64_t)sm_count() * 1024;
-  p.rows_a_chunk = (int)std::min<int64_t>(std::max<int64_t>(threads / fill, 1), !p.lists.offsets && p.lists.per <= 1 ? 1 : 32);
+  p.rows_a_chunk = (int)std::min<int64_t>(std::max<int64_t>(threads / fill, 1), 32);
   p.n_chunks = (int)std::max<int64_t>((p.lists.rows + p.rows_a_chunk - 1) / p.rows_a_chunk, 1);
   switch (K) {
     case 2: return launch_conv_taps<T, V, 2>(p, s);
