@@ -210,7 +210,8 @@ int run_rows(const xb_lora_args& a, uint8_t* ws, cudaStream_t s) {
       LoraRowsParams r;
       r.l = p;
       r.W = a.W; r.ldw = a.ldw; r.Y = a.Y; r.ldy = a.ldy;
-      r.y_f32 = a.y_dtype == XB_F32; r.vec_r = vec_r;
+      r.y_f32 = a.y_dtype == XB_F32;
+      r.lanes = !vec_r ? 0 : a.r <= 8 ? 1 : a.r <= 16 ? 2 : a.r <= 32 ? 4 : a.r <= 64 ? 8 : 16;
       const int64_t tiles = ((int64_t)a.N + ROWS_BN - 1) / ROWS_BN * ((a.M + ROWS_BM - 1) / ROWS_BM);
       const int slices = (a.K + ROWS_BK - 1) / ROWS_BK;
       r.split = 1;

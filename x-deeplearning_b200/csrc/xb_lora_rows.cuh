@@ -32,7 +32,7 @@ __device__ __forceinline__ int adapter_of(const LoraParams& p, int m) {
 // depth: all of what it reads is on its way at once, it makes its own products with B meanwhile, and the partial sums are added out
 // of one another's shared memory, every CTA for its share of the rows. Sums as in gemm_half_kernel: 16 products by a matrix
 // instruction, added in fp32. What bounds it is the latency of one round to memory, the exchange and the launch.
-// [64, 1280] x [1280, 1024], 64 adapters of rank 16: 12 us less than xb_gemm with a bias matrix, and the kernel that made that.
+// [64, 1280] x [1280, 1024], 64 adapters of rank 16, the call in a graph: 17 us as xb_gemm with a bias matrix and the kernel that made that, 11.6 now.
 constexpr int ROWS_BM = 64, ROWS_BN = 32, ROWS_BK = 320, ROWS_THREADS = 256;
 constexpr int ROWS_XPITCH = ROWS_BK + 8, ROWS_WPITCH = ROWS_BN + 8;          // halves: no bank conflicts of the eight rows that are read together
 constexpr int ROWS_X_BYTES = ROWS_BM * ROWS_XPITCH * 2;
@@ -45,7 +45,8 @@ struct LoraRowsParams {
   const void* W; int64_t ldw;
   void* Y; int64_t ldy;
   int split;                              // CTAs of a tile
-  int y_f32, vec_r;
+  int y_f32;
+  int lanes;                              // that share a row of B, 16 bytes each (a power of two); 0: rows in single elements
 };
 
 // 16 bytes of which the first `bytes` exist (the rest becomes zeros)
@@ -58,8 +59,47 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr, uint32_t rank) {
   return v;
 }
 
+// u B^T for 32 columns, by a warp: LP lanes share a column's row of B, so that a load takes whole rows of 32 / LP columns, and their sums
+// change sides until lane l has those of column (l % LP) 32 / LP + l / LP. With a column a lane every load touches 32 lines: 230 rows,
+// N = 608, rank 64, the call in a graph 38 us, 15 now.
+template <int LP, typename T>
+__device__ __forceinline__ float expand_row(const T* B, int64_t ldb, const float* u, int r, int cols, int lane) {
+  const int sub = lane % LP, c0 = lane / LP, j = sub * 8;
+  uint4 t[LP];
+#pragma unroll
+  for (int g = 0; g < LP; ++g) {
+    const int c = g * (32 / LP) + c0;
+    t[g] = j < r && c < cols ? __ldg(reinterpret_cast<const uint4*>(B + (int64_t)c * ldb + j)) : make_uint4(0u, 0u, 0u, 0u);
+  }
+  float uv[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, v[LP];
+  if (j < r) {
+    const float4 u0 = *reinterpret_cast<const float4*>(u + j), u1 = *reinterpret_cast<const float4*>(u + j + 4);
+    uv[0] = u0.x; uv[1] = u0.y; uv[2] = u0.z; uv[3] = u0.w; uv[4] = u1.x; uv[5] = u1.y; uv[6] = u1.z; uv[7] = u1.w;
+  }
+#pragma unroll
+  for (int g = 0; g < LP; ++g) {
+    const T* e = reinterpret_cast<const T*>(&t[g]);
+    v[g] = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[g] = fmaf(uv[k], to_f32<T>(e[k]), v[g]);
+  }
+  int have = LP;
+#pragma unroll
+  for (int m = LP / 2; m > 0; m >>= 1) {
+    have /= 2;
+    const bool up = sub & m;
+#pragma unroll
+    for (int g = 0; g < LP / 2; ++g)
+      if (g < have) {
+        const float give = up ? v[g] : v[g + have], keep = up ? v[g + have] : v[g];
+        v[g] = keep + __shfl_xor_sync(0xffffffffu, give, m);
+      }
+  }
+  return v[0];
+}
+
 template <typename T, bool TRANS_W>
-__global__ void __launch_bounds__(ROWS_THREADS) lora_rows_gemm_kernel(const __grid_constant__ LoraRowsParams p) {
+__global__ void __launch_bounds__(ROWS_THREADS, 2) lora_rows_gemm_kernel(const __grid_constant__ LoraRowsParams p) {
   pdl_begin();
   constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
   extern __shared__ __align__(16) uint8_t rows_smem[];
@@ -96,38 +136,53 @@ __global__ void __launch_bounds__(ROWS_THREADS) lora_rows_gemm_kernel(const __gr
   if (s0 < s1) bring(s0);
 
   // the outputs that this thread ends with: OUT rows of one column; bias and U B^T for them
-  const int share = ROWS_BM / p.split, first = rank * share, col = n0 + lane, step = ROWS_THREADS / 32;
+  const int share = ROWS_BM / p.split, first = rank * share, step = ROWS_THREADS / 32;
+  const int LP = p.lanes, at_col = LP > 1 ? lane % LP * (32 / LP) + lane / LP : lane, col = n0 + at_col;
   constexpr int OUT = ROWS_BM / (ROWS_THREADS / 32);
   float out[OUT];
 #pragma unroll
   for (int i = 0; i < OUT; ++i) out[i] = 0.f;
-  if (col < l.N) {
-    const float bias = l.bias ? l.bias[col] : 0.f;
-#pragma unroll
-    for (int i = 0; i < OUT; ++i) {
+  {
+    const float bias = l.bias && col < l.N ? l.bias[col] : 0.f;
+    auto adapter_at = [&](int i) {                         // of this warp's i-th row
       const int m = m0 + first + warp + i * step;
-      if (warp + i * step >= share || m >= l.M) continue;
-      const int a = adapter_of(l, m);
-      float sum = 0.f;
-      if (a >= 0) {
-        const T* b = reinterpret_cast<const T*>(l.B) + (int64_t)a * l.stride_b + (int64_t)col * l.ldb;
-        const float* u = l.U + (int64_t)m * l.r;
-        if (p.vec_r) {
-#pragma unroll 2
-          for (int j = 0; j < l.r; j += 8) {
-            const uint4 t = __ldg(reinterpret_cast<const uint4*>(b + j));
-            const T* e = reinterpret_cast<const T*>(&t);
-            const float4 u0 = *reinterpret_cast<const float4*>(u + j), u1 = *reinterpret_cast<const float4*>(u + j + 4);
-            const float uv[8] = {u0.x, u0.y, u0.z, u0.w, u1.x, u1.y, u1.z, u1.w};
+      return i * step + warp < share && m < l.M ? adapter_of(l, m) : -1;
+    };
+    const float* u = l.U + (int64_t)(m0 + first + warp) * l.r;
+    const T* B = reinterpret_cast<const T*>(l.B) + (int64_t)n0 * l.ldb;
+    // (a loop: eight rows one behind the other are so much code that its fetching shows in a call of 12 us)
+    auto products = [&](auto lanes) {
+      constexpr int L = decltype(lanes)::value;
+      int a = adapter_at(0);
+#pragma unroll 1
+      for (int i = 0; i * step < share; ++i) {
+        const int now = a;
+        a = adapter_at(i + 1);
+        if (now < 0) continue;
+        const float v = expand_row<L, T>(B + (int64_t)now * l.stride_b, l.ldb, u + (int64_t)i * step * l.r, l.r, l.N - n0, lane);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) sum = fmaf(uv[k], to_f32<T>(e[k]), sum);
-          }
-        } else {
-          for (int j = 0; j < l.r; ++j) sum = fmaf(u[j], to_f32<T>(b[j]), sum);
-        }
+        for (int k = 0; k < OUT; ++k) out[k] = k == i ? v : out[k];
       }
-      out[i] = bias + sum;
+    };
+    switch (LP) {
+      case 1: products(std::integral_constant<int, 1>()); break;
+      case 2: products(std::integral_constant<int, 2>()); break;
+      case 4: products(std::integral_constant<int, 4>()); break;
+      case 8: products(std::integral_constant<int, 8>()); break;
+      case 16: products(std::integral_constant<int, 16>()); break;
+      default:
+        if (col < l.N) {
+#pragma unroll
+          for (int i = 0; i < OUT; ++i) {
+            const int a = adapter_at(i);
+            if (a < 0) continue;
+            const T* b = B + (int64_t)a * l.stride_b + (int64_t)lane * l.ldb;
+            for (int j = 0; j < l.r; ++j) out[i] = fmaf(u[(int64_t)i * step * l.r + j], to_f32<T>(b[j]), out[i]);
+          }
+        }
     }
+#pragma unroll
+    for (int i = 0; i < OUT; ++i) out[i] += bias;
   }
 
   // 4 x 2 warps of 16 x 16 outputs
@@ -162,12 +217,12 @@ __global__ void __launch_bounds__(ROWS_THREADS) lora_rows_gemm_kernel(const __gr
     for (int i = 0; i < OUT; ++i) {
       const int r = warp + i * step, m = m0 + first + r;
       if (r >= share || m >= l.M) continue;
-      const uint32_t at = umma::smem_u32(part + (first + r) * ROWS_BN + lane);
+      const uint32_t at = umma::smem_u32(part + (first + r) * ROWS_BN + at_col);
       float v = 0.f;
       if (p.split > 1) {
         for (int c = 0; c < p.split; ++c) v += ld_cluster_f32(at, (uint32_t)c);
       } else {
-        v = part[(first + r) * ROWS_BN + lane];
+        v = part[(first + r) * ROWS_BN + at_col];
       }
       v += out[i];
       if (p.y_f32) reinterpret_cast<float*>(p.Y)[(int64_t)m * p.ldy + col] = v;
