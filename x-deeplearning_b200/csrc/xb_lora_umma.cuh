@@ -107,19 +107,39 @@ struct LoraTiles {
   uint32_t idesc_a, idesc_ext;
 };
 
-// B as fp32, zeros behind its r columns: pieces of four from `first` on, every `step`-th
-__device__ __forceinline__ void widen_b(const LoraTiles& p, int64_t first, int64_t step) {
-  const int64_t quads = (int64_t)p.n_adapters * p.N * (p.b_cols / 4);
-  for (int64_t e = first; e < quads; e += step) {
-    const int64_t an = e / (p.b_cols / 4);
-    const int c = (int)(e - an * (p.b_cols / 4)) * 4, a = (int)(an / p.N), n = (int)(an - (int64_t)a * p.N);
-    float v[4];
+// eight 16-bit values as fp32
+__device__ __forceinline__ void widen8(const uint4& t, int dtype, float (&v)[8]) {
+  const uint32_t x[4] = {t.x, t.y, t.z, t.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int j = (c + i) % p.rb;
-      v[i] = j < p.r ? load_as_f32(p.B, (int64_t)a * p.stride_b + (int64_t)n * p.ldb + j, p.dtype) : 0.f;
+  for (int k = 0; k < 4; ++k) {
+    if (dtype == XB_BF16) {
+      v[2 * k] = __uint_as_float(x[k] << 16);
+      v[2 * k + 1] = __uint_as_float(x[k] & 0xffff0000u);
+    } else {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&x[k]));
+      v[2 * k] = f.x;
+      v[2 * k + 1] = f.y;
     }
-    reinterpret_cast<float4*>(p.B32)[e] = make_float4(v[0], v[1], v[2], v[3]);
+  }
+}
+// B as fp32, zeros behind its r columns: pieces of eight from `first` on, every `step`-th
+__device__ __forceinline__ void widen_b(const LoraTiles& p, int64_t first, int64_t step) {
+  const int pieces = p.b_cols / 8;
+  const int64_t all = (int64_t)p.n_adapters * p.N * pieces;
+  for (int64_t e = first; e < all; e += step) {
+    const int64_t an = e / pieces;
+    const int j = (int)(e - an * pieces) * 8 % p.rb, a = (int)(an / p.N), n = (int)(an - (int64_t)a * p.N);
+    const int64_t at = (int64_t)a * p.stride_b + (int64_t)n * p.ldb + j;
+    float v[8];
+    if (p.vec_b && j < p.r) {
+      widen8(__ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.B) + at)), p.dtype, v);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = j + i < p.r ? load_as_f32(p.B, at + i, p.dtype) : 0.f;
+    }
+    float4* to = reinterpret_cast<float4*>(p.B32) + 2 * e;
+    to[0] = make_float4(v[0], v[1], v[2], v[3]);
+    to[1] = make_float4(v[4], v[5], v[6], v[7]);
   }
 }
 // v as two TF32 terms (an infinity or NaN, or what rounds up to one, stays whole in hi). Columns behind the rank are zeros whatever X
@@ -682,19 +702,7 @@ lora_fused_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
             if (j >= l.rb) break;
             float v[8];
             if (l.vec_b && n < p.N && j < l.r) {
-              const uint4 t = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(l.B) + at + j));
-              const uint32_t x[4] = {t.x, t.y, t.z, t.w};
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                if (l.dtype == XB_BF16) {
-                  v[2 * k] = __uint_as_float(x[k] << 16);
-                  v[2 * k + 1] = __uint_as_float(x[k] & 0xffff0000u);
-                } else {
-                  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&x[k]));
-                  v[2 * k] = f.x;
-                  v[2 * k + 1] = f.y;
-                }
-              }
+              widen8(__ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(l.B) + at + j)), l.dtype, v);
             } else {
 #pragma unroll
               for (int k = 0; k < 8; ++k) v[k] = n < p.N && j + k < l.r ? load_as_f32(l.B, at + j + k, l.dtype) : 0.f;
@@ -922,7 +930,8 @@ int run_umma(const xb_lora_args& given, uint8_t* ws, cudaStream_t stream) {
     l.stages = std::min(MAX_STAGES, 220 * 1024 / stage);
     static PerDeviceOnce attr_set;
     XB_SET_MAX_SMEM_ONCE(attr_set, 226 * 1024, (const void*)lora_shrink_kernel);
-    launch_dependent(lora_shrink_kernel, (unsigned)std::min(l.tiles_m, sm_count()), SHRINK_THREADS, (size_t)l.stages * stage + 1024, stream, mx, ma, l);
+    // (every SM takes its share of B, with or without tiles: 520 rows, 16 adapters, N = 1024, rank 64, with a block a tile 220 us, SHRINK_NEW now)
+    launch_dependent(lora_shrink_kernel, (unsigned)sm_count(), SHRINK_THREADS, (size_t)l.stages * stage + 1024, stream, mx, ma, l);
     if (int rc = check_launch("lora_shrink_kernel")) return rc;
   }
   UmmaGemmParams p;
