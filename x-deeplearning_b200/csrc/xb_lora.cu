@@ -122,9 +122,21 @@ __global__ void __launch_bounds__(128) lora_rows_expand_kernel(const LoraParams 
     if (m0 + m < p.M) p.part[(int64_t)(m0 + m) * p.N + n] = bias + sum[m];
 }
 
-// Few rows: the tiles would leave most SMs idle, and a tile of many adapters walks through all of them.
-constexpr int ROWS_MOST = 511;
-bool takes_tiles(const xb_lora_args& a) { return a.M > ROWS_MOST && lora_umma_takes(a); }
+// Few rows: lora_rows_gemm_kernel while its tiles are at most two blocks an SM, which is what runs at once. us in a graph, 16 adapters, K = 1280,
+// the tensor-core tiles and this kernel: 960 rows, N = 152, rank 8 31 and 19, rank 64 66 and 28; 1920 rows 31 and 29, 66 and 49; 256 rows,
+// N = 2048 28 and 28, 50 and 33; past two blocks: 448 rows, N = 2048 30 and 48; 1472, N = 600 33 and 49. Few columns and more rows:
+// 4800, N = 40, rank 64 73 and 79, at K = 64 27 and 38.
+// Rows that the kernel cannot take (not on 16 bytes) are laid out for the tensor cores from 512 on.
+constexpr int ROWS_MOST = 2048, ROWS_ODD = 511;
+bool on_16_bytes(const xb_lora_args& a) {
+  auto lies = [](const void* q, int64_t ld) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0 && ld % 8 == 0; };
+  return lies(a.X, a.ldx) && lies(a.W, a.ldw);
+}
+bool takes_rows_kernel(const xb_lora_args& a) {
+  const int64_t tiles = ((int64_t)a.N + ROWS_BN - 1) / ROWS_BN * ((a.M + ROWS_BM - 1) / ROWS_BM);
+  return a.dtype != XB_F32 && on_16_bytes(a) && a.M <= ROWS_MOST && tiles <= 2 * sm_count();
+}
+bool takes_tiles(const xb_lora_args& a) { return lora_umma_takes(a) && !takes_rows_kernel(a) && (on_16_bytes(a) || a.M > ROWS_ODD); }
 
 constexpr size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
@@ -200,9 +212,8 @@ int run_rows(const xb_lora_args& a, uint8_t* ws, cudaStream_t s) {
   g.lda = a.ldx; g.B = a.W; g.ldb = a.ldw; g.ldy = a.ldy; g.ab_dtype = a.dtype; g.y_dtype = a.y_dtype;
   g.bias = p.part; g.ldbias = a.N; g.bias_kind = XB_BIAS_FULL; g.bias_dtype = XB_F32;
   if constexpr (sizeof(T) == 2) {
-    // one turn of rows whose operands lie on 16 bytes: the projection and the products with B in one kernel
-    auto lies = [](const void* q, int64_t ld) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0 && ld % 8 == 0; };
-    if (a.M <= ROWS_MOST && lies(a.X, a.ldx) && lies(a.W, a.ldw)) {
+    // the projection and the products with B in one kernel (its rows are one turn: at most 2 sm_count() tiles of 64 x 32)
+    if (takes_rows_kernel(a)) {
       p.M = a.M;
       p.X = a.X;
       p.adapter = p.n_adapters ? a.adapter : nullptr;

@@ -930,7 +930,7 @@ int run_umma(const xb_lora_args& given, uint8_t* ws, cudaStream_t stream) {
     l.stages = std::min(MAX_STAGES, 220 * 1024 / stage);
     static PerDeviceOnce attr_set;
     XB_SET_MAX_SMEM_ONCE(attr_set, 226 * 1024, (const void*)lora_shrink_kernel);
-    // (every SM takes its share of B, with or without tiles: 520 rows, 16 adapters, N = 1024, rank 64, with a block a tile 220 us, SHRINK_NEW now)
+    // (every SM takes its share of B, with or without tiles: 520 rows, 16 adapters, N = 1024, rank 64, with a block a tile 220 us, 19 now)
     launch_dependent(lora_shrink_kernel, (unsigned)sm_count(), SHRINK_THREADS, (size_t)l.stages * stage + 1024, stream, mx, ma, l);
     if (int rc = check_launch("lora_shrink_kernel")) return rc;
   }
