@@ -175,7 +175,7 @@ constexpr int SHRINK_GROUP_ROWS = 64;     // rows of A (adapters x rb) in a stag
 // Persistent, 128 rows a tile. Bound by reading X once; the adapters' A come from L2. A pass over the depth takes the A of up to 64 / rb
 // adapters with it, one MMA for all of them; tiles of more adapters take more passes, each with an accumulator of its own. (With
 // an MMA for each adapter that masks the others' rows out the warp that issues them bounded the kernel: a masked MMA takes it about
-// 150 cycles. [65536, 1280], rank 16: 54 us.)
+// 150 cycles. [65536, 1280], rank 16, 32 adapters: 54 us so, 40 now = 4.5 TB/s, 0.70 of a copy's rate.)
 __global__ void __launch_bounds__(SHRINK_THREADS, 1)
 lora_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ LoraTiles p) {
   using namespace umma;
@@ -299,6 +299,8 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
 
 // The one-CTA GEMM kernel of xb_gemm_umma.cu without batches and resident weights, whose tiles go on through the adapters' products: the
 // stages have the same size (128 rows of 128 bytes of X or U, block_n of W or B), only the maps and the MMAs differ.
+// [65536, 1280] x [1280, 1024], 32 adapters of rank 16: 155 us = 1.1 PFLOP/s, tensor pipe 62 % busy. One-CTA tiles of 128 x 256 read 48 KB
+// from L2 for 64 of the depth, which is the bound; xb_gemm's pairs of CTAs halve W's part of it (130-140 us for the projection alone).
 enum { LORA_Y_TMA, LORA_Y_ANY };
 template <typename TOut, bool B_MN, int Y>
 __global__ void __launch_bounds__(GEMM_THREADS, 1)
@@ -494,8 +496,9 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
 // Products of one column of tiles: both steps in one kernel, X read once. A tile's walk over the depth makes its projection and, in the same
 // MMAs, the U of up to `group` adapters beside it in tensor memory (further adapters: U alone, over the depth once more). Four warps
 // take U out, scale and split it, widen B to fp32 beside it, and leave both in shared memory as the operands of U B^T, which is issued
-// after the next walk, so that nobody waits for them. [74000, 324] x [324, 200], rank 8: 40 us as two kernels. What bounds it is the
-// way from L2: 42 KB of X and W for each 64 of the depth.
+// after the next walk, so that nobody waits for them. [74000, 324] x [324, 200], rank 8: 41 us as two kernels, 35
+// now. What bounds it is the way from L2, 47 KB of X, W and A for each 64 of the depth, and four tiles a CTA whose first and last
+// steps nothing overlaps.
 constexpr int FUSED_THREADS = GEMM_THREADS + 128;
 constexpr int FUSED_MAX_RB = 32;                           // (the operands of a larger rank would take the ring's space)
 struct LoraItem {                                          // one walk

@@ -71,8 +71,8 @@ struct ConvTaps {
   }
 };
 
-// One row a list: a thread has V channels of it. All that it reads, states, row and weights, is on its way at once; what the walk reads
-// one after the other is the time of a call of few rows.
+// One row a list: a thread has V channels of it. All that it reads, states, row and weights, is on its way at once, where the walk reads one
+// after the other. 4 taps: 74 rows of 72 in a graph 4.3 us as a walk, 1.95 so; 8192 rows of 256, bf16, 27 and 7.3 (4.6 TB/s).
 template <typename T, int V, int K>
 __global__ void __launch_bounds__(CONV_THREADS) ssm_conv_step_kernel(const ConvParams p) {
   pdl_begin();
@@ -107,7 +107,9 @@ __global__ void __launch_bounds__(CONV_THREADS) ssm_conv_step_kernel(const ConvP
 // The thread that has a list's first row makes its first K - 1 rows (they read the state) and its last state, so that states moved
 // on in place are read and written by one thread.
 // Pieces of 8 bytes and eight rows ahead: with 16-byte pieces and four rows the registers let half as many warps in, which is what
-// the loads in flight are. SiLU is the rest: two exponentials and a quotient for two values.
+// the loads in flight are. SiLU is the rest: two exponentials and a quotient for two values. Bound by the latency of the reads in flight:
+// 1024 lists of 262144 rows in all, D = 512, bf16 134 us = 4.0 TB/s, 0.62 of a copy's rate, 24 warps an SM, SFUs 36 % busy. The
+// next rows asked for before these are written, and longer or shorter walks, are no faster.
 template <typename T, int V, int K>
 constexpr int CONV_BLOCKS = K <= 4 && V * sizeof(T) <= 8 ? 6 : 4;         // of an SM: the registers are shared among so many
 template <typename T, int V, int K>
