@@ -146,6 +146,32 @@ int turn_rows(const xb_lora_args& a) {
   return (int)std::min<int64_t>(rows, a.M);
 }
 
+// fp32 weights as [N, K] are laid out as [K, N] first, for which xb_gemm has a faster kernel. us in a graph without and with, whatever the rows:
+// 8 rows, K = 72, N = 168 12 and 10, K = 1280, N = 1024 50 and 39; 3931 rows of the first 51 and 35; 20000 rows, K = 324, N = 200 194 and 168.
+bool lays_out_w(const xb_lora_args& a) { return a.dtype == XB_F32 && a.trans_w; }
+int64_t laid_out_ld(const xb_lora_args& a) { return ((int64_t)a.N + 3) / 4 * 4; }
+struct RowsScratch { size_t part, w, bytes; };             // U lies first
+RowsScratch rows_scratch(const xb_lora_args& a) {
+  const size_t turn = (size_t)turn_rows(a);
+  RowsScratch s;
+  s.part = align256(turn * a.r * 4);
+  s.w = s.part + align256(turn * a.N * 4);
+  s.bytes = s.w + (lays_out_w(a) ? (size_t)a.K * laid_out_ld(a) * 4 : 0);
+  return s;
+}
+__global__ void __launch_bounds__(256) lora_layout_kernel(const float* w, int64_t ldw, float* to, int64_t ld, int N, int K) {
+  pdl_begin();
+  __shared__ float tile[32][33];
+  const int across = (K + 31) / 32, n0 = (int)(blockIdx.x / across) * 32, k0 = (int)(blockIdx.x % across) * 32, x = threadIdx.x % 32, y = threadIdx.x / 32;
+#pragma unroll
+  for (int i = y; i < 32; i += 8)
+    if (n0 + i < N && k0 + x < K) tile[i][x] = w[(int64_t)(n0 + i) * ldw + k0 + x];
+  __syncthreads();
+#pragma unroll
+  for (int i = y; i < 32; i += 8)
+    if (k0 + i < K && n0 + x < N) to[(int64_t)(k0 + i) * ld + n0 + x] = tile[x][i];
+}
+
 int check_args(const xb_lora_args* a) {
   XB_REQUIRE(a, XB_ERR_ARG, "xb_lora_gemm: null arguments");
   XB_REQUIRE(a->dtype == XB_F32 || a->dtype == XB_F16 || a->dtype == XB_BF16, XB_ERR_UNSUPPORTED, "xb_lora_gemm: dtype %d", a->dtype);
@@ -200,7 +226,8 @@ int run_rows(const xb_lora_args& a, uint8_t* ws, cudaStream_t s) {
   p.A = a.A; p.lda = a.lda; p.stride_a = a.stride_a; p.B = a.B; p.ldb = a.ldb; p.stride_b = a.stride_b;
   p.scale = a.scale; p.bias = a.bias; p.ldx = a.ldx;
   p.U = reinterpret_cast<float*>(ws);
-  p.part = reinterpret_cast<float*>(ws + align256((size_t)turn * a.r * 4));
+  const RowsScratch scratch = rows_scratch(a);
+  p.part = reinterpret_cast<float*>(ws + scratch.part);
   // 16-byte pieces of X and A along K, and of B along the rank
   constexpr int V = 16 / (int)sizeof(T);
   const bool vec_k = a.K % V == 0 && a.ldx % V == 0 && a.lda % V == 0 && a.stride_a % V == 0 &&
@@ -229,6 +256,14 @@ int run_rows(const xb_lora_args& a, uint8_t* ws, cudaStream_t s) {
       while (r.split < 8 && 2 * r.split <= slices && tiles * 2 * r.split <= 2 * sm_count()) r.split *= 2;
       return a.trans_w ? launch_rows_gemm<T, true>(r, s) : launch_rows_gemm<T, false>(r, s);
     }
+  }
+  if (lays_out_w(a)) {
+    const int64_t blocks = (((int64_t)a.K + 31) / 32) * (((int64_t)a.N + 31) / 32);
+    XB_REQUIRE(blocks < ((int64_t)1 << 31), XB_ERR_LIMIT, "xb_lora_gemm: weights of %d x %d are too many for one call", a.K, a.N);
+    float* to = reinterpret_cast<float*>(ws + scratch.w);
+    launch_dependent(lora_layout_kernel, (unsigned)blocks, 256, 0, s, static_cast<const float*>(a.W), a.ldw, to, laid_out_ld(a), a.N, a.K);
+    if (int rc = check_launch("lora_layout_kernel")) return rc;
+    g.B = to; g.ldb = laid_out_ld(a); g.trans_b = 0;
   }
   for (int64_t m0 = 0; m0 < a.M; m0 += turn) {
     p.M = (int)std::min<int64_t>(turn, a.M - m0);
@@ -259,8 +294,7 @@ using namespace xb;
 extern "C" size_t xb_lora_workspace_bytes(const xb_lora_args* a) {
   if (check_args(a) != 0 || a->M == 0 || a->N == 0) return 0;
   if (takes_tiles(*a)) return lora_scratch(*a).bytes;
-  const size_t turn = (size_t)turn_rows(*a);
-  return align256(turn * a->r * 4) + turn * a->N * 4;
+  return rows_scratch(*a).bytes;
 }
 
 extern "C" int xb_lora_gemm(const xb_lora_args* a, void* workspace, size_t workspace_bytes, xb_stream_t s) {

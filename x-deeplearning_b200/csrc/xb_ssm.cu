@@ -334,7 +334,7 @@ ScanPlan scan_plan(const xb_ssm_scan_args& a) {
     const double work = K == 2 ? 155 : 80, alone = K == 1 ? 130 : p.lanes <= 4 ? 260 : 32 * p.lanes;
     const int blocks = scan_blocks(a, p.lanes, K);
     const double full = (double)a.rows * blocks * work / sms;
-    // lists of unlike lengths in more than a wave of blocks: long ones first
+    // lists of unlike lengths in more than a wave of blocks: long ones first (one block puts them in order: up to 64 rounds of its threads)
     const bool order = a.offsets && longest > 1.5 * mean && a.batch <= 65536 && (double)a.batch * blocks > 5 * sms;
     const double whole = (order ? std::max(full + 6000, alone * longest) : full + 0.6 * alone * longest) + 600.0 * a.batch * blocks / sms;
     if (best == 0 || whole < best) { best = whole; p.K = K; p.chunk = 0; p.order = order; }
