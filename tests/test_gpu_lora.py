@@ -107,7 +107,8 @@ def test_bad_values_stay_in_their_rows(M):
 @pytest.mark.parametrize("M,K,N,n,r,trans", [
     (600, 1, 24, 3, 2, True), (520, 5, 40, 2, 3, False), (511, 3, 8, 2, 1, True), (600, 72, 304, 300, 12, True), (9500, 72, 200, 300, 8, True),
     (9500, 40, 304, 2, 128, False), (700, 2000, 1, 5, 40, True),
-    (1, 64, 10000, 3, 8, True), (64, 72, 10000, 40, 16, False), (200, 136, 2800, 9, 64, True), (2048, 72, 136, 9, 24, True), (2049, 72, 136, 9, 24, False)])
+    (1, 64, 10000, 3, 8, True), (64, 72, 10000, 40, 16, False), (200, 136, 2800, 9, 64, True), (2048, 72, 136, 9, 24, True), (2049, 72, 136, 9, 24, False),
+    (70, 648, 72, 5, 128, True), (300, 64, 104, 3, 104, False), (65, 64, 33, 3, 100, True)])
 def test_shallow_products_and_tiles_of_many_adapters(dtype, out, M, K, N, n, r, trans):
     s = _case(np.random.default_rng(K + n), M, K, N, n, r, dtype, trans, 0, "mixed")
     _check(s, dtype, out, trans)
