@@ -1,0 +1,24 @@
+"""xb_lora_gemm where single lanes, tables and sizes differ from the ordinary: against its formula in 64 bits (tests/ssm_oracle.py)."""
+import numpy as np
+import pytest
+import torch
+
+import pkg
+import ssm_oracle
+from test_gpu_lora import T_, _case, _check, _np, _ops
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("M,N", [(700, 304), (9600, 72)])
+@pytest.mark.parametrize("r", [17, 32, 100, 128])
+def test_lanes_of_a_warp_with_adapters_of_their_own(M, N, r):
+    """Rows of a warp that take nothing of an adapter's U beside rows that do, for every column block of a rank above 16: one row in 32, every
+    other one, and all but one."""
+    rng = np.random.default_rng(M + r)
+    s = _case(rng, M, 72, N, 3, r, "bf16", True, 0, "none")
+    rows = np.arange(M)
+    for own in (rows % 32 == 5, rows % 2 == 1, rows % 32 != 9):
+        s["adapter"] = torch.from_numpy(np.where(own, rows // 128 % 3, -1).astype(np.int32)).cuda()
+        _check(s, "bf16", "bf16", True)
+    assert _ops()[0].device_status() == 0

@@ -266,17 +266,18 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
               uint32_t raw[16];
               tmem_ld16_nowait(acc + i * p.rb + c + ((uint32_t)(q * 32) << 16), raw);
               tmem_wait_ld(raw);
-              if (mine != pass.id[i]) continue;
+              if (mine == pass.id[i]) {
 #pragma unroll
-              for (int j = 0; j < 16; j += 4) {
-                float hi[4], lo[4];
+                for (int j = 0; j < 16; j += 4) {
+                  float hi[4], lo[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) split_tf32(c + j + e < p.r ? scale * __uint_as_float(raw[j + e]) : 0.f, hi[e], lo[e]);
-                *reinterpret_cast<float4*>(u + c + j) = make_float4(hi[0], hi[1], hi[2], hi[3]);
-                *reinterpret_cast<float4*>(u + p.rb + c + j) = make_float4(lo[0], lo[1], lo[2], lo[3]);
+                  for (int e = 0; e < 4; ++e) split_tf32(c + j + e < p.r ? scale * __uint_as_float(raw[j + e]) : 0.f, hi[e], lo[e]);
+                  *reinterpret_cast<float4*>(u + c + j) = make_float4(hi[0], hi[1], hi[2], hi[3]);
+                  *reinterpret_cast<float4*>(u + p.rb + c + j) = make_float4(lo[0], lo[1], lo[2], lo[3]);
+                }
               }
+              __syncwarp();                                // (the next load of tensor memory is the whole warp's)
             }
-            __syncwarp();
           }
           tc_fence_before_sync();
           __syncwarp();
@@ -730,17 +731,18 @@ lora_fused_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
               uint32_t raw[16];
               tmem_ld16_nowait(tmem_base + (item.it & 1) * acc_stride + p.block_n + k * l.rb + c + ((uint32_t)(q * 32) << 16), raw);
               tmem_wait_ld(raw);
-              if (mine != item.id[k]) continue;
+              if (mine == item.id[k]) {
 #pragma unroll
-              for (int j = 0; j < 16; j += 4) {
-                float hi[4], lo[4];
+                for (int j = 0; j < 16; j += 4) {
+                  float hi[4], lo[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) split_tf32(c + j + e < l.r ? scale * __uint_as_float(raw[j + e]) : 0.f, hi[e], lo[e]);
-                put(smem_u, row, c + j, hi);               // (hi and lo of 16 columns share the one block there is, of 32 they have one each)
-                put(smem_u + (l.rb >> 5) * A_STAGE_BYTES, row, (l.rb == 16 ? 16 : 0) + c + j, lo);
+                  for (int e = 0; e < 4; ++e) split_tf32(c + j + e < l.r ? scale * __uint_as_float(raw[j + e]) : 0.f, hi[e], lo[e]);
+                  put(smem_u, row, c + j, hi);             // (hi and lo of 16 columns share the one block there is, of 32 they have one each)
+                  put(smem_u + (l.rb >> 5) * A_STAGE_BYTES, row, (l.rb == 16 ? 16 : 0) + c + j, lo);
+                }
               }
+              __syncwarp();                                // (the next load of tensor memory is the whole warp's)
             }
-            __syncwarp();
           }
           tc_fence_before_sync();
           ++walks;
