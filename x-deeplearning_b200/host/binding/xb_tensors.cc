@@ -146,7 +146,7 @@ struct Call {
   void* scratch(PyObject* given, const at::Tensor& like, size_t need, size_t* have, at::Tensor& own) {
     if (given != Py_None) {
       const View v = view(given, "workspace");
-      if (v.dim != 1 || v.stride[0] > 1 || tensor(given, "workspace").element_size() != 1) refuse("the workspace is a contiguous uint8 vector");
+      if (v.dim != 1 || (v.size[0] > 1 && v.stride[0] != 1) || tensor(given, "workspace").element_size() != 1) refuse("the workspace is a contiguous uint8 vector");
       *have = (size_t)v.size[0];
       return v.at;
     }
