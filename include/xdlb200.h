@@ -524,6 +524,7 @@ int xb_augru_shared(const void* x, const void* att, void* y_final, int32_t reque
  * i). The two may be the same array: the states are then moved on in place. Two lists of a call never share a slot. A slot
  * outside [0, n_slots) begins with zeros and is not kept. First array NULL: every list begins with zeros; second NULL: nothing
  * is kept. An empty list leaves the state that it began with.
+ * Fewer than 2^31 rows; lists and channels at most 2^31 - 1024.
  * x, y, z, delta, B, C share `dtype` (XB_F32, XB_F16, XB_BF16); every sum and the scan's states are fp32. Outputs overlap no
  * input. An infinity or NaN in a row makes no other list's results bad; its own list's may be NaN where the formula has an infinity. */
 

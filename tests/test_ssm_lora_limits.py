@@ -22,3 +22,66 @@ def test_scratch_whose_bytes_are_one(bound):  # noqa: F811
     assert not seen
     ops.ssm_scan(x, x, torch.zeros(24, 16), x[:, :16], x[:, :16], workspace=torch.zeros(4096, dtype=torch.uint8)[:1])
     assert seen[-1][1][1] == 1
+
+
+AT, ARG, LIMIT = 4096, -1, -5
+
+
+def _conv(c, **k):
+    a = c.SsmConvArgs()
+    a.x = a.y = a.w = AT
+    a.y += 1 << 20
+    a.rows, a.batch, a.D, a.K, a.dtype, a.ldx, a.ldy = 12, 3, 24, 4, c.XB_F16, 24, 24
+    for n, v in k.items():
+        setattr(a, n, v)
+    return a
+
+
+def _scan(c, **k):
+    a = c.SsmScanArgs()
+    a.x = a.delta = a.B = a.C = a.A = AT
+    a.y = AT + (1 << 20)
+    a.rows, a.batch, a.D, a.N, a.groups, a.dtype = 12, 3, 24, 16, 2, c.XB_BF16
+    a.ldx = a.lddelta = a.ldy = 24
+    a.ldb = a.ldc = 32
+    for n, v in k.items():
+        setattr(a, n, v)
+    return a
+
+
+def _lora(c, **k):
+    a = c.LoraArgs()
+    a.X = a.W = a.A = a.B = a.adapter = AT
+    a.Y = AT + (1 << 20)
+    a.M, a.N, a.K, a.r, a.n_adapters, a.trans_w, a.dtype, a.y_dtype = 10, 16, 32, 8, 3, 1, c.XB_F16, c.XB_F16
+    a.ldx = a.ldw = a.lda = 32
+    a.ldy, a.ldb, a.stride_a, a.stride_b = 16, 8, 256, 128
+    for n, v in k.items():
+        setattr(a, n, v)
+    return a
+
+
+def test_channels_and_lists_that_round_up_past_32_bits():
+    m = pkg.load()
+    c, L = m.capi, m.lib()
+    most = (1 << 31) - 1
+    for k in (dict(D=most, ldx=most, ldy=most), dict(D=most - 1022, ldx=most, ldy=most), dict(batch=most, rows=4, offsets=AT), dict(batch=most, rows=0)):
+        assert L.xb_ssm_conv(C.byref(_conv(c, **k)), None) == LIMIT, k
+        assert b"xb_ssm_conv" in L.xb_last_error()
+    for k in (dict(D=most, groups=1, ldx=most, ldy=most, lddelta=most), dict(batch=most, rows=4, offsets=AT), dict(batch=most - 1022, rows=0)):
+        a = _scan(c, **k)
+        assert L.xb_ssm_scan_workspace_bytes(C.byref(a)) == 0 and L.xb_ssm_scan(C.byref(a), None, 0, None) == LIMIT, k
+        assert b"xb_ssm_scan" in L.xb_last_error()
+
+
+def test_adapters_whose_scratch_passes_64_bits():
+    """Adapters that share their memory (strides of 0 and 1) are a small tensor; what is laid out of them is not."""
+    m = pkg.load()
+    c, L = m.capi, m.lib()
+    most = (1 << 31) - 1024
+    for k in (dict(M=most, N=most, ldy=most, n_adapters=most, r=128, ldb=128, stride_a=0, stride_b=0),
+              dict(M=most, K=most, ldx=most, ldw=most, lda=most, n_adapters=most, r=128, ldb=128, stride_a=1, stride_b=0)):
+        a = _lora(c, **k)
+        assert L.xb_lora_workspace_bytes(C.byref(a)) == 0, k
+        assert L.xb_lora_gemm(C.byref(a), AT, 1 << 60, None) == LIMIT, k
+        assert b"xb_lora_gemm" in L.xb_last_error()

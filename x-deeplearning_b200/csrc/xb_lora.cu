@@ -188,6 +188,8 @@ int check_args(const xb_lora_args* a) {
   XB_REQUIRE(!adapters || (a->adapter && a->B && a->A), XB_ERR_ARG, "xb_lora_gemm: null adapter");
   XB_REQUIRE(!adapters || (a->lda >= a->K && a->ldb >= a->r && a->stride_a >= 0 && a->stride_b >= 0), XB_ERR_ARG,
              "xb_lora_gemm: a stride of the adapters is too small");
+  XB_REQUIRE(!takes_tiles(*a) || lora_scratch(*a).fits, XB_ERR_LIMIT, "xb_lora_gemm: %d adapters of rank %d beside %d x %d x %d are too many for one call",
+             a->n_adapters, a->r, a->M, a->N, a->K);
   return 0;
 }
 

@@ -871,6 +871,7 @@ struct LoraScratch {
   int rb, u_cols, b_cols;
   int fused_group;                        // adapters of a walk where both steps are one kernel, 0 where they are two
   size_t u, b, x, w, a, bytes;
+  bool fits;                              // in what the sizes above count
 };
 LoraScratch lora_scratch(const xb_lora_args& a) {
   LoraScratch w;
@@ -889,6 +890,9 @@ LoraScratch lora_scratch(const xb_lora_args& a) {
   w.w = w.x + rows(c.x, a.M);
   w.a = w.w + rows(c.w, a.N);
   w.bytes = w.a + rows(c.a, (int64_t)a.n_adapters * a.r);
+  // (adapters may share their memory, so what is laid out of them has no bound in what the caller holds)
+  const double all = 4.0 * a.M * w.u_cols + 4.0 * a.n_adapters * a.N * w.b_cols + 2.0 * c.ld * (c.x * (double)a.M + c.w * (double)a.N + c.a * (double)a.n_adapters * a.r);
+  w.fits = all < 1.0e15;
   return w;
 }
 

@@ -247,8 +247,10 @@ __global__ void __launch_bounds__(CONV_THREADS, CONV_BLOCKS<T, V, K>) ssm_conv_k
   }
 }
 
-int check_lists(const char* what, const int32_t* offsets, const int32_t* slots, bool states, int64_t rows, int32_t batch, int32_t n_slots) {
+constexpr int32_t MOST = INT32_MAX - 1023;             // of channels and lists: rounded up to whole blocks they are counted in 32 bits
+int check_lists(const char* what, const int32_t* offsets, const int32_t* slots, bool states, int64_t rows, int32_t batch, int32_t n_slots, int32_t D) {
   XB_REQUIRE(rows >= 0 && batch >= 0, XB_ERR_ARG, "%s: %lld rows, %d lists", what, (long long)rows, batch);
+  XB_REQUIRE(batch <= MOST && D <= MOST, XB_ERR_LIMIT, "%s: %d lists, %d channels, at most 2^31 - 1024", what, batch, D);
   XB_REQUIRE(rows < ((int64_t)1 << 31), XB_ERR_LIMIT, "%s: %lld rows, fewer than 2^31", what, (long long)rows);
   XB_REQUIRE(offsets || batch == 0 || rows % batch == 0, XB_ERR_ARG, "%s: without offsets %d lists divide %lld rows", what, batch, (long long)rows);
   XB_REQUIRE(!states || n_slots >= 0, XB_ERR_ARG, "%s: n_slots %d", what, n_slots);
@@ -392,7 +394,7 @@ extern "C" int xb_ssm_conv(const xb_ssm_conv_args* a, xb_stream_t s) {
   XB_REQUIRE(ssm_dtype(a->dtype), XB_ERR_UNSUPPORTED, "xb_ssm_conv: dtype %d", a->dtype);
   XB_REQUIRE(a->D >= 1, XB_ERR_ARG, "xb_ssm_conv: %d channels", a->D);
   XB_REQUIRE(a->K >= 2 && a->K <= 8, XB_ERR_LIMIT, "xb_ssm_conv: %d taps, from 2 to 8", a->K);
-  if (int rc = check_lists("xb_ssm_conv", a->offsets, a->slots, a->state_in || a->state_out, a->rows, a->batch, a->n_slots)) return rc;
+  if (int rc = check_lists("xb_ssm_conv", a->offsets, a->slots, a->state_in || a->state_out, a->rows, a->batch, a->n_slots, a->D)) return rc;
   if (a->batch == 0) return 0;
   XB_REQUIRE(a->w && (a->rows == 0 || (a->x && a->y)), XB_ERR_ARG, "xb_ssm_conv: null tensor");
   XB_REQUIRE(a->rows == 0 || (a->ldx >= a->D && a->ldy >= a->D), XB_ERR_ARG, "xb_ssm_conv: row strides %lld, %lld of %d channels",
@@ -410,7 +412,7 @@ int check_scan(const xb_ssm_scan_args* a) {
              a->D, a->groups, a->N);
   XB_REQUIRE(a->N <= 64, XB_ERR_LIMIT, "xb_ssm_scan: %d states, at most 64", a->N);
   XB_REQUIRE(a->longest >= 0, XB_ERR_ARG, "xb_ssm_scan: longest %lld", (long long)a->longest);
-  if (int rc = check_lists("xb_ssm_scan", a->offsets, a->slots, a->h_in || a->h_out, a->rows, a->batch, a->n_slots)) return rc;
+  if (int rc = check_lists("xb_ssm_scan", a->offsets, a->slots, a->h_in || a->h_out, a->rows, a->batch, a->n_slots, a->D)) return rc;
   if (a->batch == 0) return 0;
   XB_REQUIRE(a->A && (a->rows == 0 || (a->x && a->delta && a->B && a->C && a->y)), XB_ERR_ARG, "xb_ssm_scan: null tensor");
   XB_REQUIRE(a->rows == 0 || (a->ldx >= a->D && a->lddelta >= a->D && a->ldy >= a->D && (!a->z || a->ldz >= a->D)), XB_ERR_ARG,
