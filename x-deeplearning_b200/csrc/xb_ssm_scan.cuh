@@ -474,20 +474,23 @@ __global__ void __launch_bounds__(32 * CARRY_PARTS) ssm_carry_kernel(const ScanP
   const float A = mine ? LOG2E * p.A[at] : 0.f;
   const int n = p.n_ends, share = (n + CARRY_PARTS - 1) / CARRY_PARTS, j0 = min(n, part * share), j1 = min(n, j0 + share);
   float P = 1.f, e = 0.f;
+  // (a chunk that is its list's first, or none, cuts off what came before it: a product with 0 would keep another list's NaN)
   auto one = [&](int j, float& through, float& own) {
     const int kind = p.kind[j];
     const float end = mine ? p.end[j * pairs + at] : 0.f, decay = ex2(A * p.steps[(int64_t)j * p.D + c]);
     own = kind ? end : 0.f;
     through = mine && kind == 2 ? decay : 0.f;
+    return kind == 2;
   };
+  bool cut = false;
 #pragma unroll 8
   for (int j = j0; j < j1; ++j) {
     float t, o;
-    one(j, t, o);
+    cut |= !one(j, t, o);
     e = t == 0.f ? o : fmaf(t, e, o);
     P *= t;
   }
-  s_p[part][lane] = P;
+  s_p[part][lane] = cut ? 0.f : P;
   s_e[part][lane] = e;
   __syncthreads();
   e = 0.f;
