@@ -62,3 +62,31 @@ def test_growth_of_a_broken_list_and_the_next():
     s["delta"][4500:5000] = 4.0
     again, kept2 = _call(ops, s, off, h, 5000, softplus=False)
     assert torch.equal(again[5000:], y[5000:]) and torch.equal(kept2[1], kept[1])
+
+
+@pytest.mark.parametrize("value", ["nan", "inf"])
+def test_a_broken_list_stays_broken(value):
+    """A NaN (or an infinity) in the state stays to the list's end, whole or in chunks whose decay is nothing in fp32."""
+    ops, capi = _ops()
+    s, off, h = _two(np.random.default_rng(33))
+    s["A"].fill_(-16.0)
+    s["delta"].fill_(0.0)
+    s["bias"].fill_(float(np.log(np.expm1(0.2))))               # steps of 0.2: a chunk of 64 rows decays by exp(-204)
+    for longest in (5000, 0):
+        assert _chunks(capi, 10000, 2, 40, 16, longest, capi.XB_F32)
+        s["x"][100, :] = 1.0
+        y, kept = _call(ops, s, off, h, longest, delta_bias=s["bias"])
+        s["x"][100, :] = float(value)
+        again, kept2 = _call(ops, s, off, h, longest, delta_bias=s["bias"])
+        assert torch.equal(again[:100], y[:100]) and torch.equal(again[5000:], y[5000:]) and torch.equal(kept2[1], kept[1])
+        assert not torch.isfinite(again[100:5000]).any() and not torch.isfinite(kept2[0]).any()
+        # the same list alone, in rows enough lists that nothing is split
+    n, t = 2000, 300
+    rng = np.random.default_rng(34)
+    w = _scan_inputs(rng, n * t, 0, 8, 4, 1, "f32", 0, 0)
+    w["A"].fill_(-16.0)
+    w["delta"].fill_(0.0)
+    w["bias"].fill_(float(np.log(np.expm1(0.2))))
+    w["x"][100] = float(value)
+    y = ops.ssm_scan(w["x"], w["delta"], w["A"], w["B"], w["C"], delta_bias=w["bias"], T=t)
+    assert not torch.isfinite(y[100:t]).any() and torch.isfinite(y[:100]).all() and torch.isfinite(y[t:]).all()

@@ -467,6 +467,7 @@ constexpr int CARRY_PARTS = 32;
 __global__ void __launch_bounds__(32 * CARRY_PARTS) ssm_carry_kernel(const ScanParams p) {
   pdl_begin();
   __shared__ float s_p[CARRY_PARTS][32], s_e[CARRY_PARTS][32];
+  __shared__ bool s_cut[CARRY_PARTS];                   // a list begins in the part
   const int part = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int64_t pairs = (int64_t)p.D * p.N, at = (int64_t)blockIdx.x * 32 + lane;
   const bool mine = at < pairs;
@@ -474,32 +475,34 @@ __global__ void __launch_bounds__(32 * CARRY_PARTS) ssm_carry_kernel(const ScanP
   const float A = mine ? LOG2E * p.A[at] : 0.f;
   const int n = p.n_ends, share = (n + CARRY_PARTS - 1) / CARRY_PARTS, j0 = min(n, part * share), j1 = min(n, j0 + share);
   float P = 1.f, e = 0.f;
-  // (a chunk that is its list's first, or none, cuts off what came before it: a product with 0 would keep another list's NaN)
+  // (a chunk that is its list's first, or none, cuts off what came before it: a product with 0 would keep another list's NaN. A decay that is
+  // 0 is none of this: what came in may be a NaN, which stays to its list's end.)
   auto one = [&](int j, float& through, float& own) {
     const int kind = p.kind[j];
     const float end = mine ? p.end[j * pairs + at] : 0.f, decay = ex2(A * p.steps[(int64_t)j * p.D + c]);
     own = kind ? end : 0.f;
-    through = mine && kind == 2 ? decay : 0.f;
+    through = decay;
     return kind == 2;
   };
   bool cut = false;
 #pragma unroll 8
   for (int j = j0; j < j1; ++j) {
     float t, o;
-    cut |= !one(j, t, o);
-    e = t == 0.f ? o : fmaf(t, e, o);
+    const bool on = one(j, t, o);
+    cut |= !on;
+    e = on ? fmaf(t, e, o) : o;
     P *= t;
   }
-  s_p[part][lane] = cut ? 0.f : P;
+  if (lane == 0) s_cut[part] = cut;
+  s_p[part][lane] = P;
   s_e[part][lane] = e;
   __syncthreads();
   e = 0.f;
-  for (int k = 0; k < part; ++k) e = s_p[k][lane] == 0.f ? s_e[k][lane] : fmaf(s_p[k][lane], e, s_e[k][lane]);
+  for (int k = 0; k < part; ++k) e = s_cut[k] ? s_e[k][lane] : fmaf(s_p[k][lane], e, s_e[k][lane]);
 #pragma unroll 8
   for (int j = j0; j < j1; ++j) {
     float t, o;
-    one(j, t, o);
-    e = t == 0.f ? o : fmaf(t, e, o);
+    e = one(j, t, o) ? fmaf(t, e, o) : o;
     if (mine) p.end[j * pairs + at] = e;
   }
 }
