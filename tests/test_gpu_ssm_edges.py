@@ -90,3 +90,24 @@ def test_a_broken_list_stays_broken(value):
     w["x"][100] = float(value)
     y = ops.ssm_scan(w["x"], w["delta"], w["A"], w["B"], w["C"], delta_bias=w["bias"], T=t)
     assert not torch.isfinite(y[100:t]).any() and torch.isfinite(y[:100]).all() and torch.isfinite(y[t:]).all()
+
+
+@pytest.mark.parametrize("A,h0", [(8.0, 0.0), (8.0, 1e-32), (-8.0, 1e30), (-8.0, 1.0)])
+def test_chunks_whose_decay_fp32_does_not_hold(A, h0):
+    """exp of a chunk's steps above 2^128 or below 2^-126 with a state that makes the product an ordinary number, or zero."""
+    ops, capi = _ops()
+    D, N, t = 8, 4, 6000
+    rng = np.random.default_rng(35)
+    s = _scan_inputs(rng, t, 0, D, N, 1, "f32", 0, 0)
+    off = torch.tensor([0, t], dtype=torch.int32, device="cuda")
+    assert _chunks(capi, t, 1, D, N, t, capi.XB_F32)
+    s["A"].fill_(A)
+    s["x"].zero_()
+    s["delta"].zero_()
+    s["delta"][960:1024] = 0.25                                 # 64 rows: exp(+-128) = 2^+-185
+    h = torch.full((1, D, N), h0, device="cuda")
+    y, kept = _call(ops, s, off, h, t, softplus=False)
+    want, bound, last, elast = _scan_want(s, [(0, t)], 1, _np(h), "f32", bias=False, softplus=False)
+    ssm_oracle.close(_np(y), want, bound, "y")
+    ssm_oracle.close(_np(kept), np.stack(last), np.stack(elast), "states")
+    assert h0 != 0 or (y == 0).all()

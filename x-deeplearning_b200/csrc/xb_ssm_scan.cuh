@@ -458,15 +458,30 @@ __global__ void __launch_bounds__(1024) ssm_order_kernel(const ScanParams p) {
   for (int i = tid; i < p.lists.batch; i += 1024) p.order[atomicAdd(&s_at[class_of(i)], 1)] = i;
 }
 
+// 2^q for any q: the rows of a chunk each have a decay that fp32 holds where the chunk's need not, so it comes as three factors of exponents up
+// to 126 (beyond 378 no finite state but 0 gives a number that is neither infinite nor 0; an infinite q is the rows' own).
+constexpr float NEAR = 126.f;
+struct Decay {
+  float f[3];
+  __device__ __forceinline__ void of(float q) {
+    auto part = [](float v) { return fminf(fmaxf(v, -NEAR), NEAR); };
+    const float q1 = part(q), q2 = part(q - q1), rest = q - q1 - q2;
+    f[0] = ex2(q1);
+    f[1] = ex2(q2);
+    f[2] = ex2(fabsf(rest) <= 3.4028235e38f ? part(rest) : rest);
+  }
+  __device__ __forceinline__ float apply(float e, float own) const { return fmaf(f[0], f[1] * (f[2] * e), own); }
+};
+
 // What the ends are with the states that come into their chunks: end[j] += exp(A steps[j]) end[j - 1] where chunk j is not its list's first. A
-// block has 32 (channel, state) pairs and splits the chunks among its 32 warps: each makes its own part's product and sum, takes what
+// block has 32 (channel, state) pairs and splits the chunks among its 32 warps: each makes its own part's decay and sum, takes what
 // comes in from the parts before it, and walks its part again. Bound by the latency of its reads: none waits for another (what stands in
 // the place of a chunk that is none is dropped). [30011, 202], N = 10, 156 chunks: the call 145 us with 8 warps that asked first what
 // a chunk is, 128 now.
 constexpr int CARRY_PARTS = 32;
 __global__ void __launch_bounds__(32 * CARRY_PARTS) ssm_carry_kernel(const ScanParams p) {
   pdl_begin();
-  __shared__ float s_p[CARRY_PARTS][32], s_e[CARRY_PARTS][32];
+  __shared__ float s_f[3][CARRY_PARTS][32], s_e[CARRY_PARTS][32];
   __shared__ bool s_cut[CARRY_PARTS];                   // a list begins in the part
   const int part = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int64_t pairs = (int64_t)p.D * p.N, at = (int64_t)blockIdx.x * 32 + lane;
@@ -474,35 +489,48 @@ __global__ void __launch_bounds__(32 * CARRY_PARTS) ssm_carry_kernel(const ScanP
   const int c = mine ? (int)(at / p.N) : 0;
   const float A = mine ? LOG2E * p.A[at] : 0.f;
   const int n = p.n_ends, share = (n + CARRY_PARTS - 1) / CARRY_PARTS, j0 = min(n, part * share), j1 = min(n, j0 + share);
-  float P = 1.f, e = 0.f;
+  float Q = 0.f, e = 0.f;                                // the part: e <- 2^Q e + its own e
   // (a chunk that is its list's first, or none, cuts off what came before it: a product with 0 would keep another list's NaN. A decay that is
   // 0 is none of this: what came in may be a NaN, which stays to its list's end.)
-  auto one = [&](int j, float& through, float& own) {
+  auto one = [&](int j, float& q, float& own) {
     const int kind = p.kind[j];
-    const float end = mine ? p.end[j * pairs + at] : 0.f, decay = ex2(A * p.steps[(int64_t)j * p.D + c]);
+    const float end = mine ? p.end[j * pairs + at] : 0.f;
+    q = A * p.steps[(int64_t)j * p.D + c];
     own = kind ? end : 0.f;
-    through = decay;
     return kind == 2;
   };
   bool cut = false;
 #pragma unroll 8
   for (int j = j0; j < j1; ++j) {
-    float t, o;
-    const bool on = one(j, t, o);
+    float q, own;
+    const bool on = one(j, q, own);
+    Decay d;
+    d.of(q);
+    e = on ? d.apply(e, own) : own;
     cut |= !on;
-    e = on ? fmaf(t, e, o) : o;
-    P *= t;
+    Q += q;
   }
   if (lane == 0) s_cut[part] = cut;
-  s_p[part][lane] = P;
+  Decay all;
+  all.of(Q);
+#pragma unroll
+  for (int i = 0; i < 3; ++i) s_f[i][part][lane] = all.f[i];
   s_e[part][lane] = e;
   __syncthreads();
   e = 0.f;
-  for (int k = 0; k < part; ++k) e = s_cut[k] ? s_e[k][lane] : fmaf(s_p[k][lane], e, s_e[k][lane]);
+#pragma unroll 4
+  for (int k = 0; k < part; ++k) {
+    const Decay d = {{s_f[0][k][lane], s_f[1][k][lane], s_f[2][k][lane]}};
+    const float own = s_e[k][lane];
+    e = s_cut[k] ? own : d.apply(e, own);
+  }
 #pragma unroll 8
   for (int j = j0; j < j1; ++j) {
-    float t, o;
-    e = one(j, t, o) ? fmaf(t, e, o) : o;
+    float q, own;
+    const bool on = one(j, q, own);
+    Decay d;
+    d.of(q);
+    e = on ? d.apply(e, own) : own;
     if (mine) p.end[j * pairs + at] = e;
   }
 }
