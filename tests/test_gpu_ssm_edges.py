@@ -111,3 +111,34 @@ def test_chunks_whose_decay_fp32_does_not_hold(A, h0):
     ssm_oracle.close(_np(y), want, bound, "y")
     ssm_oracle.close(_np(kept), np.stack(last), np.stack(elast), "states")
     assert h0 != 0 or (y == 0).all()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("K", [2, 4])
+@pytest.mark.parametrize("D,T", [(24, 1), (24, 40), (21, 40), (21, 1)])
+def test_silu_of_sums_far_below_zero(dtype, K, D, T):
+    """v sigmoid(v) goes to zero, whatever v: masks of the type's lowest value come out as zeros. Each beside ordinary values and NaN."""
+    ops, capi = _ops()
+    lowest = float(torch.finfo(T_[dtype]).min)
+    far = [v for v in (-20.0, -41.0, -42.0, -50.0, -60.0, -80.0, -100.0, -1e4, -1e18, -1e30, lowest, lowest / 2, 41.0, 60.0, 100.0, 1e4, -lowest) if abs(v) <= -lowest]
+    x = torch.randn(40, D, device="cuda", dtype=torch.float32)
+    for i, v in enumerate(far):
+        x[2 * i, (3 * i) % D] = v
+        x[2 * i, (3 * i + 1) % D] = v
+    x = x.to(T_[dtype])
+    w = torch.zeros(D, K, device="cuda", dtype=T_[dtype])
+    w[:, K - 1] = 1.0                                           # (the sums are the inputs)
+    v = _np(x)
+    with np.errstate(over="ignore"):
+        want = v / (1 + np.exp(-v))
+    # The sum is exact; exponential, quotient and products as ssm_oracle takes them, relative to the result (not to v). The exponential's
+    # argument v log2(e) is off by the constant's rounding and the product's, 2^-24 relative each, so exp(v) by 2 |v| 2^-24 relative, which the
+    # result shows where v < 0. Below -87 the quotient is flushed (1 + exp(-v) above 2^126): less than 2^-126 times |v| < 2^7 up to where
+    # v exp(v) is itself below 2^-118.
+    far_arg = np.where(v < 0, 2 * np.minimum(np.abs(v), 128) * 2.0 ** -24, 0)
+    bound = (2.0 ** -20 + far_arg + ssm_oracle.HALF[dtype]) * np.abs(want) * (1 + 1e-3) + ssm_oracle.TINY[dtype] + 2.0 ** -118
+    ssm_oracle.close(_np(ops.ssm_conv(x, w, T=T)), want, bound, dtype)
+    x[7, 5] = float("nan")                                      # (its neighbours keep theirs)
+    y = ops.ssm_conv(x, w, T=T)
+    nan = y.isnan()
+    assert nan[7, 5] and not nan[:, [c for c in range(D) if c != 5]].any()

@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(CONV_THREADS) ssm_conv_step_kernel(const ConvP
 // The thread that has a list's first row makes its first K - 1 rows (they read the state) and its last state, so that states moved
 // on in place are read and written by one thread.
 // Pieces of 8 bytes and eight rows ahead: with 16-byte pieces and four rows the registers let half as many warps in, which is what
-// the loads in flight are. SiLU is the rest: two exponentials and a quotient for two values. Bound by the latency of the reads in flight:
+// the loads in flight are. SiLU is the rest: an exponential and a quotient a value. Bound by the latency of the reads in flight:
 // 1024 lists of 262144 rows in all, D = 512, bf16 134 us = 4.0 TB/s, 0.62 of a copy's rate, 24 warps an SM, SFUs 36 % busy. The
 // next rows asked for before these are written, and longer or shorter walks, are no faster.
 template <typename T, int V, int K>

@@ -124,15 +124,12 @@ __device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
 }
 constexpr float LOG2E = 1.4426950408889634f;
 __device__ __forceinline__ float silu(float v) { return v * rcp(1.f + ex2(-LOG2E * v)); }
-// two of them with one reciprocal: 1 / a = b / (a b). exp is cut at 2^60, so that the product of two is finite: below -41.6 the result is
-// v 2^-60 instead of v exp(v), both less than 1e-16 of what the sums before it are rounded by.
+// two of them. (One reciprocal for both, of the product, has to be kept from overflowing and one's NaN from the other: more instructions than
+// the reciprocal saves. 1024 lists of 262144 rows, D = 512, bf16 138 us so with the exponents cut, 135 now.)
 __device__ __forceinline__ f32x2 silu2(f32x2 v) {
-  float e0, e1;
-  unpack2(mul2(v, pack2(-LOG2E, -LOG2E)), e0, e1);
-  e0 = 1.f + ex2(fminf(e0, 60.f));
-  e1 = 1.f + ex2(fminf(e1, 60.f));
-  const float both = rcp(e0 * e1);
-  return mul2(v, mul2(pack2(e1, e0), pack2(both, both)));
+  float x0, x1;
+  unpack2(mul2(v, pack2(-LOG2E, -LOG2E)), x0, x1);
+  return mul2(v, pack2(rcp(1.f + ex2(x0)), rcp(1.f + ex2(x1))));
 }
 // log(1 + exp(v)) = max(v, 0) + log1p(u), u = exp(-|v|), and log1p(u) = 2 atanh(s) with s = u / (2 + u) <= 1/3 by the series of atanh, cut
 // after s^13 (the next term is 1.4e-8 of the sum at most): right in relative terms where u is small too, which log(1 + u) is not.
