@@ -526,7 +526,7 @@ int xb_augru_shared(const void* x, const void* att, void* y_final, int32_t reque
  * is kept. An empty list leaves the state that it began with.
  * Fewer than 2^31 rows; lists and channels at most 2^31 - 1024.
  * x, y, z, delta, B, C share `dtype` (XB_F32, XB_F16, XB_BF16); every sum and the scan's states are fp32. Outputs overlap no
- * input. An infinity or NaN in a row makes no other list's results bad; its own list's may be NaN where the formula has an infinity. */
+ * input (refused where both have one row stride or begin at one address). An infinity or NaN in a row makes no other list's results bad; its own list's may be NaN where the formula has an infinity. */
 
 /* y[t, c] = act(bias[c] + sum_{j < K} w[c, j] x[t - K + 1 + j, c]), x before the list's first row from its state
  * (zeros without one); act is SiLU (x * sigmoid(x)) or none. 2 <= K <= 8. */
@@ -581,7 +581,7 @@ int xb_ssm_scan(const xb_ssm_scan_args* args, void* workspace, size_t workspace_
  *   Y[m] = X[m] W + bias + scale[a] (X[m] A[a]^T) B[a]^T,  a = adapter[m];  without the last term where a is outside [0, n_adapters)
  * Stands beside xb_gemm (GemmOp, blaze/blaze/operator/op/gemm_op.h:33-107): W as its B operand, [K, N] or with trans_w [N, K].
  * The rank-r intermediate is held in fp32. r <= 128; M, N and K at most 2^31 - 1024. Adapters may share a matrix (a stride of 0). Y overlaps
- * no input. */
+ * no input (refused for X where both have one row stride in bytes or begin at one address). */
 typedef struct xb_lora_args {
   int32_t M, N, K, r, n_adapters;
   int32_t trans_w;

@@ -142,3 +142,44 @@ def test_silu_of_sums_far_below_zero(dtype, K, D, T):
     y = ops.ssm_conv(x, w, T=T)
     nan = y.isnan()
     assert nan[7, 5] and not nan[:, [c for c in range(D) if c != 5]].any()
+
+
+def test_results_beside_their_inputs_and_over_them():
+    """Columns of one matrix may hold both, the rows behind the last one too; the input itself may not."""
+    ops, capi = _ops()
+    rng = np.random.default_rng(37)
+    for dtype in (torch.float32, torch.float16):
+        m = torch.from_numpy(rng.normal(0, 1, (90, 48)).astype(np.float32)).cuda().to(dtype)
+        w = torch.from_numpy(rng.normal(0, 1, (24, 4)).astype(np.float32)).cuda().to(dtype)
+        for x, out in ((m[:90, :24], m[:90, 24:]), (m[:40, 24:], m[40:80, 24:]), (m[1:41, 24:], m[:40, :24]), (m[:1, 10:34], m[1:2, 10:34])):
+            want = ops.ssm_conv(x.clone(), w)
+            assert torch.equal(ops.ssm_conv(x, w, out=out), want)
+        x = m[:40, :24]
+        for out in (x, m[1:41, :24], m[:40, 1:25], m[:40, 23:47]):
+            with pytest.raises(capi.XbError, match="overlaps"):
+                ops.ssm_conv(x, w, out=out)
+        A, B = -torch.rand(24, 16, device="cuda"), m[:40, 24:40].clone()
+        with pytest.raises(capi.XbError, match="overlaps"):
+            ops.ssm_scan(x, x.clone(), A, B, B, out=x)
+        X, W = m[:40, :24], torch.zeros(24, 24, device="cuda", dtype=dtype)
+        a = torch.zeros(2, 4, 24, device="cuda", dtype=dtype)
+        ad = torch.zeros(40, device="cuda", dtype=torch.int32)
+        with pytest.raises(capi.XbError, match="overlaps"):
+            ops.lora_gemm(X, W, a, a.transpose(1, 2).contiguous(), ad, Y=X)
+    st = torch.zeros(9, 3, 24, device="cuda")
+    x, w = torch.zeros(8, 24, device="cuda"), torch.zeros(24, 4, device="cuda")
+    with pytest.raises(capi.XbError, match="states overlap"):
+        ops.ssm_conv(x, w, T=1, state_in=st[:8], state_out=st[1:])
+
+
+def test_lists_behind_a_broken_one_keep_their_bits_in_the_convolution():
+    ops, capi = _ops()
+    rng = np.random.default_rng(36)
+    off = torch.tensor([0, 5, 75, 75, 84, 384], dtype=torch.int32, device="cuda")
+    for dtype in (torch.float32, torch.bfloat16):
+        x, w, b = (torch.from_numpy(rng.normal(0, 1, n).astype(np.float32)).cuda().to(dtype) for n in ((384, 40), (40, 4), (40,)))
+        y = ops.ssm_conv(x, w, b, offsets=off)
+        x[10:12] = float("inf")
+        again = ops.ssm_conv(x, w, b, offsets=off)
+        others = [r for r in range(384) if not 10 <= r < 15]
+        assert torch.equal(again[others], y[others]) and not torch.isfinite(again[10:12]).all()

@@ -85,3 +85,21 @@ def test_adapters_whose_scratch_passes_64_bits():
         assert L.xb_lora_workspace_bytes(C.byref(a)) == 0, k
         assert L.xb_lora_gemm(C.byref(a), AT, 1 << 60, None) == LIMIT, k
         assert b"xb_lora_gemm" in L.xb_last_error()
+
+
+def test_results_over_inputs():
+    m = pkg.load()
+    c, L = m.capi, m.lib()
+    row = 24 * 2
+    for k in (dict(y=AT), dict(y=AT + 2), dict(y=AT + 5 * row), dict(y=AT + 11 * row + 46), dict(x=AT + row), dict(y=AT, ldy=40), dict(ldx=100, ldy=100, y=AT + 46),
+              dict(ldx=40, ldy=40, y=AT + 34), dict(ldx=40, ldy=40, y=AT + 3 * 80 + 34)):
+        k = {**dict(y=AT), **k} if "x" in k else k
+        assert L.xb_ssm_conv(C.byref(_conv(c, **k)), None) == ARG and b"overlap" in L.xb_last_error(), k
+    states = dict(n_slots=3, state_in=AT)
+    for at in (AT + 2, AT + 3 * 3 * 24 * 2 - 2, AT - 16):
+        assert L.xb_ssm_conv(C.byref(_conv(c, state_out=at, **states)), None) == ARG and b"states overlap" in L.xb_last_error()
+    for k in [dict(y=AT), dict(y=AT + row)] + [{n: AT + (1 << 20)} for n in ("delta", "B", "C")] + [dict(z=AT + (1 << 20) + row, ldz=24)]:
+        assert L.xb_ssm_scan(C.byref(_scan(c, **k)), AT, 1 << 40, None) == ARG and b"overlap" in L.xb_last_error(), k
+    assert L.xb_ssm_scan(C.byref(_scan(c, h_in=AT, h_out=AT + 4, n_slots=3)), AT, 1 << 40, None) == ARG and b"states overlap" in L.xb_last_error()
+    for k in (dict(Y=AT), dict(Y=AT, y_dtype=c.XB_F32), dict(Y=AT + 62, N=32, ldy=32, stride_b=256), dict(Y=AT + 9 * 64, N=32, ldy=32, stride_b=256)):
+        assert L.xb_lora_gemm(C.byref(_lora(c, **k)), AT, 1 << 40, None) == ARG and b"overlap" in L.xb_last_error(), k

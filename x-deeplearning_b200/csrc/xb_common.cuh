@@ -10,6 +10,7 @@
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
+#include <utility>
 
 #include "xdlb200.h"
 
@@ -44,6 +45,23 @@ inline size_t dtype_size(int dt) {
     case XB_F16: case XB_BF16: return 2;
     default: return 0;
   }
+}
+
+// Whether the rows of two matrices share memory (all in bytes): told for rows of one stride, of which one matrix may take other columns
+// than the other; with two strides only for matrices that begin at one address.
+inline bool rows_meet(const void* a, int64_t lda, int64_t wa, const void* b, int64_t ldb, int64_t wb, int64_t rows) {
+  uintptr_t p = reinterpret_cast<uintptr_t>(a), q = reinterpret_cast<uintptr_t>(b);
+  if (rows < 1 || wa < 1 || wb < 1) return false;
+  if (p == q) return true;
+  if (q < p) {
+    std::swap(p, q);
+    std::swap(lda, ldb);
+    std::swap(wa, wb);
+  }
+  if (q >= p + (uintptr_t)((rows - 1) * lda + wa)) return false;
+  if (rows > 1 && lda != ldb) return false;
+  const int64_t d = (int64_t)((q - p) % (uintptr_t)lda);
+  return d < wa || d + wb > lda;
 }
 
 // Programmatic dependent launch: a kernel launched with launch_dependent may begin while the kernel before it in the stream

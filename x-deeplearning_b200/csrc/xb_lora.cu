@@ -305,6 +305,8 @@ extern "C" int xb_lora_gemm(const xb_lora_args* a, void* workspace, size_t works
   const size_t need = xb_lora_workspace_bytes(a);
   XB_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), XB_ERR_SCRATCH, "xb_lora_gemm: workspace of %zu bytes, %zu needed", workspace_bytes, need);
   XB_REQUIRE(need == 0 || (reinterpret_cast<uintptr_t>(workspace) & 15) == 0, XB_ERR_ARG, "xb_lora_gemm: the workspace is not on 16 bytes");
+  const int64_t x_size = (int64_t)dtype_size(a->dtype), y_size = (int64_t)dtype_size(a->y_dtype);
+  XB_REQUIRE(!rows_meet(a->X, a->ldx * x_size, a->K * x_size, a->Y, a->ldy * y_size, a->N * y_size, a->M), XB_ERR_ARG, "xb_lora_gemm: Y overlaps X");
   if (takes_tiles(*a)) return run_umma(*a, static_cast<uint8_t*>(workspace), (cudaStream_t)s);
   if (a->dtype == XB_F32) return run_rows<float>(*a, static_cast<uint8_t*>(workspace), (cudaStream_t)s);
   if (a->dtype == XB_F16) return run_rows<__half>(*a, static_cast<uint8_t*>(workspace), (cudaStream_t)s);

@@ -257,6 +257,11 @@ int check_lists(const char* what, const int32_t* offsets, const int32_t* slots, 
   XB_REQUIRE(!states || slots || n_slots >= batch, XB_ERR_ARG, "%s: %d states for %d lists without slots", what, n_slots, batch);
   return 0;
 }
+// the arrays of kept states: one, or two that share nothing
+bool states_apart(const void* first, const void* last, int64_t bytes) {
+  const uintptr_t p = reinterpret_cast<uintptr_t>(first), q = reinterpret_cast<uintptr_t>(last);
+  return !first || !last || p == q || p + (uintptr_t)bytes <= q || q + (uintptr_t)bytes <= p;
+}
 Lists lists_of(const int32_t* offsets, const int32_t* slots, int64_t rows, int32_t batch, int32_t n_slots) {
   return {offsets, slots, rows, batch > 0 ? rows / batch : 0, batch, n_slots};
 }
@@ -399,6 +404,9 @@ extern "C" int xb_ssm_conv(const xb_ssm_conv_args* a, xb_stream_t s) {
   XB_REQUIRE(a->w && (a->rows == 0 || (a->x && a->y)), XB_ERR_ARG, "xb_ssm_conv: null tensor");
   XB_REQUIRE(a->rows == 0 || (a->ldx >= a->D && a->ldy >= a->D), XB_ERR_ARG, "xb_ssm_conv: row strides %lld, %lld of %d channels",
              (long long)a->ldx, (long long)a->ldy, a->D);
+  const int64_t size = (int64_t)dtype_size(a->dtype), states = (int64_t)a->n_slots * (a->K - 1) * a->D * size;
+  XB_REQUIRE(!rows_meet(a->x, a->ldx * size, a->D * size, a->y, a->ldy * size, a->D * size, a->rows), XB_ERR_ARG, "xb_ssm_conv: y overlaps x");
+  XB_REQUIRE(states_apart(a->state_in, a->state_out, states), XB_ERR_ARG, "xb_ssm_conv: the two arrays of states overlap and are not one");
   if (a->dtype == XB_F32) return launch_conv<float>(*a, (cudaStream_t)s);
   if (a->dtype == XB_F16) return launch_conv<__half>(*a, (cudaStream_t)s);
   return launch_conv<__nv_bfloat16>(*a, (cudaStream_t)s);
@@ -436,6 +444,11 @@ extern "C" int xb_ssm_scan(const xb_ssm_scan_args* a, void* workspace, size_t wo
   XB_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), XB_ERR_SCRATCH, "xb_ssm_scan: workspace of %zu bytes, %zu needed",
              workspace_bytes, need);
   XB_REQUIRE(need == 0 || (reinterpret_cast<uintptr_t>(workspace) & 15) == 0, XB_ERR_ARG, "xb_ssm_scan: the workspace is not on 16 bytes");
+  const int64_t size = (int64_t)dtype_size(a->dtype), row = a->D * size, bc = (int64_t)a->groups * a->N * size;
+  auto over = [&](const void* in, int64_t ld, int64_t width) { return in && rows_meet(in, ld * size, width, a->y, a->ldy * size, row, a->rows); };
+  XB_REQUIRE(!over(a->x, a->ldx, row) && !over(a->delta, a->lddelta, row) && !over(a->z, a->ldz, row) && !over(a->B, a->ldb, bc) && !over(a->C, a->ldc, bc),
+             XB_ERR_ARG, "xb_ssm_scan: y overlaps an input");
+  XB_REQUIRE(states_apart(a->h_in, a->h_out, (int64_t)a->n_slots * a->D * a->N * 4), XB_ERR_ARG, "xb_ssm_scan: the two arrays of states overlap and are not one");
   const ScanParams p = scan_params(*a, plan, static_cast<uint8_t*>(workspace));
   if (a->dtype == XB_F32) return ssm_scan_f32(p, plan, (cudaStream_t)s);
   if (a->dtype == XB_F16) return ssm_scan_f16(p, plan, (cudaStream_t)s);
