@@ -22,3 +22,10 @@ def test_lanes_of_a_warp_with_adapters_of_their_own(M, N, r):
         s["adapter"] = torch.from_numpy(np.where(own, rows // 128 % 3, -1).astype(np.int32)).cuda()
         _check(s, "bf16", "bf16", True)
     assert _ops()[0].device_status() == 0
+
+
+@pytest.mark.parametrize("M,K,N,r", [(3, 2, 65535 * 128 + 1, 1), (65535 * 64 + 65, 2, 1, 3)])
+@pytest.mark.parametrize("n", [0, 2])
+def test_more_columns_or_rows_than_a_grid_of_16_bits(M, K, N, r, n):
+    s = _case(np.random.default_rng(1), M, K, N, n, r, "f32", False, 0, "mixed" if n else "none")
+    _check(s, "f32", "f32", False)

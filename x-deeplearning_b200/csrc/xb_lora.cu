@@ -73,7 +73,8 @@ __global__ void __launch_bounds__(128) lora_rows_expand_kernel(const LoraParams 
   pdl_begin();
   __shared__ float s_u[ROWS][LORA_MAX_RANK];
   __shared__ int s_a[ROWS];
-  const int m0 = blockIdx.x * ROWS, n = blockIdx.y * 128 + threadIdx.x;
+  const unsigned row_blocks = ((unsigned)p.M + ROWS - 1) / ROWS;         // (of 128 columns each, one behind the other)
+  const int m0 = (int)(blockIdx.x % row_blocks) * ROWS, n = (int)(blockIdx.x / row_blocks) * 128 + threadIdx.x;
   if (threadIdx.x < ROWS) s_a[threadIdx.x] = m0 + (int)threadIdx.x < p.M ? adapter_of(p, m0 + threadIdx.x) : -1;
   __syncthreads();
   for (int i = threadIdx.x; i < ROWS * p.r; i += 128) {
@@ -140,10 +141,11 @@ bool takes_tiles(const xb_lora_args& a) { return lora_umma_takes(a) && !takes_ro
 
 constexpr size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
-// Rows of a turn: the fp32 addend of a turn (M x N) is at most 64 MB, so that it is still in L2 when the product reads it.
+// Rows of a turn: the fp32 addend of a turn (M x N) is at most 64 MB, so that it is still in L2 when the product reads it, and no more than
+// xb_gemm's CUDA cores take in a call.
 int turn_rows(const xb_lora_args& a) {
   const int64_t rows = std::max<int64_t>(((int64_t)16 << 20) / std::max(a.N, 1) / 128 * 128, 128);
-  return (int)std::min<int64_t>(rows, a.M);
+  return (int)std::min<int64_t>({rows, a.M, 32767 * 128});
 }
 
 // fp32 weights as [N, K] are laid out as [K, N] first, for which xb_gemm has a faster kernel. us in a graph without and with, whatever the rows:
@@ -206,10 +208,11 @@ int launch_shrink(const LoraParams& p, bool vec, cudaStream_t s) {
 template <typename T>
 int launch_expand(const LoraParams& p, bool vec, cudaStream_t s) {
   // eight rows a block share what they read of B; two where that would leave SMs idle
-  const unsigned cols = (unsigned)((p.N + 127) / 128);
-  XB_REQUIRE(cols <= 65535, XB_ERR_LIMIT, "xb_lora_gemm: %d columns are too many for this path", p.N);
+  const int64_t cols = ((int64_t)p.N + 127) / 128;
   const bool few = (int64_t)((p.M + 7) / 8) * cols < 4 * sm_count();
-  const dim3 grid((unsigned)(few ? (p.M + 1) / 2 : (p.M + 7) / 8), cols);
+  const int64_t blocks = (few ? (p.M + 1) / 2 : (p.M + 7) / 8) * cols;
+  XB_REQUIRE(blocks < ((int64_t)1 << 31), XB_ERR_LIMIT, "xb_lora_gemm: %d x %d are too many for one call", p.M, p.N);
+  const unsigned grid = (unsigned)blocks;
   if (few) {
     if (vec) launch_dependent(lora_rows_expand_kernel<T, true, 2>, grid, 128, 0, s, p);
     else launch_dependent(lora_rows_expand_kernel<T, false, 2>, grid, 128, 0, s, p);
