@@ -24,6 +24,18 @@ def test_lanes_of_a_warp_with_adapters_of_their_own(M, N, r):
     assert _ops()[0].device_status() == 0
 
 
+@pytest.mark.parametrize("dtype,out", [("f16", "f16"), ("bf16", "f32"), ("f32", "f32")])
+@pytest.mark.parametrize("M,K,N,trans,pad", [(20, 32, 24, True, 0), (600, 72, 304, False, 0), (700, 250, 131, True, 1), (9600, 72, 40, True, 0),
+                                             (513, 33, 17, False, 0)])
+def test_without_adapters(dtype, out, M, K, N, trans, pad):
+    """No adapters, and adapters of rank 0: the projection and its bias."""
+    for n, r in ((0, 8), (3, 0)):
+        s = _case(np.random.default_rng(M), M, K, N, n, max(r, 1), dtype, trans, pad, "none" if n == 0 else "mixed")
+        if r == 0:
+            s["A"], s["B"] = s["A"].new_empty((n, 0, K)), s["B"].new_empty((n, N, 0))
+        _check(s, dtype, out, trans)
+
+
 @pytest.mark.parametrize("M,K,N,r", [(3, 2, 65535 * 128 + 1, 1), (65535 * 64 + 65, 2, 1, 3)])
 @pytest.mark.parametrize("n", [0, 2])
 def test_more_columns_or_rows_than_a_grid_of_16_bits(M, K, N, r, n):

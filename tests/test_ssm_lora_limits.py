@@ -103,3 +103,11 @@ def test_results_over_inputs():
     assert L.xb_ssm_scan(C.byref(_scan(c, h_in=AT, h_out=AT + 4, n_slots=3)), AT, 1 << 40, None) == ARG and b"states overlap" in L.xb_last_error()
     for k in (dict(Y=AT), dict(Y=AT, y_dtype=c.XB_F32), dict(Y=AT + 62, N=32, ldy=32, stride_b=256), dict(Y=AT + 9 * 64, N=32, ldy=32, stride_b=256)):
         assert L.xb_lora_gemm(C.byref(_lora(c, **k)), AT, 1 << 40, None) == ARG and b"overlap" in L.xb_last_error(), k
+
+
+def test_no_scratch_without_adapters():
+    m = pkg.load()
+    c, L = m.capi, m.lib()
+    for dtype in (c.XB_F32, c.XB_BF16):
+        for k in (dict(n_adapters=0), dict(r=0, ldb=0), dict(n_adapters=0, M=100_000), dict(n_adapters=0, M=700, ldx=33, K=33, ldw=33, lda=33)):
+            assert L.xb_lora_workspace_bytes(C.byref(_lora(c, dtype=dtype, y_dtype=dtype, **k))) == 0, k

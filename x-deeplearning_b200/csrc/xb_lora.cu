@@ -141,6 +141,8 @@ bool takes_tiles(const xb_lora_args& a) { return lora_umma_takes(a) && !takes_ro
 
 constexpr size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
+bool has_adapters(const xb_lora_args& a) { return a.n_adapters > 0 && a.r > 0; }
+
 // Rows of a turn: the fp32 addend of a turn (M x N) is at most 64 MB, so that it is still in L2 when the product reads it, and no more than
 // xb_gemm's CUDA cores take in a call.
 int turn_rows(const xb_lora_args& a) {
@@ -150,10 +152,11 @@ int turn_rows(const xb_lora_args& a) {
 
 // fp32 weights as [N, K] are laid out as [K, N] first, for which xb_gemm has a faster kernel. us in a graph without and with, whatever the rows:
 // 8 rows, K = 72, N = 168 12 and 10, K = 1280, N = 1024 50 and 39; 3931 rows of the first 51 and 35; 20000 rows, K = 324, N = 200 194 and 168.
-bool lays_out_w(const xb_lora_args& a) { return a.dtype == XB_F32 && a.trans_w; }
+bool lays_out_w(const xb_lora_args& a) { return a.dtype == XB_F32 && a.trans_w && has_adapters(a); }
 int64_t laid_out_ld(const xb_lora_args& a) { return ((int64_t)a.N + 3) / 4 * 4; }
 struct RowsScratch { size_t part, w, bytes; };             // U lies first
 RowsScratch rows_scratch(const xb_lora_args& a) {
+  if (!has_adapters(a)) return {0, 0, 0};
   const size_t turn = (size_t)turn_rows(a);
   RowsScratch s;
   s.part = align256(turn * a.r * 4);
@@ -184,7 +187,7 @@ int check_args(const xb_lora_args* a) {
   XB_REQUIRE(std::max({a->M, a->N, a->K}) <= INT32_MAX - 1023, XB_ERR_LIMIT, "xb_lora_gemm: %d x %d x %d, at most 2^31 - 1024 each", a->M, a->N, a->K);
   XB_REQUIRE(a->r <= LORA_MAX_RANK, XB_ERR_LIMIT, "xb_lora_gemm: rank %d, at most %d", a->r, LORA_MAX_RANK);
   if (a->M == 0 || a->N == 0) return 0;
-  const bool adapters = a->n_adapters > 0 && a->r > 0;
+  const bool adapters = has_adapters(*a);
   XB_REQUIRE(a->Y && a->X && a->W, XB_ERR_ARG, "xb_lora_gemm: null tensor");
   XB_REQUIRE(a->ldx >= a->K && a->ldy >= a->N && a->ldw >= (a->trans_w ? a->K : a->N), XB_ERR_ARG, "xb_lora_gemm: a row stride is too small");
   XB_REQUIRE(!adapters || (a->adapter && a->B && a->A), XB_ERR_ARG, "xb_lora_gemm: null adapter");
@@ -227,7 +230,7 @@ template <typename T>
 int run_rows(const xb_lora_args& a, uint8_t* ws, cudaStream_t s) {
   const int turn = turn_rows(a);
   LoraParams p;
-  p.N = a.N; p.K = a.K; p.r = a.r; p.n_adapters = a.r > 0 && a.adapter ? a.n_adapters : 0;
+  p.N = a.N; p.K = a.K; p.r = a.r; p.n_adapters = has_adapters(a) ? a.n_adapters : 0;
   p.A = a.A; p.lda = a.lda; p.stride_a = a.stride_a; p.B = a.B; p.ldb = a.ldb; p.stride_b = a.stride_b;
   p.scale = a.scale; p.bias = a.bias; p.ldx = a.ldx;
   p.U = reinterpret_cast<float*>(ws);
@@ -242,7 +245,9 @@ int run_rows(const xb_lora_args& a, uint8_t* ws, cudaStream_t s) {
   memset(&g, 0, sizeof(g));
   g.N = a.N; g.K = a.K; g.trans_b = a.trans_w; g.alpha = g.beta = 1.f; g.batch = 1;
   g.lda = a.ldx; g.B = a.W; g.ldb = a.ldw; g.ldy = a.ldy; g.ab_dtype = a.dtype; g.y_dtype = a.y_dtype;
-  g.bias = p.part; g.ldbias = a.N; g.bias_kind = XB_BIAS_FULL; g.bias_dtype = XB_F32;
+  g.bias_dtype = XB_F32;
+  if (p.n_adapters) { g.bias = p.part; g.ldbias = a.N; g.bias_kind = XB_BIAS_FULL; }
+  else if (a.bias) { g.bias = a.bias; g.bias_kind = XB_BIAS_ROW; }          // without adapters: the projection alone
   if constexpr (sizeof(T) == 2) {
     // the projection and the products with B in one kernel (its rows are one turn: at most 2 sm_count() tiles of 64 x 32)
     if (takes_rows_kernel(a)) {
@@ -275,7 +280,8 @@ int run_rows(const xb_lora_args& a, uint8_t* ws, cudaStream_t s) {
     p.X = reinterpret_cast<const T*>(a.X) + m0 * a.ldx;
     p.adapter = p.n_adapters ? a.adapter + m0 : nullptr;
     if (int rc = launch_shrink<T>(p, vec_k, s)) return rc;
-    if (int rc = launch_expand<T>(p, vec_r, s)) return rc;
+    if (p.n_adapters)
+      if (int rc = launch_expand<T>(p, vec_r, s)) return rc;
     g.M = p.M;
     g.A = p.X;
     g.Y = reinterpret_cast<uint8_t*>(a.Y) + m0 * a.ldy * (int64_t)dtype_size(a.y_dtype);
