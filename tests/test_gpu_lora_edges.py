@@ -10,7 +10,7 @@ from test_gpu_lora import T_, _case, _check, _np, _ops
 pytestmark = pytest.mark.gpu
 
 
-@pytest.mark.parametrize("M,N", [(700, 304), (9600, 72)])
+@pytest.mark.parametrize("M,N", [(700, 304), (2100, 304), (9600, 72)])
 @pytest.mark.parametrize("r", [17, 32, 100, 128])
 def test_lanes_of_a_warp_with_adapters_of_their_own(M, N, r):
     """Rows of a warp that take nothing of an adapter's U beside rows that do, for every column block of a rank above 16: one row in 32, every
@@ -41,3 +41,25 @@ def test_without_adapters(dtype, out, M, K, N, trans, pad):
 def test_more_columns_or_rows_than_a_grid_of_16_bits(M, K, N, r, n):
     s = _case(np.random.default_rng(1), M, K, N, n, r, "f32", False, 0, "mixed" if n else "none")
     _check(s, "f32", "f32", False)
+
+
+@pytest.mark.parametrize("M,N", [(60, 72), (2100, 304), (9600, 72)])
+@pytest.mark.parametrize("r", [3, 16, 20, 64])
+def test_infinities_of_an_adapter_are_the_formula_s(M, N, r):
+    """An infinite weight of B gives its sign times U's in its column, for the rows of its adapter alone, whichever kernel makes it. (U, which the
+    kernels round, is of one sign as long as it is not next to 0.)"""
+    ops, capi = _ops()
+    s = _case(np.random.default_rng(M + r), M, 64, N, 3, r, "bf16", True, 0, "mixed")
+    call = lambda: ops.lora_gemm(s["X"], s["W"], s["A"], s["B"], s["adapter"], bias=s["bias"], scale=s["scale"], trans_b=True)
+    y = call()
+    s["B"][1, 5, r - 1], s["B"][1, 40, 0] = float("inf"), float("-inf")
+    again = call()
+    mine = s["adapter"] == 1
+    u = s["X"].double() @ s["A"][1].double().T
+    touched = torch.zeros_like(y, dtype=torch.bool)
+    touched[mine, 5] = touched[mine, 40] = True
+    assert torch.equal(again[~touched], y[~touched])
+    for col, j, sign in ((5, r - 1, 1.0), (40, 0, -1.0)):
+        sure = mine & (u[:, j].abs() > 1e-3)
+        assert sure.sum() > 5 and torch.equal(again[sure, col].double(), sign * u[sure, j].sign() * float("inf"))
+        assert not torch.isfinite(again[mine, col]).any()

@@ -5,7 +5,7 @@
 // Rows of a tile belong to any adapters, so neither sorting nor padding is asked of the caller; a tile of one request has one. U is made
 // for all 128 rows and up to 64 / rb adapters at once, side by side in tensor memory, and a row takes its own; the product with B
 // runs once for each adapter of the tile (ascending), with the lanes of the other rows disabled.
-// U is held as two TF32 terms, hi + lo, each rounded to nearest (|U - hi - lo| <= 2^-22 |U|), side by side along the depth, and B, whose
+// U is held as two TF32 terms, hi + lo (|U - hi - lo| <= 2^-22 |U|), side by side along the depth, and B, whose
 // 16-bit values TF32 holds exactly, is read for both: fp16 would overflow or lose U's range, one term of bf16 would show in the result.
 // The products of adapters cost ceil(r / 16) depth blocks of 32 fp32 for each adapter of a tile beside the ceil(K / 64) of the projection.
 #pragma once
@@ -142,11 +142,13 @@ __device__ __forceinline__ void widen_b(const LoraTiles& p, int64_t first, int64
     to[1] = make_float4(v[4], v[5], v[6], v[7]);
   }
 }
-// v as two TF32 terms (an infinity or NaN, or what rounds up to one, stays whole in hi). Columns behind the rank are zeros whatever X
-// holds: an infinity times the zeros of A would be a NaN there.
+// v as two TF32 terms, hi + lo = v within 2^-22 |v|, of one sign and neither of them 0 where v is not: times an infinity of B both give the
+// infinity that v would (|v| above 2^-100; hi takes v's upper bits as they are, and a lo of 0 becomes 2^-126). An infinity or NaN is in hi.
+// Columns behind the rank are zeros whatever X holds: an infinity times the zeros of A would be a NaN there.
 __device__ __forceinline__ void split_tf32(float v, float& hi, float& lo) {
-  hi = round_tf32(v);
-  lo = fabsf(hi) <= 3.4028235e38f ? round_tf32(v - hi) : 0.f;
+  hi = __uint_as_float(__float_as_uint(v) & 0xffffe000u);
+  lo = round_tf32(v - hi);
+  if (!(fabsf(lo) > 0.f)) lo = fabsf(v) > 0x1p-100f ? copysignf(0x1p-126f, v) : 0.f;
 }
 
 // The adapters of a tile, `group` at a time.
