@@ -596,7 +596,8 @@ typedef struct xb_lora_args {
   int32_t dtype;                                     /* X, W, A, B: XB_F32, XB_F16 or XB_BF16 */
   int32_t y_dtype;                                   /* dtype or XB_F32 */
 } xb_lora_args;
-/* Scratch of a call with these arguments (0 without adapters): one call uses it at a time. */
+/* Scratch of a call with these arguments (0 without adapters): one call uses it at a time. What is laid out of a large table of adapters goes by
+ * those that the rows name: of more than 32 MB there is room for no more adapters than rows. */
 size_t xb_lora_workspace_bytes(const xb_lora_args* args);
 int xb_lora_gemm(const xb_lora_args* args, void* workspace, size_t workspace_bytes, xb_stream_t stream);
 

@@ -63,3 +63,43 @@ def test_infinities_of_an_adapter_are_the_formula_s(M, N, r):
         sure = mine & (u[:, j].abs() > 1e-3)
         assert sure.sum() > 5 and torch.equal(again[sure, col].double(), sign * u[sure, j].sign() * float("inf"))
         assert not torch.isfinite(again[mine, col]).any()
+
+
+@pytest.mark.parametrize("how", ["mixed", "runs", "one", "few", "none"])
+@pytest.mark.parametrize("M,K,N,n,r,pad,trans", [(2100, 72, 304, 1000, 16, 0, True), (2100, 72, 304, 700, 40, 1, False), (520, 65, 304, 2000, 5, 1, True),
+                                                 (9600, 72, 72, 40000, 8, 1, True), (2100, 520, 40, 2000, 100, 0, True)])
+def test_tables_of_many_adapters(how, M, K, N, n, r, pad, trans):
+    """Tables of which more than 32 MB would be laid out; rows that name all, some, one or none of their adapters."""
+    s = _case(np.random.default_rng(n), M, K, N, n, r, "bf16", trans, pad, "mixed" if how == "few" else how)
+    if how == "few":
+        s["adapter"] = torch.from_numpy(np.random.default_rng(2).choice([n - 1, 7, n // 2, -1, n], M).astype(np.int32)).cuda()
+    _check(s, "bf16", "bf16", trans)
+
+
+@pytest.mark.parametrize("M,N,n", [(2100, 304, 4), (2100, 304, 2000), (9600, 72, 30000), (600, 131, 3000)])
+@pytest.mark.parametrize("pad", [0, 1])
+def test_adapters_that_share_their_matrices_in_two_steps(M, N, n, pad):
+    """One A, one B, or both for all adapters, of which most have no row; each with its own scale."""
+    for shared in ("A", "B", "AB"):
+        s = _case(np.random.default_rng(M), M, 96, N, 4, 8, "bf16", True, pad, "none")
+        for k in "AB":
+            s[k] = s[k][:1].expand(n, -1, -1) if k in shared else s[k].repeat((n + 3) // 4, 1, 1)[:n]
+        s["scale"] = torch.rand(n, device="cuda") + 0.5
+        s["adapter"] = torch.from_numpy(np.random.default_rng(n).integers(-1, min(n, 300), M).astype(np.int32)).cuda()
+        assert all(s[k].stride(0) == 0 for k in shared)
+        _check(s, "bf16", "bf16", True)
+
+
+def test_a_large_table_in_a_graph_whose_rows_name_others_at_each_replay():
+    ops, capi = _ops()
+    s = _case(np.random.default_rng(3), 2100, 72, 304, 1000, 16, "bf16", True, 1, "mixed")
+    call = lambda: ops.lora_gemm(s["X"], s["W"], s["A"], s["B"], s["adapter"], bias=s["bias"], scale=s["scale"], trans_b=True)
+    call()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = call()
+    for seed, most in ((4, 1000), (5, 3), (6, 0), (7, 300)):
+        s["adapter"].copy_(torch.from_numpy(np.random.default_rng(seed).integers(-1, most + 1, 2100) - (most == 0)).cuda())
+        g.replay()
+        assert torch.equal(y, call())

@@ -79,7 +79,7 @@ def test_adapters_whose_scratch_passes_64_bits():
     m = pkg.load()
     c, L = m.capi, m.lib()
     most = (1 << 31) - 1024
-    for k in (dict(M=most, N=most, ldy=most, n_adapters=most, r=128, ldb=128, stride_a=0, stride_b=0),
+    for k in (dict(M=most, N=most, ldy=most, n_adapters=most, r=128, ldb=128, stride_a=0, stride_b=1),
               dict(M=most, K=most, ldx=most, ldw=most, lda=most, n_adapters=most, r=128, ldb=128, stride_a=1, stride_b=0)):
         a = _lora(c, **k)
         assert L.xb_lora_workspace_bytes(C.byref(a)) == 0, k
@@ -111,3 +111,17 @@ def test_no_scratch_without_adapters():
     for dtype in (c.XB_F32, c.XB_BF16):
         for k in (dict(n_adapters=0), dict(r=0, ldb=0), dict(n_adapters=0, M=100_000), dict(n_adapters=0, M=700, ldx=33, K=33, ldw=33, lda=33)):
             assert L.xb_lora_workspace_bytes(C.byref(_lora(c, dtype=dtype, y_dtype=dtype, **k))) == 0, k
+
+
+def test_scratch_goes_by_the_rows_and_not_by_the_table():
+    m = pkg.load()
+    c, L = m.capi, m.lib()
+    for n in (1_000, 100_000, 10_000_000):
+        for k in (dict(M=600, ldx=33, K=33, ldw=33, lda=33, stride_a=264), dict(M=2100, N=304, ldy=304, stride_b=304 * 8), dict(M=2100, N=304, ldy=304, stride_a=0),
+                  dict(M=80_000, N=1024, ldy=1024, stride_b=0)):
+            a = _lora(c, n_adapters=n, **k)
+            named = min(n, a.M)
+            most = a.M * 32 * 4 + a.M * 40 * 2 + a.N * 40 * 2 + max(32 << 20, named * (a.N * 32 * 4 + a.r * 40 * 2)) + 4 * (n + 1 + named) + 8 * 256
+            assert 0 < L.xb_lora_workspace_bytes(C.byref(a)) <= most, (n, k)
+            if k.get("stride_b") == 0:                         # one B for all: its room does not go by them at all
+                assert L.xb_lora_workspace_bytes(C.byref(a)) <= a.M * 32 * 4 + a.N * 32 * 4 + 4 * 256

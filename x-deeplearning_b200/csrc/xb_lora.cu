@@ -193,8 +193,18 @@ int check_args(const xb_lora_args* a) {
   XB_REQUIRE(!adapters || (a->adapter && a->B && a->A), XB_ERR_ARG, "xb_lora_gemm: null adapter");
   XB_REQUIRE(!adapters || (a->lda >= a->K && a->ldb >= a->r && a->stride_a >= 0 && a->stride_b >= 0), XB_ERR_ARG,
              "xb_lora_gemm: a stride of the adapters is too small");
-  XB_REQUIRE(!takes_tiles(*a) || lora_scratch(*a).fits, XB_ERR_LIMIT, "xb_lora_gemm: %d adapters of rank %d beside %d x %d x %d are too many for one call",
-             a->n_adapters, a->r, a->M, a->N, a->K);
+  return 0;
+}
+
+// the scratch of a call whose arguments have been checked
+int scratch_of(const xb_lora_args& a, size_t* bytes) {
+  if (!takes_tiles(a)) {
+    *bytes = rows_scratch(a).bytes;
+    return 0;
+  }
+  const LoraScratch w = lora_scratch(a);
+  XB_REQUIRE(w.fits, XB_ERR_LIMIT, "xb_lora_gemm: %d adapters of rank %d beside %d x %d x %d are too many for one call", a.n_adapters, a.r, a.M, a.N, a.K);
+  *bytes = w.bytes;
   return 0;
 }
 
@@ -303,15 +313,16 @@ int lora_set_status_mirror(int* p) { return umma::set_status_mirror(p); }
 using namespace xb;
 
 extern "C" size_t xb_lora_workspace_bytes(const xb_lora_args* a) {
-  if (check_args(a) != 0 || a->M == 0 || a->N == 0) return 0;
-  if (takes_tiles(*a)) return lora_scratch(*a).bytes;
-  return rows_scratch(*a).bytes;
+  size_t bytes = 0;
+  if (check_args(a) != 0 || a->M == 0 || a->N == 0 || scratch_of(*a, &bytes) != 0) return 0;
+  return bytes;
 }
 
 extern "C" int xb_lora_gemm(const xb_lora_args* a, void* workspace, size_t workspace_bytes, xb_stream_t s) {
   if (int rc = check_args(a)) return rc;
   if (a->M == 0 || a->N == 0) return 0;
-  const size_t need = xb_lora_workspace_bytes(a);
+  size_t need = 0;
+  if (int rc = scratch_of(*a, &need)) return rc;
   XB_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), XB_ERR_SCRATCH, "xb_lora_gemm: workspace of %zu bytes, %zu needed", workspace_bytes, need);
   XB_REQUIRE(need == 0 || (reinterpret_cast<uintptr_t>(workspace) & 15) == 0, XB_ERR_ARG, "xb_lora_gemm: the workspace is not on 16 bytes");
   const int64_t x_size = (int64_t)dtype_size(a->dtype), y_size = (int64_t)dtype_size(a->y_dtype);

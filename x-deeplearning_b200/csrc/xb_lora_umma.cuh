@@ -92,6 +92,23 @@ __device__ __forceinline__ float round_tf32(float v) {
   return __uint_as_float(r);
 }
 
+// The adapters that some row names, in any order: what a call lays out of large tables goes by them and not by what the table holds.
+struct LoraNamed {
+  int32_t* place;                         // [n_adapters]: the place of an adapter among them, -1 where no row names it; null: all are laid out
+  int32_t* count;                         // [1]: how many there are, less one
+  int32_t* id;                            // [places]
+};
+__global__ void __launch_bounds__(256) lora_named_kernel(LoraNamed to, const int32_t* adapter, int M, int n_adapters) {
+  pdl_begin();
+  const int64_t m = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const uint32_t a = m < M ? (uint32_t)adapter[m] : NO_ADAPTER, before = __shfl_up_sync(0xffffffffu, a, 1);
+  if (a >= (uint32_t)n_adapters || ((threadIdx.x & 31) && before == a)) return;       // (rows of a request lie side by side)
+  if (*reinterpret_cast<volatile int32_t*>(to.place + a) != -1 || atomicCAS(to.place + a, -1, -2) != -1) return;
+  const int at = atomicAdd(to.count, 1) + 1;
+  to.id[at] = (int32_t)a;
+  to.place[a] = at;
+}
+
 struct LoraTiles {
   int M, N, K, r, n_adapters;
   int rb;                                 // rank, rounded up to 16, 32, 64 or 128
@@ -99,8 +116,11 @@ struct LoraTiles {
   const int32_t* adapter;
   const float* scale;
   float* U;                               // [M, u_cols]
-  float* B32;                             // [n_adapters, N, b_cols]
+  float* B32;                             // [b_adapters, N, b_cols]
   const void* B; int64_t ldb, stride_b; int dtype;
+  int b_adapters;                         // that are laid out in B32, 1 where all share one B (with `named`: no more than these)
+  LoraNamed named;                        // the adapters that are laid out, where those are not all
+  int a_step, a_named;                    // adapter a's A is number a_step a of what map_a covers, or that of its place among the named
   int vec_b;                              // rows of B in whole 16-byte pieces
   int group;                              // adapters of a pass of the shrink kernel
   int stages, tiles_m;
@@ -122,20 +142,32 @@ __device__ __forceinline__ void widen8(const uint4& t, int dtype, float (&v)[8])
     }
   }
 }
-// B as fp32, zeros behind its r columns: pieces of eight from `first` on, every `step`-th
+// B as fp32, zeros behind its r columns, of all adapters or of those that are named: pieces of eight from `first` on, every `step`-th
 __device__ __forceinline__ void widen_b(const LoraTiles& p, int64_t first, int64_t step) {
   const int pieces = p.b_cols / 8;
-  const int64_t all = (int64_t)p.n_adapters * p.N * pieces;
-  for (int64_t e = first; e < all; e += step) {
+  const int64_t all = (int64_t)(p.named.place ? min(p.b_adapters, *p.named.count + 1) : p.b_adapters) * p.N * pieces;
+  int j, n, id;
+  auto find = [&](int64_t e) {
     const int64_t an = e / pieces;
-    const int j = (int)(e - an * pieces) * 8 % p.rb, a = (int)(an / p.N), n = (int)(an - (int64_t)a * p.N);
-    const int64_t at = (int64_t)a * p.stride_b + (int64_t)n * p.ldb + j;
+    const int a = (int)(an / p.N);
+    j = (int)(e - an * pieces) * 8 % p.rb;
+    n = (int)(an - (int64_t)a * p.N);
+    id = p.named.place ? p.named.id[a] : a;
+  };
+  if (first < all) find(first);
+  for (int64_t e = first; e < all; e += step) {
+    const int64_t at = (int64_t)id * p.stride_b + (int64_t)n * p.ldb + j;
+    const int left = p.r - j;
+    const bool whole = p.vec_b && left > 0;
+    uint4 raw = make_uint4(0u, 0u, 0u, 0u);
+    if (whole) raw = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.B) + at));
+    if (e + step < all) find(e + step);                    // (while those are on their way)
     float v[8];
-    if (p.vec_b && j < p.r) {
-      widen8(__ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.B) + at)), p.dtype, v);
+    if (whole) {
+      widen8(raw, p.dtype, v);
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = j + i < p.r ? load_as_f32(p.B, at + i, p.dtype) : 0.f;
+      for (int i = 0; i < 8; ++i) v[i] = i < left ? load_as_f32(p.B, at + i, p.dtype) : 0.f;
     }
     float4* to = reinterpret_cast<float4*>(p.B32) + 2 * e;
     to[0] = make_float4(v[0], v[1], v[2], v[3]);
@@ -170,6 +202,9 @@ struct Pass {
     }
   }
 };
+
+// the number of an adapter's A among those that map_a covers
+__device__ __forceinline__ int a_number(const LoraTiles& p, uint32_t a) { return p.a_named ? p.named.place[a] : (int)a * p.a_step; }
 
 constexpr int SHRINK_THREADS = 320;       // producer, MMA, four warps for the results, four for B
 constexpr int SHRINK_GROUP_ROWS = 64;     // rows of A (adapters x rb) in a stage, or rb where that is more
@@ -229,6 +264,9 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
         const int as = it & 1;
         const uint32_t acc = tmem_base + as * acc_cols, acc_ph = (uint32_t)(it >> 1) & 1u;
         if (warp == 0) {
+          int at[SHRINK_GROUP];
+#pragma unroll
+          for (int i = 0; i < SHRINK_GROUP; ++i) at[i] = i < pass.n ? a_number(p, pass.id[i]) : 0;
           for (int kb = 0; kb < num_kb; ++kb, s = (s + 1 == STAGES ? 0 : s + 1), ph ^= (s == 0 ? 1u : 0u)) {
             ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&empty_bar[s]), ph ^ 1u, 51));
             if (!ok) break;
@@ -237,7 +275,7 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
             tma_load_3d_elect(x, &map_x, bar, kb * BLOCK_K, m0, 0);
 #pragma unroll
             for (int i = 0; i < SHRINK_GROUP; ++i)
-              if (i < pass.n) tma_load_3d_elect(x + A_STAGE_BYTES + i * box, &map_a, bar, kb * BLOCK_K, 0, (int)pass.id[i]);
+              if (i < pass.n) tma_load_3d_elect(x + A_STAGE_BYTES + i * box, &map_a, bar, kb * BLOCK_K, 0, at[i]);
           }
         } else if (warp == 1) {
           ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&acc_empty[as]), acc_ph ^ 1u, 54));
@@ -363,6 +401,11 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
       place(tile, m0, n0);
       TileAdapters<4> t;
       t.load(l.adapter, l.n_adapters, m0, p.M, lane);      // (used when the projection's loads are under way)
+      int place[4] = {0, 0, 0, 0};                         // of the rows' adapters in B32, where that holds the named ones
+      if (l.named.place && l.b_adapters > 1) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) place[w] = t.id[w] != NO_ADAPTER ? l.named.place[t.id[w]] : 0;
+      }
       for (int kb = 0; kb < num_kb && ok; ++kb, advance()) {
         ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&empty_bar[s]), ph ^ 1u, 61));
         if (ok) {
@@ -377,13 +420,20 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
         }
       }
       for (uint32_t a = t.next(0); a != NO_ADAPTER && ok; a = t.next(a + 1)) {
+        int at = l.b_adapters > 1 ? (int)a : 0;
+        if (l.named.place && l.b_adapters > 1) {
+          uint32_t mine = 0;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) mine = t.id[w] == a ? (uint32_t)place[w] : mine;
+          at = (int)__reduce_max_sync(0xffffffffu, mine);
+        }
         for (int e = 0; e < u_blocks && ok; ++e, advance()) {
           ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&empty_bar[s]), ph ^ 1u, 61));
           if (ok) {
             const uint32_t bar = smem_u32(&full_bar[s]);
             expect_tx_elect(bar, (uint32_t)(A_STAGE_BYTES + b_bytes));
             tma_load_3d_elect(smem_u32(smem_a + s * A_STAGE_BYTES), &map_u, bar, e * 32, m0, 0);
-            tma_load_3d_elect(smem_u32(smem_b + s * w_bytes), &map_b, bar, e % b_blocks * 32, n0, (int)a);
+            tma_load_3d_elect(smem_u32(smem_b + s * w_bytes), &map_b, bar, e % b_blocks * 32, n0, at);
           }
         }
       }
@@ -603,7 +653,7 @@ lora_fused_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
         }
 #pragma unroll
         for (int i = 0; i < SHRINK_GROUP; ++i)
-          if (i < item.n) tma_load_3d_elect(a + i * box, &map_a, bar, kb * BLOCK_K, 0, (int)item.id[i]);
+          if (i < item.n) tma_load_3d_elect(a + i * box, &map_a, bar, kb * BLOCK_K, 0, l.a_named ? l.named.place[item.id[i]] : (int)item.id[i] * l.a_step);
       }
       return true;
     });
@@ -832,7 +882,7 @@ int launch_lora_fused(const CUtensorMap (&m)[5], const UmmaGemmParams& p, const 
 }
 
 // Rows that TMA cannot address (they do not start on 16 bytes) are laid out again in the workspace, as K-major rows of `ld` elements; the same
-// for weights in [K, N] whose results are fp32, and for adapters that share one A.
+// for weights in [K, N] whose results are fp32.
 struct LoraCopies { bool x, w, a; int64_t ld; };
 LoraCopies lora_copies(const xb_lora_args& a) {
   auto odd = [](const void* p, int64_t ld) { return ld % 8 != 0 || (reinterpret_cast<uintptr_t>(p) & 15) != 0; };
@@ -840,12 +890,12 @@ LoraCopies lora_copies(const xb_lora_args& a) {
   c.ld = ((int64_t)a.K + 7) / 8 * 8;
   c.x = odd(a.X, a.ldx);
   c.w = odd(a.W, a.ldw) || (!a.trans_w && a.y_dtype == XB_F32);
-  c.a = odd(a.A, a.lda) || (a.n_adapters > 1 && (a.stride_a % 8 != 0 || a.stride_a == 0));
+  c.a = odd(a.A, a.lda) || (a.n_adapters > 1 && a.stride_a % 8 != 0);
   return c;
 }
 // `rows` rows of K elements, element (row, k) at from + row * step_row + k * step_k of block row / rows_a_block, into rows of ld
 struct LoraCopy { const uint16_t* from; uint16_t* to; int64_t rows, rows_a_block, step_block, step_row, step_k; };
-struct LoraCopyJobs { LoraCopy job[3]; int n, K, ld; int64_t first_block[4]; };
+struct LoraCopyJobs { LoraCopy job[3]; int n, K, ld; int64_t first_block[4]; int named_job; LoraNamed named; };
 // A thread takes eight elements of a row; the rows of a block lie side by side where those are what is adjacent in memory ([K, N] weights).
 constexpr int COPY_THREADS = 256;
 __global__ void __launch_bounds__(COPY_THREADS) lora_copy_kernel(const __grid_constant__ LoraCopyJobs p) {
@@ -859,7 +909,12 @@ __global__ void __launch_bounds__(COPY_THREADS) lora_copy_kernel(const __grid_co
   const int k0 = (int)(c.step_k == 1 ? at - row * pieces : at / c.rows) * 8;
   if (row >= c.rows || k0 >= p.ld) return;
   const int64_t block = row / c.rows_a_block;
-  const uint16_t* from = c.from + block * c.step_block + (row - block * c.rows_a_block) * c.step_row;
+  int64_t from_block = block;
+  if (j == p.named_job) {                  // (places behind the last of the named adapters stay as they are)
+    if (block > *p.named.count) return;
+    from_block = p.named.id[block];
+  }
+  const uint16_t* from = c.from + from_block * c.step_block + (row - block * c.rows_a_block) * c.step_row;
   uint32_t w[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
   for (int i = 0; i < 8; ++i)
@@ -872,40 +927,68 @@ bool lora_umma_takes(const xb_lora_args& a) { return (a.dtype == XB_F16 || a.dty
 struct LoraScratch {
   int rb, u_cols, b_cols;
   int fused_group;                        // adapters of a walk where both steps are one kernel, 0 where they are two
-  size_t u, b, x, w, a, bytes;
+  int a_adapters, b_adapters;             // that are laid out, where A or B is: one where all share it
+  bool named;                             // only the adapters that rows name are laid out
+  size_t u, b, x, w, a, place, bytes;
   bool fits;                              // in what the sizes above count
 };
+// Where more than 32 MB would be laid out of a table of adapters, only those that some row names are, which a kernel (and the clearing of its
+// table) finds out first: 6 to 8 us. us in a graph, 4096 rows, K = 256, N = 1024, rank 16 (131 KB an adapter), all laid out and the named ones:
+// every adapter named, 128 of them 20 and 27, 256 32 and 41, 512 78 and 85, 1024 155 and 161; three named, of 128 19 and 17, 256 29 and 17, 512 67 and
+// 17, 1024 134 and 14. Scratch for no more of them than there are rows.
+constexpr double LORA_HELD = 32 << 20;
 LoraScratch lora_scratch(const xb_lora_args& a) {
   LoraScratch w;
   w.rb = a.r <= 16 ? 16 : a.r <= 32 ? 32 : a.r <= 64 ? 64 : 128;
   w.u_cols = 2 * w.rb;
   w.b_cols = std::max(w.rb, 32);
-  w.u = 0;
-  w.b = ((size_t)a.M * w.u_cols * 4 + 255) / 256 * 256;
   // One column of tiles, and tensor memory for it and the U of an adapter twice: both steps in one kernel. (Two adapters a walk: a third would
   // be a longer stage for every tile. Fewer tiles than half of the SMs become narrower ones, in two steps.)
   const int whole_n = (a.N + 15) / 16 * 16;
   w.fused_group = whole_n <= 256 && w.rb <= FUSED_MAX_RB && ((int64_t)a.M + BLOCK_M - 1) / BLOCK_M >= sm_count() / 2 ? std::min(2, (256 - whole_n) / w.rb) : 0;
   const LoraCopies c = lora_copies(a);
-  auto rows = [&](bool copy, int64_t n) { return copy ? ((size_t)n * c.ld * 2 + 255) / 256 * 256 : 0; };
-  w.x = w.fused_group > 0 ? 0 : w.b + ((size_t)a.n_adapters * a.N * w.b_cols * 4 + 255) / 256 * 256;
+  const double a_each = c.a ? 2.0 * c.ld * a.r : 0, b_each = w.fused_group ? 0 : 4.0 * a.N * w.b_cols;
+  w.a_adapters = a.stride_a ? a.n_adapters : 1;
+  w.b_adapters = a.stride_b ? a.n_adapters : 1;
+  w.named = a_each * w.a_adapters + b_each * w.b_adapters > LORA_HELD && a.n_adapters > 1;
+  if (w.named) {                           // no more than there are rows
+    w.a_adapters = std::min(w.a_adapters, a.M);
+    w.b_adapters = std::min(w.b_adapters, a.M);
+  }
+  // (adapters may share their memory, so what is laid out of them has no bound in what the caller holds)
+  w.fits = 4.0 * a.M * w.u_cols + b_each * w.b_adapters + a_each * w.a_adapters + 2.0 * c.ld * (c.x * (double)a.M + c.w * (double)a.N) < 1.0e15;
+  auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+  auto rows = [&](bool copy, int64_t n) { return copy ? up((size_t)n * c.ld * 2) : 0; };
+  w.u = 0;
+  w.b = w.fused_group ? 0 : up((size_t)a.M * w.u_cols * 4);
+  w.x = w.b + (w.fused_group ? 0 : up((size_t)w.b_adapters * a.N * w.b_cols * 4));
   w.w = w.x + rows(c.x, a.M);
   w.a = w.w + rows(c.w, a.N);
-  w.bytes = w.a + rows(c.a, (int64_t)a.n_adapters * a.r);
-  // (adapters may share their memory, so what is laid out of them has no bound in what the caller holds)
-  const double all = 4.0 * a.M * w.u_cols + 4.0 * a.n_adapters * a.N * w.b_cols + 2.0 * c.ld * (c.x * (double)a.M + c.w * (double)a.N + c.a * (double)a.n_adapters * a.r);
-  w.fits = all < 1.0e15;
+  w.place = w.a + rows(c.a, (int64_t)w.a_adapters * a.r);
+  w.bytes = w.place + (w.named ? up(((size_t)a.n_adapters + 1 + std::min(a.n_adapters, a.M)) * 4) : 0);
   return w;
 }
 
 int run_umma(const xb_lora_args& given, uint8_t* ws, cudaStream_t stream) {
   const LoraScratch w = lora_scratch(given);
   xb_lora_args a = given;
+  LoraNamed named = {nullptr, nullptr, nullptr};
+  if (w.named) {
+    named.place = reinterpret_cast<int32_t*>(ws + w.place);
+    named.count = named.place + a.n_adapters;
+    named.id = named.count + 1;
+    XB_CUDA(cudaMemsetAsync(named.place, 0xff, ((size_t)a.n_adapters + 1) * 4, stream));
+    // (not launch_dependent: what it follows is no kernel)
+    lora_named_kernel<<<(unsigned)(((int64_t)a.M + 255) / 256), 256, 0, stream>>>(named, a.adapter, a.M, a.n_adapters);
+    if (int rc = check_launch("lora_named_kernel")) return rc;
+  }
   if (const LoraCopies c = lora_copies(given); c.x || c.w || c.a) {
     LoraCopyJobs jobs;
     memset(&jobs, 0, sizeof(jobs));
     jobs.K = a.K;
     jobs.ld = (int)c.ld;
+    jobs.named_job = -1;
+    jobs.named = named;
     auto add = [&](const void* from, size_t to, int64_t rows, int64_t rows_a_block, int64_t step_block, int64_t step_row, int64_t step_k) {
       jobs.job[jobs.n] = {static_cast<const uint16_t*>(from), reinterpret_cast<uint16_t*>(ws + to), rows, rows_a_block, step_block, step_row, step_k};
       jobs.first_block[jobs.n + 1] = jobs.first_block[jobs.n] + (rows * (c.ld / 8) + COPY_THREADS - 1) / COPY_THREADS;
@@ -914,7 +997,12 @@ int run_umma(const xb_lora_args& given, uint8_t* ws, cudaStream_t stream) {
     };
     if (c.x) { a.X = add(a.X, w.x, a.M, a.M, 0, a.ldx, 1); a.ldx = c.ld; }
     if (c.w) { a.W = add(a.W, w.w, a.N, a.N, 0, a.trans_w ? a.ldw : 1, a.trans_w ? 1 : a.ldw); a.ldw = c.ld; a.trans_w = 1; }
-    if (c.a) { a.A = add(a.A, w.a, (int64_t)a.n_adapters * a.r, a.r, a.stride_a, a.lda, 1); a.lda = c.ld; a.stride_a = c.ld * a.r; }
+    if (c.a) {
+      if (w.named && a.stride_a) jobs.named_job = jobs.n;
+      a.A = add(a.A, w.a, (int64_t)w.a_adapters * a.r, a.r, a.stride_a, a.lda, 1);
+      a.lda = c.ld;
+      a.stride_a = a.stride_a ? c.ld * a.r : 0;
+    }
     const int64_t blocks = jobs.first_block[jobs.n];
     XB_REQUIRE(blocks < ((int64_t)1 << 31), XB_ERR_LIMIT, "xb_lora_gemm: %d rows of %d are too many for one call", a.M, a.K);
     launch_dependent(lora_copy_kernel, (unsigned)blocks, COPY_THREADS, 0, stream, jobs);
@@ -924,6 +1012,8 @@ int run_umma(const xb_lora_args& given, uint8_t* ws, cudaStream_t stream) {
   LoraTiles l;
   memset(&l, 0, sizeof(l));
   l.M = a.M; l.N = a.N; l.K = a.K; l.r = a.r; l.n_adapters = a.n_adapters; l.rb = w.rb; l.u_cols = w.u_cols; l.b_cols = w.b_cols;
+  const bool a_laid_out = a.A != given.A;
+  l.b_adapters = w.b_adapters; l.named = named; l.a_named = w.named && a_laid_out && a.stride_a; l.a_step = a.stride_a ? 1 : 0;
   l.adapter = a.adapter; l.scale = a.scale; l.U = reinterpret_cast<float*>(ws + w.u); l.B32 = reinterpret_cast<float*>(ws + w.b);
   l.B = a.B; l.ldb = a.ldb; l.stride_b = a.stride_b; l.dtype = a.dtype;
   l.vec_b = a.r % 8 == 0 && a.ldb % 8 == 0 && a.stride_b % 8 == 0 && (reinterpret_cast<uintptr_t>(a.B) & 15) == 0;
@@ -932,7 +1022,7 @@ int run_umma(const xb_lora_args& given, uint8_t* ws, cudaStream_t stream) {
   l.idesc_a = umma::make_idesc(BLOCK_M, 0, bf16);          // (the columns are the pass's)
   CUtensorMap mx, ma;
   if (int rc = make_map(&mx, a.X, bf16, a.K, a.M, a.ldx, 1, 0, BLOCK_M, BLOCK_K, CU_TENSOR_MAP_SWIZZLE_128B, 1, CU_TENSOR_MAP_L2_PROMOTION_L2_256B)) return rc;
-  if (int rc = make_map(&ma, a.A, bf16, a.K, a.r, a.lda, a.n_adapters, a.stride_a, l.rb)) return rc;
+  if (int rc = make_map(&ma, a.A, bf16, a.K, a.r, a.lda, a_laid_out ? w.a_adapters : a.stride_a ? a.n_adapters : 1, a.stride_a, l.rb)) return rc;
   const bool fused = w.fused_group > 0;
   if (fused) {
     l.group = w.fused_group;
@@ -971,7 +1061,7 @@ int run_umma(const xb_lora_args& given, uint8_t* ws, cudaStream_t stream) {
     m[2] = m[3] = ma;
   } else {
     if (int rc = make_map_f32(&m[2], l.U, l.u_cols, a.M, 1, BLOCK_M)) return rc;
-    if (int rc = make_map_f32(&m[3], l.B32, l.b_cols, a.N, a.n_adapters, p.block_n)) return rc;
+    if (int rc = make_map_f32(&m[3], l.B32, l.b_cols, a.N, w.b_adapters, p.block_n)) return rc;
   }
   m[4] = m[0];
   const int64_t es = a.y_dtype == XB_F32 ? 4 : 2;
