@@ -103,3 +103,12 @@ def test_a_large_table_in_a_graph_whose_rows_name_others_at_each_replay():
         s["adapter"].copy_(torch.from_numpy(np.random.default_rng(seed).integers(-1, most + 1, 2100) - (most == 0)).cuda())
         g.replay()
         assert torch.equal(y, call())
+
+
+@pytest.mark.parametrize("dtype,trans", [("f16", True), ("bf16", False)])
+@pytest.mark.parametrize("M,N", [(9, 1024), (400, 304), (960, 152), (2048, 24)])
+def test_few_rows_at_every_split_of_the_depth(dtype, trans, M, N):
+    """Depths next to where a part or its slices become one more, and parts of which the last have little or nothing."""
+    for K in (248, 256, 264, 384, 392, 512, 520, 776, 1032, 1280, 1288, 1544, 2056, 3080, 6152):
+        s = _case(np.random.default_rng(K), M, K, N, 3, 8, dtype, trans, 0, "mixed")
+        _check(s, dtype, "f32", trans)

@@ -271,9 +271,11 @@ int run_rows(const xb_lora_args& a, uint8_t* ws, cudaStream_t s) {
       r.y_f32 = a.y_dtype == XB_F32;
       r.lanes = !vec_r ? 0 : a.r <= 8 ? 1 : a.r <= 16 ? 2 : a.r <= 32 ? 4 : a.r <= 64 ? 8 : 16;
       const int64_t tiles = ((int64_t)a.N + ROWS_BN - 1) / ROWS_BN * ((a.M + ROWS_BM - 1) / ROWS_BM);
-      const int slices = (a.K + ROWS_BK - 1) / ROWS_BK;
       r.split = 1;
-      while (r.split < 8 && 2 * r.split <= slices && tiles * 2 * r.split <= 2 * sm_count()) r.split *= 2;
+      while (r.split < 8 && r.split * ROWS_PART < a.K && tiles * 2 * r.split <= 2 * sm_count()) r.split *= 2;
+      auto share = [](int64_t k, int64_t n) { return (int)((k + n * 16 - 1) / (n * 16) * 16); };
+      r.part = share(a.K, r.split);
+      r.slice = share(r.part, (r.part + ROWS_BK - 1) / ROWS_BK);
       return a.trans_w ? launch_rows_gemm<T, true>(r, s) : launch_rows_gemm<T, false>(r, s);
     }
   }

@@ -28,12 +28,16 @@ __device__ __forceinline__ int adapter_of(const LoraParams& p, int m) {
   return a >= 0 && a < p.n_adapters ? a : -1;
 }
 
-// Y = X W + bias + U B_a^T for tiles of 64 rows x 32 columns. With few tiles a cluster of `split` CTAs shares one, each with its part of the
-// depth: all of what it reads is on its way at once, it makes its own products with B meanwhile, and the partial sums are added out
+// Y = X W + bias + U B_a^T for tiles of 64 rows x 32 columns. With few tiles a cluster of up to eight CTAs shares one, each with its part of
+// the depth: all of what it reads is on its way at once, it makes its own products with B meanwhile, and the partial sums are added out
 // of one another's shared memory, every CTA for its share of the rows. Sums as in gemm_half_kernel: 16 products by a matrix
 // instruction, added in fp32. What bounds it is the latency of one round to memory, the exchange and the launch.
-// [64, 1280] x [1280, 1024], 64 adapters of rank 16, the call in a graph: 17 us as xb_gemm with a bias matrix and the kernel that made that, 11.6 now.
-constexpr int ROWS_BM = 64, ROWS_BN = 32, ROWS_BK = 320, ROWS_THREADS = 256;
+// The depth is split in equal parts while those are deeper than ROWS_PART and the SMs have room, and a part comes in as few equal slices as ROWS_BK
+// allows. The call in a graph, 64 adapters of rank 16, us; slices of 320 as the unit of both (K = 1288 was five of them for four CTAs), 256 for
+// both, these: [64, K] x [K, 1024], K = 320 12.4, 10.2, 10.1; 640 11.4, 9.7, 9.7; 1280 11.4, 10.7, 10.6; 1288 15.9, 11.1, 11.2; where two or four
+// CTAs are all there is room for: [400, K] x [K, 304], K = 1280 15.6, 17.3, 14.5; 2048 22.4, 21.5, 18.6; [960, K] x [K, 152], K = 640 15.2, 15.9,
+// 15.1; 2048 30.2, 27.2, 26.9. ROWS_BK = 448 is no quicker. (xb_gemm with a bias matrix and a kernel that makes that: 17 at K = 1280, N = 1024.)
+constexpr int ROWS_BM = 64, ROWS_BN = 32, ROWS_BK = 384, ROWS_PART = 256, ROWS_THREADS = 256;
 constexpr int ROWS_XPITCH = ROWS_BK + 8, ROWS_WPITCH = ROWS_BN + 8;          // halves: no bank conflicts of the eight rows that are read together
 constexpr int ROWS_X_BYTES = ROWS_BM * ROWS_XPITCH * 2;
 constexpr int ROWS_W_BYTES = ROWS_BK * ROWS_WPITCH * 2;                      // (as [K, N]; the other form is smaller)
@@ -45,6 +49,7 @@ struct LoraRowsParams {
   const void* W; int64_t ldw;
   void* Y; int64_t ldy;
   int split;                              // CTAs of a tile
+  int part, slice;                        // of the depth: a CTA's, and what it brings at once (multiples of 16, slice <= ROWS_BK)
   int y_f32;
   int lanes;                              // that share a row of B, 16 bytes each (a power of two); 0: rows in single elements
 };
@@ -109,11 +114,11 @@ __global__ void __launch_bounds__(ROWS_THREADS, 2) lora_rows_gemm_kernel(const _
   const int rank = blockIdx.x % p.split, m0 = blockIdx.y * ROWS_BM, n0 = (int)(blockIdx.x / p.split) * ROWS_BN;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const LoraParams& l = p.l;
-  // this CTA's part of the depth, whole slices of ROWS_BK
-  const int slices = (l.K + ROWS_BK - 1) / ROWS_BK, per = (slices + p.split - 1) / p.split, s0 = rank * per, s1 = min(slices, s0 + per);
+  // this CTA's part of the depth
+  const int k_begin = (int)min((int64_t)l.K, (int64_t)rank * p.part), k_end = min(l.K, k_begin + p.part);
 
-  auto bring = [&](int slice) {
-    const int k0 = slice * ROWS_BK, depth = min(ROWS_BK, l.K - k0), wide = (depth + 15) / 16 * 2;     // pieces of 8, up to whole steps of 16
+  auto bring = [&](int k0) {
+    const int depth = min(p.slice, k_end - k0), wide = (depth + 15) / 16 * 2;        // pieces of 8, up to whole steps of 16
     const T* X = reinterpret_cast<const T*>(l.X);
     const T* W = reinterpret_cast<const T*>(p.W);
     for (int e = tid; e < ROWS_BM * wide; e += ROWS_THREADS) {
@@ -133,7 +138,7 @@ __global__ void __launch_bounds__(ROWS_THREADS, 2) lora_rows_gemm_kernel(const _
     }
     umma::cp_async_commit();
   };
-  if (s0 < s1) bring(s0);
+  if (k_begin < k_end) bring(k_begin);
 
   // the outputs that this thread ends with: OUT rows of one column; bias and U B^T for them
   const int share = ROWS_BM / p.split, first = rank * share, step = ROWS_THREADS / 32;
@@ -190,10 +195,10 @@ __global__ void __launch_bounds__(ROWS_THREADS, 2) lora_rows_gemm_kernel(const _
   const uint32_t x_at = umma::smem_u32(xs) + 2 * ((wm + g1 * 8 + l8) * ROWS_XPITCH + g2 * 8);
   const uint32_t w_at = umma::smem_u32(ws) + 2 * (TRANS_W ? (wn + g2 * 8 + l8) * ROWS_XPITCH + g1 * 8 : (g1 * 8 + l8) * ROWS_WPITCH + wn + g2 * 8);
   float acc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-  for (int s = s0; s < s1; ++s) {
+  for (int k0 = k_begin; k0 < k_end; k0 += p.slice) {
     umma::cp_async_wait_all();
     __syncthreads();
-    const int depth = min(ROWS_BK, l.K - s * ROWS_BK);
+    const int depth = min(p.slice, k_end - k0);
 #pragma unroll 4
     for (int k = 0; k < depth; k += 16) {
       uint32_t af[4], bf[4];
@@ -203,7 +208,7 @@ __global__ void __launch_bounds__(ROWS_THREADS, 2) lora_rows_gemm_kernel(const _
       mma_half<BF16>(acc[1], af, bf[2], bf[3]);
     }
     __syncthreads();
-    if (s + 1 < s1) bring(s + 1);
+    if (k0 + p.slice < k_end) bring(k0 + p.slice);
   }
 #pragma unroll
   for (int j = 0; j < 2; ++j)
