@@ -112,3 +112,10 @@ def test_few_rows_at_every_split_of_the_depth(dtype, trans, M, N):
     for K in (248, 256, 264, 384, 392, 512, 520, 776, 1032, 1280, 1288, 1544, 2056, 3080, 6152):
         s = _case(np.random.default_rng(K), M, K, N, 3, 8, dtype, trans, 0, "mixed")
         _check(s, dtype, "f32", trans)
+
+
+@pytest.mark.parametrize("dtype,out", [("f16", "f16"), ("bf16", "f32")])
+@pytest.mark.parametrize("M", [1, 63, 64, 65, 128, 129, 500])
+@pytest.mark.parametrize("K,N,r,trans", [(250, 131, 12, False), (73, 600, 40, True), (31, 40, 4, False), (1, 3, 1, True)])
+def test_few_rows_that_start_anywhere(dtype, out, M, K, N, r, trans):
+    _check(_case(np.random.default_rng(M), M, K, N, 4, r, dtype, trans, 0, "mixed"), dtype, out, trans)
