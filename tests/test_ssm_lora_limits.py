@@ -125,3 +125,12 @@ def test_scratch_goes_by_the_rows_and_not_by_the_table():
             assert 0 < L.xb_lora_workspace_bytes(C.byref(a)) <= most, (n, k)
             if k.get("stride_b") == 0:                         # one B for all: its room does not go by them at all
                 assert L.xb_lora_workspace_bytes(C.byref(a)) <= a.M * 32 * 4 + a.N * 32 * 4 + 4 * 256
+
+
+def test_the_module_of_another_torch_is_refused(monkeypatch):
+    m = pkg.load()
+    assert m.capi.tensors().torch_version == torch.__version__.split("+")[0]
+    monkeypatch.setattr(m.capi, "_tensors", None)
+    monkeypatch.setattr(torch, "__version__", "1.0.0")
+    with pytest.raises(RuntimeError, match="build it again"):
+        m.capi.tensors()

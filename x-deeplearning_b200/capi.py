@@ -236,8 +236,11 @@ def tensors():
     """The extension module whose calls check torch's tensors themselves (host/binding/xb_tensors.cc)."""
     global _tensors
     if _tensors is None:
-        import torch  # noqa: F401  (its libraries come first)
-        _tensors = _extension("xb_tensors", ("xb_ssm_conv", "xb_ssm_scan_workspace_bytes", "xb_ssm_scan", "xb_lora_workspace_bytes", "xb_lora_gemm"))
+        import torch                               # (its libraries come first)
+        m = _extension("xb_tensors", ("xb_ssm_conv", "xb_ssm_scan_workspace_bytes", "xb_ssm_scan", "xb_lora_workspace_bytes", "xb_lora_gemm"))
+        if m.torch_version != torch.__version__.split("+")[0]:
+            raise RuntimeError("xb_tensors.so reads the tensors of torch %s, this is %s: build it again" % (m.torch_version, torch.__version__))
+        _tensors = m
     return _tensors
 
 

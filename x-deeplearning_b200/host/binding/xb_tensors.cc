@@ -5,6 +5,7 @@
 #include <Python.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/version.h>
 
 #include <ATen/core/Tensor.h>
 
@@ -328,4 +329,11 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "xb_tensors", nullptr, -1, methods,
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit_xb_tensors(void) { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit_xb_tensors(void) {
+  PyObject* m = PyModule_Create(&module);
+  if (m && PyModule_AddStringConstant(m, "torch_version", TORCH_VERSION) != 0) {        // (the torch whose tensors these are)
+    Py_DECREF(m);
+    return nullptr;
+  }
+  return m;
+}
