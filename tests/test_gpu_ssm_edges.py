@@ -183,3 +183,18 @@ def test_lists_behind_a_broken_one_keep_their_bits_in_the_convolution():
         again = ops.ssm_conv(x, w, b, offsets=off)
         others = [r for r in range(384) if not 10 <= r < 15]
         assert torch.equal(again[others], y[others]) and not torch.isfinite(again[10:12]).all()
+
+
+def test_scratch_that_the_device_does_not_have():
+    """The allocator's error comes as torch's own calls raise it, and nothing is left behind. (The size is made up on the host.)"""
+    ops, capi = _ops()
+    m = capi.tensors()
+    more = C.CFUNCTYPE(C.c_size_t, C.c_void_p)(lambda a: 1 << 50)
+    m.bind("xb_ssm_scan_workspace_bytes", C.cast(more, C.c_void_p).value)
+    x, A = torch.zeros(4, 8, device="cuda"), torch.zeros(8, 4, device="cuda")
+    try:
+        with pytest.raises(torch.OutOfMemoryError):
+            ops.ssm_scan(x, x, A, x[:, :4], x[:, 4:])
+    finally:
+        m.bind("xb_ssm_scan_workspace_bytes", C.cast(capi.lib().xb_ssm_scan_workspace_bytes, C.c_void_p).value)
+    assert (ops.ssm_scan(x, x, A, x[:, :4], x[:, 4:]) == 0).all()

@@ -173,7 +173,16 @@ PyObject* checked_call(const char* what, PyObject* device, F f) {
     return PyUnicode_FromString(c.text);
   } catch (const Raised&) {
     return nullptr;
-  } catch (const std::exception& e) {                    // (the allocator's: out of memory)
+  } catch (const c10::OutOfMemoryError& e) {             // (torch.OutOfMemoryError, as from torch's own calls)
+    if (PyObject* torch = PyImport_ImportModule("torch")) {
+      if (PyObject* type = PyObject_GetAttrString(torch, "OutOfMemoryError")) {
+        PyErr_SetString(type, e.what_without_backtrace());
+        Py_DECREF(type);
+      }
+      Py_DECREF(torch);
+    }
+    return nullptr;
+  } catch (const std::exception& e) {
     PyErr_SetString(PyExc_RuntimeError, e.what());
     return nullptr;
   }
