@@ -526,7 +526,8 @@ int xb_augru_shared(const void* x, const void* att, void* y_final, int32_t reque
  * is kept. An empty list leaves the state that it began with.
  * Fewer than 2^31 rows; lists and channels at most 2^31 - 1024.
  * x, y, z, delta, B, C share `dtype` (XB_F32, XB_F16, XB_BF16); every sum and the scan's states are fp32. Outputs overlap no
- * input (refused where both have one row stride or begin at one address). An infinity or NaN in a row makes no other list's results bad; its own list's may be NaN where the formula has an infinity. */
+ * input (refused where both have one row stride or begin at one address). An infinity or NaN in a row makes no other list's results bad; its own list's may be NaN where the formula has an infinity, and
+ * a NaN stays in its list's state to the list's end. Plans (and so other lists of a call) change the order of sums and nothing else. */
 
 /* y[t, c] = act(bias[c] + sum_{j < K} w[c, j] x[t - K + 1 + j, c]), x before the list's first row from its state
  * (zeros without one); act is SiLU (x * sigmoid(x)) or none. 2 <= K <= 8. */
@@ -580,7 +581,10 @@ int xb_ssm_scan(const xb_ssm_scan_args* args, void* workspace, size_t workspace_
  * are stacked into one call share the weight of a layer and differ by a product of rank r.
  *   Y[m] = X[m] W + bias + scale[a] (X[m] A[a]^T) B[a]^T,  a = adapter[m];  without the last term where a is outside [0, n_adapters)
  * Stands beside xb_gemm (GemmOp, blaze/blaze/operator/op/gemm_op.h:33-107): W as its B operand, [K, N] or with trans_w [N, K].
- * The rank-r intermediate is held in fp32. r <= 128; M, N and K at most 2^31 - 1024. Adapters may share a matrix (a stride of 0). Y overlaps
+ * The rank-r intermediate is held in fp32, or, where sums are made in tensor memory, as two TF32 terms (2^-22 of it). Those sums are cut off where
+ * fp32 additions round, which fp32 results of 16-bit operands show: fp16, rms relative to 64 bits, K = 250 9e-8 for few rows (up to 511 off 16 bytes,
+ * else up to 2048 whose tiles of 64 x 32 fill at most two blocks an SM) and 4.6e-7 for more, K = 1280 1.1e-7 and 1.7e-6, of positive values 5e-8 and
+ * 8e-6. r <= 128; M, N and K at most 2^31 - 1024. Adapters may share a matrix (a stride of 0). Y overlaps
  * no input (refused for X where both have one row stride in bytes or begin at one address). */
 typedef struct xb_lora_args {
   int32_t M, N, K, r, n_adapters;

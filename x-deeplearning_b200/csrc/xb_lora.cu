@@ -127,10 +127,12 @@ __global__ void __launch_bounds__(128) lora_rows_expand_kernel(const LoraParams 
 // the tensor-core tiles and this kernel: 960 rows, N = 152, rank 8 31 and 19, rank 64 66 and 28; 1920 rows 31 and 29, 66 and 49; 256 rows,
 // N = 2048 28 and 28, 50 and 33; past two blocks: 448 rows, N = 2048 30 and 48; 1472, N = 600 33 and 49. Few columns and more rows:
 // 4800, N = 40, rank 64 73 and 79, at K = 64 27 and 38.
-// Rows that the kernel cannot take (not on 16 bytes) are laid out for the tensor cores where there are more than 64. us in a graph as rows and so, 8
+// Rows that the kernel cannot take (not on 16 bytes) are laid out for the tensor cores where there are more than 64, fp32 results from 512 rows on:
+// sums in tensor memory are cut off, [M, 250] x [250, 131] fp16 4.6e-7 (positive values 1.4e-6) from 64 bits, rms, where sums of 16 products that are added
+// in fp32 are 9e-8, which 16-bit results do not show; past 512 rows that would cost more than 8 us a call. us in a graph as rows and so, 8
 // adapters, bf16: [M, 250] x [250, 131], rank 12, fp32 results, M = 32 16.8 and 16.8, 64 20.0 and 17.3, 256 20.2 and 14.1, 1024 23.8 and 12.6; [M, 73] x
 // [73, 600], rank 8, 32 11.5 and 15.3, 64 14.4 and 14.4, 128 14.9 and 14.3, 256 15.2 and 11.3; [M, 31] x [31, 40], rank 4, 32 11.4 and 14.3, 64 14.5 and 13.3.
-constexpr int ROWS_MOST = 2048, ROWS_ODD = 64;
+constexpr int ROWS_MOST = 2048, ROWS_ODD = 64, ROWS_ODD_F32 = 511;
 bool on_16_bytes(const xb_lora_args& a) {
   auto lies = [](const void* q, int64_t ld) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0 && ld % 8 == 0; };
   return lies(a.X, a.ldx) && lies(a.W, a.ldw);
@@ -139,7 +141,7 @@ bool takes_rows_kernel(const xb_lora_args& a) {
   const int64_t tiles = ((int64_t)a.N + ROWS_BN - 1) / ROWS_BN * ((a.M + ROWS_BM - 1) / ROWS_BM);
   return a.dtype != XB_F32 && on_16_bytes(a) && a.M <= ROWS_MOST && tiles <= 2 * sm_count();
 }
-bool takes_tiles(const xb_lora_args& a) { return lora_umma_takes(a) && !takes_rows_kernel(a) && (on_16_bytes(a) || a.M > ROWS_ODD); }
+bool takes_tiles(const xb_lora_args& a) { return lora_umma_takes(a) && !takes_rows_kernel(a) && (on_16_bytes(a) || a.M > (a.y_dtype == XB_F32 ? ROWS_ODD_F32 : ROWS_ODD)); }
 
 constexpr size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
