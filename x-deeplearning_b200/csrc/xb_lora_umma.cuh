@@ -340,7 +340,7 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
 
 // The one-CTA GEMM kernel of xb_gemm_umma.cu without batches and resident weights, whose tiles go on through the adapters' products: the
 // stages have the same size (128 rows of 128 bytes of X or U, block_n of W or B), only the maps and the MMAs differ.
-// [65536, 1280] x [1280, 1024], 32 adapters of rank 16: 155 us = 1.1 PFLOP/s, tensor pipe 62 % busy. One-CTA tiles of 128 x 256 read 48 KB
+// [65536, 1280] x [1280, 1024], 32 adapters of rank 16: 155 us = 1.1 PFLOP/s at 1965 MHz (the call 188; 231 where power holds the clock down), tensor pipe 62 % busy. One-CTA tiles of 128 x 256 read 48 KB
 // from L2 for 64 of the depth, which is the bound; xb_gemm's pairs of CTAs halve W's part of it (130-140 us for the projection alone).
 enum { LORA_Y_TMA, LORA_Y_ANY };
 template <typename TOut, bool B_MN, int Y>

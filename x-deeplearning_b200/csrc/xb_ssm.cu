@@ -108,7 +108,7 @@ __global__ void __launch_bounds__(CONV_THREADS) ssm_conv_step_kernel(const ConvP
 // on in place are read and written by one thread.
 // Pieces of 8 bytes and eight rows ahead: with 16-byte pieces and four rows the registers let half as many warps in, which is what
 // the loads in flight are. SiLU is the rest: an exponential and a quotient a value. Bound by the latency of the reads in flight:
-// 1024 lists of 262144 rows in all, D = 512, bf16 134 us = 4.0 TB/s, 0.62 of a copy's rate, 24 warps an SM, SFUs 36 % busy. The
+// 1024 lists of 262144 rows in all, D = 512, bf16 135 us = 4.0 TB/s, 0.62 of a copy's rate, 24 warps an SM, SFUs 49 % busy. The
 // next rows asked for before these are written, and longer or shorter walks, are no faster.
 template <typename T, int V, int K>
 constexpr int CONV_BLOCKS = K <= 4 && V * sizeof(T) <= 8 ? 6 : 4;         // of an SM: the registers are shared among so many

@@ -477,7 +477,7 @@ struct Decay {
 // block has 32 (channel, state) pairs and splits the chunks among its 32 warps: each makes its own part's decay and sum, takes what
 // comes in from the parts before it, and walks its part again. Bound by the latency of its reads: none waits for another (what stands in
 // the place of a chunk that is none is dropped). [30011, 202], N = 10, 156 chunks: the call 145 us with 8 warps that asked first what
-// a chunk is, 128 now.
+// a chunk is, 129 now.
 constexpr int CARRY_PARTS = 32;
 __global__ void __launch_bounds__(32 * CARRY_PARTS) ssm_carry_kernel(const ScanParams p) {
   pdl_begin();
