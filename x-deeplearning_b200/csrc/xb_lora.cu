@@ -73,8 +73,7 @@ __global__ void __launch_bounds__(128) lora_rows_expand_kernel(const LoraParams 
   pdl_begin();
   __shared__ float s_u[ROWS][LORA_MAX_RANK];
   __shared__ int s_a[ROWS];
-  const unsigned row_blocks = ((unsigned)p.M + ROWS - 1) / ROWS;         // (of 128 columns each, one behind the other)
-  const int m0 = (int)(blockIdx.x % row_blocks) * ROWS, n = (int)(blockIdx.x / row_blocks) * 128 + threadIdx.x;
+  const int m0 = blockIdx.x * ROWS, n = blockIdx.y * 128 + threadIdx.x;
   if (threadIdx.x < ROWS) s_a[threadIdx.x] = m0 + (int)threadIdx.x < p.M ? adapter_of(p, m0 + threadIdx.x) : -1;
   __syncthreads();
   for (int i = threadIdx.x; i < ROWS * p.r; i += 128) {
@@ -127,12 +126,11 @@ __global__ void __launch_bounds__(128) lora_rows_expand_kernel(const LoraParams 
 // the tensor-core tiles and this kernel: 960 rows, N = 152, rank 8 31 and 19, rank 64 66 and 28; 1920 rows 31 and 29, 66 and 49; 256 rows,
 // N = 2048 28 and 28, 50 and 33; past two blocks: 448 rows, N = 2048 30 and 48; 1472, N = 600 33 and 49. Few columns and more rows:
 // 4800, N = 40, rank 64 73 and 79, at K = 64 27 and 38.
-// Rows that the kernel cannot take (not on 16 bytes) are laid out for the tensor cores where there are more than 64, fp32 results from 512 rows on:
-// sums in tensor memory are cut off, [M, 250] x [250, 131] fp16 4.6e-7 (positive values 1.4e-6) from 64 bits, rms, where sums of 16 products that are added
-// in fp32 are 9e-8, which 16-bit results do not show; past 512 rows that would cost more than 8 us a call. us in a graph as rows and so, 8
-// adapters, bf16: [M, 250] x [250, 131], rank 12, fp32 results, M = 32 16.8 and 16.8, 64 20.0 and 17.3, 256 20.2 and 14.1, 1024 23.8 and 12.6; [M, 73] x
-// [73, 600], rank 8, 32 11.5 and 15.3, 64 14.4 and 14.4, 128 14.9 and 14.3, 256 15.2 and 11.3; [M, 31] x [31, 40], rank 4, 32 11.4 and 14.3, 64 14.5 and 13.3.
-constexpr int ROWS_MOST = 2048, ROWS_ODD = 64, ROWS_ODD_F32 = 511;
+// Rows that the kernel cannot take (not on 16 bytes) are laid out for the tensor cores from 512 on, whatever their adapters: us in a graph as rows and
+// so, 8 adapters, bf16, [M, 250] x [250, 131], rank 12, M = 64 20.0 and 17.3, 512 21.0 and 11.4, 1024 24.0 and 11.1; [M, 73] x [73, 600], rank 8, 64 14.4
+// and 14.4, 512 16.3 and 10.1; but 350 rows of 67 requests with 50 adapters, [350, 19] x [19, 114], rank 8, fp16 13.5 and 21.1: a tile has a product
+// for each of its adapters, and few tiles have all of a call's. fp32 results also show that sums in tensor memory are cut off.
+constexpr int ROWS_MOST = 2048, ROWS_ODD = 511;
 bool on_16_bytes(const xb_lora_args& a) {
   auto lies = [](const void* q, int64_t ld) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0 && ld % 8 == 0; };
   return lies(a.X, a.ldx) && lies(a.W, a.ldw);
@@ -141,16 +139,17 @@ bool takes_rows_kernel(const xb_lora_args& a) {
   const int64_t tiles = ((int64_t)a.N + ROWS_BN - 1) / ROWS_BN * ((a.M + ROWS_BM - 1) / ROWS_BM);
   return a.dtype != XB_F32 && on_16_bytes(a) && a.M <= ROWS_MOST && tiles <= 2 * sm_count();
 }
-bool takes_tiles(const xb_lora_args& a) { return lora_umma_takes(a) && !takes_rows_kernel(a) && (on_16_bytes(a) || a.M > (a.y_dtype == XB_F32 ? ROWS_ODD_F32 : ROWS_ODD)); }
+bool takes_tiles(const xb_lora_args& a) { return lora_umma_takes(a) && !takes_rows_kernel(a) && (on_16_bytes(a) || a.M > ROWS_ODD); }
 
 constexpr size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
 bool has_adapters(const xb_lora_args& a) { return a.n_adapters > 0 && a.r > 0; }
 
+constexpr int TURN_COLS = 65535 * 128;    // columns of a turn: a grid's second dimension of lora_rows_expand_kernel's blocks
 // Rows of a turn: the fp32 addend of a turn (M x N) is at most 64 MB, so that it is still in L2 when the product reads it, and no more than
 // xb_gemm's CUDA cores take in a call.
 int turn_rows(const xb_lora_args& a) {
-  const int64_t rows = std::max<int64_t>(((int64_t)16 << 20) / std::max(a.N, 1) / 128 * 128, 128);
+  const int64_t rows = std::max<int64_t>(((int64_t)16 << 20) / std::clamp(a.N, 1, TURN_COLS) / 128 * 128, 128);
   return (int)std::min<int64_t>({rows, a.M, 32767 * 128});
 }
 
@@ -164,7 +163,7 @@ RowsScratch rows_scratch(const xb_lora_args& a) {
   const size_t turn = (size_t)turn_rows(a);
   RowsScratch s;
   s.part = align256(turn * a.r * 4);
-  s.w = s.part + align256(turn * a.N * 4);
+  s.w = s.part + align256(turn * std::min(a.N, TURN_COLS) * 4);
   s.bytes = s.w + (lays_out_w(a) ? (size_t)a.K * laid_out_ld(a) * 4 : 0);
   return s;
 }
@@ -225,11 +224,9 @@ int launch_shrink(const LoraParams& p, bool vec, cudaStream_t s) {
 template <typename T>
 int launch_expand(const LoraParams& p, bool vec, cudaStream_t s) {
   // eight rows a block share what they read of B; two where that would leave SMs idle
-  const int64_t cols = ((int64_t)p.N + 127) / 128;
+  const unsigned cols = (unsigned)((p.N + 127) / 128);
   const bool few = (int64_t)((p.M + 7) / 8) * cols < 4 * sm_count();
-  const int64_t blocks = (few ? (p.M + 1) / 2 : (p.M + 7) / 8) * cols;
-  XB_REQUIRE(blocks < ((int64_t)1 << 31), XB_ERR_LIMIT, "xb_lora_gemm: %d x %d are too many for one call", p.M, p.N);
-  const unsigned grid = (unsigned)blocks;
+  const dim3 grid((unsigned)(few ? (p.M + 1) / 2 : (p.M + 7) / 8), cols);
   if (few) {
     if (vec) launch_dependent(lora_rows_expand_kernel<T, true, 2>, grid, 128, 0, s, p);
     else launch_dependent(lora_rows_expand_kernel<T, false, 2>, grid, 128, 0, s, p);
@@ -260,8 +257,8 @@ int run_rows(const xb_lora_args& a, uint8_t* ws, cudaStream_t s) {
   g.N = a.N; g.K = a.K; g.trans_b = a.trans_w; g.alpha = g.beta = 1.f; g.batch = 1;
   g.lda = a.ldx; g.B = a.W; g.ldb = a.ldw; g.ldy = a.ldy; g.ab_dtype = a.dtype; g.y_dtype = a.y_dtype;
   g.bias_dtype = XB_F32;
-  if (p.n_adapters) { g.bias = p.part; g.ldbias = a.N; g.bias_kind = XB_BIAS_FULL; }
-  else if (a.bias) { g.bias = a.bias; g.bias_kind = XB_BIAS_ROW; }          // without adapters: the projection alone
+  if (p.n_adapters) { g.bias = p.part; g.bias_kind = XB_BIAS_FULL; }
+  else if (a.bias) g.bias_kind = XB_BIAS_ROW;                               // without adapters: the projection alone
   if constexpr (sizeof(T) == 2) {
     // the projection and the products with B in one kernel (its rows are one turn: at most 2 sm_count() tiles of 64 x 32)
     if (takes_rows_kernel(a)) {
@@ -291,20 +288,32 @@ int run_rows(const xb_lora_args& a, uint8_t* ws, cudaStream_t s) {
     if (int rc = check_launch("lora_layout_kernel")) return rc;
     g.B = to; g.ldb = laid_out_ld(a); g.trans_b = 0;
   }
+  const void* W = g.B;
   for (int64_t m0 = 0; m0 < a.M; m0 += turn) {
     p.M = (int)std::min<int64_t>(turn, a.M - m0);
     p.X = reinterpret_cast<const T*>(a.X) + m0 * a.ldx;
     p.adapter = p.n_adapters ? a.adapter + m0 : nullptr;
     if (int rc = launch_shrink<T>(p, vec_k, s)) return rc;
-    if (p.n_adapters)
-      if (int rc = launch_expand<T>(p, vec_r, s)) return rc;
-    g.M = p.M;
-    g.A = p.X;
-    g.Y = reinterpret_cast<uint8_t*>(a.Y) + m0 * a.ldy * (int64_t)dtype_size(a.y_dtype);
-    // (fp32 results of rows that TMA cannot address: matrix instructions here, where xb_gemm stays with the CUDA cores for the sake of its bits.
-    // [5003, 250] x [250, 131] bf16: 127 us there)
-    const bool half = a.dtype != XB_F32 && a.y_dtype == XB_F32 && !xb_gemm_uses_tcgen05(&g);
-    if (int rc = half ? gemm_half_sums(g, s) : xb_gemm(&g, s)) return rc;
+    for (int64_t n0 = 0; n0 < a.N; n0 += TURN_COLS) {
+      p.N = (int)std::min<int64_t>(TURN_COLS, a.N - n0);
+      p.B = reinterpret_cast<const T*>(a.B) + n0 * a.ldb;
+      p.bias = a.bias ? a.bias + n0 : nullptr;
+      if (p.n_adapters) {
+        if (int rc = launch_expand<T>(p, vec_r, s)) return rc;
+        g.ldbias = p.N;
+      } else {
+        g.bias = p.bias;
+      }
+      g.M = p.M;
+      g.N = p.N;
+      g.A = p.X;
+      g.B = reinterpret_cast<const T*>(W) + (g.trans_b ? n0 * g.ldb : n0);
+      g.Y = reinterpret_cast<uint8_t*>(a.Y) + (m0 * a.ldy + n0) * (int64_t)dtype_size(a.y_dtype);
+      // (fp32 results of rows that TMA cannot address: matrix instructions here, where xb_gemm stays with the CUDA cores for the sake of its bits.
+      // [5003, 250] x [250, 131] bf16: 127 us there)
+      const bool half = a.dtype != XB_F32 && a.y_dtype == XB_F32 && !xb_gemm_uses_tcgen05(&g);
+      if (int rc = half ? gemm_half_sums(g, s) : xb_gemm(&g, s)) return rc;
+    }
   }
   return 0;
 }
