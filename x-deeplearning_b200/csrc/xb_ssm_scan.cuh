@@ -458,19 +458,17 @@ __global__ void __launch_bounds__(1024) ssm_order_kernel(const ScanParams p) {
   for (int i = tid; i < p.lists.batch; i += 1024) p.order[atomicAdd(&s_at[class_of(i)], 1)] = i;
 }
 
-// 2^q for any q: the rows of a chunk each have a decay that fp32 holds where the chunk's need not, so it comes as three factors of exponents up
-// to 126 (beyond 378 no finite state but 0 gives a number that is neither infinite nor 0; an infinite q is the rows' own).
-constexpr float NEAR = 126.f;
+// 2^q as two factors: the rows of a chunk each have a decay that fp32 holds where the chunk's need not. Exponents from -252 to 254 leave of any
+// state that is not 0 less than 2^-124, or more than fp32 holds. (Where q is infinite or a NaN the chunk's own end is.)
 struct Decay {
-  float f[3];
+  float f[2];
   __device__ __forceinline__ void of(float q) {
-    auto part = [](float v) { return fminf(fmaxf(v, -NEAR), NEAR); };
-    const float q1 = part(q), q2 = part(q - q1), rest = q - q1 - q2;
-    f[0] = ex2(q1);
-    f[1] = ex2(q2);
-    f[2] = ex2(fabsf(rest) <= 3.4028235e38f ? part(rest) : rest);
+    auto part = [](float v) { return fminf(fmaxf(v, -126.f), 127.f); };
+    const float q0 = part(q);
+    f[0] = ex2(q0);
+    f[1] = ex2(part(q - q0));
   }
-  __device__ __forceinline__ float apply(float e, float own) const { return fmaf(f[0], f[1] * (f[2] * e), own); }
+  __device__ __forceinline__ float apply(float e, float own) const { return fmaf(f[0], f[1] * e, own); }
 };
 
 // What the ends are with the states that come into their chunks: end[j] += exp(A steps[j]) end[j - 1] where chunk j is not its list's first. A
@@ -479,9 +477,9 @@ struct Decay {
 // the place of a chunk that is none is dropped). [30011, 202], N = 10, 156 chunks: the call 145 us with 8 warps that asked first what
 // a chunk is, 129 now.
 constexpr int CARRY_PARTS = 32;
-__global__ void __launch_bounds__(32 * CARRY_PARTS) ssm_carry_kernel(const ScanParams p) {
+__global__ void __launch_bounds__(32 * CARRY_PARTS, 2) ssm_carry_kernel(const ScanParams p) {
   pdl_begin();
-  __shared__ float s_f[3][CARRY_PARTS][32], s_e[CARRY_PARTS][32];
+  __shared__ float s_f[2][CARRY_PARTS][32], s_e[CARRY_PARTS][32];
   __shared__ bool s_cut[CARRY_PARTS];                   // a list begins in the part
   const int part = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int64_t pairs = (int64_t)p.D * p.N, at = (int64_t)blockIdx.x * 32 + lane;
@@ -513,14 +511,15 @@ __global__ void __launch_bounds__(32 * CARRY_PARTS) ssm_carry_kernel(const ScanP
   if (lane == 0) s_cut[part] = cut;
   Decay all;
   all.of(Q);
-#pragma unroll
-  for (int i = 0; i < 3; ++i) s_f[i][part][lane] = all.f[i];
+  s_f[0][part][lane] = all.f[0];
+  s_f[1][part][lane] = all.f[1];
   s_e[part][lane] = e;
   __syncthreads();
+  if (j0 == j1) return;
   e = 0.f;
-#pragma unroll 4
+#pragma unroll 8
   for (int k = 0; k < part; ++k) {
-    const Decay d = {{s_f[0][k][lane], s_f[1][k][lane], s_f[2][k][lane]}};
+    const Decay d = {{s_f[0][k][lane], s_f[1][k][lane]}};
     const float own = s_e[k][lane];
     e = s_cut[k] ? own : d.apply(e, own);
   }
