@@ -203,8 +203,11 @@ struct Pass {
   }
 };
 
-// the number of an adapter's A among those that map_a covers
-__device__ __forceinline__ int a_number(const LoraTiles& p, uint32_t a) { return p.a_named ? p.named.place[a] : (int)a * p.a_step; }
+// The number of an adapter's A among those that map_a covers, of a whole warp's adapter a. (A reduction, so that it stands where the instructions that
+// issue copies take their operands from: computed at each copy it cost lora_fused_kernel 3 %.)
+__device__ __forceinline__ int a_number(const LoraTiles& p, uint32_t a) {
+  return (int)__reduce_max_sync(0xffffffffu, p.a_named ? (uint32_t)p.named.place[a] : a * (uint32_t)p.a_step);
+}
 
 constexpr int SHRINK_THREADS = 320;       // producer, MMA, four warps for the results, four for B
 constexpr int SHRINK_GROUP_ROWS = 64;     // rows of A (adapters x rb) in a stage, or rb where that is more
@@ -639,6 +642,9 @@ lora_fused_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
     uint32_t ph = 0;
     each_item([&](const LoraItem& item) {
       const uint32_t bytes = (uint32_t)(A_STAGE_BYTES + (item.first ? w_bytes : 0) + item.n * box);
+      int at[SHRINK_GROUP];
+#pragma unroll
+      for (int i = 0; i < SHRINK_GROUP; ++i) at[i] = i < item.n ? a_number(l, item.id[i]) : 0;
       for (int kb = 0; kb < num_kb; ++kb, s = (s + 1 == STAGES ? 0 : s + 1), ph ^= (s == 0 ? 1u : 0u)) {
         const uint32_t x = smem_u32(smem + s * stage_bytes), w = x + A_STAGE_BYTES, a = w + w_bytes, bar = smem_u32(&full_bar[s]);
         if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&empty_bar[s]), ph ^ 1u, 71))) return false;
@@ -653,7 +659,7 @@ lora_fused_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
         }
 #pragma unroll
         for (int i = 0; i < SHRINK_GROUP; ++i)
-          if (i < item.n) tma_load_3d_elect(a + i * box, &map_a, bar, kb * BLOCK_K, 0, l.a_named ? l.named.place[item.id[i]] : (int)item.id[i] * l.a_step);
+          if (i < item.n) tma_load_3d_elect(a + i * box, &map_a, bar, kb * BLOCK_K, 0, at[i]);
       }
       return true;
     });
