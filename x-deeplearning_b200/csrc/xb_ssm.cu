@@ -110,8 +110,10 @@ __global__ void __launch_bounds__(CONV_THREADS) ssm_conv_step_kernel(const ConvP
 // the loads in flight are. SiLU is the rest: an exponential and a quotient a value. Bound by the latency of the reads in flight:
 // 1024 lists of 262144 rows in all, D = 512, bf16 135 us = 4.0 TB/s, 0.62 of a copy's rate, 24 warps an SM, SFUs 49 % busy. The
 // next rows asked for before these are written, and longer or shorter walks, are no faster.
+// Blocks of an SM, among which the registers are shared: with fewer the compiler takes more (two taps of fp32 122 of them: 781 lists of 14810 rows, D = 24
+// 11.2 us, 8.3 so), with more it spills.
 template <typename T, int V, int K>
-constexpr int CONV_BLOCKS = K <= 4 && V * sizeof(T) <= 8 ? 6 : 4;         // of an SM: the registers are shared among so many
+constexpr int CONV_BLOCKS = K == 2 || (K <= 4 && V * sizeof(T) <= 8) ? 6 : K == 3 ? 5 : 4;
 template <typename T, int V, int K>
 __global__ void __launch_bounds__(CONV_THREADS, CONV_BLOCKS<T, V, K>) ssm_conv_kernel(const ConvParams p) {
   pdl_begin();
