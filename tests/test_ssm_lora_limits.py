@@ -134,3 +134,11 @@ def test_the_module_of_another_torch_is_refused(monkeypatch):
     monkeypatch.setattr(torch, "__version__", "1.0.0")
     with pytest.raises(RuntimeError, match="build it again"):
         m.capi.tensors()
+
+
+@pytest.mark.parametrize("suffix", ["", "+cu128", ".dev20260101+cu128", "a0+git1234567"])
+def test_builds_of_one_torch_are_one(monkeypatch, suffix):
+    m = pkg.load()
+    monkeypatch.setattr(torch, "__version__", m.capi.tensors().torch_version + suffix)
+    monkeypatch.setattr(m.capi, "_tensors", None)
+    assert m.capi.tensors().torch_version

@@ -3,6 +3,7 @@ import ctypes as C
 import importlib.machinery
 import importlib.util
 import os
+import re
 import subprocess
 import sys
 
@@ -238,7 +239,7 @@ def tensors():
     if _tensors is None:
         import torch                               # (its libraries come first)
         m = _extension("xb_tensors", ("xb_ssm_conv", "xb_ssm_scan_workspace_bytes", "xb_ssm_scan", "xb_lora_workspace_bytes", "xb_lora_gemm"))
-        if m.torch_version != torch.__version__.split("+")[0]:
+        if m.torch_version != re.match(r"\d+\.\d+\.\d+|", torch.__version__).group():        # (the headers know no more of it)
             raise RuntimeError("xb_tensors.so reads the tensors of torch %s, this is %s: build it again" % (m.torch_version, torch.__version__))
         _tensors = m
     return _tensors
