@@ -301,7 +301,8 @@ def ssm_conv(x, w, bias=None, offsets=None, T=None, state_in=None, state_out=Non
 
     w [D, K], bias [D]. Lists: `offsets` int32 [lists + 1], or of T rows each (T = 1: one new row a list; None: one list).
     state_in / state_out [slots, K - 1, D]: the inputs before each list and the last ones of it, in row slots[i] for list i (its own
-    number without `slots`); they may be one array. Returns [rows, D]; rows behind the last list are not written."""
+    number without `slots`); they may be one array. Returns [rows, D] (`out`, which may not lie over x); rows behind the last list are
+    not written."""
     return _done((_checked or _calls()).ssm_conv(x, w, bias, offsets, T, state_in, state_out, slots, silu, out, *_where()))
 
 
@@ -311,7 +312,7 @@ def ssm_scan(x, delta, A, B, C, D=None, z=None, delta_bias=None, groups=1, softp
 
     delta, z as x; B, C [rows, groups * N]; A [channels, N], D and delta_bias [channels], h_in / h_out [slots, channels, N] fp32.
     Lists and slots as in ssm_conv; `longest`: rows of the longest list where the caller knows it (the plan goes by it, no result).
-    `workspace`: uint8 scratch for callers that keep one; by default the call takes its own."""
+    `workspace`: contiguous uint8 scratch for callers that keep one; by default the call takes its own."""
     return _done((_checked or _calls()).ssm_scan(x, delta, A, B, C, D, z, delta_bias, groups, softplus, offsets, T, longest, h_in, h_out, slots,
                                                  out, workspace, *_where()))
 
