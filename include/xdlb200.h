@@ -577,6 +577,59 @@ size_t xb_ssm_scan_workspace_bytes(const xb_ssm_scan_args* args);
 int xb_ssm_scan(const xb_ssm_scan_args* args, void* workspace, size_t workspace_bytes, xb_stream_t stream);
 
 /* ------------------------------------------------------------------------- */
+/* Attention over behaviour lists. No operators of Blaze; they stand where the attention unit and xb_gru stand (an extractor over a user's
+ * behaviours, and the candidates of a request against them). Rows of several heads: element c of head h of row t is at
+ * base + t * row + h * head + c (strides in elements, >= 0), so that slices of one projection of queries, keys and values are taken as
+ * they lie. Outputs overlap no input, but for yq and yk of xb_qk_norm_rope, which may be q and k themselves. Every sum is fp32. */
+
+/* Norms of queries and keys for each head, and the position rotation of their first `rot` channels (even) in the same pass:
+ *   x' = x / sqrt(mean(x^2) + eps) * weight  (norm = 0: x' = x)
+ *   y[a] = x'[a] cos w - x'[b] sin w,  y[b] = x'[b] cos w + x'[a] sin w,  w = positions[t] freqs[j],  j < rot / 2
+ * with (a, b) = (j, j + rot / 2), or (2 j, 2 j + 1) with `adjacent`. The angle is taken in 64 bits. d <= 256. */
+typedef struct xb_qk_norm_rope_args {
+  const void* q; int64_t q_row, q_head;           /* [rows, Hq, d] */
+  const void* k; int64_t k_row, k_head;           /* [rows, Hk, d]; Hk = 0: none */
+  void* yq; int64_t yq_row, yq_head;
+  void* yk; int64_t yk_row, yk_head;
+  const float* q_weight;                          /* [d], NULL: 1 */
+  const float* k_weight;
+  const int32_t* positions;                       /* [rows] */
+  const float* freqs;                             /* [rot / 2] */
+  int64_t rows;
+  int32_t Hq, Hk, d, rot;
+  int32_t norm, adjacent;
+  float eps;
+  int32_t dtype;                                  /* XB_F32, XB_F16 or XB_BF16 */
+} xb_qk_norm_rope_args;
+int xb_qk_norm_rope(const xb_qk_norm_rope_args* args, xb_stream_t stream);
+
+/* Linear attention with a decay for each head, over lists with kept states (offsets, slots and states as for xb_ssm_scan above):
+ *   S_t = exp(log_decay[h]) S_{t-1} + k[t, h'] v[t, h']^T,   y[t, h] = scale q[t, h] S_t,   h' = h / (H / Hkv)
+ * log_decay <= 0 (-infinity: no memory; what is above 0 counts as 0). The states [n_slots, H, dk, dv] are fp32. 16-bit lists of more than
+ * a few rows go by chunks of 64 on the matrix instructions: states to 22 bits an operand and more, what makes y (scores, states) to TF32,
+ * 2^-12 of it; fp32 lists by fp32 FMAs alone. dk, dv <= 128. An infinity or NaN in a row makes no other list's results bad; its own list's
+ * may be NaN where the formula has an infinity. */
+typedef struct xb_linear_attention_args {
+  const void* q; int64_t q_row, q_head;           /* [rows, H, dk] */
+  const void* k; int64_t k_row, k_head;           /* [rows, Hkv, dk] */
+  const void* v; int64_t v_row, v_head;           /* [rows, Hkv, dv] */
+  void* y; int64_t y_row, y_head;                 /* [rows, H, dv] */
+  const float* log_decay;                         /* [H] */
+  const int32_t* offsets;
+  const int32_t* slots;                           /* [batch] */
+  const float* h_in;                              /* [n_slots, H, dk, dv] */
+  float* h_out;
+  int64_t rows;
+  int64_t longest;                                /* no list has more rows than this, or 0: not known. Only the plan goes by it. */
+  int32_t batch, n_slots, H, Hkv, dk, dv;
+  float scale;
+  int32_t dtype;                                  /* q, k, v, y: XB_F32, XB_F16 or XB_BF16 */
+} xb_linear_attention_args;
+/* Scratch of a call with these arguments (0 for many): one call uses it at a time. */
+size_t xb_linear_attention_workspace_bytes(const xb_linear_attention_args* args);
+int xb_linear_attention(const xb_linear_attention_args* args, void* workspace, size_t workspace_bytes, xb_stream_t stream);
+
+/* ------------------------------------------------------------------------- */
 /* A projection shared by all rows beside a low-rank adapter of each row's own: scenes (pages, markets, tenants) whose requests
  * are stacked into one call share the weight of a layer and differ by a product of rank r.
  *   Y[m] = X[m] W + bias + scale[a] (X[m] A[a]^T) B[a]^T,  a = adapter[m];  without the last term where a is outside [0, n_adapters)

@@ -95,6 +95,20 @@ class LoraArgs(C.Structure):
                 ("scale", vp), ("bias", vp), ("adapter", vp), ("Y", vp), ("ldy", i64), ("dtype", i32), ("y_dtype", i32)]
 
 
+class QkNormRopeArgs(C.Structure):
+    _fields_ = [("q", vp), ("q_row", i64), ("q_head", i64), ("k", vp), ("k_row", i64), ("k_head", i64), ("yq", vp), ("yq_row", i64),
+                ("yq_head", i64), ("yk", vp), ("yk_row", i64), ("yk_head", i64), ("q_weight", vp), ("k_weight", vp), ("positions", vp),
+                ("freqs", vp), ("rows", i64), ("Hq", i32), ("Hk", i32), ("d", i32), ("rot", i32), ("norm", i32), ("adjacent", i32),
+                ("eps", f32), ("dtype", i32)]
+
+
+class LinearAttentionArgs(C.Structure):
+    _fields_ = [("q", vp), ("q_row", i64), ("q_head", i64), ("k", vp), ("k_row", i64), ("k_head", i64), ("v", vp), ("v_row", i64),
+                ("v_head", i64), ("y", vp), ("y_row", i64), ("y_head", i64), ("log_decay", vp), ("offsets", vp), ("slots", vp), ("h_in", vp),
+                ("h_out", vp), ("rows", i64), ("longest", i64), ("batch", i32), ("n_slots", i32), ("H", i32), ("Hkv", i32), ("dk", i32),
+                ("dv", i32), ("scale", f32), ("dtype", i32)]
+
+
 # every symbol include/xdlb200.h declares: (restype, argtypes)
 SYMBOLS = {
     "xb_last_error": (C.c_char_p, []),
@@ -164,6 +178,9 @@ SYMBOLS = {
     "xb_ssm_scan": (i32, [C.POINTER(SsmScanArgs), vp, C.c_size_t, vp]),
     "xb_lora_workspace_bytes": (C.c_size_t, [C.POINTER(LoraArgs)]),
     "xb_lora_gemm": (i32, [C.POINTER(LoraArgs), vp, C.c_size_t, vp]),
+    "xb_qk_norm_rope": (i32, [C.POINTER(QkNormRopeArgs), vp]),
+    "xb_linear_attention_workspace_bytes": (C.c_size_t, [C.POINTER(LinearAttentionArgs)]),
+    "xb_linear_attention": (i32, [C.POINTER(LinearAttentionArgs), vp, C.c_size_t, vp]),
     "xb_dice": (i32, [vp, vp, i64, i32, vp, vp, vp, i32, i32, vp]),
     "xb_prelu": (i32, [vp, vp, i64, vp, i64, i32, i32, vp]),
     "xb_sigmoid": (i32, [vp, vp, i64, i32, vp]),
@@ -238,7 +255,8 @@ def tensors():
     global _tensors
     if _tensors is None:
         import torch                               # (its libraries come first)
-        m = _extension("xb_tensors", ("xb_ssm_conv", "xb_ssm_scan_workspace_bytes", "xb_ssm_scan", "xb_lora_workspace_bytes", "xb_lora_gemm"))
+        m = _extension("xb_tensors", ("xb_ssm_conv", "xb_ssm_scan_workspace_bytes", "xb_ssm_scan", "xb_lora_workspace_bytes", "xb_lora_gemm",
+                                      "xb_qk_norm_rope", "xb_linear_attention_workspace_bytes", "xb_linear_attention"))
         if m.torch_version != re.match(r"\d+\.\d+\.\d+|", torch.__version__).group():        # (the headers know no more of it)
             raise RuntimeError("xb_tensors.so reads the tensors of torch %s, this is %s: build it again" % (m.torch_version, torch.__version__))
         _tensors = m

@@ -1,0 +1,379 @@
+// Linear attention with a decay for each head: what its kernels share, and the one that goes row by row (formulas in xdlb200.h).
+//
+// A long list is cut into segments of `chunk` rows, counted from the list's beginning, where whole lists would leave SMs idle. Three launches:
+// every segment but a list's last makes the state at its end as if it began with zeros (the first one: with the list's state); those are carried
+// from segment to segment, in order; then all segments run from the state that they begin with.
+#pragma once
+
+#include <algorithm>
+#include <cmath>
+
+#include "xb_heads.cuh"
+#include "xb_mma_half.cuh"
+
+namespace xb {
+
+struct LinearParams {
+  Heads q, k, v, y;
+  const float* log_decay;
+  const float* h_in;
+  float* h_out;
+  Lists lists;
+  int H, share, dk, dv;                    // share: heads that read one head of k and v
+  float scale;
+  int vec_q, vec_k, vec_v, vec_y;          // rows in whole pieces: of four elements, y of two
+  int vec_h, vec_e;                        // kept states in pairs; the ends of segments in pieces of four
+  int64_t chunk;                           // 0: whole lists
+  int n_ends;                              // rows / chunk
+  float* end;                              // [n_ends][H][dk][dv]: states at the ends of segments
+  float* first;                            // the same, of lists' first segments: copies of what they begin with
+  int ends_only;                           // the first of the three launches
+};
+struct LinearPlan {
+  bool tiles;                              // by chunks of 64 rows on the matrix instructions, else row by row
+  int64_t chunk;
+};
+// the kernels of one type (xb_linear_*.cu)
+int linear_f32(const LinearParams& p, const LinearPlan& plan, cudaStream_t s);
+int linear_f16(const LinearParams& p, const LinearPlan& plan, cudaStream_t s);
+int linear_bf16(const LinearParams& p, const LinearPlan& plan, cudaStream_t s);
+
+namespace {
+
+// The rows of a block, and what it begins and ends with.
+struct Segment {
+  int64_t begin, end;                      // rows
+  int slot, number;                        // number: which segment of its list
+  int64_t at;                              // the segment's state of p.end (its list's later ones lie behind it)
+  bool last;
+};
+// false: no such segment, or one that this launch leaves out. By the first warp, the others read it off shared memory.
+__device__ __forceinline__ bool find_segment(const LinearParams& p, int u, int lane, Segment& g) {
+  int i = u;
+  int64_t b, e;
+  if (p.chunk == 0) {
+    b = p.lists.begin(i);
+    e = p.lists.begin(i + 1);
+    g.begin = b; g.end = e > b ? e : b; g.number = 0; g.last = true; g.at = 0;
+  } else {
+    i = p.lists.of_chunk(u, p.chunk, lane);
+    b = p.lists.begin(i);
+    e = p.lists.begin(i + 1);
+    if (e < b) e = b;
+    const int64_t number = u - (b / p.chunk + i);
+    if (number < 0 || (number > 0 && number * p.chunk >= e - b)) return false;
+    g.number = (int)number;
+    g.begin = b + number * p.chunk;
+    g.last = e - g.begin <= p.chunk;
+    g.end = g.last ? e : g.begin + p.chunk;
+    g.at = b / p.chunk + number;
+    if (!g.last && g.at >= p.n_ends) return false;
+  }
+  g.slot = p.lists.slot(i);
+  return !p.ends_only || !g.last;
+}
+__device__ __forceinline__ float log_decay_of(const LinearParams& p, int h) {
+  const float l = p.log_decay[h];
+  return l > 0.f ? 0.f : l;
+}
+// decay over n rows; n = 0 is 1 whatever the logarithm
+__device__ __forceinline__ float decay_over(float log_decay, int n) { return n == 0 ? 1.f : expf((float)n * log_decay); }
+// S decay + add. Near 1 the decay itself is known to 2^-25 only, which adds up over the rows that a slow one looks back on: there it is
+// S + S (decay - 1) with decay - 1 to 2^-24 of itself.
+struct Decay {
+  bool slow;
+  float by;
+  __device__ __forceinline__ explicit Decay(float log_decay) : slow(log_decay > -0.5f), by(slow ? expm1f(log_decay) : expf(log_decay)) {}
+  __device__ __forceinline__ float step(float s, float add) const { return slow ? fmaf(s, by, s + add) : fmaf(s, by, add); }
+};
+
+// What a segment's state begins with and where it goes to; null: zeros, not kept
+__device__ __forceinline__ const float* state_from(const LinearParams& p, const Segment& g, int h) {
+  const int64_t size = (int64_t)p.dk * p.dv;
+  if (g.number > 0) return p.ends_only ? nullptr : p.end + ((g.at - 1) * p.H + h) * size;
+  if (!p.h_in || g.slot < 0) return nullptr;
+  // (a split list's last segment may write over the state that its first one begins with)
+  if (!g.last && !p.ends_only) return p.first + (g.at * p.H + h) * size;
+  return p.h_in + ((int64_t)g.slot * p.H + h) * size;
+}
+__device__ __forceinline__ float* state_to(const LinearParams& p, const Segment& g, int h) {
+  const int64_t size = (int64_t)p.dk * p.dv;
+  if (p.ends_only) return p.end + (g.at * p.H + h) * size;
+  return g.last && p.h_out && g.slot >= 0 ? p.h_out + ((int64_t)g.slot * p.H + h) * size : nullptr;
+}
+
+// ---- row by row ----
+// A block has a list (or segment) and a head; a thread NV columns of dv (two where there are more than 64) and 32 of dk, PARTS lanes sharing the
+// columns, whose products with q meet in shuffles. The state stays in registers, in pairs along dk. Rows come 16 at a time through shared memory,
+// as fp32; pieces of four along dk go round the PARTS lanes, so that what a warp reads at once lies in adjacent banks.
+// Single tokens: all of the state's reads of a thread are on their way at once; bound by the states' bytes. Lists: 3 packed FMAs for two values
+// of the state a row, bound by their issue and by the broadcast reads of k and q.
+constexpr int LIN_KT = 32, LIN_ROWS = 16, LIN_MAX = 128, LIN_V = 4;
+template <typename T, int PARTS, int NV>
+__global__ void __launch_bounds__(64 * PARTS) linear_rows_kernel(const LinearParams p) {
+  pdl_wait();
+  constexpr int DK = LIN_KT * PARTS, V = LIN_V, DV = 64 * NV;
+  __shared__ Segment s_seg;
+  __shared__ int s_there;
+  __shared__ __align__(16) float s_q[LIN_ROWS][DK], s_k[LIN_ROWS][DK], s_v[LIN_ROWS][DV];
+  const int lane = threadIdx.x & 31, h = blockIdx.y, hkv = h / p.share;
+  if (threadIdx.x < 32) {
+    Segment g;
+    const bool there = find_segment(p, (int)blockIdx.x, lane, g);
+    if (lane == 0) {
+      s_seg = g;
+      s_there = there;
+    }
+  }
+  __syncthreads();
+  if (!s_there) return;
+  const Segment g = s_seg;
+  const int part = threadIdx.x % PARTS, c = threadIdx.x / PARTS * NV;
+  const bool mine = c < p.dv;
+  f32x2 S[NV][LIN_KT / 2];
+  const float* from = state_from(p, g, h);
+  auto at_dk = [&](int j) { return ((j / 4) * PARTS + part) * 4 + j % 4; };
+#pragma unroll
+  for (int j = 0; j < LIN_KT; j += 2) {
+    float x[2][NV];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const int r = at_dk(j + b);
+      const float* f = from + (int64_t)r * p.dv + c;
+#pragma unroll
+      for (int n = 0; n < NV; ++n) x[b][n] = 0.f;
+      if (from && r < p.dk && mine) {
+        if (NV == 2 && p.vec_h) {
+          const float2 t = *reinterpret_cast<const float2*>(f);
+          x[b][0] = t.x; x[b][NV - 1] = t.y;
+        } else {
+#pragma unroll
+          for (int n = 0; n < NV; ++n)
+            if (c + n < p.dv) x[b][n] = f[n];
+        }
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < NV; ++n) S[n][j / 2] = pack2(x[0][n], x[1][n]);
+  }
+  auto put_state = [&](float* to) {
+#pragma unroll
+    for (int j = 0; j < LIN_KT; j += 2) {
+      float x[2][NV];
+#pragma unroll
+      for (int n = 0; n < NV; ++n) unpack2(S[n][j / 2], x[0][n], x[1][n]);
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const int r = at_dk(j + b);
+        if (r >= p.dk || !mine) continue;
+        float* t = to + (int64_t)r * p.dv + c;
+        if (NV == 2 && p.vec_h) {
+          *reinterpret_cast<float2*>(t) = make_float2(x[b][0], x[b][NV - 1]);
+        } else {
+#pragma unroll
+          for (int n = 0; n < NV; ++n)
+            if (c + n < p.dv) t[n] = x[b][n];
+        }
+      }
+    }
+  };
+  if (from && p.ends_only) put_state(p.first + (g.at * p.H + h) * (int64_t)p.dk * p.dv);
+  const Decay decay(log_decay_of(p, h));
+  const f32x2 by = pack2(decay.by, decay.by);
+  // The next rows are read while these are worked on, where the block has the threads for it (all but narrow heads).
+  constexpr int LEAST = 32 * PARTS, PQ = LIN_ROWS * DK / V / LEAST, PV = LIN_ROWS * DV / V / LEAST;
+  const int pieces_v = (p.dv + V - 1) / V, n_threads = (int)blockDim.x;
+  const bool ahead = n_threads >= LEAST;
+  Raw<T, V> tq[PQ], tk[PQ], tv[PV];
+  auto read_qk = [&](int64_t r0, int e, Raw<T, V>& a, Raw<T, V>& b) {
+    const int r = e / (DK / V), x = e % (DK / V) * V, in = r < LIN_ROWS && r0 + r < g.end ? min(V, p.dk - x) : 0;
+    a.zero();
+    b.zero();
+    if (in <= 0) return;
+    if (!p.ends_only) a.load(p.q.get<T>(r0 + r, h) + x, in, p.vec_q);
+    b.load(p.k.get<T>(r0 + r, hkv) + x, in, p.vec_k);
+  };
+  auto put_qk = [&](int e, const Raw<T, V>& a, const Raw<T, V>& b) {
+    const int r = e / (DK / V), x = e % (DK / V) * V;
+    if (r >= LIN_ROWS) return;
+    write_floats<V>(&s_q[r][x], a.all().v);
+    write_floats<V>(&s_k[r][x], b.all().v);
+  };
+  auto read_v = [&](int64_t r0, int e, Raw<T, V>& a) {
+    const int r = e / pieces_v, x = (e - r * pieces_v) * V, in = r < LIN_ROWS && r0 + r < g.end ? min(V, p.dv - x) : 0;
+    a.zero();
+    if (in > 0) a.load(p.v.get<T>(r0 + r, hkv) + x, in, p.vec_v);
+  };
+  auto put_v = [&](int e, const Raw<T, V>& a) {
+    const int r = e / pieces_v, x = (e - r * pieces_v) * V;
+    if (r < LIN_ROWS) write_floats<V>(&s_v[r][x], a.all().v);
+  };
+  auto fetch = [&](int64_t r0) {
+#pragma unroll
+    for (int i = 0; i < PQ; ++i) read_qk(r0, threadIdx.x + i * n_threads, tq[i], tk[i]);
+#pragma unroll
+    for (int i = 0; i < PV; ++i) read_v(r0, threadIdx.x + i * n_threads, tv[i]);
+  };
+  if (ahead && g.begin < g.end) fetch(g.begin);
+  for (int64_t r0 = g.begin; r0 < g.end; r0 += LIN_ROWS) {
+    const int rows = (int)min((int64_t)LIN_ROWS, g.end - r0);
+    if (r0 > g.begin) __syncthreads();
+    if (ahead) {
+#pragma unroll
+      for (int i = 0; i < PQ; ++i) put_qk(threadIdx.x + i * n_threads, tq[i], tk[i]);
+#pragma unroll
+      for (int i = 0; i < PV; ++i) put_v(threadIdx.x + i * n_threads, tv[i]);
+    } else {
+      for (int e = threadIdx.x; e < LIN_ROWS * (DK / V); e += n_threads) {
+        Raw<T, V> a, b;
+        read_qk(r0, e, a, b);
+        put_qk(e, a, b);
+      }
+      for (int e = threadIdx.x; e < LIN_ROWS * pieces_v; e += n_threads) {
+        Raw<T, V> a;
+        read_v(r0, e, a);
+        put_v(e, a);
+      }
+    }
+    __syncthreads();
+    if (ahead && r0 + LIN_ROWS < g.end) fetch(r0 + LIN_ROWS);
+#pragma unroll 1
+    for (int r = 0; r < rows; ++r) {
+      f32x2 v2[NV], y2[NV];
+#pragma unroll
+      for (int n = 0; n < NV; ++n) {
+        const float v = mine ? s_v[r][c + n] : 0.f;
+        v2[n] = pack2(v, v);
+        y2[n] = pack2(0.f, 0.f);
+      }
+      auto move = [&](auto slow) {
+#pragma unroll
+        for (int j = 0; j < LIN_KT / 4; ++j) {
+          const ulonglong2 k4 = *reinterpret_cast<const ulonglong2*>(&s_k[r][(j * PARTS + part) * 4]);
+          const ulonglong2 q4 = *reinterpret_cast<const ulonglong2*>(&s_q[r][(j * PARTS + part) * 4]);
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            const f32x2 k2 = b ? k4.y : k4.x, q2 = b ? q4.y : q4.x;
+#pragma unroll
+            for (int n = 0; n < NV; ++n) {
+              f32x2& a = S[n][2 * j + b];
+              a = fma2(a, by, decltype(slow)::value ? fma2(k2, v2[n], a) : mul2(k2, v2[n]));
+              y2[n] = fma2(q2, a, y2[n]);
+            }
+          }
+        }
+      };
+      if (decay.slow) move(std::true_type());
+      else move(std::false_type());
+      if (p.ends_only) continue;
+      float y[2] = {0.f, 0.f};
+#pragma unroll
+      for (int n = 0; n < NV; ++n) {
+        float a, b;
+        unpack2(y2[n], a, b);
+        y[n] = a + b;
+#pragma unroll
+        for (int o = 1; o < PARTS; o *= 2) y[n] += __shfl_xor_sync(0xffffffffu, y[n], o);
+        y[n] *= p.scale;
+      }
+      if (part != 0 || !mine) continue;
+      T* to = const_cast<T*>(p.y.get<T>(r0 + r, h)) + c;
+      if (NV == 2 && p.vec_y) {
+        Raw<T, 2> out;
+        out.put_all(y);
+        out.store_piece(to);
+      } else {
+#pragma unroll
+        for (int n = 0; n < NV; ++n)
+          if (c + n < p.dv) to[n] = from_f32<T>(y[n]);
+      }
+    }
+  }
+  float* to = state_to(p, g, h);
+  if (to) put_state(to);
+}
+
+// ends[j] += decay over a segment * ends[j - 1], for all segments of a list but the first and the last. A thread has four values of a state.
+constexpr int CARRY_THREADS = 128, CARRY_AHEAD = 8;
+__global__ void __launch_bounds__(CARRY_THREADS) linear_carry_kernel(const LinearParams p) {
+  pdl_begin();
+  const int h = blockIdx.y, size = p.dk * p.dv, e = (blockIdx.x * CARRY_THREADS + threadIdx.x) * 4;
+  const float log_decay = log_decay_of(p, h);
+  const Decay decay((float)p.chunk * log_decay);
+  const bool vec = p.vec_e;
+  if (e >= size) return;
+  for (int i = blockIdx.z; i < p.lists.batch; i += gridDim.z) {
+    const int64_t b = p.lists.begin(i), rows = p.lists.begin(i + 1) - b;
+    if (rows <= 2 * p.chunk) continue;
+    const int64_t at = b / p.chunk, n = min((rows + p.chunk - 1) / p.chunk - 1, (int64_t)p.n_ends - at);      // segments whose end is kept
+    float* s = p.end + (at * p.H + h) * (int64_t)size + e;
+    const int64_t step = (int64_t)p.H * size;
+    float held[4];
+    auto get = [&](int64_t j, float (&t)[4]) {
+      if (vec) {
+        const float4 f = *reinterpret_cast<const float4*>(s + j * step);
+        t[0] = f.x; t[1] = f.y; t[2] = f.z; t[3] = f.w;
+      } else {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) t[x] = e + x < size ? s[j * step + x] : 0.f;
+      }
+    };
+    if (n < 2) continue;
+    get(0, held);
+    for (int64_t j = 1; j < n; j += CARRY_AHEAD) {
+      float t[CARRY_AHEAD][4];
+#pragma unroll
+      for (int a = 0; a < CARRY_AHEAD; ++a)
+        if (j + a < n) get(j + a, t[a]);
+#pragma unroll
+      for (int a = 0; a < CARRY_AHEAD; ++a) {
+        if (j + a >= n) break;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) held[x] = decay.step(held[x], t[a][x]);
+        if (vec) {
+          *reinterpret_cast<float4*>(s + (j + a) * step) = make_float4(held[0], held[1], held[2], held[3]);
+        } else {
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            if (e + x < size) s[(j + a) * step + x] = held[x];
+        }
+      }
+    }
+  }
+}
+
+template <typename T, int PARTS>
+void launch_linear_columns(const LinearParams& p, dim3 grid, cudaStream_t s) {
+  const int nv = p.dv <= 64 ? 1 : 2;
+  const unsigned threads = (unsigned)(((p.dv + nv - 1) / nv * PARTS + 31) / 32 * 32);
+  if (nv == 1) launch_dependent(linear_rows_kernel<T, PARTS, 1>, grid, threads, 0, s, p);
+  else launch_dependent(linear_rows_kernel<T, PARTS, 2>, grid, threads, 0, s, p);
+}
+template <typename T>
+int launch_linear_rows(const LinearParams& p, dim3 grid, cudaStream_t s) {
+  if (p.dk <= LIN_KT) launch_linear_columns<T, 1>(p, grid, s);
+  else if (p.dk <= 2 * LIN_KT) launch_linear_columns<T, 2>(p, grid, s);
+  else launch_linear_columns<T, 4>(p, grid, s);
+  return check_launch("linear_rows_kernel");
+}
+
+// The launches of a call, with `run` for the segments (or lists) of a grid
+template <typename F>
+int launch_linear_parts(LinearParams p, cudaStream_t s, F run) {
+  const int64_t units = p.chunk ? p.n_ends + (int64_t)p.lists.batch : p.lists.batch;
+  XB_REQUIRE(units < ((int64_t)1 << 31), XB_ERR_LIMIT, "xb_linear_attention: too many rows and lists");
+  const dim3 grid((unsigned)units, (unsigned)p.H);
+  if (p.chunk) {
+    p.ends_only = 1;
+    if (int rc = run(p, grid)) return rc;
+    const int quads = (p.dk * p.dv + 3) / 4;
+    launch_dependent(linear_carry_kernel, dim3((unsigned)((quads + CARRY_THREADS - 1) / CARRY_THREADS), (unsigned)p.H, (unsigned)std::min(p.lists.batch, 64)),
+                     CARRY_THREADS, 0, s, p);
+    if (int rc = check_launch("linear_carry_kernel")) return rc;
+    p.ends_only = 0;
+  }
+  return run(p, grid);
+}
+
+}  // namespace
+}  // namespace xb

@@ -23,6 +23,9 @@ struct Api {
   int (*ssm_scan)(const xb_ssm_scan_args*, void*, size_t, xb_stream_t) = nullptr;
   size_t (*lora_bytes)(const xb_lora_args*) = nullptr;
   int (*lora)(const xb_lora_args*, void*, size_t, xb_stream_t) = nullptr;
+  int (*rope)(const xb_qk_norm_rope_args*, xb_stream_t) = nullptr;
+  size_t (*linear_bytes)(const xb_linear_attention_args*) = nullptr;
+  int (*linear)(const xb_linear_attention_args*, void*, size_t, xb_stream_t) = nullptr;
 } api;
 
 struct Refused {};                         // `text` of Call holds why
@@ -31,7 +34,7 @@ struct Raised {};                          // a Python exception is set
 struct View {
   void* at = nullptr;
   int dim = 0;
-  int64_t size[3] = {0, 0, 0}, stride[3] = {0, 0, 0};
+  int64_t size[4] = {0, 0, 0, 0}, stride[4] = {0, 0, 0, 0};
   int32_t dtype = 0;
   explicit operator bool() const { return dim > 0; }
 };
@@ -65,10 +68,10 @@ struct Call {
     }
     return THPVariable_Unpack(t);
   }
-  View view(const at::Tensor& t, const char* name) {
+  View view(const at::Tensor& t, const char* name, int most = 3) {
     View v;
     v.dim = (int)t.dim();
-    if (v.dim < 1 || v.dim > 3 || t.layout() != at::kStrided) refuse("%s has 1 to 3 dimensions", name);
+    if (v.dim < 1 || v.dim > most || t.layout() != at::kStrided) refuse("%s has 1 to %d dimensions", name, most);
     for (int i = 0; i < v.dim; ++i) {
       v.size[i] = t.sizes()[i];
       v.stride[i] = t.strides()[i];
@@ -79,12 +82,21 @@ struct Call {
     return v;
   }
   // None: an empty view
-  View view(PyObject* t, const char* name) { return t == Py_None ? View() : view(tensor(t, name), name); }
+  View view(PyObject* t, const char* name, int most = 3) { return t == Py_None ? View() : view(tensor(t, name), name, most); }
   // [rows, width] of a type with adjacent columns; the row stride
   int64_t rows(const View& v, const char* name, int64_t rows, int64_t width, int32_t dtype) {
     if (v.dim != 2 || v.size[0] != rows || v.size[1] != width || v.dtype != dtype || (width > 1 && v.stride[1] != 1))
       refuse("%s is [%lld, %lld] of the call's type with adjacent columns", name, (long long)rows, (long long)width);
     return rows <= 1 && v.stride[0] < width ? width : v.stride[0];
+  }
+  // [rows, heads, width] of a type whose heads have adjacent elements; the strides of rows and heads (of one row or head any do)
+  template <typename Row>
+  void heads(const View& v, const char* name, int64_t rows, int64_t heads, int64_t width, int32_t dtype, const void** at, Row* row, Row* head) {
+    if (v.dim != 3 || v.size[0] != rows || v.size[1] != heads || v.size[2] != width || v.dtype != dtype || (width > 1 && v.stride[2] != 1))
+      refuse("%s is [%lld, %lld, %lld] of the call's type with adjacent elements", name, (long long)rows, (long long)heads, (long long)width);
+    *at = v.at;
+    *head = heads <= 1 && v.stride[1] < width ? width : v.stride[1];
+    *row = rows <= 1 ? *head * heads : v.stride[0];
   }
   void dense(const View& v, const char* name, int dim, int64_t a, int64_t b, int64_t c, int32_t dtype) {
     const int64_t want[3] = {a, b, c};
@@ -120,10 +132,37 @@ struct Call {
     if (x < 0) throw Raised();
     return x;
   }
+  // the tensor that was handed in for a result, or a new one of a shape
+  const at::Tensor& result(PyObject* given, const char* name, const at::Tensor& like, at::IntArrayRef shape, at::Tensor& own) {
+    if (given != Py_None) return tensor(given, name);
+    own = like.new_empty(shape);
+    return own;
+  }
+  void* stream(PyObject* v) {
+    void* s = PyLong_AsVoidPtr(v);
+    if (!s && PyErr_Occurred()) throw Raised();
+    return s;
+  }
+  float real(PyObject* v) {
+    const double x = PyFloat_AsDouble(v);
+    if (x == -1.0 && PyErr_Occurred()) throw Raised();
+    return (float)x;
+  }
   // lists, slots and kept states; first and last [slots, a, b]
   template <typename Args>
   void lists(Args& g, int64_t n_rows, const View& offsets, PyObject* T, const View& slots, const View& first, const View& last, int64_t a, int64_t b,
              int32_t dtype) {
+    batch(g, n_rows, offsets, T);
+    if (slots) {
+      dense(slots, "slots", 1, g.batch, 0, 0, XB_I32);
+      g.slots = static_cast<const int32_t*>(slots.at);
+    }
+    if (first) dense(first, "the array of first states", 3, -1, a, b, dtype);
+    if (last) dense(last, "the array of last states", 3, first ? first.size[0] : -1, a, b, dtype);
+    g.n_slots = first ? i32(first.size[0], "slots") : last ? i32(last.size[0], "slots") : 0;
+  }
+  template <typename Args>
+  void batch(Args& g, int64_t n_rows, const View& offsets, PyObject* T) {
     g.rows = n_rows;
     if (offsets) {
       dense(offsets, "offsets", 1, -1, 0, 0, XB_I32);
@@ -135,13 +174,6 @@ struct Call {
       if (t < 0 || (n_rows && (t < 1 || n_rows % t))) refuse("lists of %lld rows in %lld rows", (long long)t, (long long)n_rows);
       g.batch = t ? i32(n_rows / t, "lists") : 0;
     }
-    if (slots) {
-      dense(slots, "slots", 1, g.batch, 0, 0, XB_I32);
-      g.slots = static_cast<const int32_t*>(slots.at);
-    }
-    if (first) dense(first, "the array of first states", 3, -1, a, b, dtype);
-    if (last) dense(last, "the array of last states", 3, first ? first.size[0] : -1, a, b, dtype);
-    g.n_slots = first ? i32(first.size[0], "slots") : last ? i32(last.size[0], "slots") : 0;
   }
   // the scratch that was handed in, or the call's own, which outlives the launch: its memory is the stream's
   void* scratch(PyObject* given, const at::Tensor& like, size_t need, size_t* have, at::Tensor& own) {
@@ -309,6 +341,114 @@ PyObject* py_lora(PyObject*, PyObject* const* v, Py_ssize_t n) {
   });
 }
 
+// qk_norm_rope(q, k, positions, freqs, q_weight, k_weight, eps, norm, adjacent, out_q, out_k, device, stream) -> (q', k' or None)
+PyObject* py_rope(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  if (n != 13) { PyErr_SetString(PyExc_TypeError, "qk_norm_rope: 13 arguments"); return nullptr; }
+  at::Tensor of_k;
+  PyObject* first = checked_call("qk_norm_rope", v[11], [&](Call& c, at::Tensor& result) {
+    const View q = c.view(v[0], "q"), k = c.view(v[1], "k"), positions = c.view(v[2], "positions"), freqs = c.view(v[3], "freqs"),
+               wq = c.view(v[4], "q_weight"), wk = c.view(v[5], "k_weight");
+    if (q.dim != 3) c.refuse("q is [rows, heads, d]");
+    const int64_t rows = q.size[0], d = q.size[2];
+    xb_qk_norm_rope_args a;
+    memset(&a, 0, sizeof(a));
+    const void* at = nullptr;
+    at::Tensor own;
+    c.heads(q, "q", rows, q.size[1], d, q.dtype, &a.q, &a.q_row, &a.q_head);
+    result = c.result(v[9], "out_q", c.tensor(v[0], "q"), {rows, q.size[1], d}, own);
+    c.heads(c.view(result, "out_q"), "out_q", rows, q.size[1], d, q.dtype, &at, &a.yq_row, &a.yq_head);
+    a.yq = const_cast<void*>(at);
+    if (k) {
+      c.heads(k, "k", rows, k.dim == 3 ? k.size[1] : 0, d, q.dtype, &a.k, &a.k_row, &a.k_head);
+      a.Hk = c.i32(k.size[1], "heads");
+      of_k = c.result(v[10], "out_k", c.tensor(v[1], "k"), {rows, k.size[1], d}, own);
+      c.heads(c.view(of_k, "out_k"), "out_k", rows, k.size[1], d, q.dtype, &at, &a.yk_row, &a.yk_head);
+      a.yk = const_cast<void*>(at);
+    } else if (v[10] != Py_None || wk) {
+      c.refuse("out_k and k_weight need k");
+    }
+    if (positions) c.dense(positions, "positions", 1, rows, 0, 0, XB_I32);
+    if (freqs) c.dense(freqs, "freqs", 1, -1, 0, 0, XB_F32);
+    if (freqs && !positions) c.refuse("freqs need positions");
+    if (wq) c.dense(wq, "q_weight", 1, d, 0, 0, XB_F32);
+    if (wk) c.dense(wk, "k_weight", 1, d, 0, 0, XB_F32);
+    if (freqs && freqs.size[0] > d) c.refuse("%lld freqs for heads of %lld", (long long)freqs.size[0], (long long)d);
+    a.q_weight = static_cast<const float*>(wq.at); a.k_weight = static_cast<const float*>(wk.at);
+    a.positions = static_cast<const int32_t*>(positions.at); a.freqs = static_cast<const float*>(freqs.at);
+    a.rows = rows; a.Hq = c.i32(q.size[1], "heads"); a.d = c.i32(d, "d"); a.rot = freqs ? (int32_t)(2 * freqs.size[0]) : 0;
+    a.eps = c.real(v[6]); a.norm = c.flag(v[7]); a.adjacent = c.flag(v[8]); a.dtype = q.dtype;
+    void* stream = c.stream(v[12]);
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = api.rope(&a, stream);
+    Py_END_ALLOW_THREADS
+    return rc;
+  });
+  if (!first || !THPVariable_Check(first)) return first;
+  PyObject* second = Py_None;
+  if (of_k.defined()) second = THPVariable_Wrap(of_k);
+  else Py_INCREF(second);
+  if (!second) { Py_DECREF(first); return nullptr; }
+  PyObject* both = PyTuple_Pack(2, first, second);
+  Py_DECREF(first);
+  Py_DECREF(second);
+  return both;
+}
+
+// linear_attention(q, k, v, log_decay, scale, offsets, T, longest, h_in, h_out, slots, out, workspace, device, stream)
+PyObject* py_linear(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  if (n != 15) { PyErr_SetString(PyExc_TypeError, "linear_attention: 15 arguments"); return nullptr; }
+  return checked_call("linear_attention", v[13], [&](Call& c, at::Tensor& result) {
+    const View q = c.view(v[0], "q"), k = c.view(v[1], "k"), x = c.view(v[2], "v"), decay = c.view(v[3], "log_decay"), offsets = c.view(v[5], "offsets"),
+               first = c.view(v[8], "h_in", 4), last = c.view(v[9], "h_out", 4), slots = c.view(v[10], "slots");
+    if (q.dim != 3 || k.dim != 3 || x.dim != 3) c.refuse("q, k and v are [rows, heads, width]");
+    const int64_t rows = q.size[0], H = q.size[1], Hkv = k.size[1], dk = q.size[2], dv = x.size[2];
+    xb_linear_attention_args a;
+    memset(&a, 0, sizeof(a));
+    const void* at = nullptr;
+    at::Tensor own;
+    c.heads(q, "q", rows, H, dk, q.dtype, &a.q, &a.q_row, &a.q_head);
+    c.heads(k, "k", rows, Hkv, dk, q.dtype, &a.k, &a.k_row, &a.k_head);
+    c.heads(x, "v", rows, Hkv, dv, q.dtype, &a.v, &a.v_row, &a.v_head);
+    result = c.result(v[11], "out", c.tensor(v[0], "q"), {rows, H, dv}, own);
+    c.heads(c.view(result, "out"), "out", rows, H, dv, q.dtype, &at, &a.y_row, &a.y_head);
+    a.y = const_cast<void*>(at);
+    c.dense(decay, "log_decay", 1, H, 0, 0, XB_F32);
+    c.batch(a, rows, offsets, v[6]);
+    if (slots) {
+      c.dense(slots, "slots", 1, a.batch, 0, 0, XB_I32);
+      a.slots = static_cast<const int32_t*>(slots.at);
+    }
+    // (states [slots, H, dk, dv])
+    auto states = [&](const View& t, const char* name) {
+      const int64_t want[4] = {-1, H, dk, dv};
+      bool ok = t.dim == 4 && t.dtype == XB_F32;
+      int64_t step = 1;
+      for (int i = 3; ok && i >= 0; --i) {
+        ok = (want[i] < 0 || t.size[i] == want[i]) && (t.size[0] == 0 || t.size[i] <= 1 || t.stride[i] == step);
+        step *= t.size[i];
+      }
+      if (!ok) c.refuse("%s is not a contiguous fp32 [slots, %lld, %lld, %lld]", name, (long long)H, (long long)dk, (long long)dv);
+    };
+    if (first) states(first, "h_in");
+    if (last) states(last, "h_out");
+    if (first && last && first.size[0] != last.size[0]) c.refuse("h_in and h_out have different numbers of slots");
+    a.n_slots = first ? c.i32(first.size[0], "slots") : last ? c.i32(last.size[0], "slots") : 0;
+    a.log_decay = static_cast<const float*>(decay.at); a.h_in = static_cast<const float*>(first.at); a.h_out = static_cast<float*>(last.at);
+    a.longest = c.number(v[7]);
+    a.H = c.i32(H, "heads"); a.Hkv = c.i32(Hkv, "heads"); a.dk = c.i32(dk, "dk"); a.dv = c.i32(dv, "dv"); a.scale = c.real(v[4]); a.dtype = q.dtype;
+    size_t have = 0;
+    at::Tensor scratch;
+    void* ws = c.scratch(v[12], c.tensor(v[0], "q"), api.linear_bytes(&a), &have, scratch);
+    void* stream = c.stream(v[14]);
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = api.linear(&a, ws, have, stream);
+    Py_END_ALLOW_THREADS
+    return rc;
+  });
+}
+
 // bind(name, address): where a C function is
 PyObject* py_bind(PyObject*, PyObject* args) {
   const char* name = nullptr;
@@ -324,6 +464,9 @@ PyObject* py_bind(PyObject*, PyObject* args) {
   else if (!strcmp(name, "xb_ssm_scan")) api.ssm_scan = reinterpret_cast<decltype(api.ssm_scan)>(f);
   else if (!strcmp(name, "xb_lora_workspace_bytes")) api.lora_bytes = reinterpret_cast<decltype(api.lora_bytes)>(f);
   else if (!strcmp(name, "xb_lora_gemm")) api.lora = reinterpret_cast<decltype(api.lora)>(f);
+  else if (!strcmp(name, "xb_qk_norm_rope")) api.rope = reinterpret_cast<decltype(api.rope)>(f);
+  else if (!strcmp(name, "xb_linear_attention_workspace_bytes")) api.linear_bytes = reinterpret_cast<decltype(api.linear_bytes)>(f);
+  else if (!strcmp(name, "xb_linear_attention")) api.linear = reinterpret_cast<decltype(api.linear)>(f);
   else { PyErr_Format(PyExc_KeyError, "bind: %s", name); return nullptr; }
   Py_RETURN_NONE;
 }
@@ -332,6 +475,8 @@ PyMethodDef methods[] = {
     {"ssm_conv", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_ssm_conv)), METH_FASTCALL, nullptr},
     {"ssm_scan", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_ssm_scan)), METH_FASTCALL, nullptr},
     {"lora_gemm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_lora)), METH_FASTCALL, nullptr},
+    {"qk_norm_rope", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_rope)), METH_FASTCALL, nullptr},
+    {"linear_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_linear)), METH_FASTCALL, nullptr},
     {"bind", py_bind, METH_VARARGS, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "xb_tensors", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

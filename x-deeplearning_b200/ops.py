@@ -323,3 +323,24 @@ def lora_gemm(X, W, A, B, adapter, bias=None, scale=None, trans_b=False, out_dty
     X [M, K]; W [K, N], or [N, K] with trans_b; A [adapters, r, K]; B [adapters, N, r]; adapter int32 [M], outside [0, adapters) for a
     row without one; bias [N] and scale [adapters] fp32. Results in X's type or fp32."""
     return _done((_checked or _calls()).lora_gemm(X, W, A, B, adapter, bias, scale, trans_b, Y, out_dtype, workspace, *_where()))
+
+
+def qk_norm_rope(q, k, positions, freqs, q_weight=None, k_weight=None, eps=1e-6, norm=True, adjacent=False, out_q=None, out_k=None):
+    """Norms of queries and keys for each head and the rotation of their first channels by position, in one pass. Returns (q', k').
+
+    q [rows, heads, d], k [rows, key heads, d] (None: queries alone), in any strides with adjacent elements, such as slices of one
+    projection. positions int32 [rows]; freqs fp32 [turned channels / 2], the angle of one position (both None: the norm alone);
+    q_weight, k_weight fp32 [d]. `adjacent`: channels 2j and 2j + 1 are turned into one another, else j and j + half of the turned ones.
+    out_q, out_k may be q and k themselves."""
+    return _done((_checked or _calls()).qk_norm_rope(q, k, positions, freqs, q_weight, k_weight, eps, norm, adjacent, out_q, out_k, *_where()))
+
+
+def linear_attention(q, k, v, log_decay, scale=1.0, offsets=None, T=None, longest=0, h_in=None, h_out=None, slots=None, out=None, workspace=None):
+    """Linear attention with a decay for each head over lists that lie one after the other in the rows of q [rows, heads, dk]:
+    S = exp(log_decay) S + k v^T, y = scale q S.
+
+    k [rows, key heads, dk], v [rows, key heads, dv], their heads shared by as many of q's; log_decay fp32 [heads], at most 0.
+    h_in / h_out fp32 [slots, heads, dk, dv]. Lists and slots as in ssm_conv; `longest` and `workspace` as in ssm_scan. Returns
+    [rows, heads, dv]."""
+    return _done((_checked or _calls()).linear_attention(q, k, v, log_decay, scale, offsets, T, longest, h_in, h_out, slots, out, workspace,
+                                                         *_where()))
