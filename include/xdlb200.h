@@ -629,6 +629,40 @@ typedef struct xb_linear_attention_args {
 size_t xb_linear_attention_workspace_bytes(const xb_linear_attention_args* args);
 int xb_linear_attention(const xb_linear_attention_args* args, void* workspace, size_t workspace_bytes, xb_stream_t stream);
 
+/* Softmax attention of lists that share prefixes: the candidates (or branches) of a request against the behaviours that it keeps, which are read
+ * once for all of its lists, and against their own rows.
+ *   y[t, h] = sum_j w_j v_j / sum_j w_j,  w_j = exp(scale q[t, h] k_j)
+ * over all rows j of the list's prefix, and over the list's own rows up to t's place counted from the end: the last of a list's n queries sees all
+ * of its l own rows, the one before it l - 1, and so on (l = 1, n = 1: a candidate sees itself; own rows of the same number: causal order).
+ * Lists are rows of q as for xb_ssm_scan (offsets NULL: rows / batch each; what lies behind the last list is left as it was). Own rows of list i are
+ * [own_offsets[i], own_offsets[i + 1]) of k and v; own_offsets NULL: those with the numbers of its queries (own_rows = rows); no own rows: own_rows 0.
+ * Lists [members[p], members[p + 1]) have prefix p, rows [prefix_offsets[p], prefix_offsets[p + 1]) of prefix_k and prefix_v; what lies ahead of the
+ * first member and behind the last has none. members NULL: batch / prefixes lists each; prefix_offsets NULL: prefix_rows / prefixes rows each.
+ * Offsets and members ascend and are cut to what exists; where they do not, results are open, and nothing outside the arrays is touched. A query
+ * that sees no row gets zeros. Heads h of q read head h / (H / Hkv) of the keys. fp16 or bf16; d a multiple of 8, at most 128; at most 128 heads on one;
+ * rows of q, k, v, prefix_k and prefix_v on 16 bytes, their strides at least d. Scores, maxima, sums and products are fp32, the weights of a product
+ * with values rounded to the inputs' type (half a step, of a weight at most 256 times the largest). An infinity or NaN in a row reaches the queries
+ * that see it and no others. */
+typedef struct xb_prefix_attention_args {
+  const void* q; int64_t q_row, q_head;                        /* [rows, H, d] */
+  const void* k; int64_t k_row, k_head;                        /* [own_rows, Hkv, d] */
+  const void* v; int64_t v_row, v_head;
+  const void* prefix_k; int64_t prefix_k_row, prefix_k_head;   /* [prefix_rows, Hkv, d] */
+  const void* prefix_v; int64_t prefix_v_row, prefix_v_head;
+  void* y; int64_t y_row, y_head;                              /* [rows, H, d] */
+  const int32_t* offsets;                                      /* [batch + 1] */
+  const int32_t* own_offsets;                                  /* [batch + 1] */
+  const int32_t* members;                                      /* [prefixes + 1] */
+  const int32_t* prefix_offsets;                               /* [prefixes + 1] */
+  int64_t rows, own_rows, prefix_rows;
+  int32_t batch, prefixes, H, Hkv, d;
+  float scale;                                                 /* above 0 */
+  int32_t dtype;
+} xb_prefix_attention_args;
+/* Scratch of a call with these arguments: one call uses it at a time. */
+size_t xb_prefix_attention_workspace_bytes(const xb_prefix_attention_args* args);
+int xb_prefix_attention(const xb_prefix_attention_args* args, void* workspace, size_t workspace_bytes, xb_stream_t stream);
+
 /* ------------------------------------------------------------------------- */
 /* A projection shared by all rows beside a low-rank adapter of each row's own: scenes (pages, markets, tenants) whose requests
  * are stacked into one call share the weight of a layer and differ by a product of rank r.

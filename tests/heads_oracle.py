@@ -59,3 +59,39 @@ def linear(q, k, v, log_decay, scale, lists, h0, dtype):
         last.append(S)
         elast.append(E + 2.0 ** -126)
     return y, ey, last, elast
+
+
+def prefix(q, k, v, lists, own, prefixes, pk, pv, scale, dtype):
+    """q [rows, H, d]; lists, own: (first, last) of every list's queries and own rows; prefixes: (first, last) of its prefix, None: none.
+    Returns y and its bound.
+
+    A score is a sum of d products in fp32, which a matrix instruction cuts off (2^-23 of the running sum a step of 16, at most d / 16 + 1 of them); its
+    exponential turns what it is off by into as much of the weight; ex2 is right to 2^-21 and fp32 holds the exponent, as large as `e`, to 2^-23 of it.
+    Weights are rounded to the inputs' type beside values (half a step, of fp16 at least 2^-25 of the largest, since a maximum in use is not above the largest), and sums of n
+    weights or products are off by 2^-23 a step of 16, joined in order."""
+    rows, H, d = q.shape
+    share = H // (k if k is not None else pk).shape[1]
+    y, e = np.full(q.shape, np.nan), np.full(q.shape, np.nan)
+    for (r0, r1), (o0, o1), pre in zip(lists, own, prefixes):
+        n = r1 - r0
+        for r in range(r0, r1):
+            seen = max((o1 - o0) - (n - 1 - (r - r0)), 0)
+            parts = ([(pk[pre[0]:pre[1]], pv[pre[0]:pre[1]])] if pre else []) + ([(k[o0:o0 + seen], v[o0:o0 + seen])] if k is not None else [])
+            kk = np.repeat(np.concatenate([a for a, _ in parts]), share, 1) if parts else np.zeros((0, H, d))
+            vv = np.repeat(np.concatenate([b for _, b in parts]), share, 1) if parts else np.zeros((0, H, d))
+            if len(kk) == 0:
+                y[r], e[r] = 0, 0
+                continue
+            s = scale * np.einsum("hd,khd->hk", q[r], kk)
+            off = scale * np.einsum("hd,khd->hk", np.abs(q[r]), np.abs(kk)) * ((d / 16 + 4) * 2.0 ** -23) + np.abs(s) * 2.0 ** -22
+            w = np.exp(s - s.max(1, keepdims=True))
+            w /= w.sum(1, keepdims=True)
+            off_w = off + 2.0 ** -20
+            out = np.einsum("hk,khd->hd", w, vv)
+            size = np.abs(vv)
+            lost = np.einsum("hk,khd->hd", w * (off_w + HALF[dtype] * (1 + off_w)), size) + (len(kk) / 16 + 8) * 2.0 ** -23 * np.einsum("hk,khd->hd", w, size)
+            if dtype == "f16":
+                lost = lost + 2.0 ** -25 * w.max(1, keepdims=True) * size.sum(0)
+            lost = lost + np.abs(out) * (np.einsum("hk,hk->h", w, off_w)[:, None] + (len(kk) / 16 + 8) * 2.0 ** -23)
+            y[r], e[r] = out, lost + HALF[dtype] * (np.abs(out) + lost) + TINY[dtype]
+    return y, e

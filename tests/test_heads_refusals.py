@@ -67,3 +67,35 @@ def test_linear():
     assert L.xb_linear_attention(C.byref(_linear(c, **long)), AT, need - 1, None) == SCRATCH
     assert L.xb_linear_attention(C.byref(_linear(c, **long)), None, need, None) == SCRATCH
     assert L.xb_linear_attention(C.byref(_linear(c, **long)), AT + 4, need, None) == ARG
+
+
+def _prefix(c, **k):
+    a = c.PrefixAttentionArgs()
+    a.q, a.k, a.v, a.prefix_k, a.prefix_v, a.y = AT, AT, AT, AT, AT, FAR
+    a.rows, a.own_rows, a.prefix_rows, a.batch, a.prefixes, a.H, a.Hkv, a.d, a.scale, a.dtype = 12, 12, 40, 4, 2, 4, 2, 64, 0.125, c.XB_BF16
+    a.q_row, a.y_row, a.k_row, a.v_row, a.prefix_k_row, a.prefix_v_row = 256, 256, 128, 128, 128, 128
+    a.q_head = a.k_head = a.v_head = a.prefix_k_head = a.prefix_v_head = a.y_head = 64
+    return _with(a, k)
+
+
+def test_prefix():
+    m = pkg.load()
+    c, L = m.capi, m.lib()
+    assert L.xb_prefix_attention(None, None, 0, None) == ARG and L.xb_prefix_attention_workspace_bytes(None) == 0
+    for rc, k in ((UNSUPPORTED, dict(dtype=c.XB_F32)), (ARG, dict(H=0)), (ARG, dict(Hkv=3)), (ARG, dict(d=0)), (UNSUPPORTED, dict(d=60)), (LIMIT, dict(d=136)),
+                  (LIMIT, dict(H=258)), (LIMIT, dict(H=65536, Hkv=65536)), (ARG, dict(rows=-1)), (ARG, dict(prefixes=-1)), (ARG, dict(own_rows=-1)),
+                  (LIMIT, dict(batch=2**31 - 1)), (LIMIT, dict(rows=1 << 31)), (LIMIT, dict(prefix_rows=1 << 31)), (ARG, dict(scale=0.0)), (ARG, dict(scale=-1.0)),
+                  (ARG, dict(scale=float("nan"))), (ARG, dict(scale=float("inf"))), (ARG, dict(batch=5)), (ARG, dict(k=None)), (ARG, dict(v=None)),
+                  (ARG, dict(k=None, v=None)), (ARG, dict(prefix_v=None)), (ARG, dict(q=None)), (ARG, dict(y=None)), (ARG, dict(own_rows=11)), (ARG, dict(prefixes=0)),
+                  (ARG, dict(prefixes=3)), (ARG, dict(prefix_rows=41)), (UNSUPPORTED, dict(q=AT + 2)), (UNSUPPORTED, dict(prefix_k=AT + 8)),
+                  (UNSUPPORTED, dict(k_row=132)), (UNSUPPORTED, dict(v_head=63)), (UNSUPPORTED, dict(prefix_v_row=56)), (UNSUPPORTED, dict(q_head=0)),
+                  (LIMIT, dict(k_row=1 << 39)), (ARG, dict(y_row=-1))):
+        assert L.xb_prefix_attention(C.byref(_prefix(c, **k)), None, 0, None) == rc, k
+        assert b"xb_prefix_attention" in L.xb_last_error()
+        assert L.xb_prefix_attention_workspace_bytes(C.byref(_prefix(c, **k))) == 0
+    need = L.xb_prefix_attention_workspace_bytes(C.byref(_prefix(c)))
+    assert need > 0
+    for rc, k, ws, n in ((SCRATCH, {}, AT, need - 1), (SCRATCH, {}, None, need), (ARG, {}, AT + 8, need), (ARG, dict(y=AT), AT, need), (ARG, dict(y_row=255), AT, need),
+                         (ARG, dict(y_head=63), AT, need), (ARG, dict(prefix_v=FAR + 256), AT, need), (ARG, dict(k=FAR + 16 * 64), AT, need)):
+        assert L.xb_prefix_attention(C.byref(_prefix(c, **k)), ws, n, None) == rc, k
+    assert L.xb_prefix_attention(C.byref(_prefix(c, batch=0, rows=0, q=None)), None, 0, None) == 0

@@ -109,6 +109,14 @@ class LinearAttentionArgs(C.Structure):
                 ("dv", i32), ("scale", f32), ("dtype", i32)]
 
 
+class PrefixAttentionArgs(C.Structure):
+    _fields_ = [("q", vp), ("q_row", i64), ("q_head", i64), ("k", vp), ("k_row", i64), ("k_head", i64), ("v", vp), ("v_row", i64),
+                ("v_head", i64), ("prefix_k", vp), ("prefix_k_row", i64), ("prefix_k_head", i64), ("prefix_v", vp), ("prefix_v_row", i64),
+                ("prefix_v_head", i64), ("y", vp), ("y_row", i64), ("y_head", i64), ("offsets", vp), ("own_offsets", vp), ("members", vp),
+                ("prefix_offsets", vp), ("rows", i64), ("own_rows", i64), ("prefix_rows", i64), ("batch", i32), ("prefixes", i32),
+                ("H", i32), ("Hkv", i32), ("d", i32), ("scale", f32), ("dtype", i32)]
+
+
 # every symbol include/xdlb200.h declares: (restype, argtypes)
 SYMBOLS = {
     "xb_last_error": (C.c_char_p, []),
@@ -181,6 +189,8 @@ SYMBOLS = {
     "xb_qk_norm_rope": (i32, [C.POINTER(QkNormRopeArgs), vp]),
     "xb_linear_attention_workspace_bytes": (C.c_size_t, [C.POINTER(LinearAttentionArgs)]),
     "xb_linear_attention": (i32, [C.POINTER(LinearAttentionArgs), vp, C.c_size_t, vp]),
+    "xb_prefix_attention_workspace_bytes": (C.c_size_t, [C.POINTER(PrefixAttentionArgs)]),
+    "xb_prefix_attention": (i32, [C.POINTER(PrefixAttentionArgs), vp, C.c_size_t, vp]),
     "xb_dice": (i32, [vp, vp, i64, i32, vp, vp, vp, i32, i32, vp]),
     "xb_prelu": (i32, [vp, vp, i64, vp, i64, i32, i32, vp]),
     "xb_sigmoid": (i32, [vp, vp, i64, i32, vp]),
@@ -256,7 +266,8 @@ def tensors():
     if _tensors is None:
         import torch                               # (its libraries come first)
         m = _extension("xb_tensors", ("xb_ssm_conv", "xb_ssm_scan_workspace_bytes", "xb_ssm_scan", "xb_lora_workspace_bytes", "xb_lora_gemm",
-                                      "xb_qk_norm_rope", "xb_linear_attention_workspace_bytes", "xb_linear_attention"))
+                                      "xb_qk_norm_rope", "xb_linear_attention_workspace_bytes", "xb_linear_attention",
+                                      "xb_prefix_attention_workspace_bytes", "xb_prefix_attention"))
         if m.torch_version != re.match(r"\d+\.\d+\.\d+|", torch.__version__).group():        # (the headers know no more of it)
             raise RuntimeError("xb_tensors.so reads the tensors of torch %s, this is %s: build it again" % (m.torch_version, torch.__version__))
         _tensors = m

@@ -26,6 +26,8 @@ struct Api {
   int (*rope)(const xb_qk_norm_rope_args*, xb_stream_t) = nullptr;
   size_t (*linear_bytes)(const xb_linear_attention_args*) = nullptr;
   int (*linear)(const xb_linear_attention_args*, void*, size_t, xb_stream_t) = nullptr;
+  size_t (*prefix_bytes)(const xb_prefix_attention_args*) = nullptr;
+  int (*prefix)(const xb_prefix_attention_args*, void*, size_t, xb_stream_t) = nullptr;
 } api;
 
 struct Refused {};                         // `text` of Call holds why
@@ -449,6 +451,66 @@ PyObject* py_linear(PyObject*, PyObject* const* v, Py_ssize_t n) {
   });
 }
 
+// prefix_attention(q, k, v, offsets, T, own_offsets, prefix_k, prefix_v, prefix_offsets, members, scale, out, workspace, device, stream)
+PyObject* py_prefix(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  if (n != 15) { PyErr_SetString(PyExc_TypeError, "prefix_attention: 15 arguments"); return nullptr; }
+  return checked_call("prefix_attention", v[13], [&](Call& c, at::Tensor& result) {
+    const View q = c.view(v[0], "q"), k = c.view(v[1], "k"), x = c.view(v[2], "v"), offsets = c.view(v[3], "offsets"), own = c.view(v[5], "own_offsets"),
+               pk = c.view(v[6], "prefix_k"), pv = c.view(v[7], "prefix_v"), at_prefix = c.view(v[8], "prefix_offsets"), members = c.view(v[9], "members");
+    if (q.dim != 3) c.refuse("q is [rows, heads, d]");
+    if (!k != !x || !pk != !pv) c.refuse("keys and values come together");
+    if (own && !k) c.refuse("own_offsets need k and v");
+    if ((at_prefix || members) && !pk) c.refuse("prefix_offsets and members need prefix_k and prefix_v");
+    const View& keys = k ? k : pk;
+    if (keys && keys.dim != 3) c.refuse("keys and values are [rows, heads, d]");
+    const int64_t rows = q.size[0], H = q.size[1], d = q.size[2], Hkv = keys ? keys.size[1] : H;
+    xb_prefix_attention_args a;
+    memset(&a, 0, sizeof(a));
+    const void* at = nullptr;
+    at::Tensor fresh;
+    c.heads(q, "q", rows, H, d, q.dtype, &a.q, &a.q_row, &a.q_head);
+    if (k) {
+      a.own_rows = k.size[0];
+      c.heads(k, "k", a.own_rows, Hkv, d, q.dtype, &a.k, &a.k_row, &a.k_head);
+      c.heads(x, "v", a.own_rows, Hkv, d, q.dtype, &a.v, &a.v_row, &a.v_head);
+    }
+    if (pk) {
+      a.prefix_rows = pk.dim == 3 ? pk.size[0] : 0;
+      c.heads(pk, "prefix_k", a.prefix_rows, Hkv, d, q.dtype, &a.prefix_k, &a.prefix_k_row, &a.prefix_k_head);
+      c.heads(pv, "prefix_v", a.prefix_rows, Hkv, d, q.dtype, &a.prefix_v, &a.prefix_v_row, &a.prefix_v_head);
+      if (at_prefix) {
+        c.dense(at_prefix, "prefix_offsets", 1, -1, 0, 0, XB_I32);
+        if (at_prefix.size[0] < 1) c.refuse("prefix_offsets are [prefixes + 1]");
+        a.prefix_offsets = static_cast<const int32_t*>(at_prefix.at);
+      }
+      if (members) {
+        c.dense(members, "members", 1, at_prefix ? at_prefix.size[0] : -1, 0, 0, XB_I32);
+        if (members.size[0] < 1) c.refuse("members are [prefixes + 1]");
+        a.members = static_cast<const int32_t*>(members.at);
+      }
+      a.prefixes = at_prefix ? c.i32(at_prefix.size[0] - 1, "prefixes") : members ? c.i32(members.size[0] - 1, "prefixes") : 1;
+    }
+    result = c.result(v[11], "out", c.tensor(v[0], "q"), {rows, H, d}, fresh);
+    c.heads(c.view(result, "out"), "out", rows, H, d, q.dtype, &at, &a.y_row, &a.y_head);
+    a.y = const_cast<void*>(at);
+    c.batch(a, rows, offsets, v[4]);
+    if (own) {
+      c.dense(own, "own_offsets", 1, (int64_t)a.batch + 1, 0, 0, XB_I32);
+      a.own_offsets = static_cast<const int32_t*>(own.at);
+    }
+    a.H = c.i32(H, "heads"); a.Hkv = c.i32(Hkv, "heads"); a.d = c.i32(d, "d"); a.scale = c.real(v[10]); a.dtype = q.dtype;
+    size_t have = 0;
+    at::Tensor scratch;
+    void* ws = c.scratch(v[12], c.tensor(v[0], "q"), api.prefix_bytes(&a), &have, scratch);
+    void* stream = c.stream(v[14]);
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = api.prefix(&a, ws, have, stream);
+    Py_END_ALLOW_THREADS
+    return rc;
+  });
+}
+
 // bind(name, address): where a C function is
 PyObject* py_bind(PyObject*, PyObject* args) {
   const char* name = nullptr;
@@ -467,6 +529,8 @@ PyObject* py_bind(PyObject*, PyObject* args) {
   else if (!strcmp(name, "xb_qk_norm_rope")) api.rope = reinterpret_cast<decltype(api.rope)>(f);
   else if (!strcmp(name, "xb_linear_attention_workspace_bytes")) api.linear_bytes = reinterpret_cast<decltype(api.linear_bytes)>(f);
   else if (!strcmp(name, "xb_linear_attention")) api.linear = reinterpret_cast<decltype(api.linear)>(f);
+  else if (!strcmp(name, "xb_prefix_attention_workspace_bytes")) api.prefix_bytes = reinterpret_cast<decltype(api.prefix_bytes)>(f);
+  else if (!strcmp(name, "xb_prefix_attention")) api.prefix = reinterpret_cast<decltype(api.prefix)>(f);
   else { PyErr_Format(PyExc_KeyError, "bind: %s", name); return nullptr; }
   Py_RETURN_NONE;
 }
@@ -477,6 +541,7 @@ PyMethodDef methods[] = {
     {"lora_gemm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_lora)), METH_FASTCALL, nullptr},
     {"qk_norm_rope", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_rope)), METH_FASTCALL, nullptr},
     {"linear_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_linear)), METH_FASTCALL, nullptr},
+    {"prefix_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_prefix)), METH_FASTCALL, nullptr},
     {"bind", py_bind, METH_VARARGS, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "xb_tensors", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

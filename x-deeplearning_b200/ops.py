@@ -344,3 +344,16 @@ def linear_attention(q, k, v, log_decay, scale=1.0, offsets=None, T=None, longes
     [rows, heads, dv]."""
     return _done((_checked or _calls()).linear_attention(q, k, v, log_decay, scale, offsets, T, longest, h_in, h_out, slots, out, workspace,
                                                          *_where()))
+
+
+def prefix_attention(q, k=None, v=None, offsets=None, T=None, own_offsets=None, prefix_k=None, prefix_v=None, prefix_offsets=None, members=None,
+                     scale=1.0, out=None, workspace=None):
+    """Softmax attention of lists that share prefixes: every row of q [rows, heads, d] against its list's prefix and its list's own rows.
+
+    Lists of q's rows: `offsets` int32 [lists + 1], or of T rows each (T = 1: one new row a list; None: one list). k, v [own rows, key heads,
+    d]: list i's own rows are [own_offsets[i], own_offsets[i + 1]), or without own_offsets those with its queries' numbers; its last query sees
+    all of them, the one before it one less. prefix_k, prefix_v [prefix rows, key heads, d]: prefix p is [prefix_offsets[p],
+    prefix_offsets[p + 1]), shared by lists [members[p], members[p + 1]) (None: by as many lists each; both None: one prefix for all).
+    fp16 or bf16. Returns [rows, heads, d], zeros for a row that sees nothing; rows behind the last list are not written."""
+    return _done((_checked or _calls()).prefix_attention(q, k, v, offsets, T, own_offsets, prefix_k, prefix_v, prefix_offsets, members, scale,
+                                                         out, workspace, *_where()))
