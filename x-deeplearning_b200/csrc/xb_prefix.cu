@@ -11,20 +11,25 @@ constexpr int PFX_MAX_D = 128;
 constexpr float LOG2_E = 1.4426950408889634f;
 
 struct PrefixScratch {
-  size_t ends, first_tile, part, part_ml, bytes;      // (the tiles lie first)
-  int max_tiles, ctas;
+  size_t own_weight, groups, begins, records, part, part_ml, bytes;      // (the items lie first)
+  int max_items, ctas, part_rows, n_groups;
 };
 PrefixScratch prefix_scratch(const xb_prefix_attention_args& a) {
   auto align256 = [](size_t n) { return (n + 255) / 256 * 256; };
   PrefixScratch w;
-  const int64_t share = a.H / a.Hkv, R = PFX_ROWS / share, groups = (int64_t)a.prefixes + 2;
-  w.ctas = std::max(sm_count(), 1);
-  w.max_tiles = (int)(a.rows / R + std::min<int64_t>(a.rows, groups));
-  w.ends = align256((size_t)w.max_tiles * sizeof(PrefixTile));
-  w.first_tile = w.ends + align256(((size_t)w.max_tiles + 1) * 8);
-  w.part = w.first_tile + align256(((size_t)groups + 1) * 4);
-  w.part_ml = w.part + align256((size_t)w.ctas * 2 * PFX_ROWS * a.d * 4);
-  w.bytes = w.part_ml + align256((size_t)w.ctas * 2 * PFX_ROWS * 8);
+  const int64_t share = a.H / a.Hkv, R = PFX_ROWS / share;
+  w.ctas = std::min(std::max(sm_count(), 1), JOIN_MOST / PFX_SLOTS);
+  w.n_groups = a.prefixes == 0 ? 1 : a.prefixes + 2;
+  w.max_items = (int)(a.rows / (2 * R) + std::min<int64_t>(a.rows, w.n_groups));
+  w.part_rows = (int)std::min<int64_t>(2 * R, a.rows) * (int)share;
+  const size_t slots = (size_t)w.ctas * PFX_SLOTS;
+  w.own_weight = align256((size_t)w.max_items * sizeof(PrefixItem));
+  w.groups = w.own_weight + align256(((size_t)w.max_items + 1) * 8);
+  w.begins = w.groups + align256(((size_t)w.n_groups + 1) * sizeof(PrefixGroup));
+  w.records = w.begins + align256(((size_t)w.ctas + 1) * sizeof(PrefixAt));
+  w.part = w.records + align256(slots * sizeof(PrefixRecord));
+  w.part_ml = w.part + align256(slots * w.part_rows * a.d * 4);
+  w.bytes = w.part_ml + align256(slots * w.part_rows * 8);
   return w;
 }
 
@@ -87,12 +92,13 @@ template <bool BF16, int DP>
 int launch_prefix(const CUtensorMap (&m)[5], const PrefixParams& p, cudaStream_t s) {
   static PerDeviceOnce once;
   XB_SET_MAX_SMEM_ONCE(once, PrefixShape<DP>::SMEM, (const void*)prefix_attention_kernel<BF16, DP>);
-  launch_dependent(prefix_plan_kernel, 1, PLAN_THREADS, 0, s, p);
+  // (a thread a group, an item and a CTA, while there are threads)
+  const int want = std::max({p.n_groups, p.max_items, p.ctas + 1});
+  launch_dependent(prefix_plan_kernel, 1, (unsigned)std::min((want + 31) / 32 * 32, PLAN_THREADS), 0, s, p);
   if (int rc = check_launch("prefix_plan_kernel")) return rc;
   launch_dependent(prefix_attention_kernel<BF16, DP>, (unsigned)p.ctas, PFX_THREADS, PrefixShape<DP>::SMEM, s, m[0], m[1], m[2], m[3], m[4], p);
   if (int rc = check_launch("prefix_attention_kernel")) return rc;
-  if (p.ctas < 2) return 0;
-  launch_dependent(prefix_join_kernel<BF16>, dim3((unsigned)p.ctas - 1, 8), JOIN_THREADS, 0, s, p);
+  launch_dependent(prefix_join_kernel<BF16>, (unsigned)p.ctas * 4, JOIN_THREADS, 0, s, p);
   return check_launch("prefix_join_kernel");
 }
 
@@ -135,12 +141,14 @@ extern "C" int xb_prefix_attention(const xb_prefix_attention_args* a, void* work
   p.y = y; p.v = v;
   p.vec_y = heads_whole(y, 2, 16);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  p.tiles = reinterpret_cast<PrefixTile*>(ws);
-  p.ends = reinterpret_cast<int64_t*>(ws + w.ends);
-  p.first_tile = reinterpret_cast<int*>(ws + w.first_tile);
-  p.part = reinterpret_cast<float*>(ws + w.part);
+  p.items = reinterpret_cast<PrefixItem*>(ws);
+  p.own_weight = reinterpret_cast<int64_t*>(ws + w.own_weight);
+  p.groups = reinterpret_cast<PrefixGroup*>(ws + w.groups);
+  p.begins = reinterpret_cast<PrefixAt*>(ws + w.begins);
+  p.records = reinterpret_cast<PrefixRecord*>(ws + w.records);
+  p.part = reinterpret_cast<float4*>(ws + w.part);
   p.part_ml = reinterpret_cast<float2*>(ws + w.part_ml);
-  p.max_tiles = w.max_tiles; p.ctas = w.ctas;
+  p.max_items = w.max_items; p.ctas = w.ctas; p.n_groups = w.n_groups; p.part_rows = w.part_rows;
   CUtensorMap m[5];
   if (int rc = make_heads_map(&m[0], a->dtype, a->q, a->q_row, a->q_head, a->rows, a->H, p.share, a->d, p.R)) return rc;
   // (a map that no block of keys is read by is that of the queries)

@@ -1,16 +1,19 @@
 // Softmax attention of lists that share a prefix, on the 5th-generation tensor cores (formulas in xdlb200.h).
 //
-// A tile is 128 rows of scores: R = 128 / share query rows of one prefix's lists, with the `share` heads that read one head of keys side by side.
-// It meets the keys of its prefix, and those of its lists' own that lie between the first that its first row sees and the last that its last row
-// does, 128 at a time; a row's own keys are one interval, so that lists and the order in a list are one comparison with two ends. The prefix is
-// read once for all rows of a tile, whatever lists they are of.
-// An item is a tile and a head of keys, a unit one block of keys of an item. The units of all items lie in one line that is cut into equal parts,
-// one a CTA; a part that ends inside an item leaves its sums (fp32, with the running maximum and sum) in the workspace, and a last kernel joins
-// them in order. prefix_plan_kernel lays the line out from the offsets, which only the device knows.
+// An item is one or two tiles of 128 rows of scores (R = 128 / share query rows of one prefix's lists, with the `share` heads that read one head of
+// keys side by side) and that head of keys. It meets the keys of its prefix, and those of its lists' own that lie between the first that its first
+// row sees and the last that its last row does, in blocks of 128 (units). A row's own keys are one interval, so that lists and the order in a list
+// are one comparison with two ends. The prefix is read once for all rows of an item, whatever lists they are of.
 //
-// In a CTA one warp loads (TMA), one issues the MMAs, and two groups of four warps take the blocks of keys in turn, each with scores, weights and
-// sums of its own in tensor memory: while one makes weights of its scores, the tensor cores are at the other's. A thread has a row; a maximum
-// that has not grown by more than 2^8 leaves the sums as they are (weights up to 256 fit both types), so that they are seldom moved.
+// prefix_plan_kernel puts the units of all items in a line, from the offsets that only the device knows, and cuts it into equal parts, one a CTA.
+// Where the items of a prefix are longer than a part, they lie side by side in chunks of a part's length: CTAs that run at the same time then read
+// the same keys, which come from memory once. (512 rows of 4 heads on 100003 keys, one item after another: 4 times the bytes.) What a CTA has of an
+// item that is not whole goes to the workspace as sums in fp32 with their running maximum, and a last kernel joins those in order.
+//
+// In a CTA one warp loads (TMA), and and two groups of four warps, each with a warp that issues its MMAs, have scores, weights and sums of their own in
+// tensor memory: one tile each of an item of two, whose keys they share, or of a single tile every other block of keys. While one makes weights of
+// its scores, the tensor cores are at the other's. A thread has a row; a maximum that has not grown by more than 2^8 leaves the sums as they are
+// (weights up to 256 fit both types), so that they are seldom moved.
 #pragma once
 
 #include <algorithm>
@@ -21,16 +24,26 @@
 namespace xb {
 namespace {
 
-constexpr int PFX_KEYS = 128, PFX_ROWS = 128, PFX_THREADS = 320, PFX_LOADER = 8, PFX_MMA = 9;
+constexpr int PFX_KEYS = 128, PFX_ROWS = 128, PFX_THREADS = 384, PFX_LOADER = 8, PFX_MMA = 9, PFX_SLOTS = 4;
 constexpr float PFX_GROWTH = 8.f;
 
-struct PrefixTile {
+struct PrefixItem {
   int row0, rows;                          // query rows
   int prefix0, prefix_n;
-  int own0, own_n;                         // the own keys that any of its rows sees
-  int own_full;                            // the first of them that all of its rows see
-  int list0, list1;                        // its first row's list, and its last row's
-  int units;
+  int own0, own_n;                         // the own keys that any of its rows sees; from here on counted from the first of them
+  int end0, begin1;                        // where those of the first tile's rows end and those of the second's begin
+  int full0, full1;                        // up to where all rows of a tile see them, if its rows are of one list (else 0)
+  int list[4];                             // the lists of the first and the last row of either tile
+};
+struct PrefixGroup {                       // the lists of a prefix
+  int64_t weight;                          // units of tiles ahead of it (for one head of keys)
+  int first, blocks, chunks, tiles;        // its first item; blocks of its prefix's keys, and the chunks that they go by; tiles of its items
+};
+struct PrefixAt {                          // a place in the line: group, head of keys, chunk, item, block of keys
+  int group, head, chunk, item, unit;
+};
+struct PrefixRecord {                      // sums in the workspace: of which item and head, from which block of keys on (item -1: none)
+  int item, head, unit, pad;
 };
 struct PrefixParams {
   Lists lists, own;                        // rows of q; rows of k and v
@@ -42,14 +55,15 @@ struct PrefixParams {
   Heads y, v;
   int vec_y;
   // workspace
-  PrefixTile* tiles;
-  int64_t* ends;                           // [tiles + 1]: units before a tile (of one head)
-  int* first_tile;                         // [groups + 1]
-  float* part;                             // [2 CTAs][128][d]
-  float2* part_ml;                         // [2 CTAs][128]
-  int max_tiles, ctas;
+  PrefixItem* items;
+  int64_t* own_weight;                     // [items + 1]: units of tiles of own keys ahead of an item
+  PrefixGroup* groups;                     // [groups + 1]
+  PrefixAt* begins;                        // [CTAs + 1]
+  PrefixRecord* records;                   // [CTAs][PFX_SLOTS]
+  float4* part;                            // [CTAs][PFX_SLOTS][d / 4][part_rows]: the rows' pieces of four side by side
+  float2* part_ml;                         // [CTAs][PFX_SLOTS][part_rows]
+  int max_items, ctas, n_groups, part_rows;
 };
-
 // ---- the plan ----
 // Lists of group g: those ahead of the first member (no prefix), of prefix g - 1, and those behind the last member (no prefix).
 __device__ __forceinline__ int group_begin(const PrefixParams& p, int g) {
@@ -77,10 +91,10 @@ __device__ __forceinline__ int list_of(const Lists& l, int64_t row, int lo, int 
 // the own keys that a row sees: a list's last row sees all of them, each row before it one less
 __device__ __forceinline__ void own_of(const PrefixParams& p, int64_t row, int list, int64_t& lo, int64_t& hi) {
   lo = p.own.begin(list);
-  hi = p.own.begin(list + 1) - (p.lists.begin(list + 1) - 1 - row);
+  hi = p.own.begin(list + 1) - max(p.lists.begin(list + 1) - 1 - row, (int64_t)0);
   if (hi < lo) hi = lo;
 }
-template <int WARPS>
+constexpr int PLAN_THREADS = 1024, PLAN_GROUPS = 1024, PLAN_ITEMS = 2048;      // (what shared memory holds of a plan; larger ones are in the workspace alone)
 __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* s_sums, int64_t& total) {      // exclusive
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int64_t x = v;
@@ -89,118 +103,217 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* s_sums, int64_
     const int64_t t = __shfl_up_sync(0xffffffffu, x, o);
     if (lane >= o) x += t;
   }
-  __syncthreads();
+  __syncthreads();                         // (what stands there of the scan before has been read)
   if (lane == 31) s_sums[warp] = x;
   __syncthreads();
-  int64_t before = 0;
-  total = 0;
-  for (int w = 0; w < WARPS; ++w) {
-    if (w < warp) before += s_sums[w];
-    total += s_sums[w];
+  int64_t sums = lane < (int)blockDim.x / 32 ? s_sums[lane] : 0;
+#pragma unroll
+  for (int o = 1; o < 32; o *= 2) {
+    const int64_t t = __shfl_up_sync(0xffffffffu, sums, o);
+    if (lane >= o) sums += t;
   }
-  return before + x - v;
+  total = __shfl_sync(0xffffffffu, sums, 31);
+  const int64_t before = __shfl_sync(0xffffffffu, sums, (warp + 31) & 31);
+  return (warp > 0 ? before : 0) + x - v;
 }
-constexpr int PLAN_THREADS = 1024;
+
+// Chunk c of a prefix's blocks begins at c blocks / chunks. All items of a group and a head of keys, in the line: for every chunk but the last its
+// blocks of item after item, then item after item the last chunk's with the own keys behind them. A block of an item of two tiles counts twice.
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {      // (of numbers that are not negative; 64-bit division takes 100 instructions)
+  return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
+}
+__device__ __forceinline__ int chunk_begin(const PrefixGroup& g, int c) { return g.chunks == 1 ? c * g.blocks : (int)quotient((int64_t)c * g.blocks, g.chunks); }
+__device__ __forceinline__ int item_blocks(const PrefixItem& x, int prefix_blocks) {
+  return max(prefix_blocks + (x.own_n + PFX_KEYS - 1) / PFX_KEYS, 1);        // (an item without keys is one block, for its rows' zeros)
+}
+__device__ __forceinline__ PrefixAt line_place(const PrefixParams& p, const PrefixGroup* groups, const int64_t* own_weight, int64_t x, int64_t all, int ctas) {
+  int lo = 0, hi = p.n_groups - 1;
+  while (lo < hi) {                        // the last group that begins at x or ahead of it
+    const int mid = lo + (hi - lo + 1) / 2;
+    if (groups[mid].weight * p.Hkv <= x) lo = mid;
+    else hi = mid - 1;
+  }
+  const PrefixGroup g = groups[lo];
+  const int n = groups[lo + 1].first - g.first;
+  const int64_t weight = groups[lo + 1].weight - g.weight;
+  PrefixAt at;
+  at.group = lo;
+  at.head = (int)quotient(x - g.weight * p.Hkv, weight);
+  int64_t r = x - g.weight * p.Hkv - at.head * weight;
+  const int last = chunk_begin(g, g.chunks - 1);
+  if (r < (int64_t)g.tiles * last) {
+    const int u = (int)quotient(r, g.tiles);
+    int c = (int)quotient((int64_t)u * g.chunks, g.blocks);
+    while (chunk_begin(g, c + 1) <= u) ++c;
+    const int b = chunk_begin(g, c), len = chunk_begin(g, c + 1) - b;
+    r -= (int64_t)g.tiles * b;
+    const int i = (int)min(quotient(r, 2 * len), (int64_t)n - 1), w = i == n - 1 ? g.tiles - 2 * i : 2;
+    at.chunk = c; at.item = g.first + i; at.unit = b + (int)(w == 2 ? (r - (int64_t)i * 2 * len) >> 1 : r - (int64_t)i * 2 * len);
+    return at;
+  }
+  r -= (int64_t)g.tiles * last;
+  const int rem = g.blocks - last;
+  const int64_t own = own_weight[g.first];
+  lo = 0;
+  hi = n - 1;
+  while (lo < hi) {
+    const int mid = lo + (hi - lo + 1) / 2;
+    if ((int64_t)mid * 2 * rem + own_weight[g.first + mid] - own <= r) lo = mid;
+    else hi = mid - 1;
+  }
+  r -= (int64_t)lo * 2 * rem + own_weight[g.first + lo] - own;
+  const int w = lo == n - 1 ? g.tiles - 2 * lo : 2;
+  at.chunk = g.chunks - 1; at.item = g.first + lo; at.unit = last + (int)(w == 2 ? r >> 1 : r);
+  // small items stay whole: what a cut saves is less than joining costs
+  if (g.chunks == 1 && at.unit > 0) {
+    const int blocks = g.blocks + (int)((own_weight[at.item + 1] - own_weight[at.item]) >> (w - 1));
+    if ((int64_t)blocks * w * ctas * 4 <= all) {
+      if (2 * at.unit >= blocks) {
+        if (lo + 1 < n) {
+          ++at.item;
+        } else {
+          at.item = g.first;
+          if (++at.head == p.Hkv) {
+            at.head = 0;
+            ++at.group;
+            while (at.group < p.n_groups && groups[at.group + 1].first == groups[at.group].first) ++at.group;      // (groups without rows)
+            at.chunk = 0;
+            at.item = at.group < p.n_groups ? groups[at.group].first : 0;
+          }
+        }
+      }
+      at.unit = 0;
+    }
+  }
+  return at;
+}
+
+// One block: three sums over groups and items and a search a CTA, each behind a read or two from memory. 74 requests of 1000 candidates: 11 us with the
+// sums in the workspace, whose every read takes 0.4 us.
 __global__ void __launch_bounds__(PLAN_THREADS) prefix_plan_kernel(const PrefixParams p) {
   pdl_begin();
-  __shared__ int64_t s_sums[PLAN_THREADS / 32];
-  const int groups = p.prefixes == 0 ? 1 : p.prefixes + 2;
+  __shared__ int64_t s_sums[PLAN_THREADS / 32], s_own[PLAN_ITEMS + 1];
+  __shared__ PrefixGroup s_groups[PLAN_GROUPS + 1];
+  const int threads = blockDim.x, n_groups = p.n_groups, step = 2 * p.R;
+  PrefixGroup* groups = n_groups <= PLAN_GROUPS ? s_groups : p.groups;
   int64_t total = 0, sum;
-  for (int g0 = 0; g0 < groups; g0 += PLAN_THREADS) {
+  for (int g0 = 0; g0 < n_groups; g0 += threads) {
     const int g = g0 + (int)threadIdx.x;
+    PrefixGroup x = {};
     int64_t n = 0;
-    if (g < groups) {
+    if (g < n_groups) {
       const int64_t rows = p.lists.begin(group_begin(p, g + 1)) - p.lists.begin(group_begin(p, g));
-      n = rows > 0 ? (rows + p.R - 1) / p.R : 0;
+      n = rows > 0 ? (rows + step - 1) / step : 0;
+      x.tiles = rows > 0 ? (int)((rows + p.R - 1) / p.R) : 0;
+      if (g > 0 && g <= p.prefixes) x.blocks = (int)((max(prefix_begin(p, g) - prefix_begin(p, g - 1), (int64_t)0) + PFX_KEYS - 1) / PFX_KEYS);
     }
-    const int64_t at = total + block_scan<PLAN_THREADS / 32>(n, s_sums, sum);
-    if (g < groups) p.first_tile[g] = (int)min(at, (int64_t)p.max_tiles);
+    const int64_t at = total + block_scan(n, s_sums, sum);
+    x.first = (int)min(at, (int64_t)p.max_items);
+    if (g < n_groups) groups[g] = x;
     total += sum;
   }
-  const int tiles = (int)min(total, (int64_t)p.max_tiles);
-  if (threadIdx.x == 0) p.first_tile[groups] = tiles;
+  const int items = (int)min(total, (int64_t)p.max_items);
+  int64_t* own_weight = items <= PLAN_ITEMS ? s_own : p.own_weight;
+  if (threadIdx.x == 0) {
+    const PrefixGroup x = {0, items, 0, 1, 0};
+    groups[n_groups] = x;
+  }
   __syncthreads();
-  int64_t units = 0;
-  for (int t0 = 0; t0 < tiles; t0 += PLAN_THREADS) {
+  int64_t own_total = 0;
+  for (int t0 = 0; t0 < items; t0 += threads) {
     const int t = t0 + (int)threadIdx.x;
-    PrefixTile x = {};
-    if (t < tiles) {
-      int lo = 0, hi = groups - 1;                        // the group: the last that begins at the tile or ahead of it
+    int64_t weight = 0;
+    if (t < items) {
+      int lo = 0, hi = n_groups - 1;                      // the group: the last that begins at the item or ahead of it
       while (lo < hi) {
         const int mid = lo + (hi - lo + 1) / 2;
-        if (p.first_tile[mid] <= t) lo = mid;
+        if (groups[mid].first <= t) lo = mid;
         else hi = mid - 1;
       }
-      const int l0 = group_begin(p, lo), l1 = group_begin(p, lo + 1);
-      const int64_t begin = p.lists.begin(l0) + (int64_t)(t - p.first_tile[lo]) * p.R, end = min(begin + p.R, p.lists.begin(l1));
-      x.row0 = (int)begin; x.rows = (int)max(end - begin, (int64_t)0);
+      PrefixItem x = {};
+      const int l0 = group_begin(p, lo), l1 = max(group_begin(p, lo + 1) - 1, l0);
+      const int64_t begin = p.lists.begin(l0) + (int64_t)(t - groups[lo].first) * step;
+      const int64_t end = max(min(begin + step, p.lists.begin(l1 + 1)), begin + 1), mid = min(begin + p.R, end);
+      x.row0 = (int)begin; x.rows = (int)(end - begin);
       if (lo > 0 && lo <= p.prefixes) {
         const int64_t a = prefix_begin(p, lo - 1), b = prefix_begin(p, lo);
         x.prefix0 = (int)a; x.prefix_n = (int)max(b - a, (int64_t)0);
       }
-      x.list0 = list_of(p.lists, begin, l0, max(l1 - 1, l0));
-      x.list1 = list_of(p.lists, max(end - 1, begin), x.list0, max(l1 - 1, l0));
+      x.list[0] = list_of(p.lists, begin, l0, l1);
+      x.list[1] = list_of(p.lists, mid - 1, x.list[0], l1);
+      x.list[2] = mid < end ? list_of(p.lists, mid, x.list[1], l1) : x.list[1];
+      x.list[3] = mid < end ? list_of(p.lists, end - 1, x.list[2], l1) : x.list[1];
       if (p.own.rows > 0) {
-        int64_t a, b, c, e;
-        own_of(p, begin, x.list0, a, b);
-        own_of(p, max(end - 1, begin), x.list1, c, e);
-        x.own0 = (int)a; x.own_n = (int)max(e - a, (int64_t)0);
-        x.own_full = x.list0 == x.list1 ? (int)(b - a) : 0;
+        // (first and last row of either tile: where their own keys begin and end)
+        int64_t b0, e0, b1, e1, b2, e2, b3, e3;
+        own_of(p, begin, x.list[0], b0, e0);
+        own_of(p, mid - 1, x.list[1], b1, e1);
+        b2 = b1; e2 = e1; b3 = b1; e3 = e1;
+        if (mid < end) {
+          own_of(p, mid, x.list[2], b2, e2);
+          own_of(p, end - 1, x.list[3], b3, e3);
+        }
+        const int64_t n = max(e3 - b0, (int64_t)0);
+        auto in = [&](int64_t k) { return (int)min(max(k - b0, (int64_t)0), n); };
+        x.own0 = (int)b0; x.own_n = (int)n; x.end0 = in(e1); x.begin1 = mid < end ? in(b2) : 0;
+        x.full0 = x.list[0] == x.list[1] ? in(e0) : 0;
+        x.full1 = x.list[2] == x.list[3] ? in(e2) : 0;
       }
-      x.units = max((x.prefix_n + PFX_KEYS - 1) / PFX_KEYS + (x.own_n + PFX_KEYS - 1) / PFX_KEYS, 1);
-      p.tiles[t] = x;
+      p.items[t] = x;
+      const int blocks = (x.prefix_n + PFX_KEYS - 1) / PFX_KEYS;
+      weight = (int64_t)(item_blocks(x, blocks) - blocks) * (mid < end ? 2 : 1);
     }
-    const int64_t at = units + block_scan<PLAN_THREADS / 32>(x.units, s_sums, sum);
-    if (t < tiles) p.ends[t] = at;
-    units += sum;
+    const int64_t at = own_total + block_scan(weight, s_sums, sum);
+    if (t < items) own_weight[t] = at;
+    own_total += sum;
   }
-  if (threadIdx.x == 0) p.ends[tiles] = units;
-}
-
-// Where a CTA's part of the line begins: tile, head of keys, block of keys.
-struct PrefixAt {
-  int tile, head, unit;
-};
-__device__ __forceinline__ PrefixAt part_begin(const PrefixParams& p, int tiles, int64_t all, int cta, int ctas) {
-  PrefixAt at = {tiles, 0, 0};
-  if (cta >= ctas) return at;
-  const int64_t x = all * cta / ctas;
-  int lo = 0, hi = tiles - 1;
-  while (lo < hi) {
-    const int mid = lo + (hi - lo + 1) / 2;
-    if (p.ends[mid] * p.Hkv <= x) lo = mid;
-    else hi = mid - 1;
+  if (threadIdx.x == 0) own_weight[items] = own_total;
+  __syncthreads();
+  int64_t all = 0;
+  for (int g0 = 0; g0 < n_groups; g0 += threads) {
+    const int g = g0 + (int)threadIdx.x;
+    int64_t weight = 0;
+    if (g < n_groups) weight = (int64_t)groups[g].tiles * groups[g].blocks + own_weight[groups[g + 1].first] - own_weight[groups[g].first];
+    const int64_t at = all + block_scan(weight, s_sums, sum);
+    if (g < n_groups) groups[g].weight = at;
+    all += sum;
   }
-  const int64_t units = p.ends[lo + 1] - p.ends[lo], in = x - p.ends[lo] * p.Hkv;
-  at.tile = lo; at.head = (int)(in / units); at.unit = (int)(in % units);
-  // small items stay whole: what a cut saves is less than joining costs
-  if (units * ctas * 4 <= all && at.unit > 0) {
-    if (2 * at.unit >= units && ++at.head == p.Hkv) {
-      at.head = 0;
-      ++at.tile;
-    }
-    at.unit = 0;
+  if (threadIdx.x == 0) groups[n_groups].weight = all;
+  all *= p.Hkv;
+  const int ctas = (int)min(all, (int64_t)p.ctas);
+  for (int g = threadIdx.x; g < n_groups; g += threads) {
+    // (several items, each longer than a part: as many chunks as parts of an item)
+    const int64_t chunks = groups[g].tiles > 2 && all > 0 ? quotient(2 * (int64_t)groups[g].blocks * ctas, all) : 1;
+    groups[g].chunks = (int)max(min(chunks, (int64_t)groups[g].blocks), (int64_t)1);
   }
-  return at;
+  __syncthreads();
+  for (int c = threadIdx.x; c <= p.ctas; c += threads) {
+    PrefixAt at = {n_groups, 0, 0, 0, 0};
+    if (c < ctas) at = line_place(p, groups, own_weight, quotient(all * c, ctas), all, ctas);
+    p.begins[c] = at;
+  }
+  if (groups == s_groups)
+    for (int g = threadIdx.x; g <= n_groups; g += threads) p.groups[g] = s_groups[g];
 }
 
 // ---- the kernel ----
 template <int DP>
 struct PrefixShape {
-  static constexpr int Q = 2, K = DP == 128 ? 3 : 5, V = DP == 128 ? 2 : 5;                     // buffers
+  static constexpr int Q = DP == 128 ? 1 : 2, K = DP == 128 ? 3 : 5, V = DP == 128 ? 2 : 5;     // buffers (of queries: an item's)
   static constexpr int TILE = 128 * DP * 2, BOX = 128 * 128;
   struct Control {                         // behind the buffers (the kernel has no other shared memory, so that its buffers begin on 1024 bytes)
     uint64_t q_full[Q], q_empty[Q], k_full[K], k_empty[K], v_full[V], v_empty[V];
-    uint64_t s_full[2], p_ready[2], o_done[2], o_free, met, drained;
+    uint64_t s_full[2], s_read[2], p_ready[2], o_done[2], o_free[2], met, drained[2];
     float2 ml[2][PFX_ROWS];                // maximum and sum of either group's rows
-    PrefixAt part[2];
-    int bad[2];
+    int bad[2], lock;
     uint32_t tmem;
   };
-  static constexpr int SMEM = (Q + K + V) * TILE + (int)sizeof(Control);
+  static constexpr int SMEM = (2 * Q + K + V) * TILE + (int)sizeof(Control);
   static_assert(SMEM <= 227 * 1024, "");
-  // columns of tensor memory: the scores of both groups, their sums; weights where there is room, else over the scores that they are made of
-  static constexpr uint32_t S = 0, O = 256, P = DP == 128 ? 0 : 384, P_STEP = DP == 128 ? 128 : 64;
+  // Columns of tensor memory: the scores of both groups, their sums; weights where there is room, else over the scores that they are made of
+  // (whose next ones then wait for the weights' product).
+  static constexpr bool APART = DP == 64;
+  static constexpr uint32_t S = 0, O = 256, P = APART ? 384 : 0, P_STEP = APART ? 64 : 128;
 };
 
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2, int c3) {
@@ -208,6 +321,44 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
                "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
                : "memory");
 }
+// mbar_wait whose tries go one after the other: what waits here is woken many times a microsecond, and there is no other warp to give way to
+__device__ __forceinline__ bool mbar_spin(uint32_t bar, uint32_t parity, int site) {
+  using namespace umma;
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long t0 = clock64(), limit = wait_limit();
+  while (!mbar_try_wait(bar, parity)) {
+    if (clock64() - t0 > limit) {
+      wait_gave_up(site);
+      return false;
+    }
+  }
+  return true;
+}
+__device__ __forceinline__ void mbar_arrive_twice(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], 2;" ::"r"(bar) : "memory"); }
+// A lock between two warps, held for the time of a few instructions. False: it was not to be had (with the limit of the waits).
+__device__ __forceinline__ bool take(int* lock, int lane) {
+  int ok = 1;
+  if (lane == 0) {
+    const long long t0 = clock64(), limit = umma::wait_limit();
+    while (atomicCAS(lock, 0, 1) != 0)
+      if (clock64() - t0 > limit) {
+        umma::wait_gave_up(99);
+        ok = 0;
+        break;
+      }
+  }
+  return __shfl_sync(0xffffffffu, ok, 0) != 0;
+}
+__device__ __forceinline__ void let_go(int* lock, int lane) {
+  __syncwarp();
+  if (lane == 0) atomicExch(lock, 0);
+  __syncwarp();
+}
+// shares of a launch's registers: every warp of four that begin at a multiple of four
+template <int N>
+__device__ __forceinline__ void registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack_weights(float lo, float hi) {
   uint32_t r;
@@ -222,32 +373,78 @@ __device__ __forceinline__ bool half_is_bad(uint32_t h) {
   return (h & E) == E;
 }
 
+// A value that all lanes have, told to the compiler as such: what the MMAs take then stands in uniform registers.
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
+// sum + 0 * t, two halves: NaN once a t was infinite or NaN
+template <bool BF16>
+__device__ __forceinline__ uint32_t fma_zero(uint32_t t, uint32_t sum) {
+  uint32_t r;
+  if constexpr (BF16) asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(t), "r"(0u), "r"(sum));
+  else asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(t), "r"(0u), "r"(sum));
+  return r;
+}
+// the lowest n bits, n cut to [0, 32]
+__device__ __forceinline__ uint32_t bits_below(int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u; }
+
 // A CTA's pieces in order: an item, its blocks of keys [k0, k1), and whether these are all of them.
 struct PrefixPiece {
-  PrefixTile t;
-  int head, k0, k1, prefix_tiles, n;       // n: blocks of keys
-  bool whole, head_part;                   // head_part: the item began in a CTA before
+  PrefixItem t;
+  int item, head, k0, k1, prefix_blocks, slot;
+  bool whole, two;                         // two tiles
+  bool empty;                              // no keys: the rows' zeros
+  // whether group w (of warps) has block j: every other one of a single tile, else what its tile's rows see
+  __device__ __forceinline__ bool uses(int w, int j) const {
+    if (!two) return ((j - k0) & 1) == w;
+    if (j < prefix_blocks) return true;
+    const int own = (j - prefix_blocks) * PFX_KEYS;
+    return w == 0 ? own < t.end0 : own + PFX_KEYS > t.begin1;
+  }
+  // its next block from j on (k1: none)
+  __device__ __forceinline__ int next(int w, int j) const {
+    while (j < k1 && !uses(w, j)) ++j;
+    return j;
+  }
 };
 template <typename F>
-__device__ __forceinline__ void each_piece(const PrefixParams& p, const PrefixAt& from, const PrefixAt& to, F visit) {
-  PrefixAt at = from;
-  while (at.tile < to.tile || (at.tile == to.tile && (at.head < to.head || (at.head == to.head && at.unit < to.unit)))) {
+__device__ __forceinline__ void each_piece(const PrefixParams& p, F visit) {
+  PrefixAt at = p.begins[blockIdx.x];
+  const PrefixAt to = p.begins[blockIdx.x + 1];
+  int slot = 0;
+  while (at.group < to.group || (at.group == to.group && at.group < p.n_groups)) {
+    const bool here = at.group == to.group && at.head == to.head && at.chunk == to.chunk && at.item == to.item;
+    if (here && at.unit >= to.unit) return;
+    const PrefixGroup g = p.groups[at.group];
+    const int behind = p.groups[at.group + 1].first;
     PrefixPiece x;
-    x.t = p.tiles[at.tile];
+    x.t = p.items[at.item];
+    x.item = at.item;
     x.head = at.head;
+    x.prefix_blocks = g.blocks;
+    const int blocks = item_blocks(x.t, g.blocks), end = at.chunk == g.chunks - 1 ? blocks : chunk_begin(g, at.chunk + 1);
     x.k0 = at.unit;
-    const bool ends_inside = at.tile == to.tile && at.head == to.head;
-    x.k1 = ends_inside ? to.unit : x.t.units;
-    x.prefix_tiles = (x.t.prefix_n + PFX_KEYS - 1) / PFX_KEYS;
-    x.n = x.t.prefix_n + x.t.own_n > 0 ? x.k1 - x.k0 : 0;
-    x.whole = x.k0 == 0 && x.k1 == x.t.units;
-    x.head_part = x.k0 > 0;
+    x.k1 = here ? to.unit : end;
+    x.whole = x.k0 == 0 && x.k1 == blocks;
+    x.two = x.t.rows > p.R;
+    x.empty = x.t.prefix_n + x.t.own_n == 0;
+    x.slot = min(slot, PFX_SLOTS - 1);
+    asm volatile("prefetch.global.L1 [%0];" ::"l"(p.items + min(at.item + 1, p.max_items - 1)));
     if (!visit(x)) return;
-    at.unit = 0;
-    if (++at.head == p.Hkv) {
-      at.head = 0;
-      ++at.tile;
+    if (here) return;
+    if (!x.whole) ++slot;
+    if (++at.item == behind) {
+      at.item = g.first;
+      if (++at.chunk == g.chunks) {
+        at.chunk = 0;
+        if (++at.head == p.Hkv) {
+          at.head = 0;
+          do ++at.group;
+          while (at.group < p.n_groups && p.groups[at.group + 1].first == p.groups[at.group].first);
+          if (at.group >= p.n_groups) return;
+          at.item = p.groups[at.group].first;
+        }
+      }
     }
+    at.unit = chunk_begin(p.groups[at.group], at.chunk);
   }
 }
 
@@ -258,34 +455,31 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
   using namespace umma;
   using T = PrefixShape<DP>;
   extern __shared__ __align__(1024) uint8_t smem[];
-  uint8_t *smem_q = smem, *smem_k = smem_q + T::Q * T::TILE, *smem_v = smem_k + T::K * T::TILE;
+  uint8_t *smem_q = smem, *smem_k = smem_q + 2 * T::Q * T::TILE, *smem_v = smem_k + T::K * T::TILE;
   typename T::Control& ctl = *reinterpret_cast<typename T::Control*>(smem_v + T::V * T::TILE);
-  auto &q_full = ctl.q_full, &q_empty = ctl.q_empty;
-  auto &k_full = ctl.k_full, &k_empty = ctl.k_empty;
-  auto &v_full = ctl.v_full, &v_empty = ctl.v_empty;
-  auto &s_full = ctl.s_full, &p_ready = ctl.p_ready, &o_done = ctl.o_done;
-  auto &o_free = ctl.o_free, &met = ctl.met, &drained = ctl.drained;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < T::Q; ++s) { mbar_init(smem_u32(&q_full[s]), 1); mbar_init(smem_u32(&q_empty[s]), 1); }
-    for (int s = 0; s < T::K; ++s) { mbar_init(smem_u32(&k_full[s]), 1); mbar_init(smem_u32(&k_empty[s]), 1); }
-    for (int s = 0; s < T::V; ++s) { mbar_init(smem_u32(&v_full[s]), 1); mbar_init(smem_u32(&v_empty[s]), 1); }
+    for (int s = 0; s < T::Q; ++s) { mbar_init(smem_u32(&ctl.q_full[s]), 1); mbar_init(smem_u32(&ctl.q_empty[s]), 10); }
+    for (int s = 0; s < T::K; ++s) { mbar_init(smem_u32(&ctl.k_full[s]), 1); mbar_init(smem_u32(&ctl.k_empty[s]), 2); }
+    for (int s = 0; s < T::V; ++s) { mbar_init(smem_u32(&ctl.v_full[s]), 1); mbar_init(smem_u32(&ctl.v_empty[s]), 2); }
     for (int w = 0; w < 2; ++w) {
-      mbar_init(smem_u32(&s_full[w]), 1);
-      mbar_init(smem_u32(&p_ready[w]), 128);
-      mbar_init(smem_u32(&o_done[w]), 1);
+      mbar_init(smem_u32(&ctl.s_full[w]), 1);
+      mbar_init(smem_u32(&ctl.s_read[w]), 128);
+      mbar_init(smem_u32(&ctl.p_ready[w]), 128);
+      mbar_init(smem_u32(&ctl.o_done[w]), 1);
+      mbar_init(smem_u32(&ctl.o_free[w]), 256);
+      mbar_init(smem_u32(&ctl.drained[w]), 1);
+      ctl.bad[w] = 0;
     }
-    mbar_init(smem_u32(&o_free), 256);
-    mbar_init(smem_u32(&met), 256);
-    mbar_init(smem_u32(&drained), 1);
+    mbar_init(smem_u32(&ctl.met), 256);
+    ctl.lock = 0;
     fence_barrier_init();
     prefetch_tensormap(&map_q);
     prefetch_tensormap(&map_k);
     prefetch_tensormap(&map_v);
     prefetch_tensormap(&map_pk);
     prefetch_tensormap(&map_pv);
-    ctl.bad[0] = ctl.bad[1] = 0;
   }
   if (warp == PFX_MMA) tmem_alloc(smem_u32(&ctl.tmem), 512);
   tc_fence_before_sync();
@@ -293,276 +487,403 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
   tc_fence_after_sync();
   const uint32_t tmem = ctl.tmem;
   pdl_wait();
-  if (threadIdx.x < 2) {
-    const int tiles = p.first_tile[p.prefixes == 0 ? 1 : p.prefixes + 2];
-    const int64_t all = tiles > 0 ? p.ends[tiles] * p.Hkv : 0;
-    const int ctas = (int)min(all, (int64_t)gridDim.x);
-    ctl.part[threadIdx.x] = part_begin(p, tiles, all, blockIdx.x + threadIdx.x, ctas);
-  }
-  __syncthreads();
-  const PrefixAt from = ctl.part[0], to = ctl.part[1];
 
-  if (warp == PFX_LOADER) {
-    int qn = 0, kn = 0, vn = 0;            // tiles asked for so far
-    bool ok = true;
-    each_piece(p, from, to, [&](const PrefixPiece& x) {
-      if (x.n == 0) return true;
-      const int qs = qn % T::Q;
-      if (!(ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&q_empty[qs]), ((uint32_t)(qn / T::Q) & 1u) ^ 1u, 81)))) return false;
-      if (lane == 0) {
-        const uint32_t bar = smem_u32(&q_full[qs]), dst = smem_u32(smem_q + qs * T::TILE);
-        mbar_arrive_expect_tx(bar, (uint32_t)(DP / 64 * 128 * p.share * p.R));
-#pragma unroll
-        for (int b = 0; b < DP / 64; ++b) tma_load_4d(dst + b * T::BOX, &map_q, bar, b * 64, 0, x.head, x.t.row0);
-      }
-      ++qn;
-      auto load = [&](bool keys, int j) {
-        const bool prefix = j < x.prefix_tiles;
-        const int row = prefix ? x.t.prefix0 + j * PFX_KEYS : x.t.own0 + (j - x.prefix_tiles) * PFX_KEYS;
-        int& n = keys ? kn : vn;
-        const int S = keys ? T::K : T::V, s = n % S;
-        const uint32_t empty = smem_u32(keys ? &k_empty[s] : &v_empty[s]), full = smem_u32(keys ? &k_full[s] : &v_full[s]);
-        if (!(ok = __all_sync(0xffffffffu, mbar_wait(empty, ((uint32_t)(n / S) & 1u) ^ 1u, keys ? 82 : 83)))) return false;
+  if (warp >= 8) {
+    registers_down<104>();                 // (a launch gives 384 threads 168 each: 2 x 128 x 200 + 128 x 104 is the same)
+    if (warp == PFX_LOADER) {
+      int qn = 0, kn = 0, vn = 0;          // items and blocks asked for so far
+      bool ok = true;
+      each_piece(p, [&](const PrefixPiece& x) {
+        if (x.empty) return true;
+        const int qs = qn % T::Q;
+        if (!(ok = __all_sync(0xffffffffu, mbar_spin(smem_u32(&ctl.q_empty[qs]), ((uint32_t)(qn / T::Q) & 1u) ^ 1u, 81)))) return false;
         if (lane == 0) {
-          const uint32_t dst = smem_u32((keys ? smem_k : smem_v) + s * T::TILE);
-          const CUtensorMap* map = keys ? (prefix ? &map_pk : &map_k) : (prefix ? &map_pv : &map_v);
-          mbar_arrive_expect_tx(full, (uint32_t)T::TILE);
+          const uint32_t bar = smem_u32(&ctl.q_full[qs]), dst = smem_u32(smem_q + qs * 2 * T::TILE);
+          mbar_arrive_expect_tx(bar, (uint32_t)((x.two ? 2 : 1) * DP / 64 * 128 * p.share * p.R));
+          for (int t = 0; t < (x.two ? 2 : 1); ++t)
 #pragma unroll
-          for (int b = 0; b < DP / 64; ++b) tma_load_3d(dst + b * T::BOX, map, full, b * 64, x.head, row);
+            for (int b = 0; b < DP / 64; ++b) tma_load_4d(dst + t * T::TILE + b * T::BOX, &map_q, bar, b * 64, 0, x.head, x.t.row0 + t * p.R);
         }
-        ++n;
-        return true;
-      };
-      if (!load(true, x.k0)) return false;
-      for (int j = x.k0; j < x.k1; ++j) {
-        if (j + 1 < x.k1 && !load(true, j + 1)) return false;
-        if (!load(false, j)) return false;
-      }
-      return true;
-    });
-    if (!ok) {                             // nothing that was asked for arrives after this CTA has ended
-      for (int i = 1; i <= T::Q && i <= qn; ++i) mbar_wait(smem_u32(&q_full[(qn - i) % T::Q]), (uint32_t)((qn - i) / T::Q) & 1u, 84);
-      for (int i = 1; i <= T::K && i <= kn; ++i) mbar_wait(smem_u32(&k_full[(kn - i) % T::K]), (uint32_t)((kn - i) / T::K) & 1u, 84);
-      for (int i = 1; i <= T::V && i <= vn; ++i) mbar_wait(smem_u32(&v_full[(vn - i) % T::V]), (uint32_t)((vn - i) / T::V) & 1u, 84);
-    }
-  } else if (warp == PFX_MMA) {
-    constexpr int FMT = BF16 ? 1 : 0;
-    const uint32_t idesc_s = make_idesc(128, PFX_KEYS, FMT), idesc_o = make_idesc(128, DP, FMT) | IDESC_B_MN;
-    const int steps = (p.d + 15) / 16;
-    int qn = 0, kn = 0, vn = 0, pieces = 0;
-    int sn[2] = {0, 0};                    // blocks of either group so far (scores asked for)
-    int on[2] = {0, 0};                    // products with the weights asked for
-    bool ok = true;
-    auto wait = [&](uint64_t* bar, int phase, int site) { return ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), (uint32_t)phase & 1u, site)); };
-    each_piece(p, from, to, [&](const PrefixPiece& x) {
-      if (x.n == 0) return true;
-      const int qs = qn % T::Q;
-      if (!wait(&q_full[qs], qn / T::Q, 85)) return false;
-      const uint32_t q = smem_u32(smem_q + qs * T::TILE);
-      auto scores = [&](int i) {
-        const int w = i & 1, s = kn % T::K;
-        if (!wait(&k_full[s], kn / T::K, 86)) return false;
-        // the group's weights lie over its scores (or its scores' next ones are made into them): the product that reads them has ended
-        if (on[w] > 0 && !wait(&o_done[w], on[w] - 1, 87)) return false;
-        tc_fence_after_sync();
-        const uint32_t k = smem_u32(smem_k + s * T::TILE), to_s = tmem + T::S + w * 128;
+        ++qn;
+        auto load = [&](bool keys, int j) {
+          const bool prefix = j < x.prefix_blocks;
+          const int row = prefix ? x.t.prefix0 + j * PFX_KEYS : x.t.own0 + (j - x.prefix_blocks) * PFX_KEYS;
+          int& n = keys ? kn : vn;
+          const int S = keys ? T::K : T::V, s = n % S;
+          const uint32_t empty = smem_u32(keys ? &ctl.k_empty[s] : &ctl.v_empty[s]), full = smem_u32(keys ? &ctl.k_full[s] : &ctl.v_full[s]);
+          if (!(ok = __all_sync(0xffffffffu, mbar_spin(empty, ((uint32_t)(n / S) & 1u) ^ 1u, keys ? 82 : 83)))) return false;
+          if (lane == 0) {
+            const uint32_t dst = smem_u32((keys ? smem_k : smem_v) + s * T::TILE);
+            const CUtensorMap* map = keys ? (prefix ? &map_pk : &map_k) : (prefix ? &map_pv : &map_v);
+            mbar_arrive_expect_tx(full, (uint32_t)T::TILE);
 #pragma unroll
-        for (int kk = 0; kk < DP / 16; ++kk)
-          if (kk < steps)
-            mma_f16_ss_elect(to_s, make_desc_sw128(q + (kk / 4) * T::BOX + (kk % 4) * 32, 1024), make_desc_sw128(k + (kk / 4) * T::BOX + (kk % 4) * 32, 1024),
-                             idesc_s, kk > 0 ? 1u : 0u);
-        mma_commit_elect(smem_u32(&k_empty[s]));
-        mma_commit_elect(smem_u32(&s_full[w]));
-        ++kn;
-        ++sn[w];
-        if (i == x.n - 1) mma_commit_elect(smem_u32(&q_empty[qs]));
+            for (int b = 0; b < DP / 64; ++b) tma_load_3d(dst + b * T::BOX, map, full, b * 64, x.head, row);
+          }
+          ++n;
+          return true;
+        };
+        if (!load(true, x.k0)) return false;
+        for (int j = x.k0; j < x.k1; ++j) {
+          if (j + 1 < x.k1 && !load(true, j + 1)) return false;
+          if (!load(false, j)) return false;
+        }
         return true;
-      };
-      if (!scores(0)) return false;
-      if (x.n > 1 && !scores(1)) return false;
-      for (int i = 0; i < x.n; ++i) {
-        const int w = i & 1, s = vn % T::V;
-        if (!wait(&p_ready[w], on[w], 88)) return false;
-        if (!wait(&v_full[s], vn / T::V, 89)) return false;
-        if (i < 2 && pieces > 0 && !wait(&o_free, pieces - 1, 90)) return false;
-        tc_fence_after_sync();
-        const uint32_t v = smem_u32(smem_v + s * T::TILE), to_o = tmem + T::O + w * DP, from_p = tmem + T::P + w * T::P_STEP;
-#pragma unroll
-        for (int kk = 0; kk < PFX_KEYS / 16; ++kk)
-          mma_f16_ts_elect(to_o, from_p + kk * 8, make_desc_sw128_mn(v + kk * 2048, T::BOX), idesc_o, (i >= 2 || kk > 0) ? 1u : 0u);
-        mma_commit_elect(smem_u32(&v_empty[s]));
-        mma_commit_elect(smem_u32(&o_done[w]));
-        ++vn;
-        ++on[w];
-        if (i + 2 < x.n && !scores(i + 2)) return false;
+      });
+      if (!ok) {                           // nothing that was asked for arrives after this CTA has ended
+        for (int i = 1; i <= T::Q && i <= qn; ++i) mbar_spin(smem_u32(&ctl.q_full[(qn - i) % T::Q]), (uint32_t)((qn - i) / T::Q) & 1u, 84);
+        for (int i = 1; i <= T::K && i <= kn; ++i) mbar_spin(smem_u32(&ctl.k_full[(kn - i) % T::K]), (uint32_t)((kn - i) / T::K) & 1u, 84);
+        for (int i = 1; i <= T::V && i <= vn; ++i) mbar_spin(smem_u32(&ctl.v_full[(vn - i) % T::V]), (uint32_t)((vn - i) / T::V) & 1u, 84);
       }
-      ++qn;
-      ++pieces;
-      return true;
-    });
-    if (!ok) {                             // the products in flight end before their tensor memory is given back
-      mma_commit_elect(smem_u32(&drained));
-      mbar_wait(smem_u32(&drained), 0, 91);
+    } else if (warp < PFX_MMA + 2) {
+      // A warp for each group. Where a group's weights lie over its scores, its product and the scores after it are asked for at a stretch, one group
+      // at a time (the lock): the groups fall out of step, one's MMAs beside the other's weights. (Without: the tensor cores take turns between the two,
+      // both groups wait for both, 6500 cycles for two blocks of 128; one warp for both spends 400 cycles between MMAs looking for what is ready.)
+      constexpr int FMT = BF16 ? 1 : 0;
+      const int w = warp - PFX_MMA;
+      const uint32_t idesc_s = make_idesc(128, PFX_KEYS, FMT), idesc_o = make_idesc(128, DP, FMT) | IDESC_B_MN;
+      const uint32_t to_s = uniform(tmem + T::S + w * 128), to_o = uniform(tmem + T::O + w * DP), from_p = uniform(tmem + T::P + w * T::P_STEP);
+      int qn = 0, kn = 0, vn = 0, pieces = 0;              // items; blocks whose keys and values are behind this warp
+      int on = 0;                                          // its products so far
+      bool ok = true;
+      auto wait = [&](uint64_t* bar, int phase, int site) { return ok = __all_sync(0xffffffffu, mbar_spin(smem_u32(bar), (uint32_t)phase & 1u, site)); };
+      each_piece(p, [&](const PrefixPiece& x) {
+        if (x.empty) return true;
+        const int qs = qn % T::Q, k_first = kn, v_first = vn;
+        if (!wait(&ctl.q_full[qs], qn / T::Q, 85)) return false;
+        const uint64_t q = make_desc_sw128(uniform(smem_u32(smem_q + (qs * 2 + (x.two ? w : 0)) * T::TILE)), 1024);
+        // Blocks ahead of j that this group has no use for are given back: one after the other, keys and values, as they are loaded (keys alone
+        // only where a block or two lie between: a loader that waits for buffers of values loads no keys either).
+        auto give_back = [&](int j, bool values) {
+          const int n = j - x.k0;
+          while (kn - k_first < n || (values && vn - v_first < n)) {
+            if (kn - k_first < n) {
+              if (!wait(&ctl.k_full[kn % T::K], kn / T::K, 86)) return false;
+              if (lane == 0) mbar_arrive(smem_u32(&ctl.k_empty[kn % T::K]));
+              ++kn;
+            }
+            if (values && vn - v_first < min(kn - k_first, n)) {
+              if (!wait(&ctl.v_full[vn % T::V], vn / T::V, 86)) return false;
+              if (lane == 0) mbar_arrive(smem_u32(&ctl.v_empty[vn % T::V]));
+              ++vn;
+            }
+          }
+          return true;
+        };
+        auto keys_of = [&](int j, bool values) { return give_back(j, values) && wait(&ctl.k_full[kn % T::K], kn / T::K, 86); };
+        auto scores = [&]() {              // of the block whose keys are there
+          const int s = kn % T::K;
+          // (a descriptor's address counts 16 bytes: a step of 16 elements is 2, a box of 64 columns 1024)
+          const uint64_t k = make_desc_sw128(uniform(smem_u32(smem_k + s * T::TILE)), 1024);
+          tc_fence_after_sync();
+#pragma unroll
+          for (int kk = 0; kk < DP / 16; ++kk)
+            mma_f16_ss_elect(to_s, q + (kk / 4) * (T::BOX / 16) + (kk % 4) * 2, k + (kk / 4) * (T::BOX / 16) + (kk % 4) * 2, idesc_s, kk > 0 ? 1u : 0u);
+          mma_commit_elect(smem_u32(&ctl.s_full[w]));
+          mma_commit_elect(smem_u32(&ctl.k_empty[s]));
+          ++kn;
+        };
+        int j = x.next(w, x.k0);
+        bool first = true;
+        if (j < x.k1) {
+          if (!keys_of(j, true)) return false;
+          scores();
+        }
+        while (j < x.k1) {
+          const int then = x.next(w, j + 1);
+          const bool near = then < x.k1 && then - j <= 2;  // (else the loader may wait for this block's values to be done with)
+          if (near) {
+            if (!keys_of(then, false)) return false;
+            if (T::APART) {                // the next scores, as soon as these have been read
+              if (!wait(&ctl.s_read[w], on, 87)) return false;
+              scores();
+            }
+          }
+          if (!give_back(j, true)) return false;
+          const int s = vn % T::V;
+          const uint64_t v = make_desc_sw128_mn(uniform(smem_u32(smem_v + s * T::TILE)), T::BOX);
+          if (!wait(&ctl.v_full[s], vn / T::V, 89)) return false;
+          if (first && pieces > 0 && !wait(&ctl.o_free[w], pieces - 1, 90)) return false;
+          if (!wait(&ctl.p_ready[w], on, 88)) return false;
+          if (!T::APART && !(ok = take(&ctl.lock, lane))) return false;
+          tc_fence_after_sync();
+#pragma unroll
+          for (int kk = 0; kk < PFX_KEYS / 16; ++kk) mma_f16_ts_elect(to_o, from_p + kk * 8, v + kk * 128, idesc_o, (!first || kk > 0) ? 1u : 0u);
+          mma_commit_elect(smem_u32(&ctl.o_done[w]));
+          mma_commit_elect(smem_u32(&ctl.v_empty[s]));
+          ++vn;
+          ++on;
+          first = false;
+          // Scores over weights that the product before them reads: MMAs of one thread and shape are executed in the order of their issue.
+          if (!T::APART && near) scores();
+          if (!T::APART) let_go(&ctl.lock, lane);
+          if (!near && then < x.k1) {
+            if (!keys_of(then, true)) return false;
+            scores();
+          }
+          j = then;
+        }
+        if (!give_back(x.k1, true)) return false;
+        if (first) {
+          if (lane == 0) mbar_arrive(smem_u32(&ctl.q_empty[qs]));
+        } else {
+          mma_commit_elect(smem_u32(&ctl.q_empty[qs]));
+        }
+        ++qn;
+        ++pieces;
+        return true;
+      });
+      if (!ok) {                           // the products in flight end before their tensor memory is given back
+        mma_commit_elect(smem_u32(&ctl.drained[w]));
+        mbar_spin(smem_u32(&ctl.drained[w]), 0, 91);
+      }
     }
   } else {
+    registers_up<200>();
     const int w = warp >> 2, row = threadIdx.x & 127;
     const uint32_t lanes = (uint32_t)(warp & 3) * 32u << 16;
     const uint32_t my_s = tmem + T::S + w * 128 + lanes, my_p = tmem + T::P + w * T::P_STEP + lanes, my_o = tmem + T::O + w * DP + lanes;
-    int sn = 0, on[2] = {0, 0}, seq = 0, pieces = 0;       // blocks of this group; products of either; blocks of the CTA; pieces with blocks
-    each_piece(p, from, to, [&](const PrefixPiece& x) {
-      const int g = row % p.share;
-      const bool there = row < x.t.rows * p.share;
-      const int64_t q_row = x.t.row0 + row / p.share;
-      const int q_head = x.head * p.share + g;
-      // the own keys that the row sees, counted from the tile's first
+    int sn = 0, seq = 0, pieces = 0, mets = 0;             // this group's blocks; the CTA's; pieces with keys; meetings of the groups
+    int other = 0;                                         // the other group's blocks
+    int slots = 0;
+    auto wait = [&](uint64_t* bar, int phase, int site) { return __all_sync(0xffffffffu, mbar_spin(smem_u32(bar), (uint32_t)phase & 1u, site)); };
+    each_piece(p, [&](const PrefixPiece& x) {
+      const int tile = x.two ? w : 0, tile_row = tile * p.R + row / p.share;
+      const bool there = row < p.R * p.share && tile_row < x.t.rows;
+      const int64_t q_row = (int64_t)x.t.row0 + tile_row;
+      const int q_head = x.head * p.share + row % p.share;
+      // The own keys that the row sees, counted from the item's first: read when the first block is out of hand.
       int lo = 0, hi = 0;
-      if (there && x.t.own_n > 0) {
-        int64_t a, b;
-        own_of(p, q_row, list_of(p.lists, q_row, x.t.list0, x.t.list1), a, b);
-        lo = (int)min(max(a - x.t.own0, (int64_t)0), (int64_t)x.t.own_n);
-        hi = (int)min(max(b - x.t.own0, (int64_t)0), (int64_t)x.t.own_n);
-      }
-      float m = -INFINITY, l = 0.f;
-      for (int i = w; i < x.n; i += 2) {
-        const int j = x.k0 + i;
-        const bool prefix = j < x.prefix_tiles;
-        const int key0 = prefix ? j * PFX_KEYS : (j - x.prefix_tiles) * PFX_KEYS;
-        const int in = min(PFX_KEYS, (prefix ? x.t.prefix_n : x.t.own_n) - key0);             // keys of the block
-        const bool masked = in < PFX_KEYS || (!prefix && (x.t.list0 != x.t.list1 || key0 + PFX_KEYS > x.t.own_full));
-        if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&s_full[w]), (uint32_t)sn & 1u, 92))) return false;
-        tc_fence_after_sync();
-        uint32_t s[4][32];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32_nowait(my_s + c * 32, s[c]);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_wait_ld(s[c]);
-        if (masked) {
-          const int c0 = prefix ? 0 : max(lo - key0, 0), c1 = prefix ? in : min(hi - key0, in);
-#pragma unroll
-          for (int c = 0; c < 128; ++c)
-            if (c < c0 || c >= c1) s[c / 32][c % 32] = 0xff800000u;
+      bool known = x.t.own_n == 0;
+      auto know = [&]() {
+        known = true;
+        if (there) {
+          int64_t a, b;
+          own_of(p, q_row, list_of(p.lists, q_row, tile ? x.t.list[2] : x.t.list[0], tile ? x.t.list[3] : x.t.list[1]), a, b);
+          lo = (int)min(max(a - x.t.own0, (int64_t)0), (int64_t)x.t.own_n);
+          hi = (int)min(max(b - x.t.own0, (int64_t)0), (int64_t)x.t.own_n);
         }
-        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int c = 0; c < 128; ++c) top[c % 4] = fmaxf(top[c % 4], __uint_as_float(s[c / 32][c % 32]));
-        const float next = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
-        if (__any_sync(0xffffffffu, (next - m) * p.scale > PFX_GROWTH)) {
-          // (m is -infinity: nothing has been summed; no maximum yet: nothing to move)
-          const float by = m == next || m == -INFINITY ? 1.f : ex2((m - next) * p.scale);
-          m = next;
-          l *= by;
-          if (i >= 2) {
-            if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&o_done[w]), (uint32_t)(on[w] - 1) & 1u, 93))) return false;
-            tc_fence_after_sync();
+        __syncwarp();
+      };
+      float m = -INFINITY, l = 0.f;
+      int mine = 0;
+      if (!x.empty) {
+        for (int j = x.next(w, x.k0); j < x.k1; j = x.next(w, j + 1), ++mine) {
+          const bool prefix = j < x.prefix_blocks;
+          const int key0 = (prefix ? j : j - x.prefix_blocks) * PFX_KEYS;
+          const int in = min(PFX_KEYS, (prefix ? x.t.prefix_n : x.t.own_n) - key0);           // keys of the block
+          const bool masked = in < PFX_KEYS || (!prefix && (key0 < (tile ? x.t.begin1 : 0) || key0 + PFX_KEYS > (tile ? x.t.full1 : x.t.full0)));
+          if (masked && !prefix && !known) know();
+          if (!wait(&ctl.s_full[w], sn, 92)) return false;
+          tc_fence_after_sync();
+          // Blocks that all rows see whole: the scores stay in registers. Others go by quarters of 32 keys, read once for the maximum and once for the
+          // weights, and quarters in which no row of the warp sees a key by zeros alone (a word has a bit a key that the row sees).
+          const int c0 = prefix ? 0 : max(lo - key0, 0), c1 = prefix ? in : min(hi - key0, in);
+          auto quarter = [&](int c) { return bits_below(c1 - 32 * c) & ~bits_below(c0 - 32 * c); };
+          // Sums so far are moved to a maximum that has grown. (m is -infinity: nothing has been summed; no maximum yet: nothing to move.)
+          auto move_sums = [&](float next) {
+            if (__any_sync(0xffffffffu, (next - m) * p.scale > PFX_GROWTH)) {
+              const float by = m == next || m == -INFINITY ? 1.f : ex2((m - next) * p.scale);
+              m = next;
+              l *= by;
+              if (mine == 0) return true;
+              if (!wait(&ctl.o_done[w], sn - 1, 93)) return false;
+              tc_fence_after_sync();
 #pragma unroll 1
-            for (int c = 0; c < DP; c += 32) {
-              uint32_t o[32];
-              tmem_ld32_nowait(my_o + c, o);
-              tmem_wait_ld(o);
+              for (int c = 0; c < DP; c += 16) {
+                uint32_t o[16];
+                tmem_ld16_nowait(my_o + c, o);
+                tmem_wait_ld(o);
 #pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * by);
-              tmem_st16(my_o + c, o);
-              tmem_st16(my_o + c + 16, o + 16);
+                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * by);
+                tmem_st16(my_o + c, o);
+              }
+              return true;
+            }
+            return !T::APART || mine == 0 || wait(&ctl.o_done[w], sn - 1, 93);                // (the weights before these have been read)
+          };
+          // The exponents: scale s - scale m in one FMA. A rounded scale m is the same factor to all of a row's weights, but of scores far beyond
+          // what a softmax tells apart (masks of the type's lowest value) it would be a large one: those have m taken off first.
+          const f32x2 by2 = pack2(p.scale, p.scale);
+          f32x2 sum[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
+          auto weigh = [&](const uint32_t (&q)[32], float base, uint32_t (&to)[16]) {
+            const f32x2 base2 = pack2(-base, -base);
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              float a, b;
+              unpack2(fma2(pack2(__uint_as_float(q[e]), __uint_as_float(q[e + 1])), by2, base2), a, b);
+              a = ex2(a);
+              b = ex2(b);
+              sum[e / 2 % 2] = add2(sum[e / 2 % 2], pack2(a, b));
+              to[e / 2] = pack_weights<BF16>(a, b);
+            }
+          };
+          if (!masked) {
+            uint32_t s[4][32];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) tmem_ld32_nowait(my_s + c * 32, s[c]);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) tmem_wait_ld(s[c]);
+            if (T::APART) {
+              tc_fence_before_sync();
+              mbar_arrive(smem_u32(&ctl.s_read[w]));
+            }
+            float top[4] = {m, m, m, m};
+#pragma unroll
+            for (int c = 0; c < 128; ++c) top[c % 4] = fmaxf(top[c % 4], __uint_as_float(s[c / 32][c % 32]));
+            if (!move_sums(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])))) return false;
+            float base = m == -INFINITY ? 0.f : m * p.scale;
+            if (__any_sync(0xffffffffu, fabsf(base) > 1e6f)) {
+              const float off = m == -INFINITY ? 0.f : m;
+#pragma unroll
+              for (int c = 0; c < 128; ++c) s[c / 32][c % 32] = __float_as_uint(__uint_as_float(s[c / 32][c % 32]) - off);
+              base = 0.f;
+            }
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              uint32_t weights[16];
+              weigh(s[c], base, weights);
+              tmem_st16(my_p + c * 16, weights);
+            }
+          } else {
+            float next = m;
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+              const uint32_t seen = quarter(c);
+              if (!__any_sync(0xffffffffu, seen != 0u)) continue;
+              uint32_t q[32];
+              tmem_ld32_nowait(my_s + c * 32, q);
+              tmem_wait_ld(q);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) next = fmaxf(next, seen >> e & 1 ? __uint_as_float(q[e]) : -INFINITY);
+            }
+            if (!move_sums(next)) return false;
+            const float off = m == -INFINITY ? 0.f : m;
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {                  // (weights over scores: a quarter's lie in columns that have been read)
+              const uint32_t seen = quarter(c);
+              uint32_t weights[16];
+#pragma unroll
+              for (int e = 0; e < 16; ++e) weights[e] = 0u;
+              if (__any_sync(0xffffffffu, seen != 0u)) {
+                uint32_t q[32];
+                tmem_ld32_nowait(my_s + c * 32, q);
+                tmem_wait_ld(q);
+#pragma unroll
+                for (int e = 0; e < 32; ++e) q[e] = seen >> e & 1 ? __float_as_uint(__uint_as_float(q[e]) - off) : 0xff800000u;
+                weigh(q, 0.f, weights);
+              }
+              tmem_st16(my_p + c * 16, weights);
+            }
+            if (T::APART) {
+              tc_fence_before_sync();
+              mbar_arrive(smem_u32(&ctl.s_read[w]));
             }
           }
-        }
-        // The exponents: scale s - scale m in one FMA. A rounded scale m is the same factor to all of a row's weights, but of scores far beyond what
-        // a softmax tells apart (masks of the type's lowest value) it would be a large one: those have m taken off first.
-        float base = m == -INFINITY ? 0.f : m * p.scale;
-        if (__any_sync(0xffffffffu, fabsf(base) > 1e6f)) {
-          const float off = m == -INFINITY ? 0.f : m;
+          float sums[4];
+          unpack2(sum[0], sums[0], sums[1]);
+          unpack2(sum[1], sums[2], sums[3]);
+          l += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+          if (masked) {
+            // Zero weights take no part only beside finite values: rows behind the keys become zeros, and where rows see different keys, infinities
+            // and NaN too (what they are to the rows that see them is made up for at the end; both groups may find and write the same).
+            const int at = seq + j - x.k0, vs = at % T::V;
+            if (!wait(&ctl.v_full[vs], at / T::V, 94)) return false;
+            uint8_t* v = smem_v + vs * T::TILE;
+            for (int e = in * 8 + row; e < 1024; e += 128)
 #pragma unroll
-          for (int c = 0; c < 128; ++c) s[c / 32][c % 32] = __float_as_uint(__uint_as_float(s[c / 32][c % 32]) - off);
-          base = 0.f;
-        }
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+              for (int b = 0; b < DP / 64; ++b) *reinterpret_cast<uint4*>(v + b * T::BOX + e * 16) = make_uint4(0u, 0u, 0u, 0u);
+            if (!prefix) {
+              // (0 * t is 0 but for those)
+              uint32_t sick = 0u;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t weights[16];
-#pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            const float a = ex2(fmaf(__uint_as_float(s[c][e]), p.scale, -base)), b = ex2(fmaf(__uint_as_float(s[c][e + 1]), p.scale, -base));
-            sum[e / 2 % 2] += a;
-            sum[2 + e / 2 % 2] += b;
-            weights[e / 2] = pack_weights<BF16>(a, b);
-          }
-          tmem_st16(my_p + c * 16, weights);
-        }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        if (masked) {
-          // Zero weights take no part only beside finite values: rows behind the keys become zeros, and where rows see different keys, infinities and
-          // NaN too (what they are to the rows that see them is made up for at the end).
-          const int vs = (seq + i) % T::V;
-          if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&v_full[vs]), (uint32_t)((seq + i) / T::V) & 1u, 94))) return false;
-          uint8_t* v = smem_v + vs * T::TILE;
-#pragma unroll 4
-          for (int e = row; e < DP / 64 * 1024; e += 128) {
-            const int r = e >> 3 & 127;
-            uint4* at = reinterpret_cast<uint4*>(v + (e >> 10) * T::BOX + r * 128 + (e & 7) * 16);
-            if (r >= in) {
-              *at = make_uint4(0u, 0u, 0u, 0u);
-            } else if (!prefix) {
-              uint4 t = *at;
-              uint32_t* h = reinterpret_cast<uint32_t*>(&t);
-              bool bad = false;
-#pragma unroll
-              for (int z = 0; z < 4; ++z) bad |= half_is_bad<BF16>(h[z]) || half_is_bad<BF16>(h[z] >> 16);
-              if (bad) {
-#pragma unroll
-                for (int z = 0; z < 4; ++z) h[z] &= (half_is_bad<BF16>(h[z]) ? 0u : 0xffffu) | (half_is_bad<BF16>(h[z] >> 16) ? 0u : 0xffff0000u);
-                *at = t;
-                ctl.bad[pieces & 1] = pieces + 1;
+              for (int e = 0; e < DP / 64 * 8; ++e) {
+                if (row + e % 8 * 128 >= in * 8) continue;
+                const uint4 t = *reinterpret_cast<const uint4*>(v + e / 8 * T::BOX + (row + e % 8 * 128) * 16);
+                sick = fma_zero<BF16>(t.x, sick);
+                sick = fma_zero<BF16>(t.y, sick);
+                sick = fma_zero<BF16>(t.z, sick);
+                sick = fma_zero<BF16>(t.w, sick);
+              }
+              if (half_is_bad<BF16>(sick) || half_is_bad<BF16>(sick >> 16)) {
+                // (told ahead of the writes: who finds zeros there finds this too)
+                *reinterpret_cast<volatile int*>(&ctl.bad[pieces & 1]) = pieces + 1;
+                __threadfence_block();
+                for (int e = row; e < in * 8; e += 128)
+                  for (int b = 0; b < DP / 64; ++b) {
+                    uint32_t* h = reinterpret_cast<uint32_t*>(v + b * T::BOX + e * 16);
+                    for (int z = 0; z < 4; ++z) h[z] &= (half_is_bad<BF16>(h[z]) ? 0u : 0xffffu) | (half_is_bad<BF16>(h[z] >> 16) ? 0u : 0xffff0000u);
+                  }
               }
             }
+            fence_proxy_async_smem();
+            __syncwarp();
           }
-          fence_proxy_async_smem();
-          __syncwarp();
+          tmem_wait_st();
+          tc_fence_before_sync();
+          mbar_arrive(smem_u32(&ctl.p_ready[w]));
+          ++sn;
+          if (!known) know();
         }
-        tmem_wait_st();
-        tc_fence_before_sync();
-        mbar_arrive(smem_u32(&p_ready[w]));
-        ++sn;
-        ++on[w];
       }
-      // both groups' sums together: a thread has half of its row's columns
-      float f[2] = {1.f, 0.f}, top = -INFINITY, all = 0.f;
-      bool bad = false;
-      if (x.n > 0) {
-        on[w ^ 1] += (x.n + w) / 2;                        // (this group counted its own)
-        // (what stands there of the piece before has been read)
-        if (pieces > 0 && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&o_free), (uint32_t)(pieces - 1) & 1u, 98))) return false;
-        ctl.ml[w][row] = make_float2(m, l);
-        mbar_arrive(smem_u32(&met));
-        if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&met), (uint32_t)pieces & 1u, 95))) return false;
-        const float2 a = ctl.ml[0][row], b = ctl.ml[1][row];
-        bad = ctl.bad[pieces & 1] == pieces + 1;
-        top = fmaxf(a.x, b.x);
-        f[0] = a.x == -INFINITY ? 0.f : ex2((a.x - top) * p.scale);
-        f[1] = b.x == -INFINITY ? 0.f : ex2((b.x - top) * p.scale);
-        all = a.y * f[0] + b.y * f[1];
-        if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&o_done[0]), (uint32_t)(on[0] - 1) & 1u, 96))) return false;
-        if (x.n > 1 && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&o_done[1]), (uint32_t)(on[1] - 1) & 1u, 97))) return false;
-        tc_fence_after_sync();
-      }
-      const int slot = 2 * blockIdx.x + (x.head_part ? 0 : 1);
-      const float by = x.whole && all > 0.f ? 1.f / all : x.whole && all == 0.f ? 0.f : x.whole ? all : 1.f;       // (NaN: as it is)
-#pragma unroll 1
-      for (int c0 = w * (DP / 2); c0 < (w + 1) * (DP / 2); c0 += 32) {
-        float o[32];
-        if (x.n > 0) {
-          uint32_t a[32], b[32];
-          tmem_ld32_nowait(tmem + T::O + lanes + c0, a);
-          if (x.n > 1) tmem_ld32_nowait(tmem + T::O + DP + lanes + c0, b);
-          tmem_wait_ld(a);
-          if (x.n > 1) tmem_wait_ld(b);
-#pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = (__uint_as_float(a[e]) * f[0] + (x.n > 1 ? __uint_as_float(b[e]) * f[1] : 0.f)) * by;
+      // What a thread has of its row: all columns of a tile of its own, half of them of a tile that both groups share.
+      float f[2] = {1.f, 0.f}, top = m, all = l;
+      int of[2] = {w, w ^ 1};                              // whose sums; a tile of its own has the first alone
+      bool bad = false, have[2] = {mine > 0, false};
+      if (!x.empty) {
+        const int theirs = other;
+        if (x.two) {
+          for (int j = x.next(w ^ 1, x.k0); j < x.k1; j = x.next(w ^ 1, j + 1)) ++other;
         } else {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = 0.f;
+          other += (x.k1 - x.k0 + w) / 2;
         }
+        if (!x.two) {
+          // (what stands there of the piece before has been read)
+          if (pieces > 0 && !wait(&ctl.o_free[w], pieces - 1, 98)) return false;
+          ctl.ml[w][row] = make_float2(m, l);
+          mbar_arrive(smem_u32(&ctl.met));
+          if (!wait(&ctl.met, mets, 95)) return false;
+          ++mets;
+          const float2 t = ctl.ml[w ^ 1][row];
+          top = fmaxf(m, t.x);
+          f[0] = m == -INFINITY ? 0.f : ex2((m - top) * p.scale);
+          f[1] = t.x == -INFINITY ? 0.f : ex2((t.x - top) * p.scale);
+          // (the same order in both groups: their columns are divided by the same sum)
+          all = w == 0 ? l * f[0] + t.y * f[1] : t.y * f[1] + l * f[0];
+          have[1] = other > theirs;
+        }
+        if (have[0] && !wait(&ctl.o_done[w], sn - 1, 96)) return false;
+        if (have[1] && !wait(&ctl.o_done[w ^ 1], other - 1, 97)) return false;
+        tc_fence_after_sync();
+        bad = x.k1 > x.prefix_blocks && *reinterpret_cast<volatile int*>(&ctl.bad[pieces & 1]) == pieces + 1;
+        if (bad && !known) know();
+      }
+      const int slot = blockIdx.x * PFX_SLOTS + x.slot, part_row = tile * p.R * p.share + row;
+      const float by = !x.whole ? 1.f : all > 0.f ? 1.f / all : all;                          // (no weight: zeros; NaN as it is)
+      // Results of 16-byte pieces go through shared memory, so that a warp writes whole rows (a thread's pieces lie in 32 of them: 5000 cycles for 128 rows
+      // of 64). The queries' buffer is free for it: the last scores have been made, and the second half of it where there is one tile.
+      const int qs = pieces % T::Q;
+      const bool staged = p.vec_y && x.whole && !x.empty;
+      uint4* stage = reinterpret_cast<uint4*>(smem_q + (qs * 2 + w) * T::TILE);
+      if (staged && !wait(&ctl.q_full[qs], pieces / T::Q, 99)) return false;
+      const int c_begin = x.two ? 0 : w * (DP / 2), c_end = x.two ? DP : (w + 1) * (DP / 2);
+#pragma unroll 1
+      for (int c0 = c_begin; c0 < c_end; c0 += 32) {
+        float o[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) o[e] = 0.f;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (!have[h]) continue;
+          uint32_t a[32];
+          tmem_ld32_nowait(tmem + T::O + of[h] * DP + lanes + c0, a);
+          tmem_wait_ld(a);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = fmaf(__uint_as_float(a[e]), f[h], o[e]);
+        }
+#pragma unroll
+        for (int e = 0; e < 32; ++e) o[e] *= by;
         if (there && bad) {                                // infinities and NaN among the own values that the row sees in these blocks
-          const int k_lo = max(lo, max(x.k0 - x.prefix_tiles, 0) * PFX_KEYS), k_hi = min(hi, (x.k1 - x.prefix_tiles) * PFX_KEYS);
+          const int k_lo = max(lo, max(x.k0 - x.prefix_blocks, 0) * PFX_KEYS), k_hi = min(hi, (x.k1 - x.prefix_blocks) * PFX_KEYS);
           for (int k = k_lo; k < k_hi; ++k) {
             const uint16_t* v = p.v.get<uint16_t>((int64_t)x.t.own0 + k, x.head);
 #pragma unroll
@@ -573,41 +894,65 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
             }
           }
         }
-        if (there && x.whole) {
-          uint16_t* y = const_cast<uint16_t*>(p.y.get<uint16_t>(q_row, q_head)) + c0;
+        if (x.whole && (there || staged)) {
 #pragma unroll
           for (int e = 0; e < 32; e += 8) {
             if (c0 + e >= p.d) break;                      // (d is whole pieces of 8)
             uint4 t;
             t.x = pack_weights<BF16>(o[e], o[e + 1]); t.y = pack_weights<BF16>(o[e + 2], o[e + 3]);
             t.z = pack_weights<BF16>(o[e + 4], o[e + 5]); t.w = pack_weights<BF16>(o[e + 6], o[e + 7]);
-            if (p.vec_y) {
-              *reinterpret_cast<uint4*>(y + e) = t;
+            if (staged) {
+              stage[row * (DP / 8) + (((c0 + e) / 8) ^ (row & 7))] = t;
             } else {
+              uint16_t* y = const_cast<uint16_t*>(p.y.get<uint16_t>(q_row, q_head)) + c0;
               const uint32_t h[4] = {t.x, t.y, t.z, t.w};
 #pragma unroll
               for (int z = 0; z < 8; ++z) y[e + z] = (uint16_t)(h[z / 2] >> (16 * (z & 1)));
             }
           }
         } else if (there) {
-          float* part = p.part + ((int64_t)slot * PFX_ROWS + row) * p.d + c0;
+          float4* part = p.part + ((int64_t)slot * (p.d / 4) + c0 / 4) * p.part_rows + part_row;
 #pragma unroll
           for (int e = 0; e < 32; e += 4) {
             if (c0 + e >= p.d) break;
-            *reinterpret_cast<float4*>(part + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+            part[(int64_t)(e / 4) * p.part_rows] = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
           }
         }
         __syncwarp();                                      // the lanes meet ahead of the next loads from tensor memory
       }
-      if (!x.whole && there && w == 0) p.part_ml[(int64_t)slot * PFX_ROWS + row] = make_float2(top, all);
-      if (x.n > 0) {
+      if (staged) {
+        uint16_t* mine_y = const_cast<uint16_t*>(p.y.get<uint16_t>(q_row, q_head));
+        const int from = c_begin / 8, n = (min(c_end, p.d) + 7) / 8 - from, first_row = (warp & 3) * 32;
+        for (int i = 0; i < n; ++i) {
+          const int e = i * 32 + lane, r = e / n, c = from + e - r * n;
+          uint16_t* to = reinterpret_cast<uint16_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine_y), r));
+          const bool is = __shfl_sync(0xffffffffu, (int)there, r) != 0;
+          if (is) *reinterpret_cast<uint4*>(to + c * 8) = stage[(first_row + r) * (DP / 8) + (c ^ (r & 7))];
+        }
+      }
+      if (!x.whole) {
+        if (there && (x.two || w == 0)) p.part_ml[(int64_t)slot * p.part_rows + part_row] = make_float2(top, all);
+        if (threadIdx.x == 0) p.records[slot] = {x.item, x.head, x.k0, 0};
+        slots = x.slot + 1;
+      }
+      if (!x.empty) {
         tc_fence_before_sync();
-        mbar_arrive(smem_u32(&o_free));
-        seq += x.n;
+        if (x.two) {
+          mbar_arrive_twice(smem_u32(&ctl.o_free[w]));
+        } else {
+          mbar_arrive(smem_u32(&ctl.o_free[0]));
+          mbar_arrive(smem_u32(&ctl.o_free[1]));
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&ctl.q_empty[qs]));
+        seq += x.k1 - x.k0;
         ++pieces;
       }
       return true;
     });
+    if (threadIdx.x == 0)
+      for (; slots < PFX_SLOTS; ++slots) p.records[blockIdx.x * PFX_SLOTS + slots] = {-1, 0, 0, 0};
   }
   tc_fence_before_sync();
   __syncthreads();
@@ -618,55 +963,99 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
   pdl_release();
 }
 
-// The parts of items that were cut, joined in the order of their CTAs. Block (c, y) has the item in which CTA c's part begins, if it began in the CTA
-// before: every gridDim.y-th of its rows from y on, a warp a row.
-constexpr int JOIN_THREADS = 128;
+// The pieces of items that were cut, joined in the order of their keys. Every block reads all records, then takes its share of the cut items' rows and
+// columns: 32 rows, a lane each, and 16 columns, four a warp.
+constexpr int JOIN_THREADS = 128, JOIN_MOST = 1024, JOIN_AHEAD = 8;
 template <bool BF16>
 __global__ void __launch_bounds__(JOIN_THREADS) prefix_join_kernel(const PrefixParams p) {
   pdl_begin();
-  const int tiles = p.first_tile[p.prefixes == 0 ? 1 : p.prefixes + 2];
-  const int64_t units = tiles > 0 ? p.ends[tiles] * p.Hkv : 0;
-  const int ctas = (int)min(units, (int64_t)p.ctas), c = blockIdx.x + 1, lane = threadIdx.x & 31;
-  if (c >= ctas) return;
-  const PrefixAt at = part_begin(p, tiles, units, c, ctas);
-  if (at.unit == 0) return;
-  const PrefixAt before = part_begin(p, tiles, units, c - 1, ctas);
-  if (before.tile == at.tile && before.head == at.head && before.unit > 0) return;      // cut before already
-  int last = c;                                                                          // the CTA with the item's end
-  while (last + 1 < ctas) {
-    const PrefixAt next = part_begin(p, tiles, units, last + 1, ctas);
-    if (next.tile != at.tile || next.head != at.head || next.unit == 0) break;
-    ++last;
+  __shared__ int s_item[JOIN_MOST], s_head[JOIN_MOST], s_unit[JOIN_MOST];
+  __shared__ int s_first[JOIN_MOST / 2], s_rows[JOIN_MOST / 2], s_ends[JOIN_MOST / 2];
+  __shared__ int s_slot[JOIN_MOST], s_sorted[JOIN_MOST], s_n;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, records = p.ctas * PFX_SLOTS;
+  for (int i = threadIdx.x; i < records; i += JOIN_THREADS) {
+    const PrefixRecord o = p.records[i];
+    s_item[i] = o.item; s_head[i] = o.head; s_unit[i] = o.unit;
   }
-  const PrefixTile t = p.tiles[at.tile];
-  auto slot_of = [&](int cta) { return (int64_t)(cta == c - 1 ? 2 * cta + 1 : 2 * cta) * PFX_ROWS; };
-  for (int row = blockIdx.y * (JOIN_THREADS / 32) + threadIdx.x / 32; row < t.rows * p.share; row += gridDim.y * (JOIN_THREADS / 32)) {
-    float top = -INFINITY;
-    for (int i = c - 1 + lane; i <= last; i += 32) top = fmaxf(top, p.part_ml[slot_of(i) + row].x);
+  __syncthreads();
+  if (warp == 0) {                       
+    int n = 0;
+    for (int i = lane; i - lane < records; i += 32) {
+      const bool first = i < records && s_item[i] >= 0 && s_unit[i] == 0;
+      const unsigned mask = __ballot_sync(0xffffffffu, first);
+      const int at = n + __popc(mask & ((1u << lane) - 1));
+      if (first && at < JOIN_MOST / 2) s_first[at] = i;
+      n += __popc(mask);
+    }
+    __syncwarp();
+    int ends = 0;
+    const int cols = (p.d + 15) / 16;
+    for (int i = lane; i - lane < n; i += 32) {
+      const int rows = i < n ? p.items[s_item[s_first[i]]].rows * p.share : 0;
+      int x = (rows + 31) / 32 * cols;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      for (int o = 1; o < 32; o *= 2) {
+        const int t = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += t;
+      }
+      if (i < n) { s_rows[i] = rows; s_ends[i] = ends + x; }
+      ends += __shfl_sync(0xffffffffu, x, 31);
+    }
+    if (lane == 0) s_n = n;
+  }
+  __syncthreads();
+  const int firsts = s_n, all_units = firsts > 0 ? s_ends[firsts - 1] : 0;
+  int held = -1, n = 0;
+  for (int u = blockIdx.x; u < all_units; u += gridDim.x) {
+    int k = 0;
+    while (s_ends[k] <= u) ++k;
+    const int first = s_first[k], item = s_item[first], head = s_head[first], in = u - (k > 0 ? s_ends[k - 1] : 0), row_blocks = (s_rows[k] + 31) / 32;
+    if (k != held) {
+      held = k;
+      __syncthreads();
+      if (threadIdx.x == 0) s_n = 0;
+      __syncthreads();
+      for (int i = threadIdx.x; i < records; i += JOIN_THREADS)
+        if (s_item[i] == item && s_head[i] == head) s_slot[atomicAdd(&s_n, 1)] = i;
+      __syncthreads();
+      n = s_n;
+      for (int i = threadIdx.x; i < n; i += JOIN_THREADS) {
+        int before = 0;
+        for (int o = 0; o < n; ++o) before += s_unit[s_slot[o]] < s_unit[s_slot[i]];
+        s_sorted[before] = s_slot[i];
+      }
+      __syncthreads();
+    }
+    const int row = in % row_blocks * 32 + lane, col = in / row_blocks * 16 + warp * 4;
+    if (row >= s_rows[k] || col >= p.d) continue;
+    float top = -INFINITY, all = 0.f;
+#pragma unroll 8
+    for (int i = 0; i < n; ++i) top = fmaxf(top, p.part_ml[(int64_t)s_sorted[i] * p.part_rows + row].x);
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    float all = 0.f;
-    const int col = lane * 4;
-#pragma unroll 4
-    for (int i = c - 1; i <= last; ++i) {
-      const float2 ml = p.part_ml[slot_of(i) + row];
-      const float f = ml.x == -INFINITY ? 0.f : ex2((ml.x - top) * p.scale);
-      all += ml.y * f;
-      if (col < p.d) {
-        const float4 v = *reinterpret_cast<const float4*>(p.part + (slot_of(i) + row) * p.d + col);
-        o.x = fmaf(v.x, f, o.x); o.y = fmaf(v.y, f, o.y); o.z = fmaf(v.z, f, o.z); o.w = fmaf(v.w, f, o.w);
+    for (int i0 = 0; i0 < n; i0 += JOIN_AHEAD) {
+      float4 v[JOIN_AHEAD];
+      float2 ml[JOIN_AHEAD];
+#pragma unroll
+      for (int i = 0; i < JOIN_AHEAD; ++i) {
+        const int64_t s = s_sorted[min(i0 + i, n - 1)];
+        ml[i] = p.part_ml[s * p.part_rows + row];
+        v[i] = p.part[(s * (p.d / 4) + col / 4) * p.part_rows + row];
+      }
+#pragma unroll
+      for (int i = 0; i < JOIN_AHEAD; ++i) {
+        if (i0 + i >= n) break;
+        const float f = ml[i].x == -INFINITY ? 0.f : ex2((ml[i].x - top) * p.scale);
+        all = fmaf(ml[i].y, f, all);
+        o.x = fmaf(v[i].x, f, o.x); o.y = fmaf(v[i].y, f, o.y); o.z = fmaf(v[i].z, f, o.z); o.w = fmaf(v[i].w, f, o.w);
       }
     }
     const float by = all > 0.f ? 1.f / all : all;
-    if (col < p.d) {
-      uint16_t* y = const_cast<uint16_t*>(p.y.get<uint16_t>(t.row0 + row / p.share, at.head * p.share + row % p.share)) + col;
-      const uint32_t lo = pack_weights<BF16>(o.x * by, o.y * by), hi = pack_weights<BF16>(o.z * by, o.w * by);
-      if (p.vec_y) {
-        *reinterpret_cast<uint2*>(y) = make_uint2(lo, hi);
-      } else {
-        y[0] = (uint16_t)lo; y[1] = (uint16_t)(lo >> 16); y[2] = (uint16_t)hi; y[3] = (uint16_t)(hi >> 16);
-      }
+    uint16_t* y = const_cast<uint16_t*>(p.y.get<uint16_t>((int64_t)p.items[item].row0 + row / p.share, head * p.share + row % p.share)) + col;
+    const uint32_t low = pack_weights<BF16>(o.x * by, o.y * by), high = pack_weights<BF16>(o.z * by, o.w * by);
+    if (p.vec_y) {
+      *reinterpret_cast<uint2*>(y) = make_uint2(low, high);
+    } else {
+      y[0] = (uint16_t)low; y[1] = (uint16_t)(low >> 16); y[2] = (uint16_t)high; y[3] = (uint16_t)(high >> 16);
     }
   }
 }
