@@ -35,7 +35,8 @@ def linear(q, k, v, log_decay, scale, lists, h0, dtype):
     `A` is the state with |k| |v| for k v. fp32 goes row by row: a row's three roundings are of the state's own size, (the decay less 1) is known to
     2^-21 of itself, and y is a sum of dk products. 16-bit types go by rows or by chunks of 64: there the state's operands are known to 2^-22 of
     themselves, what a matrix instruction adds is cut off (2^-23 of the running sum, 12 of them a chunk), and of what y is made of scores and states are
-    rounded to TF32 (half a step, 2^-12). A decay over n rows is exp(n log_decay), off by (n |log_decay| + 2) u and 2^-21."""
+    rounded once, of fp16 to fp16 (half a step: it keeps 10 bits behind the leading one, so neighbours are 2^-10 of a value just above a power of two
+    apart and a rounding is off by 2^-11 of it; every term of y has one such rounding, of its score or of the state), of bf16 to two bf16 terms (2^-17). A decay over n rows is exp(n log_decay), off by (n |log_decay| + 2) u and 2^-21."""
     rows, H, dk = q.shape
     share, dv = H // k.shape[1], v.shape[2]
     y, ey = np.full((rows, H, dv), np.nan), np.full((rows, H, dv), np.nan)
@@ -54,7 +55,7 @@ def linear(q, k, v, log_decay, scale, lists, h0, dtype):
             S, A = g * S + kv, g * A + np.abs(kv)
             out = scale * np.einsum("hk,hkv->hv", q[t], S)
             sized = abs(scale) * np.einsum("hk,hkv->hv", np.abs(q[t]), A)
-            off = abs(scale) * np.einsum("hk,hkv->hv", np.abs(q[t]), E) + sized * ((dk + 4) * U + (2.0 ** -12 + 2.0 ** -17 if half_type else 0))
+            off = abs(scale) * np.einsum("hk,hkv->hv", np.abs(q[t]), E) + sized * ((dk + 4) * U + ({'f16': 2.0 ** -11, 'bf16': 2.0 ** -16}.get(dtype, 0) + (2.0 ** -17 if half_type else 0)))
             y[t], ey[t] = out, off + HALF[dtype] * (np.abs(out) + off) + TINY[dtype]
         last.append(S)
         elast.append(E + 2.0 ** -126)

@@ -11,19 +11,23 @@ constexpr size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 LinearPlan linear_plan(const xb_linear_attention_args& a) {
   LinearPlan p = {};
   const int64_t mean = a.batch > 0 ? a.rows / a.batch : 0;
+  p.step = !a.offsets && a.rows == a.batch && a.dv % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.h_in) | reinterpret_cast<uintptr_t>(a.h_out)) & 15) == 0;
+  if (p.step) return p;
+  p.tiles = a.dtype != XB_F32 && mean >= 8;      // (a list of a few rows is a chunk of 64 all the same)
   const int64_t longest = !a.offsets ? mean : a.longest > 0 ? std::min(a.longest, a.rows) : a.rows;
-  // lists are cut where whole ones would not fill the SMs
-  const int64_t blocks = (int64_t)a.batch * a.H, fill = (int64_t)sm_count() * 4;
-  if (longest > 256 && (blocks < fill || longest > 4 * mean)) {
-    int64_t chunk = 256;
-    while (a.rows / chunk * a.H > 4 * fill) chunk *= 2;
-    if (longest > 2 * chunk) p.chunk = chunk;
-  }
+  // Lists are cut where some are so long that whole ones would leave SMs idle: into segments of what a block has of the rows where all are busy, 256
+  // rows at least (both ways of a segment, and its state in memory, cost about half as much again).
+  const int64_t slots = (int64_t)std::max(sm_count(), 1) * (p.tiles ? a.dv <= 64 ? (a.dk <= 64 ? 4 : 2) : (a.dk <= 64 ? 2 : 1) : 4);
+  const int64_t share = (a.rows * a.H + slots - 1) / slots, chunk = std::max<int64_t>((share + 63) / 64 * 64, 256);
+  if (longest > 3 * chunk) p.chunk = chunk;
+  // whole lists of unlike lengths in more than a wave of blocks: long ones first
+  p.order = p.chunk == 0 && a.offsets && longest > mean + mean / 2 && a.batch <= 65536 && (int64_t)a.batch * a.H > slots;
   return p;
 }
-struct LinearScratch { size_t first, bytes; };      // (the ends lie first)
+struct LinearScratch { size_t first, bytes; };      // (the ends lie first; a plan has chunks or an order)
 LinearScratch linear_scratch(const xb_linear_attention_args& a, const LinearPlan& p) {
   LinearScratch w = {};
+  if (p.order) w.bytes = align256((size_t)a.batch * 4);
   if (p.chunk == 0 || a.rows / p.chunk == 0) return w;
   const size_t states = align256((size_t)(a.rows / p.chunk) * a.H * a.dk * a.dv * 4);
   w.first = states;
@@ -87,9 +91,12 @@ extern "C" int xb_linear_attention(const xb_linear_attention_args* a, void* work
   p.H = a->H; p.share = a->H / a->Hkv; p.dk = a->dk; p.dv = a->dv; p.scale = a->scale;
   p.vec_q = heads_whole(q, size, 4 * size); p.vec_k = heads_whole(k, size, 4 * size); p.vec_v = heads_whole(v, size, 4 * size);
   p.vec_y = heads_whole(y, size, 2 * size) && a->dv % 2 == 0;
+  auto unit = [&](const Heads& x) { return heads_whole(x, size, 16) ? 16 : heads_whole(x, size, 8) ? 8 : heads_whole(x, size, 4) ? 4 : 2; };
+  p.unit_q = unit(q); p.unit_k = unit(k); p.unit_v = unit(v);
   p.vec_h = a->dv % 2 == 0 && (hi | ho) % 8 == 0;
   p.vec_e = a->dk * a->dv % 4 == 0;
-  if (w.bytes) {
+  if (plan.order) p.order = static_cast<int*>(workspace);
+  if (plan.chunk && w.bytes) {
     p.chunk = plan.chunk;
     p.n_ends = (int)(a->rows / plan.chunk);
     p.end = static_cast<float*>(workspace);

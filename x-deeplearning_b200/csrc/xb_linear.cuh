@@ -22,7 +22,9 @@ struct LinearParams {
   int H, share, dk, dv;                    // share: heads that read one head of k and v
   float scale;
   int vec_q, vec_k, vec_v, vec_y;          // rows in whole pieces: of four elements, y of two
+  int unit_q, unit_k, unit_v;              // bytes that rows may be read by: 16, 8, 4 or an element
   int vec_h, vec_e;                        // kept states in pairs; the ends of segments in pieces of four
+  int* order;                              // [batch]: whole lists, long ones first; null: as they come
   int64_t chunk;                           // 0: whole lists
   int n_ends;                              // rows / chunk
   float* end;                              // [n_ends][H][dk][dv]: states at the ends of segments
@@ -30,8 +32,10 @@ struct LinearParams {
   int ends_only;                           // the first of the three launches
 };
 struct LinearPlan {
+  bool step;                               // one row a list, states in pieces of four columns
   bool tiles;                              // by chunks of 64 rows on the matrix instructions, else row by row
   int64_t chunk;
+  bool order;                              // whole lists, long ones first
 };
 // the kernels of one type (xb_linear_*.cu)
 int linear_f32(const LinearParams& p, const LinearPlan& plan, cudaStream_t s);
@@ -52,6 +56,7 @@ __device__ __forceinline__ bool find_segment(const LinearParams& p, int u, int l
   int i = u;
   int64_t b, e;
   if (p.chunk == 0) {
+    if (p.order) i = p.order[u];
     b = p.lists.begin(i);
     e = p.lists.begin(i + 1);
     g.begin = b; g.end = e > b ? e : b; g.number = 0; g.last = true; g.at = 0;
@@ -116,10 +121,10 @@ __global__ void __launch_bounds__(64 * PARTS) linear_rows_kernel(const LinearPar
   __shared__ Segment s_seg;
   __shared__ int s_there;
   __shared__ __align__(16) float s_q[LIN_ROWS][DK], s_k[LIN_ROWS][DK], s_v[LIN_ROWS][DV];
-  const int lane = threadIdx.x & 31, h = blockIdx.y, hkv = h / p.share;
+  const int lane = threadIdx.x & 31, h = (int)(blockIdx.x % (unsigned)p.H), hkv = h / p.share;
   if (threadIdx.x < 32) {
     Segment g;
-    const bool there = find_segment(p, (int)blockIdx.x, lane, g);
+    const bool there = find_segment(p, (int)(blockIdx.x / (unsigned)p.H), lane, g);
     if (lane == 0) {
       s_seg = g;
       s_there = there;
@@ -237,14 +242,15 @@ __global__ void __launch_bounds__(64 * PARTS) linear_rows_kernel(const LinearPar
     }
     __syncthreads();
     if (ahead && r0 + LIN_ROWS < g.end) fetch(r0 + LIN_ROWS);
-#pragma unroll 1
+    // (a row's product with q beside the next row's step: 74 lists of 100 rows, 2 heads of 36, fp32 37 us with one after the other)
+#pragma unroll 4
     for (int r = 0; r < rows; ++r) {
-      f32x2 v2[NV], y2[NV];
+      f32x2 v2[NV], y2[NV][2];
 #pragma unroll
       for (int n = 0; n < NV; ++n) {
         const float v = mine ? s_v[r][c + n] : 0.f;
         v2[n] = pack2(v, v);
-        y2[n] = pack2(0.f, 0.f);
+        y2[n][0] = y2[n][1] = pack2(0.f, 0.f);
       }
       auto move = [&](auto slow) {
 #pragma unroll
@@ -258,7 +264,7 @@ __global__ void __launch_bounds__(64 * PARTS) linear_rows_kernel(const LinearPar
             for (int n = 0; n < NV; ++n) {
               f32x2& a = S[n][2 * j + b];
               a = fma2(a, by, decltype(slow)::value ? fma2(k2, v2[n], a) : mul2(k2, v2[n]));
-              y2[n] = fma2(q2, a, y2[n]);
+              y2[n][j & 1] = fma2(q2, a, y2[n][j & 1]);
             }
           }
         }
@@ -270,7 +276,7 @@ __global__ void __launch_bounds__(64 * PARTS) linear_rows_kernel(const LinearPar
 #pragma unroll
       for (int n = 0; n < NV; ++n) {
         float a, b;
-        unpack2(y2[n], a, b);
+        unpack2(add2(y2[n][0], y2[n][1]), a, b);
         y[n] = a + b;
 #pragma unroll
         for (int o = 1; o < PARTS; o *= 2) y[n] += __shfl_xor_sync(0xffffffffu, y[n], o);
@@ -291,6 +297,79 @@ __global__ void __launch_bounds__(64 * PARTS) linear_rows_kernel(const LinearPar
   }
   float* to = state_to(p, g, h);
   if (to) put_state(to);
+}
+
+// ---- single tokens ----
+// One row a list, columns of the states in pieces of four: a block has a list and a head, LANES threads a row of the state, each STEP_AHEAD rows
+// at a time, whose reads are on their way at once; y is summed over the rows' groups in shared memory. Bound by the states' bytes, which is a matter
+// of reads in flight: few registers, eight blocks an SM. 2048 lists, 8 heads of 64 x 64: 216 us row by row with the state in registers.
+constexpr int STEP_THREADS = 128, STEP_AHEAD = 8;
+template <typename T, int LANES>
+__global__ void __launch_bounds__(STEP_THREADS, 8) linear_step_kernel(const LinearParams p) {
+  pdl_wait();
+  constexpr int GROUPS = STEP_THREADS / LANES;
+  __shared__ float s_q[LIN_MAX], s_k[LIN_MAX];
+  __shared__ __align__(16) float s_y[GROUPS][LANES * 4];
+  const int h = (int)(blockIdx.x % (unsigned)p.H), i = (int)(blockIdx.x / (unsigned)p.H), hkv = h / p.share;
+  const int group = threadIdx.x / LANES, c = threadIdx.x % LANES * 4, slot = p.lists.slot(i);
+  const bool mine = c < p.dv;
+  const int64_t at = ((int64_t)slot * p.H + h) * p.dk * p.dv;
+  const float* from = p.h_in && slot >= 0 && mine ? p.h_in + at + c : nullptr;
+  float* to = p.h_out && slot >= 0 && mine ? p.h_out + at + c : nullptr;
+  float4 s[STEP_AHEAD];
+  auto fetch = [&](int k0) {
+#pragma unroll
+    for (int a = 0; a < STEP_AHEAD; ++a) {
+      const int k = k0 + a * GROUPS;
+      s[a] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (from && k < p.dk) s[a] = *reinterpret_cast<const float4*>(from + k * p.dv);
+    }
+  };
+  fetch(group);
+  for (int k = threadIdx.x; k < p.dk; k += STEP_THREADS) {
+    s_q[k] = to_f32<T>(p.q.get<T>(i, h)[k]);
+    s_k[k] = to_f32<T>(p.k.get<T>(i, hkv)[k]);
+  }
+  float v[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
+  if (mine) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = to_f32<T>(p.v.get<T>(i, hkv)[c + e]);
+  }
+  const Decay decay(log_decay_of(p, h));
+  const float keep = decay.slow ? 1.f : 0.f;
+  __syncthreads();
+  for (int k0 = group; k0 < p.dk; k0 += STEP_AHEAD * GROUPS) {
+    if (k0 > group) fetch(k0);
+#pragma unroll
+    for (int a = 0; a < STEP_AHEAD; ++a) {
+      const int k = k0 + a * GROUPS;
+      if (k >= p.dk) break;
+      const float kk = s_k[k], q = s_q[k];
+      float x[4] = {s[a].x, s[a].y, s[a].z, s[a].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[e] = fmaf(x[e], decay.by, fmaf(kk, v[e], x[e] * keep));
+        y[e] = fmaf(q, x[e], y[e]);
+      }
+      if (to) *reinterpret_cast<float4*>(to + k * p.dv) = make_float4(x[0], x[1], x[2], x[3]);
+    }
+  }
+  *reinterpret_cast<float4*>(&s_y[group][c]) = make_float4(y[0], y[1], y[2], y[3]);
+  __syncthreads();
+  for (int j = threadIdx.x; j < p.dv; j += STEP_THREADS) {
+    float sum = 0.f;
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) sum += s_y[g][j];
+    const_cast<T*>(p.y.get<T>(i, h))[j] = from_f32<T>(sum * p.scale);
+  }
+}
+template <typename T>
+int launch_linear_step(const LinearParams& p, dim3 grid, cudaStream_t s) {
+  const int lanes = (p.dv + 3) / 4;
+  if (lanes <= 8) launch_dependent(linear_step_kernel<T, 8>, grid, STEP_THREADS, 0, s, p);
+  else if (lanes <= 16) launch_dependent(linear_step_kernel<T, 16>, grid, STEP_THREADS, 0, s, p);
+  else launch_dependent(linear_step_kernel<T, 32>, grid, STEP_THREADS, 0, s, p);
+  return check_launch("linear_step_kernel");
 }
 
 // ends[j] += decay over a segment * ends[j - 1], for all segments of a list but the first and the last. A thread has four values of a state.
@@ -361,8 +440,13 @@ int launch_linear_rows(const LinearParams& p, dim3 grid, cudaStream_t s) {
 template <typename F>
 int launch_linear_parts(LinearParams p, cudaStream_t s, F run) {
   const int64_t units = p.chunk ? p.n_ends + (int64_t)p.lists.batch : p.lists.batch;
-  XB_REQUIRE(units < ((int64_t)1 << 31), XB_ERR_LIMIT, "xb_linear_attention: too many rows and lists");
-  const dim3 grid((unsigned)units, (unsigned)p.H);
+  // (a list's heads side by side: long lists start first in all of them, and heads that share keys and values run at the same time)
+  XB_REQUIRE(units * p.H < ((int64_t)1 << 31), XB_ERR_LIMIT, "xb_linear_attention: too many rows, lists and heads");
+  const dim3 grid((unsigned)(units * p.H));
+  if (p.order) {
+    launch_dependent(lists_order_kernel, 1, 1024, 0, s, p.lists, p.order);
+    if (int rc = check_launch("lists_order_kernel")) return rc;
+  }
   if (p.chunk) {
     p.ends_only = 1;
     if (int rc = run(p, grid)) return rc;

@@ -29,4 +29,20 @@ __device__ __forceinline__ void mma_half(float (&c)[4], const uint32_t (&a)[4], 
   for (int e = 0; e < 4; ++e) c[e] += d[e];
 }
 
+// halves that are infinite or NaN
+template <bool BF16>
+__device__ __forceinline__ bool half_is_bad(uint32_t h) {
+  constexpr uint32_t E = BF16 ? 0x7f80u : 0x7c00u;
+  return (h & E) == E;
+}
+
+// sum + 0 * t, two halves: NaN once a t was infinite or NaN
+template <bool BF16>
+__device__ __forceinline__ uint32_t fma_zero(uint32_t t, uint32_t sum) {
+  uint32_t r;
+  if constexpr (BF16) asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(t), "r"(0u), "r"(sum));
+  else asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(t), "r"(0u), "r"(sum));
+  return r;
+}
+
 }  // namespace xb

@@ -19,6 +19,7 @@
 #include <algorithm>
 
 #include "xb_heads.cuh"
+#include "xb_mma_half.cuh"
 #include "xb_umma.cuh"
 
 namespace xb {
@@ -366,23 +367,8 @@ __device__ __forceinline__ uint32_t pack_weights(float lo, float hi) {
   else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-// halves that are infinite or NaN
-template <bool BF16>
-__device__ __forceinline__ bool half_is_bad(uint32_t h) {
-  constexpr uint32_t E = BF16 ? 0x7f80u : 0x7c00u;
-  return (h & E) == E;
-}
-
 // A value that all lanes have, told to the compiler as such: what the MMAs take then stands in uniform registers.
 __device__ __forceinline__ uint32_t uniform(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
-// sum + 0 * t, two halves: NaN once a t was infinite or NaN
-template <bool BF16>
-__device__ __forceinline__ uint32_t fma_zero(uint32_t t, uint32_t sum) {
-  uint32_t r;
-  if constexpr (BF16) asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(t), "r"(0u), "r"(sum));
-  else asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(t), "r"(0u), "r"(sum));
-  return r;
-}
 // the lowest n bits, n cut to [0, 32]
 __device__ __forceinline__ uint32_t bits_below(int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u; }
 

@@ -274,6 +274,36 @@ __device__ __forceinline__ void write_floats(float* p, const float (&v)[V]) {
   }
 }
 
+// The lists with long ones first, by classes of length (a quarter of a power of two each): the blocks of a launch start in this order, and a
+// long list that starts last keeps a few SMs busy while the others have nothing left. Within a class the order is any; results do
+// not depend on it.
+__global__ void __launch_bounds__(1024) lists_order_kernel(const Lists lists, int* order) {
+  pdl_begin();
+  constexpr int CLASSES = 33 * 4;
+  __shared__ int s_at[CLASSES];
+  const int tid = threadIdx.x;
+  auto class_of = [&](int i) {
+    const int64_t n = lists.begin(i + 1) - lists.begin(i);
+    const unsigned len = n > 0 ? (unsigned)n : 0u;
+    const int zeros = __clz(len);
+    return len ? zeros * 4 + 3 - (int)(((len << zeros) >> 29) & 3u) : CLASSES - 1;
+  };
+  for (int c = tid; c < CLASSES; c += 1024) s_at[c] = 0;
+  __syncthreads();
+  for (int i = tid; i < lists.batch; i += 1024) atomicAdd(&s_at[class_of(i)], 1);
+  __syncthreads();
+  if (tid == 0) {
+    int sum = 0;
+    for (int c = 0; c < CLASSES; ++c) {
+      const int n = s_at[c];
+      s_at[c] = sum;
+      sum += n;
+    }
+  }
+  __syncthreads();
+  for (int i = tid; i < lists.batch; i += 1024) order[atomicAdd(&s_at[class_of(i)], 1)] = i;
+}
+
 constexpr int SPL = 4;                    // states of a lane
 constexpr int SCAN_THREADS = 128;
 

@@ -428,36 +428,6 @@ __global__ void __launch_bounds__(SCAN_THREADS, SCAN_BLOCKS<K>) ssm_scan_kernel(
   }
 }
 
-// The lists with long ones first, by classes of length (a quarter of a power of two each): the blocks of a launch start in this order, and a
-// long list that starts last keeps a few SMs busy while the others have nothing left. Within a class the order is any; results do
-// not depend on it.
-__global__ void __launch_bounds__(1024) ssm_order_kernel(const ScanParams p) {
-  pdl_begin();
-  constexpr int CLASSES = 33 * 4;
-  __shared__ int s_at[CLASSES];
-  const int tid = threadIdx.x;
-  auto class_of = [&](int i) {
-    const int64_t n = p.lists.begin(i + 1) - p.lists.begin(i);
-    const unsigned len = n > 0 ? (unsigned)n : 0u;
-    const int zeros = __clz(len);
-    return len ? zeros * 4 + 3 - (int)(((len << zeros) >> 29) & 3u) : CLASSES - 1;
-  };
-  for (int c = tid; c < CLASSES; c += 1024) s_at[c] = 0;
-  __syncthreads();
-  for (int i = tid; i < p.lists.batch; i += 1024) atomicAdd(&s_at[class_of(i)], 1);
-  __syncthreads();
-  if (tid == 0) {
-    int sum = 0;
-    for (int c = 0; c < CLASSES; ++c) {
-      const int n = s_at[c];
-      s_at[c] = sum;
-      sum += n;
-    }
-  }
-  __syncthreads();
-  for (int i = tid; i < p.lists.batch; i += 1024) p.order[atomicAdd(&s_at[class_of(i)], 1)] = i;
-}
-
 // 2^q as two factors: the rows of a chunk each have a decay that fp32 holds where the chunk's need not. Exponents from -252 to 254 leave of any
 // state that is not 0 less than 2^-124, or more than fp32 holds. (Where q is infinite or a NaN the chunk's own end is.)
 struct Decay {
@@ -541,8 +511,8 @@ int launch_tiles(const ScanParams& p, const ScanPlan& plan, cudaStream_t s) {
   const int64_t units = p.lists.batch + (int64_t)p.n_ends;
   XB_REQUIRE(units * blocks < ((int64_t)1 << 31), XB_ERR_LIMIT, "xb_ssm_scan: too many lists and channels");
   if (p.order) {
-    launch_dependent(ssm_order_kernel, 1, 1024, 0, s, p);
-    if (int rc = check_launch("ssm_order_kernel")) return rc;
+    launch_dependent(lists_order_kernel, 1, 1024, 0, s, p.lists, p.order);
+    if (int rc = check_launch("lists_order_kernel")) return rc;
   }
   if (p.chunk > 0) {
     launch_dependent(ssm_scan_kernel<T, LPC, K, SCAN_ENDS>, (unsigned)((int64_t)p.n_ends * blocks), SCAN_THREADS, 0, s, p, a_group);
