@@ -89,7 +89,6 @@ extern "C" int xb_linear_attention(const xb_linear_attention_args* a, void* work
   p.log_decay = a->log_decay; p.h_in = a->h_in; p.h_out = a->h_out;
   p.lists = {a->offsets, a->slots, a->rows, a->rows / a->batch, a->batch, a->n_slots};
   p.H = a->H; p.share = a->H / a->Hkv; p.dk = a->dk; p.dv = a->dv; p.scale = a->scale;
-  p.vec_q = heads_whole(q, size, 4 * size); p.vec_k = heads_whole(k, size, 4 * size); p.vec_v = heads_whole(v, size, 4 * size);
   p.vec_y = heads_whole(y, size, 2 * size) && a->dv % 2 == 0;
   auto unit = [&](const Heads& x) { return heads_whole(x, size, 16) ? 16 : heads_whole(x, size, 8) ? 8 : heads_whole(x, size, 4) ? 4 : 2; };
   p.unit_q = unit(q); p.unit_k = unit(k); p.unit_v = unit(v);

@@ -21,7 +21,7 @@ struct LinearParams {
   Lists lists;
   int H, share, dk, dv;                    // share: heads that read one head of k and v
   float scale;
-  int vec_q, vec_k, vec_v, vec_y;          // rows in whole pieces: of four elements, y of two
+  int vec_y;                               // rows of y in pieces of two
   int unit_q, unit_k, unit_v;              // bytes that rows may be read by: 16, 8, 4 or an element
   int vec_h, vec_e;                        // kept states in pairs; the ends of segments in pieces of four
   int* order;                              // [batch]: whole lists, long ones first; null: as they come
@@ -108,19 +108,33 @@ __device__ __forceinline__ float* state_to(const LinearParams& p, const Segment&
 }
 
 // ---- row by row ----
-// A block has a list (or segment) and a head; a thread NV columns of dv (two where there are more than 64) and 32 of dk, PARTS lanes sharing the
-// columns, whose products with q meet in shuffles. The state stays in registers, in pairs along dk. Rows come 16 at a time through shared memory,
-// as fp32; pieces of four along dk go round the PARTS lanes, so that what a warp reads at once lies in adjacent banks.
-// Single tokens: all of the state's reads of a thread are on their way at once; bound by the states' bytes. Lists: 3 packed FMAs for two values
-// of the state a row, bound by their issue and by the broadcast reads of k and q.
-constexpr int LIN_KT = 32, LIN_ROWS = 16, LIN_MAX = 128, LIN_V = 4;
-template <typename T, int PARTS, int NV>
+// A block has a list (or segment) and a head; a thread NV columns of dv (two where there are more than 64) and KT of dk, PARTS lanes sharing the
+// columns, whose products with q meet in shuffles. KT is 32, or 8 where there are so few lists that the row's latency counts. The state stays in registers, in pairs along dk. Rows come eight at a time through shared memory,
+// three such tiles ahead; pieces of four along dk go round the PARTS lanes, so that what a warp reads at once lies in adjacent banks.
+// 3 packed FMAs for two values of the state a row, bound by the latency of a row's steps where there are few lists, by the FMAs' issue and the
+// broadcast reads of k and q where there are many. 74 lists of 100 rows, 2 heads of 36, fp32: 37 us with rows that pass through registers.
+constexpr int LIN_ROWS = 8, LIN_TILES = 4, LIN_MAX = 128;
+// four adjacent elements of shared memory, as two pairs of fp32
+template <typename T>
+__device__ __forceinline__ void read_four(const T* p, f32x2& lo, f32x2& hi) {
+  if constexpr (sizeof(T) == 4) {
+    const ulonglong2 t = *reinterpret_cast<const ulonglong2*>(p);
+    lo = t.x; hi = t.y;
+  } else {
+    const uint2 t = *reinterpret_cast<const uint2*>(p);
+    Raw<T, 4> r;
+    r.w[0] = t.x; r.w[1] = t.y;
+    lo = pack2(r.get(0), r.get(1)); hi = pack2(r.get(2), r.get(3));
+  }
+}
+template <typename T, int KT, int PARTS, int NV>
 __global__ void __launch_bounds__(64 * PARTS) linear_rows_kernel(const LinearParams p) {
   pdl_wait();
-  constexpr int DK = LIN_KT * PARTS, V = LIN_V, DV = 64 * NV;
+  constexpr int DK = KT * PARTS, DV = 64 * NV, TILE = LIN_ROWS * (2 * DK + DV);
+  extern __shared__ __align__(128) uint8_t smem[];          // [tiles][q, k, v][rows][DK or DV]
+  T* s_rows = reinterpret_cast<T*>(smem);
   __shared__ Segment s_seg;
   __shared__ int s_there;
-  __shared__ __align__(16) float s_q[LIN_ROWS][DK], s_k[LIN_ROWS][DK], s_v[LIN_ROWS][DV];
   const int lane = threadIdx.x & 31, h = (int)(blockIdx.x % (unsigned)p.H), hkv = h / p.share;
   if (threadIdx.x < 32) {
     Segment g;
@@ -135,11 +149,11 @@ __global__ void __launch_bounds__(64 * PARTS) linear_rows_kernel(const LinearPar
   const Segment g = s_seg;
   const int part = threadIdx.x % PARTS, c = threadIdx.x / PARTS * NV;
   const bool mine = c < p.dv;
-  f32x2 S[NV][LIN_KT / 2];
+  f32x2 S[NV][KT / 2];
   const float* from = state_from(p, g, h);
   auto at_dk = [&](int j) { return ((j / 4) * PARTS + part) * 4 + j % 4; };
 #pragma unroll
-  for (int j = 0; j < LIN_KT; j += 2) {
+  for (int j = 0; j < KT; j += 2) {
     float x[2][NV];
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
@@ -163,7 +177,7 @@ __global__ void __launch_bounds__(64 * PARTS) linear_rows_kernel(const LinearPar
   }
   auto put_state = [&](float* to) {
 #pragma unroll
-    for (int j = 0; j < LIN_KT; j += 2) {
+    for (int j = 0; j < KT; j += 2) {
       float x[2][NV];
 #pragma unroll
       for (int n = 0; n < NV; ++n) unpack2(S[n][j / 2], x[0][n], x[1][n]);
@@ -185,81 +199,88 @@ __global__ void __launch_bounds__(64 * PARTS) linear_rows_kernel(const LinearPar
   if (from && p.ends_only) put_state(p.first + (g.at * p.H + h) * (int64_t)p.dk * p.dv);
   const Decay decay(log_decay_of(p, h));
   const f32x2 by = pack2(decay.by, decay.by);
-  // The next rows are read while these are worked on, where the block has the threads for it (all but narrow heads).
-  constexpr int LEAST = 32 * PARTS, PQ = LIN_ROWS * DK / V / LEAST, PV = LIN_ROWS * DV / V / LEAST;
-  const int pieces_v = (p.dv + V - 1) / V, n_threads = (int)blockDim.x;
-  const bool ahead = n_threads >= LEAST;
-  Raw<T, V> tq[PQ], tk[PQ], tv[PV];
-  auto read_qk = [&](int64_t r0, int e, Raw<T, V>& a, Raw<T, V>& b) {
-    const int r = e / (DK / V), x = e % (DK / V) * V, in = r < LIN_ROWS && r0 + r < g.end ? min(V, p.dk - x) : 0;
-    a.zero();
-    b.zero();
-    if (in <= 0) return;
-    if (!p.ends_only) a.load(p.q.get<T>(r0 + r, h) + x, in, p.vec_q);
-    b.load(p.k.get<T>(r0 + r, hkv) + x, in, p.vec_k);
+  // Rows [r0, r0 + 8) of q, k and v into a tile, in pieces of the bytes that their rows lie on; what lies behind the list and behind the width is zero.
+  // Piece e of a tile is the same row, tensor and column in every tile: where a thread's first pieces come from and go to is worked out once.
+  const int n_threads = (int)blockDim.x;
+  struct Piece {
+    const char* src;                       // in tile 0 (null: none)
+    int64_t step;                          // bytes from tile to tile
+    uint32_t to;                           // in tile 0
+    int row, unit, bytes;
   };
-  auto put_qk = [&](int e, const Raw<T, V>& a, const Raw<T, V>& b) {
-    const int r = e / (DK / V), x = e % (DK / V) * V;
-    if (r >= LIN_ROWS) return;
-    write_floats<V>(&s_q[r][x], a.all().v);
-    write_floats<V>(&s_k[r][x], b.all().v);
+  auto pieces_of = [&](int width, int unit) { return (width * (int)sizeof(T) + unit - 1) / unit; };
+  const int n_q = p.ends_only ? 0 : pieces_of(p.dk, p.unit_q), n_k = pieces_of(p.dk, p.unit_k), n_v = pieces_of(p.dv, p.unit_v);
+  const int row_pieces = n_q + n_k + n_v, tile_pieces = LIN_ROWS * row_pieces;
+  auto piece = [&](int e) {
+    Piece x;
+    x.row = e / row_pieces;
+    int c = e - x.row * row_pieces;
+    const int which = c < n_q ? 0 : c < n_q + n_k ? 1 : 2;
+    c -= which == 0 ? 0 : which == 1 ? n_q : n_q + n_k;
+    const Heads& from = which == 0 ? p.q : which == 1 ? p.k : p.v;
+    const int D = which == 2 ? DV : DK, width = which == 2 ? p.dv : p.dk;
+    x.unit = which == 0 ? p.unit_q : which == 1 ? p.unit_k : p.unit_v;
+    x.src = e < tile_pieces ? reinterpret_cast<const char*>(from.get<T>(g.begin + x.row, which == 0 ? h : hkv)) + c * x.unit : nullptr;
+    x.step = from.row * (int64_t)sizeof(T) * LIN_ROWS;
+    x.to = (uint32_t)__cvta_generic_to_shared(reinterpret_cast<char*>(s_rows + which * LIN_ROWS * DK + x.row * D) + c * x.unit);
+    x.bytes = min(x.unit, width * (int)sizeof(T) - c * x.unit);
+    return x;
   };
-  auto read_v = [&](int64_t r0, int e, Raw<T, V>& a) {
-    const int r = e / pieces_v, x = (e - r * pieces_v) * V, in = r < LIN_ROWS && r0 + r < g.end ? min(V, p.dv - x) : 0;
-    a.zero();
-    if (in > 0) a.load(p.v.get<T>(r0 + r, hkv) + x, in, p.vec_v);
+  auto copy = [&](const Piece& x, int tile) {
+    if (!x.src) return;
+    const bool in = g.begin + (int64_t)tile * LIN_ROWS + x.row < g.end;
+    const char* f = in ? x.src + tile * x.step : x.src;    // (nothing is read of a piece behind the end)
+    const uint32_t at = x.to + tile % LIN_TILES * (TILE * (uint32_t)sizeof(T));
+    const int bytes = in ? x.bytes : 0;
+    if (x.unit == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at), "l"(f), "r"(bytes) : "memory");
+    else if (x.unit == 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(at), "l"(f), "r"(bytes) : "memory");
+    else if (x.unit == 4) asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(at), "l"(f), "r"(bytes) : "memory");
+    else asm volatile("st.shared.u16 [%0], %1;" ::"r"(at), "h"(bytes ? *reinterpret_cast<const uint16_t*>(f) : (uint16_t)0) : "memory");
   };
-  auto put_v = [&](int e, const Raw<T, V>& a) {
-    const int r = e / pieces_v, x = (e - r * pieces_v) * V;
-    if (r < LIN_ROWS) write_floats<V>(&s_v[r][x], a.all().v);
-  };
-  auto fetch = [&](int64_t r0) {
+  constexpr int KNOWN = 2;
+  Piece known[KNOWN];
 #pragma unroll
-    for (int i = 0; i < PQ; ++i) read_qk(r0, threadIdx.x + i * n_threads, tq[i], tk[i]);
+  for (int i = 0; i < KNOWN; ++i) known[i] = piece(threadIdx.x + i * n_threads);
+  auto load_tile = [&](int tile) {
+    if (g.begin + (int64_t)tile * LIN_ROWS < g.end) {
 #pragma unroll
-    for (int i = 0; i < PV; ++i) read_v(r0, threadIdx.x + i * n_threads, tv[i]);
-  };
-  if (ahead && g.begin < g.end) fetch(g.begin);
-  for (int64_t r0 = g.begin; r0 < g.end; r0 += LIN_ROWS) {
-    const int rows = (int)min((int64_t)LIN_ROWS, g.end - r0);
-    if (r0 > g.begin) __syncthreads();
-    if (ahead) {
-#pragma unroll
-      for (int i = 0; i < PQ; ++i) put_qk(threadIdx.x + i * n_threads, tq[i], tk[i]);
-#pragma unroll
-      for (int i = 0; i < PV; ++i) put_v(threadIdx.x + i * n_threads, tv[i]);
-    } else {
-      for (int e = threadIdx.x; e < LIN_ROWS * (DK / V); e += n_threads) {
-        Raw<T, V> a, b;
-        read_qk(r0, e, a, b);
-        put_qk(e, a, b);
-      }
-      for (int e = threadIdx.x; e < LIN_ROWS * pieces_v; e += n_threads) {
-        Raw<T, V> a;
-        read_v(r0, e, a);
-        put_v(e, a);
-      }
+      for (int i = 0; i < KNOWN; ++i) copy(known[i], tile);
+      for (int e = threadIdx.x + KNOWN * n_threads; e < tile_pieces; e += n_threads) copy(piece(e), tile);
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  if (p.dk != DK || p.dv != DV || p.ends_only) {
+    for (int e = threadIdx.x; e < LIN_TILES * TILE * (int)sizeof(T) / 16; e += n_threads) reinterpret_cast<uint4*>(smem)[e] = make_uint4(0u, 0u, 0u, 0u);
     __syncthreads();
-    if (ahead && r0 + LIN_ROWS < g.end) fetch(r0 + LIN_ROWS);
-    // (a row's product with q beside the next row's step: 74 lists of 100 rows, 2 heads of 36, fp32 37 us with one after the other)
+  }
+#pragma unroll
+  for (int t = 0; t < LIN_TILES - 1; ++t) load_tile(t);
+  int tile = 0;
+  for (int64_t r0 = g.begin; r0 < g.end; r0 += LIN_ROWS, ++tile) {
+    const int rows = (int)min((int64_t)LIN_ROWS, g.end - r0);
+    asm volatile("cp.async.wait_group %0;" ::"n"(LIN_TILES - 2) : "memory");
+    __syncthreads();                       // (the tile is there, and all have done with the one before)
+    load_tile(tile + LIN_TILES - 1);
+    const T *s_q = s_rows + tile % LIN_TILES * TILE, *s_k = s_q + LIN_ROWS * DK, *s_v = s_k + LIN_ROWS * DK;
+    T* y_at = const_cast<T*>(p.y.get<T>(r0, h)) + c;
 #pragma unroll 4
-    for (int r = 0; r < rows; ++r) {
+    for (int r = 0; r < rows; ++r) {       // (a row's product with q beside the next row's step)
       f32x2 v2[NV], y2[NV][2];
 #pragma unroll
       for (int n = 0; n < NV; ++n) {
-        const float v = mine ? s_v[r][c + n] : 0.f;
+        const float v = mine ? to_f32<T>(s_v[r * DV + c + n]) : 0.f;
         v2[n] = pack2(v, v);
         y2[n][0] = y2[n][1] = pack2(0.f, 0.f);
       }
       auto move = [&](auto slow) {
 #pragma unroll
-        for (int j = 0; j < LIN_KT / 4; ++j) {
-          const ulonglong2 k4 = *reinterpret_cast<const ulonglong2*>(&s_k[r][(j * PARTS + part) * 4]);
-          const ulonglong2 q4 = *reinterpret_cast<const ulonglong2*>(&s_q[r][(j * PARTS + part) * 4]);
+        for (int j = 0; j < KT / 4; ++j) {
+          f32x2 k4[2], q4[2];
+          read_four(s_k + r * DK + (j * PARTS + part) * 4, k4[0], k4[1]);
+          read_four(s_q + r * DK + (j * PARTS + part) * 4, q4[0], q4[1]);
 #pragma unroll
           for (int b = 0; b < 2; ++b) {
-            const f32x2 k2 = b ? k4.y : k4.x, q2 = b ? q4.y : q4.x;
+            const f32x2 k2 = k4[b], q2 = q4[b];
 #pragma unroll
             for (int n = 0; n < NV; ++n) {
               f32x2& a = S[n][2 * j + b];
@@ -283,7 +304,7 @@ __global__ void __launch_bounds__(64 * PARTS) linear_rows_kernel(const LinearPar
         y[n] *= p.scale;
       }
       if (part != 0 || !mine) continue;
-      T* to = const_cast<T*>(p.y.get<T>(r0 + r, h)) + c;
+      T* to = y_at + r * p.y.row;
       if (NV == 2 && p.vec_y) {
         Raw<T, 2> out;
         out.put_all(y);
@@ -421,19 +442,32 @@ __global__ void __launch_bounds__(CARRY_THREADS) linear_carry_kernel(const Linea
   }
 }
 
-template <typename T, int PARTS>
-void launch_linear_columns(const LinearParams& p, dim3 grid, cudaStream_t s) {
-  const int nv = p.dv <= 64 ? 1 : 2;
-  const unsigned threads = (unsigned)(((p.dv + nv - 1) / nv * PARTS + 31) / 32 * 32);
-  if (nv == 1) launch_dependent(linear_rows_kernel<T, PARTS, 1>, grid, threads, 0, s, p);
-  else launch_dependent(linear_rows_kernel<T, PARTS, 2>, grid, threads, 0, s, p);
+template <typename T, int KT, int PARTS, int NV>
+int launch_linear_columns(const LinearParams& p, dim3 grid, cudaStream_t s) {
+  constexpr int SMEM = LIN_TILES * LIN_ROWS * (2 * KT * PARTS + 64 * NV) * (int)sizeof(T);
+  if constexpr (SMEM > 46 * 1024) {           // (48 KB with what the kernel has besides)
+    static PerDeviceOnce once;
+    XB_SET_MAX_SMEM_ONCE(once, SMEM, (const void*)linear_rows_kernel<T, KT, PARTS, NV>);
+  }
+  const unsigned threads = (unsigned)(((p.dv + NV - 1) / NV * PARTS + 31) / 32 * 32);
+  launch_dependent(linear_rows_kernel<T, KT, PARTS, NV>, grid, threads, SMEM, s, p);
+  return check_launch("linear_rows_kernel");
 }
+template <typename T, int KT, int PARTS>
+int launch_linear_parts_of(const LinearParams& p, dim3 grid, cudaStream_t s) {
+  return p.dv <= 64 ? launch_linear_columns<T, KT, PARTS, 1>(p, grid, s) : launch_linear_columns<T, KT, PARTS, 2>(p, grid, s);
+}
+// us with 32 and 8 of dk a thread: 74 lists of 100 rows, 2 heads of 36, fp32 TODO
 template <typename T>
 int launch_linear_rows(const LinearParams& p, dim3 grid, cudaStream_t s) {
-  if (p.dk <= LIN_KT) launch_linear_columns<T, 1>(p, grid, s);
-  else if (p.dk <= 2 * LIN_KT) launch_linear_columns<T, 2>(p, grid, s);
-  else launch_linear_columns<T, 4>(p, grid, s);
-  return check_launch("linear_rows_kernel");
+  if ((int64_t)grid.x < 4 * (int64_t)sm_count()) {
+    if (p.dk <= 32) return launch_linear_parts_of<T, 8, 4>(p, grid, s);
+    if (p.dk <= 64) return launch_linear_parts_of<T, 8, 8>(p, grid, s);
+    return launch_linear_parts_of<T, 16, 8>(p, grid, s);
+  }
+  if (p.dk <= 32) return launch_linear_parts_of<T, 32, 1>(p, grid, s);
+  if (p.dk <= 64) return launch_linear_parts_of<T, 32, 2>(p, grid, s);
+  return launch_linear_parts_of<T, 32, 4>(p, grid, s);
 }
 
 // The launches of a call, with `run` for the segments (or lists) of a grid
