@@ -10,10 +10,17 @@
 // the same keys, which come from memory once. (512 rows of 4 heads on 100003 keys, one item after another: 4 times the bytes.) What a CTA has of an
 // item that is not whole goes to the workspace as sums in fp32 with their running maximum, and a last kernel joins those in order.
 //
-// In a CTA one warp loads (TMA), and and two groups of four warps, each with a warp that issues its MMAs, have scores, weights and sums of their own in
-// tensor memory: one tile each of an item of two, whose keys they share, or of a single tile every other block of keys. While one makes weights of
-// its scores, the tensor cores are at the other's. A thread has a row; a maximum that has not grown by more than 2^8 leaves the sums as they are
-// (weights up to 256 fit both types), so that they are seldom moved.
+// In a CTA (16 warps) two groups of four warps make weights of scores, each with a warp that issues its MMAs and with scores, weights and sums of its own
+// in tensor memory: one tile each of an item of two, whose keys they share, or of a single tile every other block of keys. While one makes weights,
+// the tensor cores are at the other's. A thread has a row; a maximum that has not grown by more than 2^8 leaves the sums as they are (weights up to
+// 256 fit both types), so that they are seldom moved. One more warp loads (TMA), one works the pieces out ahead of the others, and four clear what must
+// not take part of the blocks of values that some row sees in part (in the groups themselves that was a sixth of the time of short lists).
+//
+// What bounds it is neither memory nor the tensor cores but the way from scores to weights: 128 exponentials a row and block at 16 a cycle and SM, 1024
+// cycles for a block of 128 rows, with the maximum, the packing and the loads and stores of tensor memory 1500 to 2100; and some 18000 cycles an item of
+// few blocks (offsets, the first keys, the results). 512 candidates of 4 heads of 128 on one prefix of 100003 rows: 165 us (its bytes: 62); 74 requests of
+// 1000 candidates on 100 rows each, 4 heads of 64: 122 us (24); 256 lists of up to 300 rows that 8 prefixes of up to 4000 serve, 32 heads on 8 of 128, one
+// new row each: 206 us (69); 64 lists of up to 500 rows, whole, 16 prefixes of up to 1000, 8 heads of 64: 376 us (48).
 #pragma once
 
 #include <algorithm>
@@ -25,7 +32,8 @@
 namespace xb {
 namespace {
 
-constexpr int PFX_KEYS = 128, PFX_ROWS = 128, PFX_THREADS = 384, PFX_LOADER = 8, PFX_MMA = 9, PFX_SLOTS = 4;
+constexpr int PFX_KEYS = 128, PFX_ROWS = 128, PFX_THREADS = 512, PFX_LOADER = 8, PFX_MMA = 9, PFX_SLOTS = 4;
+constexpr int PFX_RING = 2, PFX_TAKERS = 15;               // pieces ahead; warps that take them
 constexpr float PFX_GROWTH = 8.f;
 
 struct PrefixItem {
@@ -80,8 +88,9 @@ __device__ __forceinline__ int64_t prefix_begin(const PrefixParams& p, int i) {
   return o < 0 ? 0 : o > p.prefix_rows ? p.prefix_rows : o;
 }
 // the list of a row, from lo to hi (that of a later row): the last that begins at it or ahead of it
-__device__ __forceinline__ int list_of(const Lists& l, int64_t row, int lo, int hi) {
-  if (!l.offsets) return l.per > 0 ? (int)(row / l.per) : 0;
+__device__ __noinline__ int list_of(const Lists& l, int64_t row, int lo, int hi) {
+  if (!l.offsets) return l.per > 0 ? (int)((uint32_t)row / (uint32_t)l.per) : 0;      // (rows are counted in 31 bits)
+#pragma unroll 1
   while (lo < hi) {
     const int mid = lo + (hi - lo + 1) / 2;
     if (l.begin(mid) <= row) lo = mid;
@@ -90,10 +99,16 @@ __device__ __forceinline__ int list_of(const Lists& l, int64_t row, int lo, int 
   return lo;
 }
 // the own keys that a row sees: a list's last row sees all of them, each row before it one less
-__device__ __forceinline__ void own_of(const PrefixParams& p, int64_t row, int list, int64_t& lo, int64_t& hi) {
-  lo = p.own.begin(list);
-  hi = p.own.begin(list + 1) - max(p.lists.begin(list + 1) - 1 - row, (int64_t)0);
+__device__ __noinline__ void own_of(const Lists& lists, const Lists& own, int64_t row, int list, int64_t& lo, int64_t& hi) {
+  lo = own.begin(list);
+  hi = own.begin(list + 1) - max(lists.begin(list + 1) - 1 - row, (int64_t)0);
   if (hi < lo) hi = lo;
+}
+// the same of a row in one of some lists, counted from key own0 and cut to own_n
+__device__ __noinline__ int2 row_keys(const PrefixParams& p, int row, int list_a, int list_b, int own0, int own_n) {
+  int64_t a, b;
+  own_of(p.lists, p.own, row, list_of(p.lists, row, list_a, list_b), a, b);
+  return make_int2((int)min(max(a - own0, (int64_t)0), (int64_t)own_n), (int)min(max(b - own0, (int64_t)0), (int64_t)own_n));
 }
 constexpr int PLAN_THREADS = 1024, PLAN_GROUPS = 1024, PLAN_ITEMS = 2048;      // (what shared memory holds of a plan; larger ones are in the workspace alone)
 __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* s_sums, int64_t& total) {      // exclusive
@@ -120,8 +135,9 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* s_sums, int64_
 
 // Chunk c of a prefix's blocks begins at c blocks / chunks. All items of a group and a head of keys, in the line: for every chunk but the last its
 // blocks of item after item, then item after item the last chunk's with the own keys behind them. A block of an item of two tiles counts twice.
+__device__ __noinline__ int64_t quotient64(int64_t a, int64_t b) { return a / b; }
 __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {      // (of numbers that are not negative; 64-bit division takes 100 instructions)
-  return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
+  return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : quotient64(a, b);
 }
 __device__ __forceinline__ int chunk_begin(const PrefixGroup& g, int c) { return g.chunks == 1 ? c * g.blocks : (int)quotient((int64_t)c * g.blocks, g.chunks); }
 __device__ __forceinline__ int item_blocks(const PrefixItem& x, int prefix_blocks) {
@@ -129,6 +145,7 @@ __device__ __forceinline__ int item_blocks(const PrefixItem& x, int prefix_block
 }
 __device__ __forceinline__ PrefixAt line_place(const PrefixParams& p, const PrefixGroup* groups, const int64_t* own_weight, int64_t x, int64_t all, int ctas) {
   int lo = 0, hi = p.n_groups - 1;
+#pragma unroll 1
   while (lo < hi) {                        // the last group that begins at x or ahead of it
     const int mid = lo + (hi - lo + 1) / 2;
     if (groups[mid].weight * p.Hkv <= x) lo = mid;
@@ -157,6 +174,7 @@ __device__ __forceinline__ PrefixAt line_place(const PrefixParams& p, const Pref
   const int64_t own = own_weight[g.first];
   lo = 0;
   hi = n - 1;
+#pragma unroll 1
   while (lo < hi) {
     const int mid = lo + (hi - lo + 1) / 2;
     if ((int64_t)mid * 2 * rem + own_weight[g.first + mid] - own <= r) lo = mid;
@@ -191,13 +209,14 @@ __device__ __forceinline__ PrefixAt line_place(const PrefixParams& p, const Pref
 
 // One block: three sums over groups and items and a search a CTA, each behind a read or two from memory. 74 requests of 1000 candidates: 11 us with the
 // sums in the workspace, whose every read takes 0.4 us.
-__global__ void __launch_bounds__(PLAN_THREADS) prefix_plan_kernel(const PrefixParams p) {
+__global__ void __launch_bounds__(PLAN_THREADS) prefix_plan_kernel(const __grid_constant__ PrefixParams p) {
   pdl_begin();
   __shared__ int64_t s_sums[PLAN_THREADS / 32], s_own[PLAN_ITEMS + 1];
   __shared__ PrefixGroup s_groups[PLAN_GROUPS + 1];
   const int threads = blockDim.x, n_groups = p.n_groups, step = 2 * p.R;
   PrefixGroup* groups = n_groups <= PLAN_GROUPS ? s_groups : p.groups;
   int64_t total = 0, sum;
+#pragma unroll 1
   for (int g0 = 0; g0 < n_groups; g0 += threads) {
     const int g = g0 + (int)threadIdx.x;
     PrefixGroup x = {};
@@ -221,11 +240,13 @@ __global__ void __launch_bounds__(PLAN_THREADS) prefix_plan_kernel(const PrefixP
   }
   __syncthreads();
   int64_t own_total = 0;
+#pragma unroll 1
   for (int t0 = 0; t0 < items; t0 += threads) {
     const int t = t0 + (int)threadIdx.x;
     int64_t weight = 0;
     if (t < items) {
       int lo = 0, hi = n_groups - 1;                      // the group: the last that begins at the item or ahead of it
+#pragma unroll 1
       while (lo < hi) {
         const int mid = lo + (hi - lo + 1) / 2;
         if (groups[mid].first <= t) lo = mid;
@@ -245,15 +266,14 @@ __global__ void __launch_bounds__(PLAN_THREADS) prefix_plan_kernel(const PrefixP
       x.list[2] = mid < end ? list_of(p.lists, mid, x.list[1], l1) : x.list[1];
       x.list[3] = mid < end ? list_of(p.lists, end - 1, x.list[2], l1) : x.list[1];
       if (p.own.rows > 0) {
-        // (first and last row of either tile: where their own keys begin and end)
-        int64_t b0, e0, b1, e1, b2, e2, b3, e3;
-        own_of(p, begin, x.list[0], b0, e0);
-        own_of(p, mid - 1, x.list[1], b1, e1);
-        b2 = b1; e2 = e1; b3 = b1; e3 = e1;
-        if (mid < end) {
-          own_of(p, mid, x.list[2], b2, e2);
-          own_of(p, end - 1, x.list[3], b3, e3);
-        }
+        // first and last row of either tile: where their own keys begin and end (all reads at once)
+        const int64_t row[4] = {begin, mid - 1, min(mid, end - 1), end - 1};
+        int64_t from[4], to[4], last[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) { from[k] = p.own.begin(x.list[k]); to[k] = p.own.begin(x.list[k] + 1); last[k] = p.lists.begin(x.list[k] + 1) - 1; }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) to[k] = max(to[k] - max(last[k] - row[k], (int64_t)0), from[k]);
+        const int64_t b0 = from[0], e0 = to[0], e1 = to[1], b2 = from[2], e2 = to[2], e3 = to[3];
         const int64_t n = max(e3 - b0, (int64_t)0);
         auto in = [&](int64_t k) { return (int)min(max(k - b0, (int64_t)0), n); };
         x.own0 = (int)b0; x.own_n = (int)n; x.end0 = in(e1); x.begin1 = mid < end ? in(b2) : 0;
@@ -271,6 +291,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) prefix_plan_kernel(const PrefixP
   if (threadIdx.x == 0) own_weight[items] = own_total;
   __syncthreads();
   int64_t all = 0;
+#pragma unroll 1
   for (int g0 = 0; g0 < n_groups; g0 += threads) {
     const int g = g0 + (int)threadIdx.x;
     int64_t weight = 0;
@@ -282,35 +303,61 @@ __global__ void __launch_bounds__(PLAN_THREADS) prefix_plan_kernel(const PrefixP
   if (threadIdx.x == 0) groups[n_groups].weight = all;
   all *= p.Hkv;
   const int ctas = (int)min(all, (int64_t)p.ctas);
+#pragma unroll 1
   for (int g = threadIdx.x; g < n_groups; g += threads) {
     // (several items, each longer than a part: as many chunks as parts of an item)
     const int64_t chunks = groups[g].tiles > 2 && all > 0 ? quotient(2 * (int64_t)groups[g].blocks * ctas, all) : 1;
     groups[g].chunks = (int)max(min(chunks, (int64_t)groups[g].blocks), (int64_t)1);
   }
   __syncthreads();
+#pragma unroll 1
   for (int c = threadIdx.x; c <= p.ctas; c += threads) {
     PrefixAt at = {n_groups, 0, 0, 0, 0};
     if (c < ctas) at = line_place(p, groups, own_weight, quotient(all * c, ctas), all, ctas);
     p.begins[c] = at;
   }
   if (groups == s_groups)
+#pragma unroll 1
     for (int g = threadIdx.x; g <= n_groups; g += threads) p.groups[g] = s_groups[g];
 }
 
 // ---- the kernel ----
+// A CTA's pieces in order: an item, its blocks of keys [k0, k1), and whether these are all of them.
+struct PrefixPiece {
+  PrefixItem t;
+  int item, head, k0, k1, prefix_blocks, slot;
+  int clean0, clean1, clean2;              // blocks [clean0, clean1) and from clean2 on hold values that some row does not see beside ones that it does
+  bool valid;                              // (false: there are no more)
+  bool whole, two;                         // two tiles
+  bool empty;                              // no keys: the rows' zeros
+  // The blocks of either group of warps: of a single tile every other one, else what its tile's rows see: all but [hole0, hole1), up to `end`.
+  struct Walk {
+    int begin, end, n;
+  } walk[2];
+  int step, hole0, hole1;
+  // (by comparison: a place counted at run time would put the piece into memory)
+  __device__ __forceinline__ Walk of(int w) const { return {w ? walk[1].begin : walk[0].begin, w ? walk[1].end : walk[0].end, w ? walk[1].n : walk[0].n}; }
+  __device__ __forceinline__ bool cleaned(int j) const { return (j >= clean0 && j < clean1) || j >= clean2; }
+  __device__ __forceinline__ int next(int w, int j) const {
+    j += step;
+    return w == 1 && j >= hole0 && j < hole1 ? hole1 : j;
+  }
+};
 template <int DP>
 struct PrefixShape {
   static constexpr int Q = DP == 128 ? 1 : 2, K = DP == 128 ? 3 : 5, V = DP == 128 ? 2 : 5;     // buffers (of queries: an item's)
   static constexpr int TILE = 128 * DP * 2, BOX = 128 * 128;
   struct Control {                         // behind the buffers (the kernel has no other shared memory, so that its buffers begin on 1024 bytes)
-    uint64_t q_full[Q], q_empty[Q], k_full[K], k_empty[K], v_full[V], v_empty[V];
+    uint64_t q_full[Q], q_empty[Q], k_full[K], k_empty[K], v_full[V], v_clean[V], v_empty[V];
     uint64_t s_full[2], s_read[2], p_ready[2], o_done[2], o_free[2], met, drained[2];
+    uint64_t piece_full[PFX_RING], piece_empty[PFX_RING];
+    PrefixPiece ring[PFX_RING];
     float2 ml[2][PFX_ROWS];                // maximum and sum of either group's rows
     int bad[2], lock;
     uint32_t tmem;
   };
   static constexpr int SMEM = (2 * Q + K + V) * TILE + (int)sizeof(Control);
-  static_assert(SMEM <= 227 * 1024, "");
+  static_assert(SMEM <= 227 * 1024 - 64, "");
   // Columns of tensor memory: the scores of both groups, their sums; weights where there is room, else over the scores that they are made of
   // (whose next ones then wait for the weights' product).
   static constexpr bool APART = DP == 64;
@@ -322,31 +369,29 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
                "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
                : "memory");
 }
-// mbar_wait whose tries go one after the other: what waits here is woken many times a microsecond, and there is no other warp to give way to
+// mbar_wait with a limit on its tries, each of which ends after a microsecond at the latest: it stands in the code in many places, and takes a
+// quarter of the instructions of one that looks at the clock.
+constexpr int PFX_TRIES = 1 << 21;
 __device__ __forceinline__ bool mbar_spin(uint32_t bar, uint32_t parity, int site) {
-  using namespace umma;
-  if (mbar_try_wait(bar, parity)) return true;
-  const long long t0 = clock64(), limit = wait_limit();
-  while (!mbar_try_wait(bar, parity)) {
-    if (clock64() - t0 > limit) {
-      wait_gave_up(site);
-      return false;
-    }
-  }
-  return true;
+  if (umma::mbar_try_wait(bar, parity)) return true;
+#pragma unroll 1
+  for (int i = 0; i < PFX_TRIES; ++i)
+    if (umma::mbar_try_wait_for(bar, parity, 1000u)) return true;
+  umma::wait_gave_up(site);
+  return false;
 }
 __device__ __forceinline__ void mbar_arrive_twice(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], 2;" ::"r"(bar) : "memory"); }
 // A lock between two warps, held for the time of a few instructions. False: it was not to be had (with the limit of the waits).
 __device__ __forceinline__ bool take(int* lock, int lane) {
   int ok = 1;
   if (lane == 0) {
-    const long long t0 = clock64(), limit = umma::wait_limit();
-    while (atomicCAS(lock, 0, 1) != 0)
-      if (clock64() - t0 > limit) {
-        umma::wait_gave_up(99);
-        ok = 0;
-        break;
-      }
+    int tries = 0;
+#pragma unroll 1
+    while (atomicCAS(lock, 0, 1) != 0 && ++tries < PFX_TRIES) {}
+    if (tries == PFX_TRIES) {
+      umma::wait_gave_up(99);
+      ok = 0;
+    }
   }
   return __shfl_sync(0xffffffffu, ok, 0) != 0;
 }
@@ -372,30 +417,14 @@ __device__ __forceinline__ uint32_t uniform(uint32_t v) { return __reduce_max_sy
 // the lowest n bits, n cut to [0, 32]
 __device__ __forceinline__ uint32_t bits_below(int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u; }
 
-// A CTA's pieces in order: an item, its blocks of keys [k0, k1), and whether these are all of them.
-struct PrefixPiece {
-  PrefixItem t;
-  int item, head, k0, k1, prefix_blocks, slot;
-  bool whole, two;                         // two tiles
-  bool empty;                              // no keys: the rows' zeros
-  // whether group w (of warps) has block j: every other one of a single tile, else what its tile's rows see
-  __device__ __forceinline__ bool uses(int w, int j) const {
-    if (!two) return ((j - k0) & 1) == w;
-    if (j < prefix_blocks) return true;
-    const int own = (j - prefix_blocks) * PFX_KEYS;
-    return w == 0 ? own < t.end0 : own + PFX_KEYS > t.begin1;
-  }
-  // its next block from j on (k1: none)
-  __device__ __forceinline__ int next(int w, int j) const {
-    while (j < k1 && !uses(w, j)) ++j;
-    return j;
-  }
-};
+// A CTA's pieces are worked out by a warp of their own, ahead of the others, which take them from a ring in shared memory: the plan's reads, each
+// behind the other, stand in nobody's way, and the walk is in the code once.
 template <typename F>
-__device__ __forceinline__ void each_piece(const PrefixParams& p, F visit) {
+__device__ __forceinline__ void make_pieces(const PrefixParams& p, F put) {
   PrefixAt at = p.begins[blockIdx.x];
   const PrefixAt to = p.begins[blockIdx.x + 1];
   int slot = 0;
+#pragma unroll 1
   while (at.group < to.group || (at.group == to.group && at.group < p.n_groups)) {
     const bool here = at.group == to.group && at.head == to.head && at.chunk == to.chunk && at.item == to.item;
     if (here && at.unit >= to.unit) return;
@@ -412,10 +441,21 @@ __device__ __forceinline__ void each_piece(const PrefixParams& p, F visit) {
     x.whole = x.k0 == 0 && x.k1 == blocks;
     x.two = x.t.rows > p.R;
     x.empty = x.t.prefix_n + x.t.own_n == 0;
+    x.valid = true;
     x.slot = min(slot, PFX_SLOTS - 1);
-    asm volatile("prefetch.global.L1 [%0];" ::"l"(p.items + min(at.item + 1, p.max_items - 1)));
-    if (!visit(x)) return;
-    if (here) return;
+    // (a prefix's last block, if it is not full; own blocks but those that all rows see whole: of one list, which all of the item's rows are in)
+    x.clean0 = x.t.prefix_n % PFX_KEYS ? g.blocks - 1 : g.blocks;
+    x.clean1 = g.blocks;
+    x.clean2 = g.blocks + (x.t.list[0] == x.t.list[3] ? min(x.t.full0, x.t.own_n) / PFX_KEYS : 0);
+    x.step = x.two ? 1 : 2;
+    x.hole0 = x.two ? g.blocks : 0;
+    x.hole1 = x.two ? g.blocks + x.t.begin1 / PFX_KEYS : 0;
+    const int end0 = x.two ? min(x.k1, g.blocks + (x.t.end0 + PFX_KEYS - 1) / PFX_KEYS) : x.k1;
+    x.walk[0] = {x.k0, end0, max((end0 - x.k0 + x.step - 1) / x.step, 0)};
+    const int first1 = x.two ? (x.k0 >= x.hole0 && x.k0 < x.hole1 ? x.hole1 : x.k0) : x.k0 + 1;
+    const int left_out = x.two ? max(min(x.hole1, x.k1) - max(x.hole0, first1), 0) : 0;
+    x.walk[1] = {first1, x.k1, max((x.k1 - first1 + x.step - 1) / x.step - left_out, 0)};
+    if (!put(x) || here) return;
     if (!x.whole) ++slot;
     if (++at.item == behind) {
       at.item = g.first;
@@ -433,6 +473,34 @@ __device__ __forceinline__ void each_piece(const PrefixParams& p, F visit) {
     at.unit = chunk_begin(p.groups[at.group], at.chunk);
   }
 }
+// false: a wait ran out
+template <typename C, typename F>
+__device__ __forceinline__ bool each_piece(C& ctl, int lane, F visit) {
+#pragma unroll 1
+  for (int n = 0;; ++n) {
+    if (!__all_sync(0xffffffffu, mbar_spin(umma::smem_u32(&ctl.piece_full[n % PFX_RING]), (uint32_t)(n / PFX_RING) & 1u, 80))) return false;
+    const PrefixPiece x = ctl.ring[n % PFX_RING];
+    __syncwarp();
+    if (lane == 0) umma::mbar_arrive(umma::smem_u32(&ctl.piece_empty[n % PFX_RING]));
+    if (!x.valid) return true;
+    if (!visit(x)) return false;
+  }
+}
+
+// Infinities and NaN among own values, which the products were made without: they are what they are whatever is added to them. For a row's columns [c0, c1) and keys [k0, k1).
+template <bool BF16>
+__device__ __noinline__ void spread_bad(const Heads v, int64_t row0, int head, int c0, int c1, int k0, int k1, uint16_t* y, float* part, int64_t part_step) {
+  for (int c = c0; c < c1; ++c) {
+    float sum = 0.f;
+    for (int k = k0; k < k1; ++k) {
+      const uint16_t t = v.get<uint16_t>(row0 + k, head)[c];
+      if (half_is_bad<BF16>(t)) sum += BF16 ? __uint_as_float((uint32_t)t << 16) : __half2float(__ushort_as_half(t));
+    }
+    if (sum == 0.f) continue;
+    if (y) y[c] = (uint16_t)pack_weights<BF16>(sum, sum);
+    else part[(c / 4) * part_step + c % 4] = sum;
+  }
+}
 
 template <bool BF16, int DP>
 __global__ void __launch_bounds__(PFX_THREADS, 1)
@@ -448,7 +516,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
   if (threadIdx.x == 0) {
     for (int s = 0; s < T::Q; ++s) { mbar_init(smem_u32(&ctl.q_full[s]), 1); mbar_init(smem_u32(&ctl.q_empty[s]), 10); }
     for (int s = 0; s < T::K; ++s) { mbar_init(smem_u32(&ctl.k_full[s]), 1); mbar_init(smem_u32(&ctl.k_empty[s]), 2); }
-    for (int s = 0; s < T::V; ++s) { mbar_init(smem_u32(&ctl.v_full[s]), 1); mbar_init(smem_u32(&ctl.v_empty[s]), 2); }
+    for (int s = 0; s < T::V; ++s) { mbar_init(smem_u32(&ctl.v_full[s]), 1); mbar_init(smem_u32(&ctl.v_clean[s]), 128); mbar_init(smem_u32(&ctl.v_empty[s]), 3); }
     for (int w = 0; w < 2; ++w) {
       mbar_init(smem_u32(&ctl.s_full[w]), 1);
       mbar_init(smem_u32(&ctl.s_read[w]), 128);
@@ -458,6 +526,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       mbar_init(smem_u32(&ctl.drained[w]), 1);
       ctl.bad[w] = 0;
     }
+    for (int r = 0; r < PFX_RING; ++r) { mbar_init(smem_u32(&ctl.piece_full[r]), 1); mbar_init(smem_u32(&ctl.piece_empty[r]), PFX_TAKERS); }
     mbar_init(smem_u32(&ctl.met), 256);
     ctl.lock = 0;
     fence_barrier_init();
@@ -474,12 +543,69 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
   const uint32_t tmem = ctl.tmem;
   pdl_wait();
 
-  if (warp >= 8) {
-    registers_down<104>();                 // (a launch gives 384 threads 168 each: 2 x 128 x 200 + 128 x 104 is the same)
+  if (warp >= 12) {
+    registers_down<48>();                  // (a launch gives 512 threads 128 each: 2 x 192 + 80 + 48 is the same)
+    // Zero weights take no part only beside finite values: in blocks that not all rows see whole, rows behind the keys become zeros, and of own keys
+    // infinities and NaN too (what they are to the rows that see them is made up for at the end).
+    const int thread = threadIdx.x & 127;
+    int vn = 0, pieces = 0;
+    each_piece(ctl, lane, [&](const PrefixPiece& x) {
+      if (x.empty) return true;
+#pragma unroll 1
+      for (int j = x.k0; j < x.k1; ++j, ++vn) {
+        const int s = vn % T::V;
+        if (!__all_sync(0xffffffffu, mbar_spin(smem_u32(&ctl.v_full[s]), (uint32_t)(vn / T::V) & 1u, 94))) return false;
+        if (x.cleaned(j)) {
+          const bool prefix = j < x.prefix_blocks;
+          const int in = min(PFX_KEYS, prefix ? x.t.prefix_n - j * PFX_KEYS : x.t.own_n - (j - x.prefix_blocks) * PFX_KEYS);      // keys of the block
+          uint8_t* v = smem_v + s * T::TILE;
+#pragma unroll 1
+          for (int e = in * 8 + thread; e < 1024; e += 128)
+#pragma unroll
+            for (int b = 0; b < DP / 64; ++b) *reinterpret_cast<uint4*>(v + b * T::BOX + e * 16) = make_uint4(0u, 0u, 0u, 0u);
+          if (!prefix) {
+            uint32_t sick = 0u;            // (0 * t is 0 but for those)
+#pragma unroll 4
+            for (int e = 0; e < DP / 64 * 8; ++e) {
+              if (thread + e % 8 * 128 >= in * 8) continue;
+              const uint4 t = *reinterpret_cast<const uint4*>(v + e / 8 * T::BOX + (thread + e % 8 * 128) * 16);
+              sick = fma_zero<BF16>(t.x, sick);
+              sick = fma_zero<BF16>(t.y, sick);
+              sick = fma_zero<BF16>(t.z, sick);
+              sick = fma_zero<BF16>(t.w, sick);
+            }
+            if (half_is_bad<BF16>(sick) || half_is_bad<BF16>(sick >> 16)) {
+              *reinterpret_cast<volatile int*>(&ctl.bad[pieces & 1]) = pieces + 1;
+#pragma unroll 1
+              for (int e = thread; e < in * 8; e += 128)
+#pragma unroll 1
+                for (int b = 0; b < DP / 64; ++b) {
+                  uint32_t* h = reinterpret_cast<uint32_t*>(v + b * T::BOX + e * 16);
+#pragma unroll 1
+                  for (int z = 0; z < 4; ++z) h[z] &= (half_is_bad<BF16>(h[z]) ? 0u : 0xffffu) | (half_is_bad<BF16>(h[z] >> 16) ? 0u : 0xffff0000u);
+                }
+            }
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+        mbar_arrive(smem_u32(&ctl.v_clean[s]));
+        bool fine = true;                  // (its buffer is loaded again only when all have been here)
+        if (thread == 0) {
+          fine = mbar_spin(smem_u32(&ctl.v_clean[s]), (uint32_t)(vn / T::V) & 1u, 94);
+          mbar_arrive(smem_u32(&ctl.v_empty[s]));
+        }
+        if (!__all_sync(0xffffffffu, fine)) return false;
+      }
+      ++pieces;
+      return true;
+    });
+  } else if (warp >= 8) {
+    registers_down<80>();
     if (warp == PFX_LOADER) {
       int qn = 0, kn = 0, vn = 0;          // items and blocks asked for so far
       bool ok = true;
-      each_piece(p, [&](const PrefixPiece& x) {
+      each_piece(ctl, lane, [&](const PrefixPiece& x) {
         if (x.empty) return true;
         const int qs = qn % T::Q;
         if (!(ok = __all_sync(0xffffffffu, mbar_spin(smem_u32(&ctl.q_empty[qs]), ((uint32_t)(qn / T::Q) & 1u) ^ 1u, 81)))) return false;
@@ -491,13 +617,19 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
             for (int b = 0; b < DP / 64; ++b) tma_load_4d(dst + t * T::TILE + b * T::BOX, &map_q, bar, b * 64, 0, x.head, x.t.row0 + t * p.R);
         }
         ++qn;
-        auto load = [&](bool keys, int j) {
+        // keys a block ahead of values
+        const int n = 2 * (x.k1 - x.k0);
+#pragma unroll 1
+        for (int i = 0; i < n + 1; ++i) {
+          // K0, K1, V0, K2, V1, ..: odd places but the first are keys
+          const bool keys = i == 0 || (i & 1) == 1;
+          const int j = x.k0 + (i == 0 ? 0 : keys ? (i + 1) / 2 : i / 2 - 1);
+          if (j >= x.k1) continue;
           const bool prefix = j < x.prefix_blocks;
           const int row = prefix ? x.t.prefix0 + j * PFX_KEYS : x.t.own0 + (j - x.prefix_blocks) * PFX_KEYS;
-          int& n = keys ? kn : vn;
-          const int S = keys ? T::K : T::V, s = n % S;
+          const int s = keys ? kn % T::K : vn % T::V, turn = keys ? kn / T::K : vn / T::V;
           const uint32_t empty = smem_u32(keys ? &ctl.k_empty[s] : &ctl.v_empty[s]), full = smem_u32(keys ? &ctl.k_full[s] : &ctl.v_full[s]);
-          if (!(ok = __all_sync(0xffffffffu, mbar_spin(empty, ((uint32_t)(n / S) & 1u) ^ 1u, keys ? 82 : 83)))) return false;
+          if (!(ok = __all_sync(0xffffffffu, mbar_spin(empty, ((uint32_t)turn & 1u) ^ 1u, keys ? 82 : 83)))) return false;
           if (lane == 0) {
             const uint32_t dst = smem_u32((keys ? smem_k : smem_v) + s * T::TILE);
             const CUtensorMap* map = keys ? (prefix ? &map_pk : &map_k) : (prefix ? &map_pv : &map_v);
@@ -505,13 +637,8 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
 #pragma unroll
             for (int b = 0; b < DP / 64; ++b) tma_load_3d(dst + b * T::BOX, map, full, b * 64, x.head, row);
           }
-          ++n;
-          return true;
-        };
-        if (!load(true, x.k0)) return false;
-        for (int j = x.k0; j < x.k1; ++j) {
-          if (j + 1 < x.k1 && !load(true, j + 1)) return false;
-          if (!load(false, j)) return false;
+          kn += keys;
+          vn += !keys;
         }
         return true;
       });
@@ -519,6 +646,24 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         for (int i = 1; i <= T::Q && i <= qn; ++i) mbar_spin(smem_u32(&ctl.q_full[(qn - i) % T::Q]), (uint32_t)((qn - i) / T::Q) & 1u, 84);
         for (int i = 1; i <= T::K && i <= kn; ++i) mbar_spin(smem_u32(&ctl.k_full[(kn - i) % T::K]), (uint32_t)((kn - i) / T::K) & 1u, 84);
         for (int i = 1; i <= T::V && i <= vn; ++i) mbar_spin(smem_u32(&ctl.v_full[(vn - i) % T::V]), (uint32_t)((vn - i) / T::V) & 1u, 84);
+      }
+    } else if (warp == PFX_MMA + 2) {
+      int n = 0;
+      bool ok = true;
+      auto put = [&](const PrefixPiece& x) {
+        if (!(ok = __all_sync(0xffffffffu, mbar_spin(smem_u32(&ctl.piece_empty[n % PFX_RING]), ((uint32_t)(n / PFX_RING) & 1u) ^ 1u, 79)))) return false;
+        if (lane == 0) {
+          ctl.ring[n % PFX_RING] = x;
+          mbar_arrive(smem_u32(&ctl.piece_full[n % PFX_RING]));
+        }
+        __syncwarp();
+        ++n;
+        return true;
+      };
+      make_pieces(p, put);
+      if (ok) {
+        PrefixPiece none = {};
+        put(none);
       }
     } else if (warp < PFX_MMA + 2) {
       // A warp for each group. Where a group's weights lie over its scores, its product and the scores after it are asked for at a stretch, one group
@@ -532,7 +677,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       int on = 0;                                          // its products so far
       bool ok = true;
       auto wait = [&](uint64_t* bar, int phase, int site) { return ok = __all_sync(0xffffffffu, mbar_spin(smem_u32(bar), (uint32_t)phase & 1u, site)); };
-      each_piece(p, [&](const PrefixPiece& x) {
+      each_piece(ctl, lane, [&](const PrefixPiece& x) {
         if (x.empty) return true;
         const int qs = qn % T::Q, k_first = kn, v_first = vn;
         if (!wait(&ctl.q_full[qs], qn / T::Q, 85)) return false;
@@ -541,6 +686,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         // only where a block or two lie between: a loader that waits for buffers of values loads no keys either).
         auto give_back = [&](int j, bool values) {
           const int n = j - x.k0;
+#pragma unroll 1
           while (kn - k_first < n || (values && vn - v_first < n)) {
             if (kn - k_first < n) {
               if (!wait(&ctl.k_full[kn % T::K], kn / T::K, 86)) return false;
@@ -556,57 +702,60 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
           return true;
         };
         auto keys_of = [&](int j, bool values) { return give_back(j, values) && wait(&ctl.k_full[kn % T::K], kn / T::K, 86); };
-        auto scores = [&]() {              // of the block whose keys are there
-          const int s = kn % T::K;
-          // (a descriptor's address counts 16 bytes: a step of 16 elements is 2, a box of 64 columns 1024)
-          const uint64_t k = make_desc_sw128(uniform(smem_u32(smem_k + s * T::TILE)), 1024);
-          tc_fence_after_sync();
-#pragma unroll
-          for (int kk = 0; kk < DP / 16; ++kk)
-            mma_f16_ss_elect(to_s, q + (kk / 4) * (T::BOX / 16) + (kk % 4) * 2, k + (kk / 4) * (T::BOX / 16) + (kk % 4) * 2, idesc_s, kk > 0 ? 1u : 0u);
-          mma_commit_elect(smem_u32(&ctl.s_full[w]));
-          mma_commit_elect(smem_u32(&ctl.k_empty[s]));
-          ++kn;
-        };
-        int j = x.next(w, x.k0);
+        // The blocks in order, a step behind: scores of block `ask`, then the product with the weights of the block before it. Where these lie over the
+        // scores, the product comes first.
+        const int end = x.of(w).end;
+        int ask = x.of(w).begin, j = end;                // (j: the block whose weights come next; none yet)
         bool first = true;
-        if (j < x.k1) {
-          if (!keys_of(j, true)) return false;
-          scores();
-        }
-        while (j < x.k1) {
-          const int then = x.next(w, j + 1);
-          const bool near = then < x.k1 && then - j <= 2;  // (else the loader may wait for this block's values to be done with)
-          if (near) {
-            if (!keys_of(then, false)) return false;
-            if (T::APART) {                // the next scores, as soon as these have been read
-              if (!wait(&ctl.s_read[w], on, 87)) return false;
-              scores();
+#pragma unroll 1
+        while (ask < end || j < end) {
+          // a block further on than two: the loader may wait for this block's values to be done with
+          const bool near = j >= end || ask - j <= 2;
+          const bool product_first = j < end && (!T::APART || !near || ask >= end);
+          bool held = false;
+#pragma unroll 1
+          for (int turn = 0; turn < 2; ++turn) {
+            if ((turn == 0) == product_first) {
+              if (j >= end) continue;
+              if (near && ask < end && product_first && !keys_of(ask, false)) return false;
+              if (!give_back(j, true)) return false;
+              const int s = vn % T::V;
+              const uint64_t v = make_desc_sw128_mn(uniform(smem_u32(smem_v + s * T::TILE)), T::BOX);
+              if (!wait(x.cleaned(j) ? &ctl.v_clean[s] : &ctl.v_full[s], vn / T::V, 89)) return false;
+              if (first && pieces > 0 && !wait(&ctl.o_free[w], pieces - 1, 90)) return false;
+              if (!wait(&ctl.p_ready[w], on, 88)) return false;
+              if (!T::APART && !(ok = held = take(&ctl.lock, lane))) return false;
+              tc_fence_after_sync();
+#pragma unroll
+              for (int kk = 0; kk < PFX_KEYS / 16; ++kk) mma_f16_ts_elect(to_o, from_p + kk * 8, v + kk * 128, idesc_o, (!first || kk > 0) ? 1u : 0u);
+              mma_commit_elect(smem_u32(&ctl.o_done[w]));
+              mma_commit_elect(smem_u32(&ctl.v_empty[s]));
+              ++vn;
+              ++on;
+              first = false;
+              if (held && !near) {
+                let_go(&ctl.lock, lane);
+                held = false;
+              }
+            } else if (ask < end) {
+              if (!held && !keys_of(ask, j >= end || !near)) return false;
+              if (T::APART && j < end && !product_first && !wait(&ctl.s_read[w], on, 87)) return false;      // (the scores before these have been read)
+              const int s = kn % T::K;
+              // (a descriptor's address counts 16 bytes: a step of 16 elements is 2, a box of 64 columns 1024)
+              const uint64_t k = make_desc_sw128(uniform(smem_u32(smem_k + s * T::TILE)), 1024);
+              tc_fence_after_sync();
+              // Scores over weights that the product before them reads: MMAs of one thread and shape are executed in the order of their issue.
+#pragma unroll
+              for (int kk = 0; kk < DP / 16; ++kk)
+                mma_f16_ss_elect(to_s, q + (kk / 4) * (T::BOX / 16) + (kk % 4) * 2, k + (kk / 4) * (T::BOX / 16) + (kk % 4) * 2, idesc_s, kk > 0 ? 1u : 0u);
+              mma_commit_elect(smem_u32(&ctl.s_full[w]));
+              mma_commit_elect(smem_u32(&ctl.k_empty[s]));
+              ++kn;
             }
           }
-          if (!give_back(j, true)) return false;
-          const int s = vn % T::V;
-          const uint64_t v = make_desc_sw128_mn(uniform(smem_u32(smem_v + s * T::TILE)), T::BOX);
-          if (!wait(&ctl.v_full[s], vn / T::V, 89)) return false;
-          if (first && pieces > 0 && !wait(&ctl.o_free[w], pieces - 1, 90)) return false;
-          if (!wait(&ctl.p_ready[w], on, 88)) return false;
-          if (!T::APART && !(ok = take(&ctl.lock, lane))) return false;
-          tc_fence_after_sync();
-#pragma unroll
-          for (int kk = 0; kk < PFX_KEYS / 16; ++kk) mma_f16_ts_elect(to_o, from_p + kk * 8, v + kk * 128, idesc_o, (!first || kk > 0) ? 1u : 0u);
-          mma_commit_elect(smem_u32(&ctl.o_done[w]));
-          mma_commit_elect(smem_u32(&ctl.v_empty[s]));
-          ++vn;
-          ++on;
-          first = false;
-          // Scores over weights that the product before them reads: MMAs of one thread and shape are executed in the order of their issue.
-          if (!T::APART && near) scores();
-          if (!T::APART) let_go(&ctl.lock, lane);
-          if (!near && then < x.k1) {
-            if (!keys_of(then, true)) return false;
-            scores();
-          }
-          j = then;
+          if (held) let_go(&ctl.lock, lane);
+          j = ask;
+          if (ask < end) ask = x.next(w, ask);
         }
         if (!give_back(x.k1, true)) return false;
         if (first) {
@@ -624,36 +773,51 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       }
     }
   } else {
-    registers_up<200>();
+    registers_up<192>();
     const int w = warp >> 2, row = threadIdx.x & 127;
     const uint32_t lanes = (uint32_t)(warp & 3) * 32u << 16;
     const uint32_t my_s = tmem + T::S + w * 128 + lanes, my_p = tmem + T::P + w * T::P_STEP + lanes, my_o = tmem + T::O + w * DP + lanes;
-    int sn = 0, seq = 0, pieces = 0, mets = 0;             // this group's blocks; the CTA's; pieces with keys; meetings of the groups
+    int sn = 0, pieces = 0, mets = 0;      // this group's blocks; pieces with keys; meetings of the groups
     int other = 0;                                         // the other group's blocks
     int slots = 0;
     auto wait = [&](uint64_t* bar, int phase, int site) { return __all_sync(0xffffffffu, mbar_spin(smem_u32(bar), (uint32_t)phase & 1u, site)); };
-    each_piece(p, [&](const PrefixPiece& x) {
+    each_piece(ctl, lane, [&](const PrefixPiece& x) {
       const int tile = x.two ? w : 0, tile_row = tile * p.R + row / p.share;
       const bool there = row < p.R * p.share && tile_row < x.t.rows;
       const int64_t q_row = (int64_t)x.t.row0 + tile_row;
       const int q_head = x.head * p.share + row % p.share;
-      // The own keys that the row sees, counted from the item's first: read when the first block is out of hand.
+      // The own keys that the row sees, counted from the item's first. Where its list needs no search the offsets are read now and used when the first
+      // own block comes; else when the first block is out of hand.
       int lo = 0, hi = 0;
       bool known = x.t.own_n == 0;
+      const int list_a = tile ? x.t.list[2] : x.t.list[0], list_b = tile ? x.t.list[3] : x.t.list[1];
+      const int list = !p.lists.offsets ? (int)((uint32_t)q_row / (uint32_t)p.lists.per) : list_a == list_b ? list_a : -1;
+      const bool early = there && !known && list >= 0 && list < p.lists.batch;
+      int raw_own[2] = {0, 0}, raw_behind = 0;             // (as they stand in memory: nothing is made of them before they are needed)
+      if (early) {
+        if (p.own.offsets) { raw_own[0] = p.own.offsets[list]; raw_own[1] = p.own.offsets[list + 1]; }
+        if (p.lists.offsets) raw_behind = p.lists.offsets[list + 1];
+      }
       auto know = [&]() {
         known = true;
-        if (there) {
-          int64_t a, b;
-          own_of(p, q_row, list_of(p.lists, q_row, tile ? x.t.list[2] : x.t.list[0], tile ? x.t.list[3] : x.t.list[1]), a, b);
-          lo = (int)min(max(a - x.t.own0, (int64_t)0), (int64_t)x.t.own_n);
-          hi = (int)min(max(b - x.t.own0, (int64_t)0), (int64_t)x.t.own_n);
+        if (early) {
+          auto cut = [](const Lists& of, int raw, int i) { return of.offsets ? min(max((int64_t)raw, (int64_t)0), of.rows) : (int64_t)i * of.per; };
+          const int64_t begin = cut(p.own, raw_own[0], list), last = cut(p.own, raw_own[1], list + 1) - max(cut(p.lists, raw_behind, list + 1) - 1 - q_row, (int64_t)0);
+          lo = (int)min(max(begin - x.t.own0, (int64_t)0), (int64_t)x.t.own_n);
+          hi = (int)min(max(max(last, begin) - x.t.own0, (int64_t)0), (int64_t)x.t.own_n);
+        } else if (there) {
+          const int2 keys = row_keys(p, (int)q_row, list_a, list_b, x.t.own0, x.t.own_n);
+          lo = keys.x;
+          hi = keys.y;
         }
         __syncwarp();
       };
       float m = -INFINITY, l = 0.f;
       int mine = 0;
       if (!x.empty) {
-        for (int j = x.next(w, x.k0); j < x.k1; j = x.next(w, j + 1), ++mine) {
+        const int end = x.of(w).end;
+#pragma unroll 1
+        for (int j = x.of(w).begin; j < end; j = x.next(w, j), ++mine) {
           const bool prefix = j < x.prefix_blocks;
           const int key0 = (prefix ? j : j - x.prefix_blocks) * PFX_KEYS;
           const int in = min(PFX_KEYS, (prefix ? x.t.prefix_n : x.t.own_n) - key0);           // keys of the block
@@ -661,10 +825,6 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
           if (masked && !prefix && !known) know();
           if (!wait(&ctl.s_full[w], sn, 92)) return false;
           tc_fence_after_sync();
-          // Blocks that all rows see whole: the scores stay in registers. Others go by quarters of 32 keys, read once for the maximum and once for the
-          // weights, and quarters in which no row of the warp sees a key by zeros alone (a word has a bit a key that the row sees).
-          const int c0 = prefix ? 0 : max(lo - key0, 0), c1 = prefix ? in : min(hi - key0, in);
-          auto quarter = [&](int c) { return bits_below(c1 - 32 * c) & ~bits_below(c0 - 32 * c); };
           // Sums so far are moved to a maximum that has grown. (m is -infinity: nothing has been summed; no maximum yet: nothing to move.)
           auto move_sums = [&](float next) {
             if (__any_sync(0xffffffffu, (next - m) * p.scale > PFX_GROWTH)) {
@@ -703,7 +863,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
               to[e / 2] = pack_weights<BF16>(a, b);
             }
           };
-          if (!masked) {
+          if (!masked || prefix) {
             uint32_t s[4][32];
 #pragma unroll
             for (int c = 0; c < 4; ++c) tmem_ld32_nowait(my_s + c * 32, s[c]);
@@ -713,9 +873,18 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
               tc_fence_before_sync();
               mbar_arrive(smem_u32(&ctl.s_read[w]));
             }
+            if (masked) {                  // (a prefix's last keys: the same for all rows)
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                if (in >= 32 * c + 32) continue;
+                const uint32_t seen = bits_below(in - 32 * c);
+#pragma unroll
+                for (int e = 0; e < 32; ++e) s[c][e] = seen >> e & 1 ? s[c][e] : 0xff800000u;
+              }
+            }
             float top[4] = {m, m, m, m};
 #pragma unroll
-            for (int c = 0; c < 128; ++c) top[c % 4] = fmaxf(top[c % 4], __uint_as_float(s[c / 32][c % 32]));
+            for (int c = 0; c < 128; c += 2) top[c / 2 % 4] = fmaxf(top[c / 2 % 4], fmaxf(__uint_as_float(s[c / 32][c % 32]), __uint_as_float(s[c / 32][c % 32 + 1])));
             if (!move_sums(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])))) return false;
             float base = m == -INFINITY ? 0.f : m * p.scale;
             if (__any_sync(0xffffffffu, fabsf(base) > 1e6f)) {
@@ -731,6 +900,10 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
               tmem_st16(my_p + c * 16, weights);
             }
           } else {
+            // By quarters of 32 keys, read once for the maximum and once for the weights; those in which no row of the warp sees a key are left out, and
+            // their weights are zero. A word has a bit a key that the row sees.
+            const int c0 = max(lo - key0, 0), c1 = min(hi - key0, in);
+            auto quarter = [&](int c) { return bits_below(c1 - 32 * c) & ~bits_below(c0 - 32 * c); };
             float next = m;
 #pragma unroll 1
             for (int c = 0; c < 4; ++c) {
@@ -739,8 +912,10 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
               uint32_t q[32];
               tmem_ld32_nowait(my_s + c * 32, q);
               tmem_wait_ld(q);
+              float top[2] = {next, next};
 #pragma unroll
-              for (int e = 0; e < 32; ++e) next = fmaxf(next, seen >> e & 1 ? __uint_as_float(q[e]) : -INFINITY);
+              for (int e = 0; e < 32; ++e) top[e % 2] = fmaxf(top[e % 2], seen >> e & 1 ? __uint_as_float(q[e]) : -INFINITY);
+              next = fmaxf(top[0], top[1]);
             }
             if (!move_sums(next)) return false;
             const float off = m == -INFINITY ? 0.f : m;
@@ -769,41 +944,6 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
           unpack2(sum[0], sums[0], sums[1]);
           unpack2(sum[1], sums[2], sums[3]);
           l += (sums[0] + sums[1]) + (sums[2] + sums[3]);
-          if (masked) {
-            // Zero weights take no part only beside finite values: rows behind the keys become zeros, and where rows see different keys, infinities
-            // and NaN too (what they are to the rows that see them is made up for at the end; both groups may find and write the same).
-            const int at = seq + j - x.k0, vs = at % T::V;
-            if (!wait(&ctl.v_full[vs], at / T::V, 94)) return false;
-            uint8_t* v = smem_v + vs * T::TILE;
-            for (int e = in * 8 + row; e < 1024; e += 128)
-#pragma unroll
-              for (int b = 0; b < DP / 64; ++b) *reinterpret_cast<uint4*>(v + b * T::BOX + e * 16) = make_uint4(0u, 0u, 0u, 0u);
-            if (!prefix) {
-              // (0 * t is 0 but for those)
-              uint32_t sick = 0u;
-#pragma unroll
-              for (int e = 0; e < DP / 64 * 8; ++e) {
-                if (row + e % 8 * 128 >= in * 8) continue;
-                const uint4 t = *reinterpret_cast<const uint4*>(v + e / 8 * T::BOX + (row + e % 8 * 128) * 16);
-                sick = fma_zero<BF16>(t.x, sick);
-                sick = fma_zero<BF16>(t.y, sick);
-                sick = fma_zero<BF16>(t.z, sick);
-                sick = fma_zero<BF16>(t.w, sick);
-              }
-              if (half_is_bad<BF16>(sick) || half_is_bad<BF16>(sick >> 16)) {
-                // (told ahead of the writes: who finds zeros there finds this too)
-                *reinterpret_cast<volatile int*>(&ctl.bad[pieces & 1]) = pieces + 1;
-                __threadfence_block();
-                for (int e = row; e < in * 8; e += 128)
-                  for (int b = 0; b < DP / 64; ++b) {
-                    uint32_t* h = reinterpret_cast<uint32_t*>(v + b * T::BOX + e * 16);
-                    for (int z = 0; z < 4; ++z) h[z] &= (half_is_bad<BF16>(h[z]) ? 0u : 0xffffu) | (half_is_bad<BF16>(h[z] >> 16) ? 0u : 0xffff0000u);
-                  }
-              }
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
-          }
           tmem_wait_st();
           tc_fence_before_sync();
           mbar_arrive(smem_u32(&ctl.p_ready[w]));
@@ -813,15 +953,10 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       }
       // What a thread has of its row: all columns of a tile of its own, half of them of a tile that both groups share.
       float f[2] = {1.f, 0.f}, top = m, all = l;
-      int of[2] = {w, w ^ 1};                              // whose sums; a tile of its own has the first alone
       bool bad = false, have[2] = {mine > 0, false};
       if (!x.empty) {
         const int theirs = other;
-        if (x.two) {
-          for (int j = x.next(w ^ 1, x.k0); j < x.k1; j = x.next(w ^ 1, j + 1)) ++other;
-        } else {
-          other += (x.k1 - x.k0 + w) / 2;
-        }
+        other += x.of(w ^ 1).n;
         if (!x.two) {
           // (what stands there of the piece before has been read)
           if (pieces > 0 && !wait(&ctl.o_free[w], pieces - 1, 98)) return false;
@@ -857,28 +992,15 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         float o[32];
 #pragma unroll
         for (int e = 0; e < 32; ++e) o[e] = 0.f;
-#pragma unroll
+#pragma unroll 1
         for (int h = 0; h < 2; ++h) {
-          if (!have[h]) continue;
+          if (!(h ? have[1] : have[0])) continue;
+          const float times = (h ? f[1] : f[0]) * by;
           uint32_t a[32];
-          tmem_ld32_nowait(tmem + T::O + of[h] * DP + lanes + c0, a);
+          tmem_ld32_nowait(tmem + T::O + (w ^ h) * DP + lanes + c0, a);
           tmem_wait_ld(a);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = fmaf(__uint_as_float(a[e]), f[h], o[e]);
-        }
-#pragma unroll
-        for (int e = 0; e < 32; ++e) o[e] *= by;
-        if (there && bad) {                                // infinities and NaN among the own values that the row sees in these blocks
-          const int k_lo = max(lo, max(x.k0 - x.prefix_blocks, 0) * PFX_KEYS), k_hi = min(hi, (x.k1 - x.prefix_blocks) * PFX_KEYS);
-          for (int k = k_lo; k < k_hi; ++k) {
-            const uint16_t* v = p.v.get<uint16_t>((int64_t)x.t.own0 + k, x.head);
-#pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              if (c0 + e >= p.d) break;
-              const uint16_t t = v[c0 + e];
-              if (half_is_bad<BF16>(t)) o[e] += BF16 ? __uint_as_float((uint32_t)t << 16) : __half2float(__ushort_as_half(t));
-            }
-          }
+          for (int e = 0; e < 32; ++e) o[e] = fmaf(__uint_as_float(a[e]), times, o[e]);
         }
         if (x.whole && (there || staged)) {
 #pragma unroll
@@ -908,13 +1030,28 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       }
       if (staged) {
         uint16_t* mine_y = const_cast<uint16_t*>(p.y.get<uint16_t>(q_row, q_head));
-        const int from = c_begin / 8, n = (min(c_end, p.d) + 7) / 8 - from, first_row = (warp & 3) * 32;
-        for (int i = 0; i < n; ++i) {
-          const int e = i * 32 + lane, r = e / n, c = from + e - r * n;
-          uint16_t* to = reinterpret_cast<uint16_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine_y), r));
-          const bool is = __shfl_sync(0xffffffffu, (int)there, r) != 0;
-          if (is) *reinterpret_cast<uint4*>(to + c * 8) = stage[(first_row + r) * (DP / 8) + (c ^ (r & 7))];
-        }
+        auto copy_out = [&](auto width) {
+          constexpr int N = decltype(width)::value;        // pieces of a row that are here
+          const int from = c_begin / 8, n = (min(c_end, p.d) + 7) / 8 - from, first_row = (warp & 3) * 32;
+#pragma unroll 2
+          for (int i = 0; i < N; ++i) {
+            const int e = i * 32 + lane, r = e / N, c = from + e % N;
+            uint16_t* to = reinterpret_cast<uint16_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine_y), r));
+            const bool is = __shfl_sync(0xffffffffu, (int)there, r) != 0 && c < from + n;
+            if (is) *reinterpret_cast<uint4*>(to + c * 8) = stage[(first_row + r) * (DP / 8) + (c ^ (r & 7))];
+          }
+        };
+        __syncwarp();
+        if (x.two) copy_out(std::integral_constant<int, DP / 8>());
+        else copy_out(std::integral_constant<int, DP / 16>());
+      }
+      if (bad) {                           // (behind what the warp's lanes have stored)
+        __syncwarp();
+        const int k_lo = max(lo, max(x.k0 - x.prefix_blocks, 0) * PFX_KEYS), k_hi = min(hi, (x.k1 - x.prefix_blocks) * PFX_KEYS);
+        if (there && k_lo < k_hi)
+          spread_bad<BF16>(p.v, x.t.own0, x.head, c_begin, min(c_end, p.d), k_lo, k_hi, x.whole ? const_cast<uint16_t*>(p.y.get<uint16_t>(q_row, q_head)) : nullptr,
+                           reinterpret_cast<float*>(p.part + (int64_t)slot * (p.d / 4) * p.part_rows + part_row), (int64_t)p.part_rows * 4);
+        __syncwarp();
       }
       if (!x.whole) {
         if (there && (x.two || w == 0)) p.part_ml[(int64_t)slot * p.part_rows + part_row] = make_float2(top, all);
@@ -932,12 +1069,12 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&ctl.q_empty[qs]));
-        seq += x.k1 - x.k0;
         ++pieces;
       }
       return true;
     });
     if (threadIdx.x == 0)
+#pragma unroll 1
       for (; slots < PFX_SLOTS; ++slots) p.records[blockIdx.x * PFX_SLOTS + slots] = {-1, 0, 0, 0};
   }
   tc_fence_before_sync();
@@ -959,38 +1096,46 @@ __global__ void __launch_bounds__(JOIN_THREADS) prefix_join_kernel(const PrefixP
   __shared__ int s_first[JOIN_MOST / 2], s_rows[JOIN_MOST / 2], s_ends[JOIN_MOST / 2];
   __shared__ int s_slot[JOIN_MOST], s_sorted[JOIN_MOST], s_n;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, records = p.ctas * PFX_SLOTS;
+#pragma unroll 1
   for (int i = threadIdx.x; i < records; i += JOIN_THREADS) {
     const PrefixRecord o = p.records[i];
     s_item[i] = o.item; s_head[i] = o.head; s_unit[i] = o.unit;
   }
   __syncthreads();
-  if (warp == 0) {                       
-    int n = 0;
-    for (int i = lane; i - lane < records; i += 32) {
-      const bool first = i < records && s_item[i] >= 0 && s_unit[i] == 0;
-      const unsigned mask = __ballot_sync(0xffffffffu, first);
-      const int at = n + __popc(mask & ((1u << lane) - 1));
-      if (first && at < JOIN_MOST / 2) s_first[at] = i;
-      n += __popc(mask);
+  // the items' first pieces, in the order of their places (the same in every block)
+  if (threadIdx.x == 0) s_n = 0;
+  __syncthreads();
+#pragma unroll 1
+  for (int i = threadIdx.x; i < records; i += JOIN_THREADS)
+    if (s_item[i] >= 0 && s_unit[i] == 0) {
+      const int at = atomicAdd(&s_n, 1);
+      if (at < JOIN_MOST / 2) s_slot[at] = i;              // (a cut item has two records or more)
     }
-    __syncwarp();
+  __syncthreads();
+  for (int i = threadIdx.x; i < min(s_n, JOIN_MOST / 2); i += JOIN_THREADS) {
+    int before = 0;
+#pragma unroll 1
+    for (int o = 0; o < min(s_n, JOIN_MOST / 2); ++o) before += s_slot[o] < s_slot[i];
+    s_first[before] = s_slot[i];
+    s_rows[before] = p.items[s_item[s_slot[i]]].rows * p.share;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    const int n = min(s_n, JOIN_MOST / 2), cols = (p.d + 15) / 16;
     int ends = 0;
-    const int cols = (p.d + 15) / 16;
     for (int i = lane; i - lane < n; i += 32) {
-      const int rows = i < n ? p.items[s_item[s_first[i]]].rows * p.share : 0;
-      int x = (rows + 31) / 32 * cols;
+      int x = i < n ? (s_rows[i] + 31) / 32 * cols : 0;
 #pragma unroll
       for (int o = 1; o < 32; o *= 2) {
         const int t = __shfl_up_sync(0xffffffffu, x, o);
         if (lane >= o) x += t;
       }
-      if (i < n) { s_rows[i] = rows; s_ends[i] = ends + x; }
+      if (i < n) s_ends[i] = ends + x;
       ends += __shfl_sync(0xffffffffu, x, 31);
     }
-    if (lane == 0) s_n = n;
   }
   __syncthreads();
-  const int firsts = s_n, all_units = firsts > 0 ? s_ends[firsts - 1] : 0;
+  const int firsts = min(s_n, JOIN_MOST / 2), all_units = firsts > 0 ? s_ends[firsts - 1] : 0;
   int held = -1, n = 0;
   for (int u = blockIdx.x; u < all_units; u += gridDim.x) {
     int k = 0;
@@ -1001,12 +1146,14 @@ __global__ void __launch_bounds__(JOIN_THREADS) prefix_join_kernel(const PrefixP
       __syncthreads();
       if (threadIdx.x == 0) s_n = 0;
       __syncthreads();
+#pragma unroll 1
       for (int i = threadIdx.x; i < records; i += JOIN_THREADS)
         if (s_item[i] == item && s_head[i] == head) s_slot[atomicAdd(&s_n, 1)] = i;
       __syncthreads();
       n = s_n;
       for (int i = threadIdx.x; i < n; i += JOIN_THREADS) {
         int before = 0;
+#pragma unroll 1
         for (int o = 0; o < n; ++o) before += s_unit[s_slot[o]] < s_unit[s_slot[i]];
         s_sorted[before] = s_slot[i];
       }
@@ -1014,9 +1161,8 @@ __global__ void __launch_bounds__(JOIN_THREADS) prefix_join_kernel(const PrefixP
     }
     const int row = in % row_blocks * 32 + lane, col = in / row_blocks * 16 + warp * 4;
     if (row >= s_rows[k] || col >= p.d) continue;
+    // (sums so far, and what the next piece moves them by)
     float top = -INFINITY, all = 0.f;
-#pragma unroll 8
-    for (int i = 0; i < n; ++i) top = fmaxf(top, p.part_ml[(int64_t)s_sorted[i] * p.part_rows + row].x);
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int i0 = 0; i0 < n; i0 += JOIN_AHEAD) {
       float4 v[JOIN_AHEAD];
@@ -1030,9 +1176,11 @@ __global__ void __launch_bounds__(JOIN_THREADS) prefix_join_kernel(const PrefixP
 #pragma unroll
       for (int i = 0; i < JOIN_AHEAD; ++i) {
         if (i0 + i >= n) break;
-        const float f = ml[i].x == -INFINITY ? 0.f : ex2((ml[i].x - top) * p.scale);
-        all = fmaf(ml[i].y, f, all);
-        o.x = fmaf(v[i].x, f, o.x); o.y = fmaf(v[i].y, f, o.y); o.z = fmaf(v[i].z, f, o.z); o.w = fmaf(v[i].w, f, o.w);
+        const float next = fmaxf(top, ml[i].x);
+        const float f = ml[i].x == -INFINITY ? 0.f : ex2((ml[i].x - next) * p.scale), back = top == next || top == -INFINITY ? 1.f : ex2((top - next) * p.scale);
+        top = next;
+        all = fmaf(ml[i].y, f, all * back);
+        o.x = fmaf(v[i].x, f, o.x * back); o.y = fmaf(v[i].y, f, o.y * back); o.z = fmaf(v[i].z, f, o.z * back); o.w = fmaf(v[i].w, f, o.w * back);
       }
     }
     const float by = all > 0.f ? 1.f / all : all;
