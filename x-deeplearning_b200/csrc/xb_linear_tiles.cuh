@@ -59,6 +59,15 @@ __device__ __forceinline__ float warp_top(float v) {
   return v;
 }
 
+// (several at once: their shuffles wait beside one another)
+template <int N>
+__device__ __forceinline__ void warp_tops(float (&v)[N]) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+    for (int z = 0; z < N; ++z) v[z] = fmaxf(v[z], __shfl_xor_sync(0xffffffffu, v[z], o));
+}
+
 // The largest of a warp's sizes, told by `each`, which calls its argument with every value of a lane. Infinities have no say in it: they are what
 // they are at any scale, and the finite values beside them keep theirs.
 template <typename F>
@@ -198,62 +207,104 @@ __global__ void __launch_bounds__(LinearTiles<BF16, DK, DV>::THREADS, LinearTile
     umma::cp_async_wait_all();
     __syncthreads();
     if (!p.ends_only) {
-      // scores, times the decay: ten blocks of 16 x 16 on and below the diagonal
-      for (int b = warp; b < 10; b += L::WARPS) {
-        const int i = b < 1 ? 0 : b < 3 ? 1 : b < 6 ? 2 : 3, j = b - i * (i + 1) / 2;
-        if (16 * i >= n) break;
-        float c[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+      // scores, times the decay: ten blocks of 16 x 16 on and below the diagonal, those of a warp side by side
+      const int row_blocks = (n + 15) / 16, blocks = row_blocks * (row_blocks + 1) / 2;
+      auto scores = [&](auto count) {
+        constexpr int N = decltype(count)::value;
+        float c[N][2][4];
+        uint32_t at_q[N], at_k[N];
+        int back[N];                       // blocks between
+#pragma unroll
+        for (int z = 0; z < N; ++z) {
+          const int b = warp + z * L::WARPS, i = b < 1 ? 0 : b < 3 ? 1 : b < 6 ? 2 : 3, j = b - i * (i + 1) / 2;
+          at_q[z] = sq + 16 * i * DK * 2;
+          at_k[z] = sk + 16 * j * DK * 2;
+          back[z] = i - j;
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) c[z][x][e] = 0.f;
+        }
 #pragma unroll
         for (int k = 0; k < DK / 16; ++k) {
-          uint32_t a[4], bk[4];
-          ldmatrix4<0>(a, sq + tile_at<DK>(16 * i + (lane & 15), 2 * k + (lane >> 4)));
-          ldmatrix4<0>(bk, sk + tile_at<DK>(16 * j + (lane & 15), 2 * k + (lane >> 4)));
-          mma_add<BF16>(c[0], a, bk[0], bk[2]);
-          mma_add<BF16>(c[1], a, bk[1], bk[3]);
-        }
-        if (i == j) {
+          const uint32_t at = tile_at<DK>(lane & 15, 2 * k + (lane >> 4));
+          uint32_t a[N][4], bk[N][4];
 #pragma unroll
-          for (int x = 0; x < 2; ++x)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int back = g8 + (e >> 1) * 8 - 8 * x - 2 * t4 - (e & 1);
-              c[x][e] = back >= 0 ? c[x][e] * s_power[max(back, 0)] : 0.f;
-            }
-        } else {
-          const float far = s_power[16 * (i - j - 1)];
-#pragma unroll
-          for (int x = 0; x < 2; ++x)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) c[x][e] *= row_f[e >> 1] * far * col_f[x][e & 1];
-        }
-        if constexpr (!BF16) {
-          float up, down;
-          fp16_scale(top_of([&](auto take) {
-#pragma unroll
-                       for (int x = 0; x < 2; ++x)
-#pragma unroll
-                         for (int e = 0; e < 4; ++e) take(c[x][e]);
-                     }),
-                     up, down);
-          if (lane == 0) s_block[b] = down;
-#pragma unroll
-          for (int x = 0; x < 2; ++x)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) c[x][e] *= up;
-        }
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-#pragma unroll
-          for (int e = 0; e < 4; e += 2) {
-            const uint32_t at = score_at(b, g8 + (e >> 1) * 8, x) + 4 * t4;
-            const uint32_t hi = narrow<BF16>(c[x][e], c[x][e + 1]);
-            *reinterpret_cast<uint32_t*>(s_scores + at) = hi;
-            if constexpr (BF16) {
-              const float2 taken = widen<BF16>(hi);
-              *reinterpret_cast<uint32_t*>(s_scores + L::SCORES + at) = narrow<BF16>(c[x][e] - taken.x, c[x][e + 1] - taken.y);
-            }
+          for (int z = 0; z < N; ++z) {
+            ldmatrix4<0>(a[z], at_q[z] + at);
+            ldmatrix4<0>(bk[z], at_k[z] + at);
           }
+#pragma unroll
+          for (int z = 0; z < N; ++z) {
+            mma_add<BF16>(c[z][0], a[z], bk[z][0], bk[z][2]);
+            mma_add<BF16>(c[z][1], a[z], bk[z][1], bk[z][3]);
+          }
+        }
+        float tops[N];
+#pragma unroll
+        for (int z = 0; z < N; ++z) {
+          if (back[z] == 0) {
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int rows = g8 + (e >> 1) * 8 - 8 * x - 2 * t4 - (e & 1);
+                c[z][x][e] = rows >= 0 ? c[z][x][e] * s_power[max(rows, 0)] : 0.f;
+              }
+          } else {
+            const float far = s_power[16 * (back[z] - 1)];
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) c[z][x][e] *= row_f[e >> 1] * far * col_f[x][e & 1];
+          }
+          tops[z] = 0.f;
+          if constexpr (!BF16) {
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) tops[z] = fmaxf(tops[z], fabsf(c[z][x][e]));
+          }
+        }
+        if constexpr (!BF16) warp_tops(tops);
+#pragma unroll
+        for (int z = 0; z < N; ++z) {
+          const int b = warp + z * L::WARPS;
+          if constexpr (!BF16) {
+            auto each = [&](auto take) {
+#pragma unroll
+              for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) take(c[z][x][e]);
+            };
+            float up, down;
+            fp16_scale(tops[z] == INFINITY ? top_of(each) : tops[z], up, down);
+            if (lane == 0) s_block[b] = down;
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) c[z][x][e] *= up;
+          }
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int e = 0; e < 4; e += 2) {
+              const uint32_t at = score_at(b, g8 + (e >> 1) * 8, x) + 4 * t4;
+              const uint32_t hi = narrow<BF16>(c[z][x][e], c[z][x][e + 1]);
+              *reinterpret_cast<uint32_t*>(s_scores + at) = hi;
+              if constexpr (BF16) {
+                const float2 taken = widen<BF16>(hi);
+                *reinterpret_cast<uint32_t*>(s_scores + L::SCORES + at) = narrow<BF16>(c[z][x][e] - taken.x, c[z][x][e + 1] - taken.y);
+              }
+            }
+        }
+      };
+      const int mine = warp < blocks ? (blocks - warp + L::WARPS - 1) / L::WARPS : 0;
+      if constexpr (L::WARPS < 5) {
+        if (mine == 3) scores(std::integral_constant<int, 3>());
       }
+      if (mine == 2) scores(std::integral_constant<int, 2>());
+      if (mine == 1) scores(std::integral_constant<int, 1>());
     }
     // the warp's columns of V, for both products: rows 16 i + .., pairs along the rows
     uint32_t v[4][4];
@@ -298,17 +349,19 @@ __global__ void __launch_bounds__(LinearTiles<BF16, DK, DV>::THREADS, LinearTile
             lo[w] = narrow<BF16>(a - taken.x, b - taken.y);
           }
         }
+        // (two blocks of rows at a time: those behind the end are zeros)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 4; i += 2) {
           if (16 * i >= n) break;
-          uint32_t a[4];
-          ldmatrix4<0>(a, sq + tile_at<DK>(16 * i + (lane & 15), 2 * k + (lane >> 4)));
+          uint32_t a[2][4];
+#pragma unroll
+          for (int z = 0; z < 2; ++z) ldmatrix4<0>(a[z], sq + tile_at<DK>(16 * (i + z) + (lane & 15), 2 * k + (lane >> 4)));
           if constexpr (BF16) {
-            mma_add<BF16>(o[i][0], a, lo[0], lo[1]);
-            mma_add<BF16>(o[i][1], a, lo[2], lo[3]);
+#pragma unroll
+            for (int z = 0; z < 4; ++z) mma_add<BF16>(o[i + z / 2][z % 2], a[z / 2], lo[z % 2 * 2], lo[z % 2 * 2 + 1]);
           }
-          mma_add<BF16>(o[i][0], a, hi[0], hi[1]);
-          mma_add<BF16>(o[i][1], a, hi[2], hi[3]);
+#pragma unroll
+          for (int z = 0; z < 4; ++z) mma_add<BF16>(o[i + z / 2][z % 2], a[z / 2], hi[z % 2 * 2], hi[z % 2 * 2 + 1]);
         }
       }
       __syncthreads();
@@ -317,47 +370,83 @@ __global__ void __launch_bounds__(LinearTiles<BF16, DK, DV>::THREADS, LinearTile
       const int64_t step_y = p.y.row * 8;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        if (16 * i >= n) break;
         const float f0 = s_power[16 * i + g8 + 1] * down, f1 = s_power[16 * i + g8 + 9] * down;
 #pragma unroll
         for (int x = 0; x < 2; ++x) { o[i][x][0] *= f0; o[i][x][1] *= f0; o[i][x][2] *= f1; o[i][x][3] *= f1; }
-#pragma unroll
-        for (int j = 0; j <= i; ++j) {
-          const int block = i * (i + 1) / 2 + j;
+      }
+      // a column of blocks of scores at a time: their products wait for one another only where they are of the same rows
+      auto column = [&](auto place) {
+        constexpr int j = decltype(place)::value;
+        if (bad) {
+          const int block = j * (j + 1) / 2 + j;
           const float f = BF16 ? 1.f : s_block[block];
-          if (bad && j == i) {
-            for (int s = 0; s < 16; ++s)
+#pragma unroll 1
+          for (int s = 0; s < 16; ++s)
 #pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                const int row = g8 + (e >> 1 & 1) * 8, c = warp * 16 + (e >> 2) * 8 + 2 * t4 + (e & 1);
-                const uint32_t at = score_at(block, row, s >> 3) + (s & 7) * 2;
-                float w = widen<BF16>(*reinterpret_cast<const uint16_t*>(s_scores + at)).x;
-                if constexpr (BF16) w += widen<BF16>(*reinterpret_cast<const uint16_t*>(s_scores + L::SCORES + at)).x;
-                const uint16_t u = *reinterpret_cast<const uint16_t*>(smem + (sv - base) + tile_at<DV>(16 * j + s, c >> 3) + (c & 7) * 2);
-                if (s <= row) o[i][e >> 2][e & 3] = fmaf(w * f, widen<BF16>(u).x, o[i][e >> 2][e & 3]);
-              }
-            __syncwarp();
-            continue;
-          }
-          uint32_t a[4];
-          ldmatrix4<0>(a, scores_at + score_at(block, lane & 15, lane >> 4));
-          if constexpr (BF16) {
-            uint32_t b[4];
-            ldmatrix4<0>(b, scores_at + L::SCORES + score_at(block, lane & 15, lane >> 4));
-            mma_add<BF16>(o[i][0], b, v[j][0], v[j][1]);
-            mma_add<BF16>(o[i][1], b, v[j][2], v[j][3]);
-            mma_add<BF16>(o[i][0], a, v[j][0], v[j][1]);
-            mma_add<BF16>(o[i][1], a, v[j][2], v[j][3]);
-          } else {
-            float c[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-            mma_add<BF16>(c[0], a, v[j][0], v[j][1]);
-            mma_add<BF16>(c[1], a, v[j][2], v[j][3]);
-#pragma unroll
-            for (int x = 0; x < 2; ++x)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) o[i][x][e] = fmaf(c[x][e], f, o[i][x][e]);
-          }
+            for (int e = 0; e < 8; ++e) {
+              const int row = g8 + (e >> 1 & 1) * 8, c = warp * 16 + (e >> 2) * 8 + 2 * t4 + (e & 1);
+              const uint32_t at = score_at(block, row, s >> 3) + (s & 7) * 2;
+              float w = widen<BF16>(*reinterpret_cast<const uint16_t*>(s_scores + at)).x;
+              if constexpr (BF16) w += widen<BF16>(*reinterpret_cast<const uint16_t*>(s_scores + L::SCORES + at)).x;
+              const uint16_t u = *reinterpret_cast<const uint16_t*>(smem + (sv - base) + tile_at<DV>(16 * j + s, c >> 3) + (c & 7) * 2);
+              if (s <= row) o[j][e >> 2][e & 3] = fmaf(w * f, widen<BF16>(u).x, o[j][e >> 2][e & 3]);
+            }
+          __syncwarp();
         }
+        auto products = [&](auto from) {
+          constexpr int I = decltype(from)::value;
+          if constexpr (I < 4) {
+            uint32_t a[4 - I][4];
+            [[maybe_unused]] uint32_t b[4 - I][4];
+#pragma unroll
+            for (int i = I; i < 4; ++i) {
+              const uint32_t at = score_at(i * (i + 1) / 2 + j, lane & 15, lane >> 4);
+              ldmatrix4<0>(a[i - I], scores_at + at);
+              if constexpr (BF16) ldmatrix4<0>(b[i - I], scores_at + L::SCORES + at);
+            }
+            if constexpr (BF16) {
+#pragma unroll
+              for (int i = I; i < 4; ++i) {
+                mma_add<BF16>(o[i][0], b[i - I], v[j][0], v[j][1]);
+                mma_add<BF16>(o[i][1], b[i - I], v[j][2], v[j][3]);
+              }
+#pragma unroll
+              for (int i = I; i < 4; ++i) {
+                mma_add<BF16>(o[i][0], a[i - I], v[j][0], v[j][1]);
+                mma_add<BF16>(o[i][1], a[i - I], v[j][2], v[j][3]);
+              }
+            } else {
+              float c[4 - I][2][4];
+#pragma unroll
+              for (int i = I; i < 4; ++i) {
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) c[i - I][x][e] = 0.f;
+                mma_add<BF16>(c[i - I][0], a[i - I], v[j][0], v[j][1]);
+                mma_add<BF16>(c[i - I][1], a[i - I], v[j][2], v[j][3]);
+              }
+#pragma unroll
+              for (int i = I; i < 4; ++i) {
+                const float f = s_block[i * (i + 1) / 2 + j];
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) o[i][x][e] = fmaf(c[i - I][x][e], f, o[i][x][e]);
+              }
+            }
+          }
+        };
+        if (bad) products(std::integral_constant<int, j + 1>());
+        else products(place);
+      };
+      column(std::integral_constant<int, 0>());
+      if (n > 16) column(std::integral_constant<int, 1>());
+      if (n > 32) column(std::integral_constant<int, 2>());
+      if (n > 48) column(std::integral_constant<int, 3>());
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (16 * i >= n) break;
 #pragma unroll
         for (int e = 0; e < 4; e += 2, y += step_y) {
           if (16 * i + g8 + (e >> 1) * 8 >= n) continue;
