@@ -457,7 +457,9 @@ template <typename T, int KT, int PARTS>
 int launch_linear_parts_of(const LinearParams& p, dim3 grid, cudaStream_t s) {
   return p.dv <= 64 ? launch_linear_columns<T, KT, PARTS, 1>(p, grid, s) : launch_linear_columns<T, KT, PARTS, 2>(p, grid, s);
 }
-// us with 32 and 8 of dk a thread: 74 lists of 100 rows, 2 heads of 36, fp32 TODO
+// Few lists: fewer of dk a thread, so that there are more of them (a row's FMAs of a thread wait for one another). us with 32 and 8 (or 16) of dk a
+// thread, 74 lists of 100 rows, 2 heads, fp32: heads of 32 41.9 and 26.6, of 36 36.8 and 30.6, of 64 36.8 and 37.5, of 128 69.5 and 67.5. From 4
+// blocks an SM on both take as long (296 lists of 100 rows: 55).
 template <typename T>
 int launch_linear_rows(const LinearParams& p, dim3 grid, cudaStream_t s) {
   if ((int64_t)grid.x < 4 * (int64_t)sm_count()) {
