@@ -82,6 +82,8 @@ __device__ __forceinline__ int group_begin(const PrefixParams& p, int g) {
   const int m = p.members[g - 1];
   return m < 0 ? 0 : m > p.lists.batch ? p.lists.batch : m;
 }
+// (members that do not ascend: no list)
+__device__ __forceinline__ int group_end(const PrefixParams& p, int g) { return max(group_begin(p, g + 1), group_begin(p, g)); }
 __device__ __forceinline__ int64_t prefix_begin(const PrefixParams& p, int i) {
   if (!p.prefix_offsets) return (int64_t)i * (p.prefix_rows / p.prefixes);
   const int64_t o = p.prefix_offsets[i];
@@ -222,13 +224,15 @@ __global__ void __launch_bounds__(PLAN_THREADS) prefix_plan_kernel(const __grid_
     PrefixGroup x = {};
     int64_t n = 0;
     if (g < n_groups) {
-      const int64_t rows = p.lists.begin(group_begin(p, g + 1)) - p.lists.begin(group_begin(p, g));
+      const int64_t rows = p.lists.begin(group_end(p, g)) - p.lists.begin(group_begin(p, g));
       n = rows > 0 ? (rows + step - 1) / step : 0;
       x.tiles = rows > 0 ? (int)((rows + p.R - 1) / p.R) : 0;
       if (g > 0 && g <= p.prefixes) x.blocks = (int)((max(prefix_begin(p, g) - prefix_begin(p, g - 1), (int64_t)0) + PFX_KEYS - 1) / PFX_KEYS);
     }
     const int64_t at = total + block_scan(n, s_sums, sum);
     x.first = (int)min(at, (int64_t)p.max_items);
+    // (members that do not ascend name lists twice: a group has the tiles of the items that there is room for)
+    if (at + n > p.max_items) x.tiles = min(x.tiles, 2 * (p.max_items - x.first));
     if (g < n_groups) groups[g] = x;
     total += sum;
   }
@@ -253,7 +257,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) prefix_plan_kernel(const __grid_
         else hi = mid - 1;
       }
       PrefixItem x = {};
-      const int l0 = group_begin(p, lo), l1 = max(group_begin(p, lo + 1) - 1, l0);
+      const int l0 = group_begin(p, lo), l1 = group_end(p, lo) - 1;
       const int64_t begin = p.lists.begin(l0) + (int64_t)(t - groups[lo].first) * step;
       const int64_t end = max(min(begin + step, p.lists.begin(l1 + 1)), begin + 1), mid = min(begin + p.R, end);
       x.row0 = (int)begin; x.rows = (int)(end - begin);
