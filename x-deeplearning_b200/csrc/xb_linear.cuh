@@ -263,21 +263,28 @@ __global__ void __launch_bounds__(64 * PARTS) linear_rows_kernel(const LinearPar
     load_tile(tile + LIN_TILES - 1);
     const T *s_q = s_rows + tile % LIN_TILES * TILE, *s_k = s_q + LIN_ROWS * DK, *s_v = s_k + LIN_ROWS * DK;
     T* y_at = const_cast<T*>(p.y.get<T>(r0, h)) + c;
-#pragma unroll 4
-    for (int r = 0; r < rows; ++r) {       // (a row's product with q beside the next row's step)
-      f32x2 v2[NV], y2[NV][2];
+    // N rows: the state goes from row to row, their products with q wait for one another only in the sums over the parts. There a part gives half of its
+    // rows to its neighbour and takes the neighbour's half of the others, until it has N / PARTS rows of whole sums: 7 shuffles for 8 rows and parts, not
+    // 24. (A row alone: all parts have the same sum, made in the same order.)
+    auto steps = [&](auto slow, auto count, int first) {
+      constexpr int N = decltype(count)::value, HAVE = N < PARTS ? 1 : N / PARTS;
+      static_assert(N == 1 || N % PARTS == 0, "");
+      float y[N][NV];
 #pragma unroll
-      for (int n = 0; n < NV; ++n) {
-        const float v = mine ? to_f32<T>(s_v[r * DV + c + n]) : 0.f;
-        v2[n] = pack2(v, v);
-        y2[n][0] = y2[n][1] = pack2(0.f, 0.f);
-      }
-      auto move = [&](auto slow) {
+      for (int r = 0; r < N; ++r) {
+        const int row = first + r;
+        f32x2 v2[NV], y2[NV][2];
+#pragma unroll
+        for (int n = 0; n < NV; ++n) {
+          const float v = mine ? to_f32<T>(s_v[row * DV + c + n]) : 0.f;
+          v2[n] = pack2(v, v);
+          y2[n][0] = y2[n][1] = pack2(0.f, 0.f);
+        }
 #pragma unroll
         for (int j = 0; j < KT / 4; ++j) {
           f32x2 k4[2], q4[2];
-          read_four(s_k + r * DK + (j * PARTS + part) * 4, k4[0], k4[1]);
-          read_four(s_q + r * DK + (j * PARTS + part) * 4, q4[0], q4[1]);
+          read_four(s_k + row * DK + (j * PARTS + part) * 4, k4[0], k4[1]);
+          read_four(s_q + row * DK + (j * PARTS + part) * 4, q4[0], q4[1]);
 #pragma unroll
           for (int b = 0; b < 2; ++b) {
             const f32x2 k2 = k4[b], q2 = q4[b];
@@ -289,32 +296,60 @@ __global__ void __launch_bounds__(64 * PARTS) linear_rows_kernel(const LinearPar
             }
           }
         }
-      };
-      if (decay.slow) move(std::true_type());
-      else move(std::false_type());
-      if (p.ends_only) continue;
-      float y[2] = {0.f, 0.f};
 #pragma unroll
-      for (int n = 0; n < NV; ++n) {
-        float a, b;
-        unpack2(add2(y2[n][0], y2[n][1]), a, b);
-        y[n] = a + b;
-#pragma unroll
-        for (int o = 1; o < PARTS; o *= 2) y[n] += __shfl_xor_sync(0xffffffffu, y[n], o);
-        y[n] *= p.scale;
+        for (int n = 0; n < NV; ++n) {
+          float lo, hi;
+          unpack2(add2(y2[n][0], y2[n][1]), lo, hi);
+          y[r][n] = lo + hi;
+        }
       }
-      if (part != 0 || !mine) continue;
-      T* to = y_at + r * p.y.row;
-      if (NV == 2 && p.vec_y) {
-        Raw<T, 2> out;
-        out.put_all(y);
-        out.store_piece(to);
+      if (p.ends_only) return;
+#pragma unroll
+      for (int o = PARTS / 2, m = N / 2; o > 0; o /= 2, m /= 2) {
+        if constexpr (N == 1) {
+#pragma unroll
+          for (int n = 0; n < NV; ++n) y[0][n] += __shfl_xor_sync(0xffffffffu, y[0][n], o);
+        } else {
+          const bool upper = (part & o) != 0;
+#pragma unroll
+          for (int r = 0; r < N / 2; ++r) {
+            if (r >= m) break;
+#pragma unroll
+            for (int n = 0; n < NV; ++n) {
+              const float other = __shfl_xor_sync(0xffffffffu, upper ? y[r][n] : y[r + m][n], o);
+              y[r][n] = (upper ? y[r + m][n] : y[r][n]) + other;
+            }
+          }
+        }
+      }
+      if (!mine || (N == 1 && part != 0)) return;
+#pragma unroll
+      for (int i = 0; i < HAVE; ++i) {
+        T* to = y_at + (first + (N == 1 ? 0 : part * HAVE + i)) * p.y.row;
+#pragma unroll
+        for (int n = 0; n < NV; ++n) y[i][n] *= p.scale;
+        if (NV == 2 && p.vec_y) {
+          const float two[2] = {y[i][0], y[i][NV - 1]};
+          Raw<T, 2> out;
+          out.put_all(two);
+          out.store_piece(to);
+        } else {
+#pragma unroll
+          for (int n = 0; n < NV; ++n)
+            if (c + n < p.dv) to[n] = from_f32<T>(y[i][n]);
+        }
+      }
+    };
+    auto tile_steps = [&](auto slow) {
+      if (rows == LIN_ROWS) {
+        steps(slow, std::integral_constant<int, LIN_ROWS>(), 0);
       } else {
-#pragma unroll
-        for (int n = 0; n < NV; ++n)
-          if (c + n < p.dv) to[n] = from_f32<T>(y[n]);
+#pragma unroll 1
+        for (int r = 0; r < rows; ++r) steps(slow, std::integral_constant<int, 1>(), r);
       }
-    }
+    };
+    if (decay.slow) tile_steps(std::true_type());
+    else tile_steps(std::false_type());
   }
   float* to = state_to(p, g, h);
   if (to) put_state(to);
