@@ -108,11 +108,12 @@ __device__ __forceinline__ float* state_to(const LinearParams& p, const Segment&
 }
 
 // ---- row by row ----
-// A block has a list (or segment) and a head; a thread NV columns of dv (two where there are more than 64) and KT of dk, PARTS lanes sharing the
-// columns, whose products with q meet in shuffles. KT is 32, or 8 where there are so few lists that the row's latency counts. The state stays in registers, in pairs along dk. Rows come eight at a time through shared memory,
-// three such tiles ahead; pieces of four along dk go round the PARTS lanes, so that what a warp reads at once lies in adjacent banks.
-// 3 packed FMAs for two values of the state a row, bound by the latency of a row's steps where there are few lists, by the FMAs' issue and the
-// broadcast reads of k and q where there are many. 74 lists of 100 rows, 2 heads of 36, fp32: 37 us with rows that pass through registers.
+// A block has a list (or segment) and a head; a thread NV columns of dv (two where there are more than 64, and see below) and KT of dk, PARTS lanes sharing the
+// columns, whose products with q meet in shuffles. KT is 32, or 8 where there are so few lists that the row's latency counts. The state stays in
+// registers, in pairs along dk. Rows come eight at a time through shared memory, three such tiles ahead; pieces of four along dk go round the PARTS
+// lanes, so that what a warp reads at once lies in adjacent banks. 3 packed FMAs for two values of the state a row, bound by the reads of k and q from
+// shared memory (512 bytes an instruction to registers, however few they are in memory). 74 lists of 100 rows, 2 heads of 36, fp32: 22 us; 31 with
+// a row's sums made before the next row's (24 shuffles for 8 rows in place of 7), 37 with rows that pass through registers.
 constexpr int LIN_ROWS = 8, LIN_TILES = 4, LIN_MAX = 128;
 // four adjacent elements of shared memory, as two pairs of fp32
 template <typename T>
@@ -127,10 +128,10 @@ __device__ __forceinline__ void read_four(const T* p, f32x2& lo, f32x2& hi) {
     lo = pack2(r.get(0), r.get(1)); hi = pack2(r.get(2), r.get(3));
   }
 }
-template <typename T, int KT, int PARTS, int NV>
-__global__ void __launch_bounds__(64 * PARTS) linear_rows_kernel(const LinearParams p) {
+template <typename T, int KT, int PARTS, int NV, int DV>
+__global__ void __launch_bounds__(DV / NV * PARTS) linear_rows_kernel(const LinearParams p) {
   pdl_wait();
-  constexpr int DK = KT * PARTS, DV = 64 * NV, TILE = LIN_ROWS * (2 * DK + DV);
+  constexpr int DK = KT * PARTS, TILE = LIN_ROWS * (2 * DK + DV);
   extern __shared__ __align__(128) uint8_t smem[];          // [tiles][q, k, v][rows][DK or DV]
   T* s_rows = reinterpret_cast<T*>(smem);
   __shared__ Segment s_seg;
@@ -477,24 +478,29 @@ __global__ void __launch_bounds__(CARRY_THREADS) linear_carry_kernel(const Linea
   }
 }
 
-template <typename T, int KT, int PARTS, int NV>
+template <typename T, int KT, int PARTS, int NV, int DV>
 int launch_linear_columns(const LinearParams& p, dim3 grid, cudaStream_t s) {
-  constexpr int SMEM = LIN_TILES * LIN_ROWS * (2 * KT * PARTS + 64 * NV) * (int)sizeof(T);
+  constexpr int SMEM = LIN_TILES * LIN_ROWS * (2 * KT * PARTS + DV) * (int)sizeof(T);
   if constexpr (SMEM > 46 * 1024) {           // (48 KB with what the kernel has besides)
     static PerDeviceOnce once;
-    XB_SET_MAX_SMEM_ONCE(once, SMEM, (const void*)linear_rows_kernel<T, KT, PARTS, NV>);
+    XB_SET_MAX_SMEM_ONCE(once, SMEM, (const void*)linear_rows_kernel<T, KT, PARTS, NV, DV>);
   }
   const unsigned threads = (unsigned)(((p.dv + NV - 1) / NV * PARTS + 31) / 32 * 32);
-  launch_dependent(linear_rows_kernel<T, KT, PARTS, NV>, grid, threads, SMEM, s, p);
+  launch_dependent(linear_rows_kernel<T, KT, PARTS, NV, DV>, grid, threads, SMEM, s, p);
   return check_launch("linear_rows_kernel");
 }
+// Up to 64 columns: two a thread where what is read of k and q is widened for them (16 bits), or where few threads of dk read it (fewer of
+// dk a thread, more of those). us with one and two, fp32: 74 lists of 100 rows, 2 heads of 64 29 and 24, one of 74000 433 and 273; 1024 lists of 100
+// 176 and 208 (32 of dk a thread: fewer warps for the registers). bf16, 4096 lists of 6 rows, 4 heads of 64: 258 and 180.
 template <typename T, int KT, int PARTS>
 int launch_linear_parts_of(const LinearParams& p, dim3 grid, cudaStream_t s) {
-  return p.dv <= 64 ? launch_linear_columns<T, KT, PARTS, 1>(p, grid, s) : launch_linear_columns<T, KT, PARTS, 2>(p, grid, s);
+  if (p.dv <= 32) return launch_linear_columns<T, KT, PARTS, 1, 32>(p, grid, s);
+  if (p.dv <= 64) return launch_linear_columns<T, KT, PARTS, sizeof(T) == 2 || (KT == 8 && PARTS == 8) ? 2 : 1, 64>(p, grid, s);
+  return launch_linear_columns<T, KT, PARTS, 2, 128>(p, grid, s);
 }
 // Few lists: fewer of dk a thread, so that there are more of them (a row's FMAs of a thread wait for one another). us with 32 and 8 (or 16) of dk a
-// thread, 74 lists of 100 rows, 2 heads, fp32: heads of 32 41.9 and 26.6, of 36 36.8 and 30.6, of 64 36.8 and 37.5, of 128 69.5 and 67.5. From 4
-// blocks an SM on both take as long (296 lists of 100 rows: 55).
+// thread, 74 lists of 100 rows, 2 heads, fp32: heads of 32 39 and 18, of 36 29 and 22, of 64 27 and 24, of 128 53 and 51. From 4 blocks an SM on
+// both take as long (296 lists of 100 rows: 45).
 template <typename T>
 int launch_linear_rows(const LinearParams& p, dim3 grid, cudaStream_t s) {
   if ((int64_t)grid.x < 4 * (int64_t)sm_count()) {
