@@ -86,7 +86,10 @@ __device__ __forceinline__ float top_of(F each) {
 template <bool BF16, int DK, int DV>
 struct LinearTiles {
   static constexpr int WARPS = DV / 16, THREADS = WARPS * 32;
-  static constexpr int Q = LT_ROWS * DK * 2, V = LT_ROWS * DV * 2, BUFFER = 2 * Q + V;         // bytes: queries, keys, values
+  // Bytes: queries, keys, values. With an SM's registers in one block or two nobody else hides the wait for keys and values: there the next chunk's are
+  // on their way while this one is worked on. LTNOTE
+  static constexpr int BUFFERS = DK == 128 || DV == 128 ? 2 : 1;
+  static constexpr int Q = LT_ROWS * DK * 2, V = LT_ROWS * DV * 2, KV = Q + V, BUFFER = Q + BUFFERS * KV;
   static constexpr int SCORES = 10 * 512, TERMS_Y = BF16 ? 2 : 1, TERMS_S = BF16 ? 3 : 2;      // (blocks of 16 x 16 on and below the diagonal)
   static constexpr int SMEM = BUFFER + TERMS_Y * SCORES + (LT_ROWS + 4) * 4 + 16 * 4;
   // Blocks of an SM, as registers and shared memory have it: what hides a block's waits is the others. (64 x 64, two buffers and three blocks: 4400
@@ -161,13 +164,13 @@ __global__ void __launch_bounds__(LinearTiles<BF16, DK, DV>::THREADS, LinearTile
   auto load_q = [&](int64_t r0) {
     if (!p.ends_only) load(p.q, h, p.dk, p.unit_q, 0, std::integral_constant<int, DK>(), r0);
   };
-  auto load_kv = [&](int64_t r0) {
-    load(p.k, hkv, p.dk, p.unit_k, L::Q, std::integral_constant<int, DK>(), r0);
-    load(p.v, hkv, p.dv, p.unit_v, 2 * L::Q, std::integral_constant<int, DV>(), r0);
+  auto load_kv = [&](int64_t r0, uint32_t buffer) {
+    load(p.k, hkv, p.dk, p.unit_k, L::Q + buffer, std::integral_constant<int, DK>(), r0);
+    load(p.v, hkv, p.dv, p.unit_v, 2 * L::Q + buffer, std::integral_constant<int, DV>(), r0);
     umma::cp_async_commit();
   };
   load_q(g.begin);
-  load_kv(g.begin);
+  load_kv(g.begin, 0);
 
   // S^T: rows 16 warp + g8 (and + 8) of dv, columns 8 j + 2 t4 (and + 1) of dk
   float S[DK / 8][4];
@@ -201,11 +204,17 @@ __global__ void __launch_bounds__(LinearTiles<BF16, DK, DV>::THREADS, LinearTile
     for (int b = 0; b < 2; ++b) col_f[x][b] = s_power[16 - 8 * x - 2 * t4 - b];
   const float last_f[2] = {s_power[7 - 2 * t4], s_power[6 - 2 * t4]};
   const bool vec_y = p.vec_y;
-  const uint32_t sq = base, sk = sq + L::Q, sv = sk + L::Q;
+  const uint32_t sq = base;
+  uint32_t buffer = 0;                     // bytes to this chunk's keys and values
   for (int64_t r0 = g.begin; r0 < g.end; r0 += LT_ROWS) {
+    const uint32_t sk = sq + L::Q + buffer, sv = sk + L::Q;
     const int n = (int)min((int64_t)LT_ROWS, g.end - r0);
     umma::cp_async_wait_all();
     __syncthreads();
+    if (L::BUFFERS > 1) {                  // (all have done with the chunk before, whose buffer this is)
+      buffer = L::KV - buffer;
+      if (r0 + LT_ROWS < g.end) load_kv(r0 + LT_ROWS, buffer);
+    }
     if (!p.ends_only) {
       // scores, times the decay: ten blocks of 16 x 16 on and below the diagonal, those of a warp side by side
       const int row_blocks = (n + 15) / 16, blocks = row_blocks * (row_blocks + 1) / 2;
@@ -540,9 +549,9 @@ __global__ void __launch_bounds__(LinearTiles<BF16, DK, DV>::THREADS, LinearTile
           s = fmaf(s, decay.by, fmaf(s, keep, BF16 ? c[x][e] : c[x][e] * down));
         }
     }
-    if (r0 + LT_ROWS < g.end) {
+    if (L::BUFFERS == 1 && r0 + LT_ROWS < g.end) {
       __syncthreads();
-      load_kv(r0 + LT_ROWS);
+      load_kv(r0 + LT_ROWS, 0);
     }
   }
   float* to = state_to(p, g, h);
