@@ -162,8 +162,11 @@ __global__ void __launch_bounds__(LinearTiles<BF16, DK, DV>::THREADS, LinearTile
       else asm volatile("st.shared.u16 [%0], %1;" ::"r"(to), "h"(bytes ? *reinterpret_cast<const uint16_t*>(f) : (uint16_t)0) : "memory");
     }
   };
+  // (a group of their own: with two buffers of keys and values nothing is asked for behind the queries that would take them in)
   auto load_q = [&](int64_t r0) {
-    if (!p.ends_only) load(p.q, h, p.dk, p.unit_q, 0, std::integral_constant<int, DK>(), r0);
+    if (p.ends_only) return;
+    load(p.q, h, p.dk, p.unit_q, 0, std::integral_constant<int, DK>(), r0);
+    umma::cp_async_commit();
   };
   auto load_kv = [&](int64_t r0, uint32_t buffer) {
     load(p.k, hkv, p.dk, p.unit_k, L::Q + buffer, std::integral_constant<int, DK>(), r0);
