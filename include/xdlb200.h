@@ -607,7 +607,8 @@ int xb_qk_norm_rope(const xb_qk_norm_rope_args* args, xb_stream_t stream);
  *   S_t = exp(log_decay[h]) S_{t-1} + k[t, h'] v[t, h']^T,   y[t, h] = scale q[t, h] S_t,   h' = h / (H / Hkv)
  * log_decay <= 0 (-infinity: no memory; what is above 0 counts as 0). The states [n_slots, H, dk, dv] are fp32. 16-bit lists of more than
  * a few rows go by chunks of 64 on the matrix instructions: what states are made of to 24 bits (fp16: 22), what makes y (scores, states) to 2^-17
- * of it (fp16: 2^-11, a result's own rounding); fp32 lists by fp32 FMAs alone. dk, dv <= 128. An infinity or NaN in a row makes no other list's results bad; its own list's
+ * of it (fp16: 2^-11, a result's own rounding; below fp16's range, to 2^-39 of the largest of a column of the chunk's values or of the state, or of a
+ * query's scores in a block of 16); fp32 lists by fp32 FMAs alone. dk, dv <= 128. An infinity or NaN in a row makes no other list's results bad; its own list's
  * may be NaN where the formula has an infinity. */
 typedef struct xb_linear_attention_args {
   const void* q; int64_t q_row, q_head;           /* [rows, H, dk] */

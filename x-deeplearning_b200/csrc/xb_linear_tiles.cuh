@@ -8,7 +8,8 @@
 //
 // Rounding. S is fp32, and what it is made of is known to fp32's last bits: k as it is, g^.. v as three bf16 terms (24 bits) or two fp16 terms (22).
 // For y, scores and S are two bf16 terms (2^-17 of each) or one of fp16 (2^-11, as a result's own rounding). What becomes fp16 is first multiplied by
-// a power of two that puts the largest of a warp's values at 2^14: nothing is beyond fp16's numbers, and what is below them is 2^-28 of the largest.
+// powers of two that put the largest values at 2^14: nothing is beyond fp16's numbers, and what is below them is off by 2^-39 of the largest at most.
+// S and v have one such power for each column of dv, scores for each row of a block, so that no result is off by the size of another.
 #pragma once
 
 #include "xb_linear.cuh"
@@ -53,34 +54,27 @@ __device__ __forceinline__ void fp16_scale(float top, float& up, float& down) {
   up = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
   down = __uint_as_float((uint32_t)(127 - 14 + e) << 23);
 }
-__device__ __forceinline__ float warp_top(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
-}
-
-// (several at once: their shuffles wait beside one another)
+// the largest of the four lanes that share a row of an accumulator, several at once: their shuffles wait beside one another
 template <int N>
-__device__ __forceinline__ void warp_tops(float (&v)[N]) {
+__device__ __forceinline__ void quad_tops(float (&v)[N]) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
+  for (int o = 2; o > 0; o >>= 1)
 #pragma unroll
     for (int z = 0; z < N; ++z) v[z] = fmaxf(v[z], __shfl_xor_sync(0xffffffffu, v[z], o));
 }
 
-// The largest of a warp's sizes, told by `each`, which calls its argument with every value of a lane. Infinities have no say in it: they are what
-// they are at any scale, and the finite values beside them keep theirs.
+// The largest sizes in an accumulator's rows g8 and g8 + 8, told by `each`, which calls its argument with every value of a lane and which of the two rows
+// it is of. Infinities have no say in it: they are what they are at any scale, and the finite values beside them keep theirs.
 template <typename F>
-__device__ __forceinline__ float top_of(F each) {
-  float top = 0.f;
-  each([&](float v) { top = fmaxf(top, fabsf(v)); });
-  top = warp_top(top);
-  if (top == INFINITY) {
-    top = 0.f;
-    each([&](float v) { top = fabsf(v) < INFINITY ? fmaxf(top, fabsf(v)) : top; });
-    top = warp_top(top);
+__device__ __forceinline__ void tops_of(F each, float (&top)[2]) {
+  top[0] = top[1] = 0.f;
+  each([&](int row, float v) { top[row] = fmaxf(top[row], fabsf(v)); });
+  quad_tops(top);
+  if (__any_sync(0xffffffffu, fmaxf(top[0], top[1]) == INFINITY)) {
+    top[0] = top[1] = 0.f;
+    each([&](int row, float v) { top[row] = fabsf(v) < INFINITY ? fmaxf(top[row], fabsf(v)) : top[row]; });
+    quad_tops(top);
   }
-  return top;
 }
 
 template <bool BF16, int DK, int DV>
@@ -93,7 +87,7 @@ struct LinearTiles {
   static constexpr int BUFFERS = DK == 128 || DV == 128 ? 2 : 1;
   static constexpr int Q = LT_ROWS * DK * 2, V = LT_ROWS * DV * 2, KV = Q + V, BUFFER = Q + BUFFERS * KV;
   static constexpr int SCORES = 10 * 512, TERMS_Y = BF16 ? 2 : 1, TERMS_S = BF16 ? 3 : 2;      // (blocks of 16 x 16 on and below the diagonal)
-  static constexpr int SMEM = BUFFER + TERMS_Y * SCORES + (LT_ROWS + 4) * 4 + 16 * 4;
+  static constexpr int SMEM = BUFFER + TERMS_Y * SCORES + (LT_ROWS + 4) * 4 + (BF16 ? 0 : 10 * 16 * 4);
   // Blocks of an SM, as registers and shared memory have it: what hides a block's waits is the others.
   static constexpr int BLOCKS = DV == 128 ? (DK == 128 ? 1 : 2) : DK == 128 ? 2 : 4;
 };
@@ -107,7 +101,7 @@ __global__ void __launch_bounds__(LinearTiles<BF16, DK, DV>::THREADS, LinearTile
   extern __shared__ __align__(128) uint8_t smem[];
   uint8_t* s_scores = smem + L::BUFFER;                                       // [terms][10][16][16]
   float* s_power = reinterpret_cast<float*>(s_scores + L::TERMS_Y * L::SCORES);      // decay over 0 to 64 rows
-  float* s_block = s_power + LT_ROWS + 4;                                     // what the scores of a block of 16 x 16 are to be multiplied by
+  float* s_down = s_power + LT_ROWS + 4;                                      // fp16: what the scores of a block's 16 rows are to be multiplied by, ten blocks
   __shared__ Segment s_seg;
   __shared__ int s_there;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, h = (int)(blockIdx.x % (unsigned)p.H), hkv = h / p.share;
@@ -253,7 +247,7 @@ __global__ void __launch_bounds__(LinearTiles<BF16, DK, DV>::THREADS, LinearTile
             mma_add<BF16>(c[z][1], a[z], bk[z][1], bk[z][3]);
           }
         }
-        float tops[N];
+        [[maybe_unused]] float tops[2 * N];
 #pragma unroll
         for (int z = 0; z < N; ++z) {
           if (back[z] == 0) {
@@ -271,15 +265,13 @@ __global__ void __launch_bounds__(LinearTiles<BF16, DK, DV>::THREADS, LinearTile
 #pragma unroll
               for (int e = 0; e < 4; ++e) c[z][x][e] *= row_f[e >> 1] * far * col_f[x][e & 1];
           }
-          tops[z] = 0.f;
           if constexpr (!BF16) {
 #pragma unroll
-            for (int x = 0; x < 2; ++x)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) tops[z] = fmaxf(tops[z], fabsf(c[z][x][e]));
+            for (int r = 0; r < 2; ++r)
+              tops[2 * z + r] = fmaxf(fmaxf(fabsf(c[z][0][2 * r]), fabsf(c[z][0][2 * r + 1])), fmaxf(fabsf(c[z][1][2 * r]), fabsf(c[z][1][2 * r + 1])));
           }
         }
-        if constexpr (!BF16) warp_tops(tops);
+        if constexpr (!BF16) quad_tops(tops);
 #pragma unroll
         for (int z = 0; z < N; ++z) {
           const int b = warp + z * L::WARPS;
@@ -288,15 +280,21 @@ __global__ void __launch_bounds__(LinearTiles<BF16, DK, DV>::THREADS, LinearTile
 #pragma unroll
               for (int x = 0; x < 2; ++x)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) take(c[z][x][e]);
+                for (int e = 0; e < 4; ++e) take(e >> 1, c[z][x][e]);
             };
-            float up, down;
-            fp16_scale(tops[z] == INFINITY ? top_of(each) : tops[z], up, down);
-            if (lane == 0) s_block[b] = down;
+            float top[2] = {tops[2 * z], tops[2 * z + 1]};
+            if (__any_sync(0xffffffffu, fmaxf(top[0], top[1]) == INFINITY)) tops_of(each, top);
 #pragma unroll
-            for (int x = 0; x < 2; ++x)
+            for (int r = 0; r < 2; ++r) {
+              float up, down;
+              fp16_scale(top[r], up, down);
+              if (t4 == 0) s_down[b * 16 + g8 + 8 * r] = down;
 #pragma unroll
-              for (int e = 0; e < 4; ++e) c[z][x][e] *= up;
+              for (int x = 0; x < 2; ++x) {
+                c[z][x][2 * r] *= up;
+                c[z][x][2 * r + 1] *= up;
+              }
+            }
           }
 #pragma unroll
           for (int x = 0; x < 2; ++x)
@@ -338,15 +336,23 @@ __global__ void __launch_bounds__(LinearTiles<BF16, DK, DV>::THREADS, LinearTile
         for (int x = 0; x < 2; ++x)
 #pragma unroll
           for (int e = 0; e < 4; ++e) o[i][x][e] = 0.f;
-      float up = 1.f, down = 1.f;
+      [[maybe_unused]] float up[2], down[2][2];              // (of columns g8 and g8 + 8; of an accumulator's columns)
       if constexpr (!BF16) {
-        fp16_scale(top_of([&](auto take) {
+        float top[2], of_column[2];
+        tops_of(
+            [&](auto take) {
 #pragma unroll
-                     for (int j = 0; j < DK / 8; ++j)
+              for (int j = 0; j < DK / 8; ++j)
 #pragma unroll
-                       for (int e = 0; e < 4; ++e) take(S[j][e]);
-                   }),
-                   up, down);
+                for (int e = 0; e < 4; ++e) take(e >> 1, S[j][e]);
+            },
+            top);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          fp16_scale(top[x], up[x], of_column[x]);
+#pragma unroll
+          for (int b = 0; b < 2; ++b) down[x][b] = __shfl_sync(0xffffffffu, of_column[x], (2 * t4 + b) * 4);
+        }
       }
 #pragma unroll
       for (int k = 0; k < DK / 16; ++k) {
@@ -355,7 +361,7 @@ __global__ void __launch_bounds__(LinearTiles<BF16, DK, DV>::THREADS, LinearTile
         for (int w = 0; w < 4; ++w) {
           const float(&s)[4] = S[2 * k + (w & 1)];
           float a = s[w & 2], b = s[(w & 2) + 1];
-          if constexpr (!BF16) { a *= up; b *= up; }
+          if constexpr (!BF16) { a *= up[w >> 1]; b *= up[w >> 1]; }
           hi[w] = narrow<BF16>(a, b);
           if constexpr (BF16) {
             const float2 taken = widen<BF16>(hi[w]);
@@ -383,16 +389,21 @@ __global__ void __launch_bounds__(LinearTiles<BF16, DK, DV>::THREADS, LinearTile
       const int64_t step_y = p.y.row * 8;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float f0 = s_power[16 * i + g8 + 1] * down, f1 = s_power[16 * i + g8 + 9] * down;
+        const float f0 = s_power[16 * i + g8 + 1], f1 = s_power[16 * i + g8 + 9];
 #pragma unroll
-        for (int x = 0; x < 2; ++x) { o[i][x][0] *= f0; o[i][x][1] *= f0; o[i][x][2] *= f1; o[i][x][3] *= f1; }
+        for (int x = 0; x < 2; ++x) {
+          if constexpr (!BF16) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[i][x][e] *= down[x][e & 1];
+          }
+          o[i][x][0] *= f0; o[i][x][1] *= f0; o[i][x][2] *= f1; o[i][x][3] *= f1;
+        }
       }
       // a column of blocks of scores at a time: their products wait for one another only where they are of the same rows
       auto column = [&](auto place) {
         constexpr int j = decltype(place)::value;
         if (bad) {
           const int block = j * (j + 1) / 2 + j;
-          const float f = BF16 ? 1.f : s_block[block];
 #pragma unroll 1
           for (int s = 0; s < 16; ++s)
 #pragma unroll
@@ -402,7 +413,7 @@ __global__ void __launch_bounds__(LinearTiles<BF16, DK, DV>::THREADS, LinearTile
               float w = widen<BF16>(*reinterpret_cast<const uint16_t*>(s_scores + at)).x;
               if constexpr (BF16) w += widen<BF16>(*reinterpret_cast<const uint16_t*>(s_scores + L::SCORES + at)).x;
               const uint16_t u = *reinterpret_cast<const uint16_t*>(smem + (sv - base) + tile_at<DV>(16 * j + s, c >> 3) + (c & 7) * 2);
-              if (s <= row) o[j][e >> 2][e & 3] = fmaf(w * f, widen<BF16>(u).x, o[j][e >> 2][e & 3]);
+              if (s <= row) o[j][e >> 2][e & 3] = fmaf(BF16 ? w : w * s_down[block * 16 + row], widen<BF16>(u).x, o[j][e >> 2][e & 3]);
             }
           __syncwarp();
         }
@@ -441,11 +452,12 @@ __global__ void __launch_bounds__(LinearTiles<BF16, DK, DV>::THREADS, LinearTile
               }
 #pragma unroll
               for (int i = I; i < 4; ++i) {
-                const float f = s_block[i * (i + 1) / 2 + j];
+                const float* f = s_down + (i * (i + 1) / 2 + j) * 16 + g8;
+                const float of_row[2] = {f[0], f[8]};
 #pragma unroll
                 for (int x = 0; x < 2; ++x)
 #pragma unroll
-                  for (int e = 0; e < 4; ++e) o[i][x][e] = fmaf(c[i - I][x][e], f, o[i][x][e]);
+                  for (int e = 0; e < 4; ++e) o[i][x][e] = fmaf(c[i - I][x][e], of_row[e >> 1], o[i][x][e]);
               }
             }
           }
@@ -478,19 +490,23 @@ __global__ void __launch_bounds__(LinearTiles<BF16, DK, DV>::THREADS, LinearTile
       }
     }
     // S' = g^n S + (g^.. V)^T K
-    float up = 1.f, down = 1.f;
+    [[maybe_unused]] float up[2], down[2];                                     // (of columns g8 and g8 + 8)
     if constexpr (!BF16) {
-      fp16_scale(top_of([&](auto take) {
+      float top[2];
+      tops_of(
+          [&](auto take) {
 #pragma unroll
-                   for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
-                     for (int e = 0; e < 4; ++e) {
-                       const float2 x = widen<BF16>(v[i][e]);
-                       take(x.x);
-                       take(x.y);
-                     }
-                 }),
-                 up, down);
+              for (int e = 0; e < 4; ++e) {
+                const float2 x = widen<BF16>(v[i][e]);
+                take(e >> 1, x.x);
+                take(e >> 1, x.y);
+              }
+          },
+          top);
+#pragma unroll
+      for (int x = 0; x < 2; ++x) fp16_scale(top[x], up[x], down[x]);
     }
     // decay behind rows 16 i + 8 e + 2 t4 and the next (rows behind the end are zeros)
     float weight[4][2][2];
@@ -499,7 +515,7 @@ __global__ void __launch_bounds__(LinearTiles<BF16, DK, DV>::THREADS, LinearTile
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float f = s_power[LT_ROWS - 8 - 16 * i - 8 * e] * up;
+          const float f = s_power[LT_ROWS - 8 - 16 * i - 8 * e];
           weight[i][e][0] = f * last_f[0];
           weight[i][e][1] = f * last_f[1];
         }
@@ -507,7 +523,7 @@ __global__ void __launch_bounds__(LinearTiles<BF16, DK, DV>::THREADS, LinearTile
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) weight[i][e >> 1][e & 1] = s_power[max(n - 1 - 16 * i - (e >> 1) * 8 - 2 * t4 - (e & 1), 0)] * up;
+        for (int e = 0; e < 4; ++e) weight[i][e >> 1][e & 1] = s_power[max(n - 1 - 16 * i - (e >> 1) * 8 - 2 * t4 - (e & 1), 0)];
     }
     uint32_t term[L::TERMS_S][4][4];
 #pragma unroll
@@ -515,7 +531,8 @@ __global__ void __launch_bounds__(LinearTiles<BF16, DK, DV>::THREADS, LinearTile
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         // (a word is two rows of one column: 16 i + 2 t4, eight further for odd words)
-        const float2 x = widen<BF16>(v[i][e]);
+        float2 x = widen<BF16>(v[i][e]);
+        if constexpr (!BF16) { x.x *= up[e >> 1]; x.y *= up[e >> 1]; }
         float a = x.x * weight[i][e & 1][0], b = x.y * weight[i][e & 1][1];
         // an operand's words: dv g8, rows first half; dv g8 + 8; dv g8, second half; dv g8 + 8
         const int w = (e & 1) * 2 + (e >> 1);
@@ -550,7 +567,7 @@ __global__ void __launch_bounds__(LinearTiles<BF16, DK, DV>::THREADS, LinearTile
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           float& s = S[2 * j + x][e];
-          s = fmaf(s, decay.by, fmaf(s, keep, BF16 ? c[x][e] : c[x][e] * down));
+          s = fmaf(s, decay.by, fmaf(s, keep, BF16 ? c[x][e] : c[x][e] * down[e >> 1]));
         }
     }
     if (L::BUFFERS == 1 && r0 + LT_ROWS < g.end) {
