@@ -73,3 +73,13 @@ def test_rows_of_queries(dtype, dk, dv):
     q = q.clamp(-3.5, 3.5) * _sizes(1570, -13, 14, 7)[:, None, None]
     for big in (1.0, 2.0 ** 12):
         _check(*(t.to(T_[dtype]) for t in (q, k.clamp(-3.5, 3.5) * big, v)), None, 1.0 / big, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("size", [1e-26, 1e-20, 1e20, 1e30, 1e33, 1e36])
+def test_states_near_the_end_of_fp32(dtype, size):
+    q, k, v = _normal(1570, 2, 64, seed=1), _normal(1570, 1, 64, seed=2), _normal(1570, 1, 64, seed=3)
+    h = (_normal(3, 2, 64, 64, seed=5).double() * size).float()
+    if size < 1:
+        k, v = k * 0, v * 0                                              # (else nothing of the kept states would be left to see)
+    _check(*(t.to(T_[dtype]) for t in (q, k, v)), h, 1.0 / size, dtype, slowest=9.0)

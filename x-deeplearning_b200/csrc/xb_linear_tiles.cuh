@@ -49,8 +49,8 @@ __device__ __forceinline__ uint32_t tile_at(int row, int piece) { return (uint32
 
 // the power of two that puts `top`, the largest of some sizes, at 2^14 (and one over it)
 __device__ __forceinline__ void fp16_scale(float top, float& up, float& down) {
-  // (0: as it is; small numbers of fp32: the end of what has a reciprocal)
-  const int e = top > 0.f ? min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 100) : 14;
+  // (0: as it is; small numbers of fp32: the end of what has a reciprocal. Any finite exponent above has one.)
+  const int e = top > 0.f ? max((int)(__float_as_uint(top) >> 23) - 127, -100) : 14;
   up = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
   down = __uint_as_float((uint32_t)(127 - 14 + e) << 23);
 }
