@@ -23,11 +23,11 @@ inline bool heads_meet_ends(const Heads& a, int na, int da, int64_t rows_a, cons
   return p < q + (uintptr_t)(((rows_b - 1) * b.row + heads_width(b.head, nb, db)) * size) && q < p + (uintptr_t)(((rows_a - 1) * a.row + heads_width(a.head, na, da)) * size);
 }
 // Whether two sets of rows share memory. Told exactly where both have one row stride and the heads of a row
-// lie within it (one set may take other columns than the other), else by where they begin and end.
+// lie within it (one set may take other columns than the other), else by where they begin and end (one row's stride says nothing).
 inline bool heads_meet(const Heads& a, int na, int da, const Heads& b, int nb, int db, int64_t rows, int64_t size) {
   if (!a.at || !b.at || rows < 1 || na < 1 || nb < 1) return false;
   const int64_t wa = heads_width(a.head, na, da), wb = heads_width(b.head, nb, db);
-  if (rows == 1 || (a.row == b.row && wa <= a.row && wb <= b.row)) return rows_meet(a.at, a.row * size, wa * size, b.at, b.row * size, wb * size, rows);
+  if (rows > 1 && a.row == b.row && wa <= a.row && wb <= b.row) return rows_meet(a.at, a.row * size, wa * size, b.at, b.row * size, wb * size, rows);
   return heads_meet_ends(a, na, da, rows, b, nb, db, rows, size);
 }
 inline bool heads_whole(const Heads& a, int64_t size, int64_t unit) {
