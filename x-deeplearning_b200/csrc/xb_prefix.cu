@@ -14,13 +14,17 @@ struct PrefixScratch {
   size_t own_weight, groups, begins, records, part, part_ml, bytes;      // (the items lie first)
   int max_items, ctas, part_rows, n_groups;
 };
+// items that a call may have: two tiles each, and one more for every prefix
+int64_t most_items(const xb_prefix_attention_args& a) {
+  return a.rows / (2 * (PFX_ROWS / (a.H / a.Hkv))) + std::min<int64_t>(a.rows, a.prefixes == 0 ? 1 : (int64_t)a.prefixes + 2);
+}
 PrefixScratch prefix_scratch(const xb_prefix_attention_args& a) {
   auto align256 = [](size_t n) { return (n + 255) / 256 * 256; };
   PrefixScratch w;
   const int64_t share = a.H / a.Hkv, R = PFX_ROWS / share;
   w.ctas = std::min(std::max(sm_count(), 1), JOIN_MOST / PFX_SLOTS);
   w.n_groups = a.prefixes == 0 ? 1 : a.prefixes + 2;
-  w.max_items = (int)(a.rows / (2 * R) + std::min<int64_t>(a.rows, w.n_groups));
+  w.max_items = (int)most_items(a);
   w.part_rows = (int)std::min<int64_t>(2 * R, a.rows) * (int)share;
   const size_t slots = (size_t)w.ctas * PFX_SLOTS;
   w.own_weight = align256((size_t)w.max_items * sizeof(PrefixItem));
@@ -41,10 +45,13 @@ int check_prefix(const xb_prefix_attention_args* a) {
   XB_REQUIRE(a->d <= PFX_MAX_D && a->H / a->Hkv <= PFX_ROWS && a->H <= 65535, XB_ERR_LIMIT, "xb_prefix_attention: %d heads on %d of %d, at most 65535, 128 on one, of 128",
              a->H, a->Hkv, a->d);
   XB_REQUIRE(a->rows >= 0 && a->own_rows >= 0 && a->prefix_rows >= 0 && a->batch >= 0 && a->prefixes >= 0, XB_ERR_ARG, "xb_prefix_attention: a negative size");
-  XB_REQUIRE(a->batch <= MOST && a->prefixes <= MOST, XB_ERR_LIMIT, "xb_prefix_attention: %d lists, %d prefixes, at most 2^31 - 1024", a->batch, a->prefixes);
+  // (groups and items are counted in 32 bits, a block of 1024 threads at a time)
+  XB_REQUIRE(a->batch <= MOST && a->prefixes <= MOST - 1024, XB_ERR_LIMIT, "xb_prefix_attention: %d lists, at most 2^31 - 1024, %d prefixes, at most 2^31 - 2048", a->batch,
+             a->prefixes);
   constexpr int64_t ROWS = ((int64_t)1 << 31) - 1024;      // (blocks of 128 rows are counted in 32 bits)
   XB_REQUIRE(a->rows <= ROWS && a->own_rows <= ROWS && a->prefix_rows <= ROWS, XB_ERR_LIMIT, "xb_prefix_attention: %lld, %lld and %lld rows, at most 2^31 - 1024",
              (long long)a->rows, (long long)a->own_rows, (long long)a->prefix_rows);
+  XB_REQUIRE(most_items(*a) <= MOST, XB_ERR_LIMIT, "xb_prefix_attention: %lld rows and %d prefixes are too many for one call", (long long)a->rows, a->prefixes);
   XB_REQUIRE(a->scale > 0 && a->scale <= 3.0e38f, XB_ERR_ARG, "xb_prefix_attention: scale %g", (double)a->scale);
   if (a->batch == 0 || a->rows == 0) return 0;
   XB_REQUIRE(a->offsets || a->rows % a->batch == 0, XB_ERR_ARG, "xb_prefix_attention: without offsets %d lists divide %lld rows", a->batch, (long long)a->rows);

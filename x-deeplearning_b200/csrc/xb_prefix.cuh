@@ -232,7 +232,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) prefix_plan_kernel(const __grid_
     const int64_t at = total + block_scan(n, s_sums, sum);
     x.first = (int)min(at, (int64_t)p.max_items);
     // (members that do not ascend name lists twice: a group has the tiles of the items that there is room for)
-    if (at + n > p.max_items) x.tiles = min(x.tiles, 2 * (p.max_items - x.first));
+    if (at + n > p.max_items) x.tiles = (int)min((int64_t)x.tiles, 2 * ((int64_t)p.max_items - x.first));
     if (g < n_groups) groups[g] = x;
     total += sum;
   }
