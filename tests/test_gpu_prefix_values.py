@@ -1,0 +1,57 @@
+"""xb_prefix_attention on infinities and NaN of several rows at once."""
+import numpy as np
+import pytest
+import torch
+
+import pkg
+
+pytestmark = pytest.mark.gpu
+
+T_ = {"f16": torch.float16, "bf16": torch.bfloat16}
+
+
+def _ops():
+    pkg.load()
+    from x_deeplearning_b200 import ops
+    return ops
+
+
+def _normal(*shape, dtype, seed, std=0.3):
+    return torch.from_numpy(np.random.default_rng(seed).normal(0, std, shape)).to("cuda", T_[dtype])
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("lists,T,prefix", [(1, 300, 0), (1, 300, 70), (1, 40, 20_000), (1, 300, 3000), (2500, 40, 0), (2500, 40, 70)])
+def test_two_bad_rows(dtype, d, lists, T, prefix):
+    """A NaN among the keys of one row and an infinity among the values of another: whoever sees both has NaN. So has who sees infinities of both signs."""
+    ops = _ops()
+    q, k, v = (_normal(lists * T, 2, d, dtype=dtype, seed=s) for s in range(3))
+    kw = dict(scale=d ** -0.5, T=T)
+    if prefix:
+        kw.update(prefix_k=_normal(prefix, 2, d, dtype=dtype, seed=3), prefix_v=_normal(prefix, 2, d, dtype=dtype, seed=4))
+    good = ops.prefix_attention(q, k, v, **kw)
+    first = lists // 2 * T
+    a, b, end = first + 10, first + 25, first + T
+    for nan, inf in ((a, b), (b, a)):
+        bad_k, bad_v = k.clone(), v.clone()
+        bad_k[nan, 0, 5], bad_v[inf, 0, 3] = float("nan"), float("inf")
+        y = ops.prefix_attention(q, bad_k, bad_v, **kw)
+        assert torch.equal(y[:a], good[:a]) and torch.equal(y[end:], good[end:]) and torch.equal(y[:, 1], good[:, 1])
+        assert torch.isnan(y[nan:end, 0].float()).all()
+        if inf < nan:
+            assert (y[inf:nan, 0, 3] == float("inf")).all() and torch.equal(y[inf:nan, 0, 4:], good[inf:nan, 0, 4:])
+    bad_v = v.clone()
+    bad_v[a, 0, 3], bad_v[b, 0, 3] = float("inf"), float("-inf")
+    y = ops.prefix_attention(q, k, bad_v, **kw)
+    assert (y[a:b, 0, 3] == float("inf")).all() and torch.isnan(y[b:end, 0, 3].float()).all()
+    assert torch.equal(y[:, 0, 4:], good[:, 0, 4:]) and torch.equal(y[:a], good[:a]) and torch.equal(y[end:], good[end:])
+    if prefix:
+        for at in (0, prefix - 1):
+            bad_v, bad_pv = v.clone(), kw["prefix_v"].clone()
+            bad_pv[at, 0, 3], bad_v[a, 0, 3] = float("inf"), float("-inf")
+            y = ops.prefix_attention(q, k, bad_v, **{**kw, "prefix_v": bad_pv})
+            assert torch.isnan(y[a:end, 0, 3].float()).all()
+            assert (y[:a, 0, 3] == float("inf")).all() and (y[end:, 0, 3] == float("inf")).all()
+            assert torch.equal(y[:, 0, 4:], good[:, 0, 4:]) and torch.equal(y[:, 1], good[:, 1])
+    assert ops.device_status() == 0

@@ -491,7 +491,8 @@ __device__ __forceinline__ bool each_piece(C& ctl, int lane, F visit) {
   }
 }
 
-// Infinities and NaN among own values, which the products were made without: they are what they are whatever is added to them. For a row's columns [c0, c1) and keys [k0, k1).
+// Infinities and NaN among own values, which the products were made without, added to a row's results or sums (whose own, of a prefix or of scores, they
+// meet there). For columns [c0, c1) and keys [k0, k1).
 template <bool BF16>
 __device__ __noinline__ void spread_bad(const Heads v, int64_t row0, int head, int c0, int c1, int k0, int k1, uint16_t* y, float* part, int64_t part_step) {
   for (int c = c0; c < c1; ++c) {
@@ -501,8 +502,12 @@ __device__ __noinline__ void spread_bad(const Heads v, int64_t row0, int head, i
       if (half_is_bad<BF16>(t)) sum += BF16 ? __uint_as_float((uint32_t)t << 16) : __half2float(__ushort_as_half(t));
     }
     if (sum == 0.f) continue;
-    if (y) y[c] = (uint16_t)pack_weights<BF16>(sum, sum);
-    else part[(c / 4) * part_step + c % 4] = sum;
+    if (y) {
+      sum += BF16 ? __uint_as_float((uint32_t)y[c] << 16) : __half2float(__ushort_as_half(y[c]));
+      y[c] = (uint16_t)pack_weights<BF16>(sum, sum);
+    } else {
+      part[(c / 4) * part_step + c % 4] += sum;
+    }
   }
 }
 
