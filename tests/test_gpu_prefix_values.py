@@ -1,4 +1,4 @@
-"""xb_prefix_attention on infinities and NaN of several rows at once."""
+"""xb_prefix_attention: infinities and NaN of several rows at once, and scores that are all -infinity."""
 import numpy as np
 import pytest
 import torch
@@ -54,4 +54,45 @@ def test_two_bad_rows(dtype, d, lists, T, prefix):
             assert torch.isnan(y[a:end, 0, 3].float()).all()
             assert (y[:a, 0, 3] == float("inf")).all() and (y[end:, 0, 3] == float("inf")).all()
             assert torch.equal(y[:, 0, 4:], good[:, 0, 4:]) and torch.equal(y[:, 1], good[:, 1])
+    assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_scores_that_are_all_minus_infinity(dtype, d):
+    """Rows that see such keys alone are 0 / 0; with a finite score beside them these keys take no part; a row that sees no key has zeros."""
+    ops = _ops()
+    inf = float("inf")
+    lens, own = [3, 1, 130, 2, 300], [3, 0, 130, 1, 300]
+    off, own_off = (torch.tensor(np.r_[0, np.cumsum(n)], dtype=torch.int32, device="cuda") for n in (lens, own))
+    starts, own_starts = np.r_[0, np.cumsum(lens)], np.r_[0, np.cumsum(own)]
+    q, k, v = _normal(sum(lens), 2, d, dtype=dtype, seed=0), _normal(sum(own), 1, d, dtype=dtype, seed=1), _normal(sum(own), 1, d, dtype=dtype, seed=2)
+    q[:, :, 0] = 1.0
+    kw = dict(offsets=off, own_offsets=own_off, scale=0.25)
+    k[:, :, 0] = -inf
+    y = ops.prefix_attention(q, k, v, **kw)
+    none = torch.zeros(len(q), dtype=torch.bool, device="cuda")
+    none[int(starts[1])] = True                                          # a list without own rows
+    none[int(starts[3])] = True                                          # two queries, one own row: the first sees none
+    assert (y[none] == 0).all() and torch.isnan(y[~none].float()).all()
+    # a finite key in the middle of the last list
+    k[int(own_starts[4]) + 140, 0, 0] = 0.0
+    y = ops.prefix_attention(q, k, v, **kw)
+    at = int(starts[4]) + 140
+    assert torch.isnan(y[int(starts[4]):at].float()).all()
+    assert torch.equal(y[at:], v[int(own_starts[4]) + 140].expand(2, d)[None].expand(len(q) - at, 2, d))
+    # prefixes, short and of many CTAs, with and without such a key
+    for n in (70, 256, 30_000):
+        for rows in (1, 50, 300):
+            pk, pv = _normal(n, 1, d, dtype=dtype, seed=3), _normal(n, 1, d, dtype=dtype, seed=4)
+            pk[:, :, 0] = -inf
+            call = dict(T=1, prefix_k=pk, prefix_v=pv, scale=0.25)
+            q1 = q[:rows]
+            assert torch.isnan(ops.prefix_attention(q1, **call).float()).all()
+            pk[n // 3, 0, 0] = 0.0
+            assert torch.equal(ops.prefix_attention(q1, **call), pv[n // 3].expand(2, d)[None].expand(rows, 2, d))
+            pk[n // 3, 0, 0] = -inf
+            k1, v1 = k[:rows].clone(), v[:rows]
+            k1[:, :, 0] = 0.0
+            assert torch.equal(ops.prefix_attention(q1, k1, v1, **call), v1.expand(rows, 2, d))
     assert ops.device_status() == 0

@@ -986,6 +986,14 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         tc_fence_after_sync();
         bad = x.k1 > x.prefix_blocks && *reinterpret_cast<volatile int*>(&ctl.bad[pieces & 1]) == pieces + 1;
         if (bad && !known) know();
+        // A row that sees keys and has no weight: its scores are all -infinity, 0 / 0. In a piece a sum of 1 says so (without a maximum it adds nothing).
+        if (__any_sync(0xffffffffu, there && all == 0.f)) {
+          if (!known) know();
+          // (of the own blocks that its tile went through: offsets that do not ascend name others too)
+          const int from = x.two && w == 1 ? max(x.k0, x.hole1) : x.k0, to = x.two && w == 0 ? x.of(0).end : x.k1;
+          const int own_lo = max(lo, max(from - x.prefix_blocks, 0) * PFX_KEYS), own_hi = min(hi, max(to - x.prefix_blocks, 0) * PFX_KEYS);
+          if (there && all == 0.f && (x.k0 < x.prefix_blocks || own_lo < own_hi)) all = x.whole ? NAN : 1.f;
+        }
       }
       const int slot = blockIdx.x * PFX_SLOTS + x.slot, part_row = tile * p.R * p.share + row;
       const float by = !x.whole ? 1.f : all > 0.f ? 1.f / all : all;                          // (no weight: zeros; NaN as it is)
@@ -1172,6 +1180,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) prefix_join_kernel(const PrefixP
     if (row >= s_rows[k] || col >= p.d) continue;
     // (sums so far, and what the next piece moves them by)
     float top = -INFINITY, all = 0.f;
+    bool seen = false;                     // scores of -infinity
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int i0 = 0; i0 < n; i0 += JOIN_AHEAD) {
       float4 v[JOIN_AHEAD];
@@ -1188,11 +1197,12 @@ __global__ void __launch_bounds__(JOIN_THREADS) prefix_join_kernel(const PrefixP
         const float next = fmaxf(top, ml[i].x);
         const float f = ml[i].x == -INFINITY ? 0.f : ex2((ml[i].x - next) * p.scale), back = top == next || top == -INFINITY ? 1.f : ex2((top - next) * p.scale);
         top = next;
+        seen |= ml[i].x == -INFINITY && ml[i].y != 0.f;
         all = fmaf(ml[i].y, f, all * back);
         o.x = fmaf(v[i].x, f, o.x * back); o.y = fmaf(v[i].y, f, o.y * back); o.z = fmaf(v[i].z, f, o.z * back); o.w = fmaf(v[i].w, f, o.w * back);
       }
     }
-    const float by = all > 0.f ? 1.f / all : all;
+    const float by = all > 0.f ? 1.f / all : seen ? NAN : all;
     uint16_t* y = const_cast<uint16_t*>(p.y.get<uint16_t>((int64_t)p.items[item].row0 + row / p.share, head * p.share + row % p.share)) + col;
     const uint32_t low = pack_weights<BF16>(o.x * by, o.y * by), high = pack_weights<BF16>(o.z * by, o.w * by);
     if (p.vec_y) {
