@@ -642,7 +642,7 @@ int xb_linear_attention(const xb_linear_attention_args* args, void* workspace, s
  * Offsets and members ascend and are cut to what exists; where they do not, results are open, and nothing outside the arrays is touched. A query
  * that sees no row gets zeros, one whose scores are all -infinity NaN. Heads h of q read head h / (H / Hkv) of the keys. fp16 or bf16; d a multiple of 8, at most 128; at most 128 heads on one;
  * rows of q, k, v, prefix_k and prefix_v on 16 bytes, their strides at least d. Scores, maxima, sums and products are fp32, the weights of a product
- * with values rounded to the inputs' type (half a step, of a weight at most 256 times the largest). An infinity or NaN in a row reaches the queries
+ * with values rounded to the inputs' type (half a step; those below fp16's range to 2^-32 of the largest). An infinity or NaN in a row reaches the queries
  * that see it and no others. */
 typedef struct xb_prefix_attention_args {
   const void* q; int64_t q_row, q_head;                        /* [rows, H, d] */

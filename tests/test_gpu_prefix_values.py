@@ -1,4 +1,4 @@
-"""xb_prefix_attention: infinities and NaN of several rows at once, and scores that are all -infinity."""
+"""xb_prefix_attention: infinities and NaN of several rows at once, scores that are all -infinity, and many small weights beside a large one."""
 import numpy as np
 import pytest
 import torch
@@ -96,3 +96,21 @@ def test_scores_that_are_all_minus_infinity(dtype, d):
             k1[:, :, 0] = 0.0
             assert torch.equal(ops.prefix_attention(q1, k1, v1, **call), v1.expand(rows, 2, d))
     assert ops.device_status() == 0
+
+
+def test_many_small_weights():
+    """fp16, 200 prefixes of 20 000 keys: one key of each takes all but 2^-26 for every other, whose values are 1 and the first one's 0.
+    A weight is known to half of fp16's smallest step, 2^-25, where the largest is 2^7 or more: to 2^-32 of that, and 20 000 of them to 2^-17.7."""
+    ops = _ops()
+    n, d = 20_000, 8
+    q = torch.zeros(200, 1, d, device="cuda", dtype=torch.float16)
+    q[:, :, 0] = 1.0
+    pk = torch.zeros(200, n, 1, d, device="cuda", dtype=torch.float16)
+    pk[:, :, :, 0] = -18.0
+    pk[:, 0] = 0.0
+    pv = torch.ones(200, n, 1, d, device="cuda", dtype=torch.float16)
+    pv[:, 0] = 0.0
+    y = ops.prefix_attention(q, T=1, prefix_k=pk.flatten(0, 1), prefix_v=pv.flatten(0, 1), prefix_offsets=torch.arange(201, device="cuda", dtype=torch.int32) * n)
+    rest = (n - 1) * np.exp(-18.0)
+    want = rest / (1 + rest)
+    assert np.abs(y.double().cpu().numpy() - want).max() <= n * 2.0 ** -32 + want * (2.0 ** -11 + 2.0 ** -15) + 2.0 ** -25

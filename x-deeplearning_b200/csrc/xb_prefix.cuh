@@ -13,7 +13,8 @@
 // In a CTA (16 warps) two groups of four warps make weights of scores, each with a warp that issues its MMAs and with scores, weights and sums of its own
 // in tensor memory: one tile each of an item of two, whose keys they share, or of a single tile every other block of keys. While one makes weights,
 // the tensor cores are at the other's. A thread has a row; a maximum that has not grown by more than 2^8 leaves the sums as they are (weights up to
-// 256 fit both types), so that they are seldom moved. One more warp loads (TMA), one works the pieces out ahead of the others, and four clear what must
+// 256 times that of the maximum in use fit both types), so that they are seldom moved. fp16 weights are 2^7 times as large: below that one's range they are known to
+// 2^-32 of the largest, not 2^-25. One more warp loads (TMA), one works the pieces out ahead of the others, and four clear what must
 // not take part of the blocks of values that some row sees in part (in the groups themselves that was a sixth of the time of short lists).
 //
 // What bounds it is neither memory nor the tensor cores but the way from scores to weights: 128 exponentials a row and block at 16 a cycle and SM, 1024
@@ -35,6 +36,8 @@ namespace {
 constexpr int PFX_KEYS = 128, PFX_ROWS = 128, PFX_THREADS = 512, PFX_LOADER = 8, PFX_MMA = 9, PFX_SLOTS = 4;
 constexpr int PFX_RING = 2, PFX_TAKERS = 15;               // pieces ahead; warps that take them
 constexpr float PFX_GROWTH = 8.f;
+template <bool BF16>
+constexpr float PFX_UP = BF16 ? 0.f : 7.f;                 // the power of two that the weight of a row's maximum is
 
 struct PrefixItem {
   int row0, rows;                          // query rows
@@ -895,12 +898,12 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
 #pragma unroll
             for (int c = 0; c < 128; c += 2) top[c / 2 % 4] = fmaxf(top[c / 2 % 4], fmaxf(__uint_as_float(s[c / 32][c % 32]), __uint_as_float(s[c / 32][c % 32 + 1])));
             if (!move_sums(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])))) return false;
-            float base = m == -INFINITY ? 0.f : m * p.scale;
+            float base = (m == -INFINITY ? 0.f : m * p.scale) - PFX_UP<BF16>;
             if (__any_sync(0xffffffffu, fabsf(base) > 1e6f)) {
               const float off = m == -INFINITY ? 0.f : m;
 #pragma unroll
               for (int c = 0; c < 128; ++c) s[c / 32][c % 32] = __float_as_uint(__uint_as_float(s[c / 32][c % 32]) - off);
-              base = 0.f;
+              base = -PFX_UP<BF16>;
             }
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
@@ -940,7 +943,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                 tmem_wait_ld(q);
 #pragma unroll
                 for (int e = 0; e < 32; ++e) q[e] = seen >> e & 1 ? __float_as_uint(__uint_as_float(q[e]) - off) : 0xff800000u;
-                weigh(q, 0.f, weights);
+                weigh(q, -PFX_UP<BF16>, weights);
               }
               tmem_st16(my_p + c * 16, weights);
             }
