@@ -114,3 +114,34 @@ def test_many_small_weights():
     rest = (n - 1) * np.exp(-18.0)
     want = rest / (1 + rest)
     assert np.abs(y.double().cpu().numpy() - want).max() <= n * 2.0 ** -32 + want * (2.0 ** -11 + 2.0 ** -15) + 2.0 ** -25
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_bad_values_of_long_lists(dtype, d):
+    """One infinity in lists of 60 000 rows, whole, costs what its block costs: the call takes at most three times as long, and the rows ahead of it keep their bits."""
+    ops = _ops()
+    n = 60_000
+    q, k, v = (_normal(2 * n, 1, d, dtype=dtype, seed=s) for s in range(3))
+    kw = dict(scale=d ** -0.5, T=n)
+
+    def run():
+        at = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+        ops.prefix_attention(q, k, v, **kw)
+        at[0].record()
+        y = ops.prefix_attention(q, k, v, **kw)
+        at[1].record()
+        torch.cuda.synchronize()
+        return y, at[0].elapsed_time(at[1])
+
+    good, ms = run()
+    for at in (0, 31_000, n - 1, n, n + 40_100):
+        kept = v[at].clone()
+        v[at, 0, 3] = float("inf")
+        y, bad_ms = run()
+        v[at] = kept
+        end = n if at < n else 2 * n
+        assert (y[at:end, 0, 3] == float("inf")).all()
+        assert torch.equal(y[:at], good[:at]) and torch.equal(y[end:], good[end:]) and torch.equal(y[:, :, 4:], good[:, :, 4:])
+        assert bad_ms < 3 * ms, (bad_ms, ms)
+    assert ops.device_status() == 0

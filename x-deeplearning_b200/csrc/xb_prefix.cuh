@@ -360,7 +360,10 @@ struct PrefixShape {
     uint64_t piece_full[PFX_RING], piece_empty[PFX_RING];
     PrefixPiece ring[PFX_RING];
     float2 ml[2][PFX_ROWS];                // maximum and sum of either group's rows
-    int bad[2], lock;
+    // Of the two pieces that are under way the first and the last block in which bad values were found: the piece's number + 1 in the high word, the block
+    // (the first one's counted down) in the low one.
+    unsigned long long bad_first[2], bad_last[2];
+    int lock;
     uint32_t tmem;
   };
   static constexpr int SMEM = (2 * Q + K + V) * TILE + (int)sizeof(Control);
@@ -498,18 +501,28 @@ __device__ __forceinline__ bool each_piece(C& ctl, int lane, F visit) {
 // meet there). For columns [c0, c1) and keys [k0, k1).
 template <bool BF16>
 __device__ __noinline__ void spread_bad(const Heads v, int64_t row0, int head, int c0, int c1, int k0, int k1, uint16_t* y, float* part, int64_t part_step) {
-  for (int c = c0; c < c1; ++c) {
-    float sum = 0.f;
+#pragma unroll 1
+  for (int c = c0; c < c1; c += 8) {       // (rows are on 16 bytes, columns whole pieces of 8)
+    float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
     for (int k = k0; k < k1; ++k) {
-      const uint16_t t = v.get<uint16_t>(row0 + k, head)[c];
-      if (half_is_bad<BF16>(t)) sum += BF16 ? __uint_as_float((uint32_t)t << 16) : __half2float(__ushort_as_half(t));
+      const uint4 t = *reinterpret_cast<const uint4*>(v.get<uint16_t>(row0 + k, head) + c);
+      const uint32_t h[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint16_t x = (uint16_t)(h[e / 2] >> (16 * (e & 1)));
+        if (half_is_bad<BF16>(x)) sum[e] += BF16 ? __uint_as_float((uint32_t)x << 16) : __half2float(__ushort_as_half(x));
+      }
     }
-    if (sum == 0.f) continue;
-    if (y) {
-      sum += BF16 ? __uint_as_float((uint32_t)y[c] << 16) : __half2float(__ushort_as_half(y[c]));
-      y[c] = (uint16_t)pack_weights<BF16>(sum, sum);
-    } else {
-      part[(c / 4) * part_step + c % 4] += sum;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (sum[e] == 0.f) continue;
+      if (y) {
+        const float all = sum[e] + (BF16 ? __uint_as_float((uint32_t)y[c + e] << 16) : __half2float(__ushort_as_half(y[c + e])));
+        y[c + e] = (uint16_t)pack_weights<BF16>(all, all);
+      } else {
+        part[((c + e) / 4) * part_step + e % 4] += sum[e];
+      }
     }
   }
 }
@@ -536,7 +549,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       mbar_init(smem_u32(&ctl.o_done[w]), 1);
       mbar_init(smem_u32(&ctl.o_free[w]), 256);
       mbar_init(smem_u32(&ctl.drained[w]), 1);
-      ctl.bad[w] = 0;
+      ctl.bad_first[w] = ctl.bad_last[w] = 0;
     }
     for (int r = 0; r < PFX_RING; ++r) { mbar_init(smem_u32(&ctl.piece_full[r]), 1); mbar_init(smem_u32(&ctl.piece_empty[r]), PFX_TAKERS); }
     mbar_init(smem_u32(&ctl.met), 256);
@@ -587,7 +600,9 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
               sick = fma_zero<BF16>(t.w, sick);
             }
             if (half_is_bad<BF16>(sick) || half_is_bad<BF16>(sick >> 16)) {
-              *reinterpret_cast<volatile int*>(&ctl.bad[pieces & 1]) = pieces + 1;
+              const unsigned long long piece = (unsigned long long)(pieces + 1) << 32;
+              atomicMax(&ctl.bad_first[pieces & 1], piece | (unsigned)(INT32_MAX - j));
+              atomicMax(&ctl.bad_last[pieces & 1], piece | (unsigned)j);
 #pragma unroll 1
               for (int e = thread; e < in * 8; e += 128)
 #pragma unroll 1
@@ -989,7 +1004,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         if (have[0] && !wait(&ctl.o_done[w], sn - 1, 96)) return false;
         if (have[1] && !wait(&ctl.o_done[w ^ 1], other - 1, 97)) return false;
         tc_fence_after_sync();
-        bad = x.k1 > x.prefix_blocks && *reinterpret_cast<volatile int*>(&ctl.bad[pieces & 1]) == pieces + 1;
+        bad = x.k1 > x.prefix_blocks && reinterpret_cast<volatile int*>(&ctl.bad_last[pieces & 1])[1] == pieces + 1;
         if (bad && !known) know();
         // A row that sees keys and has no weight: its scores are all -infinity, 0 / 0. In a piece a sum of 1 says so (without a maximum it adds nothing).
         if (__any_sync(0xffffffffu, there && all == 0.f)) {
@@ -1069,7 +1084,8 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       }
       if (bad) {                           // (behind what the warp's lanes have stored)
         __syncwarp();
-        const int k_lo = max(lo, max(x.k0 - x.prefix_blocks, 0) * PFX_KEYS), k_hi = min(hi, (x.k1 - x.prefix_blocks) * PFX_KEYS);
+        const int first = INT32_MAX - reinterpret_cast<volatile int*>(&ctl.bad_first[pieces & 1])[0], last = reinterpret_cast<volatile int*>(&ctl.bad_last[pieces & 1])[0];
+        const int k_lo = max(lo, (first - x.prefix_blocks) * PFX_KEYS), k_hi = min(hi, (last + 1 - x.prefix_blocks) * PFX_KEYS);
         if (there && k_lo < k_hi)
           spread_bad<BF16>(p.v, x.t.own0, x.head, c_begin, min(c_end, p.d), k_lo, k_hi, x.whole ? const_cast<uint16_t*>(p.y.get<uint16_t>(q_row, q_head)) : nullptr,
                            reinterpret_cast<float*>(p.part + (int64_t)slot * (p.d / 4) * p.part_rows + part_row), (int64_t)p.part_rows * 4);
