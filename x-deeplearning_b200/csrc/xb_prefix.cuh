@@ -363,7 +363,7 @@ struct PrefixShape {
     // Of the two pieces that are under way the first and the last block in which bad values were found: the piece's number + 1 in the high word, the block
     // (the first one's counted down) in the low one.
     unsigned long long bad_first[2], bad_last[2];
-    int lock;
+    int lock, progress;
     uint32_t tmem;
   };
   static constexpr int SMEM = (2 * Q + K + V) * TILE + (int)sizeof(Control);
@@ -387,6 +387,22 @@ __device__ __forceinline__ bool mbar_spin(uint32_t bar, uint32_t parity, int sit
 #pragma unroll 1
   for (int i = 0; i < PFX_TRIES; ++i)
     if (umma::mbar_try_wait_for(bar, parity, 1000u)) return true;
+  umma::wait_gave_up(site);
+  return false;
+}
+// One that may last as long as a piece, whose blocks only the memory bounds (a group of warps that has nothing to do in it waits for what comes behind): the limit
+// is on the time in which nothing goes on (`progress`: blocks asked for). Everywhere it would cost 4 to 8 %.
+__device__ __forceinline__ bool mbar_spin_long(uint32_t bar, uint32_t parity, const int* progress, int site) {
+  if (umma::mbar_try_wait(bar, parity)) return true;
+  int seen = -1;
+#pragma unroll 1
+  for (int now = 0; now != seen;) {
+    seen = now;
+#pragma unroll 1
+    for (int i = 0; i < PFX_TRIES; ++i)
+      if (umma::mbar_try_wait_for(bar, parity, 1000u)) return true;
+    now = *reinterpret_cast<const volatile int*>(progress);
+  }
   umma::wait_gave_up(site);
   return false;
 }
@@ -483,12 +499,13 @@ __device__ __forceinline__ void make_pieces(const PrefixParams& p, F put) {
     at.unit = chunk_begin(p.groups[at.group], at.chunk);
   }
 }
-// false: a wait ran out
-template <typename C, typename F>
+// false: a wait ran out. AHEAD: a warp that may be done with pieces that others are still at (the loader, the MMAs and the clearing go through all blocks).
+template <bool AHEAD, typename C, typename F>
 __device__ __forceinline__ bool each_piece(C& ctl, int lane, F visit) {
 #pragma unroll 1
   for (int n = 0;; ++n) {
-    if (!__all_sync(0xffffffffu, mbar_spin(umma::smem_u32(&ctl.piece_full[n % PFX_RING]), (uint32_t)(n / PFX_RING) & 1u, 80))) return false;
+    const uint32_t full = umma::smem_u32(&ctl.piece_full[n % PFX_RING]), parity = (uint32_t)(n / PFX_RING) & 1u;
+    if (!__all_sync(0xffffffffu, AHEAD ? mbar_spin_long(full, parity, &ctl.progress, 80) : mbar_spin(full, parity, 80))) return false;
     const PrefixPiece x = ctl.ring[n % PFX_RING];
     __syncwarp();
     if (lane == 0) umma::mbar_arrive(umma::smem_u32(&ctl.piece_empty[n % PFX_RING]));
@@ -553,7 +570,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
     }
     for (int r = 0; r < PFX_RING; ++r) { mbar_init(smem_u32(&ctl.piece_full[r]), 1); mbar_init(smem_u32(&ctl.piece_empty[r]), PFX_TAKERS); }
     mbar_init(smem_u32(&ctl.met), 256);
-    ctl.lock = 0;
+    ctl.lock = ctl.progress = 0;
     fence_barrier_init();
     prefetch_tensormap(&map_q);
     prefetch_tensormap(&map_k);
@@ -574,7 +591,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
     // infinities and NaN too (what they are to the rows that see them is made up for at the end).
     const int thread = threadIdx.x & 127;
     int vn = 0, pieces = 0;
-    each_piece(ctl, lane, [&](const PrefixPiece& x) {
+    each_piece<false>(ctl, lane, [&](const PrefixPiece& x) {
       if (x.empty) return true;
 #pragma unroll 1
       for (int j = x.k0; j < x.k1; ++j, ++vn) {
@@ -632,7 +649,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
     if (warp == PFX_LOADER) {
       int qn = 0, kn = 0, vn = 0;          // items and blocks asked for so far
       bool ok = true;
-      each_piece(ctl, lane, [&](const PrefixPiece& x) {
+      each_piece<false>(ctl, lane, [&](const PrefixPiece& x) {
         if (x.empty) return true;
         const int qs = qn % T::Q;
         if (!(ok = __all_sync(0xffffffffu, mbar_spin(smem_u32(&ctl.q_empty[qs]), ((uint32_t)(qn / T::Q) & 1u) ^ 1u, 81)))) return false;
@@ -663,6 +680,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
             mbar_arrive_expect_tx(full, (uint32_t)T::TILE);
 #pragma unroll
             for (int b = 0; b < DP / 64; ++b) tma_load_3d(dst + b * T::BOX, map, full, b * 64, x.head, row);
+            atomicAdd(&ctl.progress, 1);
           }
           kn += keys;
           vn += !keys;
@@ -678,7 +696,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       int n = 0;
       bool ok = true;
       auto put = [&](const PrefixPiece& x) {
-        if (!(ok = __all_sync(0xffffffffu, mbar_spin(smem_u32(&ctl.piece_empty[n % PFX_RING]), ((uint32_t)(n / PFX_RING) & 1u) ^ 1u, 79)))) return false;
+        if (!(ok = __all_sync(0xffffffffu, mbar_spin_long(smem_u32(&ctl.piece_empty[n % PFX_RING]), ((uint32_t)(n / PFX_RING) & 1u) ^ 1u, &ctl.progress, 79)))) return false;
         if (lane == 0) {
           ctl.ring[n % PFX_RING] = x;
           mbar_arrive(smem_u32(&ctl.piece_full[n % PFX_RING]));
@@ -704,7 +722,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       int on = 0;                                          // its products so far
       bool ok = true;
       auto wait = [&](uint64_t* bar, int phase, int site) { return ok = __all_sync(0xffffffffu, mbar_spin(smem_u32(bar), (uint32_t)phase & 1u, site)); };
-      each_piece(ctl, lane, [&](const PrefixPiece& x) {
+      each_piece<false>(ctl, lane, [&](const PrefixPiece& x) {
         if (x.empty) return true;
         const int qs = qn % T::Q, k_first = kn, v_first = vn;
         if (!wait(&ctl.q_full[qs], qn / T::Q, 85)) return false;
@@ -810,7 +828,10 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
     int other = 0;                                         // the other group's blocks
     int slots = 0;
     auto wait = [&](uint64_t* bar, int phase, int site) { return __all_sync(0xffffffffu, mbar_spin(smem_u32(bar), (uint32_t)phase & 1u, site)); };
-    each_piece(ctl, lane, [&](const PrefixPiece& x) {
+    auto wait_long = [&](uint64_t* bar, int phase, int site) {
+      return __all_sync(0xffffffffu, mbar_spin_long(smem_u32(bar), (uint32_t)phase & 1u, &ctl.progress, site));
+    };
+    each_piece<true>(ctl, lane, [&](const PrefixPiece& x) {
       const int tile = x.two ? w : 0, tile_row = tile * p.R + row / p.share;
       const bool there = row < p.R * p.share && tile_row < x.t.rows;
       const int64_t q_row = (int64_t)x.t.row0 + tile_row;
@@ -852,7 +873,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
           const int in = min(PFX_KEYS, (prefix ? x.t.prefix_n : x.t.own_n) - key0);           // keys of the block
           const bool masked = in < PFX_KEYS || (!prefix && (key0 < (tile ? x.t.begin1 : 0) || key0 + PFX_KEYS > (tile ? x.t.full1 : x.t.full0)));
           if (masked && !prefix && !known) know();
-          if (!wait(&ctl.s_full[w], sn, 92)) return false;
+          if (!wait_long(&ctl.s_full[w], sn, 92)) return false;
           tc_fence_after_sync();
           // Sums so far are moved to a maximum that has grown. (m is -infinity: nothing has been summed; no maximum yet: nothing to move.)
           auto move_sums = [&](float next) {
@@ -1022,7 +1043,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       const int qs = pieces % T::Q;
       const bool staged = p.vec_y && x.whole && !x.empty;
       uint4* stage = reinterpret_cast<uint4*>(smem_q + (qs * 2 + w) * T::TILE);
-      if (staged && !wait(&ctl.q_full[qs], pieces / T::Q, 99)) return false;
+      if (staged && !wait_long(&ctl.q_full[qs], pieces / T::Q, 99)) return false;
       const int c_begin = x.two ? 0 : w * (DP / 2), c_end = x.two ? DP : (w + 1) * (DP / 2);
 #pragma unroll 1
       for (int c0 = c_begin; c0 < c_end; c0 += 32) {
