@@ -22,3 +22,34 @@ def test_pieces_of_seconds():
     torch.cuda.synchronize()
     assert ops.device_status() == 0
     assert (y[:127] == 0).all() and (y[127] == -1).all() and (y[128:] == 1).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("d", [64, 104])
+@pytest.mark.parametrize("rows,rising", [(1, False), (1, True), (200, True)])
+def test_long_sums(dtype, d, rows, rising):
+    """4 000 000 keys of every head in pieces of one block, values about 3, with scores of one size or such that the maximum grows all the way. A weight is
+    off by half a step, a result by one, and a sum by 2^-23 for each 16 of the 16 384 keys that the tensor cores add up at most; 2^-16 is left for the rest (exponentials 2^-21, scores
+    2^-20, sums in fp32)."""
+    pkg.load()
+    from x_deeplearning_b200 import ops
+    n, H = 1 << 22, 160
+    n = n // 8 if rows > 1 else n
+    g = torch.Generator(device="cuda").manual_seed(d)
+    normal = lambda *s: torch.empty(s, device="cuda").normal_(generator=g)
+    k, v = normal(n + H, d), normal(n + H, d) + 3
+    if rising:
+        k[:, 0] = torch.linspace(-40, 40, n + H, device="cuda")
+    k, v = (t.to(dtype).flatten().as_strided((n, H, d), (d, d, 1)) for t in (k, v))
+    q = normal(rows, H, d).to(dtype)
+    q[:, :, 0] = 1.0
+    y = ops.prefix_attention(q, T=1, prefix_k=k, prefix_v=v, scale=0.125)
+    torch.cuda.synchronize()
+    assert ops.device_status() == 0
+    half = torch.finfo(dtype).eps / 2
+    for h in (0, 77, 159):
+        kh, vh = k[:, h].double(), v[:, h].double()
+        for r in {0, rows // 2, rows - 1}:
+            w = torch.softmax(kh @ q[r, h].double() * 0.125, 0)
+            want, size = w @ vh, w @ vh.abs()
+            assert ((y[r, h].double() - want).abs() <= size * (2 * half + 16_384 / 16 * 2.0 ** -23 + 2.0 ** -16)).all()

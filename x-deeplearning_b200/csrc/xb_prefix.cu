@@ -11,7 +11,7 @@ constexpr int PFX_MAX_D = 128;
 constexpr float LOG2_E = 1.4426950408889634f;
 
 struct PrefixScratch {
-  size_t own_weight, groups, begins, records, part, part_ml, bytes;      // (the items lie first)
+  size_t own_weight, groups, begins, records, part, part_ml, kept, bytes;      // (the items lie first)
   int max_items, ctas, part_rows, n_groups;
 };
 // items that a call may have: two tiles each, and one more for every prefix
@@ -33,7 +33,10 @@ PrefixScratch prefix_scratch(const xb_prefix_attention_args& a) {
   w.records = w.begins + align256(((size_t)w.ctas + 1) * sizeof(PrefixAt));
   w.part = w.records + align256(slots * sizeof(PrefixRecord));
   w.part_ml = w.part + align256(slots * w.part_rows * a.d * 4);
-  w.bytes = w.part_ml + align256(slots * w.part_rows * 8);
+  w.kept = w.part_ml + align256(slots * w.part_rows * 8);
+  // (an item has no more blocks than this)
+  const bool long_items = (a.prefix_rows + PFX_KEYS - 1) / PFX_KEYS + (a.own_rows + PFX_KEYS - 1) / PFX_KEYS > PFX_KEPT;
+  w.bytes = w.kept + (long_items ? (size_t)w.ctas * 2 * PFX_ROWS * a.d * 4 : 0);
   return w;
 }
 
@@ -155,6 +158,7 @@ extern "C" int xb_prefix_attention(const xb_prefix_attention_args* a, void* work
   p.records = reinterpret_cast<PrefixRecord*>(ws + w.records);
   p.part = reinterpret_cast<float4*>(ws + w.part);
   p.part_ml = reinterpret_cast<float2*>(ws + w.part_ml);
+  p.kept = w.bytes > w.kept ? reinterpret_cast<float4*>(ws + w.kept) : nullptr;
   p.max_items = w.max_items; p.ctas = w.ctas; p.n_groups = w.n_groups; p.part_rows = w.part_rows;
   CUtensorMap m[5];
   if (int rc = make_heads_map(&m[0], a->dtype, a->q, a->q_row, a->q_head, a->rows, a->H, p.share, a->d, p.R)) return rc;

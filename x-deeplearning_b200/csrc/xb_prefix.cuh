@@ -36,6 +36,7 @@ namespace {
 constexpr int PFX_KEYS = 128, PFX_ROWS = 128, PFX_THREADS = 512, PFX_LOADER = 8, PFX_MMA = 9, PFX_SLOTS = 4;
 constexpr int PFX_RING = 2, PFX_TAKERS = 15;               // pieces ahead; warps that take them
 constexpr float PFX_GROWTH = 8.f;
+constexpr int PFX_KEPT = 128;                              // blocks after which a group's sums are taken out of the tensor cores
 template <bool BF16>
 constexpr float PFX_UP = BF16 ? 0.f : 7.f;                 // the power of two that the weight of a row's maximum is
 
@@ -74,6 +75,7 @@ struct PrefixParams {
   PrefixRecord* records;                   // [CTAs][PFX_SLOTS]
   float4* part;                            // [CTAs][PFX_SLOTS][d / 4][part_rows]: the rows' pieces of four side by side
   float2* part_ml;                         // [CTAs][PFX_SLOTS][part_rows]
+  float4* kept;                            // [CTAs][d / 4][2][128]: sums of either group's rows in long pieces (null: there are none)
   int max_items, ctas, n_groups, part_rows;
 };
 // ---- the plan ----
@@ -544,6 +546,44 @@ __device__ __noinline__ void spread_bad(const Heads v, int64_t row0, int head, i
   }
 }
 
+// The tensor cores cut off what they add below 2^-23 of a running sum, 8 times a block: over 1000 blocks of equal keys that is 0.04 % of the sum, over 32 768
+// 1.4 %. So sums of long pieces leave them every PFX_KEPT blocks, for fp32 ones in the workspace, which are rounded: (those so far, moved from their maximum to m)
+// + the tensor cores', of a row's d columns, when `done` has come to its phase. `back`: the sum goes to tensor memory. False: a wait ran out.
+__device__ __noinline__ bool keep_sums(uint32_t done, uint32_t phase, uint32_t tmem, float4* kept, int d, float* max, float m, float scale, bool more, bool back) {
+  if (!__all_sync(0xffffffffu, mbar_spin(done, phase & 1u, 78))) return false;
+  umma::tc_fence_after_sync();
+  const float before = *max, by = before == m || before == -INFINITY ? 1.f : ex2((before - m) * scale);
+  *max = m;
+#pragma unroll 1
+  for (int c = 0; c < d; c += 16) {
+    uint32_t o[16];
+    umma::tmem_ld16_nowait(tmem + c, o);
+    umma::tmem_wait_ld(o);
+#pragma unroll
+    for (int e = 0; e < 16; e += 4) {
+      if (c + e >= d) break;
+      float4* at = kept + (c + e) / 4 * (2 * PFX_ROWS);
+      float4 t = make_float4(__uint_as_float(o[e]), __uint_as_float(o[e + 1]), __uint_as_float(o[e + 2]), __uint_as_float(o[e + 3]));
+      if (more) {
+        const float4 k = *at;
+        t.x = fmaf(k.x, by, t.x); t.y = fmaf(k.y, by, t.y); t.z = fmaf(k.z, by, t.z); t.w = fmaf(k.w, by, t.w);
+      }
+      if (back) {
+        o[e] = __float_as_uint(t.x); o[e + 1] = __float_as_uint(t.y); o[e + 2] = __float_as_uint(t.z); o[e + 3] = __float_as_uint(t.w);
+      } else {
+        *at = t;
+      }
+    }
+    __syncwarp();                          // the lanes meet ahead of the next access to tensor memory
+    if (back) umma::tmem_st16(tmem + c, o);
+  }
+  if (back) {
+    umma::tmem_wait_st();
+    umma::tc_fence_before_sync();
+  }
+  return true;
+}
+
 template <bool BF16, int DP>
 __global__ void __launch_bounds__(PFX_THREADS, 1)
 prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
@@ -752,6 +792,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         const int end = x.of(w).end;
         int ask = x.of(w).begin, j = end;                // (j: the block whose weights come next; none yet)
         bool first = true;
+        int since = 0;                                   // products since the sums have last been taken out
 #pragma unroll 1
         while (ask < end || j < end) {
           // a block further on than two: the loader may wait for this block's values to be done with
@@ -772,12 +813,13 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
               if (!T::APART && !(ok = held = take(&ctl.lock, lane))) return false;
               tc_fence_after_sync();
 #pragma unroll
-              for (int kk = 0; kk < PFX_KEYS / 16; ++kk) mma_f16_ts_elect(to_o, from_p + kk * 8, v + kk * 128, idesc_o, (!first || kk > 0) ? 1u : 0u);
+              for (int kk = 0; kk < PFX_KEYS / 16; ++kk) mma_f16_ts_elect(to_o, from_p + kk * 8, v + kk * 128, idesc_o, (since > 0 || kk > 0) ? 1u : 0u);
               mma_commit_elect(smem_u32(&ctl.o_done[w]));
               mma_commit_elect(smem_u32(&ctl.v_empty[s]));
               ++vn;
               ++on;
               first = false;
+              if (++since == PFX_KEPT) since = 0;
               if (held && !near) {
                 let_go(&ctl.lock, lane);
                 held = false;
@@ -864,6 +906,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       };
       float m = -INFINITY, l = 0.f;
       int mine = 0;
+      int stop = x.of(w).n > PFX_KEPT ? PFX_KEPT - 1 : -1;                                    // the block behind which sums are taken out, at the last one put back
       if (!x.empty) {
         const int end = x.of(w).end;
 #pragma unroll 1
@@ -881,7 +924,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
               const float by = m == next || m == -INFINITY ? 1.f : ex2((m - next) * p.scale);
               m = next;
               l *= by;
-              if (mine == 0) return true;
+              if (mine % PFX_KEPT == 0) return true;       // (the tensor cores have none)
               if (!wait(&ctl.o_done[w], sn - 1, 93)) return false;
               tc_fence_after_sync();
 #pragma unroll 1
@@ -999,6 +1042,13 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
           mbar_arrive(smem_u32(&ctl.p_ready[w]));
           ++sn;
           if (!known) know();
+          if (mine == stop) {
+            const int last = x.of(w).n - 1;
+            if (!keep_sums(smem_u32(&ctl.o_done[w]), sn - 1, my_o, p.kept + (blockIdx.x * (p.d / 4) * 2 + w) * PFX_ROWS + row, p.d, &ctl.ml[w][row].x, m, p.scale,
+                           mine >= PFX_KEPT, mine == last))
+              return false;
+            stop = min(stop + PFX_KEPT, last);
+          }
         }
       }
       // What a thread has of its row: all columns of a tile of its own, half of them of a tile that both groups share.
