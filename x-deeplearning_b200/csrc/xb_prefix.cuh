@@ -807,7 +807,9 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
               if (!give_back(j, true)) return false;
               const int s = vn % T::V;
               const uint64_t v = make_desc_sw128_mn(uniform(smem_u32(smem_v + s * T::TILE)), T::BOX);
-              if (!wait(x.cleaned(j) ? &ctl.v_clean[s] : &ctl.v_full[s], vn / T::V, 89)) return false;
+              // (v_full first: a buffer is loaded again when the one before has been cleaned, and a phase of v_clean is told from the one before it only then;
+              // blocks that this group gave back may not have been)
+              if (!wait(&ctl.v_full[s], vn / T::V, 89) || (x.cleaned(j) && !wait(&ctl.v_clean[s], vn / T::V, 89))) return false;
               if (first && pieces > 0 && !wait(&ctl.o_free[w], pieces - 1, 90)) return false;
               if (!wait(&ctl.p_ready[w], on, 88)) return false;
               if (!T::APART && !(ok = held = take(&ctl.lock, lane))) return false;
