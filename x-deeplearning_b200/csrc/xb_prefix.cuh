@@ -810,8 +810,9 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
               // (v_full first: a buffer is loaded again when the one before has been cleaned, and a phase of v_clean is told from the one before it only then;
               // blocks that this group gave back may not have been)
               if (!wait(&ctl.v_full[s], vn / T::V, 89) || (x.cleaned(j) && !wait(&ctl.v_clean[s], vn / T::V, 89))) return false;
-              if (first && pieces > 0 && !wait(&ctl.o_free[w], pieces - 1, 90)) return false;
+              // (in this order: with its first weights of the piece the group has seen the phase ahead of o_free's, which is told from it only then)
               if (!wait(&ctl.p_ready[w], on, 88)) return false;
+              if (first && pieces > 0 && !wait(&ctl.o_free[w], pieces - 1, 90)) return false;
               if (!T::APART && !(ok = held = take(&ctl.lock, lane))) return false;
               tc_fence_after_sync();
 #pragma unroll
@@ -1056,12 +1057,15 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       // What a thread has of its row: all columns of a tile of its own, half of them of a tile that both groups share.
       float f[2] = {1.f, 0.f}, top = m, all = l;
       bool bad = false, have[2] = {mine > 0, false};
+      const int qs = pieces % T::Q;
       if (!x.empty) {
         const int theirs = other;
         other += x.of(w ^ 1).n;
-        if (!x.two) {
-          // (what stands there of the piece before has been read)
-          if (pieces > 0 && !wait(&ctl.o_free[w], pieces - 1, 98)) return false;
+        // A group without blocks in a piece stays behind the loader and the other group: what it gives back counts for this piece only when all of the piece before
+        // has been given back (both groups count on one barrier), and its queries have come.
+        if (mine == 0 && !wait_long(&ctl.q_full[qs], pieces / T::Q, 99)) return false;
+        if ((mine == 0 || !x.two) && pieces > 0 && !wait(&ctl.o_free[w], pieces - 1, 98)) return false;
+        if (!x.two) {                      // (what stands there of the piece before has been read)
           ctl.ml[w][row] = make_float2(m, l);
           mbar_arrive(smem_u32(&ctl.met));
           if (!wait(&ctl.met, mets, 95)) return false;
@@ -1092,10 +1096,8 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       const float by = !x.whole ? 1.f : all > 0.f ? 1.f / all : all;                          // (no weight: zeros; NaN as it is)
       // Results of 16-byte pieces go through shared memory, so that a warp writes whole rows (a thread's pieces lie in 32 of them: 5000 cycles for 128 rows
       // of 64). The queries' buffer is free for it: the last scores have been made, and the second half of it where there is one tile.
-      const int qs = pieces % T::Q;
       const bool staged = p.vec_y && x.whole && !x.empty;
       uint4* stage = reinterpret_cast<uint4*>(smem_q + (qs * 2 + w) * T::TILE);
-      if (staged && !wait_long(&ctl.q_full[qs], pieces / T::Q, 99)) return false;
       const int c_begin = x.two ? 0 : w * (DP / 2), c_end = x.two ? DP : (w + 1) * (DP / 2);
 #pragma unroll 1
       for (int c0 = c_begin; c0 < c_end; c0 += 32) {
