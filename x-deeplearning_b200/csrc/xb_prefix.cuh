@@ -923,7 +923,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
           tc_fence_after_sync();
           // Sums so far are moved to a maximum that has grown. (m is -infinity: nothing has been summed; no maximum yet: nothing to move.)
           auto move_sums = [&](float next) {
-            if (__any_sync(0xffffffffu, (next - m) * p.scale > PFX_GROWTH)) {
+            if (__any_sync(0xffffffffu, there && (next - m) * p.scale > PFX_GROWTH)) {       // (what stands in rows that are none has no say in the others' roundings)
               const float by = m == next || m == -INFINITY ? 1.f : ex2((m - next) * p.scale);
               m = next;
               l *= by;
@@ -983,7 +983,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
             for (int c = 0; c < 128; c += 2) top[c / 2 % 4] = fmaxf(top[c / 2 % 4], fmaxf(__uint_as_float(s[c / 32][c % 32]), __uint_as_float(s[c / 32][c % 32 + 1])));
             if (!move_sums(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])))) return false;
             float base = (m == -INFINITY ? 0.f : m * p.scale) - PFX_UP<BF16>;
-            if (__any_sync(0xffffffffu, fabsf(base) > 1e6f)) {
+            if (__any_sync(0xffffffffu, there && fabsf(base) > 1e6f)) {
               const float off = m == -INFINITY ? 0.f : m;
 #pragma unroll
               for (int c = 0; c < 128; ++c) s[c / 32][c % 32] = __float_as_uint(__uint_as_float(s[c / 32][c % 32]) - off);
