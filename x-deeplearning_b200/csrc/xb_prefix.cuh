@@ -19,9 +19,10 @@
 //
 // What bounds it is neither memory nor the tensor cores but the way from scores to weights: 128 exponentials a row and block at 16 a cycle and SM, 1024
 // cycles for a block of 128 rows, with the maximum, the packing and the loads and stores of tensor memory 1500 to 2100; and some 18000 cycles an item of
-// few blocks (offsets, the first keys, the results). 512 candidates of 4 heads of 128 on one prefix of 100003 rows: 165 us (its bytes: 62); 74 requests of
-// 1000 candidates on 100 rows each, 4 heads of 64: 122 us (24); 256 lists of up to 300 rows that 8 prefixes of up to 4000 serve, 32 heads on 8 of 128, one
-// new row each: 206 us (69); 64 lists of up to 500 rows, whole, 16 prefixes of up to 1000, 8 heads of 64: 376 us (48).
+// few blocks (offsets, the first keys, the results). Single calls (back to back 3 to 13 us less): 512 candidates of 4 heads of 128 on one prefix of 100003 rows: 165 us
+// (its products: 62); 74 requests of 1000 candidates on 100 rows each, 4 heads of 64: 127 us (bytes 24); 256 lists of up to 300 rows that 8 prefixes of up to 4000
+// serve, 32 heads on 8 of 128, one new row each: 205 us (bytes 69); 64 lists of up to 500 rows, whole, 16 prefixes of up to 1000, 8 heads of 64: 400 us (products 48).
+// Instructions are not always at hand (no_instruction 0.9 to 1.5 stalls an issue): one more wait in line costs 1 to 6 % of some calls.
 #pragma once
 
 #include <algorithm>
