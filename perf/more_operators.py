@@ -182,7 +182,8 @@ def run(s):
     if own:
         ops = _ops()
         if s["kind"] == "rope":
-            return ops.qk_norm_rope(s["q"], s["k"], s["positions"], s["freqs"], q_weight=s["wq"], k_weight=s["wk"], norm=s["norm"],
+            return ops.qk_norm_rope(s["q"], s["k"], s["positions"], s["freqs"], q_weight=s["wq"],
+                                    k_weight=s["wk"] if s["k"] is not None else None, norm=s["norm"],
                                     adjacent=s["adjacent"])
         if s["kind"] == "lin":
             lists = dict(T=s["equal"]) if s["equal"] else dict(offsets=s["offsets"])
